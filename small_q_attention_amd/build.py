@@ -29,7 +29,7 @@ CSRC = PKG_DIR / "csrc"
 INCLUDE = REPO_DIR / "include"
 LIB_PATH = PKG_DIR / "libsqa.so"
 SOURCES = [CSRC / "sqa_kernels.hip", CSRC / "sqa_capi.hip"]
-HEADERS = [CSRC / "sqa_internal.h", INCLUDE / "sqa.h"]
+HEADERS = [CSRC / "sqa_internal.h", CSRC / "sqa_device.h", INCLUDE / "sqa.h"]
 ARCH = "gfx950"
 
 

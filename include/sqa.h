@@ -40,6 +40,7 @@ extern "C" {
 #define SQA_DTYPE_F16 0
 #define SQA_DTYPE_BF16 1
 #define SQA_DTYPE_FP8_E4M3 2
+#define SQA_DTYPE_INT8 3 /* caches with block scales only */
 
 /*
  * Chooses the split-KV decomposition.
@@ -244,6 +245,85 @@ typedef struct sqa_attention_args {
  * Same plan, workspace, status codes and asynchrony as sqa_paged_mtp_attention.
  */
 int sqa_paged_attention(const sqa_attention_args* args);
+
+/*
+ * Caches held in 8 bits with a scale for each cache page and kv head (no counterpart in
+ * the reference). Code c (e4m3 or int8) of page p and head h stands for
+ * c * k[p * page_stride + h * head_stride] (V alike); strides count floats. Scales are
+ * finite and not negative; 0 marks a block of zeros.
+ */
+typedef struct sqa_block_scales {
+  const float* k;
+  const float* v;
+  int64_t page_stride;
+  int64_t head_stride;
+} sqa_block_scales;
+
+/*
+ * Partial slots (*num_splits >= batch) of an sqa_paged_attention_scaled call: the work
+ * items that fill the device once, or fewer where sequences of max_seq_len tokens
+ * (max_seq_len <= 0: of the table's max_pages 16-token pages) do not need as many.
+ * The device cuts the pages from seq_lens alone, so any such count serves any lengths;
+ * max_seq_len only sizes the call. sqa_workspace_bytes(..., *num_splits, 0) is the
+ * workspace.
+ */
+int sqa_plan_scaled(int device, int batch, int num_kv_heads, int max_seq_len, int max_pages,
+                    int* num_splits);
+
+/*
+ * sqa_paged_attention over such a cache: kv_dtype SQA_DTYPE_FP8_E4M3 or SQA_DTYPE_INT8,
+ * num_splits from sqa_plan_scaled, pages_per_split 0, flags 0; everything else as there.
+ * A sequence's splits follow from all lengths of the batch, so its last bits may differ
+ * between batches; equal inputs give equal bits.
+ */
+int sqa_paged_attention_scaled(const sqa_attention_args* args, const sqa_block_scales* scales);
+
+/*
+ * Arguments of sqa_append_scaled (set struct_size = sizeof(sqa_append_args)).
+ *   key, value     [batch, q_len, num_kv_heads, head_dim] of `dtype`, 16-byte aligned;
+ *                  key_strides / value_strides: elements between batches, tokens and
+ *                  heads (multiples of 8), the head dimension contiguous.
+ *   kv, scales     the cache, both written.
+ *   seq_lens       lengths with the new tokens; new_lens NULL or the new tokens of each
+ *                  sequence (at most q_len; key[b][i] for i < new_lens[b]), which go to
+ *                  positions seq_lens[b] - new_lens[b] on. Both are held to the range
+ *                  where they make sense (0 .. q_len new tokens, no more than the length).
+ * max_pages here counts block_tables columns. Positions past the table row, and pages
+ * whose id is outside the pool, are not written.
+ */
+typedef struct sqa_append_args {
+  size_t struct_size;
+  const void* key;
+  const void* value;
+  int64_t key_strides[3];
+  int64_t value_strides[3];
+  sqa_kv_cache kv;
+  sqa_block_scales scales;
+  const int32_t* block_tables;
+  const int32_t* seq_lens;
+  const int32_t* new_lens;
+  int max_pages;
+  int batch;
+  int q_len;
+  int num_kv_heads;
+  int head_dim;
+  int page_size;
+  int dtype;
+  int kv_dtype;
+  void* stream;
+} sqa_append_args;
+
+/*
+ * Writes the new tokens of every sequence into an 8-bit cache. A block (the tokens of one
+ * page and head, K or V) gets the scale max|x| / M over its new tokens, M = 448 (e4m3) or
+ * 127 (int8), and at least its old scale where earlier tokens of the sequence stay in it;
+ * the new tokens' codes are x / scale rounded to nearest even, and where the scale grew
+ * the earlier tokens' codes are rounded again, code * old / new. A page whose first slot
+ * is written starts afresh. Infinities count as the type's largest finite value; NaN does
+ * not count and is stored as NaN (e4m3) or 0 (int8). Slots past a sequence's end stay as
+ * they are. No two sequences may write the same page in one call.
+ */
+int sqa_append_scaled(const sqa_append_args* args);
 
 /* Compute units of `device` (256 on MI355X), or -1 on error. */
 int sqa_device_cu_count(int device);

@@ -31,6 +31,9 @@ _SIGNATURES = [
     ("sqa_paged_mtp_attention_noalloc", _C.c_int,
      [_C.c_void_p] * 6 + [_C.c_int] * 5 + [_C.c_int64] + [_C.c_int] * 4 + [_C.c_void_p]),
     ("sqa_paged_attention", _C.c_int, [_C.c_void_p]),
+    ("sqa_plan_scaled", _C.c_int, [_C.c_int] * 5 + [_C.POINTER(_C.c_int)]),
+    ("sqa_paged_attention_scaled", _C.c_int, [_C.c_void_p, _C.c_void_p]),
+    ("sqa_append_scaled", _C.c_int, [_C.c_void_p]),
     ("sqa_device_cu_count", _C.c_int, [_C.c_int]),
     ("sqa_last_error", _C.c_char_p, []),
     ("sqa_version", _C.c_char_p, []),
@@ -61,11 +64,34 @@ class AttentionArgs(ctypes.Structure):
                 ("flags", _C.c_int)]
 
 
+class BlockScales(ctypes.Structure):
+    """``sqa_block_scales`` of include/sqa.h (strides in floats)."""
+
+    _fields_ = [("k", _C.c_void_p), ("v", _C.c_void_p), ("page_stride", _C.c_int64),
+                ("head_stride", _C.c_int64)]
+
+
+class AppendArgs(ctypes.Structure):
+    """``sqa_append_args`` of include/sqa.h."""
+
+    _fields_ = [("struct_size", _C.c_size_t), ("key", _C.c_void_p), ("value", _C.c_void_p),
+                ("key_strides", _C.c_int64 * 3), ("value_strides", _C.c_int64 * 3),
+                ("kv", KVCache), ("scales", BlockScales), ("block_tables", _C.c_void_p),
+                ("seq_lens", _C.c_void_p), ("new_lens", _C.c_void_p), ("max_pages", _C.c_int),
+                ("batch", _C.c_int), ("q_len", _C.c_int), ("num_kv_heads", _C.c_int),
+                ("head_dim", _C.c_int), ("page_size", _C.c_int), ("dtype", _C.c_int),
+                ("kv_dtype", _C.c_int), ("stream", _C.c_void_p)]
+
+
 # AttentionArgs as one packed record (native sizes and alignment, padded as C does).
 _ARGS = struct.Struct("@N2P2P4q2PiPi2f8iPN2P3i0q")
 assert _ARGS.size == ctypes.sizeof(AttentionArgs)
+_SCALES = struct.Struct("@2P2q")
+assert _SCALES.size == ctypes.sizeof(BlockScales)
+_APPEND = struct.Struct("@N2P6q2P4q2P2q3P8iP0q")
+assert _APPEND.size == ctypes.sizeof(AppendArgs)
 
-DTYPE_F16, DTYPE_BF16, DTYPE_FP8_E4M3 = 0, 1, 2
+DTYPE_F16, DTYPE_BF16, DTYPE_FP8_E4M3, DTYPE_INT8 = 0, 1, 2, 3
 FLAG_ADAPTIVE_PAIRS = 1  # SQA_FLAG_ADAPTIVE_PAIRS
 
 
@@ -222,6 +248,74 @@ def launch_general(query, output, k_view, v_view, block_tables, seq_lens, draft_
     rc = lib.sqa_paged_attention(a)
     if rc != SQA_OK:
         raise RuntimeError(f"sqa_paged_attention failed: {last_error(lib)}")
+
+
+def dtype_code(dtype) -> int:
+    """``SQA_DTYPE_*`` of a torch type."""
+    import torch
+
+    return {torch.float16: DTYPE_F16, torch.bfloat16: DTYPE_BF16,
+            torch.float8_e4m3fn: DTYPE_FP8_E4M3, torch.int8: DTYPE_INT8}[dtype]
+
+
+@functools.lru_cache(maxsize=4096)
+def plan_scaled(device_index: int, batch: int, num_kv_heads: int, max_seq_len: int,
+                max_pages: int) -> int:
+    """``sqa_plan_scaled``: partial slots of a call over a cache with block scales."""
+    lib = load()
+    ns = ctypes.c_int(0)
+    rc = lib.sqa_plan_scaled(device_index, batch, num_kv_heads, max_seq_len, max_pages,
+                             ctypes.byref(ns))
+    if rc != SQA_OK:
+        raise RuntimeError(f"sqa_plan_scaled failed: {last_error(lib)}")
+    return ns.value
+
+
+def launch_scaled(query, output, k_view, v_view, k_scale, v_scale, block_tables, seq_lens,
+                  draft_mask, scale: float, out_scale: float, num_splits: int, workspace,
+                  stream_handle: int, timing_events=None):
+    """Call ``sqa_paged_attention_scaled``: as :func:`launch_general`, over e4m3 or int8
+    views with ``[num_pages, Hkv]`` float32 scales of equal strides."""
+    lib = _LIB if _LIB is not None else load()
+    b, q_len, hq, d = query.shape
+    strides, sstrides = k_view.stride(), k_scale.stride()
+    num_pages, page, hkv, _ = k_view.shape
+    words, mask_words = (0, 0) if draft_mask is None else (draft_mask.data_ptr(),
+                                                           draft_mask.shape[-1])
+    ev = None
+    if timing_events is not None:
+        ev = (ctypes.c_void_p * 3)(*[ctypes.c_void_p(int(e)) for e in timing_events])
+    a = _ARGS.pack(
+        _ARGS.size, query.data_ptr(), output.data_ptr(), k_view.data_ptr(), v_view.data_ptr(),
+        num_pages, strides[0], strides[1], strides[2], block_tables.data_ptr(),
+        seq_lens.data_ptr(), block_tables.shape[1], words, mask_words, scale, out_scale, b, q_len,
+        hq, hkv, d, page, num_splits, 0, workspace.data_ptr(),
+        workspace.numel() * workspace.element_size(), stream_handle or 0,
+        0 if ev is None else ctypes.addressof(ev), dtype_code(query.dtype),
+        dtype_code(k_view.dtype), 0)
+    s = _SCALES.pack(k_scale.data_ptr(), v_scale.data_ptr(), sstrides[0], sstrides[1])
+    rc = lib.sqa_paged_attention_scaled(a, s)
+    if rc != SQA_OK:
+        raise RuntimeError(f"sqa_paged_attention_scaled failed: {last_error(lib)}")
+
+
+def launch_append(key, value, k_view, v_view, k_scale, v_scale, block_tables, seq_lens, new_lens,
+                  stream_handle: int):
+    """Call ``sqa_append_scaled`` (``key``/``value`` ``[B, Q, Hkv, D]``, their last dimension
+    contiguous; views and scales as for :func:`launch_scaled`)."""
+    lib = _LIB if _LIB is not None else load()
+    b, q_len, hkv, d = key.shape
+    strides, sstrides = k_view.stride(), k_scale.stride()
+    a = _APPEND.pack(
+        _APPEND.size, key.data_ptr(), value.data_ptr(), *key.stride()[:3], *value.stride()[:3],
+        k_view.data_ptr(), v_view.data_ptr(), k_view.shape[0], strides[0], strides[1], strides[2],
+        k_scale.data_ptr(), v_scale.data_ptr(), sstrides[0], sstrides[1], block_tables.data_ptr(),
+        seq_lens.data_ptr(), 0 if new_lens is None else new_lens.data_ptr(),
+        block_tables.shape[1], b, q_len, hkv, d, k_view.shape[1], dtype_code(key.dtype),
+        dtype_code(k_view.dtype), stream_handle or 0)
+    rc = lib.sqa_append_scaled(a)
+    if rc != SQA_OK:
+        raise RuntimeError(f"sqa_append_scaled failed: {last_error(lib)}")
 
 
 def run(query, key_cache, value_cache, block_tables, seq_lens, num_splits: int,

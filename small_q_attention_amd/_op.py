@@ -81,3 +81,45 @@ def _paged_attention_planned_fake(query, k_view, v_view, block_tables, seq_lens,
 def _paged_mtp_attention_fake(query, key_cache, value_cache, block_tables, seq_lens,
                               num_splits, pages_per_split):
     return torch.empty_like(query)
+
+
+@torch.library.custom_op("sqa::paged_attention_scaled", mutates_args=())
+def paged_attention_scaled(query: torch.Tensor, key_cache: torch.Tensor,
+                           value_cache: torch.Tensor, key_scale: torch.Tensor,
+                           value_scale: torch.Tensor, block_tables: torch.Tensor,
+                           seq_lens: torch.Tensor, draft_mask: Optional[torch.Tensor],
+                           scale: float, out_scale: float, max_seq_len: int) -> torch.Tensor:
+    """Attention over an 8-bit cache with block scales (``scaled_cache``), planned and given
+    its workspace at run time."""
+    from . import scaled_cache
+
+    return scaled_cache.on_device(query.device, lambda: scaled_cache.run_attention(
+        query, key_cache, value_cache, key_scale, value_scale, block_tables, seq_lens, draft_mask,
+        scale, out_scale, max_seq_len, None, None))
+
+
+@paged_attention_scaled.register_fake
+def _paged_attention_scaled_fake(query, key_cache, value_cache, key_scale, value_scale,
+                                 block_tables, seq_lens, draft_mask, scale, out_scale,
+                                 max_seq_len):
+    return torch.empty_like(query)
+
+
+@torch.library.custom_op("sqa::append_scaled_kv",
+                         mutates_args=("key_cache", "value_cache", "key_scale", "value_scale"))
+def append_scaled_kv(key: torch.Tensor, value: torch.Tensor, key_cache: torch.Tensor,
+                     value_cache: torch.Tensor, key_scale: torch.Tensor,
+                     value_scale: torch.Tensor, block_tables: torch.Tensor,
+                     seq_lens: torch.Tensor, new_lens: Optional[torch.Tensor]) -> None:
+    """The quantising append (``scaled_cache.append_scaled_kv``)."""
+    from . import scaled_cache
+
+    scaled_cache.on_device(key.device, lambda: _lib.launch_append(
+        key, value, key_cache, value_cache, key_scale, value_scale, block_tables, seq_lens,
+        new_lens, _lib.raw_stream(key.device.index)))
+
+
+@append_scaled_kv.register_fake
+def _append_scaled_kv_fake(key, value, key_cache, value_cache, key_scale, value_scale,
+                           block_tables, seq_lens, new_lens):
+    return None

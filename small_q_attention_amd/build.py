@@ -21,6 +21,7 @@ import os
 import shutil
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PKG_DIR = Path(__file__).resolve().parent
@@ -28,8 +29,10 @@ REPO_DIR = PKG_DIR.parent
 CSRC = PKG_DIR / "csrc"
 INCLUDE = REPO_DIR / "include"
 LIB_PATH = PKG_DIR / "libsqa.so"
-SOURCES = [CSRC / "sqa_kernels.hip", CSRC / "sqa_capi.hip"]
-HEADERS = [CSRC / "sqa_internal.h", CSRC / "sqa_device.h", INCLUDE / "sqa.h"]
+SOURCES = [CSRC / name for name in ("sqa_kernels.hip", "sqa_capi.hip", "sqa_scaled.hip",
+                                    "sqa_cache_capi.hip")]
+HEADERS = [CSRC / "sqa_internal.h", CSRC / "sqa_device.h", CSRC / "sqa_cache.h",
+           INCLUDE / "sqa.h"]
 ARCH = "gfx950"
 
 
@@ -81,6 +84,33 @@ def build_command(output: Path = LIB_PATH, src_hash: str = ""):
     ]
 
 
+def _compile(output: Path, verbose: bool):
+    """:func:`build_command` with its sources compiled side by side: one hipcc takes them
+    one after the other. Returns whether a step failed, and what the steps printed."""
+    whole = build_command(output)
+    first = whole.index(str(SOURCES[0]))
+    head = [arg for arg in whole[:first] if arg != "-shared"]
+    objects = [output.with_name(f"{output.name}.{src.stem}.o") for src in SOURCES]
+    steps = [[*head, "-c", str(src), "-o", str(obj)] for src, obj in zip(SOURCES, objects)]
+    link = [hipcc_path(), f"--offload-arch={ARCH}", "-fPIC", "-shared",
+            *[str(obj) for obj in objects], "-o", str(output)]
+    if verbose:
+        print("\n".join(" ".join(cmd) for cmd in [*steps, link]), flush=True)
+
+    def run(cmd):
+        return subprocess.run(cmd, capture_output=True, text=True)
+
+    try:
+        with ThreadPoolExecutor(max_workers=4) as pool:
+            done = list(pool.map(run, steps))
+        if not any(res.returncode for res in done):
+            done.append(run(link))
+    finally:
+        for obj in objects:
+            obj.unlink(missing_ok=True)
+    return any(res.returncode for res in done), "".join(res.stdout + res.stderr for res in done)
+
+
 def built_hash(path: Path = LIB_PATH):
     """The source hash stamped into a built library, or None (missing or unstamped)."""
     try:
@@ -105,13 +135,10 @@ def is_stale() -> bool:
 def build(verbose: bool = False) -> Path:
     """Compile ``libsqa.so`` (always; callers decide whether a rebuild is due)."""
     tmp = LIB_PATH.with_name(f"{LIB_PATH.name}.tmp{os.getpid()}")
-    cmd = build_command(tmp)
-    if verbose:
-        print(" ".join(cmd), flush=True)
-    res = subprocess.run(cmd, capture_output=True, text=True)
-    errors = [ln for ln in (res.stdout + res.stderr).splitlines()
+    failed, text = _compile(tmp, verbose)
+    errors = [ln for ln in text.splitlines()
               if "packed-fp32-ops" not in ln and "unknown target feature" not in ln.lower()]
-    if res.returncode != 0:
+    if failed:
         tmp.unlink(missing_ok=True)
         raise RuntimeError("hipcc failed building libsqa.so:\n" + "\n".join(errors))
     if verbose and errors:

@@ -1,0 +1,52 @@
+// Internal interface between the C ABI (sqa_cache_capi.hip) and the kernels around the
+// paged cache: the quantising append and attention over 8-bit caches with block scales
+// (sqa_scaled.hip), attention weights and eviction (sqa_evict.hip).
+#pragma once
+
+#include "sqa_internal.h"
+
+namespace sqa {
+
+// Element types of caches and tokens, as the public header numbers them.
+enum { kF16 = 0, kBF16 = 1, kE4M3 = 2, kInt8 = 3 };
+
+// The largest magnitude a code stands for, in units of its block's scale.
+__host__ __device__ inline float code_max(int kv_type) { return kv_type == kInt8 ? 127.f : 448.f; }
+
+// Scales of an 8-bit cache: one float for each cache page and kv head, for K and for V.
+struct BlockScales {
+  float* k;
+  float* v;
+  long long page_stride;  // bytes between consecutive pages
+  unsigned head_stride;   // bytes between consecutive kv heads
+};
+
+// Attention over an 8-bit cache with block scales. Of `p` the fields that name buffers,
+// shapes, strides and scales; the plan is the kernel's own (sqa_scaled.hip): `items`
+// work items, partial slot i for item i, p.seq_splits written by the kernel.
+struct ScaledArgs {
+  PartialArgs p;
+  BlockScales scales;
+  int items;
+  int int8;      // codes: 0 e4m3, 1 int8
+  int wg_heads;  // kv heads a workgroup serves (1, 2 or 4); its other waves take more items
+};
+hipError_t launch_scaled(const ScaledArgs& a, hipStream_t stream);
+
+struct AppendArgs {
+  const void* src[2];               // K and V of the new tokens, [B, Q, Hkv, D]
+  long long src_batch[2], src_token[2], src_head[2];  // strides in bytes
+  void* cache[2];                   // K and V codes
+  BlockScales scales;
+  const int32_t* block_tables;
+  const int32_t* seq_lens;
+  const int32_t* new_lens;          // NULL: q_len new tokens everywhere
+  long long num_pages, page_stride; // strides in bytes (codes)
+  long long token_stride, head_stride;
+  int batch, q_len, hkv, head_dim, page_size, bt_stride;
+  int touched;                      // most pages the new tokens of a sequence lie on
+  int bf16, int8;
+};
+hipError_t launch_append(const AppendArgs& a, hipStream_t stream);
+
+}  // namespace sqa

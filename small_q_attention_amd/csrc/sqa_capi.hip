@@ -17,11 +17,10 @@
 #include <vector>
 
 namespace {
-
 thread_local std::string g_last_error;
+}  // namespace
 
-int fail(int code, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
-int fail(int code, const char* fmt, ...) {
+int sqa::fail(int code, const char* fmt, ...) {
   char buf[512];
   va_list ap;
   va_start(ap, fmt);
@@ -34,9 +33,14 @@ int fail(int code, const char* fmt, ...) {
   return code;
 }
 
-int hip_fail(hipError_t e, const char* what) {
+int sqa::hip_fail(hipError_t e, const char* what) {
   return fail(SQA_ERR_HIP, "%s: %s", what, hipGetErrorString(e));
 }
+
+namespace {
+
+using sqa::fail;
+using sqa::hip_fail;
 
 std::mutex g_cu_mutex;
 std::vector<int> g_cu_count;  // cached per device

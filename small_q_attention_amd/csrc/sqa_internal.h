@@ -320,6 +320,10 @@ inline int merge_row_threads(long long rows, int per_row, int chunks, int cus) {
   return rows >= 1024 && per_row <= 8 * (kWave / chunks) ? kWave : 4 * kWave;
 }
 
+// Store the thread's error message (sqa_last_error) and return the status.
+int fail(int code, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
+int hip_fail(hipError_t e, const char* what);
+
 hipError_t launch_partial(const PartialArgs& a, hipStream_t stream);
 hipError_t launch_merge(const MergeArgs& a, int cus, hipStream_t stream);
 

@@ -1,0 +1,621 @@
+// gfx950 kernels for caches held in 8 bits with a scale for each page and kv head:
+// the quantising append and small-q attention.
+//
+// A code c of page p and head h stands for c * s, s = scale[p][h]. With x the tokens of
+// the block, s = max|x| / M (M = 448 for e4m3, 127 for int8) and c = x / s rounded to
+// nearest even. Attention folds the scales into the softmax and the probabilities:
+//   score(row, t)  = (scale * k_scale[page of t]) * (q . k_code[t])
+//   out(row)       = sum_t (p(row, t) * v_scale[page of t]) v_code[t] / sum_t p(row, t)
+// so the codes go to the MFMAs as they are (both types widen exactly to 16 bits) and a
+// page costs two scalars.
+#include "sqa_cache.h"
+#include "sqa_device.h"
+
+namespace sqa {
+namespace {
+
+// ---------------------------------------------------------------------------------
+// Attention.
+// ---------------------------------------------------------------------------------
+
+// V of a page as the PV product's A operand: av[mb] = this lane's dim mb of its four
+// tokens in bf16. bf16 holds every e4m3 value and every integer up to 256 exactly.
+template <int HD>
+struct CodesFp8 : KvFp8<HD> {
+  using Regs = typename KvFp8<HD>::Regs;
+  static constexpr int MB = Dims<HD>::MB, VW = Dims<HD>::VW;
+  static constexpr bool kNan = true;  // codes may be NaN
+  static __device__ __forceinline__ void operand_v(const Regs& r, u2 (&av)[MB]) {
+#pragma unroll
+    for (int i = 0; i < VW / 2; ++i) {
+      // Bytes of two token rows interleaved, so that a conversion yields two tokens of
+      // one dim.
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const unsigned sel = half ? 0x07030602u : 0x05010400u;
+        const unsigned t01 = __builtin_amdgcn_perm(r.v[1][i], r.v[0][i], sel);
+        const unsigned t23 = __builtin_amdgcn_perm(r.v[3][i], r.v[2][i], sel);
+        const u2 a = ElemBF16::widen_fp8x4(t01), b = ElemBF16::widen_fp8x4(t23);
+        av[4 * i + 2 * half] = u2{a[0], b[0]};
+        av[4 * i + 2 * half + 1] = u2{a[1], b[1]};
+      }
+    }
+  }
+};
+
+template <int HD>
+struct CodesInt8 : KvFp8<HD> {
+  using Regs = typename KvFp8<HD>::Regs;
+  static constexpr int KK = Dims<HD>::KK, MB = Dims<HD>::MB, VW = Dims<HD>::VW;
+  static constexpr bool kNan = false;
+  static __device__ __forceinline__ float byte(unsigned w, int i) {
+    return (float)(signed char)(w >> (8 * i));
+  }
+  template <typename E>
+  static __device__ __forceinline__ void expand_k(const Regs& r, u4 (&k)[KK]) {
+#pragma unroll
+    for (int i = 0; i < KK; ++i) {
+#pragma unroll
+      for (int w = 0; w < 2; ++w) {
+        const unsigned x = r.k[i / 2][2 * (i & 1) + w];
+        k[i][2 * w] = E::pack2(byte(x, 0), byte(x, 1));
+        k[i][2 * w + 1] = E::pack2(byte(x, 2), byte(x, 3));
+      }
+    }
+  }
+  static __device__ __forceinline__ void operand_v(const Regs& r, u2 (&av)[MB]) {
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb) {
+      const int i = mb / 4, e = mb % 4;
+      av[mb] = u2{ElemBF16::pack2(byte(r.v[0][i], e), byte(r.v[1][i], e)),
+                  ElemBF16::pack2(byte(r.v[2][i], e), byte(r.v[3][i], e))};
+    }
+  }
+};
+
+// A split of one sequence.
+struct Split {
+  int b, len;          // sequence and its length
+  int p_begin, p_end;  // kernel pages
+  int count;           // splits of the sequence
+  int slot;            // partial slot
+};
+
+__device__ __forceinline__ int wave_sum_int(int x) {
+  return __builtin_amdgcn_readlane(wave_inclusive_scan_int(x), 63);
+}
+
+// The cut of the batch into work items, found by every wave for itself from the lengths:
+// sequence b takes n_b = max(1, ceil(pages_b / P)) items of nearly equal size, with P the
+// smallest page count of at least kMinSplitPages for which they sum to at most `items`
+// (or P the longest sequence, one item each, where the batch has more sequences than
+// that). All items are resident at once, so the longest, P pages, sets the time.
+// Returns whether item `item` exists; `table` (one wave of the grid) also receives each
+// sequence's first item and count for the merge kernel.
+__device__ __forceinline__ bool find_split(const PartialArgs& a, int items, int item,
+                                           SeqSplits* table, Split& out) {
+  const int lane = threadIdx.x & 63;
+  const int groups = (a.batch + 63) / 64;
+  auto length_of = [&](int k) {
+    const int i = 64 * k + lane;
+    return i < a.batch ? max(a.seq_lens[i], 0) : 0;
+  };
+  const int len0 = length_of(0);
+  auto pages_at = [&](int k) {
+    const int len = k == 0 ? len0 : length_of(k);
+    return min((len + kPageSize - 1) / kPageSize, a.max_pages);
+  };
+  auto splits_of = [&](int k, int P) {
+    return 64 * k + lane < a.batch ? max((pages_at(k) + P - 1) / P, 1) : 0;
+  };
+  int total = 0;
+  for (int k = 0; k < groups; ++k) total += wave_sum_int(pages_at(k));
+  auto fits = [&](int P) {
+    int n = 0;
+    for (int k = 0; k < groups; ++k) n += wave_sum_int(splits_of(k, P));
+    return n <= items;
+  };
+  int lo = max(kMinSplitPages, (total + items - 1) / items);
+  if (!fits(lo)) {
+    // ceil(pages_b / P) sum to at most total / P + batch.
+    int hi = items > a.batch ? max(lo, (total + items - a.batch - 1) / (items - a.batch))
+                             : max(a.max_pages, 1);
+    while (lo + 1 < hi) {  // lo does not fit, hi does (or is one item each)
+      const int mid = lo + (hi - lo) / 2;
+      if (fits(mid))
+        hi = mid;
+      else
+        lo = mid;
+    }
+    lo = hi;
+  }
+  const int P = lo;
+  int base = 0;
+  bool found = false;
+  for (int k = 0; k < groups; ++k) {
+    const int n = splits_of(k, P);
+    const int incl = wave_inclusive_scan_int(n);
+    const int first = base + incl - n;
+    if (table != nullptr && 64 * k + lane < a.batch) table[64 * k + lane] = SeqSplits{first, n};
+    const unsigned long long hit = __ballot(item >= first && item < first + n);
+    if (hit && !found) {
+      const int src = __builtin_ctzll(hit);
+      const int pages = __builtin_amdgcn_readlane(pages_at(k), src);
+      out.b = 64 * k + src;
+      out.len = __builtin_amdgcn_readlane(k == 0 ? len0 : length_of(k), src);
+      out.count = __builtin_amdgcn_readlane(n, src);
+      out.slot = item;
+      const int size = (pages + out.count - 1) / out.count;
+      out.p_begin = (item - __builtin_amdgcn_readlane(first, src)) * size;
+      out.p_end = min(out.p_begin + size, pages);
+      found = true;
+      if (table == nullptr) return true;
+    }
+    base += __builtin_amdgcn_readlane(incl, 63);
+  }
+  return found;
+}
+
+// Scores of a page in the exponent's units: (K code . Q^T) * c.
+template <int NB, int HD, typename E, typename KV>
+__device__ __forceinline__ void code_scores(f4 (&s)[NB], const typename KV::Regs& r,
+                                            const u4 (&q)[NB][Dims<HD>::KK], float c) {
+  constexpr int KK = Dims<HD>::KK;
+  u4 k[KK];
+  KV::template expand_k<E>(r, k);
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb) {
+    s[nb] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) s[nb] = E::mma_qk(k[kk], q[nb][kk], s[nb]);
+    s[nb] *= c;
+  }
+}
+
+// A masked page's NaN codes of V: in the PV product one would reach every row of its
+// block, those that do not see its token too (0 * NaN). They become 0 here, and NaN the
+// sums of the rows that do see them. Rare: decoding pages without one costs a few
+// instructions on the pages of the draft block only.
+template <int NB, int HD, typename KV>
+__device__ __forceinline__ void nan_values(WaveState<NB, HD>& st, typename KV::Regs& r,
+                                           const f4 (&s)[NB]) {
+  constexpr int MB = Dims<HD>::MB, VW = Dims<HD>::VW;
+  typename KV::Regs marks;
+  unsigned any = 0u;
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+#pragma unroll
+    for (int w = 0; w < VW / 2; ++w) {
+      // Bytes of magnitude 0x7f, as 0x80.
+      const unsigned nan = ((r.v[e][w] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+      any |= nan;
+      marks.v[e][w] = (nan >> 7) * 0x38u;  // 1.0 in e4m3
+      r.v[e][w] &= ~((nan >> 7) * 0xffu);
+    }
+  if (!__any(any != 0u)) return;  // uniform
+  u2 av[MB];
+  KV::operand_v(marks, av);
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb) {
+    float seen[4], sum = 0.f;
+    u2 lo;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) seen[e] = s[nb][e] == -INFINITY ? 0.f : 1.f;
+    const u2 hi = ElemBF16::round_p(seen[0], seen[1], seen[2], seen[3], sum, lo);
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb) {
+      const f4 hits = ElemBF16::mma_pv(av[mb], hi, lo, f4{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        st.acc[mb][nb][e] = hits[e] > 0.f ? __builtin_nanf("") : st.acc[mb][nb][e];
+    }
+  }
+}
+
+// One workgroup = four waves on their own: wave w serves kv head w % wg_heads of the
+// workgroup's heads and work item w / wg_heads of its items, with all query rows of the
+// head (NB blocks of 16). A wave keeps a ring of D pages of codes and their two scales in
+// flight in registers; the ids of the next 64 to 128 pages sit in two registers, one page
+// per lane. No barrier: waves of a workgroup meet only in the memory system, where the
+// heads' slices of a token row are neighbours.
+// P enters the PV product as two bf16 parts of p * v_scale (together within 2^-17 of it,
+// at the cost of one product, as in the bf16 kernels): fp16 would lose the small scales
+// of quiet blocks. The row sums take p itself.
+template <int NB, int D, int HD, typename E, typename KV>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1)))
+void sqa_scaled_attention_kernel(ScaledArgs args) {
+  const PartialArgs& a = args.p;
+  constexpr int KK = Dims<HD>::KK, MB = Dims<HD>::MB;
+  static_assert(64 % D == 0, "a ring turn lies within one run of 64 page ids");
+  __shared__ float sm_stage[4 * 16 * (HD + 4)];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+  const int g16 = lane >> 4, l16 = lane & 15;
+  const int wgh = args.wg_heads;
+  const int head_groups = (a.hkv + wgh - 1) / wgh;
+  const int kvh = (blockIdx.x % head_groups) * wgh + wave % wgh;
+  const int item = (blockIdx.x / head_groups) * (4 / wgh) + wave / wgh;
+  if (kvh >= a.hkv) return;
+
+  Split it;
+  it.b = it.len = it.p_begin = it.p_end = it.slot = 0;
+  it.count = 1;
+  const bool writer = blockIdx.x == 0 && wave == 0;
+  if (!find_split(a, args.items, item, writer ? a.seq_splits : nullptr, it)) return;  // uniform
+  const int b = __builtin_amdgcn_readfirstlane(it.b);
+  const int len = __builtin_amdgcn_readfirstlane(it.len);
+  const int p_begin = __builtin_amdgcn_readfirstlane(it.p_begin);
+  const int n_pages = max(__builtin_amdgcn_readfirstlane(it.p_end) - p_begin, 0);
+  const int shift = a.page_shift, sub_mask = (1 << shift) - 1;
+
+  // Page ids p_begin + 64 c + lane of the item, clamped into the table row and the pool.
+  const int32_t* row = a.block_tables + (size_t)b * a.bt_stride;
+  auto load_ids = [&](int c) {
+    const long long p = (long long)p_begin + 64 * c + lane;
+    return row[min(p, (long long)a.max_pages - 1) >> shift];
+  };
+  int ids = load_ids(0), ids_next = load_ids(1);
+
+  const WaveRows<NB, 1> map{kvh, a.rows, a.hkv};
+  u4 q[NB][KK];
+  RegBits<NB> bits;
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb) {
+    const int r = map.row(nb, l16);
+    const bool real = map.real(nb, l16);
+    const int qi = real ? r / a.by_group : 0;
+    const int hh = kvh * a.group + (real ? r - qi * a.group : 0);
+    const _Float16* qp = a.q + ((size_t)(b * a.q_len + qi) * a.hq + hh) * HD;
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) {
+      const u4 x = *(const u4*)(qp + KV::q_dims(kk, g16));
+      q[nb][kk] = real ? x : u4{0u, 0u, 0u, 0u};
+    }
+    bits.b[nb] = draft_bits(a, b, qi, real);
+  }
+
+  const unsigned tok_bytes = a.token_stride;
+  const unsigned k_lane = l16 * tok_bytes + kvh * a.head_stride + KV::k_lane_bytes(g16);
+  const unsigned v_lane = 4 * g16 * tok_bytes + kvh * a.head_stride + KV::v_lane_bytes(l16);
+  const size_t sub_bytes = (size_t)kPageSize * tok_bytes;
+  // Lanes 0-31 load the page's K scale, 32-63 its V scale: one instruction, one register.
+  const char* scale_lane =
+      (const char*)(lane < 32 ? args.scales.k : args.scales.v) + kvh * args.scales.head_stride;
+  struct Slot {
+    typename KV::Regs kv;
+    float scale;
+  };
+  // pid < 0: zeros, without touching memory (and some page's scales).
+  auto load_page = [&](int pid, int p, Slot& s) {
+    pid = __builtin_amdgcn_readfirstlane(pid);
+    const size_t off =
+        pid >= 0 ? (size_t)pid * (size_t)a.page_stride + (size_t)(p & sub_mask) * sub_bytes : 0;
+    const int nrec = pid >= 0 ? (int)a.page_extent : 0;
+    const __amdgpu_buffer_rsrc_t kr = __builtin_amdgcn_make_buffer_rsrc(
+        (void*)((const char*)a.k + off), (short)0, nrec, kBufferFlags);
+    const __amdgpu_buffer_rsrc_t vr = __builtin_amdgcn_make_buffer_rsrc(
+        (void*)((const char*)a.v + off), (short)0, nrec, kBufferFlags);
+    s.scale = *(const float*)(scale_lane + max(pid, 0) * args.scales.page_stride);
+    KV::load(s.kv, kr, vr, k_lane, v_lane, tok_bytes);
+  };
+  auto page_id = [&](int i) {  // i within the 64 ids at hand
+    return clamp_page(__builtin_amdgcn_readlane(ids, i & 63), a.num_pages);
+  };
+  Slot ring[D];
+#pragma unroll
+  for (int j = 0; j < D; ++j) load_page(j < n_pages ? page_id(j) : -1, p_begin + j, ring[j]);
+
+  WaveState<NB, HD> st;
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb) {
+    st.m[nb] = -INFINITY;
+    st.l[nb] = 0.f;
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb) st.acc[mb][nb] = f4{0.f, 0.f, 0.f, 0.f};
+  }
+  const int mask_from = len - a.q_len;  // pages with a token from here on are masked
+
+  for (int i = 0; i < n_pages; i += D) {
+    if (((i + D) & 63) == 0) {  // the ring's refills enter the next run of ids
+      ids = ids_next;
+      ids_next = load_ids((i + D) / 64 + 1);
+    }
+#pragma unroll
+    for (int j = 0; j < D; ++j) {
+      const int ii = i + j;
+      if (ii < n_pages) {
+        const int p = p_begin + ii;
+        const float ks = __builtin_bit_cast(
+            float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, ring[j].scale), 0));
+        const float vs = __builtin_bit_cast(
+            float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, ring[j].scale), 32));
+        f4 s[NB];
+        code_scores<NB, HD, E, KV>(s, ring[j].kv, q, a.scale_log2 * ks);
+        const bool masked = (p + 1) * kPageSize > mask_from;  // uniform
+        if (masked) {
+          // After the scale, so that a scale of 0, infinity or NaN leaves them -inf.
+          const int tok0 = p * kPageSize + 4 * g16;
+          mask_scores<NB>(s, bits.b, mask_from, tok0, len);
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (tok0 + e >= len)
+#pragma unroll
+              for (int w = 0; w < Dims<HD>::VW / 2; ++w) ring[j].kv.v[e][w] = 0u;
+        }
+        float lm[NB];
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) lm[nb] = max4(s[nb]);
+        raise_max<NB, HD>(st, lm);
+        if constexpr (KV::kNan)
+          if (masked) nan_values<NB, HD, KV>(st, ring[j].kv, s);
+        u2 hi[NB], lo[NB];
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+          const float mu = st.m[nb] == -INFINITY ? 0.f : st.m[nb];
+          float pr[4], pv[4], sum = 0.f;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            pr[e] = fast_exp2(s[nb][e] - mu);
+            pv[e] = pr[e] * vs;
+          }
+          st.l[nb] += (pr[0] + pr[1]) + (pr[2] + pr[3]);
+          if (masked) {  // a scale that is not finite stays with the tokens that are seen
+#pragma unroll
+            for (int e = 0; e < 4; ++e) pv[e] = pr[e] == 0.f ? 0.f : pv[e];
+          }
+          hi[nb] = ElemBF16::round_p(pv[0], pv[1], pv[2], pv[3], sum, lo[nb]);
+        }
+        u2 av[MB];
+        KV::operand_v(ring[j].kv, av);
+#pragma unroll
+        for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb)
+            st.acc[mb][nb] = ElemBF16::mma_pv(av[mb], hi[nb], lo[nb], st.acc[mb][nb]);
+      }
+      load_page(ii + D < n_pages ? page_id(ii + D) : -1, p_begin + ii + D, ring[j]);
+    }
+  }
+  write_results<NB, HD, E>(a, st, sm_stage + wave * 16 * (HD + 4), map, it.count <= 1, false, b,
+                           (size_t)it.slot, a.hkv, 0);
+}
+
+// ---------------------------------------------------------------------------------
+// Append.
+// ---------------------------------------------------------------------------------
+
+template <bool BF16>
+__device__ __forceinline__ float from_half(unsigned bits) {
+  if constexpr (BF16)
+    return __builtin_bit_cast(float, bits << 16);
+  else
+    return (float)__builtin_bit_cast(_Float16, (unsigned short)bits);
+}
+
+// The token as it is stored: infinities count as the type's largest finite value.
+template <bool BF16>
+__device__ __forceinline__ float finite(float x) {
+  const float top = BF16 ? 3.3895313892515355e38f : 65504.f;
+  return x != x ? x : fminf(fmaxf(x, -top), top);
+}
+
+// Four values in units of the scale -> four codes (bytes, low first). e4m3: no magnitude
+// exceeds 448 by more than a rounding of the quotient, which rounds to 448.
+template <bool INT8>
+__device__ __forceinline__ unsigned encode4(const float (&y)[4]) {
+  if constexpr (INT8) {
+    unsigned w = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float r = fminf(fmaxf(rintf(y[i] == y[i] ? y[i] : 0.f), -127.f), 127.f);
+      w |= ((unsigned)(int)r & 0xffu) << (8 * i);
+    }
+    return w;
+  } else {
+    int w = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
+    return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], w, true);
+  }
+}
+
+template <bool INT8>
+__device__ __forceinline__ float decode(unsigned w, int i) {
+  if constexpr (INT8) {
+    return (float)(signed char)(w >> (8 * i));
+  } else {
+    typedef float f2 __attribute__((ext_vector_type(2)));
+    const f2 lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false);
+    const f2 hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
+    return i < 2 ? lo[i] : hi[i - 2];
+  }
+}
+
+// One block: a cache page's tokens of one kv head, K or V. Its waves (page / 16, at most
+// four) take TPW runs of 16 tokens each and meet for the block's largest magnitude; the
+// workgroup's other waves take other heads. The new tokens are read once and held in
+// registers from the maximum to the codes. A block that keeps earlier tokens of its
+// sequence (the first one, if the new tokens start inside a page) keeps their scale as a
+// lower bound; where it grows, their codes are rounded again in the new one. Slots past
+// the last new token stay as they are.
+template <int HD, int TPW, bool BF16, bool INT8>
+__global__ __launch_bounds__(256) void sqa_append_kernel(AppendArgs a) {
+  constexpr int LPT = HD / 8;       // lanes per token, 8 dims each
+  constexpr int TPI = 64 / LPT;     // tokens per instruction
+  constexpr int NI = 16 / TPI;      // instructions per run of 16 tokens
+  __shared__ float sm_top[4];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+  const int runs = a.page_size / 16;
+  const int wpb = runs < 4 ? runs : 4;  // waves per block
+  const int heads = 4 / wpb;            // heads per workgroup
+  const int head_groups = (a.hkv + heads - 1) / heads;
+  const int which = blockIdx.y;
+  const int h = (blockIdx.x % head_groups) * heads + wave / wpb;
+  const int rest = blockIdx.x / head_groups;
+  const int b = rest / a.touched, at = rest % a.touched;
+  const int len = max(a.seq_lens[b], 0);
+  int fresh = a.new_lens ? a.new_lens[b] : a.q_len;
+  fresh = min(max(fresh, 0), min(a.q_len, len));
+  const int first = len - fresh;             // position of the first new token
+  const int pg = first / a.page_size + at;   // page within the sequence
+  const int base = pg * a.page_size;
+  if (fresh == 0 || base >= len || pg >= a.bt_stride) return;  // uniform over the workgroup
+  const int pid = a.block_tables[(size_t)b * a.bt_stride + pg];
+  if (pid < 0 || pid >= a.num_pages) return;  // uniform: a page that is not there is not written
+  const bool active = h < a.hkv;
+  const int lo = max(first - base, 0), hi = min(len - base, a.page_size);
+  const int token = lane / LPT, dim = 8 * (lane % LPT);
+
+  char* codes = (char*)a.cache[which] + (size_t)pid * a.page_stride + (size_t)h * a.head_stride;
+  const char* src = (const char*)a.src[which] + (long long)b * a.src_batch[which] +
+                    (long long)h * a.src_head[which];
+  float* scale_at = (float*)((char*)(which ? a.scales.v : a.scales.k) +
+                             (size_t)pid * a.scales.page_stride + (size_t)h * a.scales.head_stride);
+  u4 x[TPW][NI];
+  const float old = active ? *scale_at : 0.f;
+  float top = 0.f;
+#pragma unroll
+  for (int t = 0; t < TPW; ++t) {
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const int slot = 16 * ((wave % wpb) * TPW + t) + i * TPI + token;
+      x[t][i] = u4{0u, 0u, 0u, 0u};
+      if (active && slot >= lo && slot < hi)
+        x[t][i] = *(const u4*)(src + (long long)(base + slot - first) * a.src_token[which] +
+                               2 * dim);
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < TPW; ++t)
+#pragma unroll
+    for (int i = 0; i < NI; ++i)
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        // fmaxf passes over NaN.
+        top = fmaxf(top, fabsf(finite<BF16>(from_half<BF16>(x[t][i][w] & 0xffffu))));
+        top = fmaxf(top, fabsf(finite<BF16>(from_half<BF16>(x[t][i][w] >> 16))));
+      }
+#pragma unroll
+  for (int o = 1; o < 64; o *= 2) top = fmaxf(top, __shfl_xor(top, o));
+  if (wpb > 1) {  // uniform
+    if (lane == 0) sm_top[wave] = top;
+    __syncthreads();
+    for (int i = 0; i < wpb; ++i) top = fmaxf(top, sm_top[wave / wpb * wpb + i]);
+  }
+  if (!active) return;
+  float scale = top / code_max(INT8 ? kInt8 : kE4M3);
+  if (lo > 0) scale = fmaxf(scale, old);
+  if (wave % wpb == 0 && lane == 0) *scale_at = scale;
+  const bool again = lo > 0 && scale != old;  // uniform over the block
+#pragma unroll
+  for (int t = 0; t < TPW; ++t) {
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const int slot = 16 * ((wave % wpb) * TPW + t) + i * TPI + token;
+      u2* to = (u2*)(codes + (size_t)slot * a.token_stride + dim);
+      float y[2][4];
+      if (slot >= lo && slot < hi) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const unsigned w = x[t][i][e / 2];
+          const float v = finite<BF16>(from_half<BF16>(e & 1 ? w >> 16 : w & 0xffffu));
+          y[e / 4][e % 4] = scale > 0.f ? v / scale : 0.f;
+        }
+        *to = u2{encode4<INT8>(y[0]), encode4<INT8>(y[1])};
+      } else if (again && slot < lo) {
+        const u2 w = *to;
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          y[e / 4][e % 4] = decode<INT8>(w[e / 4], e % 4) * old / scale;
+        *to = u2{encode4<INT8>(y[0]), encode4<INT8>(y[1])};
+      }
+    }
+  }
+}
+
+template <int HD, bool BF16, bool INT8>
+void launch_append_hd(const AppendArgs& a, dim3 grid, hipStream_t stream) {
+  if (a.page_size <= 64)
+    hipLaunchKernelGGL((sqa_append_kernel<HD, 1, BF16, INT8>), grid, dim3(256), 0, stream, a);
+  else if (a.page_size == 128)
+    hipLaunchKernelGGL((sqa_append_kernel<HD, 2, BF16, INT8>), grid, dim3(256), 0, stream, a);
+  else
+    hipLaunchKernelGGL((sqa_append_kernel<HD, 4, BF16, INT8>), grid, dim3(256), 0, stream, a);
+}
+
+template <bool BF16, bool INT8>
+void launch_append_as(const AppendArgs& a, dim3 grid, hipStream_t stream) {
+  if (a.head_dim == 64)
+    launch_append_hd<64, BF16, INT8>(a, grid, stream);
+  else if (a.head_dim == 128)
+    launch_append_hd<128, BF16, INT8>(a, grid, stream);
+  else
+    launch_append_hd<256, BF16, INT8>(a, grid, stream);
+}
+
+template <typename E, template <int> class KV>
+void launch_scaled_as(const ScaledArgs& a, dim3 grid, hipStream_t stream) {
+  const dim3 block(256);
+  const int rows = a.p.rows;
+  if (a.p.head_dim == 64) {
+    if (rows <= 16)
+      hipLaunchKernelGGL((sqa_scaled_attention_kernel<1, 8, 64, E, KV<64>>), grid, block, 0, stream, a);
+    else if (rows <= 32)
+      hipLaunchKernelGGL((sqa_scaled_attention_kernel<2, 8, 64, E, KV<64>>), grid, block, 0, stream, a);
+    else
+      hipLaunchKernelGGL((sqa_scaled_attention_kernel<4, 4, 64, E, KV<64>>), grid, block, 0, stream, a);
+  } else if (a.p.head_dim == 128) {
+    if (rows <= 16)
+      hipLaunchKernelGGL((sqa_scaled_attention_kernel<1, 4, 128, E, KV<128>>), grid, block, 0, stream, a);
+    else if (rows <= 32)
+      hipLaunchKernelGGL((sqa_scaled_attention_kernel<2, 4, 128, E, KV<128>>), grid, block, 0, stream, a);
+    else
+      hipLaunchKernelGGL((sqa_scaled_attention_kernel<4, 4, 128, E, KV<128>>), grid, block, 0, stream, a);
+  } else {
+    if (rows <= 16)
+      hipLaunchKernelGGL((sqa_scaled_attention_kernel<1, 2, 256, E, KV<256>>), grid, block, 0, stream, a);
+    else
+      hipLaunchKernelGGL((sqa_scaled_attention_kernel<2, 2, 256, E, KV<256>>), grid, block, 0, stream, a);
+  }
+}
+
+}  // namespace
+
+hipError_t launch_scaled(const ScaledArgs& a, hipStream_t stream) {
+  const int head_groups = (a.p.hkv + a.wg_heads - 1) / a.wg_heads;
+  const int per_wg = 4 / a.wg_heads;
+  const int items = a.items > a.p.batch ? a.items : a.p.batch;
+  const dim3 grid((unsigned)((items + per_wg - 1) / per_wg * head_groups));
+  if (a.p.bf16) {
+    if (a.int8)
+      launch_scaled_as<ElemBF16, CodesInt8>(a, grid, stream);
+    else
+      launch_scaled_as<ElemBF16, CodesFp8>(a, grid, stream);
+  } else {
+    if (a.int8)
+      launch_scaled_as<ElemF16, CodesInt8>(a, grid, stream);
+    else
+      launch_scaled_as<ElemF16, CodesFp8>(a, grid, stream);
+  }
+  return hipGetLastError();
+}
+
+hipError_t launch_append(const AppendArgs& a, hipStream_t stream) {
+  const int runs = a.page_size / 16;
+  const int heads = 4 / (runs < 4 ? runs : 4);
+  const int head_groups = (a.hkv + heads - 1) / heads;
+  const dim3 grid((unsigned)((long long)a.batch * a.touched * head_groups), 2);
+  if (a.bf16) {
+    if (a.int8)
+      launch_append_as<true, true>(a, grid, stream);
+    else
+      launch_append_as<true, false>(a, grid, stream);
+  } else {
+    if (a.int8)
+      launch_append_as<false, true>(a, grid, stream);
+    else
+      launch_append_as<false, false>(a, grid, stream);
+  }
+  return hipGetLastError();
+}
+
+}  // namespace sqa

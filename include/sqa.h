@@ -325,6 +325,118 @@ typedef struct sqa_append_args {
  */
 int sqa_append_scaled(const sqa_append_args* args);
 
+/*
+ * Arguments of sqa_attention_weights (set struct_size = sizeof(sqa_weights_args)).
+ *   kv            K of the cache (v is not read); kv_dtype: `dtype`, or e4m3 or int8 codes
+ *   k_scale       block scales of codes (strides in floats); NULL: codes as they are (e4m3)
+ *   weights       [batch, num_kv_heads, weights_width] fp32, strides in floats
+ *   max_seq_len   > 0: no sequence is longer (tokens past it are not looked at)
+ *   max_pages     block_tables columns
+ *   query, seq_lens, draft_mask, scale, dtype as for sqa_paged_attention;
+ *   workspace     sqa_weights_workspace_bytes(...) bytes, 16-byte aligned
+ */
+typedef struct sqa_weights_args {
+  size_t struct_size;
+  const void* query;
+  sqa_kv_cache kv;
+  const float* k_scale;
+  int64_t scale_page_stride;
+  int64_t scale_head_stride;
+  const int32_t* block_tables;
+  const int32_t* seq_lens;
+  const uint32_t* draft_mask;
+  float* weights;
+  int64_t weights_batch_stride;
+  int64_t weights_head_stride;
+  int weights_width;
+  int max_pages;
+  int mask_words;
+  float scale;
+  int batch;
+  int q_len;
+  int num_query_heads;
+  int num_kv_heads;
+  int head_dim;
+  int page_size;
+  int max_seq_len;
+  int dtype;
+  int kv_dtype;
+  void* workspace;
+  size_t workspace_bytes;
+  void* stream;
+} sqa_weights_args;
+
+/* Workspace of sqa_attention_weights on `device`; max_pages counts 16-token pages here. 0
+ * on error. */
+size_t sqa_weights_workspace_bytes(int device, int batch, int q_len, int num_query_heads,
+                                   int num_kv_heads, int head_dim, int max_seq_len, int max_pages,
+                                   int kv_dtype);
+
+/*
+ * Adds up the attention weight every cached token receives: weights[b][h][t] +=
+ * the softmax probabilities of token t over the rows of kv head h (q_len draft tokens x
+ * the head's query heads), for the tokens before the draft block; the last q_len tokens'
+ * weights are set to theirs (they start with this call). Tokens at weights_width and past
+ * it are not recorded. Equal inputs give equal bits.
+ */
+int sqa_attention_weights(const sqa_weights_args* args);
+
+/*
+ * Arguments of sqa_evict (set struct_size = sizeof(sqa_evict_args)).
+ *   weights       [batch, num_kv_heads, weights_width], of every token
+ *   new_weights   [batch, num_kv_heads, new_weights_width >= budget]; may be `weights`
+ *   kept          [batch, num_kv_heads, budget] int32, contiguous
+ *   kv, scales    the cache the tokens are in (scales.k NULL: none), tables
+ *                 [batch, max_pages], lengths seq_lens
+ *   into, into_scales  where they go, pages new_tables [batch, new_max_pages]; may be the
+ *                 same pool, on pages no row of block_tables uses
+ *   new_lens      [batch], written
+ * Strides of kv and into must be multiples of 16 bytes.
+ */
+typedef struct sqa_evict_args {
+  size_t struct_size;
+  const float* weights;
+  int64_t weights_batch_stride;
+  int64_t weights_head_stride;
+  float* new_weights;
+  int64_t new_weights_batch_stride;
+  int64_t new_weights_head_stride;
+  int32_t* kept;
+  const int32_t* seq_lens;
+  int32_t* new_lens;
+  sqa_kv_cache kv;
+  sqa_kv_cache into;
+  sqa_block_scales scales;
+  sqa_block_scales into_scales;
+  const int32_t* block_tables;
+  const int32_t* new_tables;
+  int weights_width;
+  int new_weights_width;
+  int max_pages;
+  int new_max_pages;
+  int budget;
+  int sink;
+  int recent;
+  int batch;
+  int num_kv_heads;
+  int head_dim;
+  int page_size;
+  int kv_dtype;
+  void* stream;
+} sqa_evict_args;
+
+/*
+ * Keeps at most `budget` tokens of every sequence, for each kv head its own: the first
+ * `sink`, the last `recent`, and the heaviest of those between (NaN the lightest; of equal
+ * ones the earlier). They move in their order to the slots 0 .. of the new pages, their
+ * positions before go to kept (-1 past them), their weights to new_weights (0 past them),
+ * min(seq_lens[b], budget) to new_lens. Sequences within the budget move whole. In scaled
+ * caches a new block's scale is the largest of those its tokens come from, and codes from
+ * blocks of smaller scales are rounded again, code * old / new. Slots past a sequence's
+ * end, and pages whose id is outside the pool, are not written.
+ */
+int sqa_evict(const sqa_evict_args* args);
+
 /* Compute units of `device` (256 on MI355X), or -1 on error. */
 int sqa_device_cu_count(int device);
 

@@ -34,6 +34,9 @@ _SIGNATURES = [
     ("sqa_plan_scaled", _C.c_int, [_C.c_int] * 5 + [_C.POINTER(_C.c_int)]),
     ("sqa_paged_attention_scaled", _C.c_int, [_C.c_void_p, _C.c_void_p]),
     ("sqa_append_scaled", _C.c_int, [_C.c_void_p]),
+    ("sqa_weights_workspace_bytes", _C.c_size_t, [_C.c_int] * 9),
+    ("sqa_attention_weights", _C.c_int, [_C.c_void_p]),
+    ("sqa_evict", _C.c_int, [_C.c_void_p]),
     ("sqa_device_cu_count", _C.c_int, [_C.c_int]),
     ("sqa_last_error", _C.c_char_p, []),
     ("sqa_version", _C.c_char_p, []),
@@ -83,6 +86,39 @@ class AppendArgs(ctypes.Structure):
                 ("kv_dtype", _C.c_int), ("stream", _C.c_void_p)]
 
 
+class WeightsArgs(ctypes.Structure):
+    """``sqa_weights_args`` of include/sqa.h."""
+
+    _fields_ = [("struct_size", _C.c_size_t), ("query", _C.c_void_p), ("kv", KVCache),
+                ("k_scale", _C.c_void_p), ("scale_page_stride", _C.c_int64),
+                ("scale_head_stride", _C.c_int64), ("block_tables", _C.c_void_p),
+                ("seq_lens", _C.c_void_p), ("draft_mask", _C.c_void_p), ("weights", _C.c_void_p),
+                ("weights_batch_stride", _C.c_int64), ("weights_head_stride", _C.c_int64),
+                ("weights_width", _C.c_int), ("max_pages", _C.c_int), ("mask_words", _C.c_int),
+                ("scale", _C.c_float), ("batch", _C.c_int), ("q_len", _C.c_int),
+                ("num_query_heads", _C.c_int), ("num_kv_heads", _C.c_int),
+                ("head_dim", _C.c_int), ("page_size", _C.c_int), ("max_seq_len", _C.c_int),
+                ("dtype", _C.c_int), ("kv_dtype", _C.c_int), ("workspace", _C.c_void_p),
+                ("workspace_bytes", _C.c_size_t), ("stream", _C.c_void_p)]
+
+
+class EvictArgs(ctypes.Structure):
+    """``sqa_evict_args`` of include/sqa.h."""
+
+    _fields_ = [("struct_size", _C.c_size_t), ("weights", _C.c_void_p),
+                ("weights_batch_stride", _C.c_int64), ("weights_head_stride", _C.c_int64),
+                ("new_weights", _C.c_void_p), ("new_weights_batch_stride", _C.c_int64),
+                ("new_weights_head_stride", _C.c_int64), ("kept", _C.c_void_p),
+                ("seq_lens", _C.c_void_p), ("new_lens", _C.c_void_p), ("kv", KVCache),
+                ("into", KVCache), ("scales", BlockScales), ("into_scales", BlockScales),
+                ("block_tables", _C.c_void_p), ("new_tables", _C.c_void_p),
+                ("weights_width", _C.c_int), ("new_weights_width", _C.c_int),
+                ("max_pages", _C.c_int), ("new_max_pages", _C.c_int), ("budget", _C.c_int),
+                ("sink", _C.c_int), ("recent", _C.c_int), ("batch", _C.c_int),
+                ("num_kv_heads", _C.c_int), ("head_dim", _C.c_int), ("page_size", _C.c_int),
+                ("kv_dtype", _C.c_int), ("stream", _C.c_void_p)]
+
+
 # AttentionArgs as one packed record (native sizes and alignment, padded as C does).
 _ARGS = struct.Struct("@N2P2P4q2PiPi2f8iPN2P3i0q")
 assert _ARGS.size == ctypes.sizeof(AttentionArgs)
@@ -90,6 +126,10 @@ _SCALES = struct.Struct("@2P2q")
 assert _SCALES.size == ctypes.sizeof(BlockScales)
 _APPEND = struct.Struct("@N2P6q2P4q2P2q3P8iP0q")
 assert _APPEND.size == ctypes.sizeof(AppendArgs)
+_WEIGHTS = struct.Struct("@N3P4qP2q4P2q3if9iPNP0q")
+assert _WEIGHTS.size == ctypes.sizeof(WeightsArgs)
+_EVICT = struct.Struct("@NP2qP2q3P2P4q2P4q2P2q2P2q2P12iP0q")
+assert _EVICT.size == ctypes.sizeof(EvictArgs)
 
 DTYPE_F16, DTYPE_BF16, DTYPE_FP8_E4M3, DTYPE_INT8 = 0, 1, 2, 3
 FLAG_ADAPTIVE_PAIRS = 1  # SQA_FLAG_ADAPTIVE_PAIRS
@@ -316,6 +356,67 @@ def launch_append(key, value, k_view, v_view, k_scale, v_scale, block_tables, se
     rc = lib.sqa_append_scaled(a)
     if rc != SQA_OK:
         raise RuntimeError(f"sqa_append_scaled failed: {last_error(lib)}")
+
+
+@functools.lru_cache(maxsize=4096)
+def weights_workspace_bytes(device_index: int, batch: int, q_len: int, num_query_heads: int,
+                            num_kv_heads: int, head_dim: int, max_seq_len: int, max_pages: int,
+                            kv_dtype: int) -> int:
+    """``sqa_weights_workspace_bytes`` (``max_pages``: 16-token pages)."""
+    lib = load()
+    need = lib.sqa_weights_workspace_bytes(device_index, batch, q_len, num_query_heads,
+                                           num_kv_heads, head_dim, max_seq_len, max_pages,
+                                           kv_dtype)
+    if need == 0:
+        raise RuntimeError(f"sqa_weights_workspace_bytes failed: {last_error(lib)}")
+    return need
+
+
+def launch_weights(query, k_view, k_scale, block_tables, seq_lens, draft_mask, weights,
+                   scale: float, max_seq_len: int, workspace, stream_handle: int):
+    """Call ``sqa_attention_weights`` (``k_scale`` ``None``: none; ``weights`` ``[B, Hkv, T]``
+    float32 with a contiguous last dimension)."""
+    lib = _LIB if _LIB is not None else load()
+    b, q_len, hq, d = query.shape
+    ks, ws = k_view.stride(), weights.stride()
+    sc = (0, 0, 0) if k_scale is None else (k_scale.data_ptr(), *k_scale.stride())
+    words, mask_words = (0, 0) if draft_mask is None else (draft_mask.data_ptr(),
+                                                           draft_mask.shape[-1])
+    a = _WEIGHTS.pack(
+        _WEIGHTS.size, query.data_ptr(), k_view.data_ptr(), 0, k_view.shape[0], ks[0], ks[1], ks[2],
+        *sc, block_tables.data_ptr(), seq_lens.data_ptr(), words, weights.data_ptr(), ws[0], ws[1],
+        weights.shape[2], block_tables.shape[1], mask_words, scale, b, q_len, hq, k_view.shape[2],
+        d, k_view.shape[1], max_seq_len, dtype_code(query.dtype), dtype_code(k_view.dtype),
+        workspace.data_ptr(), workspace.numel() * workspace.element_size(), stream_handle or 0)
+    rc = lib.sqa_attention_weights(a)
+    if rc != SQA_OK:
+        raise RuntimeError(f"sqa_attention_weights failed: {last_error(lib)}")
+
+
+def launch_evict(weights, new_weights, kept, seq_lens, new_lens, source, into, block_tables,
+                 new_tables, budget: int, sink: int, recent: int, stream_handle: int):
+    """Call ``sqa_evict``. ``source``, ``into``: (K view, V view, K scale, V scale), the
+    scales ``None`` where the cache has none."""
+    lib = _LIB if _LIB is not None else load()
+
+    def pool(k, v, *_):
+        return (k.data_ptr(), v.data_ptr(), k.shape[0], *k.stride()[:3])
+
+    def scales(_k, _v, ks, vs):
+        return (0, 0, 0, 0) if ks is None else (ks.data_ptr(), vs.data_ptr(), *ks.stride())
+
+    k = source[0]
+    a = _EVICT.pack(
+        _EVICT.size, weights.data_ptr(), weights.stride(0), weights.stride(1),
+        new_weights.data_ptr(), new_weights.stride(0), new_weights.stride(1), kept.data_ptr(),
+        seq_lens.data_ptr(), new_lens.data_ptr(), *pool(*source), *pool(*into), *scales(*source),
+        *scales(*into), block_tables.data_ptr(), new_tables.data_ptr(), weights.shape[2],
+        new_weights.shape[2], block_tables.shape[1], new_tables.shape[1], budget, sink, recent,
+        weights.shape[0], weights.shape[1], k.shape[3], k.shape[1], dtype_code(k.dtype),
+        stream_handle or 0)
+    rc = lib.sqa_evict(a)
+    if rc != SQA_OK:
+        raise RuntimeError(f"sqa_evict failed: {last_error(lib)}")
 
 
 def run(query, key_cache, value_cache, block_tables, seq_lens, num_splits: int,

@@ -123,3 +123,22 @@ def append_scaled_kv(key: torch.Tensor, value: torch.Tensor, key_cache: torch.Te
 def _append_scaled_kv_fake(key, value, key_cache, value_cache, key_scale, value_scale,
                            block_tables, seq_lens, new_lens):
     return None
+
+
+@torch.library.custom_op("sqa::accumulate_attention_weights", mutates_args=("weights",))
+def accumulate_attention_weights(query: torch.Tensor, key_cache: torch.Tensor,
+                                 key_scale: Optional[torch.Tensor], block_tables: torch.Tensor,
+                                 seq_lens: torch.Tensor, draft_mask: Optional[torch.Tensor],
+                                 weights: torch.Tensor, scale: float, max_seq_len: int) -> None:
+    """Attention weights added up in place (``eviction``)."""
+    from . import eviction, scaled_cache
+
+    scaled_cache.on_device(query.device, lambda: eviction.run_weights(
+        query, key_cache, key_scale, block_tables, seq_lens, draft_mask, weights, scale,
+        max_seq_len))
+
+
+@accumulate_attention_weights.register_fake
+def _accumulate_attention_weights_fake(query, key_cache, key_scale, block_tables, seq_lens,
+                                       draft_mask, weights, scale, max_seq_len):
+    return None

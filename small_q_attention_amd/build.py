@@ -30,9 +30,9 @@ CSRC = PKG_DIR / "csrc"
 INCLUDE = REPO_DIR / "include"
 LIB_PATH = PKG_DIR / "libsqa.so"
 SOURCES = [CSRC / name for name in ("sqa_kernels.hip", "sqa_capi.hip", "sqa_scaled.hip",
-                                    "sqa_cache_capi.hip")]
-HEADERS = [CSRC / "sqa_internal.h", CSRC / "sqa_device.h", CSRC / "sqa_cache.h",
-           INCLUDE / "sqa.h"]
+                                    "sqa_evict.hip", "sqa_cache_capi.hip")]
+HEADERS = [CSRC / "sqa_internal.h", CSRC / "sqa_device.h", CSRC / "sqa_cache_device.h",
+           CSRC / "sqa_cache.h", INCLUDE / "sqa.h"]
 ARCH = "gfx950"
 
 
@@ -101,7 +101,7 @@ def _compile(output: Path, verbose: bool):
         return subprocess.run(cmd, capture_output=True, text=True)
 
     try:
-        with ThreadPoolExecutor(max_workers=4) as pool:
+        with ThreadPoolExecutor(max_workers=len(SOURCES)) as pool:
             done = list(pool.map(run, steps))
         if not any(res.returncode for res in done):
             done.append(run(link))

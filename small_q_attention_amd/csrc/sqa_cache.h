@@ -49,4 +49,52 @@ struct AppendArgs {
 };
 hipError_t launch_append(const AppendArgs& a, hipStream_t stream);
 
+// Whether the scores of a call travel from its first to its second kernel through memory:
+// 4 bytes per row and token written and read again, against K read a second time.
+__host__ __device__ constexpr bool weights_stored(long long rows, int head_dim, int kv_bytes) {
+  return 8 * rows <= (long long)head_dim * kv_bytes;
+}
+
+// Attention weights added up. Of `p` the fields of the query side, of K and of the tables.
+struct WeighArgs {
+  PartialArgs p;
+  const float* k_scale;        // NULL: 1
+  long long scale_page;        // strides in bytes
+  unsigned scale_head;
+  int items;                   // work items of the cut
+  int wg_heads;
+  int kv_type;                 // kF16, kBF16, kE4M3 or kInt8
+  float* weights;              // [B, Hkv, width]
+  long long w_batch, w_head;   // strides in floats
+  int width;
+  float2* stats;               // [Hkv][rows][items]: (max in log2 units, sum) of each item
+  float* scores;               // [B][Hkv][pages][rows][16] in log2 units, or NULL: the second
+                               // kernel computes them again
+};
+hipError_t launch_weigh(const WeighArgs& a, hipStream_t stream);
+
+struct EvictArgs {
+  const float* weights;        // [B, Hkv, width]
+  long long w_batch, w_head;   // strides in floats
+  int width;
+  float* new_weights;          // [B, Hkv, new_width]; may be `weights`
+  long long nw_batch, nw_head;
+  int new_width;
+  int32_t* kept;               // [B, Hkv, budget]
+  const int32_t* seq_lens;
+  int32_t* new_lens;
+  int budget, sink, recent;
+  const char* src[2];          // K and V
+  char* dst[2];
+  long long src_page, src_token, src_head, dst_page, dst_token, dst_head;  // bytes
+  BlockScales src_scales, dst_scales;
+  const int32_t* block_tables;
+  const int32_t* new_tables;
+  int bt_stride, new_stride;
+  long long num_pages, new_pages;
+  int batch, hkv, head_dim, page_size;
+  int kv_type, scaled;
+};
+hipError_t launch_evict(const EvictArgs& a, hipStream_t stream);
+
 }  // namespace sqa

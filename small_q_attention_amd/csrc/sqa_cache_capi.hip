@@ -86,6 +86,35 @@ long long scaled_items(int cus, int num_kv_heads) {
   return ceil_div(cus, ceil_div(num_kv_heads, wgh)) * (4 / wgh);
 }
 
+// Plan of sqa_attention_weights: work items and the parts of its workspace.
+struct WeighPlan {
+  long long rows, pages, items;
+  size_t stats, scores;  // bytes
+};
+
+// Scores past this are computed twice instead (a wide table under a large batch).
+constexpr size_t kMostScores = (size_t)1 << 30;
+
+int weigh_plan(int device, int batch, int q_len, int num_query_heads, int num_kv_heads,
+               int head_dim, int max_seq_len, int max_pages, int kv_dtype, WeighPlan* plan) {
+  if (batch <= 0 || q_len <= 0 || num_kv_heads <= 0 || num_query_heads <= 0 || max_pages <= 0)
+    return fail(SQA_ERR_INVALID, "batch, q_len, heads and max_pages must be positive");
+  const int cus = sqa_device_cu_count(device);
+  if (cus <= 0) return SQA_ERR_HIP;
+  plan->rows = (long long)q_len * (num_query_heads / num_kv_heads);
+  plan->pages = max_pages;
+  if (max_seq_len > 0) plan->pages = std::min(plan->pages, ceil_div(max_seq_len, sqa::kPageSize));
+  const long long most = batch * ceil_div(plan->pages, sqa::kMinSplitPages);
+  // Two workgroups per compute unit.
+  plan->items = std::max((long long)batch, std::min(2 * scaled_items(cus, num_kv_heads), most));
+  plan->stats = (size_t)plan->items * num_kv_heads * plan->rows * sizeof(float2);
+  plan->scores = (size_t)batch * num_kv_heads * plan->pages * sqa::kPageSize * plan->rows * 4;
+  if (!sqa::weights_stored(plan->rows, head_dim, is_codes(kv_dtype) ? 1 : 2) ||
+      plan->scores > kMostScores)
+    plan->scores = 0;
+  return SQA_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -309,6 +338,225 @@ int sqa_append_scaled(const sqa_append_args* args) {
     return fail(SQA_ERR_INVALID, "grid too large");
   hipError_t e = sqa::launch_append(k, (hipStream_t)a.stream);
   return e == hipSuccess ? SQA_OK : hip_fail(e, "append kernel launch");
+}
+
+size_t sqa_weights_workspace_bytes(int device, int batch, int q_len, int num_query_heads,
+                                   int num_kv_heads, int head_dim, int max_seq_len, int max_pages,
+                                   int kv_dtype) {
+  WeighPlan plan;
+  if (weigh_plan(device, batch, q_len, num_query_heads, num_kv_heads, head_dim, max_seq_len,
+                 max_pages, kv_dtype, &plan))
+    return 0;
+  return plan.stats + plan.scores;
+}
+
+int sqa_attention_weights(const sqa_weights_args* args) {
+  if (!args) return fail(SQA_ERR_INVALID, "null argument struct");
+  if (args->struct_size != sizeof(sqa_weights_args))
+    return fail(SQA_ERR_INVALID, "struct_size %zu does not match this library's %zu",
+                args->struct_size, sizeof(sqa_weights_args));
+  const sqa_weights_args& a = *args;
+  if (!a.query || !a.kv.k || !a.block_tables || !a.seq_lens || !a.weights)
+    return fail(SQA_ERR_INVALID, "null tensor pointer");
+  if (int rc = check_cache(a.batch, a.num_kv_heads, a.head_dim, a.page_size, a.kv.num_pages,
+                           a.max_pages))
+    return rc;
+  if (a.q_len <= 0 || a.num_query_heads <= 0 || a.num_query_heads % a.num_kv_heads)
+    return fail(SQA_ERR_INVALID,
+                "q_len and num_query_heads must be positive, heads divisible by num_kv_heads");
+  const int group = a.num_query_heads / a.num_kv_heads;
+  const long long rows = (long long)a.q_len * group;
+  const int max_rows = a.head_dim == 256 ? sqa::kMaxRowsHd256 : sqa::kMaxRows;
+  if (rows > max_rows)
+    return fail(SQA_ERR_UNSUPPORTED, "q_len * group = %lld exceeds %d at head_dim %d", rows,
+                max_rows, a.head_dim);
+  if (a.dtype != SQA_DTYPE_F16 && a.dtype != SQA_DTYPE_BF16)
+    return fail(SQA_ERR_UNSUPPORTED, "dtype must be SQA_DTYPE_F16 or SQA_DTYPE_BF16 (got %d)",
+                a.dtype);
+  if (a.kv_dtype != a.dtype && !is_codes(a.kv_dtype))
+    return fail(SQA_ERR_UNSUPPORTED, "kv_dtype must be dtype or an 8-bit type (got %d)",
+                a.kv_dtype);
+  if (a.k_scale && !is_codes(a.kv_dtype))
+    return fail(SQA_ERR_INVALID, "scales belong to 8-bit caches");
+  if (a.kv_dtype == SQA_DTYPE_INT8 && !a.k_scale)
+    return fail(SQA_ERR_INVALID, "int8 caches need scales");
+  if (a.k_scale) {
+    const sqa_block_scales sc = {a.k_scale, nullptr, a.scale_page_stride, a.scale_head_stride};
+    if (int rc = check_scales(sc, false)) return rc;
+  }
+  const int bytes = is_codes(a.kv_dtype) ? 1 : 2;
+  long long extent = 0;
+  sqa_kv_cache kv = a.kv;
+  kv.v = nullptr;
+  if (int rc = check_strides(kv, bytes, a.num_kv_heads, a.head_dim, &extent)) return rc;
+  if ((uintptr_t)a.query % 16) return fail(SQA_ERR_INVALID, "query must be 16-byte aligned");
+  if (((uintptr_t)a.block_tables | (uintptr_t)a.seq_lens | (uintptr_t)a.draft_mask |
+       (uintptr_t)a.weights) % 4)
+    return fail(SQA_ERR_INVALID,
+                "block_tables, seq_lens, draft_mask and weights must be 4-byte aligned");
+  if (a.draft_mask && (a.mask_words < (a.q_len + 31) / 32 || a.mask_words > 2))
+    return fail(SQA_ERR_INVALID, "draft_mask needs %d..2 words per row, got %d",
+                (a.q_len + 31) / 32, a.mask_words);
+  if (!(a.scale > 0.f) || !isfinite(a.scale))
+    return fail(SQA_ERR_INVALID, "scale must be positive and finite");
+  if (a.weights_width <= 0 || a.weights_batch_stride < 0 || a.weights_head_stride < 0)
+    return fail(SQA_ERR_INVALID, "weights need a positive width and non-negative strides");
+  int device = -1;
+  if (hipError_t e = hipGetDevice(&device); e != hipSuccess) return hip_fail(e, "hipGetDevice");
+  const int shift = page_shift_of(a.page_size);
+  WeighPlan plan;
+  if (int rc = weigh_plan(device, a.batch, a.q_len, a.num_query_heads, a.num_kv_heads, a.head_dim,
+                          a.max_seq_len, a.max_pages << shift, a.kv_dtype, &plan))
+    return rc;
+  if (plan.items * a.num_kv_heads > 0x7fffffffLL) return fail(SQA_ERR_INVALID, "grid too large");
+  const size_t need = plan.stats + plan.scores;
+  if (!a.workspace || a.workspace_bytes < need)
+    return fail(SQA_ERR_WORKSPACE, "workspace of %zu bytes needed, %zu given", need,
+                a.workspace ? a.workspace_bytes : (size_t)0);
+  if ((uintptr_t)a.workspace % 16)
+    return fail(SQA_ERR_WORKSPACE, "workspace must be 16-byte aligned");
+
+  sqa::WeighArgs w;
+  memset(&w, 0, sizeof(w));
+  sqa::PartialArgs& p = w.p;
+  p.q = (const _Float16*)a.query;
+  p.k = (const _Float16*)a.kv.k;
+  p.block_tables = a.block_tables;
+  p.seq_lens = a.seq_lens;
+  p.draft_mask = a.draft_mask;
+  p.mask_words = a.draft_mask ? a.mask_words : 0;
+  p.num_pages = a.kv.num_pages;
+  p.page_stride = bytes * a.kv.page_stride;
+  p.token_stride = (unsigned)(bytes * a.kv.token_stride);
+  p.head_stride = (unsigned)(bytes * a.kv.head_stride);
+  p.page_extent = (unsigned)extent;
+  p.batch = a.batch;
+  p.q_len = a.q_len;
+  p.hq = a.num_query_heads;
+  p.hkv = a.num_kv_heads;
+  p.group = group;
+  p.rows = (int)rows;
+  p.head_dim = a.head_dim;
+  p.bt_stride = a.max_pages;
+  p.page_shift = shift;
+  p.max_pages = (int)plan.pages;
+  p.by_group = sqa::fast_div(group);
+  p.scale_log2 = (float)(1.4426950408889634 * (double)a.scale);
+  p.bf16 = a.dtype == SQA_DTYPE_BF16;
+  w.k_scale = a.k_scale;
+  w.scale_page = 4 * (long long)a.scale_page_stride;
+  w.scale_head = (unsigned)(4 * a.scale_head_stride);
+  w.items = (int)plan.items;
+  w.wg_heads = wg_heads(a.num_kv_heads);
+  w.kv_type = a.kv_dtype;
+  w.weights = a.weights;
+  w.w_batch = a.weights_batch_stride;
+  w.w_head = a.weights_head_stride;
+  w.width = a.weights_width;
+  // The scores first: 16-byte stores.
+  w.scores = plan.scores ? (float*)a.workspace : nullptr;
+  w.stats = (float2*)((char*)a.workspace + plan.scores);
+  hipError_t e = sqa::launch_weigh(w, (hipStream_t)a.stream);
+  return e == hipSuccess ? SQA_OK : hip_fail(e, "attention weights kernel launch");
+}
+
+int sqa_evict(const sqa_evict_args* args) {
+  if (!args) return fail(SQA_ERR_INVALID, "null argument struct");
+  if (args->struct_size != sizeof(sqa_evict_args))
+    return fail(SQA_ERR_INVALID, "struct_size %zu does not match this library's %zu",
+                args->struct_size, sizeof(sqa_evict_args));
+  const sqa_evict_args& a = *args;
+  if (!a.weights || !a.new_weights || !a.kept || !a.seq_lens || !a.new_lens || !a.kv.k ||
+      !a.kv.v || !a.into.k || !a.into.v || !a.block_tables || !a.new_tables)
+    return fail(SQA_ERR_INVALID, "null tensor pointer");
+  if (int rc = check_cache(a.batch, a.num_kv_heads, a.head_dim, a.page_size, a.kv.num_pages,
+                           a.max_pages))
+    return rc;
+  if (int rc = check_cache(a.batch, a.num_kv_heads, a.head_dim, a.page_size, a.into.num_pages,
+                           a.new_max_pages))
+    return rc;
+  if (a.kv_dtype != SQA_DTYPE_F16 && a.kv_dtype != SQA_DTYPE_BF16 && !is_codes(a.kv_dtype))
+    return fail(SQA_ERR_UNSUPPORTED, "unknown kv_dtype %d", a.kv_dtype);
+  const int bytes = is_codes(a.kv_dtype) ? 1 : 2;
+  long long extent = 0;
+  for (const sqa_kv_cache* c : {&a.kv, &a.into}) {
+    if (int rc = check_strides(*c, bytes, a.num_kv_heads, a.head_dim, &extent)) return rc;
+    const int64_t any = c->page_stride | c->token_stride | c->head_stride;
+    if (any * bytes % 16)
+      return fail(SQA_ERR_INVALID, "cache strides must be multiples of 16 bytes");
+  }
+  const bool scaled = a.scales.k != nullptr;
+  if (scaled && !is_codes(a.kv_dtype))
+    return fail(SQA_ERR_INVALID, "scales belong to 8-bit caches");
+  if (a.kv_dtype == SQA_DTYPE_INT8 && !scaled)
+    return fail(SQA_ERR_INVALID, "int8 caches need scales");
+  if (scaled) {
+    if (int rc = check_scales(a.scales, true)) return rc;
+    if (int rc = check_scales(a.into_scales, true)) return rc;
+  }
+  if (a.budget <= 0 || a.sink < 0 || a.recent < 0 || (long long)a.sink + a.recent > a.budget)
+    return fail(SQA_ERR_INVALID,
+                "budget must be positive and hold sink + recent tokens (got %d, %d, %d)", a.budget,
+                a.sink, a.recent);
+  if (a.budget > (long long)a.new_max_pages * a.page_size)
+    return fail(SQA_ERR_INVALID, "new_tables rows hold %lld tokens, the budget is %d",
+                (long long)a.new_max_pages * a.page_size, a.budget);
+  if (a.weights_width <= 0 || a.new_weights_width < a.budget)
+    return fail(SQA_ERR_INVALID, "weights must not be empty, new_weights hold the budget");
+  if (a.weights_batch_stride < 0 || a.weights_head_stride < 0 || a.new_weights_batch_stride < 0 ||
+      a.new_weights_head_stride < 0)
+    return fail(SQA_ERR_INVALID, "strides must not be negative");
+  if (((uintptr_t)a.weights | (uintptr_t)a.new_weights | (uintptr_t)a.kept |
+       (uintptr_t)a.seq_lens | (uintptr_t)a.new_lens | (uintptr_t)a.block_tables |
+       (uintptr_t)a.new_tables) % 4)
+    return fail(SQA_ERR_INVALID, "weights, lengths and tables must be 4-byte aligned");
+  const long long grid =
+      (long long)a.batch * ceil_div(a.budget, sqa::kPageSize) * ceil_div(a.num_kv_heads, 4);
+  if (grid > 0x7fffffffLL || (long long)a.batch * a.num_kv_heads > 0x7fffffffLL)
+    return fail(SQA_ERR_INVALID, "grid too large");
+
+  sqa::EvictArgs k;
+  memset(&k, 0, sizeof(k));
+  k.weights = a.weights;
+  k.w_batch = a.weights_batch_stride;
+  k.w_head = a.weights_head_stride;
+  k.width = a.weights_width;
+  k.new_weights = a.new_weights;
+  k.nw_batch = a.new_weights_batch_stride;
+  k.nw_head = a.new_weights_head_stride;
+  k.new_width = a.new_weights_width;
+  k.kept = a.kept;
+  k.seq_lens = a.seq_lens;
+  k.new_lens = a.new_lens;
+  k.budget = a.budget;
+  k.sink = a.sink;
+  k.recent = a.recent;
+  k.src[0] = (const char*)a.kv.k;
+  k.src[1] = (const char*)a.kv.v;
+  k.dst[0] = (char*)a.into.k;
+  k.dst[1] = (char*)a.into.v;
+  k.src_page = bytes * a.kv.page_stride;
+  k.src_token = bytes * a.kv.token_stride;
+  k.src_head = bytes * a.kv.head_stride;
+  k.dst_page = bytes * a.into.page_stride;
+  k.dst_token = bytes * a.into.token_stride;
+  k.dst_head = bytes * a.into.head_stride;
+  k.src_scales = scales_of(a.scales);
+  k.dst_scales = scales_of(a.into_scales);
+  k.block_tables = a.block_tables;
+  k.new_tables = a.new_tables;
+  k.bt_stride = a.max_pages;
+  k.new_stride = a.new_max_pages;
+  k.num_pages = a.kv.num_pages;
+  k.new_pages = a.into.num_pages;
+  k.batch = a.batch;
+  k.hkv = a.num_kv_heads;
+  k.head_dim = a.head_dim;
+  k.page_size = a.page_size;
+  k.kv_type = a.kv_dtype;
+  k.scaled = scaled;
+  hipError_t e = sqa::launch_evict(k, (hipStream_t)a.stream);
+  return e == hipSuccess ? SQA_OK : hip_fail(e, "eviction kernel launch");
 }
 
 }  // extern "C"

@@ -1,0 +1,128 @@
+// Device code of the kernels around the paged cache: the cut of a batch of sequences into
+// work items, and the codes of 8-bit caches.
+#pragma once
+
+#include "sqa_device.h"
+
+#include <type_traits>
+
+namespace sqa {
+namespace {
+
+// A split of one sequence.
+struct Split {
+  int b, len;          // sequence and its length
+  int p_begin, p_end;  // kernel pages
+  int count;           // splits of the sequence
+  int slot;            // its work item, and partial slot
+  int first;           // work item of the sequence's first split
+};
+
+__device__ __forceinline__ int wave_sum_int(int x) {
+  return __builtin_amdgcn_readlane(wave_inclusive_scan_int(x), 63);
+}
+
+// The cut of the batch into work items, found by every wave for itself from the lengths:
+// sequence b takes n_b = max(1, ceil(pages_b / P)) items of nearly equal size, with P the
+// smallest page count of at least kMinSplitPages for which they sum to at most `items`
+// (or P the longest sequence, one item each, where the batch has more sequences than
+// that). All items are resident at once, so the longest, P pages, sets the time.
+// Returns whether item `item` exists; `table` (one wave of the grid) also receives each
+// sequence's first item and count for the merge kernel.
+__device__ __forceinline__ bool find_split(const PartialArgs& a, int items, int item,
+                                           SeqSplits* table, Split& out) {
+  const int lane = threadIdx.x & 63;
+  const int groups = (a.batch + 63) / 64;
+  auto length_of = [&](int k) {
+    const int i = 64 * k + lane;
+    return i < a.batch ? max(a.seq_lens[i], 0) : 0;
+  };
+  const int len0 = length_of(0);
+  auto pages_at = [&](int k) {
+    const int len = k == 0 ? len0 : length_of(k);
+    return min((len + kPageSize - 1) / kPageSize, a.max_pages);
+  };
+  auto splits_of = [&](int k, int P) {
+    return 64 * k + lane < a.batch ? max((pages_at(k) + P - 1) / P, 1) : 0;
+  };
+  int total = 0;
+  for (int k = 0; k < groups; ++k) total += wave_sum_int(pages_at(k));
+  auto fits = [&](int P) {
+    int n = 0;
+    for (int k = 0; k < groups; ++k) n += wave_sum_int(splits_of(k, P));
+    return n <= items;
+  };
+  int lo = max(kMinSplitPages, (total + items - 1) / items);
+  if (!fits(lo)) {
+    // ceil(pages_b / P) sum to at most total / P + batch.
+    int hi = items > a.batch ? max(lo, (total + items - a.batch - 1) / (items - a.batch))
+                             : max(a.max_pages, 1);
+    while (lo + 1 < hi) {  // lo does not fit, hi does (or is one item each)
+      const int mid = lo + (hi - lo) / 2;
+      if (fits(mid))
+        hi = mid;
+      else
+        lo = mid;
+    }
+    lo = hi;
+  }
+  const int P = lo;
+  int base = 0;
+  bool found = false;
+  for (int k = 0; k < groups; ++k) {
+    const int n = splits_of(k, P);
+    const int incl = wave_inclusive_scan_int(n);
+    const int first = base + incl - n;
+    if (table != nullptr && 64 * k + lane < a.batch) table[64 * k + lane] = SeqSplits{first, n};
+    const unsigned long long hit = __ballot(item >= first && item < first + n);
+    if (hit && !found) {
+      const int src = __builtin_ctzll(hit);
+      const int pages = __builtin_amdgcn_readlane(pages_at(k), src);
+      out.b = 64 * k + src;
+      out.len = __builtin_amdgcn_readlane(k == 0 ? len0 : length_of(k), src);
+      out.count = __builtin_amdgcn_readlane(n, src);
+      out.slot = item;
+      out.first = __builtin_amdgcn_readlane(first, src);
+      const int size = (pages + out.count - 1) / out.count;
+      out.p_begin = (item - out.first) * size;
+      out.p_end = min(out.p_begin + size, pages);
+      found = true;
+      if (table == nullptr) return true;
+    }
+    base += __builtin_amdgcn_readlane(incl, 63);
+  }
+  return found;
+}
+
+// Four values in units of the scale -> four codes (bytes, low first). e4m3: no magnitude
+// exceeds 448 by more than a rounding of the quotient, which rounds to 448.
+template <bool INT8>
+__device__ __forceinline__ unsigned encode4(const float (&y)[4]) {
+  if constexpr (INT8) {
+    unsigned w = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float r = fminf(fmaxf(rintf(y[i] == y[i] ? y[i] : 0.f), -127.f), 127.f);
+      w |= ((unsigned)(int)r & 0xffu) << (8 * i);
+    }
+    return w;
+  } else {
+    int w = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
+    return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], w, true);
+  }
+}
+
+template <bool INT8>
+__device__ __forceinline__ float decode(unsigned w, int i) {
+  if constexpr (INT8) {
+    return (float)(signed char)(w >> (8 * i));
+  } else {
+    typedef float f2 __attribute__((ext_vector_type(2)));
+    const f2 lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false);
+    const f2 hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
+    return i < 2 ? lo[i] : hi[i - 2];
+  }
+}
+
+}  // namespace
+}  // namespace sqa

@@ -169,3 +169,67 @@ def _encode(y, dtype, most):
     # Products and quotients of 32-bit values: within three roundings.
     near = code(y * (1 + 2.0 ** -22)) != code(y * (1 - 2.0 ** -22))
     return code(y), near
+
+
+def weights_after(old, mass, lens, q_len):
+    """``(weights, bound)`` after a call whose probabilities are ``mass`` (:func:`attention`)."""
+    want = old.double().clone()
+    bound = torch.zeros_like(want)
+    width = old.shape[2]
+    for i, n in enumerate(max(int(x), 0) for x in lens):
+        p, far = (x.sum(1)[:, :width] for x in mass[i])
+        draft = max(n - q_len, 0)
+        want[i, :, draft:n] = 0.0
+        want[i, :, :n] += p
+        # The rows' sum and the addition to the old value, in 32 bits.
+        bound[i, :, :n] = far + 80 * 2.0 ** -24 * p + 2.0 ** -24 * want[i, :, :n].abs() + 1e-30
+    return want, bound
+
+
+def kept_tokens(weights, n, budget, sink, recent):
+    """Positions that stay of a sequence of ``n`` tokens with these weights (a list)."""
+    if n <= budget:
+        return list(range(n))
+    middle = range(sink, n - recent)
+    w = [float(x) for x in weights]
+    order = sorted(middle, key=lambda t: (math.isnan(w[t]), -w[t] if w[t] == w[t] else 0.0, t))
+    chosen = order[:budget - sink - recent]
+    return sorted(list(range(sink)) + chosen + list(range(n - recent, n)))
+
+
+def evict(weights, caches, scales, tables, lens, new_tables, budget, sink, recent, into,
+          into_scales):
+    """Eviction on CPU tensors: moves into ``into`` (and ``into_scales``) and returns
+    ``(new_lens, new_weights, kept)``."""
+    b, hkv, _ = weights.shape
+    page = caches[0].shape[1]
+    kept = torch.full((b, hkv, budget), -1, dtype=torch.int32)
+    new_w = torch.zeros(b, hkv, budget)
+    new_lens = torch.clamp(lens, min=0).clamp(max=budget)
+    for i in range(b):
+        n = max(int(lens[i]), 0)
+        for h in range(hkv):
+            stay = kept_tokens(weights[i, h], n, budget, sink, recent)
+            kept[i, h, :len(stay)] = torch.tensor(stay, dtype=torch.int32)
+            new_w[i, h, :len(stay)] = weights[i, h, stay]
+            for which in range(2):
+                cache, new = caches[which], into[which]
+                raw = cache.view(torch.uint8) if cache.element_size() == 1 else cache
+                raw_new = new.view(torch.uint8) if new.element_size() == 1 else new
+                for p in range(-(-len(stay) // page)):
+                    to = int(new_tables[i, p])
+                    part = stay[p * page:(p + 1) * page]
+                    from_pages = [int(tables[i, t // page]) for t in part]
+                    if scales is not None:
+                        now = max(scales[which][f, h] for f in from_pages)
+                        into_scales[which][to, h] = now
+                    for slot, (t, f) in enumerate(zip(part, from_pages)):
+                        x = raw[f, t % page, h]
+                        if scales is not None and scales[which][f, h] != now:
+                            # In 32 bits, operation by operation: part of the definition.
+                            y = cache[f, t % page, h].float() * scales[which][f, h] / now
+                            y = (y.round() if cache.dtype is torch.int8 else y)
+                            x = y.clamp(-CODE_MAX[cache.dtype], CODE_MAX[cache.dtype]) \
+                                .to(cache.dtype).view(torch.uint8)
+                        raw_new[to, slot, h] = x
+    return new_lens, new_w, kept

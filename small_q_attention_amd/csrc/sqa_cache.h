@@ -67,8 +67,8 @@ struct WeighArgs {
   float* weights;              // [B, Hkv, width]
   long long w_batch, w_head;   // strides in floats
   int width;
-  float2* stats;               // [Hkv][rows][items]: (max in log2 units, sum) of each item
-  float* scores;               // [B][Hkv][pages][rows][16] in log2 units, or NULL: the second
+  float2* stats;               // [items][Hkv][rows]: (max in log2 units, sum)
+  float* scores;               // [B][pages][Hkv][rows][16] in log2 units, or NULL: the second
                                // kernel computes them again
 };
 hipError_t launch_weigh(const WeighArgs& a, hipStream_t stream);

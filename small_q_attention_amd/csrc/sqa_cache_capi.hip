@@ -104,14 +104,18 @@ int weigh_plan(int device, int batch, int q_len, int num_query_heads, int num_kv
   plan->rows = (long long)q_len * (num_query_heads / num_kv_heads);
   plan->pages = max_pages;
   if (max_seq_len > 0) plan->pages = std::min(plan->pages, ceil_div(max_seq_len, sqa::kPageSize));
-  const long long most = batch * ceil_div(plan->pages, sqa::kMinSplitPages);
-  // Two workgroups per compute unit.
-  plan->items = std::max((long long)batch, std::min(2 * scaled_items(cus, num_kv_heads), most));
-  plan->stats = (size_t)plan->items * num_kv_heads * plan->rows * sizeof(float2);
   plan->scores = (size_t)batch * num_kv_heads * plan->pages * sqa::kPageSize * plan->rows * 4;
   if (!sqa::weights_stored(plan->rows, head_dim, is_codes(kv_dtype) ? 1 : 2) ||
       plan->scores > kMostScores)
     plan->scores = 0;
+  // Two workgroups per compute unit; four where the second kernel only adds the stored
+  // scores up, a wait for memory after the other (16 x 32K keys, four rows: its share of
+  // the call 27.4 us with two, 22.3 with four; but with K read again, 64 rows, 8
+  // sequences of up to 12K keys, 32 us with two and 60 with four).
+  const long long most = batch * ceil_div(plan->pages, sqa::kMinSplitPages);
+  plan->items = std::max((long long)batch, std::min((plan->scores ? 4 : 2) *
+                                                        scaled_items(cus, num_kv_heads), most));
+  plan->stats = (size_t)plan->items * num_kv_heads * plan->rows * sizeof(float2);
   return SQA_OK;
 }
 

@@ -94,6 +94,26 @@ __device__ __forceinline__ bool find_split(const PartialArgs& a, int items, int 
   return found;
 }
 
+// x / s for many x, rounded as the division is. With r = 1/s rounded to nearest, two
+// corrections q += r (x - q s), the remainders exact in an fma, leave the quotient
+// correctly rounded (Markstein's division) while nothing under- or overflows: s within
+// 2^+-100, as all but freak scales are, and x no larger than 448 s (a remainder of an x so
+// small that it underflows belongs to a quotient far below the smallest code). Five
+// operations in place of the division's dozen.
+struct Quotient {
+  float s, r;
+  bool fast;
+};
+__device__ __forceinline__ Quotient quotient(float s) {
+  return {s, 1.f / s, s >= 0x1p-100f && s <= 0x1p100f};
+}
+__device__ __forceinline__ float divide_fast(float x, const Quotient& d) {
+  // The remainder as -(q s - x): so written, -0 / s stays -0.
+  float q = x * d.r;
+  q = fmaf(-fmaf(q, d.s, -x), d.r, q);
+  return fmaf(-fmaf(q, d.s, -x), d.r, q);
+}
+
 // Four values in units of the scale -> four codes (bytes, low first). e4m3: no magnitude
 // exceeds 448 by more than a rounding of the quotient, which rounds to 448.
 template <bool INT8>

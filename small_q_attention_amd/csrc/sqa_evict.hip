@@ -75,29 +75,38 @@ __device__ __forceinline__ float row16_sum(float x) {
   return x;
 }
 
-// The log-sum-exp (log2 units) of a row from its sequence's items: lanes over items. A
-// row that saw nothing: +inf, which makes every weight 0.
-__device__ __forceinline__ float join_stats(const float2* st, int count) {
+// (max, sum) of two sets of a row's scores joined. A set that saw nothing has maximum
+// -inf; a NaN sum travels with a finite maximum and stays.
+__device__ __forceinline__ float2 join(float2 a, float2 b) {
+  const float m = fmaxf(a.x, b.x);
+  const float l = (a.x == -INFINITY ? 0.f : a.y * fast_exp2(a.x - m)) +
+                  (b.x == -INFINITY ? 0.f : b.y * fast_exp2(b.x - m));
+  return float2{m, l};
+}
+
+// The log-sum-exp (log2 units) of a sequence's rows from its items' [item][row] records
+// `stride` apart: row r in lane r (and, for fewer than 64 rows, in lanes further on). A
+// row that saw nothing: +inf, which makes every weight 0. Lanes lie over rows first, then
+// over items, so the records of an item come in one line and few exchanges follow (one
+// row after the other, lanes over items: 72 us of a call of 64 rows, 8 sequences of up to
+// 12K keys; so 14).
+__device__ __forceinline__ float rows_lse(const float2* st, int stride, int rows, int count) {
   const int lane = threadIdx.x & 63;
-  float m = -INFINITY, l = 0.f;
-  for (int i = lane; i < count; i += 64) {
-    const float2 x = st[i];
-    const float nm = fmaxf(m, x.x);
-    // A NaN sum must stay: its maximum travels as a finite number.
-    const float a = m == -INFINITY ? 0.f : fast_exp2(m - nm);
-    const float b = x.x == -INFINITY ? 0.f : fast_exp2(x.x - nm);
-    l = (m == -INFINITY ? 0.f : l * a) + (x.x == -INFINITY ? 0.f : x.y * b);
-    m = nm;
-  }
+  int span = 1;
+  while (span < rows) span *= 2;
+  const int r = min(lane & (span - 1), rows - 1), parts = 64 / span;
+  float2 x = {-INFINITY, 0.f};
+  for (int i = lane / span; i < count; i += 4 * parts) {
+    float2 y[4];
 #pragma unroll
-  for (int o = 1; o < 64; o *= 2) {
-    const float m2 = __shfl_xor(m, o), l2 = __shfl_xor(l, o);
-    const float nm = fmaxf(m, m2);
-    l = (m == -INFINITY ? 0.f : l * fast_exp2(m - nm)) +
-        (m2 == -INFINITY ? 0.f : l2 * fast_exp2(m2 - nm));
-    m = nm;
+    for (int u = 0; u < 4; ++u) y[u] = st[(size_t)min(i + u * parts, count - 1) * stride + r];
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (i + u * parts < count) x = join(x, y[u]);
   }
-  return l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
+  for (int o = span; o < 64; o *= 2)
+    x = join(x, float2{__shfl_xor(x.x, o), __shfl_xor(x.y, o)});
+  return x.y == 0.f ? INFINITY : x.x + __builtin_amdgcn_logf(x.y);
 }
 
 // What a wave works on: a work item of one kv head.
@@ -169,16 +178,12 @@ void sqa_weigh_kernel(WeighArgs args) {
   }
   float lse[NB];
   if constexpr (SUM) {
-    // Lane l takes the log-sum-exp of row 16 nb + l % 16.
+    const float x = rows_lse(args.stats + ((size_t)w.it.first * a.hkv + kvh) * a.rows,
+                             a.hkv * a.rows, a.rows, w.it.count);
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
-      lse[nb] = INFINITY;
-      for (int r = 0; r < 16 && 16 * nb + r < a.rows; ++r) {  // uniform
-        const float x = join_stats(
-            args.stats + (size_t)(kvh * a.rows + 16 * nb + r) * args.items + w.it.first,
-            w.it.count);
-        lse[nb] = l16 == r ? x : lse[nb];
-      }
+      const float mine = __shfl(x, 16 * nb + l16);
+      lse[nb] = map.real(nb, l16) ? mine : INFINITY;
     }
   }
 
@@ -201,7 +206,7 @@ void sqa_weigh_kernel(WeighArgs args) {
 #pragma unroll
     for (int i = 0; i < KEYS::kLoads; ++i)
       s.k.k[i] = __builtin_amdgcn_raw_buffer_load_b128(kr, k_lane + 64 * i, 0,
-                                                       SUM || STORE ? kStreamAux : 0);
+                                                       SUM ? kStreamAux : 0);
   };
   auto page_id = [&](int i) {
     return clamp_page(__builtin_amdgcn_readlane(ids, i & 63), a.num_pages);
@@ -218,8 +223,19 @@ void sqa_weigh_kernel(WeighArgs args) {
     l[nb] = 0.f;
   }
   float* wrow = args.weights + b * args.w_batch + kvh * args.w_head;
-  f4* out = (f4*)args.scores +
-            ((size_t)(b * a.hkv + kvh) * a.max_pages + p_begin) * a.rows * 4;
+  // Scores leave through a resource bounded to the item's, rows that are not there sent
+  // past its end: a store under a branch would leave the compiler guessing what is in
+  // flight, and its waits for the ring's pages would drain part of the ring (16 x 32K
+  // keys, one row block: 248 us under a branch, TODO so).
+  const unsigned head_scores = a.rows * kPageSize * 4u, page_scores = a.hkv * head_scores;  // bytes
+  const __amdgpu_buffer_rsrc_t out = __builtin_amdgcn_make_buffer_rsrc(
+      (void*)((char*)args.scores + ((size_t)b * a.max_pages + p_begin) * page_scores),
+      (short)0, STORE ? (int)(n_pages * page_scores) : 0, kBufferFlags);
+  unsigned out_lane[NB];
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb)
+    out_lane[nb] = map.real(nb, l16) ? kvh * head_scores + 64u * map.row(nb, l16) + 16u * g16
+                                     : kDroppedOffset;
 
   for (int i = 0; i < n_pages; i += D) {
     if (((i + D) & 63) == 0) {
@@ -242,7 +258,7 @@ void sqa_weigh_kernel(WeighArgs args) {
         }
       }
       if (ii < n_pages) {
-        const float c =
+        float c =
             a.scale_log2 * __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(
                                                          __builtin_bit_cast(int, ring[j].scale)));
         u4 k[KK];
@@ -253,33 +269,61 @@ void sqa_weigh_kernel(WeighArgs args) {
           s[nb] = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int kk = 0; kk < KK; ++kk) s[nb] = E::mma_qk(k[kk], q[nb][kk], s[nb]);
-          s[nb] *= c;
         }
-        if ((p + 1) * kPageSize > mask_from)  // uniform
+        const bool masked = (p + 1) * kPageSize > mask_from;  // uniform
+        if (masked) {
+          // After the scale, so that a scale of 0, infinity or NaN leaves them -inf.
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb) s[nb] *= c;
+          c = 1.f;
           mask_scores<NB>(s, bits.b, mask_from, p * kPageSize + 4 * g16, len);
+        }
         if constexpr (SUM) {
           f4 t = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              t[e] += s[nb][e] == -INFINITY ? 0.f : fast_exp2(s[nb][e] - lse[nb]);
+            for (int e = 0; e < 4; ++e) {
+              const float x = fast_exp2(fmaf(s[nb][e], c, -lse[nb]));
+              t[e] += masked && s[nb][e] == -INFINITY ? 0.f : x;
+            }
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const float x = row16_sum(t[e]);
             mine = l16 == 4 * (j & 3) + e ? x : mine;
           }
         } else {
+          if constexpr (STORE) {
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) {
+              s[nb] *= c;
+              __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4, s[nb]), out,
+                                                     out_lane[nb], ii * page_scores, 0);
+            }
+            c = 1.f;
+          }
+          // The running maximum of a lane's scores may trail them by kMaxLag, as in the
+          // attention kernels.
+          float lm[NB];
+          bool grow = false;
 #pragma unroll
           for (int nb = 0; nb < NB; ++nb) {
-            const float mn = fmaxf(m[nb], max4(s[nb]));
-            const float mu = mn == -INFINITY ? 0.f : mn;
-            l[nb] = l[nb] * fast_exp2(m[nb] - mu) +
-                    ((fast_exp2(s[nb][0] - mu) + fast_exp2(s[nb][1] - mu)) +
-                     (fast_exp2(s[nb][2] - mu) + fast_exp2(s[nb][3] - mu)));
-            m[nb] = mn;
-            if constexpr (STORE)
-              if (map.real(nb, l16)) out[((size_t)ii * a.rows + map.row(nb, l16)) * 4 + g16] = s[nb];
+            lm[nb] = max4(s[nb]) * c;
+            grow |= lm[nb] > m[nb] + kMaxLag;
+          }
+          if (__any(grow)) {
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) {
+              const float mn = fmaxf(m[nb], lm[nb]);
+              l[nb] *= fast_exp2(m[nb] - (mn == -INFINITY ? 0.f : mn));
+              m[nb] = mn;
+            }
+          }
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb) {
+            const float mu = m[nb] == -INFINITY ? 0.f : m[nb];
+            l[nb] += (fast_exp2(fmaf(s[nb][0], c, -mu)) + fast_exp2(fmaf(s[nb][1], c, -mu))) +
+                     (fast_exp2(fmaf(s[nb][2], c, -mu)) + fast_exp2(fmaf(s[nb][3], c, -mu)));
           }
         }
       }
@@ -301,14 +345,17 @@ void sqa_weigh_kernel(WeighArgs args) {
       const float sum = xor_sum(part);
       if (g16 == 0 && map.real(nb, l16))
         // A NaN sum travels with a finite maximum, so that the join counts it.
-        args.stats[(size_t)(kvh * a.rows + map.row(nb, l16)) * args.items + w.it.slot] =
+        args.stats[((size_t)w.it.slot * a.hkv + kvh) * a.rows + map.row(nb, l16)] =
             float2{sum == sum ? top : 0.f, sum};
     }
   }
 }
 
-// The second pass from the stored scores: a lane per token, 64 tokens at a time.
-template <int U>
+// The second pass from the stored scores: a lane takes four consecutive tokens, a wave
+// 256 at a time. The scores of four rows are requested before any is used: one row after
+// the other, each round of a few hundred tokens waited for memory once per row (16 x 32K
+// keys, four rows: 25 us, TODO so).
+typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
 __global__ __launch_bounds__(256) void sqa_weigh_join_kernel(WeighArgs args) {
   const PartialArgs& a = args.p;
   WaveItem w;
@@ -317,40 +364,48 @@ __global__ __launch_bounds__(256) void sqa_weigh_join_kernel(WeighArgs args) {
   const int rows = a.rows, kvh = w.kvh;
   const int mask_from = w.it.len - a.q_len;
   const int t_end = min(min(w.it.p_end * kPageSize, w.it.len), args.width);
-  const float2* stats = args.stats + (size_t)kvh * rows * args.items + w.it.first;
-  const float* scores =
-      args.scores + (size_t)(w.it.b * a.hkv + kvh) * a.max_pages * rows * kPageSize;
+  const size_t page_scores = (size_t)a.hkv * rows * kPageSize;
+  const float* scores = args.scores + (size_t)w.it.b * a.max_pages * page_scores +
+                        (size_t)kvh * rows * kPageSize;
   float* wrow = args.weights + w.it.b * args.w_batch + kvh * args.w_head;
   // Lane r holds row r's log-sum-exp.
-  float lse = INFINITY;
-  for (int r = 0; r < rows; ++r) {
-    const float x = join_stats(stats + (size_t)r * args.items, w.it.count);
-    lse = lane == r ? x : lse;
-  }
-  for (int t0 = w.it.p_begin * kPageSize; t0 < t_end; t0 += 64 * U) {
-    float sum[U], old[U];
+  const float lse = rows_lse(args.stats + ((size_t)w.it.first * a.hkv + kvh) * rows, a.hkv * rows,
+                             rows, w.it.count);
+  for (int t0 = w.it.p_begin * kPageSize; t0 < t_end; t0 += 256) {
+    const int t = t0 + 4 * lane;
+    const bool whole = t + 4 <= t_end;
+    f4 old = f4{0.f, 0.f, 0.f, 0.f}, sum = old;
+    if (whole) {
+      old = *(const f4u*)(wrow + t);
+    } else {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int t = t0 + 64 * u + lane;
-      sum[u] = 0.f;
-      old[u] = t < min(mask_from, t_end) ? wrow[t] : 0.f;
+      for (int e = 0; e < 4; ++e)
+        if (t + e < t_end) old[e] = wrow[t + e];
     }
-    for (int r = 0; r < rows; ++r) {
-      const float lr = __builtin_bit_cast(
-          float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, lse), r));
-      float x[U];
+    // Past the item's end: its last page again, unused.
+    const float* at = scores + (size_t)(min(t, t_end - 1) >> 4) * page_scores + (t & 12);
+    for (int r0 = 0; r0 < rows; r0 += 4) {
+      f4 x[4];
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int t = min(t0 + 64 * u + lane, t_end - 1);
-        x[u] = scores[((size_t)(t >> 4) * rows + r) * kPageSize + (t & 15)];
+      for (int i = 0; i < 4; ++i) x[i] = *(const f4*)(at + min(r0 + i, rows - 1) * kPageSize);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (r0 + i >= rows) break;  // uniform
+        const float lr = __builtin_bit_cast(
+            float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, lse), r0 + i));
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          sum[e] += x[i][e] == -INFINITY ? 0.f : fast_exp2(x[i][e] - lr);
       }
-#pragma unroll
-      for (int u = 0; u < U; ++u) sum[u] += x[u] == -INFINITY ? 0.f : fast_exp2(x[u] - lr);
     }
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int t = t0 + 64 * u + lane;
-      if (t < t_end) wrow[t] = t < mask_from ? old[u] + sum[u] : sum[u];
+    for (int e = 0; e < 4; ++e) sum[e] += t + e < mask_from ? old[e] : 0.f;
+    if (whole) {
+      *(f4u*)(wrow + t) = sum;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (t + e < t_end) wrow[t + e] = sum[e];
     }
   }
 }
@@ -373,6 +428,9 @@ constexpr int kSelectThreads = 1024, kSelectWaves = kSelectThreads / 64;
 // 10 bits, histograms in LDS); tokens above it stay, and of those that equal it the first.
 // Each wave then counts its own run of tokens, and after one exchange writes its kept
 // tokens in order. All counts are integers: the same weights give the same tokens.
+// R > 0: a thread holds the weights of its R tokens in registers through all of it (up to
+// 1024 R tokens); R = 0 reads them again each time.
+template <int R>
 __global__ __launch_bounds__(kSelectThreads) void sqa_select_kernel(EvictArgs a) {
   __shared__ int hist[2048];
   __shared__ int wave_tot[kSelectWaves], wave_sure[kSelectWaves], wave_tie[kSelectWaves];
@@ -392,23 +450,49 @@ __global__ __launch_bounds__(kSelectThreads) void sqa_select_kernel(EvictArgs a)
     for (int j = tid; j < a.new_width; j += kSelectThreads) nw[j] = j < n ? w[j] : 0.f;
     return;
   }
+  // A wave's run: `steps` times 64 consecutive tokens.
+  const int steps = (n + kSelectThreads - 1) / kSelectThreads;
+  const int begin = min(wave * steps * 64, n);
+  constexpr int kHeld = R > 0 ? R : 1;
+  float held[kHeld];
+  if constexpr (R > 0) {
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const int t = begin + 64 * i + lane;
+      held[i] = i < steps ? w[min(t, n - 1)] : 0.f;
+    }
+  }
+  // each(f): f(token, weight) for the thread's tokens of the run in order.
+  auto each = [&](auto f) {
+    if constexpr (R > 0) {
+#pragma unroll
+      for (int i = 0; i < R; ++i)
+        if (i < steps) f(begin + 64 * i + lane, held[i]);  // uniform
+    } else {
+      for (int i = 0; i < steps; ++i) {
+        const int t = begin + 64 * i + lane;
+        f(t, w[min(t, n - 1)]);
+      }
+    }
+  };
+  const int end = min(begin + steps * 64, n);
   const int lo = a.sink, hi = n - a.recent;
   const int free = a.budget - a.sink - a.recent;
-  unsigned threshold = 0xffffffffu;  // no key: keys of finite weights and infinities lie below
+  unsigned threshold = 0xffffffffu;  // no key: those of all weights lie below
   int ties = 0;                      // how many of the tokens at the threshold stay
   if (free > 0) {
     int want = free;
     unsigned prefix = 0, mask = 0;
-#pragma unroll
     for (int pass = 0; pass < 3; ++pass) {
       const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0);
       const unsigned digits = pass == 2 ? 0x3ffu : 0x7ffu;
       for (int i = tid; i < 2048; i += kSelectThreads) hist[i] = 0;
       __syncthreads();
-      for (int t = lo + tid; t < hi; t += kSelectThreads) {
-        const unsigned k = weight_key(w[t]);
-        if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & digits], 1);
-      }
+      each([&](int t, float x) {
+        const unsigned k = weight_key(x);
+        if (t >= lo && t < min(hi, end) && (k & mask) == prefix)
+          atomicAdd(&hist[(k >> shift) & digits], 1);
+      });
       __syncthreads();
       // Bins from the top: thread i takes bins 2047 - 2 i and 2046 - 2 i.
       const int c0 = hist[2047 - 2 * tid], c1 = hist[2046 - 2 * tid];
@@ -430,23 +514,20 @@ __global__ __launch_bounds__(kSelectThreads) void sqa_select_kernel(EvictArgs a)
     threshold = prefix;
     ties = want;
   }
-  // Runs of whole waves' widths, one per wave.
-  const int run = ((n + kSelectThreads - 1) / kSelectThreads) * 64;
-  const int begin = min(wave * run, n), end = min(begin + run, n);
-  auto look = [&](int t, bool& sure, bool& tie) {
+  auto look = [&](int t, float x, bool& sure, bool& tie) {
     const bool in = t < end;
     const bool always = in && (t < lo || t >= hi);
-    const unsigned k = in && !always ? weight_key(w[t]) : 0u;
-    sure = always || (in && free > 0 && k > threshold);
-    tie = in && !always && free > 0 && k == threshold;
+    const unsigned k = weight_key(x);
+    sure = always || (in && k > threshold);
+    tie = in && !always && ties > 0 && k == threshold;
   };
   int sures = 0, tied = 0;
-  for (int t = begin; t < end; t += 64) {
+  each([&](int t, float x) {
     bool sure, tie;
-    look(t + lane, sure, tie);
+    look(t, x, sure, tie);
     sures += __popcll(__ballot(sure));
     tied += __popcll(__ballot(tie));
-  }
+  });
   if (lane == 0) {
     wave_sure[wave] = sures;
     wave_tie[wave] = tied;
@@ -459,104 +540,117 @@ __global__ __launch_bounds__(kSelectThreads) void sqa_select_kernel(EvictArgs a)
   }
   at += min(seen, ties);
   const unsigned long long below = lane ? ~0ull >> (64 - lane) : 0ull;
-  for (int t = begin; t < end; t += 64) {
+  each([&](int t, float x) {
     bool sure, tie;
-    look(t + lane, sure, tie);
+    look(t, x, sure, tie);
     const unsigned long long tie_mask = __ballot(tie);
     const bool keep = sure || (tie && seen + __popcll(tie_mask & below) < ties);
     const unsigned long long keep_mask = __ballot(keep);
-    if (keep) kept[at + __popcll(keep_mask & below)] = t + lane;
+    if (keep) {
+      const int to = at + __popcll(keep_mask & below);
+      kept[to] = t;
+      if constexpr (R > 0) nw[to] = x;  // every weight has been read: nw may be w
+    }
     at += __popcll(keep_mask);
     seen += __popcll(tie_mask);
-  }
-  __syncthreads();
-  // The weights move along, 1024 at a time: new_weights may be the old ones, and a token
-  // never moves to a later position.
-  for (int j0 = 0; j0 < a.new_width; j0 += kSelectThreads) {
-    const int j = j0 + tid;
-    const float x = j < m ? w[kept[j]] : 0.f;
+  });
+  if constexpr (R > 0) {
+    for (int j = m + tid; j < a.new_width; j += kSelectThreads) nw[j] = 0.f;
+  } else {
     __syncthreads();
-    if (j < a.new_width) nw[j] = x;
-    __syncthreads();
+    // The weights move along, 1024 at a time: new_weights may be the old ones, and a token
+    // never moves to a later position.
+    for (int j0 = 0; j0 < a.new_width; j0 += kSelectThreads) {
+      const int j = j0 + tid;
+      const float x = j < m ? w[kept[j]] : 0.f;
+      __syncthreads();
+      if (j < a.new_width) nw[j] = x;
+      __syncthreads();
+    }
   }
 }
 
-// The kept tokens of 16 new slots of one kv head, K or V, moved to their new page. 16
-// bytes a lane. Scaled caches: the new block's scale is the largest of the scales its
-// tokens come from, and codes from blocks of other scales are rounded again.
+// The kept tokens of 64 new slots of one kv head, K or V, moved to their new pages: a lane
+// looks one token's places up, then the wave moves the rows, 16 bytes a lane, all loads
+// before the first store. Scaled caches: the new block's scale is the largest of the
+// scales its tokens come from, and codes from blocks of other scales are rounded again.
 template <int ROW, bool SCALED, bool INT8>
 __global__ __launch_bounds__(256) void sqa_move_kernel(EvictArgs a) {
   constexpr int LPT = ROW / 16;   // lanes per token (ROW: bytes of a token and head)
   constexpr int TPI = 64 / LPT;   // tokens per instruction
-  constexpr int NI = 16 / TPI;
+  constexpr int NI = 64 / TPI;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;
   const int head_groups = (a.hkv + 3) / 4;
   const int h = (blockIdx.x % head_groups) * 4 + wave;
-  const int tiles = (a.budget + 15) / 16;
+  const int tiles = (a.budget + 63) / 64;
   const int rest = blockIdx.x / head_groups;
-  const int b = rest / tiles, j0 = rest % tiles * 16;
+  const int b = rest / tiles, j0 = rest % tiles * 64;
   const int which = blockIdx.y;
   const int m = a.new_lens[b];
   if (h >= a.hkv || j0 >= m) return;
   const int page = a.page_size;
-  const int np = j0 / page;
-  if (np >= a.new_stride) return;
-  const int to = a.new_tables[(size_t)b * a.new_stride + np];
-  if (to < 0 || to >= a.new_pages) return;  // uniform: a page that is not there
   const int32_t* kept = a.kept + (size_t)(b * a.hkv + h) * a.budget;
   const int32_t* table = a.block_tables + (size_t)b * a.bt_stride;
-  // Lane l: where new token j0 + l % 16 comes from.
-  const int jt = min(j0 + (lane & 15), m - 1);
-  const int from = max(kept[jt], 0);
+  // Lane l: new token j0 + l (past the last one: it again), where from and where to.
+  const int j = min(j0 + lane, m - 1);
+  const int from = max(kept[j], 0);
+  const int np = j / page;
+  const int to = np < a.new_stride ? a.new_tables[(size_t)b * a.new_stride + np] : -1;
+  // A page that is not there is not written.
+  const bool there = j0 + lane < m && to >= 0 && to < a.new_pages;
   const int fp = clamp_page(table[from / page], a.num_pages);
-  const long long off = (long long)fp * a.src_page + (long long)(from % page) * a.src_token;
+  const long long src_at = (long long)fp * a.src_page + (long long)(from % page) * a.src_token;
+  const long long dst_at =
+      there ? (long long)to * a.dst_page + (long long)(j % page) * a.dst_token : -1;
   float old = 1.f, scale = 1.f;
   if constexpr (SCALED) {
     const char* sc = (const char*)(which ? a.src_scales.v : a.src_scales.k) +
                      (size_t)h * a.src_scales.head_stride;
     old = *(const float*)(sc + fp * a.src_scales.page_stride);
-    scale = 0.f;
-    const int first = np * page;
-    for (int j = first + lane; j < min(first + page, m); j += 64) {
-      const int p = clamp_page(table[max(kept[j], 0) / page], a.num_pages);
-      scale = fmaxf(scale, *(const float*)(sc + p * a.src_scales.page_stride));
+    scale = old;
+    if (page > 64) {  // the page's other tokens
+      for (int i = np * page + lane; i < min(np * page + page, m); i += 64) {
+        const int p = clamp_page(table[max(kept[i], 0) / page], a.num_pages);
+        scale = fmaxf(scale, *(const float*)(sc + p * a.src_scales.page_stride));
+      }
     }
-#pragma unroll
-    for (int o = 1; o < 64; o *= 2) scale = fmaxf(scale, __shfl_xor(scale, o));
-    if (j0 == first && lane == 0)
+    for (int o = 1; o < min(page, 64); o *= 2) scale = fmaxf(scale, __shfl_xor(scale, o));
+    if (there && j % page == 0)
       *(float*)((char*)(which ? a.dst_scales.v : a.dst_scales.k) +
                 (size_t)h * a.dst_scales.head_stride + to * a.dst_scales.page_stride) = scale;
   }
   const char* src = a.src[which] + (size_t)h * a.src_head + 16 * (lane % LPT);
-  char* dst = a.dst[which] + (size_t)h * a.dst_head + (size_t)to * a.dst_page +
-              (size_t)(j0 % page) * a.dst_token + 16 * (lane % LPT);
+  char* dst = a.dst[which] + (size_t)h * a.dst_head + 16 * (lane % LPT);
+  auto of_token = [&](long long x, int t) {
+    return (long long)__shfl((int)(x >> 32), t) << 32 | (unsigned)__shfl((int)x, t);
+  };
   u4 x[NI];
-  float so[NI];
 #pragma unroll
-  for (int i = 0; i < NI; ++i) {
-    const int t = i * TPI + lane / LPT;
-    const long long o = (long long)__shfl((int)(off >> 32), t) << 32 |
-                        (unsigned)__shfl((int)off, t);
-    x[i] = *(const u4*)(src + o);
-    so[i] = SCALED ? __shfl(old, t) : 1.f;
-  }
+  for (int i = 0; i < NI; ++i) x[i] = *(const u4*)(src + of_token(src_at, i * TPI + lane / LPT));
+  const Quotient by = quotient(scale);
+  const bool fast = __all(by.fast);
 #pragma unroll
   for (int i = 0; i < NI; ++i) {
     const int t = i * TPI + lane / LPT;
     if constexpr (SCALED) {
-      if (so[i] != scale) {
+      const float so = __shfl(old, t);
+      const Quotient q = {__shfl(scale, t), __shfl(by.r, t), true};
+      if (so != q.s) {
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
           float y[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            y[e] = scale > 0.f ? decode<INT8>(x[i][w], e) * so[i] / scale : 0.f;
+          for (int e = 0; e < 4; ++e) {
+            const float v = decode<INT8>(x[i][w], e) * so;
+            y[e] = fast ? divide_fast(v, q) : (q.s > 0.f ? v / q.s : 0.f);
+          }
           x[i][w] = encode4<INT8>(y);
         }
       }
     }
-    if (j0 + t < m) *(u4*)(dst + (size_t)t * a.dst_token) = x[i];
+    const long long o = of_token(dst_at, t);
+    if (o >= 0) *(u4*)(dst + o) = x[i];
   }
 }
 
@@ -568,7 +662,7 @@ void launch_weigh_rows(const WeighArgs& a, dim3 grid, hipStream_t stream) {
     if (a.scores) {
       hipLaunchKernelGGL((sqa_weigh_kernel<NB, D, HD, E, KEYS<HD>, false, true>), grid, block, 0,
                          stream, a);
-      hipLaunchKernelGGL((sqa_weigh_join_kernel<4>), grid, block, 0, stream, a);
+      hipLaunchKernelGGL(sqa_weigh_join_kernel, grid, block, 0, stream, a);
       return;
     }
   }
@@ -642,11 +736,19 @@ hipError_t launch_weigh(const WeighArgs& a, hipStream_t stream) {
 }
 
 hipError_t launch_evict(const EvictArgs& a, hipStream_t stream) {
-  hipLaunchKernelGGL(sqa_select_kernel, dim3((unsigned)(a.batch * a.hkv)), dim3(kSelectThreads), 0,
-                     stream, a);
+  const dim3 each((unsigned)(a.batch * a.hkv)), threads(kSelectThreads);
+  const long long most = std::min((long long)a.width, (long long)a.bt_stride * a.page_size);
+  if (most <= 4 * kSelectThreads)
+    hipLaunchKernelGGL((sqa_select_kernel<4>), each, threads, 0, stream, a);
+  else if (most <= 16 * kSelectThreads)
+    hipLaunchKernelGGL((sqa_select_kernel<16>), each, threads, 0, stream, a);
+  else if (most <= 40 * kSelectThreads)
+    hipLaunchKernelGGL((sqa_select_kernel<40>), each, threads, 0, stream, a);
+  else
+    hipLaunchKernelGGL((sqa_select_kernel<0>), each, threads, 0, stream, a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  const int tiles = (a.budget + 15) / 16;
+  const int tiles = (a.budget + 63) / 64;
   const dim3 grid((unsigned)((long long)a.batch * tiles * ((a.hkv + 3) / 4)), 2);
   const int row = a.head_dim * (a.kv_type >= kE4M3 ? 1 : 2);
   if (row == 64)

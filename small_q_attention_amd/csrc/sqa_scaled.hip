@@ -359,7 +359,6 @@ __global__ __launch_bounds__(256) void sqa_append_kernel(AppendArgs a) {
                              (size_t)pid * a.scales.page_stride + (size_t)h * a.scales.head_stride);
   u4 x[TPW][NI];
   const float old = active ? *scale_at : 0.f;
-  float top = 0.f;
 #pragma unroll
   for (int t = 0; t < TPW; ++t) {
 #pragma unroll
@@ -371,16 +370,35 @@ __global__ __launch_bounds__(256) void sqa_append_kernel(AppendArgs a) {
                                2 * dim);
     }
   }
+  // The largest magnitude as the largest bit pattern; at the infinity's and past it
+  // (rare) the values are looked at again.
+  typedef unsigned short us2 __attribute__((ext_vector_type(2)));
+  constexpr unsigned kInfinity = BF16 ? 0x7f80u : 0x7c00u;
+  us2 most = {0, 0};
 #pragma unroll
   for (int t = 0; t < TPW; ++t)
 #pragma unroll
     for (int i = 0; i < NI; ++i)
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        // fmaxf passes over NaN.
-        top = fmaxf(top, fabsf(finite<BF16>(from_half<BF16>(x[t][i][w] & 0xffffu))));
-        top = fmaxf(top, fabsf(finite<BF16>(from_half<BF16>(x[t][i][w] >> 16))));
-      }
+      for (int w = 0; w < 4; ++w)
+        most = __builtin_elementwise_max(most,
+                                         __builtin_bit_cast(us2, x[t][i][w] & 0x7fff7fffu));
+  const unsigned bits = max((unsigned)most[0], (unsigned)most[1]);
+  float top = from_half<BF16>(bits);
+  const bool wild = __any(bits >= kInfinity);  // uniform
+  if (wild) {
+    top = 0.f;
+#pragma unroll
+    for (int t = 0; t < TPW; ++t)
+#pragma unroll
+      for (int i = 0; i < NI; ++i)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          // fmaxf passes over NaN.
+          top = fmaxf(top, fabsf(finite<BF16>(from_half<BF16>(x[t][i][w] & 0xffffu))));
+          top = fmaxf(top, fabsf(finite<BF16>(from_half<BF16>(x[t][i][w] >> 16))));
+        }
+  }
 #pragma unroll
   for (int o = 1; o < 64; o *= 2) top = fmaxf(top, __shfl_xor(top, o));
   if (wpb > 1) {  // uniform
@@ -393,30 +411,37 @@ __global__ __launch_bounds__(256) void sqa_append_kernel(AppendArgs a) {
   if (lo > 0) scale = fmaxf(scale, old);
   if (wave % wpb == 0 && lane == 0) *scale_at = scale;
   const bool again = lo > 0 && scale != old;  // uniform over the block
+  const Quotient by = quotient(scale);
+  const bool plain = __all(by.fast) && !wild;  // uniform
+  auto store = [&](auto divide, auto value) {
 #pragma unroll
-  for (int t = 0; t < TPW; ++t) {
+    for (int t = 0; t < TPW; ++t) {
 #pragma unroll
-    for (int i = 0; i < NI; ++i) {
-      const int slot = 16 * ((wave % wpb) * TPW + t) + i * TPI + token;
-      u2* to = (u2*)(codes + (size_t)slot * a.token_stride + dim);
-      float y[2][4];
-      if (slot >= lo && slot < hi) {
+      for (int i = 0; i < NI; ++i) {
+        const int slot = 16 * ((wave % wpb) * TPW + t) + i * TPI + token;
+        u2* to = (u2*)(codes + (size_t)slot * a.token_stride + dim);
+        float y[2][4];
+        if (slot >= lo && slot < hi) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const unsigned w = x[t][i][e / 2];
-          const float v = finite<BF16>(from_half<BF16>(e & 1 ? w >> 16 : w & 0xffffu));
-          y[e / 4][e % 4] = scale > 0.f ? v / scale : 0.f;
+          for (int e = 0; e < 8; ++e) {
+            const unsigned w = x[t][i][e / 2];
+            y[e / 4][e % 4] = divide(value(from_half<BF16>(e & 1 ? w >> 16 : w & 0xffffu)));
+          }
+          *to = u2{encode4<INT8>(y[0]), encode4<INT8>(y[1])};
+        } else if (again && slot < lo) {
+          const u2 w = *to;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) y[e / 4][e % 4] = divide(decode<INT8>(w[e / 4], e % 4) * old);
+          *to = u2{encode4<INT8>(y[0]), encode4<INT8>(y[1])};
         }
-        *to = u2{encode4<INT8>(y[0]), encode4<INT8>(y[1])};
-      } else if (again && slot < lo) {
-        const u2 w = *to;
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          y[e / 4][e % 4] = decode<INT8>(w[e / 4], e % 4) * old / scale;
-        *to = u2{encode4<INT8>(y[0]), encode4<INT8>(y[1])};
       }
     }
-  }
+  };
+  if (plain)
+    store([&](float v) { return divide_fast(v, by); }, [](float v) { return v; });
+  else
+    store([&](float v) { return scale > 0.f ? v / scale : 0.f; },
+          [](float v) { return finite<BF16>(v); });
 }
 
 template <int HD, bool BF16, bool INT8>

@@ -292,10 +292,11 @@ def launch_general(query, output, k_view, v_view, block_tables, seq_lens, draft_
 
 def dtype_code(dtype) -> int:
     """``SQA_DTYPE_*`` of a torch type."""
-    import torch
+    return _DTYPE_CODES[str(dtype)]
 
-    return {torch.float16: DTYPE_F16, torch.bfloat16: DTYPE_BF16,
-            torch.float8_e4m3fn: DTYPE_FP8_E4M3, torch.int8: DTYPE_INT8}[dtype]
+
+_DTYPE_CODES = {"torch.float16": DTYPE_F16, "torch.bfloat16": DTYPE_BF16,
+                "torch.float8_e4m3fn": DTYPE_FP8_E4M3, "torch.int8": DTYPE_INT8}
 
 
 @functools.lru_cache(maxsize=4096)
@@ -311,49 +312,61 @@ def plan_scaled(device_index: int, batch: int, num_kv_heads: int, max_seq_len: i
     return ns.value
 
 
+def scaled_fields(query, k_view, k_scale, block_tables, draft_mask):
+    """What of the arguments of ``sqa_paged_attention_scaled`` follows from the tensors'
+    layouts."""
+    b, q_len, hq, d = query.shape
+    num_pages, page, hkv, _ = k_view.shape
+    return ((num_pages, *k_view.stride()[:3]), block_tables.shape[1],
+            0 if draft_mask is None else draft_mask.shape[-1], (b, q_len, hq, hkv, d, page),
+            (dtype_code(query.dtype), dtype_code(k_view.dtype), 0), k_scale.stride())
+
+
 def launch_scaled(query, output, k_view, v_view, k_scale, v_scale, block_tables, seq_lens,
                   draft_mask, scale: float, out_scale: float, num_splits: int, workspace,
-                  stream_handle: int, timing_events=None):
+                  stream_handle: int, timing_events=None, fields=None):
     """Call ``sqa_paged_attention_scaled``: as :func:`launch_general`, over e4m3 or int8
-    views with ``[num_pages, Hkv]`` float32 scales of equal strides."""
+    views with ``[num_pages, Hkv]`` float32 scales of equal strides (``fields`` from
+    :func:`scaled_fields`)."""
     lib = _LIB if _LIB is not None else load()
-    b, q_len, hq, d = query.shape
-    strides, sstrides = k_view.stride(), k_scale.stride()
-    num_pages, page, hkv, _ = k_view.shape
-    words, mask_words = (0, 0) if draft_mask is None else (draft_mask.data_ptr(),
-                                                           draft_mask.shape[-1])
+    pool, max_pages, words, shape, types, scales = fields or scaled_fields(
+        query, k_view, k_scale, block_tables, draft_mask)
     ev = None
     if timing_events is not None:
         ev = (ctypes.c_void_p * 3)(*[ctypes.c_void_p(int(e)) for e in timing_events])
     a = _ARGS.pack(
         _ARGS.size, query.data_ptr(), output.data_ptr(), k_view.data_ptr(), v_view.data_ptr(),
-        num_pages, strides[0], strides[1], strides[2], block_tables.data_ptr(),
-        seq_lens.data_ptr(), block_tables.shape[1], words, mask_words, scale, out_scale, b, q_len,
-        hq, hkv, d, page, num_splits, 0, workspace.data_ptr(),
-        workspace.numel() * workspace.element_size(), stream_handle or 0,
-        0 if ev is None else ctypes.addressof(ev), dtype_code(query.dtype),
-        dtype_code(k_view.dtype), 0)
-    s = _SCALES.pack(k_scale.data_ptr(), v_scale.data_ptr(), sstrides[0], sstrides[1])
-    rc = lib.sqa_paged_attention_scaled(a, s)
+        *pool, block_tables.data_ptr(), seq_lens.data_ptr(), max_pages,
+        0 if draft_mask is None else draft_mask.data_ptr(), words, scale, out_scale, *shape,
+        num_splits, 0, workspace.data_ptr(), workspace.numel() * workspace.element_size(),
+        stream_handle or 0, 0 if ev is None else ctypes.addressof(ev), *types)
+    rc = lib.sqa_paged_attention_scaled(
+        a, _SCALES.pack(k_scale.data_ptr(), v_scale.data_ptr(), *scales))
     if rc != SQA_OK:
         raise RuntimeError(f"sqa_paged_attention_scaled failed: {last_error(lib)}")
 
 
-def launch_append(key, value, k_view, v_view, k_scale, v_scale, block_tables, seq_lens, new_lens,
-                  stream_handle: int):
-    """Call ``sqa_append_scaled`` (``key``/``value`` ``[B, Q, Hkv, D]``, their last dimension
-    contiguous; views and scales as for :func:`launch_scaled`)."""
-    lib = _LIB if _LIB is not None else load()
+def append_fields(key, value, k_view, k_scale, block_tables):
+    """What of an ``sqa_append_args`` follows from the tensors' layouts (in its order, the
+    pointers between)."""
     b, q_len, hkv, d = key.shape
-    strides, sstrides = k_view.stride(), k_scale.stride()
-    a = _APPEND.pack(
-        _APPEND.size, key.data_ptr(), value.data_ptr(), *key.stride()[:3], *value.stride()[:3],
-        k_view.data_ptr(), v_view.data_ptr(), k_view.shape[0], strides[0], strides[1], strides[2],
-        k_scale.data_ptr(), v_scale.data_ptr(), sstrides[0], sstrides[1], block_tables.data_ptr(),
-        seq_lens.data_ptr(), 0 if new_lens is None else new_lens.data_ptr(),
-        block_tables.shape[1], b, q_len, hkv, d, k_view.shape[1], dtype_code(key.dtype),
-        dtype_code(k_view.dtype), stream_handle or 0)
-    rc = lib.sqa_append_scaled(a)
+    return ((*key.stride()[:3], *value.stride()[:3]), (k_view.shape[0], *k_view.stride()[:3]),
+            k_scale.stride(), (block_tables.shape[1], b, q_len, hkv, d, k_view.shape[1],
+                               dtype_code(key.dtype), dtype_code(k_view.dtype)))
+
+
+def launch_append(key, value, k_view, v_view, k_scale, v_scale, block_tables, seq_lens, new_lens,
+                  stream_handle: int, fields=None):
+    """Call ``sqa_append_scaled`` (``key``/``value`` ``[B, Q, Hkv, D]``, their last dimension
+    contiguous; views and scales as for :func:`launch_scaled`; ``fields`` from
+    :func:`append_fields`)."""
+    lib = _LIB if _LIB is not None else load()
+    tokens, pool, scales, rest = fields or append_fields(key, value, k_view, k_scale, block_tables)
+    rc = lib.sqa_append_scaled(_APPEND.pack(
+        _APPEND.size, key.data_ptr(), value.data_ptr(), *tokens, k_view.data_ptr(),
+        v_view.data_ptr(), *pool, k_scale.data_ptr(), v_scale.data_ptr(), *scales,
+        block_tables.data_ptr(), seq_lens.data_ptr(),
+        0 if new_lens is None else new_lens.data_ptr(), *rest, stream_handle or 0))
     if rc != SQA_OK:
         raise RuntimeError(f"sqa_append_scaled failed: {last_error(lib)}")
 
@@ -372,49 +385,63 @@ def weights_workspace_bytes(device_index: int, batch: int, q_len: int, num_query
     return need
 
 
-def launch_weights(query, k_view, k_scale, block_tables, seq_lens, draft_mask, weights,
-                   scale: float, max_seq_len: int, workspace, stream_handle: int):
-    """Call ``sqa_attention_weights`` (``k_scale`` ``None``: none; ``weights`` ``[B, Hkv, T]``
-    float32 with a contiguous last dimension)."""
-    lib = _LIB if _LIB is not None else load()
+def weights_fields(query, k_view, k_scale, block_tables, draft_mask, weights, max_seq_len: int):
+    """What of an ``sqa_weights_args`` follows from the tensors' layouts."""
     b, q_len, hq, d = query.shape
-    ks, ws = k_view.stride(), weights.stride()
-    sc = (0, 0, 0) if k_scale is None else (k_scale.data_ptr(), *k_scale.stride())
-    words, mask_words = (0, 0) if draft_mask is None else (draft_mask.data_ptr(),
-                                                           draft_mask.shape[-1])
-    a = _WEIGHTS.pack(
-        _WEIGHTS.size, query.data_ptr(), k_view.data_ptr(), 0, k_view.shape[0], ks[0], ks[1], ks[2],
-        *sc, block_tables.data_ptr(), seq_lens.data_ptr(), words, weights.data_ptr(), ws[0], ws[1],
-        weights.shape[2], block_tables.shape[1], mask_words, scale, b, q_len, hq, k_view.shape[2],
-        d, k_view.shape[1], max_seq_len, dtype_code(query.dtype), dtype_code(k_view.dtype),
-        workspace.data_ptr(), workspace.numel() * workspace.element_size(), stream_handle or 0)
-    rc = lib.sqa_attention_weights(a)
+    return ((k_view.shape[0], *k_view.stride()[:3]), (0, 0) if k_scale is None
+            else k_scale.stride(),
+            (*weights.stride()[:2], weights.shape[2], block_tables.shape[1],
+             0 if draft_mask is None else draft_mask.shape[-1]),
+            (b, q_len, hq, k_view.shape[2], d, k_view.shape[1], max_seq_len,
+             dtype_code(query.dtype), dtype_code(k_view.dtype)))
+
+
+def launch_weights(query, k_view, k_scale, block_tables, seq_lens, draft_mask, weights,
+                   scale: float, max_seq_len: int, workspace, stream_handle: int, fields=None):
+    """Call ``sqa_attention_weights`` (``k_scale`` ``None``: none; ``weights`` ``[B, Hkv, T]``
+    float32 with a contiguous last dimension; ``fields`` from :func:`weights_fields`)."""
+    lib = _LIB if _LIB is not None else load()
+    pool, scales, store, rest = fields or weights_fields(query, k_view, k_scale, block_tables,
+                                                         draft_mask, weights, max_seq_len)
+    rc = lib.sqa_attention_weights(_WEIGHTS.pack(
+        _WEIGHTS.size, query.data_ptr(), k_view.data_ptr(), 0, *pool,
+        0 if k_scale is None else k_scale.data_ptr(), *scales, block_tables.data_ptr(),
+        seq_lens.data_ptr(), 0 if draft_mask is None else draft_mask.data_ptr(),
+        weights.data_ptr(), *store, scale, *rest, workspace.data_ptr(),
+        workspace.numel() * workspace.element_size(), stream_handle or 0))
     if rc != SQA_OK:
         raise RuntimeError(f"sqa_attention_weights failed: {last_error(lib)}")
 
 
-def launch_evict(weights, new_weights, kept, seq_lens, new_lens, source, into, block_tables,
-                 new_tables, budget: int, sink: int, recent: int, stream_handle: int):
-    """Call ``sqa_evict``. ``source``, ``into``: (K view, V view, K scale, V scale), the
-    scales ``None`` where the cache has none."""
-    lib = _LIB if _LIB is not None else load()
-
-    def pool(k, v, *_):
-        return (k.data_ptr(), v.data_ptr(), k.shape[0], *k.stride()[:3])
-
-    def scales(_k, _v, ks, vs):
-        return (0, 0, 0, 0) if ks is None else (ks.data_ptr(), vs.data_ptr(), *ks.stride())
+def evict_fields(weights, new_weights, source, into, block_tables, new_tables, budget: int,
+                 sink: int, recent: int):
+    """What of an ``sqa_evict_args`` follows from the tensors' layouts."""
+    def strides(k, _v, ks, _vs):
+        return (k.shape[0], *k.stride()[:3]), (0, 0) if ks is None else ks.stride()
 
     k = source[0]
-    a = _EVICT.pack(
-        _EVICT.size, weights.data_ptr(), weights.stride(0), weights.stride(1),
-        new_weights.data_ptr(), new_weights.stride(0), new_weights.stride(1), kept.data_ptr(),
-        seq_lens.data_ptr(), new_lens.data_ptr(), *pool(*source), *pool(*into), *scales(*source),
-        *scales(*into), block_tables.data_ptr(), new_tables.data_ptr(), weights.shape[2],
-        new_weights.shape[2], block_tables.shape[1], new_tables.shape[1], budget, sink, recent,
-        weights.shape[0], weights.shape[1], k.shape[3], k.shape[1], dtype_code(k.dtype),
-        stream_handle or 0)
-    rc = lib.sqa_evict(a)
+    return (weights.stride()[:2], new_weights.stride()[:2], *strides(*source), *strides(*into),
+            (weights.shape[2], new_weights.shape[2], block_tables.shape[1], new_tables.shape[1],
+             budget, sink, recent, weights.shape[0], weights.shape[1], k.shape[3], k.shape[1],
+             dtype_code(k.dtype)))
+
+
+def launch_evict(weights, new_weights, kept, seq_lens, new_lens, source, into, block_tables,
+                 new_tables, budget: int, sink: int, recent: int, stream_handle: int, fields=None):
+    """Call ``sqa_evict``. ``source``, ``into``: (K view, V view, K scale, V scale), the
+    scales ``None`` where the cache has none; ``fields`` from :func:`evict_fields`."""
+    lib = _LIB if _LIB is not None else load()
+    (w, nw, pool, scales, new_pool, new_scales, rest) = fields or evict_fields(
+        weights, new_weights, source, into, block_tables, new_tables, budget, sink, recent)
+    k, v, ks, vs = source
+    k2, v2, ks2, vs2 = into
+    sp = (0, 0) if ks is None else (ks.data_ptr(), vs.data_ptr())
+    sp2 = (0, 0) if ks is None else (ks2.data_ptr(), vs2.data_ptr())
+    rc = lib.sqa_evict(_EVICT.pack(
+        _EVICT.size, weights.data_ptr(), *w, new_weights.data_ptr(), *nw, kept.data_ptr(),
+        seq_lens.data_ptr(), new_lens.data_ptr(), k.data_ptr(), v.data_ptr(), *pool,
+        k2.data_ptr(), v2.data_ptr(), *new_pool, *sp, *scales, *sp2, *new_scales,
+        block_tables.data_ptr(), new_tables.data_ptr(), *rest, stream_handle or 0))
     if rc != SQA_OK:
         raise RuntimeError(f"sqa_evict failed: {last_error(lib)}")
 

@@ -143,7 +143,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2)))
 void sqa_weigh_kernel(WeighArgs args) {
   const PartialArgs& a = args.p;
   constexpr int KK = Dims<HD>::KK;
-  static_assert(64 % D == 0 && D % 4 == 0, "ring turns within 64 ids, weights four pages at a time");
+  static_assert(D % 4 == 0, "weights are added up four pages at a time");
   WaveItem w;
   if (!wave_item(args, w)) return;  // uniform
   const int lane = threadIdx.x & 63;
@@ -152,12 +152,19 @@ void sqa_weigh_kernel(WeighArgs args) {
   const int n_pages = w.it.p_end - p_begin;
   const int shift = a.page_shift, sub_mask = (1 << shift) - 1;
 
+  // Ids of the ring's next refills, and of those a turn later on their way: scalar loads,
+  // so that no wait for an id is a wait for the pages behind it (a vector load of the next
+  // 64 ids drained the ring where it was taken over).
   const int32_t* row = a.block_tables + (size_t)b * a.bt_stride;
-  auto load_ids = [&](int c) {
-    const long long p = (long long)p_begin + 64 * c + lane;
-    return row[min(p, (long long)a.max_pages - 1) >> shift];
+  auto load_ids = [&](int i, int (&ids)[D]) {
+#pragma unroll
+    for (int j = 0; j < D; ++j)
+      ids[j] = scalar_load(row + (min(p_begin + max(min(i + j, n_pages - 1), 0), a.max_pages - 1) >>
+                                  shift));
   };
-  int ids = load_ids(0), ids_next = load_ids(1);
+  int first_ids[D], ids[D], ids_next[D];
+  load_ids(0, first_ids);
+  load_ids(D, ids);
 
   const WaveRows<NB, 1> map{kvh, a.rows, a.hkv};
   u4 q[NB][KK];
@@ -208,12 +215,9 @@ void sqa_weigh_kernel(WeighArgs args) {
       s.k.k[i] = __builtin_amdgcn_raw_buffer_load_b128(kr, k_lane + 64 * i, 0,
                                                        SUM ? kStreamAux : 0);
   };
-  auto page_id = [&](int i) {
-    return clamp_page(__builtin_amdgcn_readlane(ids, i & 63), a.num_pages);
-  };
   Slot ring[D];
 #pragma unroll
-  for (int j = 0; j < D; ++j) load_page(j < n_pages ? page_id(j) : -1, p_begin + j, ring[j]);
+  for (int j = 0; j < D; ++j) load_page(j < n_pages ? clamp_page(first_ids[j], a.num_pages) : -1, p_begin + j, ring[j]);
 
   const int mask_from = len - a.q_len;
   float m[NB], l[NB];
@@ -238,10 +242,7 @@ void sqa_weigh_kernel(WeighArgs args) {
                                      : kDroppedOffset;
 
   for (int i = 0; i < n_pages; i += D) {
-    if (((i + D) & 63) == 0) {
-      ids = ids_next;
-      ids_next = load_ids((i + D) / 64 + 1);
-    }
+    load_ids(i + 2 * D, ids_next);
     float mine = 0.f, old = 0.f;
 #pragma unroll
     for (int j = 0; j < D; ++j) {
@@ -333,8 +334,10 @@ void sqa_weigh_kernel(WeighArgs args) {
             wrow[wt] = wt < mask_from ? old + mine : mine;
         }
       }
-      load_page(ii + D < n_pages ? page_id(ii + D) : -1, p + D, ring[j]);
+      load_page(ii + D < n_pages ? clamp_page(ids[j], a.num_pages) : -1, p + D, ring[j]);
     }
+#pragma unroll
+    for (int j = 0; j < D; ++j) ids[j] = ids_next[j];
   }
   if constexpr (!SUM) {
 #pragma unroll
@@ -656,7 +659,7 @@ __global__ __launch_bounds__(256) void sqa_move_kernel(EvictArgs a) {
 
 template <int HD, typename E, template <int> class KEYS, int NB>
 void launch_weigh_rows(const WeighArgs& a, dim3 grid, hipStream_t stream) {
-  constexpr int D = HD == 256 ? 4 : 8;
+  constexpr int D = 4;
   const dim3 block(256);
   if constexpr (weights_stored(16 * (NB - 1) + 1, HD, KEYS<HD>::kBytes)) {
     if (a.scores) {

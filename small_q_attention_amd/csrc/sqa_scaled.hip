@@ -73,10 +73,10 @@ struct CodesInt8 : KvFp8<HD> {
   }
 };
 
-// Scores of a page in the exponent's units: (K code . Q^T) * c.
+// Raw scores of a page, K code . Q^T.
 template <int NB, int HD, typename E, typename KV>
 __device__ __forceinline__ void code_scores(f4 (&s)[NB], const typename KV::Regs& r,
-                                            const u4 (&q)[NB][Dims<HD>::KK], float c) {
+                                            const u4 (&q)[NB][Dims<HD>::KK]) {
   constexpr int KK = Dims<HD>::KK;
   u4 k[KK];
   KV::template expand_k<E>(r, k);
@@ -85,7 +85,6 @@ __device__ __forceinline__ void code_scores(f4 (&s)[NB], const typename KV::Regs
     s[nb] = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int kk = 0; kk < KK; ++kk) s[nb] = E::mma_qk(k[kk], q[nb][kk], s[nb]);
-    s[nb] *= c;
   }
 }
 
@@ -132,18 +131,16 @@ __device__ __forceinline__ void nan_values(WaveState<NB, HD>& st, typename KV::R
 // One workgroup = four waves on their own: wave w serves kv head w % wg_heads of the
 // workgroup's heads and work item w / wg_heads of its items, with all query rows of the
 // head (NB blocks of 16). A wave keeps a ring of D pages of codes and their two scales in
-// flight in registers; the ids of the next 64 to 128 pages sit in two registers, one page
-// per lane. No barrier: waves of a workgroup meet only in the memory system, where the
+// flight in registers. No barrier: waves of a workgroup meet only in the memory system, where the
 // heads' slices of a token row are neighbours.
 // P enters the PV product as two bf16 parts of p * v_scale (together within 2^-17 of it,
 // at the cost of one product, as in the bf16 kernels): fp16 would lose the small scales
 // of quiet blocks. The row sums take p itself.
-template <int NB, int D, int HD, typename E, typename KV>
+template <int NB, int D, int HD, typename E, typename KV, bool PIPE>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1)))
 void sqa_scaled_attention_kernel(ScaledArgs args) {
   const PartialArgs& a = args.p;
   constexpr int KK = Dims<HD>::KK, MB = Dims<HD>::MB;
-  static_assert(64 % D == 0, "a ring turn lies within one run of 64 page ids");
   __shared__ float sm_stage[4 * 16 * (HD + 4)];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;
@@ -165,13 +162,19 @@ void sqa_scaled_attention_kernel(ScaledArgs args) {
   const int n_pages = max(__builtin_amdgcn_readfirstlane(it.p_end) - p_begin, 0);
   const int shift = a.page_shift, sub_mask = (1 << shift) - 1;
 
-  // Page ids p_begin + 64 c + lane of the item, clamped into the table row and the pool.
+  // Ids of the ring's next refills, and of those a turn later on their way: scalar loads,
+  // so that no wait for an id is a wait for the pages behind it (a vector load of the next
+  // 64 ids drained the ring where it was taken over).
   const int32_t* row = a.block_tables + (size_t)b * a.bt_stride;
-  auto load_ids = [&](int c) {
-    const long long p = (long long)p_begin + 64 * c + lane;
-    return row[min(p, (long long)a.max_pages - 1) >> shift];
+  auto load_ids = [&](int i, int (&ids)[D]) {
+#pragma unroll
+    for (int j = 0; j < D; ++j)
+      ids[j] = scalar_load(row + (min(p_begin + max(min(i + j, n_pages - 1), 0), a.max_pages - 1) >>
+                                  shift));
   };
-  int ids = load_ids(0), ids_next = load_ids(1);
+  int first_ids[D], ids[D], ids_next[D];
+  load_ids(0, first_ids);
+  load_ids(D, ids);
 
   const WaveRows<NB, 1> map{kvh, a.rows, a.hkv};
   u4 q[NB][KK];
@@ -215,12 +218,9 @@ void sqa_scaled_attention_kernel(ScaledArgs args) {
     s.scale = *(const float*)(scale_lane + max(pid, 0) * args.scales.page_stride);
     KV::load(s.kv, kr, vr, k_lane, v_lane, tok_bytes);
   };
-  auto page_id = [&](int i) {  // i within the 64 ids at hand
-    return clamp_page(__builtin_amdgcn_readlane(ids, i & 63), a.num_pages);
-  };
   Slot ring[D];
 #pragma unroll
-  for (int j = 0; j < D; ++j) load_page(j < n_pages ? page_id(j) : -1, p_begin + j, ring[j]);
+  for (int j = 0; j < D; ++j) load_page(j < n_pages ? clamp_page(first_ids[j], a.num_pages) : -1, p_begin + j, ring[j]);
 
   WaveState<NB, HD> st;
 #pragma unroll
@@ -232,11 +232,10 @@ void sqa_scaled_attention_kernel(ScaledArgs args) {
   }
   const int mask_from = len - a.q_len;  // pages with a token from here on are masked
 
+  f4 ahead[NB];
+  if constexpr (PIPE) code_scores<NB, HD, E, KV>(ahead, ring[0].kv, q);
   for (int i = 0; i < n_pages; i += D) {
-    if (((i + D) & 63) == 0) {  // the ring's refills enter the next run of ids
-      ids = ids_next;
-      ids_next = load_ids((i + D) / 64 + 1);
-    }
+    load_ids(i + 2 * D, ids_next);
 #pragma unroll
     for (int j = 0; j < D; ++j) {
       const int ii = i + j;
@@ -246,11 +245,21 @@ void sqa_scaled_attention_kernel(ScaledArgs args) {
             float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, ring[j].scale), 0));
         const float vs = __builtin_bit_cast(
             float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, ring[j].scale), 32));
+        float c = a.scale_log2 * ks;
         f4 s[NB];
-        code_scores<NB, HD, E, KV>(s, ring[j].kv, q, a.scale_log2 * ks);
+        if constexpr (PIPE) {
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb) s[nb] = ahead[nb];
+          code_scores<NB, HD, E, KV>(ahead, ring[(j + 1) % D].kv, q);
+        } else {
+          code_scores<NB, HD, E, KV>(s, ring[j].kv, q);
+        }
         const bool masked = (p + 1) * kPageSize > mask_from;  // uniform
         if (masked) {
           // After the scale, so that a scale of 0, infinity or NaN leaves them -inf.
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb) s[nb] *= c;
+          c = 1.f;
           const int tok0 = p * kPageSize + 4 * g16;
           mask_scores<NB>(s, bits.b, mask_from, tok0, len);
 #pragma unroll
@@ -261,7 +270,7 @@ void sqa_scaled_attention_kernel(ScaledArgs args) {
         }
         float lm[NB];
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb) lm[nb] = max4(s[nb]);
+        for (int nb = 0; nb < NB; ++nb) lm[nb] = max4(s[nb]) * c;
         raise_max<NB, HD>(st, lm);
         if constexpr (KV::kNan)
           if (masked) nan_values<NB, HD, KV>(st, ring[j].kv, s);
@@ -272,7 +281,7 @@ void sqa_scaled_attention_kernel(ScaledArgs args) {
           float pr[4], pv[4], sum = 0.f;
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            pr[e] = fast_exp2(s[nb][e] - mu);
+            pr[e] = fast_exp2(fmaf(s[nb][e], c, -mu));
             pv[e] = pr[e] * vs;
           }
           st.l[nb] += (pr[0] + pr[1]) + (pr[2] + pr[3]);
@@ -290,8 +299,10 @@ void sqa_scaled_attention_kernel(ScaledArgs args) {
           for (int nb = 0; nb < NB; ++nb)
             st.acc[mb][nb] = ElemBF16::mma_pv(av[mb], hi[nb], lo[nb], st.acc[mb][nb]);
       }
-      load_page(ii + D < n_pages ? page_id(ii + D) : -1, p_begin + ii + D, ring[j]);
+      load_page(ii + D < n_pages ? clamp_page(ids[j], a.num_pages) : -1, p_begin + ii + D, ring[j]);
     }
+#pragma unroll
+    for (int j = 0; j < D; ++j) ids[j] = ids_next[j];
   }
   write_results<NB, HD, E>(a, st, sm_stage + wave * 16 * (HD + 4), map, it.count <= 1, false, b,
                            (size_t)it.slot, a.hkv, 0);
@@ -464,29 +475,30 @@ void launch_append_as(const AppendArgs& a, dim3 grid, hipStream_t stream) {
     launch_append_hd<256, BF16, INT8>(a, grid, stream);
 }
 
+constexpr bool PIPE1 = false, PIPE2 = true, PIPE4 = false;
 template <typename E, template <int> class KV>
 void launch_scaled_as(const ScaledArgs& a, dim3 grid, hipStream_t stream) {
   const dim3 block(256);
   const int rows = a.p.rows;
   if (a.p.head_dim == 64) {
     if (rows <= 16)
-      hipLaunchKernelGGL((sqa_scaled_attention_kernel<1, 8, 64, E, KV<64>>), grid, block, 0, stream, a);
+      hipLaunchKernelGGL((sqa_scaled_attention_kernel<1, 8, 64, E, KV<64>, PIPE1>), grid, block, 0, stream, a);
     else if (rows <= 32)
-      hipLaunchKernelGGL((sqa_scaled_attention_kernel<2, 8, 64, E, KV<64>>), grid, block, 0, stream, a);
+      hipLaunchKernelGGL((sqa_scaled_attention_kernel<2, 8, 64, E, KV<64>, PIPE2>), grid, block, 0, stream, a);
     else
-      hipLaunchKernelGGL((sqa_scaled_attention_kernel<4, 4, 64, E, KV<64>>), grid, block, 0, stream, a);
+      hipLaunchKernelGGL((sqa_scaled_attention_kernel<4, 4, 64, E, KV<64>, PIPE4>), grid, block, 0, stream, a);
   } else if (a.p.head_dim == 128) {
     if (rows <= 16)
-      hipLaunchKernelGGL((sqa_scaled_attention_kernel<1, 4, 128, E, KV<128>>), grid, block, 0, stream, a);
+      hipLaunchKernelGGL((sqa_scaled_attention_kernel<1, 4, 128, E, KV<128>, PIPE1>), grid, block, 0, stream, a);
     else if (rows <= 32)
-      hipLaunchKernelGGL((sqa_scaled_attention_kernel<2, 4, 128, E, KV<128>>), grid, block, 0, stream, a);
+      hipLaunchKernelGGL((sqa_scaled_attention_kernel<2, 4, 128, E, KV<128>, PIPE2>), grid, block, 0, stream, a);
     else
-      hipLaunchKernelGGL((sqa_scaled_attention_kernel<4, 4, 128, E, KV<128>>), grid, block, 0, stream, a);
+      hipLaunchKernelGGL((sqa_scaled_attention_kernel<4, 4, 128, E, KV<128>, PIPE4>), grid, block, 0, stream, a);
   } else {
     if (rows <= 16)
-      hipLaunchKernelGGL((sqa_scaled_attention_kernel<1, 2, 256, E, KV<256>>), grid, block, 0, stream, a);
+      hipLaunchKernelGGL((sqa_scaled_attention_kernel<1, 2, 256, E, KV<256>, PIPE1>), grid, block, 0, stream, a);
     else
-      hipLaunchKernelGGL((sqa_scaled_attention_kernel<2, 2, 256, E, KV<256>>), grid, block, 0, stream, a);
+      hipLaunchKernelGGL((sqa_scaled_attention_kernel<2, 2, 256, E, KV<256>, PIPE2>), grid, block, 0, stream, a);
   }
 }
 

@@ -20,6 +20,7 @@ import torch
 from . import _lib
 from . import scaled_cache as sc
 from .cuda import _tracing
+from .masks import as_words
 
 _HALF = (torch.float16, torch.bfloat16)
 
@@ -41,18 +42,42 @@ def _check_scaled(cache, *scales):
             sc.check_scale(s, cache, "a cache's scale")
 
 
+_WEIGHS, _EVICTIONS = sc.Layouts(), sc.Layouts()
+
+
 def run_weights(query, key_cache, key_scale, block_tables, seq_lens, words, weights, scale,
-                max_seq_len):
-    """Plan and launch a checked call."""
-    batch, q_len, hq, d = query.shape
+                max_seq_len, known=None):
+    """Plan and launch a checked call (``known``: its :func:`_weights_plan`)."""
+    need, fields = known or _weights_plan(query, key_cache, key_scale, block_tables, words,
+                                          weights, max_seq_len)
     index = query.device.index
-    need = _lib.weights_workspace_bytes(index, batch, q_len, hq, key_cache.shape[2], d, max_seq_len,
-                                        block_tables.shape[1] * (key_cache.shape[1] // 16),
-                                        _lib.dtype_code(key_cache.dtype))
     stream = _lib.raw_stream(index)
     workspace = _lib.workspace_for(need, query, index, stream)
     _lib.launch_weights(query, key_cache, key_scale, block_tables, seq_lens, words, weights, scale,
-                        max_seq_len, workspace, stream)
+                        max_seq_len, workspace, stream, fields)
+
+
+def _weights_plan(query, key_cache, key_scale, block_tables, words, weights, max_seq_len):
+    batch, q_len, hq, d = query.shape
+    need = _lib.weights_workspace_bytes(query.device.index, batch, q_len, hq, key_cache.shape[2], d,
+                                        max_seq_len,
+                                        block_tables.shape[1] * (key_cache.shape[1] // 16),
+                                        _lib.dtype_code(key_cache.dtype))
+    return need, _lib.weights_fields(query, key_cache, key_scale, block_tables, words, weights,
+                                     max_seq_len)
+
+
+def _check_accumulate(query, key_cache, block_tables, seq_lens, weights, key_scale, words):
+    sc.check_pool(key_cache)
+    sc.check_query(query, key_cache)
+    if key_cache.dtype != query.dtype and key_cache.dtype not in sc.CODE_DTYPES:
+        raise ValueError("key_cache must hold the query's type, torch.float8_e4m3fn or torch.int8")
+    _check_scaled(key_cache, key_scale)
+    batch = query.shape[0]
+    sc.check_batch(batch, block_tables, seq_lens)
+    _check_weights(weights, batch, key_cache.shape[2])
+    sc.check_on(query.device, key_cache=key_cache, key_scale=key_scale, block_tables=block_tables,
+                seq_lens=seq_lens, weights=weights, mask=words, query=query)
 
 
 def accumulate_attention_weights(query, key_cache, block_tables, seq_lens, weights, key_scale=None,
@@ -67,42 +92,91 @@ def accumulate_attention_weights(query, key_cache, block_tables, seq_lens, weigh
     ``T`` on are not recorded, entries past a sequence's end not touched. ``max_seq_len``
     > 0 promises that no sequence is longer. Returns ``weights``.
     """
-    sc.check_pool(key_cache)
-    sc.check_query(query, key_cache)
-    if key_cache.dtype != query.dtype and key_cache.dtype not in sc.CODE_DTYPES:
-        raise ValueError("key_cache must hold the query's type, torch.float8_e4m3fn or torch.int8")
-    _check_scaled(key_cache, key_scale)
-    batch, q_len = query.shape[:2]
-    sc.check_batch(batch, block_tables, seq_lens)
-    _check_weights(weights, batch, key_cache.shape[2])
-    device = query.device
-    sc.check_on(device, key_cache=key_cache, key_scale=key_scale, block_tables=block_tables,
-                seq_lens=seq_lens, weights=weights)
+    if query.dim() != 4:
+        raise ValueError("query must be a contiguous [B, Q, Hq, D] tensor")
     scale = sc.check_softmax_scale(scale, query.shape[3])
-    words = sc.mask_words(mask, batch, q_len, device)
+    words = None if mask is None else as_words(mask, query.shape[0], query.shape[1])
     max_seq_len = max(int(max_seq_len), 0)
     if _tracing():
+        _check_accumulate(query, key_cache, block_tables, seq_lens, weights, key_scale, words)
         from . import _op  # noqa: F401  (registers the ops)
 
         torch.ops.sqa.accumulate_attention_weights(query, key_cache, key_scale, block_tables,
                                                    seq_lens, words, weights, scale, max_seq_len)
         return weights
-    sc.on_device(device, lambda: run_weights(query, key_cache, key_scale, block_tables, seq_lens,
-                                             words, weights, scale, max_seq_len))
+    layout = sc.layout
+    seen = (layout(query), layout(key_cache), layout(key_scale), layout(block_tables),
+            layout(seq_lens), layout(weights), layout(words), max_seq_len)
+    known = _WEIGHS.get(seen)
+    if known is None:
+        _check_accumulate(query, key_cache, block_tables, seq_lens, weights, key_scale, words)
+        known = _WEIGHS.keep(seen, sc.on_device(query.device, _weights_plan, query, key_cache,
+                                                key_scale, block_tables, words, weights,
+                                                max_seq_len))
+    sc.check_aligned(16, query, key_cache)
+    sc.on_device(query.device, run_weights, query, key_cache, key_scale, block_tables, seq_lens,
+                 words, weights, scale, max_seq_len, known)
     return weights
 
 
 def run_evict(weights, new_weights, source, block_tables, seq_lens, into, new_tables, budget, sink,
-              recent):
+              recent, fields=None):
     """Allocate what a checked call returns and launch it."""
-    kept = torch.empty(weights.shape[0], weights.shape[1], budget, dtype=torch.int32,
-                       device=weights.device)
+    batch, hkv, _ = weights.shape
+    device = weights.device
+    kept = torch.empty((batch, hkv, budget), dtype=torch.int32, device=device)
     new_lens = torch.empty_like(seq_lens)
     if new_weights is None:
-        new_weights = torch.empty(kept.shape, dtype=torch.float32, device=weights.device)
+        new_weights = torch.empty((batch, hkv, budget), dtype=torch.float32, device=device)
     _lib.launch_evict(weights, new_weights, kept, seq_lens, new_lens, source, into, block_tables,
-                      new_tables, budget, sink, recent, _lib.raw_stream(weights.device.index))
+                      new_tables, budget, sink, recent, _lib.raw_stream(device.index), fields)
     return new_lens, new_weights, kept
+
+
+def _check_evict(weights, source, block_tables, seq_lens, new_block_tables, budget, sink, recent,
+                 into, new_weights):
+    key_cache, value_cache, key_scale, value_scale = source
+    sc.check_pool(key_cache)
+    if key_cache.dtype not in _HALF + sc.CODE_DTYPES:
+        raise ValueError("caches must hold float16, bfloat16, float8_e4m3fn or int8")
+    sc.check_same_layout(key_cache, value_cache, "key_cache and value_cache")
+    if (key_scale is None) != (value_scale is None):
+        raise ValueError("key_scale and value_scale come together")
+    if len(into) != 4 or into[0] is None or into[1] is None:
+        raise ValueError("into must be (key_cache, value_cache[, key_scale, value_scale])")
+    sc.check_pool(into[0], "into's key_cache")
+    sc.check_same_layout(into[0], into[1], "into's caches")
+    if into[0].dtype != key_cache.dtype or into[0].shape[1:] != key_cache.shape[1:]:
+        raise ValueError("into's caches must match in type, page size, kv heads and head_dim")
+    if (into[2] is None) != (key_scale is None) or (into[3] is None) != (key_scale is None):
+        raise ValueError("into needs scales where the cache has them, and only there")
+    _check_scaled(key_cache, key_scale, value_scale)
+    _check_scaled(into[0], into[2], into[3])
+    if key_scale is not None:
+        sc.check_same_layout(key_scale, value_scale, "key_scale and value_scale")
+        sc.check_same_layout(into[2], into[3], "into's scales")
+    for cache in (key_cache, into[0]):
+        if any(x * cache.element_size() % 16 for x in cache.stride()[:3]):
+            raise ValueError("cache strides must be multiples of 16 bytes")
+    batch, hkv = seq_lens.shape[0] if seq_lens.dim() == 1 else 0, key_cache.shape[2]
+    if batch == 0:
+        raise ValueError("seq_lens must be a [batch] tensor and not empty")
+    sc.check_batch(batch, block_tables, seq_lens)
+    sc.check_batch(batch, new_block_tables, seq_lens, "new_block_tables")
+    _check_weights(weights, batch, hkv)
+    if budget <= 0 or sink < 0 or recent < 0 or sink + recent > budget:
+        raise ValueError("budget must be positive and hold sink + recent tokens")
+    if budget > new_block_tables.shape[1] * key_cache.shape[1]:
+        raise ValueError("new_block_tables must have pages for budget tokens")
+    if new_weights is not None:
+        _check_weights(new_weights, batch, hkv, "new_weights")
+        if new_weights.shape[2] < budget:
+            raise ValueError("new_weights must hold budget tokens")
+    sc.check_on(weights.device, new_weights=new_weights, key_cache=key_cache,
+                value_cache=value_cache, key_scale=key_scale, value_scale=value_scale,
+                block_tables=block_tables, seq_lens=seq_lens, new_block_tables=new_block_tables,
+                into_key_cache=into[0], into_value_cache=into[1], into_key_scale=into[2],
+                into_value_scale=into[3])
 
 
 def evict_by_weight(weights, key_cache, value_cache, block_tables, seq_lens, new_block_tables,
@@ -129,57 +203,29 @@ def evict_by_weight(weights, key_cache, value_cache, block_tables, seq_lens, new
     ``min(seq_lens, budget)``, the moved weights (0 past them) and the positions the tokens
     had before (-1 past them).
     """
-    sc.check_pool(key_cache)
-    if key_cache.dtype not in _HALF + sc.CODE_DTYPES:
-        raise ValueError("caches must hold float16, bfloat16, float8_e4m3fn or int8")
-    sc.check_same_layout(key_cache, value_cache, "key_cache and value_cache")
-    if (key_scale is None) != (value_scale is None):
-        raise ValueError("key_scale and value_scale come together")
-    source = (key_cache, value_cache, key_scale, value_scale)
-    into = source if into is None else tuple(into) + (None,) * (4 - len(tuple(into)))
-    if len(into) != 4 or into[0] is None or into[1] is None:
-        raise ValueError("into must be (key_cache, value_cache[, key_scale, value_scale])")
-    sc.check_pool(into[0], "into's key_cache")
-    sc.check_same_layout(into[0], into[1], "into's caches")
-    if into[0].dtype != key_cache.dtype or into[0].shape[1:] != key_cache.shape[1:]:
-        raise ValueError("into's caches must match in type, page size, kv heads and head_dim")
-    if (into[2] is None) != (key_scale is None) or (into[3] is None) != (key_scale is None):
-        raise ValueError("into needs scales where the cache has them, and only there")
-    _check_scaled(key_cache, key_scale, value_scale)
-    _check_scaled(into[0], into[2], into[3])
-    if key_scale is not None:
-        sc.check_same_layout(key_scale, value_scale, "key_scale and value_scale")
-        sc.check_same_layout(into[2], into[3], "into's scales")
-    for cache in (key_cache, into[0]):
-        if any(x * cache.element_size() % 16 for x in cache.stride()[:3]):
-            raise ValueError("cache strides must be multiples of 16 bytes")
-    if sc.misaligned(value_cache, 16) or sc.misaligned(into[1], 16):
-        raise ValueError("caches must be 16-byte aligned")
-    batch, hkv = seq_lens.shape[0] if seq_lens.dim() == 1 else 0, key_cache.shape[2]
-    if batch == 0:
-        raise ValueError("seq_lens must be a [batch] tensor and not empty")
-    sc.check_batch(batch, block_tables, seq_lens)
-    sc.check_batch(batch, new_block_tables, seq_lens, "new_block_tables")
-    _check_weights(weights, batch, hkv)
-    budget, sink, recent = int(budget), int(sink), int(recent)
-    if budget <= 0 or sink < 0 or recent < 0 or sink + recent > budget:
-        raise ValueError("budget must be positive and hold sink + recent tokens")
-    if budget > new_block_tables.shape[1] * key_cache.shape[1]:
-        raise ValueError("new_block_tables must have pages for budget tokens")
-    if new_weights is not None:
-        _check_weights(new_weights, batch, hkv, "new_weights")
-        if new_weights.shape[2] < budget:
-            raise ValueError("new_weights must hold budget tokens")
-    sc.check_on(weights.device, new_weights=new_weights, key_cache=key_cache,
-                value_cache=value_cache, key_scale=key_scale, value_scale=value_scale,
-                block_tables=block_tables, seq_lens=seq_lens, new_block_tables=new_block_tables,
-                into_key_cache=into[0], into_value_cache=into[1], into_key_scale=into[2],
-                into_value_scale=into[3])
     if _tracing():
         raise ValueError("evict_by_weight is not traced: call it outside torch.compile")
-    return sc.on_device(weights.device, lambda: run_evict(
-        weights, new_weights, source, block_tables, seq_lens, into, new_block_tables, budget, sink,
-        recent))
+    budget, sink, recent = int(budget), int(sink), int(recent)
+    source = (key_cache, value_cache, key_scale, value_scale)
+    if into is None:
+        into = source
+    elif len(into) == 2:
+        into = (*into, None, None)
+    layout = sc.layout
+    seen = (layout(weights), layout(new_weights), layout(key_cache), layout(value_cache),
+            layout(key_scale), layout(value_scale), layout(block_tables), layout(seq_lens),
+            layout(new_block_tables), *[layout(t) for t in into], budget, sink, recent)
+    fields = _EVICTIONS.get(seen)
+    if fields is None:
+        _check_evict(weights, source, block_tables, seq_lens, new_block_tables, budget, sink,
+                     recent, into, new_weights)
+        moved = weights[:, :, :budget].new_empty((*weights.shape[:2], budget)) \
+            if new_weights is None else new_weights
+        fields = _EVICTIONS.keep(seen, _lib.evict_fields(
+            weights, moved, source, into, block_tables, new_block_tables, budget, sink, recent))
+    sc.check_aligned(16, key_cache, value_cache, into[0], into[1])
+    return sc.on_device(weights.device, run_evict, weights, new_weights, source, block_tables,
+                        seq_lens, into, new_block_tables, budget, sink, recent, fields)
 
 
 __all__ = ["accumulate_attention_weights", "evict_by_weight"]

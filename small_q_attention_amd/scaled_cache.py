@@ -27,10 +27,12 @@ from .masks import as_words
 CODE_DTYPES = (torch.float8_e4m3fn, torch.int8)
 
 
-def misaligned(t, n):
-    """Whether a tensor starts off an ``n``-byte boundary (a traced one has no address;
-    the library checks it when the graph runs)."""
-    return not _tracing() and t.data_ptr() % n != 0
+def check_aligned(n, *tensors):
+    """ValueError unless the tensors start on ``n``-byte boundaries (not for traced ones,
+    which have no address: the library checks it when the graph runs)."""
+    for t in tensors:
+        if t.data_ptr() % n:
+            raise ValueError(f"a tensor of {tuple(t.shape)} does not start on a {n}-byte boundary")
 
 
 def check_on(device, **tensors):
@@ -52,9 +54,9 @@ def check_pool(cache, what="key_cache"):
     if cache.shape[3] not in HEAD_DIMS:
         raise ValueError("this build supports head_dim 64, 128 or 256")
     s = cache.stride()
-    if s[3] != 1 or s[0] % 8 or s[1] % 8 or s[2] % 8 or misaligned(cache, 16):
-        raise ValueError(f"{what} needs a contiguous head dimension, other strides in multiples "
-                         "of 8 elements and a 16-byte aligned start")
+    if s[3] != 1 or s[0] % 8 or s[1] % 8 or s[2] % 8:
+        raise ValueError(f"{what} needs a contiguous head dimension and other strides in "
+                         "multiples of 8 elements")
 
 
 def check_same_layout(a, b, what):
@@ -79,8 +81,8 @@ def check_batch(batch, block_tables, seq_lens, name="block_tables"):
 
 def check_query(query, cache):
     if query.dim() != 4 or not query.is_contiguous() or query.shape[0] == 0 \
-            or query.shape[1] == 0 or misaligned(query, 16):
-        raise ValueError("query must be a contiguous, 16-byte aligned [B, Q, Hq, D] tensor")
+            or query.shape[1] == 0:
+        raise ValueError("query must be a contiguous [B, Q, Hq, D] tensor")
     if query.dtype not in (torch.float16, torch.bfloat16):
         raise ValueError("query must be float16 or bfloat16")
     hq, d, hkv = query.shape[2], query.shape[3], cache.shape[2]
@@ -98,20 +100,29 @@ def check_softmax_scale(scale, d):
     return scale
 
 
-def mask_words(mask, batch, q_len, device):
-    if mask is None:
-        return None
-    words = as_words(mask, batch, q_len)
-    check_on(device, mask=words)
-    return words
-
-
-def on_device(device, call):
-    """``call()`` with ``device`` as the current one."""
-    if device.index == torch.cuda.current_device():
-        return call()
+def on_device(device, call, *args):
+    """``call(*args)`` with ``device`` as the current one."""
+    current, _ = _lib._CUDA_STATE or _lib._cuda_state(torch)
+    if device.index == current():
+        return call(*args)
     with torch.cuda.device(device):
-        return call()
+        return call(*args)
+
+
+class Layouts(dict):
+    """What the checks of an entry point found for the layouts (shapes, strides, types and
+    devices, nothing of the data) of a call's tensors: a serving loop makes the same kind
+    of call again and again, and the checks cost more than the launch. Bounded."""
+
+    def keep(self, key, value):
+        if len(self) >= 1024:
+            self.clear()
+        self[key] = value
+        return value
+
+
+def layout(t):
+    return None if t is None else (t.shape, t.stride(), t.dtype, t.device)
 
 
 def _check_cache(key_cache, value_cache, key_scale, value_scale):
@@ -119,8 +130,6 @@ def _check_cache(key_cache, value_cache, key_scale, value_scale):
     if key_cache.dtype not in CODE_DTYPES:
         raise ValueError("caches must hold torch.float8_e4m3fn or torch.int8")
     check_same_layout(key_cache, value_cache, "key_cache and value_cache")
-    if misaligned(value_cache, 16):
-        raise ValueError("value_cache needs a 16-byte aligned start")
     check_scale(key_scale, key_cache)
     check_scale(value_scale, key_cache, "value_scale")
     check_same_layout(key_scale, value_scale, "key_scale and value_scale")
@@ -141,6 +150,38 @@ def append_scaled_kv(key, value, key_cache, value_cache, key_scale, value_scale,
     type's largest finite value; a NaN does not count and is stored as NaN (e4m3) or 0
     (int8). No two sequences may write the same page in one call.
     """
+    if _tracing():
+        _check_append(key, value, key_cache, value_cache, key_scale, value_scale, block_tables,
+                      seq_lens, new_lens)
+        from . import _op  # noqa: F401  (registers the ops)
+
+        torch.ops.sqa.append_scaled_kv(key, value, key_cache, value_cache, key_scale, value_scale,
+                                       block_tables, seq_lens, new_lens)
+        return
+    seen = (layout(key), layout(value), layout(key_cache), layout(value_cache), layout(key_scale),
+            layout(value_scale), layout(block_tables), layout(seq_lens), layout(new_lens))
+    fields = _APPENDS.get(seen)
+    if fields is None:
+        _check_append(key, value, key_cache, value_cache, key_scale, value_scale, block_tables,
+                      seq_lens, new_lens)
+        fields = _APPENDS.keep(seen, _lib.append_fields(key, value, key_cache, key_scale,
+                                                        block_tables))
+    check_aligned(16, key, value, key_cache, value_cache)
+    on_device(key.device, _launch_append, key, value, key_cache, value_cache, key_scale,
+              value_scale, block_tables, seq_lens, new_lens, fields)
+
+
+_APPENDS, _ATTENTIONS = Layouts(), Layouts()
+
+
+def _launch_append(key, value, key_cache, value_cache, key_scale, value_scale, block_tables,
+                   seq_lens, new_lens, fields):
+    _lib.launch_append(key, value, key_cache, value_cache, key_scale, value_scale, block_tables,
+                       seq_lens, new_lens, _lib.raw_stream(key.device.index), fields)
+
+
+def _check_append(key, value, key_cache, value_cache, key_scale, value_scale, block_tables,
+                  seq_lens, new_lens):
     if key.dim() != 4 or value.shape != key.shape or key.shape[0] == 0 or key.shape[1] == 0:
         raise ValueError("key and value must be [B, Q, Hkv, D] tensors of one shape")
     if key.dtype not in (torch.float16, torch.bfloat16) or value.dtype != key.dtype:
@@ -150,9 +191,9 @@ def append_scaled_kv(key, value, key_cache, value_cache, key_scale, value_scale,
         raise ValueError("key and value need the cache's kv heads and head_dim")
     for t in (key, value):
         s = t.stride()
-        if s[3] != 1 or s[0] % 8 or s[1] % 8 or s[2] % 8 or misaligned(t, 16):
-            raise ValueError("key and value need a contiguous head dimension, other strides in "
-                             "multiples of 8 elements and a 16-byte aligned start")
+        if s[3] != 1 or s[0] % 8 or s[1] % 8 or s[2] % 8:
+            raise ValueError("key and value need a contiguous head dimension and other strides "
+                             "in multiples of 8 elements")
     batch = key.shape[0]
     check_batch(batch, block_tables, seq_lens)
     if new_lens is not None and (new_lens.dtype != torch.int32 or new_lens.shape != seq_lens.shape
@@ -161,26 +202,14 @@ def append_scaled_kv(key, value, key_cache, value_cache, key_scale, value_scale,
     check_on(key.device, value=value, key_cache=key_cache, value_cache=value_cache,
              key_scale=key_scale, value_scale=value_scale, block_tables=block_tables,
              seq_lens=seq_lens, new_lens=new_lens)
-    if _tracing():
-        from . import _op  # noqa: F401  (registers the ops)
-
-        torch.ops.sqa.append_scaled_kv(key, value, key_cache, value_cache, key_scale, value_scale,
-                                       block_tables, seq_lens, new_lens)
-        return
-    on_device(key.device, lambda: _lib.launch_append(
-        key, value, key_cache, value_cache, key_scale, value_scale, block_tables, seq_lens,
-        new_lens, _lib.raw_stream(key.device.index)))
 
 
 def run_attention(query, key_cache, value_cache, key_scale, value_scale, block_tables, seq_lens,
-                  words, scale, out_scale, max_seq_len, out, workspace):
-    """Plan and launch a checked call."""
-    batch, q_len, hq, d = query.shape
-    page, hkv = key_cache.shape[1], key_cache.shape[2]
+                  words, scale, out_scale, max_seq_len, out, workspace, known=None):
+    """Plan and launch a checked call (``known``: its :func:`_attention_plan`)."""
+    slots, need, fields = known or _attention_plan(query, key_cache, key_scale, block_tables,
+                                                   words, max_seq_len)
     index = query.device.index
-    slots = _lib.plan_scaled(index, batch, hkv, max_seq_len,
-                             block_tables.shape[1] * (page // 16))
-    need = _lib.workspace_bytes(batch, q_len, hq, hkv, d, slots, 0)
     stream = _lib.raw_stream(index)
     if workspace is None:
         workspace = _lib.workspace_for(need, query, index, stream)
@@ -190,8 +219,30 @@ def run_attention(query, key_cache, value_cache, key_scale, value_scale, block_t
     if out is None:
         out = torch.empty_like(query)
     _lib.launch_scaled(query, out, key_cache, value_cache, key_scale, value_scale, block_tables,
-                       seq_lens, words, scale, out_scale, slots, workspace, stream)
+                       seq_lens, words, scale, out_scale, slots, workspace, stream, None, fields)
     return out
+
+
+def _attention_plan(query, key_cache, key_scale, block_tables, words, max_seq_len):
+    batch, q_len, hq, d = query.shape
+    page, hkv = key_cache.shape[1], key_cache.shape[2]
+    slots = _lib.plan_scaled(query.device.index, batch, hkv, max_seq_len,
+                             block_tables.shape[1] * (page // 16))
+    need = _lib.workspace_bytes(batch, q_len, hq, hkv, d, slots, 0)
+    return slots, need, _lib.scaled_fields(query, key_cache, key_scale, block_tables, words)
+
+
+def _check_attention(query, key_cache, value_cache, key_scale, value_scale, block_tables,
+                     seq_lens, words, out, workspace_buffer):
+    _check_cache(key_cache, value_cache, key_scale, value_scale)
+    check_query(query, key_cache)
+    check_batch(query.shape[0], block_tables, seq_lens)
+    check_on(query.device, key_cache=key_cache, value_cache=value_cache, key_scale=key_scale,
+             value_scale=value_scale, block_tables=block_tables, seq_lens=seq_lens, out=out,
+             workspace_buffer=workspace_buffer, mask=words, query=query)
+    if out is not None and (out.shape != query.shape or out.dtype != query.dtype
+                            or not out.is_contiguous()):
+        raise ValueError("out must be a contiguous tensor shaped and typed like query")
 
 
 def paged_attention_scaled(query, key_cache, value_cache, key_scale, value_scale, block_tables,
@@ -208,30 +259,33 @@ def paged_attention_scaled(query, key_cache, value_cache, key_scale, value_scale
     a caller's buffer for the split partials; ``None`` takes one kept per stream, or, under
     graph capture, one of the graph's own. Returns ``out`` (``[B, Q, Hq, D]``).
     """
-    _check_cache(key_cache, value_cache, key_scale, value_scale)
-    check_query(query, key_cache)
-    batch, q_len = query.shape[:2]
-    check_batch(batch, block_tables, seq_lens)
-    device = query.device
-    check_on(device, key_cache=key_cache, value_cache=value_cache, key_scale=key_scale,
-             value_scale=value_scale, block_tables=block_tables, seq_lens=seq_lens, out=out,
-             workspace_buffer=workspace_buffer, query=query)
+    if query.dim() != 4:
+        raise ValueError("query must be a contiguous [B, Q, Hq, D] tensor")
     scale = check_softmax_scale(scale, query.shape[3])
-    words = mask_words(mask, batch, q_len, device)
-    if out is not None and (out.shape != query.shape or out.dtype != query.dtype
-                            or not out.is_contiguous() or misaligned(out, 8)):
-        raise ValueError("out must be a contiguous tensor shaped and typed like query")
+    words = None if mask is None else as_words(mask, query.shape[0], query.shape[1])
     max_seq_len = max(int(max_seq_len), 0)
     if _tracing():
+        _check_attention(query, key_cache, value_cache, key_scale, value_scale, block_tables,
+                         seq_lens, words, out, workspace_buffer)
         from . import _op  # noqa: F401  (registers the ops)
 
         res = torch.ops.sqa.paged_attention_scaled(
             query, key_cache, value_cache, key_scale, value_scale, block_tables, seq_lens, words,
             scale, float(out_scale), max_seq_len)
         return res if out is None else out.copy_(res)
-    return on_device(device, lambda: run_attention(
-        query, key_cache, value_cache, key_scale, value_scale, block_tables, seq_lens, words,
-        scale, float(out_scale), max_seq_len, out, workspace_buffer))
+    seen = (layout(query), layout(key_cache), layout(value_cache), layout(key_scale),
+            layout(value_scale), layout(block_tables), layout(seq_lens), layout(words),
+            layout(out), workspace_buffer is None or workspace_buffer.device, max_seq_len)
+    known = _ATTENTIONS.get(seen)
+    if known is None:
+        _check_attention(query, key_cache, value_cache, key_scale, value_scale, block_tables,
+                         seq_lens, words, out, workspace_buffer)
+        known = _ATTENTIONS.keep(seen, on_device(query.device, _attention_plan, query, key_cache,
+                                                 key_scale, block_tables, words, max_seq_len))
+    check_aligned(16, query, key_cache, value_cache)
+    return on_device(query.device, run_attention, query, key_cache, value_cache, key_scale,
+                     value_scale, block_tables, seq_lens, words, scale, float(out_scale),
+                     max_seq_len, out, workspace_buffer, known)
 
 
 __all__ = ["append_scaled_kv", "paged_attention_scaled"]

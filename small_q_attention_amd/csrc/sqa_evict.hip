@@ -417,13 +417,14 @@ __global__ __launch_bounds__(256) void sqa_weigh_join_kernel(WeighArgs args) {
 // Eviction.
 // ---------------------------------------------------------------------------------
 
-// Larger weights give larger keys; -0 and 0 the same one, NaN the least of all.
+// Larger weights give larger keys; -0 and 0 the same one, NaN the least of all. Keys of
+// weights lie in [kNanKey, kAlways); 0 is no token, kAlways one that stays in any case.
+constexpr unsigned kNanKey = 1u, kAlways = 0xffffffffu;
 __device__ __forceinline__ unsigned weight_key(float w) {
-  if (w != w) return 0u;
   const unsigned u = __builtin_bit_cast(unsigned, w + 0.f);  // -0 + 0 = 0
-  return (u & 0x80000000u) ? ~u : u | 0x80000000u;
+  const unsigned k = (u & 0x80000000u) ? ~u : u | 0x80000000u;
+  return w != w ? kNanKey : k;
 }
-
 constexpr int kSelectThreads = 1024, kSelectWaves = kSelectThreads / 64;
 
 // Which tokens of one sequence and kv head stay. The smallest key that stays is found by
@@ -431,8 +432,8 @@ constexpr int kSelectThreads = 1024, kSelectWaves = kSelectThreads / 64;
 // 10 bits, histograms in LDS); tokens above it stay, and of those that equal it the first.
 // Each wave then counts its own run of tokens, and after one exchange writes its kept
 // tokens in order. All counts are integers: the same weights give the same tokens.
-// R > 0: a thread holds the weights of its R tokens in registers through all of it (up to
-// 1024 R tokens); R = 0 reads them again each time.
+// R > 0: a thread holds its R tokens' weights and keys in registers through all of it (up to
+// 1024 R tokens); R = 0 reads the weights again each time.
 template <int R>
 __global__ __launch_bounds__(kSelectThreads) void sqa_select_kernel(EvictArgs a) {
   __shared__ int hist[2048];
@@ -455,33 +456,37 @@ __global__ __launch_bounds__(kSelectThreads) void sqa_select_kernel(EvictArgs a)
   }
   // A wave's run: `steps` times 64 consecutive tokens.
   const int steps = (n + kSelectThreads - 1) / kSelectThreads;
-  const int begin = min(wave * steps * 64, n);
+  const int begin = wave * steps * 64;
+  const int lo = a.sink, hi = n - a.recent;
+  auto key_at = [&](int t, float x) {
+    const unsigned k = t >= lo && t < hi ? weight_key(x) : kAlways;
+    return t < n ? k : 0u;
+  };
   constexpr int kHeld = R > 0 ? R : 1;
-  float held[kHeld];
+  float held_w[kHeld];
+  unsigned held[kHeld];
   if constexpr (R > 0) {
 #pragma unroll
-    for (int i = 0; i < R; ++i) {
-      const int t = begin + 64 * i + lane;
-      held[i] = i < steps ? w[min(t, n - 1)] : 0.f;
-    }
+    for (int i = 0; i < R; ++i) held_w[i] = i < steps ? w[min(begin + 64 * i + lane, n - 1)] : 0.f;
+#pragma unroll
+    for (int i = 0; i < R; ++i) held[i] = key_at(begin + 64 * i + lane, held_w[i]);
   }
-  // each(f): f(token, weight) for the thread's tokens of the run in order.
+  // each(f): f(token, key, weight) for the thread's tokens of the run in order.
   auto each = [&](auto f) {
     if constexpr (R > 0) {
 #pragma unroll
       for (int i = 0; i < R; ++i)
-        if (i < steps) f(begin + 64 * i + lane, held[i]);  // uniform
+        if (i < steps) f(begin + 64 * i + lane, held[i], held_w[i]);  // uniform
     } else {
       for (int i = 0; i < steps; ++i) {
         const int t = begin + 64 * i + lane;
-        f(t, w[min(t, n - 1)]);
+        const float x = w[min(t, n - 1)];
+        f(t, key_at(t, x), x);
       }
     }
   };
-  const int end = min(begin + steps * 64, n);
-  const int lo = a.sink, hi = n - a.recent;
   const int free = a.budget - a.sink - a.recent;
-  unsigned threshold = 0xffffffffu;  // no key: those of all weights lie below
+  unsigned threshold = kAlways - 1;  // above the keys of all weights
   int ties = 0;                      // how many of the tokens at the threshold stay
   if (free > 0) {
     int want = free;
@@ -491,9 +496,8 @@ __global__ __launch_bounds__(kSelectThreads) void sqa_select_kernel(EvictArgs a)
       const unsigned digits = pass == 2 ? 0x3ffu : 0x7ffu;
       for (int i = tid; i < 2048; i += kSelectThreads) hist[i] = 0;
       __syncthreads();
-      each([&](int t, float x) {
-        const unsigned k = weight_key(x);
-        if (t >= lo && t < min(hi, end) && (k & mask) == prefix)
+      each([&](int, unsigned k, float) {
+        if (k - 1u < kAlways - 1u && (k & mask) == prefix)
           atomicAdd(&hist[(k >> shift) & digits], 1);
       });
       __syncthreads();
@@ -503,7 +507,8 @@ __global__ __launch_bounds__(kSelectThreads) void sqa_select_kernel(EvictArgs a)
       if (lane == 63) wave_tot[wave] = incl;
       __syncthreads();
       int before = incl - c0 - c1;
-      for (int i = 0; i < wave; ++i) before += wave_tot[i];
+#pragma unroll
+      for (int i = 0; i < kSelectWaves; ++i) before += i < wave ? wave_tot[i] : 0;
       if (before < want && want <= before + c0 + c1) {  // one thread
         const bool first = want <= before + c0;
         picked = first ? 2047 - 2 * tid : 2046 - 2 * tid;
@@ -517,19 +522,10 @@ __global__ __launch_bounds__(kSelectThreads) void sqa_select_kernel(EvictArgs a)
     threshold = prefix;
     ties = want;
   }
-  auto look = [&](int t, float x, bool& sure, bool& tie) {
-    const bool in = t < end;
-    const bool always = in && (t < lo || t >= hi);
-    const unsigned k = weight_key(x);
-    sure = always || (in && k > threshold);
-    tie = in && !always && ties > 0 && k == threshold;
-  };
   int sures = 0, tied = 0;
-  each([&](int t, float x) {
-    bool sure, tie;
-    look(t, x, sure, tie);
-    sures += __popcll(__ballot(sure));
-    tied += __popcll(__ballot(tie));
+  each([&](int, unsigned k, float) {
+    sures += __popcll(__ballot(k > threshold));
+    tied += __popcll(__ballot(k == threshold));
   });
   if (lane == 0) {
     wave_sure[wave] = sures;
@@ -537,20 +533,24 @@ __global__ __launch_bounds__(kSelectThreads) void sqa_select_kernel(EvictArgs a)
   }
   __syncthreads();
   int at = 0, seen = 0;  // kept tokens and ties before this wave's
-  for (int i = 0; i < wave; ++i) {
-    at += wave_sure[i];
-    seen += wave_tie[i];
+#pragma unroll
+  for (int i = 0; i < kSelectWaves; ++i) {
+    at += i < wave ? wave_sure[i] : 0;
+    seen += i < wave ? wave_tie[i] : 0;
   }
-  at += min(seen, ties);
-  const unsigned long long below = lane ? ~0ull >> (64 - lane) : 0ull;
-  each([&](int t, float x) {
-    bool sure, tie;
-    look(t, x, sure, tie);
-    const unsigned long long tie_mask = __ballot(tie);
-    const bool keep = sure || (tie && seen + __popcll(tie_mask & below) < ties);
+  at = __builtin_amdgcn_readfirstlane(at + min(seen, ties));
+  seen = __builtin_amdgcn_readfirstlane(seen);
+  auto below = [](unsigned long long mask) {  // its bits under the lane's
+    return (int)__builtin_amdgcn_mbcnt_hi((unsigned)(mask >> 32),
+                                          __builtin_amdgcn_mbcnt_lo((unsigned)mask, 0));
+  };
+  each([&](int t, unsigned k, float x) {
+    bool keep = k > threshold;
+    const unsigned long long tie_mask = __ballot(k == threshold);
+    if (tie_mask && seen < ties) keep |= k == threshold && seen + below(tie_mask) < ties;  // uniform
     const unsigned long long keep_mask = __ballot(keep);
     if (keep) {
-      const int to = at + __popcll(keep_mask & below);
+      const int to = at + below(keep_mask);
       kept[to] = t;
       if constexpr (R > 0) nw[to] = x;  // every weight has been read: nw may be w
     }
@@ -745,8 +745,8 @@ hipError_t launch_evict(const EvictArgs& a, hipStream_t stream) {
     hipLaunchKernelGGL((sqa_select_kernel<4>), each, threads, 0, stream, a);
   else if (most <= 16 * kSelectThreads)
     hipLaunchKernelGGL((sqa_select_kernel<16>), each, threads, 0, stream, a);
-  else if (most <= 40 * kSelectThreads)
-    hipLaunchKernelGGL((sqa_select_kernel<40>), each, threads, 0, stream, a);
+  else if (most <= 32 * kSelectThreads)
+    hipLaunchKernelGGL((sqa_select_kernel<32>), each, threads, 0, stream, a);
   else
     hipLaunchKernelGGL((sqa_select_kernel<0>), each, threads, 0, stream, a);
   const hipError_t e = hipGetLastError();

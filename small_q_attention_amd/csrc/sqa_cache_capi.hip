@@ -193,7 +193,7 @@ int sqa_paged_attention_scaled(const sqa_attention_args* args, const sqa_block_s
   if ((uintptr_t)a.workspace % 16)
     return fail(SQA_ERR_WORKSPACE, "workspace must be 16-byte aligned");
   const unsigned long long items = (unsigned long long)a.num_splits * a.num_kv_heads * rows;
-  const unsigned long long part_bytes = items * a.head_dim * (a.dtype == SQA_DTYPE_F16 ? 2 : 4);
+  const unsigned long long part_bytes = items * a.head_dim * 4;
   if (part_bytes > sqa::kMaxPartialBytes)
     return fail(SQA_ERR_INVALID, "the plan's partials (%llu bytes) exceed %llu bytes", part_bytes,
                 sqa::kMaxPartialBytes);
@@ -270,7 +270,7 @@ int sqa_paged_attention_scaled(const sqa_attention_args* args, const sqa_block_s
     m.by_group = p.by_group;
     m.by_spec_pps = m.by_spec_pps1 = sqa::fast_div(1);
     m.out_scale = a.out_scale;
-    m.bf16 = p.bf16;
+    m.bf16 = p.bf16 ? 1 : 2;  // fp32 partial rows for both
     if ((e = sqa::launch_merge(m, cus, stream)) != hipSuccess)
       return hip_fail(e, "merge kernel launch");
   }

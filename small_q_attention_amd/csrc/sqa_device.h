@@ -77,6 +77,11 @@ struct ElemF16 {
   }
 };
 
+// fp16 queries and outputs whose split partials stay unnormalised fp32.
+struct ElemF16Wide : ElemF16 {
+  static constexpr bool kHalfPartials = false;
+};
+
 struct ElemBF16 {
   // bf16 V can exceed fp16's range and bf16's 8 bits would cost accuracy:
   // partials stay unnormalised fp32.

@@ -217,7 +217,7 @@ struct MergeArgs {
   int hg_items[2];  // as PartialArgs::hg_items
   int hg_spec_pps1; // as PartialArgs::hg_spec_pps1
   float out_scale;
-  int bf16;
+  int bf16;         // element type of out: 0 fp16, 1 bf16, 2 fp16 with fp32 partial rows
   FastDiv by_hq, by_seq_rows, by_group;  // hq, q_len * hq (a sequence's rows), group
   FastDiv by_spec_pps, by_spec_pps1;     // spec_pps, hg_spec_pps1 (where they are > 0)
   float* tune;      // adaptive paired items: the delta record to update (null: none)

@@ -1259,7 +1259,9 @@ void launch_partial_plan(const PartialArgs& a, const LaunchShape& sh, dim3 grid,
 
 template <bool BAL>
 void launch_merge_plan(const MergeArgs& a, int per_row, int cus, hipStream_t stream) {
-  if (a.bf16)
+  if (BAL && a.bf16 == 2)
+    launch_merge_as<ElemF16Wide, true>(a, per_row, cus, stream);
+  else if (a.bf16)
     launch_merge_as<ElemBF16, BAL>(a, per_row, cus, stream);
   else
     launch_merge_as<ElemF16, BAL>(a, per_row, cus, stream);

@@ -19,7 +19,7 @@ namespace {
 // ---------------------------------------------------------------------------------
 
 // V of a page as the PV product's A operand: av[mb] = this lane's dim mb of its four
-// tokens in bf16. bf16 holds every e4m3 value and every integer up to 256 exactly.
+// tokens in fp16, which holds every e4m3 value and every 8-bit integer exactly.
 template <int HD>
 struct CodesFp8 : KvFp8<HD> {
   using Regs = typename KvFp8<HD>::Regs;
@@ -35,7 +35,7 @@ struct CodesFp8 : KvFp8<HD> {
         const unsigned sel = half ? 0x07030602u : 0x05010400u;
         const unsigned t01 = __builtin_amdgcn_perm(r.v[1][i], r.v[0][i], sel);
         const unsigned t23 = __builtin_amdgcn_perm(r.v[3][i], r.v[2][i], sel);
-        const u2 a = ElemBF16::widen_fp8x4(t01), b = ElemBF16::widen_fp8x4(t23);
+        const u2 a = ElemF16::widen_fp8x4(t01), b = ElemF16::widen_fp8x4(t23);
         av[4 * i + 2 * half] = u2{a[0], b[0]};
         av[4 * i + 2 * half + 1] = u2{a[1], b[1]};
       }
@@ -67,21 +67,34 @@ struct CodesInt8 : KvFp8<HD> {
 #pragma unroll
     for (int mb = 0; mb < MB; ++mb) {
       const int i = mb / 4, e = mb % 4;
-      av[mb] = u2{ElemBF16::pack2(byte(r.v[0][i], e), byte(r.v[1][i], e)),
-                  ElemBF16::pack2(byte(r.v[2][i], e), byte(r.v[3][i], e))};
+      av[mb] = u2{ElemF16::pack2(byte(r.v[0][i], e), byte(r.v[1][i], e)),
+                  ElemF16::pack2(byte(r.v[2][i], e), byte(r.v[3][i], e))};
     }
   }
 };
 
-// Raw scores of a page, K code . Q^T.
+// Partial rows are fp32 for both types of queries: fp16 ones, as the 16-bit kernels leave,
+// added a rounding of the size of the output's own (error against 64 bits 1.45 times that
+// of a rounded 32-bit result; so 1.1 times). TODO cost
+template <typename E>
+using PartialRows = std::conditional_t<E::kHalfPartials, ElemF16Wide, E>;
+
+// Raw scores of a page, K code . Q^T. Where Q does not fit the vector registers beside
+// the accumulators (64 rows, head dim 256) it lives in accumulation registers, which the
+// MFMAs read as they are; the empty asm says so, or the compiler copies it over for every
+// page.
 template <int NB, int HD, typename E, typename KV>
 __device__ __forceinline__ void code_scores(f4 (&s)[NB], const typename KV::Regs& r,
-                                            const u4 (&q)[NB][Dims<HD>::KK]) {
+                                            u4 (&q)[NB][Dims<HD>::KK]) {
   constexpr int KK = Dims<HD>::KK;
   u4 k[KK];
   KV::template expand_k<E>(r, k);
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) {
+    if constexpr (NB * HD >= 512) {
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) asm volatile("" : "+a"(q[nb][kk]));
+    }
     s[nb] = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int kk = 0; kk < KK; ++kk) s[nb] = E::mma_qk(k[kk], q[nb][kk], s[nb]);
@@ -114,13 +127,13 @@ __device__ __forceinline__ void nan_values(WaveState<NB, HD>& st, typename KV::R
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) {
     float seen[4], sum = 0.f;
-    u2 lo;
+    u2 none;
 #pragma unroll
     for (int e = 0; e < 4; ++e) seen[e] = s[nb][e] == -INFINITY ? 0.f : 1.f;
-    const u2 hi = ElemBF16::round_p(seen[0], seen[1], seen[2], seen[3], sum, lo);
+    const u2 rows = ElemF16::round_p(seen[0], seen[1], seen[2], seen[3], sum, none);
 #pragma unroll
     for (int mb = 0; mb < MB; ++mb) {
-      const f4 hits = ElemBF16::mma_pv(av[mb], hi, lo, f4{0.f, 0.f, 0.f, 0.f});
+      const f4 hits = ElemF16::mma_pv(av[mb], rows, none, f4{0.f, 0.f, 0.f, 0.f});
 #pragma unroll
       for (int e = 0; e < 4; ++e)
         st.acc[mb][nb][e] = hits[e] > 0.f ? __builtin_nanf("") : st.acc[mb][nb][e];
@@ -131,11 +144,17 @@ __device__ __forceinline__ void nan_values(WaveState<NB, HD>& st, typename KV::R
 // One workgroup = four waves on their own: wave w serves kv head w % wg_heads of the
 // workgroup's heads and work item w / wg_heads of its items, with all query rows of the
 // head (NB blocks of 16). A wave keeps a ring of D pages of codes and their two scales in
-// flight in registers. No barrier: waves of a workgroup meet only in the memory system, where the
-// heads' slices of a token row are neighbours.
-// P enters the PV product as two bf16 parts of p * v_scale (together within 2^-17 of it,
-// at the cost of one product, as in the bf16 kernels): fp16 would lose the small scales
-// of quiet blocks. The row sums take p itself.
+// flight in registers. No barrier: waves of a workgroup meet only in the memory system,
+// where the heads' slices of a token row are neighbours.
+//
+// The V scale of a page enters the exponent: P = 2^(c s + log2 v_scale - m), with m the
+// running maximum of exactly that, is what the page's codes weigh in the sums O, so one
+// fp16 rounding of P is relative to its part of the result (2^-11 of it, and 2^-25 of the
+// row's largest part where it is tiny beside that), however the blocks' scales differ; two
+// bf16 parts of p * v_scale cost 28 operations a page more at 32 rows (16 x 32K keys,
+// whole calls: q_len 8 201 -> 178 us, q_len 16 293 -> 245). The row sum gets P / v_scale in
+// fp32, unrounded: a quiet block's tokens weigh as much in it as a loud one's. Pages of a
+// scale under 2^-100 add to the row sums only.
 template <int NB, int D, int HD, typename E, typename KV, bool PIPE>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1)))
 void sqa_scaled_attention_kernel(ScaledArgs args) {
@@ -149,6 +168,7 @@ void sqa_scaled_attention_kernel(ScaledArgs args) {
   const int head_groups = (a.hkv + wgh - 1) / wgh;
   const int kvh = (blockIdx.x % head_groups) * wgh + wave % wgh;
   const int item = (blockIdx.x / head_groups) * (4 / wgh) + wave / wgh;
+  const WaveRows<NB, 1> map{kvh, a.rows, a.hkv};
   if (kvh >= a.hkv) return;
 
   Split it;
@@ -176,7 +196,6 @@ void sqa_scaled_attention_kernel(ScaledArgs args) {
   load_ids(0, first_ids);
   load_ids(D, ids);
 
-  const WaveRows<NB, 1> map{kvh, a.rows, a.hkv};
   u4 q[NB][KK];
   RegBits<NB> bits;
 #pragma unroll
@@ -245,7 +264,10 @@ void sqa_scaled_attention_kernel(ScaledArgs args) {
             float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, ring[j].scale), 0));
         const float vs = __builtin_bit_cast(
             float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, ring[j].scale), 32));
-        float c = a.scale_log2 * ks;
+        const bool loud = !(vs < 0x1p-100f);
+        const float lv = loud ? __builtin_amdgcn_logf(vs) : 0.f;
+        const float inv_vs = loud ? __builtin_amdgcn_rcpf(vs) : 1.f;
+        float c = a.scale_log2 * ks, add = lv;
         f4 s[NB];
         if constexpr (PIPE) {
 #pragma unroll
@@ -256,10 +278,11 @@ void sqa_scaled_attention_kernel(ScaledArgs args) {
         }
         const bool masked = (p + 1) * kPageSize > mask_from;  // uniform
         if (masked) {
-          // After the scale, so that a scale of 0, infinity or NaN leaves them -inf.
+          // After the scales, so that one of 0, infinity or NaN leaves them -inf.
 #pragma unroll
-          for (int nb = 0; nb < NB; ++nb) s[nb] *= c;
+          for (int nb = 0; nb < NB; ++nb) s[nb] = s[nb] * c + lv;
           c = 1.f;
+          add = 0.f;
           const int tok0 = p * kPageSize + 4 * g16;
           mask_scores<NB>(s, bits.b, mask_from, tok0, len);
 #pragma unroll
@@ -267,44 +290,43 @@ void sqa_scaled_attention_kernel(ScaledArgs args) {
             if (tok0 + e >= len)
 #pragma unroll
               for (int w = 0; w < Dims<HD>::VW / 2; ++w) ring[j].kv.v[e][w] = 0u;
+          if constexpr (KV::kNan) nan_values<NB, HD, KV>(st, ring[j].kv, s);
         }
         float lm[NB];
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb) lm[nb] = max4(s[nb]) * c;
+        for (int nb = 0; nb < NB; ++nb) lm[nb] = fmaf(max4(s[nb]), c, add);
         raise_max<NB, HD>(st, lm);
-        if constexpr (KV::kNan)
-          if (masked) nan_values<NB, HD, KV>(st, ring[j].kv, s);
-        u2 hi[NB], lo[NB];
+        u2 ph[NB];
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
-          const float mu = st.m[nb] == -INFINITY ? 0.f : st.m[nb];
-          float pr[4], pv[4], sum = 0.f;
+          const float off = add - (st.m[nb] == -INFINITY ? 0.f : st.m[nb]);
+          float pr[4], rounded = 0.f;
+          u2 none;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            pr[e] = fast_exp2(fmaf(s[nb][e], c, -mu));
-            pv[e] = pr[e] * vs;
-          }
-          st.l[nb] += (pr[0] + pr[1]) + (pr[2] + pr[3]);
-          if (masked) {  // a scale that is not finite stays with the tokens that are seen
-#pragma unroll
-            for (int e = 0; e < 4; ++e) pv[e] = pr[e] == 0.f ? 0.f : pv[e];
-          }
-          hi[nb] = ElemBF16::round_p(pv[0], pv[1], pv[2], pv[3], sum, lo[nb]);
+          for (int e = 0; e < 4; ++e) pr[e] = fast_exp2(fmaf(s[nb][e], c, off));
+          const float sum = (pr[0] + pr[1]) + (pr[2] + pr[3]);
+          // A V scale that is not finite stays with the rows that see its page.
+          const float l = fmaf(sum, inv_vs, st.l[nb]);
+          st.l[nb] = masked && sum == 0.f ? st.l[nb] : l;
+          ph[nb] = ElemF16::round_p(pr[0], pr[1], pr[2], pr[3], rounded, none);
         }
-        u2 av[MB];
-        KV::operand_v(ring[j].kv, av);
+        if (loud) {  // uniform
+          const u2 none = {0u, 0u};
+          u2 av[MB];
+          KV::operand_v(ring[j].kv, av);
 #pragma unroll
-        for (int mb = 0; mb < MB; ++mb)
+          for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
-          for (int nb = 0; nb < NB; ++nb)
-            st.acc[mb][nb] = ElemBF16::mma_pv(av[mb], hi[nb], lo[nb], st.acc[mb][nb]);
+            for (int nb = 0; nb < NB; ++nb)
+              st.acc[mb][nb] = ElemF16::mma_pv(av[mb], ph[nb], none, st.acc[mb][nb]);
+        }
       }
       load_page(ii + D < n_pages ? clamp_page(ids[j], a.num_pages) : -1, p_begin + ii + D, ring[j]);
     }
 #pragma unroll
     for (int j = 0; j < D; ++j) ids[j] = ids_next[j];
   }
-  write_results<NB, HD, E>(a, st, sm_stage + wave * 16 * (HD + 4), map, it.count <= 1, false, b,
+  write_results<NB, HD, PartialRows<E>>(a, st, sm_stage + wave * 16 * (HD + 4), map, it.count <= 1, false, b,
                            (size_t)it.slot, a.hkv, 0);
 }
 
@@ -475,31 +497,32 @@ void launch_append_as(const AppendArgs& a, dim3 grid, hipStream_t stream) {
     launch_append_hd<256, BF16, INT8>(a, grid, stream);
 }
 
-constexpr bool PIPE1 = false, PIPE2 = true, PIPE4 = false;
+// Ring depths: as many pages in flight as hold about 16 KiB of codes per wave; half of
+// that at 64 rows, whose accumulators take the registers. Two blocks issue a page's scores
+// under the page before (one block has little softmax to hide).
+template <int HD, typename E, typename KV>
+void launch_scaled_hd(const ScaledArgs& a, dim3 grid, hipStream_t stream) {
+  constexpr int D = 4 * 128 / HD;
+  const dim3 block(256);
+  if (a.p.rows <= 16)
+    hipLaunchKernelGGL((sqa_scaled_attention_kernel<1, D, HD, E, KV, false>), grid, block, 0,
+                       stream, a);
+  else if (a.p.rows <= 32)
+    hipLaunchKernelGGL((sqa_scaled_attention_kernel<2, D, HD, E, KV, HD != 256>), grid, block, 0,
+                       stream, a);
+  else if constexpr (HD != 256)
+    hipLaunchKernelGGL((sqa_scaled_attention_kernel<4, D / 2, HD, E, KV, false>), grid, block, 0,
+                       stream, a);
+}
+
 template <typename E, template <int> class KV>
 void launch_scaled_as(const ScaledArgs& a, dim3 grid, hipStream_t stream) {
-  const dim3 block(256);
-  const int rows = a.p.rows;
-  if (a.p.head_dim == 64) {
-    if (rows <= 16)
-      hipLaunchKernelGGL((sqa_scaled_attention_kernel<1, 8, 64, E, KV<64>, PIPE1>), grid, block, 0, stream, a);
-    else if (rows <= 32)
-      hipLaunchKernelGGL((sqa_scaled_attention_kernel<2, 8, 64, E, KV<64>, PIPE2>), grid, block, 0, stream, a);
-    else
-      hipLaunchKernelGGL((sqa_scaled_attention_kernel<4, 4, 64, E, KV<64>, PIPE4>), grid, block, 0, stream, a);
-  } else if (a.p.head_dim == 128) {
-    if (rows <= 16)
-      hipLaunchKernelGGL((sqa_scaled_attention_kernel<1, 4, 128, E, KV<128>, PIPE1>), grid, block, 0, stream, a);
-    else if (rows <= 32)
-      hipLaunchKernelGGL((sqa_scaled_attention_kernel<2, 4, 128, E, KV<128>, PIPE2>), grid, block, 0, stream, a);
-    else
-      hipLaunchKernelGGL((sqa_scaled_attention_kernel<4, 4, 128, E, KV<128>, PIPE4>), grid, block, 0, stream, a);
-  } else {
-    if (rows <= 16)
-      hipLaunchKernelGGL((sqa_scaled_attention_kernel<1, 2, 256, E, KV<256>, PIPE1>), grid, block, 0, stream, a);
-    else
-      hipLaunchKernelGGL((sqa_scaled_attention_kernel<2, 2, 256, E, KV<256>, PIPE2>), grid, block, 0, stream, a);
-  }
+  if (a.p.head_dim == 64)
+    launch_scaled_hd<64, E, KV<64>>(a, grid, stream);
+  else if (a.p.head_dim == 128)
+    launch_scaled_hd<128, E, KV<128>>(a, grid, stream);
+  else
+    launch_scaled_hd<256, E, KV<256>>(a, grid, stream);
 }
 
 }  // namespace

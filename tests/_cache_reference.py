@@ -89,10 +89,18 @@ def attention(q, k, v, k_scale, v_scale, tables, lens, trees=None, scale=None, o
             vv = vs[:, h // group]
             out[i, :, h] = out_scale * _product(p, vv, seen)
             size = abs(out_scale) * _product(p, vv.abs(), seen)
-            # P in two bf16 parts, its fp32 sums, the scores' errors (twice: numerator
-            # and denominator), fp16 partial rows, the output's rounding.
-            bound[i, :, h] = size * (2.0 ** -16 + n * 2.0 ** -23 + 2 * delta[:, None]) \
-                + (2.0 ** -11 * size if q.dtype is torch.float16 else 0.0) \
+            # P = p v_scale, rounded once to fp16 for the product with the codes: off by
+            # 2^-11 of itself, or, below 2^-14, by 2^-25. It is taken relative to a maximum
+            # no larger than the row's largest p v_scale, call it p* s*: in those units the
+            # row sum is at least 1 / s*, so the n roundings of 2^-25, each times a code,
+            # leave at most n 2^-25 (largest code) s* in the quotient. Then fp32 sums, the
+            # scores' errors (twice: numerator and denominator), the output's rounding.
+            loudest = vs.new_zeros(())
+            if v_scale is not None:
+                pages = tables[i, :-(-n // v.shape[1])].long()
+                loudest = CODE_MAX[v.dtype] * v_scale[pages, h // group].double().nan_to_num().max()
+            bound[i, :, h] = size * (2.0 ** -11 + n * 2.0 ** -23 + 2 * delta[:, None]) \
+                + abs(out_scale) * n * 2.0 ** -25 * loudest \
                 + half_step(q.dtype) * out[i, :, h].abs() * 1.01 + 2.0 ** -24
     return out, bound, mass
 

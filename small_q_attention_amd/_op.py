@@ -142,3 +142,31 @@ def accumulate_attention_weights(query: torch.Tensor, key_cache: torch.Tensor,
 def _accumulate_attention_weights_fake(query, key_cache, key_scale, block_tables, seq_lens,
                                        draft_mask, weights, scale, max_seq_len):
     return None
+
+
+@torch.library.custom_op("sqa::evict_by_weight",
+                         mutates_args=("new_key_cache", "new_value_cache", "new_key_scale",
+                                       "new_value_scale", "new_weights", "new_lens", "kept"))
+def evict_by_weight(weights: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor,
+                    key_scale: Optional[torch.Tensor], value_scale: Optional[torch.Tensor],
+                    block_tables: torch.Tensor, seq_lens: torch.Tensor,
+                    new_block_tables: torch.Tensor, new_key_cache: torch.Tensor,
+                    new_value_cache: torch.Tensor, new_key_scale: Optional[torch.Tensor],
+                    new_value_scale: Optional[torch.Tensor], new_weights: torch.Tensor,
+                    new_lens: torch.Tensor, kept: torch.Tensor, budget: int, sink: int,
+                    recent: int) -> None:
+    """Eviction by accumulated weight (``eviction.evict_by_weight``), into buffers."""
+    from . import eviction, scaled_cache
+
+    scaled_cache.on_device(weights.device, eviction.launch_evict, weights, new_weights, kept,
+                           seq_lens, new_lens, (key_cache, value_cache, key_scale, value_scale),
+                           (new_key_cache, new_value_cache, new_key_scale, new_value_scale),
+                           block_tables, new_block_tables, budget, sink, recent)
+
+
+@evict_by_weight.register_fake
+def _evict_by_weight_fake(weights, key_cache, value_cache, key_scale, value_scale, block_tables,
+                          seq_lens, new_block_tables, new_key_cache, new_value_cache,
+                          new_key_scale, new_value_scale, new_weights, new_lens, kept, budget,
+                          sink, recent):
+    return None

@@ -175,6 +175,29 @@ def _run(query, k, v, block_tables, seq_lens, max_seq_len: int, q_len: int, scal
     return out
 
 
+def _run_scaled(query, k, v, scales, block_tables, seq_lens, max_seq_len: int, q_len: int,
+                scale: float, out_scale: float, mask, workspace_buffer, out):
+    """:func:`_run` over a cache with block scales (``scaled_cache``)."""
+    from . import scaled_cache
+
+    if len(scales) != 2:
+        raise ValueError("kv_block_scales is a (key_scale, value_scale) pair")
+    if query.dim() != 3 or not query.is_contiguous():
+        raise ValueError("query must be a contiguous [B * Q, Hq, D] tensor")
+    batch = block_tables.shape[0] if block_tables.dim() == 2 else 0
+    if q_len < 1 or batch == 0 or query.shape[0] != batch * q_len:
+        raise ValueError(f"query holds {query.shape[0]} rows, expected batch {batch} x "
+                         f"q_len_per_req {q_len}")
+    shape = (batch, q_len, *query.shape[1:])
+    if out is not None and (out.shape != query.shape or not out.is_contiguous()):
+        raise ValueError("out must be a contiguous tensor shaped and typed like query")
+    res = scaled_cache.paged_attention_scaled(
+        query.view(shape), k, v, scales[0], scales[1], block_tables, seq_lens,
+        max_seq_len=max_seq_len, scale=scale, out_scale=out_scale, mask=mask,
+        out=None if out is None else out.view(shape), workspace_buffer=workspace_buffer)
+    return res.view(query.shape) if out is None else out
+
+
 def _scalar(x, name):
     if hasattr(x, "item"):
         if x.numel() != 1:
@@ -186,7 +209,7 @@ def _scalar(x, name):
 def xqa_batch_decode_with_kv_cache(query, kv_cache, workspace_buffer, block_tables, seq_lens,
                                    max_seq_len, bmm1_scale, bmm2_scale, window_left=-1,
                                    out=None, sinks=None, kv_layout="NHD", enable_pdl=None,
-                                   q_len_per_req=1, mask=None):
+                                   q_len_per_req=1, mask=None, kv_block_scales=None):
     """Paged decode of ``q_len_per_req`` draft tokens per request.
 
     Call shape of ``flashinfer.decode.xqa_batch_decode_with_kv_cache`` as the
@@ -194,12 +217,20 @@ def xqa_batch_decode_with_kv_cache(query, kv_cache, workspace_buffer, block_tabl
     the softmax scale, ``bmm2_scale`` multiplies the output; ``mask`` is the packed
     draft mask (``None``: causal draft chain). ``max_seq_len`` bounds every
     ``seq_lens[b]``. Returns ``out`` (``[B * Q, Hq, D]``).
+
+    ``kv_block_scales``: ``(key_scale, value_scale)``, float32 ``[P, Hkv]`` each, of a cache of
+    ``torch.float8_e4m3fn`` or ``torch.int8`` with a scale for each page and kv head
+    (:mod:`small_q_attention_amd.scaled_cache`); ``max_seq_len`` then only sizes the call.
     """
     if window_left not in (-1, None):
         raise ValueError("sliding windows are not supported (window_left must be -1)")
     if sinks is not None:
         raise ValueError("attention sinks are not supported")
     k, v = _kv_views(kv_cache, kv_layout)
+    if kv_block_scales is not None:
+        return _run_scaled(query, k, v, kv_block_scales, block_tables, seq_lens, int(max_seq_len),
+                           int(q_len_per_req), _scalar(bmm1_scale, "bmm1_scale"),
+                           _scalar(bmm2_scale, "bmm2_scale"), mask, workspace_buffer, out)
     _check_tensors(query, k, v)
     return _run(query, k, v, block_tables, seq_lens, int(max_seq_len), int(q_len_per_req),
                 _scalar(bmm1_scale, "bmm1_scale"), _scalar(bmm2_scale, "bmm2_scale"), mask,
@@ -209,7 +240,7 @@ def xqa_batch_decode_with_kv_cache(query, kv_cache, workspace_buffer, block_tabl
 def trtllm_batch_decode_with_kv_cache(query, kv_cache, workspace_buffer, block_tables, seq_lens,
                                       max_seq_len, bmm1_scale, bmm2_scale, window_left=-1,
                                       out=None, sinks=None, kv_layout="HND", enable_pdl=None,
-                                      q_len_per_req=1, mask=None):
+                                      q_len_per_req=1, mask=None, kv_block_scales=None):
     """Call shape of ``flashinfer.decode.trtllm_batch_decode_with_kv_cache``
     (``run_flashinfer_baseline.py:180-204``): as :func:`xqa_batch_decode_with_kv_cache`
     with the "HND" cache layout by default."""
@@ -217,7 +248,7 @@ def trtllm_batch_decode_with_kv_cache(query, kv_cache, workspace_buffer, block_t
                                           seq_lens, max_seq_len, bmm1_scale, bmm2_scale,
                                           window_left, out=out, sinks=sinks, kv_layout=kv_layout,
                                           enable_pdl=enable_pdl, q_len_per_req=q_len_per_req,
-                                          mask=mask)
+                                          mask=mask, kv_block_scales=kv_block_scales)
 
 
 def csr_to_block_table(indptr, indices, last_page_len, page_size: int = PAGE_SIZE):
@@ -306,7 +337,8 @@ class _PagedWrapper:
             raise ValueError("logits soft capping is not supported")
         ok = (None, torch.float16, "float16", "fp16", torch.bfloat16, "bfloat16", "bf16")
         fp8 = (getattr(torch, "float8_e4m3fn", None), "float8_e4m3fn", "e4m3")
-        if q_data_type not in ok or kv_data_type not in ok + fp8:
+        int8 = (torch.int8, "int8")  # with block scales, given to run()
+        if q_data_type not in ok or kv_data_type not in ok + fp8 + int8:
             raise ValueError("this build supports fp16 or bf16 query and KV "
                              "(KV also float8_e4m3fn)")
         if head_dim not in HEAD_DIMS or page_size not in PAGE_SIZES:
@@ -375,11 +407,13 @@ class _PagedWrapper:
         return g["block_tables"], g["seq_lens"], g["mask"], g["plan"]
 
     def run(self, q, paged_kv_cache, *args, q_scale=None, k_scale=None, v_scale=None, out=None,
-            lse=None, return_lse=False, enable_pdl=None, window_left=None, sinks=None, **kwargs):
+            lse=None, return_lse=False, enable_pdl=None, window_left=None, sinks=None,
+            kv_block_scales=None, **kwargs):
         """FlashInfer's ``run`` keywords: ``q_scale`` and ``k_scale`` multiply the softmax
         scale, ``v_scale`` the output (per-tensor FP8 scales); ``enable_pdl`` is a
         launch hint and has no effect here. ``lse``/``return_lse``, sliding windows,
-        sinks, extra positional arguments and unknown keywords raise ``ValueError``."""
+        sinks, extra positional arguments and unknown keywords raise ``ValueError``.
+        ``kv_block_scales``: as for :func:`xqa_batch_decode_with_kv_cache`."""
         if args:
             raise ValueError("run() takes (q, paged_kv_cache) positionally; pass the rest "
                              "by keyword")
@@ -400,7 +434,10 @@ class _PagedWrapper:
                 scale *= _scalar(x, name)
         out_scale = 1.0 if v_scale is None else _scalar(v_scale, "v_scale")
         k, v = _kv_views(paged_kv_cache, self._kv_layout)
-        _check_tensors(q, k, v, p["hq"])
+        if kv_block_scales is None:
+            _check_tensors(q, k, v, p["hq"])
+        elif q.dim() != 3 or q.shape[1] != p["hq"]:
+            raise ValueError(f"q must be [B * Q, {p['hq']}, D], as plan() was given")
         if k.shape[2] != p["hkv"]:
             raise ValueError(f"kv_cache has {k.shape[2]} kv heads, plan() was given {p['hkv']}")
         if q.shape[-1] != p["head_dim"]:
@@ -409,6 +446,10 @@ class _PagedWrapper:
         if k.shape[1] != p["page_size"]:
             raise ValueError(f"kv_cache pages hold {k.shape[1]} tokens, plan() was given "
                              f"{p['page_size']}")
+        if kv_block_scales is not None:
+            return _run_scaled(q, k, v, kv_block_scales, p["block_tables"], p["seq_lens"],
+                               p["max_seq_len"], p["q_len"], scale, out_scale, p["mask_words"],
+                               self._workspace, out)
         return _run(q, k, v, p["block_tables"], p["seq_lens"], p["max_seq_len"], p["q_len"],
                     scale, out_scale, p["mask_words"], self._workspace, out, plan=p["plan"])
 

@@ -30,6 +30,7 @@ def _check_weights(weights, batch, hkv, what="weights"):
             or weights.shape[1] != hkv or weights.shape[2] == 0 or weights.stride(2) != 1:
         raise ValueError(f"{what} must be float32 [{batch}, {hkv}, tokens] with a contiguous last "
                          "dimension")
+    sc.check_distinct(weights, what)
 
 
 def _check_scaled(cache, *scales):
@@ -119,18 +120,12 @@ def accumulate_attention_weights(query, key_cache, block_tables, seq_lens, weigh
     return weights
 
 
-def run_evict(weights, new_weights, source, block_tables, seq_lens, into, new_tables, budget, sink,
-              recent, fields=None):
-    """Allocate what a checked call returns and launch it."""
-    batch, hkv, _ = weights.shape
-    device = weights.device
-    kept = torch.empty((batch, hkv, budget), dtype=torch.int32, device=device)
-    new_lens = torch.empty_like(seq_lens)
-    if new_weights is None:
-        new_weights = torch.empty((batch, hkv, budget), dtype=torch.float32, device=device)
+def launch_evict(weights, new_weights, kept, seq_lens, new_lens, source, into, block_tables,
+                 new_tables, budget, sink, recent, fields=None):
+    """Launch a checked call on the current stream."""
     _lib.launch_evict(weights, new_weights, kept, seq_lens, new_lens, source, into, block_tables,
-                      new_tables, budget, sink, recent, _lib.raw_stream(device.index), fields)
-    return new_lens, new_weights, kept
+                      new_tables, budget, sink, recent, _lib.raw_stream(weights.device.index),
+                      fields)
 
 
 def _check_evict(weights, source, block_tables, seq_lens, new_block_tables, budget, sink, recent,
@@ -146,6 +141,7 @@ def _check_evict(weights, source, block_tables, seq_lens, new_block_tables, budg
         raise ValueError("into must be (key_cache, value_cache[, key_scale, value_scale])")
     sc.check_pool(into[0], "into's key_cache")
     sc.check_same_layout(into[0], into[1], "into's caches")
+    sc.check_distinct(into[0], "into's caches")
     if into[0].dtype != key_cache.dtype or into[0].shape[1:] != key_cache.shape[1:]:
         raise ValueError("into's caches must match in type, page size, kv heads and head_dim")
     if (into[2] is None) != (key_scale is None) or (into[3] is None) != (key_scale is None):
@@ -155,6 +151,7 @@ def _check_evict(weights, source, block_tables, seq_lens, new_block_tables, budg
     if key_scale is not None:
         sc.check_same_layout(key_scale, value_scale, "key_scale and value_scale")
         sc.check_same_layout(into[2], into[3], "into's scales")
+        sc.check_distinct(into[2], "into's scales")
     for cache in (key_cache, into[0]):
         if any(x * cache.element_size() % 16 for x in cache.stride()[:3]):
             raise ValueError("cache strides must be multiples of 16 bytes")
@@ -203,14 +200,21 @@ def evict_by_weight(weights, key_cache, value_cache, block_tables, seq_lens, new
     ``min(seq_lens, budget)``, the moved weights (0 past them) and the positions the tokens
     had before (-1 past them).
     """
-    if _tracing():
-        raise ValueError("evict_by_weight is not traced: call it outside torch.compile")
     budget, sink, recent = int(budget), int(sink), int(recent)
     source = (key_cache, value_cache, key_scale, value_scale)
     if into is None:
         into = source
     elif len(into) == 2:
         into = (*into, None, None)
+    if _tracing():
+        _check_evict(weights, source, block_tables, seq_lens, new_block_tables, budget, sink,
+                     recent, into, new_weights)
+        from . import _op  # noqa: F401  (registers the ops)
+
+        kept, new_lens, new_weights = _results(weights, seq_lens, budget, new_weights)
+        torch.ops.sqa.evict_by_weight(weights, *source, block_tables, seq_lens, new_block_tables,
+                                      *into, new_weights, new_lens, kept, budget, sink, recent)
+        return new_lens, new_weights, kept
     layout = sc.layout
     seen = (layout(weights), layout(new_weights), layout(key_cache), layout(value_cache),
             layout(key_scale), layout(value_scale), layout(block_tables), layout(seq_lens),
@@ -219,13 +223,23 @@ def evict_by_weight(weights, key_cache, value_cache, block_tables, seq_lens, new
     if fields is None:
         _check_evict(weights, source, block_tables, seq_lens, new_block_tables, budget, sink,
                      recent, into, new_weights)
-        moved = weights[:, :, :budget].new_empty((*weights.shape[:2], budget)) \
-            if new_weights is None else new_weights
-        fields = _EVICTIONS.keep(seen, _lib.evict_fields(
-            weights, moved, source, into, block_tables, new_block_tables, budget, sink, recent))
     sc.check_aligned(16, key_cache, value_cache, into[0], into[1])
-    return sc.on_device(weights.device, run_evict, weights, new_weights, source, block_tables,
-                        seq_lens, into, new_block_tables, budget, sink, recent, fields)
+    kept, new_lens, new_weights = _results(weights, seq_lens, budget, new_weights)
+    if fields is None:
+        fields = _EVICTIONS.keep(seen, _lib.evict_fields(
+            weights, new_weights, source, into, block_tables, new_block_tables, budget, sink,
+            recent))
+    sc.on_device(weights.device, launch_evict, weights, new_weights, kept, seq_lens, new_lens,
+                 source, into, block_tables, new_block_tables, budget, sink, recent, fields)
+    return new_lens, new_weights, kept
+
+
+def _results(weights, seq_lens, budget, new_weights):
+    shape, device = (weights.shape[0], weights.shape[1], budget), weights.device
+    kept = torch.empty(shape, dtype=torch.int32, device=device)
+    if new_weights is None:
+        new_weights = torch.empty(shape, dtype=torch.float32, device=device)
+    return kept, torch.empty_like(seq_lens), new_weights
 
 
 __all__ = ["accumulate_attention_weights", "evict_by_weight"]

@@ -64,6 +64,12 @@ def check_same_layout(a, b, what):
         raise ValueError(f"{what} must match in shape, type and strides")
 
 
+def check_distinct(t, what):
+    """ValueError for a tensor that is written and has elements in one place (expanded)."""
+    if any(n > 1 and s == 0 for n, s in zip(t.shape, t.stride())):
+        raise ValueError(f"{what} must not be an expanded tensor: it is written")
+
+
 def check_scale(scale, cache, what="key_scale"):
     if scale.dtype != torch.float32 or tuple(scale.shape) != (cache.shape[0], cache.shape[2]):
         raise ValueError(f"{what} must be float32 [{cache.shape[0]}, {cache.shape[2]}]")
@@ -187,6 +193,8 @@ def _check_append(key, value, key_cache, value_cache, key_scale, value_scale, bl
     if key.dtype not in (torch.float16, torch.bfloat16) or value.dtype != key.dtype:
         raise ValueError("key and value must both be float16 or bfloat16")
     _check_cache(key_cache, value_cache, key_scale, value_scale)
+    check_distinct(key_cache, "key_cache")
+    check_distinct(key_scale, "key_scale")
     if tuple(key.shape[2:]) != tuple(key_cache.shape[2:]):
         raise ValueError("key and value need the cache's kv heads and head_dim")
     for t in (key, value):

@@ -1,0 +1,259 @@
+"""How the operators around the paged cache are called on the GPU: captured in graphs, on
+several streams, traced, through the FlashInfer-shaped entries, over large pools."""
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from small_q_attention_amd import decode_api, eviction, scaled_cache  # noqa: E402
+from small_q_attention_amd.masks import pack_draft_mask  # noqa: E402
+from tests import _cache_reference as ref  # noqa: E402
+from tests.test_gpu_scaled_cache import _cuda, _inputs, _trees  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+
+E4M3, INT8, F16, BF16 = torch.float8_e4m3fn, torch.int8, torch.float16, torch.bfloat16
+
+
+def _state(seed, lens=(300, 77, 513), q_len=4, dtype=F16, kv=E4M3):
+    """Everything a step of all four operators takes, on the GPU."""
+    hq, hkv, d, page, budget = 8, 2, 128, 16, 48
+    q, caches, scales, tables, sl = _inputs(list(lens), q_len, hq, hkv, d, page, dtype, kv, seed,
+                                            width=36)
+    # A pool of one size whatever the lengths.
+    spare = 120 - caches[0].shape[0]
+    caches = [torch.cat([c.view(torch.uint8), torch.zeros(spare, page, hkv, d, dtype=torch.uint8)])
+              .view(kv) for c in caches]
+    scales = [torch.cat([s, torch.ones(spare, hkv)]) for s in scales]
+    for c, s in zip(caches, scales):  # every slot holds something
+        c.view(torch.uint8)[(c.view(torch.uint8) & 0x7F) == 0x7F] = 0x30
+        s.nan_to_num_(nan=0.01)
+    g = torch.Generator().manual_seed(seed + 1)
+    key, value = (torch.randn(len(lens), q_len, hkv, d, generator=g).to(dtype) for _ in range(2))
+    into = [torch.zeros(3 * len(lens), page, hkv, d, dtype=torch.uint8).view(kv) for _ in range(2)]
+    new_tables = torch.randperm(3 * len(lens), generator=g).view(len(lens), 3).to(torch.int32)
+    # Entries past a sequence's pages: any page, never read.
+    tables = torch.where(tables < 0, 0, tables)
+    names = ("query", "k", "v", "ks", "vs", "tables", "lens", "key", "value", "into_k", "into_v",
+             "into_ks", "into_vs", "new_tables", "weights")
+    values = (q, *caches, *scales, tables, sl, key, value, *into,
+              torch.zeros(3 * len(lens), hkv), torch.zeros(3 * len(lens), hkv), new_tables,
+              torch.rand(len(lens), hkv, 36 * page, generator=g))
+    s = dict(zip(names, _cuda(*values)))
+    s["budget"] = budget
+    return s
+
+
+def _step(s):
+    """One pass of a decoding loop, everything it returns or writes."""
+    scaled_cache.append_scaled_kv(s["key"], s["value"], s["k"], s["v"], s["ks"], s["vs"],
+                                  s["tables"], s["lens"])
+    out = scaled_cache.paged_attention_scaled(s["query"], s["k"], s["v"], s["ks"], s["vs"],
+                                              s["tables"], s["lens"])
+    eviction.accumulate_attention_weights(s["query"], s["k"], s["tables"], s["lens"], s["weights"],
+                                          key_scale=s["ks"])
+    lens, weights, kept = eviction.evict_by_weight(
+        s["weights"], s["k"], s["v"], s["tables"], s["lens"], s["new_tables"], s["budget"], sink=2,
+        recent=5, key_scale=s["ks"], value_scale=s["vs"],
+        into=(s["into_k"], s["into_v"], s["into_ks"], s["into_vs"]))
+    return [out, lens, weights, kept, s["k"], s["v"], s["ks"], s["vs"], s["weights"], s["into_k"],
+            s["into_v"], s["into_ks"], s["into_vs"]]
+
+
+def _bits(xs):
+    return [x.view(torch.uint8).clone() if x.element_size() == 1 else x.clone() for x in xs]
+
+
+def _equal(a, b):
+    return all(torch.equal(x, y) for x, y in zip(_bits(a), _bits(b)))
+
+
+def _load(s, t):
+    """New data into the state's own buffers."""
+    for k, v in t.items():
+        if torch.is_tensor(v):
+            (s[k].view(torch.uint8) if v.element_size() == 1 else s[k]).copy_(
+                v.view(torch.uint8) if v.element_size() == 1 else v)
+
+
+@pytest.mark.parametrize("dtype,kv", [(F16, E4M3), (BF16, INT8)])
+def test_a_step_captured_in_a_graph(dtype, kv):
+    """Replays with other data, lengths among it, give the eager calls' bits, with eager
+    calls and synchronisations between them."""
+    s = _state(1, dtype=dtype, kv=kv)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        _step(s)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = _step(s)
+    for seed, lens in ((2, (300, 77, 513)), (3, (64, 400, 5)), (4, (0, 576, 48)), (5, (3, 17, 16))):
+        new = _state(seed, lens, dtype=dtype, kv=kv)
+        want = _bits(_step(_state(seed, lens, dtype=dtype, kv=kv)))
+        _load(s, new)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(_bits(got), want)), (seed, lens)
+        _step(new)
+
+
+def test_two_graphs_replayed_in_turn():
+    """Each graph's workspaces are its own."""
+    states = [_state(6, (500, 33, 70)), _state(7, (20, 570, 111))]
+    graphs, outs = [], []
+    for s in states:
+        _step(s)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(_step(s))
+        graphs.append(g)
+    fresh = [(6, (500, 33, 70)), (7, (20, 570, 111))]
+    want = [_bits(_step(_state(*f))) for f in fresh]
+    for s, f in zip(states, fresh):
+        _load(s, _state(*f))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for g, st in zip(graphs, streams):
+        with torch.cuda.stream(st):
+            g.replay()
+    torch.cuda.synchronize()
+    for o, w in zip(outs, want):
+        assert all(torch.equal(a, b) for a, b in zip(_bits(o), w))
+
+
+def test_calls_on_several_streams():
+    """Calls on other streams than the tensors' own, in turn and at once, give the bits of
+    the calls made alone."""
+    want = [_bits(_step(_state(10 + i))) for i in range(4)]
+    states = [_state(10 + i) for i in range(4)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in states]
+    outs = []
+    for s, st in zip(states, streams):
+        with torch.cuda.stream(st):
+            outs.append(_step(s))
+    torch.cuda.synchronize()
+    for o, w in zip(outs, want):
+        assert all(torch.equal(a, b) for a, b in zip(_bits(o), w))
+
+
+def test_attention_into_a_callers_workspace():
+    s = _state(20)
+    args = [s[k] for k in ("query", "k", "v", "ks", "vs", "tables", "lens")]
+    want = scaled_cache.paged_attention_scaled(*args)
+    ws = torch.full((64 << 20,), 0xFF, dtype=torch.uint8, device="cuda")
+    out = torch.empty_like(want)
+    got = scaled_cache.paged_attention_scaled(*args, out=out, workspace_buffer=ws)
+    assert got is out and torch.equal(out, want)
+    with pytest.raises(ValueError, match="workspace"):
+        scaled_cache.paged_attention_scaled(*args, workspace_buffer=ws[:64])
+    with pytest.raises(ValueError, match="16-byte"):
+        scaled_cache.paged_attention_scaled(
+            torch.empty(s["query"].numel() + 1, dtype=F16, device="cuda")[1:]
+            .view(s["query"].shape), *args[1:])
+
+
+@pytest.mark.parametrize("kv", [E4M3, INT8], ids=["e4m3", "int8"])
+@pytest.mark.parametrize("layout", ["NHD", "HND"])
+def test_the_flashinfer_shaped_entries(layout, kv):
+    b, q_len, hq, hkv, d, page = 3, 4, 8, 2, 128, 16
+    q, caches, scales, tables, sl = _inputs([300, 77, 513], q_len, hq, hkv, d, page, F16, kv, 30)
+    trees = _trees(b, q_len, 31, (1,))
+    pool = torch.stack([c.view(torch.uint8) for c in caches], 1)
+    if layout == "HND":
+        pool = pool.transpose(2, 3).contiguous()
+    pool = pool.cuda().view(kv)
+    qc, ks, vs, bt, slc = _cuda(q.view(b * q_len, hq, d), *scales, tables, sl)
+    ws = torch.zeros(64 << 20, dtype=torch.uint8, device="cuda")
+    want, bound, _ = ref.attention(q, *caches, *scales, tables, sl, trees, scale=0.1, out_scale=2.0)
+    out = torch.empty_like(qc)
+    for entry in (decode_api.xqa_batch_decode_with_kv_cache,
+                  decode_api.trtllm_batch_decode_with_kv_cache):
+        got = entry(qc, pool, ws, bt, slc, 513, 0.1, 2.0, kv_layout=layout, q_len_per_req=q_len,
+                    mask=pack_draft_mask(trees).cuda(), kv_block_scales=(ks, vs), out=out)
+        assert got is out
+        ref.assert_within(got.view(q.shape), want, bound)
+    want, bound, _ = ref.attention(q, *caches, *scales, tables, sl)
+    used = [-(-n // page) for n in (300, 77, 513)]
+    indptr = torch.tensor([0, used[0], sum(used[:2]), sum(used)], dtype=torch.int32).cuda()
+    indices = torch.cat([tables[i, :n] for i, n in enumerate(used)]).cuda()
+    last = torch.tensor([(n - 1) % page + 1 for n in (300, 77, 513)], dtype=torch.int32).cuda()
+    w = decode_api.BatchDecodeWithPagedKVCacheWrapper(ws, layout)
+    w.plan(indptr, indices, last, hq, hkv, d, page, q_data_type=F16, kv_data_type=kv,
+           q_len_per_req=q_len)
+    ref.assert_within(w.run(qc, pool, kv_block_scales=(ks, vs)).view(q.shape), want, bound)
+    if kv is INT8:
+        with pytest.raises(ValueError):
+            w.run(qc, pool)
+    with pytest.raises(ValueError):
+        w.run(qc, pool, kv_block_scales=(ks,))
+
+
+def test_traced_calls():
+    """torch.compile (fullgraph) runs the custom ops; the bits are the eager calls'."""
+    def step(query, key, value, k, v, ks, vs, tables, lens, weights, new_tables, *into):
+        scaled_cache.append_scaled_kv(key, value, k, v, ks, vs, tables, lens)
+        out = scaled_cache.paged_attention_scaled(query, k, v, ks, vs, tables, lens)
+        eviction.accumulate_attention_weights(query, k, tables, lens, weights, key_scale=ks)
+        moved = eviction.evict_by_weight(weights, k, v, tables, lens, new_tables, 48, recent=7,
+                                         key_scale=ks, value_scale=vs, into=into)
+        return (out * 2, *moved)
+
+    names = ("query", "key", "value", "k", "v", "ks", "vs", "tables", "lens", "weights",
+             "new_tables", "into_k", "into_v", "into_ks", "into_vs")
+    want, got = _state(40, kv=INT8), _state(40, kv=INT8)
+    a = step(*[want[n] for n in names])
+    b = torch.compile(step, backend="eager", fullgraph=True)(*[got[n] for n in names])
+    assert _equal(a, b)
+    assert _equal([want[n] for n in names], [got[n] for n in names])
+
+
+def test_a_pool_past_32_bit_offsets():
+    """Pages past 4 GiB of a pool, read, written and moved to."""
+    page, hkv, d = 64, 8, 128
+    pages = (5 << 30) // (page * hkv * d)
+    k, v = (torch.zeros(pages, page, hkv, d, dtype=torch.uint8, device="cuda").view(E4M3)
+            for _ in range(2))
+    ks, vs = (torch.ones(pages, hkv, device="cuda") for _ in range(2))
+    lens = torch.tensor([200, 130], dtype=torch.int32)
+    tables = torch.tensor([[pages - 1, 3, pages - 2, pages - 9],
+                           [pages - 4, pages - 3, 5, 0]], dtype=torch.int32)
+    g = torch.Generator().manual_seed(50)
+    key, value = (torch.randn(2, 200, hkv, d, generator=g).half() for _ in range(2))
+    q = torch.randn(2, 4, 32, d, generator=g).half()
+    bt, sl = _cuda(tables, lens)
+    scaled_cache.append_scaled_kv(*_cuda(key, value), k, v, ks, vs, bt, sl, new_lens=sl)
+    ids = tables.flatten().unique().long()
+    small = torch.searchsorted(ids, tables.long()).to(torch.int32)
+    pick = ids.cuda()
+    caches = [c.view(torch.uint8)[pick].cpu().view(E4M3) for c in (k, v)]
+    scales = [s[pick].cpu() for s in (ks, vs)]
+    mine = [torch.zeros(len(ids), page, hkv, d, dtype=torch.uint8).view(E4M3) for _ in range(2)]
+    mine_s = [torch.ones(len(ids), hkv) for _ in range(2)]
+    ref.append(key, value, mine, mine_s, small, lens, lens)
+    for a, b in zip(scales, mine_s):
+        assert torch.equal(a, b)
+    off = sum((a.view(torch.uint8) != b.view(torch.uint8)).sum().item() for a, b in zip(caches, mine))
+    assert off < 200 * 8  # ties of the rounding only
+    want, bound, mass = ref.attention(q, *caches, *scales, small, lens)
+    out = scaled_cache.paged_attention_scaled(q.cuda(), k, v, ks, vs, bt, sl)
+    ref.assert_within(out, want, bound)
+    weights = torch.zeros(2, hkv, 256, device="cuda")
+    eviction.accumulate_attention_weights(q.cuda(), k, bt, sl, weights, key_scale=ks)
+    ref.assert_within(weights, *ref.weights_after(torch.zeros(2, hkv, 256), mass, lens, 4))
+    new = torch.tensor([[pages - 20, 21], [pages - 22, 23]], dtype=torch.int32)
+    got = eviction.evict_by_weight(weights, k, v, bt, sl, new.cuda(), 70, key_scale=ks,
+                                   value_scale=vs)
+    into = [torch.zeros(4, page, hkv, d, dtype=torch.uint8).view(E4M3) for _ in range(2)]
+    into_s = [torch.zeros(4, hkv) for _ in range(2)]
+    kept = ref.evict(weights.cpu(), caches, scales, small, lens,
+                     torch.arange(4).view(2, 2).to(torch.int32), 70, 0, 0, into, into_s)[2]
+    assert torch.equal(got[2].cpu(), kept)
+    for c, w, s, ws in zip((k, v), into, (ks, vs), into_s):
+        at = new.flatten().long().cuda()
+        assert torch.equal(c.view(torch.uint8)[at].cpu(), w.view(torch.uint8))
+        assert torch.equal(s[at].cpu(), ws)

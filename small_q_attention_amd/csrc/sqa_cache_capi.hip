@@ -229,6 +229,7 @@ int sqa_paged_attention_scaled(const sqa_attention_args* args, const sqa_block_s
   p.page_shift = page_shift_of(a.page_size);
   p.max_pages = a.max_pages << p.page_shift;
   p.num_splits = a.num_splits;
+  p.by_splits = sqa::fast_div(a.num_splits);
   p.by_group = sqa::fast_div(group);
   p.scale_log2 = (float)(1.4426950408889634 * (double)a.scale);
   p.out_scale = a.out_scale;
@@ -444,6 +445,7 @@ int sqa_attention_weights(const sqa_weights_args* args) {
   p.bt_stride = a.max_pages;
   p.page_shift = shift;
   p.max_pages = (int)plan.pages;
+  p.by_splits = sqa::fast_div((unsigned)plan.items);
   p.by_group = sqa::fast_div(group);
   p.scale_log2 = (float)(1.4426950408889634 * (double)a.scale);
   p.bf16 = a.dtype == SQA_DTYPE_BF16;

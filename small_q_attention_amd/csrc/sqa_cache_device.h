@@ -22,41 +22,54 @@ __device__ __forceinline__ int wave_sum_int(int x) {
   return __builtin_amdgcn_readlane(wave_inclusive_scan_int(x), 63);
 }
 
+// ceil(n / d) for 0 <= n < 2^27, 0 < d, by the reciprocal: the first estimate is off by a
+// few at most, the second by one. A dozen instructions; a division by a run-time value is
+// three times that, and a wave's way to its first load had up to ten.
+__device__ __forceinline__ int ceil_quotient(int n, int d, float inv) {
+  int q = (int)((float)n * inv);
+  q += (int)((float)(n - q * d) * inv);
+  int r = n - q * d;
+  q -= r < 0 ? 1 : 0;
+  r += r < 0 ? d : 0;
+  return q + (r > 0 ? 1 : 0) + (r > d ? 1 : 0);
+}
+
 // The cut of the batch into work items, found by every wave for itself from the lengths:
 // sequence b takes n_b = max(1, ceil(pages_b / P)) items of nearly equal size, with P the
 // smallest page count of at least kMinSplitPages for which they sum to at most `items`
 // (or P the longest sequence, one item each, where the batch has more sequences than
 // that). All items are resident at once, so the longest, P pages, sets the time.
 // Returns whether item `item` exists; `table` (one wave of the grid) also receives each
-// sequence's first item and count for the merge kernel.
-__device__ __forceinline__ bool find_split(const PartialArgs& a, int items, int item,
-                                           SeqSplits* table, Split& out) {
+// sequence's first item and count for the merge kernel. ONE: at most 64 sequences, one
+// per lane, whose page counts stay in a register.
+template <bool ONE>
+__device__ __forceinline__ bool find_split_of(const PartialArgs& a, int items, int item,
+                                              SeqSplits* table, Split& out) {
   const int lane = threadIdx.x & 63;
-  const int groups = (a.batch + 63) / 64;
+  const int groups = ONE ? 1 : (a.batch + 63) / 64;
   auto length_of = [&](int k) {
     const int i = 64 * k + lane;
     return i < a.batch ? max(a.seq_lens[i], 0) : 0;
   };
   const int len0 = length_of(0);
-  auto pages_at = [&](int k) {
-    const int len = k == 0 ? len0 : length_of(k);
-    return min((len + kPageSize - 1) / kPageSize, a.max_pages);
-  };
-  auto splits_of = [&](int k, int P) {
-    return 64 * k + lane < a.batch ? max((pages_at(k) + P - 1) / P, 1) : 0;
+  auto len_at = [&](int k) { return ONE || k == 0 ? len0 : length_of(k); };
+  auto pages_at = [&](int k) { return min((len_at(k) + kPageSize - 1) / kPageSize, a.max_pages); };
+  auto splits_of = [&](int k, int P, float inv) {
+    return 64 * k + lane < a.batch ? max(ceil_quotient(pages_at(k), P, inv), 1) : 0;
   };
   int total = 0;
   for (int k = 0; k < groups; ++k) total += wave_sum_int(pages_at(k));
   auto fits = [&](int P) {
+    const float inv = __builtin_amdgcn_rcpf((float)P);
     int n = 0;
-    for (int k = 0; k < groups; ++k) n += wave_sum_int(splits_of(k, P));
+    for (int k = 0; k < groups; ++k) n += wave_sum_int(splits_of(k, P, inv));
     return n <= items;
   };
-  int lo = max(kMinSplitPages, (total + items - 1) / items);
-  if (!fits(lo)) {
+  int P = max(kMinSplitPages, (total + items - 1) / a.by_splits);  // by_splits: items
+  if (!fits(P)) {
     // ceil(pages_b / P) sum to at most total / P + batch.
-    int hi = items > a.batch ? max(lo, (total + items - a.batch - 1) / (items - a.batch))
-                             : max(a.max_pages, 1);
+    int lo = P, hi = items > a.batch ? max(P, (total + items - a.batch - 1) / (items - a.batch))
+                                     : max(a.max_pages, 1);
     while (lo + 1 < hi) {  // lo does not fit, hi does (or is one item each)
       const int mid = lo + (hi - lo) / 2;
       if (fits(mid))
@@ -64,13 +77,13 @@ __device__ __forceinline__ bool find_split(const PartialArgs& a, int items, int 
       else
         lo = mid;
     }
-    lo = hi;
+    P = hi;
   }
-  const int P = lo;
+  const float inv = __builtin_amdgcn_rcpf((float)P);
   int base = 0;
   bool found = false;
   for (int k = 0; k < groups; ++k) {
-    const int n = splits_of(k, P);
+    const int n = splits_of(k, P, inv);
     const int incl = wave_inclusive_scan_int(n);
     const int first = base + incl - n;
     if (table != nullptr && 64 * k + lane < a.batch) table[64 * k + lane] = SeqSplits{first, n};
@@ -79,11 +92,12 @@ __device__ __forceinline__ bool find_split(const PartialArgs& a, int items, int 
       const int src = __builtin_ctzll(hit);
       const int pages = __builtin_amdgcn_readlane(pages_at(k), src);
       out.b = 64 * k + src;
-      out.len = __builtin_amdgcn_readlane(k == 0 ? len0 : length_of(k), src);
+      out.len = __builtin_amdgcn_readlane(len_at(k), src);
       out.count = __builtin_amdgcn_readlane(n, src);
       out.slot = item;
       out.first = __builtin_amdgcn_readlane(first, src);
-      const int size = (pages + out.count - 1) / out.count;
+      const int size = __builtin_amdgcn_readfirstlane(
+          ceil_quotient(pages, out.count, __builtin_amdgcn_rcpf((float)out.count)));
       out.p_begin = (item - out.first) * size;
       out.p_end = min(out.p_begin + size, pages);
       found = true;
@@ -92,6 +106,11 @@ __device__ __forceinline__ bool find_split(const PartialArgs& a, int items, int 
     base += __builtin_amdgcn_readlane(incl, 63);
   }
   return found;
+}
+__device__ __forceinline__ bool find_split(const PartialArgs& a, int items, int item,
+                                           SeqSplits* table, Split& out) {
+  return a.batch <= 64 ? find_split_of<true>(a, items, item, table, out)
+                       : find_split_of<false>(a, items, item, table, out);
 }
 
 // x / s for many x, rounded as the division is. With r = 1/s rounded to nearest, two

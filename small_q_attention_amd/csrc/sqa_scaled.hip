@@ -305,9 +305,10 @@ void sqa_scaled_attention_kernel(ScaledArgs args) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) pr[e] = fast_exp2(fmaf(s[nb][e], c, off));
           const float sum = (pr[0] + pr[1]) + (pr[2] + pr[3]);
+          const float l = st.l[nb];
+          st.l[nb] = fmaf(sum, inv_vs, l);
           // A V scale that is not finite stays with the rows that see its page.
-          const float l = fmaf(sum, inv_vs, st.l[nb]);
-          st.l[nb] = masked && sum == 0.f ? st.l[nb] : l;
+          if (masked) st.l[nb] = sum == 0.f ? l : st.l[nb];  // uniform
           ph[nb] = ElemF16::round_p(pr[0], pr[1], pr[2], pr[3], rounded, none);
         }
         if (loud) {  // uniform

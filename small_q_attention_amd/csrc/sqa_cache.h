@@ -49,10 +49,15 @@ struct AppendArgs {
 };
 hipError_t launch_append(const AppendArgs& a, hipStream_t stream);
 
-// Whether the scores of a call travel from its first to its second kernel through memory:
-// 4 bytes per row and token written and read again, against K read a second time.
+// Whether the scores of a call travel from its first to its second kernel through memory,
+// 4 bytes per row and token written and read again, or K is read and multiplied a second
+// time. Writes among the reads cost more than their bytes: the two meet where the scores
+// are a quarter of K. Whole calls, stored / computed again, head dim 128: 16 x 32K keys,
+// 16-bit K, 4 rows 254 / 388 us, 8 278 / 383, 16 329 / 381, 24 392 / 383, 32 436 / 384;
+// e4m3 4 rows 150 / 203, 8 173 / 201, 12 202 / 201, 16 224 / 204. 4 x 8K, 16-bit: 4 rows
+// 23 / 29, 8 25 / 29, 12 30 / 29, 16 31 / 29; e4m3: 4 rows 18 / 19, 8 21 / 19.
 __host__ __device__ constexpr bool weights_stored(long long rows, int head_dim, int kv_bytes) {
-  return 8 * rows <= (long long)head_dim * kv_bytes;
+  return 16 * rows <= (long long)head_dim * kv_bytes;
 }
 
 // Attention weights added up. Of `p` the fields of the query side, of K and of the tables.

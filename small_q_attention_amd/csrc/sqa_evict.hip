@@ -6,8 +6,12 @@
 // where the call's own draft tokens start at 0. Two kernels: the first reads K once and
 // leaves, for each row and work item, the maximum and the sum of exponentials; the second
 // joins them to the rows' log-sum-exp and adds the weights up. Between them the scores
-// either go through memory in fp32 (rows * 8 bytes a token and head, written and read) or
-// K is read and multiplied again, whichever moves fewer bytes.
+// either go through memory in fp32 or K is read and multiplied again (weights_stored()).
+//
+// What bounds them: 16 sequences of 32K keys, one token each, 16-bit K (1.07 GB): the first
+// kernel 231 us, of which the 67 MB of scores it writes take about 50 (182 us without),
+// 4.9 TB/s in all; the second 23 us. Many rows: instructions (64 rows, 8 sequences of up to
+// 12K keys, e4m3: 20 and 25 us), of which about 6 us each are the way to the first page.
 #include "sqa_cache.h"
 #include "sqa_cache_device.h"
 
@@ -89,7 +93,7 @@ __device__ __forceinline__ float2 join(float2 a, float2 b) {
 // row that saw nothing: +inf, which makes every weight 0. Lanes lie over rows first, then
 // over items, so the records of an item come in one line and few exchanges follow, and a
 // lane asks for kAtOnce of them at a time (64 rows, 8 sequences of up to 12K keys, the
-// kernel: one row after the other 72 us, four records at a time 31, TODO).
+// kernel: one row after the other 72 us, four records at a time 31, sixteen 25).
 constexpr int kAtOnce = 16;
 __device__ __forceinline__ float rows_lse(const float2* st, int stride, int rows, int count) {
   const int lane = threadIdx.x & 63;
@@ -217,6 +221,9 @@ void sqa_weigh_kernel(WeighArgs args) {
         (void*)((const char*)a.k + off), (short)0, pid >= 0 ? (int)a.page_extent : 0, kBufferFlags);
     s.scale = 1.f;
     if (args.k_scale) s.scale = *(const float*)(scale_at + max(pid, 0) * args.scale_page);
+    // The first pass reads K through the caches: non-temporal, its reads and the scores it
+    // writes got in each other's way (16 x 32K keys, four rows: 245 -> 229 us, the second
+    // kernel 20 -> 23).
 #pragma unroll
     for (int i = 0; i < KEYS::kLoads; ++i)
       s.k.k[i] = __builtin_amdgcn_raw_buffer_load_b128(kr, k_lane + 64 * i, 0,
@@ -234,10 +241,8 @@ void sqa_weigh_kernel(WeighArgs args) {
     l[nb] = 0.f;
   }
   float* wrow = args.weights + b * args.w_batch + kvh * args.w_head;
-  // Scores leave through a resource bounded to the item's, rows that are not there sent
-  // past its end: a store under a branch would leave the compiler guessing what is in
-  // flight, and its waits for the ring's pages would drain part of the ring (16 x 32K
-  // keys, one row block: 248 us under a branch, TODO so).
+  // Scores leave through a resource bounded to the item's pages, rows that are not there
+  // sent past its end, so that no branch stands around a store.
   const unsigned head_scores = a.rows * kPageSize * 4u, page_scores = a.hkv * head_scores;  // bytes
   const __amdgpu_buffer_rsrc_t out = __builtin_amdgcn_make_buffer_rsrc(
       (void*)((char*)args.scores + ((size_t)b * a.max_pages + p_begin) * page_scores),
@@ -368,9 +373,9 @@ void sqa_weigh_kernel(WeighArgs args) {
 }
 
 // The second pass from the stored scores: a lane takes four consecutive tokens, a wave
-// 256 at a time. The scores of four rows are requested before any is used: one row after
-// the other, each round of a few hundred tokens waited for memory once per row (16 x 32K
-// keys, four rows: 25 us, TODO so).
+// 256 at a time. The scores of four rows are requested before any is used (one row after
+// the other a round waited for memory once per row: 16 x 32K keys, four rows, 25 us, 20
+// so).
 typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
 __global__ __launch_bounds__(256) void sqa_weigh_join_kernel(WeighArgs args) {
   const PartialArgs& a = args.p;
@@ -439,6 +444,12 @@ __device__ __forceinline__ unsigned weight_key(float w) {
   return w != w ? kNanKey : k;
 }
 constexpr int kSelectThreads = 1024, kSelectWaves = kSelectThreads / 64;
+
+// What bounds eviction: 32 sequences of up to 4K keys, half of each kept, 16-bit (0.53 GB):
+// the selection 10 us, the moves 108 us, 4.9 TB/s, a large copy's rate. 16 of up to 32K, 4K
+// of each kept, e4m3: selection 25 us (a workgroup of one compute unit per sequence and
+// head, 126 registers a thread; 35 with the weights' keys made again each time, 59 from
+// memory), moves 60.
 
 // Which tokens of one sequence and kv head stay. The smallest key that stays is found by
 // a radix selection over the weights between the sink and the recent tokens (11, 11 and

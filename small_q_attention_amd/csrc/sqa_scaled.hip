@@ -8,6 +8,11 @@
 //   out(row)       = sum_t (p(row, t) * v_scale[page of t]) v_code[t] / sum_t p(row, t)
 // so the codes go to the MFMAs as they are (both types widen exactly to 16 bits) and a
 // page costs two scalars.
+//
+// What bounds attention: HBM up to 32 rows (16 x 32K keys, e4m3, 1.08 GB, partial kernel:
+// q_len 8 175 us, 6.2 TB/s; whole calls q_len 1, 2, 4 at 177 us, 6.1 TB/s, within 6% of the
+// per-tensor e4m3 kernel's 167), instructions at 64 (q_len 16 254 us). Append: 2 x 16K
+// tokens, 0.2 GB, 43 us, 4.7 TB/s, near a large copy's 5.1.
 #include "sqa_cache.h"
 #include "sqa_cache_device.h"
 
@@ -75,7 +80,8 @@ struct CodesInt8 : KvFp8<HD> {
 
 // Partial rows are fp32 for both types of queries: fp16 ones, as the 16-bit kernels leave,
 // added a rounding of the size of the output's own (error against 64 bits 1.45 times that
-// of a rounded 32-bit result; so 1.1 times). TODO cost
+// of a rounded 32-bit result; so 1.1 times). It costs 16 x 32K keys, q_len 8, 178 -> 181 us
+// a call, 4 x 8K 22 -> 27.
 template <typename E>
 using PartialRows = std::conditional_t<E::kHalfPartials, ElemF16Wide, E>;
 

@@ -160,7 +160,8 @@ __device__ __forceinline__ void nan_values(WaveState<NB, HD>& st, typename KV::R
 // bf16 parts of p * v_scale cost 28 operations a page more at 32 rows (16 x 32K keys,
 // whole calls: q_len 8 201 -> 178 us, q_len 16 293 -> 245). The row sum gets P / v_scale in
 // fp32, unrounded: a quiet block's tokens weigh as much in it as a loud one's. Pages of a
-// scale under 2^-100 add to the row sums only.
+// scale under 2^-64, 0 among them, count as of that scale in the maximum and the row sums
+// and add nothing to O (a scale further down would push their P out of fp32's range).
 template <int NB, int D, int HD, typename E, typename KV, bool PIPE>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1)))
 void sqa_scaled_attention_kernel(ScaledArgs args) {
@@ -270,9 +271,9 @@ void sqa_scaled_attention_kernel(ScaledArgs args) {
             float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, ring[j].scale), 0));
         const float vs = __builtin_bit_cast(
             float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, ring[j].scale), 32));
-        const bool loud = !(vs < 0x1p-100f);
-        const float lv = loud ? __builtin_amdgcn_logf(vs) : 0.f;
-        const float inv_vs = loud ? __builtin_amdgcn_rcpf(vs) : 1.f;
+        const bool loud = !(vs < 0x1p-64f);
+        const float lv = loud ? __builtin_amdgcn_logf(vs) : -64.f;
+        const float inv_vs = loud ? __builtin_amdgcn_rcpf(vs) : 0x1p64f;
         float c = a.scale_log2 * ks, add = lv;
         f4 s[NB];
         if constexpr (PIPE) {

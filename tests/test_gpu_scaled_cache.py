@@ -148,6 +148,24 @@ def test_attention_blocks_of_zeros():
     assert (out[1] == 0).all()
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=["fp16", "bf16"])
+@pytest.mark.parametrize("loud", [-30, -12, 8])
+def test_attention_blocks_of_zeros_beside_others(loud, dtype):
+    """Blocks of zeros that attract most of the attention, beside blocks of any size: what
+    those hold is still there in the result."""
+    q, caches, scales, tables, sl = _inputs([400, 90], 3, 8, 2, 128, 16, dtype, E4M3, seed=14)
+    scales[1][tables[0, ::2].long()] = 0.0
+    scales[0][tables[0, ::2].long()] *= 4.0
+    scales[1][tables[0, 1::2].long()] *= 2.0 ** loud
+    want, bound, _ = ref.attention(q, *caches, *scales, tables, sl)
+    # The output's 2^-24 is for fp16's subnormals; bf16 has the range.
+    if dtype is BF16:
+        bound = bound - 2.0 ** -24 + 2.0 ** -60
+    out = paged_attention_scaled(*_cuda(q, *caches, *scales, tables, sl))
+    ref.assert_within(out, want, bound)
+    assert dtype is F16 or (out[0].abs() > 0).float().mean() > 0.99
+
+
 @pytest.mark.parametrize("layout", ["nhd", "hnd", "scales_together"])
 def test_attention_reads_views_by_their_strides(layout):
     q, caches, scales, tables, sl = _inputs([300, 77], 4, 8, 2, 64, 32, BF16, E4M3, seed=5)

@@ -273,6 +273,8 @@ int sqa_plan_scaled(int device, int batch, int num_kv_heads, int max_seq_len, in
 /*
  * sqa_paged_attention over such a cache: kv_dtype SQA_DTYPE_FP8_E4M3 or SQA_DTYPE_INT8,
  * num_splits from sqa_plan_scaled, pages_per_split 0, flags 0; everything else as there.
+ * V blocks of a scale under 2^-64 count as zeros; the V scales of what a row sees, those of
+ * zeros taken as 2^-64, may lie a factor of 2^100 apart.
  * A sequence's splits follow from all lengths of the batch, so its last bits may differ
  * between batches; equal inputs give equal bits.
  */
@@ -321,7 +323,8 @@ typedef struct sqa_append_args {
  * the earlier tokens' codes are rounded again, code * old / new. A page whose first slot
  * is written starts afresh. Infinities count as the type's largest finite value; NaN does
  * not count and is stored as NaN (e4m3) or 0 (int8). Slots past a sequence's end stay as
- * they are. No two sequences may write the same page in one call.
+ * they are. No page may be written twice in one call, by two sequences or by two entries
+ * of one table row; keys and values have caches and scales of their own.
  */
 int sqa_append_scaled(const sqa_append_args* args);
 
@@ -384,12 +387,14 @@ int sqa_attention_weights(const sqa_weights_args* args);
 /*
  * Arguments of sqa_evict (set struct_size = sizeof(sqa_evict_args)).
  *   weights       [batch, num_kv_heads, weights_width], of every token
- *   new_weights   [batch, num_kv_heads, new_weights_width >= budget]; may be `weights`
+ *   new_weights   [batch, num_kv_heads, new_weights_width >= budget]; may be `weights`,
+ *                 not overlap it in another way
  *   kept          [batch, num_kv_heads, budget] int32, contiguous
  *   kv, scales    the cache the tokens are in (scales.k NULL: none), tables
  *                 [batch, max_pages], lengths seq_lens
  *   into, into_scales  where they go, pages new_tables [batch, new_max_pages]; may be the
- *                 same pool, on pages no row of block_tables uses
+ *                 same pool, on pages no row of block_tables uses, each once; into.k and
+ *                 into.v differ, as do their scales
  *   new_lens      [batch], written
  * Strides of kv and into must be multiples of 16 bytes.
  */

@@ -310,6 +310,8 @@ int sqa_append_scaled(const sqa_append_args* args) {
     if (st < 0 || st % 8 || st > ((int64_t)1 << 40))
       return fail(SQA_ERR_INVALID,
                   "key and value strides must be non-negative multiples of 8 elements");
+  if (a.kv.k == a.kv.v || a.scales.k == a.scales.v)
+    return fail(SQA_ERR_INVALID, "keys and values are written: each needs its own cache and scales");
   sqa::AppendArgs k;
   memset(&k, 0, sizeof(k));
   k.src[0] = a.key;
@@ -521,6 +523,8 @@ int sqa_evict(const sqa_evict_args* args) {
   if (grid > 0x7fffffffLL || (long long)a.batch * a.num_kv_heads > 0x7fffffffLL)
     return fail(SQA_ERR_INVALID, "grid too large");
 
+  if (a.into.k == a.into.v || (scaled && a.into_scales.k == a.into_scales.v))
+    return fail(SQA_ERR_INVALID, "keys and values are written: each needs its own cache and scales");
   sqa::EvictArgs k;
   memset(&k, 0, sizeof(k));
   k.weights = a.weights;

@@ -97,7 +97,7 @@ def accumulate_attention_weights(query, key_cache, block_tables, seq_lens, weigh
         raise ValueError("query must be a contiguous [B, Q, Hq, D] tensor")
     scale = sc.check_softmax_scale(scale, query.shape[3])
     words = None if mask is None else as_words(mask, query.shape[0], query.shape[1])
-    max_seq_len = max(int(max_seq_len), 0)
+    max_seq_len = min(max(int(max_seq_len), 0), 2**31 - 1)
     if _tracing():
         _check_accumulate(query, key_cache, block_tables, seq_lens, weights, key_scale, words)
         from . import _op  # noqa: F401  (registers the ops)
@@ -188,12 +188,13 @@ def evict_by_weight(weights, key_cache, value_cache, block_tables, seq_lens, new
     within the budget moves whole. Keys keep whatever position they were rotated to.
 
     The new pages belong to the same pool, and then must be pages that no sequence of the
-    call uses (the old ones may be shared by several), or to the caches of ``into``:
+    call uses, each of them once (the old ones may be shared by several), or to the caches of
+    ``into``:
     ``(key_cache, value_cache)`` of the same type, page size and heads, with
     ``(..., key_scale, value_scale)`` for scaled ones. In scaled caches a new block takes the
     largest scale among the blocks its tokens come from, and codes of other blocks are
-    rounded again. ``weights`` may be written in place: ``new_weights=weights``; ``None``
-    returns new ones, ``[B, Hkv, budget]``. ``T`` and the table bound the lengths that are
+    rounded again. ``weights`` may be written in place: ``new_weights=weights`` (a buffer that
+    overlaps it in another way may not be given); ``None`` returns new ones, ``[B, Hkv, budget]``. ``T`` and the table bound the lengths that are
     looked at.
 
     Returns ``(new_lens [B] int32, new_weights, kept [B, Hkv, budget] int32)``: the lengths
@@ -224,6 +225,7 @@ def evict_by_weight(weights, key_cache, value_cache, block_tables, seq_lens, new
         _check_evict(weights, source, block_tables, seq_lens, new_block_tables, budget, sink,
                      recent, into, new_weights)
     sc.check_aligned(16, key_cache, value_cache, into[0], into[1])
+    sc.check_apart(*into)
     kept, new_lens, new_weights = _results(weights, seq_lens, budget, new_weights)
     if fields is None:
         fields = _EVICTIONS.keep(seen, _lib.evict_fields(

@@ -70,6 +70,15 @@ def check_distinct(t, what):
         raise ValueError(f"{what} must not be an expanded tensor: it is written")
 
 
+def check_apart(key_cache, value_cache, key_scale, value_scale):
+    """ValueError for one cache, or one tensor of scales, given for keys and values both: they
+    are written."""
+    if key_cache.data_ptr() == value_cache.data_ptr() or (
+            key_scale is not None and key_scale.data_ptr() == value_scale.data_ptr()):
+        raise ValueError("keys and values each need a cache and scales of their own: they are "
+                         "written")
+
+
 def check_scale(scale, cache, what="key_scale"):
     if scale.dtype != torch.float32 or tuple(scale.shape) != (cache.shape[0], cache.shape[2]):
         raise ValueError(f"{what} must be float32 [{cache.shape[0]}, {cache.shape[2]}]")
@@ -154,7 +163,8 @@ def append_scaled_kv(key, value, key_cache, value_cache, key_scale, value_scale,
     the page; where it grows, their codes are rounded again. Slots past the sequence's end
     and pages outside the pool or the table are left as they are. Infinities count as the
     type's largest finite value; a NaN does not count and is stored as NaN (e4m3) or 0
-    (int8). No two sequences may write the same page in one call.
+    (int8). No page may be written twice in one call, by two sequences or by two entries of
+    one table row.
     """
     if _tracing():
         _check_append(key, value, key_cache, value_cache, key_scale, value_scale, block_tables,
@@ -173,6 +183,7 @@ def append_scaled_kv(key, value, key_cache, value_cache, key_scale, value_scale,
         fields = _APPENDS.keep(seen, _lib.append_fields(key, value, key_cache, key_scale,
                                                         block_tables))
     check_aligned(16, key, value, key_cache, value_cache)
+    check_apart(key_cache, value_cache, key_scale, value_scale)
     on_device(key.device, _launch_append, key, value, key_cache, value_cache, key_scale,
               value_scale, block_tables, seq_lens, new_lens, fields)
 
@@ -263,15 +274,17 @@ def paged_attention_scaled(query, key_cache, value_cache, key_scale, value_scale
     last ``Q``, those up to its own or those ``mask`` names (the packed draft mask of
     :mod:`small_q_attention_amd.masks`). Rows that see no token are 0. ``max_seq_len`` > 0
     only sizes the call (0: the block table's width); ``scale`` is the softmax scale
-    (``None``: ``D ** -0.5``), ``out_scale`` multiplies the output. ``workspace_buffer``:
-    a caller's buffer for the split partials; ``None`` takes one kept per stream, or, under
-    graph capture, one of the graph's own. Returns ``out`` (``[B, Q, Hq, D]``).
+    (``None``: ``D ** -0.5``), ``out_scale`` multiplies the output. V blocks of a scale under
+    2^-64 count as zeros; the V scales of what a row sees, those of zeros taken as 2^-64, may
+    lie a factor of 2^100 apart. ``workspace_buffer``: a caller's buffer for the split
+    partials; ``None`` takes one kept per stream, or, under graph capture, one of the graph's
+    own. Returns ``out`` (``[B, Q, Hq, D]``).
     """
     if query.dim() != 4:
         raise ValueError("query must be a contiguous [B, Q, Hq, D] tensor")
     scale = check_softmax_scale(scale, query.shape[3])
     words = None if mask is None else as_words(mask, query.shape[0], query.shape[1])
-    max_seq_len = max(int(max_seq_len), 0)
+    max_seq_len = min(max(int(max_seq_len), 0), 2**31 - 1)
     if _tracing():
         _check_attention(query, key_cache, value_cache, key_scale, value_scale, block_tables,
                          seq_lens, words, out, workspace_buffer)

@@ -295,6 +295,36 @@ def test_evict_status(lib, change, status):
     assert lib.sqa_evict(None) == INVALID
 
 
+@pytest.mark.parametrize("change", [dict(kv__v=4096), dict(scales__v=4096)],
+                         ids=["caches", "scales"])
+def test_append_needs_a_cache_each_for_keys_and_values(lib, change):
+    a = _fill(_lib.AppendArgs, **{**dict(
+        key=4096, value=4096, kv__k=4096, kv__v=1 << 20, kv__num_pages=6, kv__page_stride=2048,
+        kv__token_stride=128, kv__head_stride=64, scales__k=4096, scales__v=8192,
+        scales__page_stride=2, scales__head_stride=1, block_tables=4096, seq_lens=4096, max_pages=4,
+        batch=2, q_len=3, num_kv_heads=2, head_dim=64, page_size=16, dtype=0, kv_dtype=2), **change})
+    a.key_strides[:] = a.value_strides[:] = (384, 128, 64)
+    assert lib.sqa_append_scaled(ctypes.byref(a)) == INVALID
+    assert b"own cache" in lib.sqa_last_error()
+
+
+@pytest.mark.parametrize("change", [dict(into__v=4096), dict(into_scales__v=4096)],
+                         ids=["caches", "scales"])
+def test_evict_needs_a_cache_each_for_keys_and_values(lib, change):
+    pool = dict(k=4096, v=1 << 20, num_pages=6, page_stride=2048, token_stride=128, head_stride=64)
+    sc = dict(k=4096, v=8192, page_stride=2, head_stride=1)
+    a = _fill(_lib.EvictArgs, **{**dict(
+        weights=4096, weights_batch_stride=128, weights_head_stride=64, new_weights=4096,
+        new_weights_batch_stride=40, new_weights_head_stride=20, kept=4096, seq_lens=4096,
+        new_lens=4096, block_tables=4096, new_tables=4096, weights_width=64, new_weights_width=20,
+        max_pages=4, new_max_pages=2, budget=20, sink=2, recent=3, batch=2, num_kv_heads=2,
+        head_dim=64, page_size=16, kv_dtype=2, **{f"kv__{k}": v for k, v in pool.items()},
+        **{f"into__{k}": v for k, v in pool.items()}, **{f"scales__{k}": v for k, v in sc.items()},
+        **{f"into_scales__{k}": v for k, v in sc.items()}), **change})
+    assert lib.sqa_evict(ctypes.byref(a)) == INVALID
+    assert b"own cache" in lib.sqa_last_error()
+
+
 # ----- the traced ops -----
 
 @pytest.mark.parametrize("name,writes", [

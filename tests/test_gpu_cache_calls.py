@@ -212,6 +212,21 @@ def test_traced_calls():
     assert _equal([want[n] for n in names], [got[n] for n in names])
 
 
+def test_keys_and_values_written_to_one_place_are_refused():
+    s = _state(9)
+    before = _bits([s["k"], s["v"], s["ks"], s["vs"]])
+    for k, v, ks, vs in (("k", "k", "ks", "vs"), ("k", "v", "vs", "vs")):
+        with pytest.raises(ValueError, match="of their own"):
+            scaled_cache.append_scaled_kv(s["key"], s["value"], s[k], s[v], s[ks], s[vs],
+                                          s["tables"], s["lens"])
+    for into in (("into_k", "into_k", "into_ks", "into_vs"), ("into_k", "into_v") + 2 * ("into_ks",)):
+        with pytest.raises(ValueError, match="of their own"):
+            eviction.evict_by_weight(s["weights"], s["k"], s["v"], s["tables"], s["lens"],
+                                     s["new_tables"], s["budget"], key_scale=s["ks"],
+                                     value_scale=s["vs"], into=tuple(s[n] for n in into))
+    assert _equal(before, [s["k"], s["v"], s["ks"], s["vs"]])
+
+
 def test_a_pool_past_32_bit_offsets():
     """Pages past 4 GiB of a pool, read, written and moved to."""
     page, hkv, d = 64, 8, 128

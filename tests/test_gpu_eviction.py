@@ -91,6 +91,12 @@ def test_weights_draft_trees(q_len, types):
     _check_weigh(lens, q_len, 8, 2, 128, 16, types, seed=q_len, trees=_trees(4, q_len, 1, (0, 3)))
 
 
+@pytest.mark.parametrize("types", [TYPES[0], TYPES[3]], ids=[IDS[0], IDS[3]])
+def test_weights_of_a_wide_table(types):
+    """A table whose scores would pass 1 GiB: few rows, and K is read twice all the same."""
+    _check_weigh([700, 33], 2, 16, 4, 128, 16, types, seed=8, width=(1 << 18) + 5)
+
+
 @pytest.mark.parametrize("q_len", [2, 12])
 def test_weights_narrower_than_the_sequences(q_len):
     _check_weigh([300, 40], q_len, 8, 2, 128, 16, TYPES[1], cut=45)

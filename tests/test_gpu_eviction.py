@@ -238,6 +238,12 @@ def test_evict_a_long_sequence():
     _check_evict(_evict_case([70001, 12], 1, 64, 64, E4M3, 5001, seed=5), 5001, 10, 100)
 
 
+def test_evict_long_sequences_in_place():
+    """Weights too many to be held: they move over themselves."""
+    _check_evict(_evict_case([40001, 33000, 12], 1, 64, 64, E4M3, 5001, seed=6, ties=True), 5001,
+                 10, 100, True)
+
+
 def test_evict_within_one_pool():
     """New pages of the same pool, and pages two sequences share among the old ones."""
     weights, caches, scales, tables, sl, _, _, _ = _evict_case([300, 300], 2, 128, 16, E4M3, 64,

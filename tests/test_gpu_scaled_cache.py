@@ -166,6 +166,18 @@ def test_attention_blocks_of_zeros_beside_others(loud, dtype):
     assert dtype is F16 or (out[0].abs() > 0).float().mean() > 0.99
 
 
+def test_attention_v_scales_far_apart():
+    """Blocks of zeros beside blocks of scales up to 2^29, within the 2^100 that the scales may
+    lie apart: what the blocks of zeros weigh is not lost."""
+    q, caches, scales, tables, sl = _inputs([400, 90], 3, 8, 2, 128, 16, BF16, E4M3, seed=15)
+    scales[1][tables[0, ::2].long()] = 0.0
+    scales[0][tables[0, ::2].long()] *= 4.0
+    scales[1][tables[0, 1::2].long()] *= 2.0 ** 32
+    want, bound, _ = ref.attention(q, *caches, *scales, tables, sl)
+    out = paged_attention_scaled(*_cuda(q, *caches, *scales, tables, sl))
+    ref.assert_within(out, want, bound)
+
+
 @pytest.mark.parametrize("layout", ["nhd", "hnd", "scales_together"])
 def test_attention_reads_views_by_their_strides(layout):
     q, caches, scales, tables, sl = _inputs([300, 77], 4, 8, 2, 64, 32, BF16, E4M3, seed=5)

@@ -226,7 +226,8 @@ void sqa_scaled_attention_kernel(ScaledArgs args) {
   const size_t sub_bytes = (size_t)kPageSize * tok_bytes;
   // Lanes 0-31 load the page's K scale, 32-63 its V scale: one instruction, one register.
   const char* scale_lane =
-      (const char*)(lane < 32 ? args.scales.k : args.scales.v) + kvh * args.scales.head_stride;
+      (const char*)(lane < 32 ? args.scales.k : args.scales.v) +
+      (size_t)kvh * args.scales.head_stride;
   struct Slot {
     typename KV::Regs kv;
     float scale;

@@ -272,3 +272,38 @@ def test_a_pool_past_32_bit_offsets():
         at = new.flatten().long().cuda()
         assert torch.equal(c.view(torch.uint8)[at].cpu(), w.view(torch.uint8))
         assert torch.equal(s[at].cpu(), ws)
+
+
+def test_scales_of_heads_past_32_bit_offsets():
+    """Scales whose heads lie 1 GiB apart: the upper heads' are past 4 GiB of the tensor, and
+    each operator reads (and writes) its own head's."""
+    hkv, d, page, far = 8, 64, 16, 1 << 28
+    lens = [90, 33]
+    q, caches, scales, tables, sl = _inputs(lens, 2, 16, hkv, d, page, F16, INT8, 60)
+    pages = scales[0].shape[0]
+    store = [torch.empty(hkv * far, device="cuda") for _ in range(2)]
+    ks, vs = (x.as_strided((pages, hkv), (1, far)) for x in store)
+    for x, s in zip((ks, vs), scales):
+        x.copy_(s)
+    qc, kc, vc, bt, slc = _cuda(q, *caches, tables, sl)
+    want, bound, mass = ref.attention(q, *caches, *scales, tables, sl)
+    ref.assert_within(scaled_cache.paged_attention_scaled(qc, kc, vc, ks, vs, bt, slc), want, bound)
+    weights = torch.zeros(2, hkv, 96, device="cuda")
+    eviction.accumulate_attention_weights(qc, kc, bt, slc, weights, key_scale=ks)
+    ref.assert_within(weights, *ref.weights_after(torch.zeros(2, hkv, 96), mass, sl, 2))
+    new_tables = torch.arange(4).view(2, 2).to(torch.int32)
+    into = [torch.zeros(4, page, hkv, d, dtype=INT8) for _ in range(2)]
+    into_s = [torch.zeros(4, hkv) for _ in range(2)]
+    gi = _cuda(*into)
+    gs = [x.as_strided((4, hkv), (1, far), pages) for x in store]
+    eviction.evict_by_weight(weights, kc, vc, bt, slc, new_tables.cuda(), 32, key_scale=ks,
+                             value_scale=vs, into=(*gi, *gs))
+    ref.evict(weights.cpu(), caches, scales, tables, sl, new_tables, 32, 0, 0, into, into_s)
+    assert _equal([x.cpu() for x in gi], into)
+    assert all(torch.equal(a.cpu(), b) for a, b in zip(gs, into_s))
+    g = torch.Generator().manual_seed(61)
+    key, value = (torch.randn(2, 3, hkv, d, generator=g).half() for _ in range(2))
+    scaled_cache.append_scaled_kv(*_cuda(key, value), kc, vc, ks, vs, bt, slc)
+    ref.append(key, value, caches, scales, tables, sl)
+    for a, b in zip((ks, vs), scales):
+        assert torch.equal(a.cpu().nan_to_num(), b.nan_to_num())

@@ -386,7 +386,8 @@ int sqa_attention_weights(const sqa_weights_args* args);
 
 /*
  * Arguments of sqa_evict (set struct_size = sizeof(sqa_evict_args)).
- *   weights       [batch, num_kv_heads, weights_width], of every token
+ *   weights       [batch, num_kv_heads, weights_width]; tokens at weights_width and past
+ *                 it weigh 0
  *   new_weights   [batch, num_kv_heads, new_weights_width >= budget]; may be `weights`,
  *                 not overlap it in another way
  *   kept          [batch, num_kv_heads, budget] int32, contiguous
@@ -435,7 +436,8 @@ typedef struct sqa_evict_args {
  * `sink`, the last `recent`, and the heaviest of those between (NaN the lightest; of equal
  * ones the earlier). They move in their order to the slots 0 .. of the new pages, their
  * positions before go to kept (-1 past them), their weights to new_weights (0 past them),
- * min(seq_lens[b], budget) to new_lens. Sequences within the budget move whole. In scaled
+ * min(seq_lens[b], budget) to new_lens (seq_lens[b] no more than the table row holds).
+ * Sequences within the budget move whole. In scaled
  * caches a new block's scale is the largest of those its tokens come from, and codes from
  * blocks of smaller scales are rounded again, code * old / new. Slots past a sequence's
  * end, and pages whose id is outside the pool, are not written.

@@ -451,37 +451,34 @@ constexpr int kSelectThreads = 1024, kSelectWaves = kSelectThreads / 64;
 // head, 126 registers a thread; 35 with the weights' keys made again each time, 59 from
 // memory), moves 60.
 
+struct SelectShared {
+  int hist[2048];
+  int wave_tot[kSelectWaves], wave_sure[kSelectWaves], wave_tie[kSelectWaves];
+  int picked, above;
+};
+
 // Which tokens of one sequence and kv head stay. The smallest key that stays is found by
 // a radix selection over the weights between the sink and the recent tokens (11, 11 and
 // 10 bits, histograms in LDS); tokens above it stay, and of those that equal it the first.
 // Each wave then counts its own run of tokens, and after one exchange writes its kept
 // tokens in order. All counts are integers: the same weights give the same tokens.
 // R > 0: a thread holds its R tokens' weights and keys in registers through all of it (up to
-// 1024 R tokens); R = 0 reads the weights again each time.
+// 1024 R tokens); R = 0 reads the weights again each time. Tokens past the weights' width
+// weigh 0.
 template <int R>
-__global__ __launch_bounds__(kSelectThreads) void sqa_select_kernel(EvictArgs a) {
-  __shared__ int hist[2048];
-  __shared__ int wave_tot[kSelectWaves], wave_sure[kSelectWaves], wave_tie[kSelectWaves];
-  __shared__ int picked, above;
-  const int b = blockIdx.x / a.hkv, h = blockIdx.x % a.hkv;
+__device__ __forceinline__ void select_tokens(const EvictArgs& a, SelectShared& sm, int n,
+                                              const float* w, float* nw, int32_t* kept) {
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const float* w = a.weights + b * a.w_batch + h * a.w_head;
-  float* nw = a.new_weights + b * a.nw_batch + h * a.nw_head;
-  int32_t* kept = a.kept + (size_t)(b * a.hkv + h) * a.budget;
-  const long long room = (long long)a.bt_stride * a.page_size;
-  const int n = (int)min((long long)min(max(a.seq_lens[b], 0), a.width), room);
-  const int m = min(n, a.budget);
-  if (h == 0 && tid == 0) a.new_lens[b] = m;
-  if (n <= a.budget) {
-    for (int j = tid; j < a.budget; j += kSelectThreads) kept[j] = j < n ? j : -1;
-    for (int j = tid; j < a.new_width; j += kSelectThreads) nw[j] = j < n ? w[j] : 0.f;
-    return;
-  }
+  const int m = a.budget, weighed = min(n, a.width);
   // A wave's run: `steps` times 64 consecutive tokens.
   const int steps = (n + kSelectThreads - 1) / kSelectThreads;
   const int begin = wave * steps * 64;
   const int lo = a.sink, hi = n - a.recent;
+  auto weight_at = [&](int t) {
+    const float x = w[min(t, weighed - 1)];
+    return t < weighed ? x : 0.f;
+  };
   auto key_at = [&](int t, float x) {
     const unsigned k = t >= lo && t < hi ? weight_key(x) : kAlways;
     return t < n ? k : 0u;
@@ -491,7 +488,7 @@ __global__ __launch_bounds__(kSelectThreads) void sqa_select_kernel(EvictArgs a)
   unsigned held[kHeld];
   if constexpr (R > 0) {
 #pragma unroll
-    for (int i = 0; i < R; ++i) held_w[i] = i < steps ? w[min(begin + 64 * i + lane, n - 1)] : 0.f;
+    for (int i = 0; i < R; ++i) held_w[i] = i < steps ? weight_at(begin + 64 * i + lane) : 0.f;
 #pragma unroll
     for (int i = 0; i < R; ++i) held[i] = key_at(begin + 64 * i + lane, held_w[i]);
   }
@@ -504,7 +501,7 @@ __global__ __launch_bounds__(kSelectThreads) void sqa_select_kernel(EvictArgs a)
     } else {
       for (int i = 0; i < steps; ++i) {
         const int t = begin + 64 * i + lane;
-        const float x = w[min(t, n - 1)];
+        const float x = weight_at(t);
         f(t, key_at(t, x), x);
       }
     }
@@ -518,30 +515,30 @@ __global__ __launch_bounds__(kSelectThreads) void sqa_select_kernel(EvictArgs a)
     for (int pass = 0; pass < 3; ++pass) {
       const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0);
       const unsigned digits = pass == 2 ? 0x3ffu : 0x7ffu;
-      for (int i = tid; i < 2048; i += kSelectThreads) hist[i] = 0;
+      for (int i = tid; i < 2048; i += kSelectThreads) sm.hist[i] = 0;
       __syncthreads();
       each([&](int, unsigned k, float) {
         if (k - 1u < kAlways - 1u && (k & mask) == prefix)
-          atomicAdd(&hist[(k >> shift) & digits], 1);
+          atomicAdd(&sm.hist[(k >> shift) & digits], 1);
       });
       __syncthreads();
       // Bins from the top: thread i takes bins 2047 - 2 i and 2046 - 2 i.
-      const int c0 = hist[2047 - 2 * tid], c1 = hist[2046 - 2 * tid];
+      const int c0 = sm.hist[2047 - 2 * tid], c1 = sm.hist[2046 - 2 * tid];
       const int incl = wave_inclusive_scan_int(c0 + c1);
-      if (lane == 63) wave_tot[wave] = incl;
+      if (lane == 63) sm.wave_tot[wave] = incl;
       __syncthreads();
       int before = incl - c0 - c1;
 #pragma unroll
-      for (int i = 0; i < kSelectWaves; ++i) before += i < wave ? wave_tot[i] : 0;
+      for (int i = 0; i < kSelectWaves; ++i) before += i < wave ? sm.wave_tot[i] : 0;
       if (before < want && want <= before + c0 + c1) {  // one thread
         const bool first = want <= before + c0;
-        picked = first ? 2047 - 2 * tid : 2046 - 2 * tid;
-        above = first ? before : before + c0;
+        sm.picked = first ? 2047 - 2 * tid : 2046 - 2 * tid;
+        sm.above = first ? before : before + c0;
       }
       __syncthreads();
-      prefix |= (unsigned)picked << shift;
+      prefix |= (unsigned)sm.picked << shift;
       mask |= digits << shift;
-      want -= above;
+      want -= sm.above;
     }
     threshold = prefix;
     ties = want;
@@ -552,15 +549,15 @@ __global__ __launch_bounds__(kSelectThreads) void sqa_select_kernel(EvictArgs a)
     tied += __popcll(__ballot(k == threshold));
   });
   if (lane == 0) {
-    wave_sure[wave] = sures;
-    wave_tie[wave] = tied;
+    sm.wave_sure[wave] = sures;
+    sm.wave_tie[wave] = tied;
   }
   __syncthreads();
   int at = 0, seen = 0;  // kept tokens and ties before this wave's
 #pragma unroll
   for (int i = 0; i < kSelectWaves; ++i) {
-    at += i < wave ? wave_sure[i] : 0;
-    seen += i < wave ? wave_tie[i] : 0;
+    at += i < wave ? sm.wave_sure[i] : 0;
+    seen += i < wave ? sm.wave_tie[i] : 0;
   }
   at = __builtin_amdgcn_readfirstlane(at + min(seen, ties));
   seen = __builtin_amdgcn_readfirstlane(seen);
@@ -589,11 +586,34 @@ __global__ __launch_bounds__(kSelectThreads) void sqa_select_kernel(EvictArgs a)
     // never moves to a later position.
     for (int j0 = 0; j0 < a.new_width; j0 += kSelectThreads) {
       const int j = j0 + tid;
-      const float x = j < m ? w[kept[j]] : 0.f;
+      const int t = j < m ? kept[j] : weighed;
+      const float x = t < weighed ? w[t] : 0.f;
       __syncthreads();
       if (j < a.new_width) nw[j] = x;
       __syncthreads();
     }
+  }
+}
+
+template <int R>
+__global__ __launch_bounds__(kSelectThreads) void sqa_select_kernel(EvictArgs a) {
+  __shared__ SelectShared sm;
+  const int b = blockIdx.x / a.hkv, h = blockIdx.x % a.hkv;
+  const int tid = threadIdx.x;
+  const float* w = a.weights + b * a.w_batch + h * a.w_head;
+  float* nw = a.new_weights + b * a.nw_batch + h * a.nw_head;
+  int32_t* kept = a.kept + (size_t)(b * a.hkv + h) * a.budget;
+  const long long room = (long long)a.bt_stride * a.page_size;
+  const int n = (int)min((long long)max(a.seq_lens[b], 0), room);
+  if (h == 0 && tid == 0) a.new_lens[b] = min(n, a.budget);
+  if (n <= a.budget) {
+    const int weighed = min(n, a.width);
+    for (int j = tid; j < a.budget; j += kSelectThreads) kept[j] = j < n ? j : -1;
+    for (int j = tid; j < a.new_width; j += kSelectThreads) nw[j] = j < weighed ? w[j] : 0.f;
+  } else if (n <= R * kSelectThreads) {
+    select_tokens<R>(a, sm, n, w, nw, kept);
+  } else {
+    select_tokens<0>(a, sm, n, w, nw, kept);
   }
 }
 
@@ -764,6 +784,8 @@ hipError_t launch_weigh(const WeighArgs& a, hipStream_t stream) {
 
 hipError_t launch_evict(const EvictArgs& a, hipStream_t stream) {
   const dim3 each((unsigned)(a.batch * a.hkv)), threads(kSelectThreads);
+  // Sequences are hardly longer than their weights are wide; one that is takes the form
+  // without registers where it does not fit them.
   const long long most = std::min((long long)a.width, (long long)a.bt_stride * a.page_size);
   if (most <= 4 * kSelectThreads)
     hipLaunchKernelGGL((sqa_select_kernel<4>), each, threads, 0, stream, a);

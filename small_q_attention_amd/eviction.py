@@ -193,9 +193,13 @@ def evict_by_weight(weights, key_cache, value_cache, block_tables, seq_lens, new
     ``(key_cache, value_cache)`` of the same type, page size and heads, with
     ``(..., key_scale, value_scale)`` for scaled ones. In scaled caches a new block takes the
     largest scale among the blocks its tokens come from, and codes of other blocks are
-    rounded again. ``weights`` may be written in place: ``new_weights=weights`` (a buffer that
-    overlaps it in another way may not be given); ``None`` returns new ones, ``[B, Hkv, budget]``. ``T`` and the table bound the lengths that are
-    looked at.
+    rounded again. Tokens from ``T`` on weigh 0 (the last ``recent`` stay all the same); lengths
+    past the table's width are held to it.
+
+    ``weights`` may be written in place: ``new_weights=weights`` (a buffer that overlaps it in
+    another way may not be given); ``None`` returns new ones, ``[B, Hkv, budget]``: no wider
+    than what is kept, so a loop that goes on to add up the weights of later tokens gives a
+    buffer with room for them.
 
     Returns ``(new_lens [B] int32, new_weights, kept [B, Hkv, budget] int32)``: the lengths
     ``min(seq_lens, budget)``, the moved weights (0 past them) and the positions the tokens

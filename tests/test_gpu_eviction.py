@@ -318,3 +318,68 @@ def test_a_decoding_loop(kv):
         ref.assert_within(out, want, bound, f"step {step}")
         want, bound = ref.weights_after(old, mass, lens, q_len)
         ref.assert_within(weights, want, bound, f"step {step}")
+
+
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("lens,width,budget,sink,recent", [
+    ([300, 64, 65, 5, 0], 64, 40, 3, 9),         # the recent tokens lie past the weights
+    ([300, 120], 10, 100, 20, 7),                # so does the sink, and the budget
+    ([500, 77], 1, 1, 0, 1),
+    ([200, 3], 64, 64, 0, 0),                    # all weights fit, later tokens weigh 0
+    ([9001, 4097, 4000, 12], 4000, 1000, 4, 100),  # longer than the registers' form holds
+    ([70000, 33000], 33000, 5000, 4, 800),
+])
+def test_evict_sequences_longer_than_their_weights(lens, width, budget, sink, recent, in_place):
+    """Tokens the weights do not reach weigh 0; the first and last ones stay as ever."""
+    if in_place and width < budget:
+        pytest.skip("the buffer holds no new weights")
+    case = list(_evict_case(lens, 2, 64, 16, E4M3, budget, seed=width, ties=width % 2 == 0))
+    full = case[0]
+    full[:, :, width:] = 0.0
+    # Weights below 0 rank behind the tokens that have none.
+    full[:, :, :width:5] *= -1.0
+    case[0] = full[:, :, :width].contiguous()
+    got = _evict_narrow(case, budget, sink, recent, in_place)
+    want = ref.evict(full, *case[1:6], budget, sink, recent, *case[6:])
+    assert torch.equal(got[0], want[0]) and torch.equal(got[2], want[2])
+    assert torch.equal(got[1][:, :, :budget], want[1]) and (got[1][:, :, budget:] == 0).all()
+    for a, b in zip(got[3:], (*case[6], *case[7])):
+        assert _same(a, b) or torch.equal(a, b)
+
+
+def _evict_narrow(case, budget, sink, recent, in_place):
+    weights, caches, scales, tables, sl, new_tables, into, into_scales = case
+    w, ks, vs, bt, slc, nt, *moved = _cuda(weights, *scales, tables, sl, new_tables, *into,
+                                           *into_scales)
+    lens, nw, kept = evict_by_weight(w, *_cuda(*caches), bt, slc, nt, budget, sink=sink,
+                                     recent=recent, key_scale=ks, value_scale=vs,
+                                     into=tuple(moved), new_weights=w if in_place else None)
+    return [x.cpu() for x in (lens, nw, kept, *moved)]
+
+
+def test_evictions_in_turn_without_a_buffer_for_the_weights():
+    """The weights that an eviction returns are as wide as its budget: of the tokens decoded
+    after it the recent ones stay, whatever the weights do not say of them."""
+    g = torch.Generator().manual_seed(12)
+    b, hkv, d, page, budget, recent = 2, 2, 64, 16, 48, 20
+    pool = torch.randn(64, page, hkv, d, generator=g).half()
+    caches = [pool.cuda(), (pool * 2).cuda()]
+    tables = torch.arange(2 * 8).view(2, 8).to(torch.int32)
+    weights, lens = torch.rand(b, hkv, 128, generator=g), torch.tensor([120, 70], dtype=torch.int32)
+    for step in range(3):
+        new = (16 + 16 * step + torch.arange(2 * 8)).view(2, 8).to(torch.int32)
+        full = torch.zeros(b, hkv, 128)
+        full[:, :, :weights.shape[2]] = weights
+        mine = [c.cpu() for c in caches]
+        got = evict_by_weight(weights.cuda(), *caches, *_cuda(tables, lens, new), budget, sink=2,
+                              recent=recent)
+        want = ref.evict(full, mine, None, tables, lens, new, budget, 2, recent, mine, None)
+        for a, w in zip(got, want):
+            assert torch.equal(a.cpu(), w)
+        for a, w in zip(caches, mine):
+            assert _same(a, w)
+        assert got[1].shape[2] == budget
+        kept = got[2].cpu()
+        assert (kept[:, :, -recent:] == lens[:, None, None] - recent + torch.arange(recent)).all()
+        weights, tables, lens = got[1].cpu(), new, got[0].cpu() + torch.tensor([30, 17])
+        lens = lens.to(torch.int32)

@@ -396,7 +396,7 @@ int sqa_attention_weights(const sqa_weights_args* args);
  *   into, into_scales  where they go, pages new_tables [batch, new_max_pages]; may be the
  *                 same pool, on pages no row of block_tables uses, each once; into.k and
  *                 into.v differ, as do their scales
- *   new_lens      [batch], written
+ *   new_lens      [batch], written; not seq_lens, nor overlapping them
  * Strides of kv and into must be multiples of 16 bytes.
  */
 typedef struct sqa_evict_args {

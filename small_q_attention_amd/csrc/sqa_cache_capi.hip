@@ -525,6 +525,11 @@ int sqa_evict(const sqa_evict_args* args) {
 
   if (a.into.k == a.into.v || (scaled && a.into_scales.k == a.into_scales.v))
     return fail(SQA_ERR_INVALID, "keys and values are written: each needs its own cache and scales");
+  // Workgroups of other heads may read a length after the first one has written the new one.
+  const uintptr_t old_lens = (uintptr_t)a.seq_lens, new_lens = (uintptr_t)a.new_lens;
+  const uintptr_t lens_bytes = sizeof(int32_t) * (uintptr_t)a.batch;
+  if (old_lens < new_lens + lens_bytes && new_lens < old_lens + lens_bytes)
+    return fail(SQA_ERR_INVALID, "new_lens must not overlap seq_lens");
   sqa::EvictArgs k;
   memset(&k, 0, sizeof(k));
   k.weights = a.weights;

@@ -325,6 +325,35 @@ def test_evict_needs_a_cache_each_for_keys_and_values(lib, change):
     assert b"own cache" in lib.sqa_last_error()
 
 
+def _evict_args(**kw):
+    """Arguments of an sqa_evict call with nothing to refuse."""
+    pool = dict(k=1 << 16, v=1 << 17, num_pages=6, page_stride=2048, token_stride=128, head_stride=64)
+    sc = dict(k=1 << 18, v=1 << 19, page_stride=2, head_stride=1)
+    return _fill(_lib.EvictArgs, **{**dict(
+        weights=1 << 20, weights_batch_stride=128, weights_head_stride=64, new_weights=2 << 20,
+        new_weights_batch_stride=40, new_weights_head_stride=20, kept=3 << 20, seq_lens=4 << 20,
+        new_lens=5 << 20, block_tables=6 << 20, new_tables=7 << 20, weights_width=64,
+        new_weights_width=20, max_pages=4, new_max_pages=2, budget=20, sink=2, recent=3, batch=2,
+        num_kv_heads=2, head_dim=64, page_size=16, kv_dtype=2,
+        **{f"kv__{k}": v for k, v in pool.items()}, **{f"into__{k}": v for k, v in pool.items()},
+        **{f"scales__{k}": v for k, v in sc.items()},
+        **{f"into_scales__{k}": v for k, v in sc.items()}), **kw})
+
+
+# No test below reaches a launch where there is a GPU: made-up pointers must not get there.
+without_gpu = pytest.mark.skipif(torch.cuda.is_available(), reason="passes made-up pointers on")
+
+
+@without_gpu
+@pytest.mark.parametrize("by", [0, 4, -4])
+def test_evict_lengths_are_not_written_over(lib, by):
+    a = _evict_args(new_lens=(4 << 20) + by)
+    assert lib.sqa_evict(ctypes.byref(a)) == INVALID
+    assert b"new_lens must not overlap" in lib.sqa_last_error()
+    a = _evict_args(new_lens=(4 << 20) + 2 * by + (8 if by == 0 else 0))  # beside them
+    assert lib.sqa_evict(ctypes.byref(a)) == 4
+
+
 # ----- the traced ops -----
 
 @pytest.mark.parametrize("name,writes", [

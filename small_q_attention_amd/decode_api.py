@@ -364,7 +364,13 @@ class _PagedWrapper:
             plan = _lib.plan_splits(device.index or 0, batch, q_len, num_qo_heads, num_kv_heads,
                                     head_dim, max(max_seq_len, 1),
                                     block_tables.shape[1] * (page_size // PAGE_SIZE), 0)
-        need = _lib.workspace_bytes(batch, q_len, num_qo_heads, num_kv_heads, head_dim, *plan)
+        # A run over block scales has a plan of its own (scaled_cache).
+        slots = _lib.plan_scaled(device.index or 0, batch, num_kv_heads, max_seq_len,
+                                 block_tables.shape[1] * (page_size // PAGE_SIZE))
+        scaled_need = _lib.workspace_bytes(batch, q_len, num_qo_heads, num_kv_heads, head_dim,
+                                           slots, 0)
+        need = scaled_need if kv_data_type in int8 else _lib.workspace_bytes(
+            batch, q_len, num_qo_heads, num_kv_heads, head_dim, *plan)
         if need and self._workspace is not None:
             have = self._workspace.numel() * self._workspace.element_size()
             if have < need:
@@ -374,6 +380,7 @@ class _PagedWrapper:
                              q_len=q_len, hq=num_qo_heads, hkv=num_kv_heads,
                              max_seq_len=max_seq_len, mask_words=mask_words,
                              page_size=page_size, head_dim=head_dim,
+                             scaled_need=scaled_need,
                              scale=head_dim ** -0.5 if sm_scale is None else float(sm_scale))
 
     def _graph_plan(self, shape, block_tables, seq_lens, mask_words, device):
@@ -413,7 +420,9 @@ class _PagedWrapper:
         scale, ``v_scale`` the output (per-tensor FP8 scales); ``enable_pdl`` is a
         launch hint and has no effect here. ``lse``/``return_lse``, sliding windows,
         sinks, extra positional arguments and unknown keywords raise ``ValueError``.
-        ``kv_block_scales``: as for :func:`xqa_batch_decode_with_kv_cache`."""
+        ``kv_block_scales``: as for :func:`xqa_batch_decode_with_kv_cache`; a workspace buffer
+        that holds the partials of ``plan()``'s type but not of this call (codes planned as
+        int8 are always checked for it) is left aside for one of torch's allocator."""
         if args:
             raise ValueError("run() takes (q, paged_kv_cache) positionally; pass the rest "
                              "by keyword")
@@ -447,9 +456,12 @@ class _PagedWrapper:
             raise ValueError(f"kv_cache pages hold {k.shape[1]} tokens, plan() was given "
                              f"{p['page_size']}")
         if kv_block_scales is not None:
+            ws = self._workspace
+            if ws is not None and ws.numel() * ws.element_size() < p["scaled_need"]:
+                ws = None
             return _run_scaled(q, k, v, kv_block_scales, p["block_tables"], p["seq_lens"],
                                p["max_seq_len"], p["q_len"], scale, out_scale, p["mask_words"],
-                               self._workspace, out)
+                               ws, out)
         return _run(q, k, v, p["block_tables"], p["seq_lens"], p["max_seq_len"], p["q_len"],
                     scale, out_scale, p["mask_words"], self._workspace, out, plan=p["plan"])
 

@@ -94,3 +94,34 @@ def test_run_checks_every_pointer_argument_for_the_device():
     q, kv, _, bt, sl, msl, s1, s2 = _args()
     with pytest.raises(ValueError, match="GPU"):
         fi.xqa_batch_decode_with_kv_cache(q, kv, None, bt, sl, msl, s1, s2, q_len_per_req=4)
+
+
+def test_plans_check_the_workspace_of_the_runs_they_serve(monkeypatch):
+    """int8 caches run over block scales only, whose plan has a workspace of its own; an e4m3
+    plan serves runs with and without them, and refuses what it refused without."""
+    from small_q_attention_amd import _lib
+
+    indptr = torch.tensor([0, 4, 8], dtype=torch.int32)
+    ids = torch.arange(8, dtype=torch.int32)
+    last = torch.tensor([16, 16], dtype=torch.int32)
+
+    def plan(nbytes, kv, ordinary, slots):
+        monkeypatch.setattr(_lib, "plan_splits", lambda *a: ordinary)
+        monkeypatch.setattr(_lib, "plan_scaled", lambda *a: slots)
+        w = fi.BatchDecodeWithPagedKVCacheWrapper(torch.zeros(nbytes, dtype=torch.uint8), "NHD")
+        w.plan(indptr, ids, last, 8, 2, 64, 16, kv_data_type=kv, q_len_per_req=2)
+        return w
+
+    one, many = (1, 4), (8, 1)  # no workspace, and one for eight splits
+    assert _lib.workspace_bytes(2, 2, 8, 2, 64, *one) == 0
+    scaled = _lib.workspace_bytes(2, 2, 8, 2, 64, 2, 0)
+    more = _lib.workspace_bytes(2, 2, 8, 2, 64, *many)
+    assert 0 < scaled < more
+    for kv in (torch.int8, "int8"):
+        with pytest.raises(ValueError, match="float_workspace_buffer"):
+            plan(scaled - 1, kv, one, 2)
+        plan(scaled, kv, many, 2)
+    for kv in (torch.float8_e4m3fn, None):
+        plan(16, kv, one, 2)
+        with pytest.raises(ValueError, match="float_workspace_buffer"):
+            plan(more - 1, kv, many, 2)

@@ -307,3 +307,32 @@ def test_scales_of_heads_past_32_bit_offsets():
     ref.append(key, value, caches, scales, tables, sl)
     for a, b in zip((ks, vs), scales):
         assert torch.equal(a.cpu().nan_to_num(), b.nan_to_num())
+
+
+def test_a_wrapper_whose_workspace_fits_one_plan_only():
+    """A buffer large enough for the ordinary plan of a short sequence (none at all) serves
+    runs over block scales too, captured ones among them; an int8 plan asks for its own."""
+    q, caches, scales, tables, sl = _inputs([60], 2, 8, 2, 128, 16, F16, E4M3, 33)
+    pool = tuple(_cuda(*caches))
+    qc, ks, vs = _cuda(q.view(2, 8, 128), *scales)
+    csr = _cuda(torch.tensor([0, 4], dtype=torch.int32), tables[0, :4].contiguous(),
+                torch.tensor([12], dtype=torch.int32))
+    ws = torch.zeros(16, dtype=torch.uint8, device="cuda")
+    want, bound, _ = ref.attention(q, *caches, *scales, tables, sl)
+    w = decode_api.BatchDecodeWithPagedKVCacheWrapper(ws, "NHD")
+    w.plan(*csr, 8, 2, 128, 16, q_data_type=F16, kv_data_type=E4M3, q_len_per_req=2)
+    ref.assert_within(w.run(qc, pool, kv_block_scales=(ks, vs)).view(q.shape), want, bound)
+    w.run(qc, pool)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = w.run(qc, pool, kv_block_scales=(ks, vs))
+    for _ in range(3):
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        ref.assert_within(out.view(q.shape), want, bound)
+        w.run(qc, pool, kv_block_scales=(ks, vs))
+    assert (ws == 0).all()
+    with pytest.raises(ValueError, match="float_workspace_buffer"):
+        w.plan(*csr, 8, 2, 128, 16, q_data_type=F16, kv_data_type=INT8, q_len_per_req=2)

@@ -354,6 +354,91 @@ def test_evict_lengths_are_not_written_over(lib, by):
     assert lib.sqa_evict(ctypes.byref(a)) == 4
 
 
+def _append_args(**kw):
+    """Arguments of an sqa_append_scaled call with nothing to refuse."""
+    a = _fill(_lib.AppendArgs, **{**dict(
+        key=1 << 16, value=1 << 17, kv__k=1 << 18, kv__v=1 << 19, kv__num_pages=6,
+        kv__page_stride=2048, kv__token_stride=128, kv__head_stride=64, scales__k=1 << 20,
+        scales__v=2 << 20, scales__page_stride=2, scales__head_stride=1, block_tables=3 << 20,
+        seq_lens=4 << 20, max_pages=4, batch=2, q_len=3, num_kv_heads=2, head_dim=64, page_size=16,
+        dtype=0, kv_dtype=2), **{k: v for k, v in kw.items() if not k.endswith("_strides")}})
+    a.key_strides[:] = kw.get("key_strides", (384, 128, 64))
+    a.value_strides[:] = kw.get("value_strides", (384, 128, 64))
+    return a
+
+
+# Each row changes one thing of a call that is otherwise taken, so its message names the
+# check it is about.
+
+@without_gpu
+@pytest.mark.parametrize("change,status,message", [
+    (dict(), 4, ""),
+    (dict(struct_size=8), INVALID, "struct_size"), (dict(key=None), INVALID, "null tensor"),
+    (dict(value=None), INVALID, "null tensor"), (dict(kv__v=None), INVALID, "null tensor"),
+    (dict(block_tables=None), INVALID, "null tensor"), (dict(seq_lens=None), INVALID, "null tensor"),
+    (dict(key=(1 << 16) + 8), INVALID, "16-byte"), (dict(value=(1 << 17) + 2), INVALID, "16-byte"),
+    (dict(batch=0), INVALID, "batch"), (dict(q_len=0), INVALID, "q_len"),
+    (dict(dtype=3), UNSUPPORTED, "dtype"), (dict(kv_dtype=1), UNSUPPORTED, "kv_dtype"),
+    (dict(scales__k=None), INVALID, "null scale"), (dict(scales__v=None), INVALID, "null scale"),
+    (dict(scales__k=(1 << 20) + 2), INVALID, "scales must be 4-byte"),
+    (dict(scales__page_stride=-1), INVALID, "scale strides"),
+    (dict(scales__head_stride=1 << 30), INVALID, "scale strides"),
+    (dict(new_lens=4097), INVALID, "new_lens"), (dict(seq_lens=4098), INVALID, "seq_lens"),
+    (dict(block_tables=4098), INVALID, "block_tables"), (dict(page_size=8), UNSUPPORTED, "page_size"),
+    (dict(kv__v=(1 << 19) + 4), INVALID, "base pointers"), (dict(max_pages=0), INVALID, "empty"),
+    (dict(kv__num_pages=1 << 31), INVALID, "32 bits"), (dict(max_pages=1 << 26), INVALID, "2^30"),
+    (dict(head_dim=32), UNSUPPORTED, "head_dim"), (dict(kv__page_stride=-8), INVALID, "cache strides"),
+    (dict(kv__head_stride=4), INVALID, "cache strides"),
+    (dict(kv__token_stride=1 << 31), INVALID, "too large"),
+    (dict(kv__token_stride=1 << 29), INVALID, "2 GiB"),
+    (dict(key_strides=(384, 4, 64)), INVALID, "key and value strides"),
+    (dict(value_strides=(384, 128, -64)), INVALID, "key and value strides"),
+    (dict(kv__v=1 << 18), INVALID, "own cache"), (dict(scales__v=1 << 20), INVALID, "own cache"),
+    (dict(batch=1 << 15, q_len=1 << 20, num_kv_heads=1 << 14, max_pages=1 << 14,
+          kv__head_stride=64), INVALID, "grid"),
+])
+def test_each_refusal_of_an_append(lib, change, status, message):
+    assert lib.sqa_append_scaled(ctypes.byref(_append_args(**change))) == status
+    assert message in lib.sqa_last_error().decode()
+
+
+@without_gpu
+@pytest.mark.parametrize("change,status,message", [
+    (dict(), 4, ""),
+    (dict(struct_size=8), INVALID, "struct_size"), (dict(weights=None), INVALID, "null tensor"),
+    (dict(new_weights=None), INVALID, "null tensor"), (dict(kept=None), INVALID, "null tensor"),
+    (dict(new_lens=None), INVALID, "null tensor"), (dict(new_tables=None), INVALID, "null tensor"),
+    (dict(into__v=None), INVALID, "null tensor"),
+    (dict(kept=(3 << 20) + 1), INVALID, "4-byte aligned"),
+    (dict(weights=(1 << 20) + 2), INVALID, "4-byte aligned"),
+    (dict(new_tables=(7 << 20) + 2), INVALID, "4-byte aligned"),
+    (dict(batch=0), INVALID, "batch"), (dict(kv__num_pages=0), INVALID, "empty"),
+    (dict(into__num_pages=0), INVALID, "empty"), (dict(max_pages=0), INVALID, "empty"),
+    (dict(new_max_pages=0), INVALID, "empty"), (dict(head_dim=96), UNSUPPORTED, "head_dim"),
+    (dict(page_size=24), UNSUPPORTED, "page_size"), (dict(kv_dtype=4), UNSUPPORTED, "kv_dtype"),
+    (dict(budget=0), INVALID, "budget must be positive"), (dict(sink=-1), INVALID, "budget must be"),
+    (dict(recent=-1), INVALID, "budget must be"), (dict(sink=18), INVALID, "budget must be"),
+    (dict(budget=33, new_weights_width=33), INVALID, "new_tables rows hold"),
+    (dict(new_weights_width=19), INVALID, "new_weights hold"),
+    (dict(weights_width=0), INVALID, "must not be empty"),
+    (dict(weights_head_stride=-1), INVALID, "not be negative"),
+    (dict(new_weights_batch_stride=-1), INVALID, "not be negative"),
+    (dict(kv_dtype=3, scales__k=None), INVALID, "int8 caches need scales"),
+    (dict(kv_dtype=0), INVALID, "scales belong"), (dict(scales__v=None), INVALID, "null scale"),
+    (dict(into_scales__k=None), INVALID, "null scale"),
+    (dict(into_scales__head_stride=-1), INVALID, "scale strides"),
+    (dict(kv__head_stride=72), INVALID, "16 bytes"), (dict(into__page_stride=2056), INVALID, "16 bytes"),
+    (dict(kv__token_stride=4), INVALID, "multiples of 8"),
+    (dict(into__k=(1 << 16) + 4), INVALID, "base pointers"),
+    (dict(into__v=1 << 16), INVALID, "own cache"), (dict(into_scales__v=1 << 18), INVALID, "own cache"),
+    (dict(new_lens=4 << 20), INVALID, "overlap"),
+    (dict(batch=1 << 16, num_kv_heads=1 << 16, max_pages=1, new_max_pages=2), INVALID, "grid"),
+])
+def test_each_refusal_of_an_eviction(lib, change, status, message):
+    assert lib.sqa_evict(ctypes.byref(_evict_args(**change))) == status
+    assert message in lib.sqa_last_error().decode()
+
+
 # ----- the traced ops -----
 
 @pytest.mark.parametrize("name,writes", [

@@ -467,12 +467,20 @@ def run(query, key_cache, value_cache, block_tables, seq_lens, num_splits: int,
     return out
 
 
-# Workspaces kept per (device, stream) for eager calls: a stream runs its calls in
-# order, so one buffer serves them all and the per-call allocation is saved.
-# Plans past WORKSPACE_CACHE_BYTES, and calls under graph capture (whose buffers
-# belong to the graph's pool), allocate their own.
+# Workspaces kept per host thread, device and stream for eager calls: a stream runs a
+# thread's calls in order, so one buffer serves them all and the per-call allocation is
+# saved. Each thread has its own: a call is two kernels, and between those of one thread
+# another's may be launched on the same stream. Plans past WORKSPACE_CACHE_BYTES, and calls
+# under graph capture (whose buffers belong to the graph's pool), allocate their own.
 WORKSPACE_CACHE_BYTES = 64 << 20
-_WORKSPACES = {}
+
+
+class _Workspaces(threading.local):
+    def __init__(self):
+        self.of = {}
+
+
+_WORKSPACES = _Workspaces()
 _CUDA_STATE = None  # (current device, current stream capturing): torch's own query functions
 
 
@@ -501,10 +509,11 @@ def workspace_for(nbytes: int, like, device_index: int, stream_handle: int):
     if nbytes > WORKSPACE_CACHE_BYTES or device_index != current_device() or capturing():
         return torch.empty(nbytes, dtype=torch.uint8, device=like.device)
     key = (device_index, stream_handle)
-    ws = _WORKSPACES.get(key)
+    mine = _WORKSPACES.of
+    ws = mine.get(key)
     if ws is None or ws.numel() < nbytes:
         ws = torch.empty(max(nbytes, 1 << 20), dtype=torch.uint8, device=like.device)
-        _WORKSPACES[key] = ws
+        mine[key] = ws
     return ws
 
 

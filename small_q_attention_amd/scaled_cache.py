@@ -277,8 +277,8 @@ def paged_attention_scaled(query, key_cache, value_cache, key_scale, value_scale
     (``None``: ``D ** -0.5``), ``out_scale`` multiplies the output. V blocks of a scale under
     2^-64 count as zeros; the V scales of what a row sees, those of zeros taken as 2^-64, may
     lie a factor of 2^100 apart. ``workspace_buffer``: a caller's buffer for the split
-    partials; ``None`` takes one kept per stream, or, under graph capture, one of the graph's
-    own. Returns ``out`` (``[B, Q, Hq, D]``).
+    partials; ``None`` takes one kept per host thread and stream, or, under graph capture, one
+    of the graph's own. Returns ``out`` (``[B, Q, Hq, D]``).
     """
     if query.dim() != 4:
         raise ValueError("query must be a contiguous [B, Q, Hq, D] tensor")

@@ -336,3 +336,45 @@ def test_a_wrapper_whose_workspace_fits_one_plan_only():
     assert (ws == 0).all()
     with pytest.raises(ValueError, match="float_workspace_buffer"):
         w.plan(*csr, 8, 2, 128, 16, q_data_type=F16, kv_data_type=INT8, q_len_per_req=2)
+
+
+def test_host_threads_on_one_stream():
+    """Two threads' calls on the default stream, their kernels launched between each other's:
+    the bits of the calls made alone."""
+    import threading
+
+    lens = ((2500, 77, 513), (300, 1900, 40))
+    states = [_state(70 + i, (300, 77, 513)) for i in range(2)]
+    for s, n in zip(states, lens):  # long enough for several splits of a sequence
+        s["tables"] = s["tables"].repeat(1, 5)[:, :160].contiguous()
+        s["lens"].copy_(torch.tensor(n, dtype=torch.int32))
+
+    def call(s):
+        w = torch.zeros(3, 2, 2600, device="cuda")
+        out = scaled_cache.paged_attention_scaled(*[s[k] for k in (
+            "query", "k", "v", "ks", "vs", "tables", "lens")])
+        eviction.accumulate_attention_weights(s["query"], s["k"], s["tables"], s["lens"], w,
+                                              key_scale=s["ks"])
+        return out, w
+
+    want = [call(s) for s in states]
+    torch.cuda.synchronize()
+    got, errors, start = [[], []], [], threading.Barrier(2)
+
+    def worker(i):
+        try:
+            start.wait()
+            for _ in range(20):
+                got[i].append(call(states[i]))
+        except Exception as exc:  # reported by the main thread
+            errors.append(repr(exc))
+
+    threads = [threading.Thread(target=worker, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(timeout=60)
+    assert not any(t.is_alive() for t in threads) and not errors, errors
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert len(got[i]) == 20 and all(_equal(g, want[i]) for g in got[i])

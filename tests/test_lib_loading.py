@@ -89,3 +89,29 @@ def test_source_edit_changes_the_hash(monkeypatch, tmp_path):
     before = _build.source_hash()
     src.write_bytes(src.read_bytes() + b"\n// edit\n")
     assert _build.source_hash() != before
+
+
+def test_workspaces_of_host_threads_are_apart(monkeypatch):
+    """Two threads on one stream: the merge of one call may follow the other's first kernel,
+    so each thread has a buffer of its own, and keeps it from call to call."""
+    import threading
+
+    import torch
+
+    monkeypatch.setattr(_lib, "_CUDA_STATE", (lambda: 0, lambda: False))
+    monkeypatch.setattr(_lib, "_WORKSPACES", type(_lib._WORKSPACES)())
+    like = torch.zeros(1)
+    mine = _lib.workspace_for(4096, like, 0, 1234)
+    assert _lib.workspace_for(2048, like, 0, 1234) is mine
+    assert _lib.workspace_for(2048, like, 0, 1235) is not mine
+    others = []
+
+    def worker():
+        others.append(_lib.workspace_for(4096, like, 0, 1234))
+        others.append(_lib.workspace_for(4096, like, 0, 1234))
+
+    t = threading.Thread(target=worker)
+    t.start()
+    t.join()
+    assert others[0] is others[1] and others[0].data_ptr() != mine.data_ptr()
+    assert _lib.workspace_for(4096, like, 0, 1234) is mine

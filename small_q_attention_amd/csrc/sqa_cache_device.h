@@ -37,8 +37,10 @@ __device__ __forceinline__ int ceil_quotient(int n, int d, float inv) {
 // The cut of the batch into work items, found by every wave for itself from the lengths:
 // sequence b takes n_b = max(1, ceil(pages_b / P)) items of nearly equal size, with P the
 // smallest page count of at least kMinSplitPages for which they sum to at most `items`
-// (or P the longest sequence, one item each, where the batch has more sequences than
-// that). All items are resident at once, so the longest, P pages, sets the time.
+// (or P the longest sequence, one item each, where the batch has as many sequences as
+// that or more). Up to there all items are resident at once, and the longest, P pages,
+// sets the time: batches near the number of items, and past it, are cut unevenly or not
+// at all.
 // Returns whether item `item` exists; `table` (one wave of the grid) also receives each
 // sequence's first item and count for the merge kernel. ONE: at most 64 sequences, one
 // per lane, whose page counts stay in a register.
@@ -53,7 +55,9 @@ __device__ __forceinline__ bool find_split_of(const PartialArgs& a, int items, i
   };
   const int len0 = length_of(0);
   auto len_at = [&](int k) { return ONE || k == 0 ? len0 : length_of(k); };
-  auto pages_at = [&](int k) { return min((len_at(k) + kPageSize - 1) / kPageSize, a.max_pages); };
+  auto pages_at = [&](int k) {  // unsigned: a length may be the largest there is
+    return min((int)(((unsigned)len_at(k) + kPageSize - 1) / kPageSize), a.max_pages);
+  };
   auto splits_of = [&](int k, int P, float inv) {
     return 64 * k + lane < a.batch ? max(ceil_quotient(pages_at(k), P, inv), 1) : 0;
   };

@@ -378,3 +378,20 @@ def test_host_threads_on_one_stream():
     torch.cuda.synchronize()
     for i in range(2):
         assert len(got[i]) == 20 and all(_equal(g, want[i]) for g in got[i])
+
+
+def test_lengths_past_the_table_up_to_the_largest():
+    """Lengths are held to the table: the largest number there is acts as any other past it."""
+    tops = [2 ** 31 - 1, 2 ** 31 - 15, 2 ** 31 - 16]
+    b, width = len(tops), 30
+
+    def run(lens):
+        s = _state(80, (400,) * b)
+        s["tables"] = s["tables"][:, :width].contiguous()
+        s["lens"].copy_(torch.tensor(lens, dtype=torch.int32))
+        return _step(s)
+
+    past = run([width * 16 + 100] * b)
+    for a, w in zip(_bits(run(tops)), _bits(past)):
+        assert torch.equal(a, w)
+    assert (past[0].abs().sum(-1) > 0).all() and (past[1] == 48).all()

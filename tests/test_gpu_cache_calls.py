@@ -212,6 +212,27 @@ def test_traced_calls():
     assert _equal([want[n] for n in names], [got[n] for n in names])
 
 
+def test_traced_eviction_in_place():
+    """Within one pool and over the weights themselves, also where the trace is made free of
+    writes and put back together (aot_eager)."""
+    def thin(weights, k, v, ks, vs, tables, lens, new_tables):
+        moved = eviction.evict_by_weight(weights, k, v, tables, lens, new_tables, 48, sink=2,
+                                         recent=7, key_scale=ks, value_scale=vs,
+                                         new_weights=weights)
+        return [x * 2 for x in moved]
+
+    names = ("weights", "k", "v", "ks", "vs", "tables", "lens", "new_tables")
+    states = [_state(41, kv=INT8) for _ in range(3)]
+    for s in states:
+        s["new_tables"] = (100 + torch.arange(9)).view(3, 3).to(torch.int32).cuda()
+    calls = [thin, *(torch.compile(thin, backend=how, fullgraph=True)
+                     for how in ("eager", "aot_eager"))]
+    results = [f(*[s[n] for n in names]) for f, s in zip(calls, states)]
+    for r, s in zip(results[1:], states[1:]):
+        assert _equal(results[0], r)
+        assert _equal([states[0][n] for n in names], [s[n] for n in names])
+
+
 def test_keys_and_values_written_to_one_place_are_refused():
     s = _state(9)
     before = _bits([s["k"], s["v"], s["ks"], s["vs"]])

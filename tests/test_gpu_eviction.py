@@ -84,6 +84,15 @@ def test_weights_lengths(lens, q_len):
                  width=max(max(lens) // 16 + 2, 3))
 
 
+@pytest.mark.parametrize("q_len", [2, 9])
+@pytest.mark.parametrize("b", [65, 128, 300, 530])
+def test_weights_batches_about_as_large_as_the_chip(b, q_len):
+    """Few work items to spare, and none (eight kv heads: 512 and 256 items)."""
+    lens = [(37 * i * i) % 300 for i in range(b)]
+    lens[b // 3] = 5000
+    _check_weigh(lens, q_len, 8, 8, 64, 16, TYPES[2], seed=b)
+
+
 @pytest.mark.parametrize("types", [TYPES[0], TYPES[3]], ids=[IDS[0], IDS[3]])
 @pytest.mark.parametrize("q_len", [1, 6, 16])
 def test_weights_draft_trees(q_len, types):

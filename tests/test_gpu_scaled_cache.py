@@ -109,6 +109,19 @@ def test_attention_lengths(lens):
     _check(lens, 3, 8, 2, 64, 16, F16, E4M3, seed=len(lens), width=max(max(lens) // 16 + 2, 3))
 
 
+@pytest.mark.parametrize("b", [65, 100, 127, 128, 129, 200])
+def test_attention_batches_about_as_large_as_the_chip(b):
+    """Lengths that differ, one of them far longer, in batches with few work items to spare
+    and with none (eight kv heads: 128 items)."""
+    lens = [(37 * i * i) % 700 for i in range(b)]
+    lens[b // 3] = 9000
+    q, caches, scales, tables, sl = _inputs(lens, 2, 8, 8, 64, 16, F16, INT8, b)
+    want, bound, _ = ref.attention(q, *caches, *scales, tables, sl)
+    args = _cuda(q, *caches, *scales, tables, sl)
+    for most in (0, 9000, 1):  # the length only sizes the call
+        ref.assert_within(paged_attention_scaled(*args, max_seq_len=most), want, bound, most)
+
+
 @pytest.mark.parametrize("kv", [E4M3, INT8], ids=["e4m3", "int8"])
 @pytest.mark.parametrize("q_len", [1, 6, 16])
 def test_attention_draft_trees(q_len, kv):

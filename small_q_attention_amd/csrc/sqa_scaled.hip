@@ -162,7 +162,7 @@ __device__ __forceinline__ void nan_values(WaveState<NB, HD>& st, typename KV::R
 // fp32, unrounded: a quiet block's tokens weigh as much in it as a loud one's. Pages of a
 // scale under 2^-64, 0 among them, count as of that scale in the maximum and the row sums
 // and add nothing to O (a scale further down would push their P out of fp32's range).
-template <int NB, int D, int HD, typename E, typename KV, bool PIPE>
+template <int NB, int D, int HD, typename E, typename KV>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1)))
 void sqa_scaled_attention_kernel(ScaledArgs args) {
   const PartialArgs& a = args.p;
@@ -259,8 +259,6 @@ void sqa_scaled_attention_kernel(ScaledArgs args) {
   }
   const int mask_from = len - a.q_len;  // pages with a token from here on are masked
 
-  f4 ahead[NB];
-  if constexpr (PIPE) code_scores<NB, HD, E, KV>(ahead, ring[0].kv, q);
   for (int i = 0; i < n_pages; i += D) {
     load_ids(i + 2 * D, ids_next);
 #pragma unroll
@@ -277,13 +275,7 @@ void sqa_scaled_attention_kernel(ScaledArgs args) {
         const float inv_vs = loud ? __builtin_amdgcn_rcpf(vs) : 0x1p64f;
         float c = a.scale_log2 * ks, add = lv;
         f4 s[NB];
-        if constexpr (PIPE) {
-#pragma unroll
-          for (int nb = 0; nb < NB; ++nb) s[nb] = ahead[nb];
-          code_scores<NB, HD, E, KV>(ahead, ring[(j + 1) % D].kv, q);
-        } else {
-          code_scores<NB, HD, E, KV>(s, ring[j].kv, q);
-        }
+        code_scores<NB, HD, E, KV>(s, ring[j].kv, q);
         const bool masked = (p + 1) * kPageSize > mask_from;  // uniform
         if (masked) {
           // After the scales, so that one of 0, infinity or NaN leaves them -inf.
@@ -514,13 +506,13 @@ void launch_scaled_hd(const ScaledArgs& a, dim3 grid, hipStream_t stream) {
   constexpr int D = 4 * 128 / HD;
   const dim3 block(256);
   if (a.p.rows <= 16)
-    hipLaunchKernelGGL((sqa_scaled_attention_kernel<1, D, HD, E, KV, false>), grid, block, 0,
+    hipLaunchKernelGGL((sqa_scaled_attention_kernel<1, D, HD, E, KV>), grid, block, 0,
                        stream, a);
   else if (a.p.rows <= 32)
-    hipLaunchKernelGGL((sqa_scaled_attention_kernel<2, D, HD, E, KV, HD != 256>), grid, block, 0,
+    hipLaunchKernelGGL((sqa_scaled_attention_kernel<2, D, HD, E, KV>), grid, block, 0,
                        stream, a);
   else if constexpr (HD != 256)
-    hipLaunchKernelGGL((sqa_scaled_attention_kernel<4, D / 2, HD, E, KV, false>), grid, block, 0,
+    hipLaunchKernelGGL((sqa_scaled_attention_kernel<4, D / 2, HD, E, KV>), grid, block, 0,
                        stream, a);
 }
 

@@ -264,8 +264,8 @@ typedef struct sqa_block_scales {
  * items that fill the device once, or fewer where sequences of max_seq_len tokens
  * (max_seq_len <= 0: of the table's max_pages 16-token pages) do not need as many.
  * The device cuts the pages from seq_lens alone, so any such count serves any lengths;
- * max_seq_len only sizes the call. sqa_workspace_bytes(..., *num_splits, 0) is the
- * workspace.
+ * max_seq_len only sizes the call (results of different counts may differ in their last
+ * bits). sqa_workspace_bytes(..., *num_splits, 0) is the workspace.
  */
 int sqa_plan_scaled(int device, int batch, int num_kv_heads, int max_seq_len, int max_pages,
                     int* num_splits);
@@ -274,7 +274,9 @@ int sqa_plan_scaled(int device, int batch, int num_kv_heads, int max_seq_len, in
  * sqa_paged_attention over such a cache: kv_dtype SQA_DTYPE_FP8_E4M3 or SQA_DTYPE_INT8,
  * num_splits from sqa_plan_scaled, pages_per_split 0, flags 0; everything else as there.
  * V blocks of a scale under 2^-64 count as zeros; the V scales of what a row sees, those of
- * zeros taken as 2^-64, may lie a factor of 2^100 apart.
+ * zeros taken as 2^-64, may lie a factor of 2^100 apart. A token's probability times its V
+ * scale is rounded to fp16 in units of the row's largest: off by 2^-11 of itself, or by
+ * 2^-25 of those units.
  * A sequence's splits follow from all lengths of the batch, so its last bits may differ
  * between batches; equal inputs give equal bits.
  */

@@ -324,22 +324,19 @@ def scaled_fields(query, k_view, k_scale, block_tables, draft_mask):
 
 def launch_scaled(query, output, k_view, v_view, k_scale, v_scale, block_tables, seq_lens,
                   draft_mask, scale: float, out_scale: float, num_splits: int, workspace,
-                  stream_handle: int, timing_events=None, fields=None):
+                  stream_handle: int, fields=None):
     """Call ``sqa_paged_attention_scaled``: as :func:`launch_general`, over e4m3 or int8
     views with ``[num_pages, Hkv]`` float32 scales of equal strides (``fields`` from
     :func:`scaled_fields`)."""
     lib = _LIB if _LIB is not None else load()
     pool, max_pages, words, shape, types, scales = fields or scaled_fields(
         query, k_view, k_scale, block_tables, draft_mask)
-    ev = None
-    if timing_events is not None:
-        ev = (ctypes.c_void_p * 3)(*[ctypes.c_void_p(int(e)) for e in timing_events])
     a = _ARGS.pack(
         _ARGS.size, query.data_ptr(), output.data_ptr(), k_view.data_ptr(), v_view.data_ptr(),
         *pool, block_tables.data_ptr(), seq_lens.data_ptr(), max_pages,
         0 if draft_mask is None else draft_mask.data_ptr(), words, scale, out_scale, *shape,
         num_splits, 0, workspace.data_ptr(), workspace.numel() * workspace.element_size(),
-        stream_handle or 0, 0 if ev is None else ctypes.addressof(ev), *types)
+        stream_handle or 0, 0, *types)
     rc = lib.sqa_paged_attention_scaled(
         a, _SCALES.pack(k_scale.data_ptr(), v_scale.data_ptr(), *scales))
     if rc != SQA_OK:

@@ -55,7 +55,11 @@ hipError_t launch_append(const AppendArgs& a, hipStream_t stream);
 // are a quarter of K. Whole calls, stored / computed again, head dim 128: 16 x 32K keys,
 // 16-bit K, 4 rows 254 / 388 us, 8 278 / 383, 16 329 / 381, 24 392 / 383, 32 436 / 384;
 // e4m3 4 rows 150 / 203, 8 173 / 201, 12 202 / 201, 16 224 / 204. 4 x 8K, 16-bit: 4 rows
-// 23 / 29, 8 25 / 29, 12 30 / 29, 16 31 / 29; e4m3: 4 rows 18 / 19, 8 21 / 19.
+// 23 / 29, 8 25 / 29, 12 30 / 29, 16 31 / 29; e4m3: 4 rows 18 / 19, 8 21 / 19. Head dim 64,
+// 16 x 32K: 16-bit 4 rows 147 / 197, 8 170 / 197, 16 221 / 198, e4m3 4 rows 97 / 120, 8 122 /
+// 120; 4 x 8K: 16-bit 8 rows 21 / 19, 16 27 / 19, e4m3 4 rows 17 / 18. Head dim 256, 16 x
+// 32K: 16-bit 8 rows 461 / 708, 16 523 / 708, 32 624 / 711, e4m3 16 rows 332 / 389, 32 440 /
+// 393; 4 x 8K: 16-bit 32 rows 62 / 57, e4m3 16 rows 34 / 31.
 __host__ __device__ constexpr bool weights_stored(long long rows, int head_dim, int kv_bytes) {
   return 16 * rows <= (long long)head_dim * kv_bytes;
 }

@@ -39,8 +39,11 @@ __device__ __forceinline__ int ceil_quotient(int n, int d, float inv) {
 // smallest page count of at least kMinSplitPages for which they sum to at most `items`
 // (or P the longest sequence, one item each, where the batch has as many sequences as
 // that or more). Up to there all items are resident at once, and the longest, P pages,
-// sets the time: batches near the number of items, and past it, are cut unevenly or not
-// at all.
+// sets the time. Items do not cross sequence ends, so a batch near the number of items
+// leaves some of the chip idle, and one past it is not cut at all: attention, e4m3, 8 kv
+// heads (128 items), q_len 4, 8K keys each, whole calls beside those of the e4m3 kernel with
+// one scale per tensor, whose items do cross: 64 sequences 177 and 172 us, 65 289 and 176,
+// 100 316 and 265, 128 344 and 333, 129 593 and 336; 100 of 1K to 16K 474 and 309.
 // Returns whether item `item` exists; `table` (one wave of the grid) also receives each
 // sequence's first item and count for the merge kernel. ONE: at most 64 sequences, one
 // per lane, whose page counts stay in a register.

@@ -9,10 +9,11 @@
 // so the codes go to the MFMAs as they are (both types widen exactly to 16 bits) and a
 // page costs two scalars.
 //
-// What bounds attention: HBM up to 32 rows (16 x 32K keys, e4m3, 1.08 GB, partial kernel:
-// q_len 8 175 us, 6.2 TB/s; whole calls q_len 1, 2, 4 at 177 us, 6.1 TB/s, within 6% of the
-// per-tensor e4m3 kernel's 167), instructions at 64 (q_len 16 254 us). Append: 2 x 16K
-// tokens, 0.2 GB, 43 us, 4.7 TB/s, near a large copy's 5.1.
+// What bounds attention: HBM up to 32 rows, instructions at 64. 16 x 32K keys, e4m3, 1.08
+// GB, whole calls beside those of e4m3 with one scale per tensor, same box: q_len 1 175 and
+// 166 us, q_len 4 177 and 168, q_len 8 180 and 176 (6.0 TB/s), q_len 16 250 and 209. Batches
+// whose sequences do not divide the work items leave some of the chip idle (find_split()).
+// Append: 2 x 16K tokens, 0.2 GB, 43 us, 4.7 TB/s, near a large copy's 5.1.
 #include "sqa_cache.h"
 #include "sqa_cache_device.h"
 
@@ -158,7 +159,9 @@ __device__ __forceinline__ void nan_values(WaveState<NB, HD>& st, typename KV::R
 // fp16 rounding of P is relative to its part of the result (2^-11 of it, and 2^-25 of the
 // row's largest part where it is tiny beside that), however the blocks' scales differ; two
 // bf16 parts of p * v_scale cost 28 operations a page more at 32 rows (16 x 32K keys,
-// whole calls: q_len 8 201 -> 178 us, q_len 16 293 -> 245). The row sum gets P / v_scale in
+// whole calls: q_len 8 201 -> 178 us, q_len 16 293 -> 245). What that rounding costs: fp16
+// outputs are 2.32e-4 of their size from the 64-bit result at 16 x 32K keys, q_len 8, and
+// 2.06e-4 with P in 32 bits; bf16 outputs do not change. The row sum gets P / v_scale in
 // fp32, unrounded: a quiet block's tokens weigh as much in it as a loud one's. Pages of a
 // scale under 2^-64, 0 among them, count as of that scale in the maximum and the row sums
 // and add nothing to O (a scale further down would push their P out of fp32's range).
@@ -499,8 +502,12 @@ void launch_append_as(const AppendArgs& a, dim3 grid, hipStream_t stream) {
 }
 
 // Ring depths: as many pages in flight as hold about 16 KiB of codes per wave; half of
-// that at 64 rows, whose accumulators take the registers. Two blocks issue a page's scores
-// under the page before (one block has little softmax to hide).
+// that at 33 to 64 rows, whose accumulators take the registers. Whole calls, 16 x 32K keys,
+// e4m3, us, with half as many pages / these / twice as many: head dim 128 (4 pages) q_len 1
+// 181 / 175 / 177, q_len 8 200 / 181 / 183, q_len 16 (2 pages) 370 / 254 / 255; head dim
+// 256 (2) q_len 1 334 / 319 / 321, q_len 8 490 / 330 / 331; head dim 64 (8) q_len 1 109 /
+// 113 / -, q_len 4 105 / 107 / 109 (12 pages), q_len 8 125 / 125 / -, with int8 150 / 147 /
+// -, q_len 16 (4) 183 / 175 / 176.
 template <int HD, typename E, typename KV>
 void launch_scaled_hd(const ScaledArgs& a, dim3 grid, hipStream_t stream) {
   constexpr int D = 4 * 128 / HD;

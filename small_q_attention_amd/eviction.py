@@ -91,7 +91,8 @@ def accumulate_attention_weights(query, key_cache, block_tables, seq_lens, weigh
     of kv head ``h`` give token ``t``. The last ``Q`` tokens' weights are set, not added to:
     they start with this call, whatever a draft that was taken back left there. Tokens from
     ``T`` on are not recorded, entries past a sequence's end not touched. ``max_seq_len``
-    > 0 promises that no sequence is longer. Returns ``weights``.
+    > 0 promises that no sequence is longer and sizes the workspace, as the block table's
+    width does without it (scores of up to 1 GiB where that is wide). Returns ``weights``.
     """
     if query.dim() != 4:
         raise ValueError("query must be a contiguous [B, Q, Hq, D] tensor")

@@ -238,7 +238,7 @@ def run_attention(query, key_cache, value_cache, key_scale, value_scale, block_t
     if out is None:
         out = torch.empty_like(query)
     _lib.launch_scaled(query, out, key_cache, value_cache, key_scale, value_scale, block_tables,
-                       seq_lens, words, scale, out_scale, slots, workspace, stream, None, fields)
+                       seq_lens, words, scale, out_scale, slots, workspace, stream, fields)
     return out
 
 
@@ -273,12 +273,14 @@ def paged_attention_scaled(query, key_cache, value_cache, key_scale, value_scale
     draft row ``i`` of sequence ``b`` sees the tokens before ``seq_lens[b] - Q`` and, of the
     last ``Q``, those up to its own or those ``mask`` names (the packed draft mask of
     :mod:`small_q_attention_amd.masks`). Rows that see no token are 0. ``max_seq_len`` > 0
-    only sizes the call (0: the block table's width); ``scale`` is the softmax scale
-    (``None``: ``D ** -0.5``), ``out_scale`` multiplies the output. V blocks of a scale under
-    2^-64 count as zeros; the V scales of what a row sees, those of zeros taken as 2^-64, may
-    lie a factor of 2^100 apart. ``workspace_buffer``: a caller's buffer for the split
-    partials; ``None`` takes one kept per host thread and stream, or, under graph capture, one
-    of the graph's own. Returns ``out`` (``[B, Q, Hq, D]``).
+    only sizes the call (0: the block table's width), and with it the last bits of a result
+    may change; ``scale`` is the softmax scale (``None``: ``D ** -0.5``), ``out_scale``
+    multiplies the output. V blocks of a scale under 2^-64 count as zeros; the V scales of
+    what a row sees, those of zeros taken as 2^-64, may lie a factor of 2^100 apart. A token's
+    probability times its V scale is rounded to fp16 in units of the row's largest: off by
+    2^-11 of itself, or by 2^-25 of those units where it is small beside them.
+    ``workspace_buffer``: a caller's buffer for the split partials; ``None`` takes one kept
+    per host thread and stream, or, under graph capture, one of the graph's own. Returns ``out`` (``[B, Q, Hq, D]``).
     """
     if query.dim() != 4:
         raise ValueError("query must be a contiguous [B, Q, Hq, D] tensor")

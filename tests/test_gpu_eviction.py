@@ -340,8 +340,7 @@ def test_a_decoding_loop(kv):
 ])
 def test_evict_sequences_longer_than_their_weights(lens, width, budget, sink, recent, in_place):
     """Tokens the weights do not reach weigh 0; the first and last ones stay as ever."""
-    if in_place and width < budget:
-        pytest.skip("the buffer holds no new weights")
+    in_place = in_place and width >= budget  # else the buffer cannot hold the new weights
     case = list(_evict_case(lens, 2, 64, 16, E4M3, budget, seed=width, ties=width % 2 == 0))
     full = case[0]
     full[:, :, width:] = 0.0

@@ -283,6 +283,28 @@ int sqa_plan_scaled(int device, int batch, int num_kv_heads, int max_seq_len, in
 int sqa_paged_attention_scaled(const sqa_attention_args* args, const sqa_block_scales* scales);
 
 /*
+ * Splits per sequence (*num_splits >= 1) of an sqa_paged_attention_windowed call whose
+ * sequences have at most max_seq_len tokens (<= 0: as many as max_pages 16-token pages
+ * hold). Any count serves any lengths; this one fills the device.
+ */
+int sqa_plan_windowed(int device, int batch, int q_len, int num_query_heads, int num_kv_heads,
+                      int head_dim, int64_t window, int sink, int max_seq_len, int max_pages,
+                      int* num_splits);
+
+/*
+ * sqa_paged_attention where row qi of sequence b, at position p = seq_lens[b] - q_len + qi,
+ * sees of the tokens it would see there only those before `sink` and those after
+ * p - window (window > 0, sink >= 0). Pages that no row sees are not read, their table
+ * entries not used. kv_dtype: dtype, SQA_DTYPE_FP8_E4M3, or with `scales` (else NULL) e4m3
+ * or int8 codes as for sqa_paged_attention_scaled; flags and pages_per_split 0, num_splits
+ * from sqa_plan_windowed, workspace sqa_workspace_bytes(..., num_splits, 1) bytes (0 for one
+ * split). A value that is not finite reaches the rows that see its token. Equal inputs and
+ * splits give equal bits.
+ */
+int sqa_paged_attention_windowed(const sqa_attention_args* args, const sqa_block_scales* scales,
+                                 int64_t window, int sink);
+
+/*
  * Arguments of sqa_append_scaled (set struct_size = sizeof(sqa_append_args)).
  *   key, value     [batch, q_len, num_kv_heads, head_dim] of `dtype`, 16-byte aligned;
  *                  key_strides / value_strides: elements between batches, tokens and

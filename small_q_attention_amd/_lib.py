@@ -33,6 +33,10 @@ _SIGNATURES = [
     ("sqa_paged_attention", _C.c_int, [_C.c_void_p]),
     ("sqa_plan_scaled", _C.c_int, [_C.c_int] * 5 + [_C.POINTER(_C.c_int)]),
     ("sqa_paged_attention_scaled", _C.c_int, [_C.c_void_p, _C.c_void_p]),
+    ("sqa_plan_windowed", _C.c_int,
+     [_C.c_int] * 6 + [_C.c_int64] + [_C.c_int] * 3 + [_C.POINTER(_C.c_int)]),
+    ("sqa_paged_attention_windowed", _C.c_int,
+     [_C.c_void_p, _C.c_void_p, _C.c_int64, _C.c_int]),
     ("sqa_append_scaled", _C.c_int, [_C.c_void_p]),
     ("sqa_weights_workspace_bytes", _C.c_size_t, [_C.c_int] * 9),
     ("sqa_attention_weights", _C.c_int, [_C.c_void_p]),
@@ -341,6 +345,59 @@ def launch_scaled(query, output, k_view, v_view, k_scale, v_scale, block_tables,
         a, _SCALES.pack(k_scale.data_ptr(), v_scale.data_ptr(), *scales))
     if rc != SQA_OK:
         raise RuntimeError(f"sqa_paged_attention_scaled failed: {last_error(lib)}")
+
+
+@functools.lru_cache(maxsize=4096)
+def plan_windowed(device_index: int, batch: int, q_len: int, num_query_heads: int,
+                  num_kv_heads: int, head_dim: int, window: int, sink: int, max_seq_len: int,
+                  max_pages: int) -> int:
+    """``sqa_plan_windowed``: splits per sequence of a windowed call (``max_pages``: 16-token
+    pages)."""
+    lib = load()
+    ns = ctypes.c_int(0)
+    rc = lib.sqa_plan_windowed(device_index, batch, q_len, num_query_heads, num_kv_heads, head_dim,
+                               window, sink, max_seq_len, max_pages, ctypes.byref(ns))
+    if rc != SQA_OK:
+        raise RuntimeError(f"sqa_plan_windowed failed: {last_error(lib)}")
+    return ns.value
+
+
+def part_fields(query, k_view, k_scale, block_tables, draft_mask):
+    """:func:`scaled_fields` where a cache may have no scales."""
+    b, q_len, hq, d = query.shape
+    num_pages, page, hkv, _ = k_view.shape
+    return ((num_pages, *k_view.stride()[:3]), block_tables.shape[1],
+            0 if draft_mask is None else draft_mask.shape[-1], (b, q_len, hq, hkv, d, page),
+            (dtype_code(query.dtype), dtype_code(k_view.dtype), 0),
+            None if k_scale is None else k_scale.stride())
+
+
+def _part_args(query, output, k_view, v_view, k_scale, v_scale, block_tables, seq_lens, draft_mask,
+               scale, out_scale, num_splits, workspace, stream_handle, fields):
+    """``(sqa_attention_args, sqa_block_scales or None)`` of a call over part of a cache."""
+    pool, max_pages, words, shape, types, scales = fields
+    ws, ws_bytes = (0, 0) if workspace is None else (
+        workspace.data_ptr(), workspace.numel() * workspace.element_size())
+    a = _ARGS.pack(
+        _ARGS.size, query.data_ptr(), output.data_ptr(), k_view.data_ptr(), v_view.data_ptr(),
+        *pool, block_tables.data_ptr(), seq_lens.data_ptr(), max_pages,
+        0 if draft_mask is None else draft_mask.data_ptr(), words, scale, out_scale, *shape,
+        num_splits, 0, ws, ws_bytes, stream_handle or 0, 0, *types)
+    return a, None if scales is None else _SCALES.pack(k_scale.data_ptr(), v_scale.data_ptr(),
+                                                       *scales)
+
+
+def launch_windowed(query, output, k_view, v_view, k_scale, v_scale, block_tables, seq_lens,
+                    draft_mask, window: int, sink: int, scale: float, out_scale: float,
+                    num_splits: int, workspace, stream_handle: int, fields=None):
+    """Call ``sqa_paged_attention_windowed``: views and scales (or ``None``) as for
+    :func:`launch_scaled`, ``fields`` from :func:`part_fields`."""
+    lib = _LIB if _LIB is not None else load()
+    a, scales = _part_args(query, output, k_view, v_view, k_scale, v_scale, block_tables, seq_lens,
+                           draft_mask, scale, out_scale, num_splits, workspace, stream_handle,
+                           fields or part_fields(query, k_view, k_scale, block_tables, draft_mask))
+    if lib.sqa_paged_attention_windowed(a, scales, window, sink) != SQA_OK:
+        raise RuntimeError(f"sqa_paged_attention_windowed failed: {last_error(lib)}")
 
 
 def append_fields(key, value, k_view, k_scale, block_tables):

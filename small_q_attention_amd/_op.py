@@ -105,6 +105,29 @@ def _paged_attention_scaled_fake(query, key_cache, value_cache, key_scale, value
     return torch.empty_like(query)
 
 
+@torch.library.custom_op("sqa::paged_attention_windowed", mutates_args=())
+def paged_attention_windowed(query: torch.Tensor, key_cache: torch.Tensor,
+                             value_cache: torch.Tensor, key_scale: Optional[torch.Tensor],
+                             value_scale: Optional[torch.Tensor], block_tables: torch.Tensor,
+                             seq_lens: torch.Tensor, draft_mask: Optional[torch.Tensor],
+                             window: int, sink: int, scale: float, out_scale: float,
+                             max_seq_len: int) -> torch.Tensor:
+    """Attention over a window and the first tokens (``windowed``), planned and given its
+    workspace at run time."""
+    from . import scaled_cache, windowed
+
+    return scaled_cache.on_device(query.device, lambda: windowed.run_windowed(
+        query, key_cache, value_cache, key_scale, value_scale, block_tables, seq_lens, draft_mask,
+        window, sink, scale, out_scale, max_seq_len, None, None))
+
+
+@paged_attention_windowed.register_fake
+def _paged_attention_windowed_fake(query, key_cache, value_cache, key_scale, value_scale,
+                                   block_tables, seq_lens, draft_mask, window, sink, scale,
+                                   out_scale, max_seq_len):
+    return torch.empty_like(query)
+
+
 @torch.library.custom_op("sqa::append_scaled_kv",
                          mutates_args=("key_cache", "value_cache", "key_scale", "value_scale"))
 def append_scaled_kv(key: torch.Tensor, value: torch.Tensor, key_cache: torch.Tensor,

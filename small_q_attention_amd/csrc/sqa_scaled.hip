@@ -24,130 +24,6 @@ namespace {
 // Attention.
 // ---------------------------------------------------------------------------------
 
-// V of a page as the PV product's A operand: av[mb] = this lane's dim mb of its four
-// tokens in fp16, which holds every e4m3 value and every 8-bit integer exactly.
-template <int HD>
-struct CodesFp8 : KvFp8<HD> {
-  using Regs = typename KvFp8<HD>::Regs;
-  static constexpr int MB = Dims<HD>::MB, VW = Dims<HD>::VW;
-  static constexpr bool kNan = true;  // codes may be NaN
-  static __device__ __forceinline__ void operand_v(const Regs& r, u2 (&av)[MB]) {
-#pragma unroll
-    for (int i = 0; i < VW / 2; ++i) {
-      // Bytes of two token rows interleaved, so that a conversion yields two tokens of
-      // one dim.
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const unsigned sel = half ? 0x07030602u : 0x05010400u;
-        const unsigned t01 = __builtin_amdgcn_perm(r.v[1][i], r.v[0][i], sel);
-        const unsigned t23 = __builtin_amdgcn_perm(r.v[3][i], r.v[2][i], sel);
-        const u2 a = ElemF16::widen_fp8x4(t01), b = ElemF16::widen_fp8x4(t23);
-        av[4 * i + 2 * half] = u2{a[0], b[0]};
-        av[4 * i + 2 * half + 1] = u2{a[1], b[1]};
-      }
-    }
-  }
-};
-
-template <int HD>
-struct CodesInt8 : KvFp8<HD> {
-  using Regs = typename KvFp8<HD>::Regs;
-  static constexpr int KK = Dims<HD>::KK, MB = Dims<HD>::MB, VW = Dims<HD>::VW;
-  static constexpr bool kNan = false;
-  static __device__ __forceinline__ float byte(unsigned w, int i) {
-    return (float)(signed char)(w >> (8 * i));
-  }
-  template <typename E>
-  static __device__ __forceinline__ void expand_k(const Regs& r, u4 (&k)[KK]) {
-#pragma unroll
-    for (int i = 0; i < KK; ++i) {
-#pragma unroll
-      for (int w = 0; w < 2; ++w) {
-        const unsigned x = r.k[i / 2][2 * (i & 1) + w];
-        k[i][2 * w] = E::pack2(byte(x, 0), byte(x, 1));
-        k[i][2 * w + 1] = E::pack2(byte(x, 2), byte(x, 3));
-      }
-    }
-  }
-  static __device__ __forceinline__ void operand_v(const Regs& r, u2 (&av)[MB]) {
-#pragma unroll
-    for (int mb = 0; mb < MB; ++mb) {
-      const int i = mb / 4, e = mb % 4;
-      av[mb] = u2{ElemF16::pack2(byte(r.v[0][i], e), byte(r.v[1][i], e)),
-                  ElemF16::pack2(byte(r.v[2][i], e), byte(r.v[3][i], e))};
-    }
-  }
-};
-
-// Partial rows are fp32 for both types of queries: fp16 ones, as the 16-bit kernels leave,
-// added a rounding of the size of the output's own (error against 64 bits 1.45 times that
-// of a rounded 32-bit result; so 1.1 times). It costs 16 x 32K keys, q_len 8, 178 -> 181 us
-// a call, 4 x 8K 22 -> 27.
-template <typename E>
-using PartialRows = std::conditional_t<E::kHalfPartials, ElemF16Wide, E>;
-
-// Raw scores of a page, K code . Q^T. Where Q does not fit the vector registers beside
-// the accumulators (64 rows, head dim 256) it lives in accumulation registers, which the
-// MFMAs read as they are; the empty asm says so, or the compiler copies it over for every
-// page.
-template <int NB, int HD, typename E, typename KV>
-__device__ __forceinline__ void code_scores(f4 (&s)[NB], const typename KV::Regs& r,
-                                            u4 (&q)[NB][Dims<HD>::KK]) {
-  constexpr int KK = Dims<HD>::KK;
-  u4 k[KK];
-  KV::template expand_k<E>(r, k);
-#pragma unroll
-  for (int nb = 0; nb < NB; ++nb) {
-    if constexpr (NB * HD >= 512) {
-#pragma unroll
-      for (int kk = 0; kk < KK; ++kk) asm volatile("" : "+a"(q[nb][kk]));
-    }
-    s[nb] = f4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int kk = 0; kk < KK; ++kk) s[nb] = E::mma_qk(k[kk], q[nb][kk], s[nb]);
-  }
-}
-
-// A masked page's NaN codes of V: in the PV product one would reach every row of its
-// block, those that do not see its token too (0 * NaN). They become 0 here, and NaN the
-// sums of the rows that do see them. Rare: decoding pages without one costs a few
-// instructions on the pages of the draft block only.
-template <int NB, int HD, typename KV>
-__device__ __forceinline__ void nan_values(WaveState<NB, HD>& st, typename KV::Regs& r,
-                                           const f4 (&s)[NB]) {
-  constexpr int MB = Dims<HD>::MB, VW = Dims<HD>::VW;
-  typename KV::Regs marks;
-  unsigned any = 0u;
-#pragma unroll
-  for (int e = 0; e < 4; ++e)
-#pragma unroll
-    for (int w = 0; w < VW / 2; ++w) {
-      // Bytes of magnitude 0x7f, as 0x80.
-      const unsigned nan = ((r.v[e][w] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
-      any |= nan;
-      marks.v[e][w] = (nan >> 7) * 0x38u;  // 1.0 in e4m3
-      r.v[e][w] &= ~((nan >> 7) * 0xffu);
-    }
-  if (!__any(any != 0u)) return;  // uniform
-  u2 av[MB];
-  KV::operand_v(marks, av);
-#pragma unroll
-  for (int nb = 0; nb < NB; ++nb) {
-    float seen[4], sum = 0.f;
-    u2 none;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) seen[e] = s[nb][e] == -INFINITY ? 0.f : 1.f;
-    const u2 rows = ElemF16::round_p(seen[0], seen[1], seen[2], seen[3], sum, none);
-#pragma unroll
-    for (int mb = 0; mb < MB; ++mb) {
-      const f4 hits = ElemF16::mma_pv(av[mb], rows, none, f4{0.f, 0.f, 0.f, 0.f});
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        st.acc[mb][nb][e] = hits[e] > 0.f ? __builtin_nanf("") : st.acc[mb][nb][e];
-    }
-  }
-}
-
 // One workgroup = four waves on their own: wave w serves kv head w % wg_heads of the
 // workgroup's heads and work item w / wg_heads of its items, with all query rows of the
 // head (NB blocks of 16). A wave keeps a ring of D pages of codes and their two scales in

@@ -305,6 +305,64 @@ int sqa_paged_attention_windowed(const sqa_attention_args* args, const sqa_block
                                  int64_t window, int sink);
 
 /*
+ * What sqa_plan_shared_prefix decides, the shape it decided it for, and the sizes of the
+ * table that goes with it. Read-only for callers, but for table_bytes.
+ */
+typedef struct sqa_shared_plan {
+  size_t struct_size;
+  int batch;
+  int q_len;
+  int num_query_heads;
+  int num_kv_heads;
+  int head_dim;
+  int page_size;
+  int num_groups;  /* that share something */
+  int num_items;
+  int block_rows;
+  int most_pages;  /* block_tables columns that the plan reads */
+  int least_pages; /* of them every sequence shares at least these */
+  int64_t partial_rows;
+  size_t table_bytes;
+} sqa_shared_plan;
+
+/*
+ * Plans attention over a batch whose sequences share prefixes. groups: num_groups x (first,
+ * count, pages): sequences first .. first + count - 1 begin with the same `pages` entries of
+ * their block tables; in ascending order, apart, within the batch. Sequences of no group,
+ * and groups of one sequence or no page, share nothing. Writes *plan, and, where `table` is
+ * not NULL, the plan's table (table_bytes bytes of host memory, 8-byte aligned; a first call
+ * with NULL tells how many): the caller copies it to the device. Lengths and pages may
+ * change under a plan; only the shape, the groups and what they share are in it.
+ */
+int sqa_plan_shared_prefix(int device, int batch, int q_len, int num_query_heads,
+                           int num_kv_heads, int head_dim, int page_size, int num_groups,
+                           const int32_t* groups, sqa_shared_plan* plan, void* table);
+
+/*
+ * Splits (*num_splits >= 1) of what follows the shared pages, for sequences of at most
+ * max_seq_len tokens (<= 0: as many as max_pages 16-token pages hold), shared ones counted.
+ * Any count serves any lengths.
+ */
+int sqa_plan_shared_own(int device, const sqa_shared_plan* plan, int max_seq_len, int max_pages,
+                        int* num_splits);
+
+/* Workspace bytes of a call (0: none needed, or not a plan). */
+size_t sqa_shared_workspace_bytes(const sqa_shared_plan* plan, int num_splits);
+
+/*
+ * sqa_paged_attention of a batch with shared prefixes: the same result, the shared pages
+ * read once for each group. `table`: the plan's, in device memory, 16-byte aligned. The
+ * shared pages are read through the table row of the group's first sequence that reaches
+ * past them with all of its rows (seq_lens[b] - q_len >= shared tokens); sequences that do
+ * not (a padded batch's) go over their own pages from the first on. kv_dtype and `scales` as
+ * for sqa_paged_attention_windowed; flags and pages_per_split 0, num_splits from
+ * sqa_plan_shared_own. Equal inputs, plan and splits give equal bits.
+ */
+int sqa_paged_attention_shared_prefix(const sqa_attention_args* args,
+                                      const sqa_block_scales* scales, const sqa_shared_plan* plan,
+                                      const void* table);
+
+/*
  * Arguments of sqa_append_scaled (set struct_size = sizeof(sqa_append_args)).
  *   key, value     [batch, q_len, num_kv_heads, head_dim] of `dtype`, 16-byte aligned;
  *                  key_strides / value_strides: elements between batches, tokens and

@@ -37,6 +37,13 @@ _SIGNATURES = [
      [_C.c_int] * 6 + [_C.c_int64] + [_C.c_int] * 3 + [_C.POINTER(_C.c_int)]),
     ("sqa_paged_attention_windowed", _C.c_int,
      [_C.c_void_p, _C.c_void_p, _C.c_int64, _C.c_int]),
+    ("sqa_plan_shared_prefix", _C.c_int,
+     [_C.c_int] * 8 + [_C.c_void_p, _C.c_void_p, _C.c_void_p]),
+    ("sqa_plan_shared_own", _C.c_int,
+     [_C.c_int, _C.c_void_p, _C.c_int, _C.c_int, _C.POINTER(_C.c_int)]),
+    ("sqa_shared_workspace_bytes", _C.c_size_t, [_C.c_void_p, _C.c_int]),
+    ("sqa_paged_attention_shared_prefix", _C.c_int,
+     [_C.c_void_p, _C.c_void_p, _C.c_void_p, _C.c_void_p]),
     ("sqa_append_scaled", _C.c_int, [_C.c_void_p]),
     ("sqa_weights_workspace_bytes", _C.c_size_t, [_C.c_int] * 9),
     ("sqa_attention_weights", _C.c_int, [_C.c_void_p]),
@@ -76,6 +83,17 @@ class BlockScales(ctypes.Structure):
 
     _fields_ = [("k", _C.c_void_p), ("v", _C.c_void_p), ("page_stride", _C.c_int64),
                 ("head_stride", _C.c_int64)]
+
+
+class SharedPlan(ctypes.Structure):
+    """``sqa_shared_plan`` of include/sqa.h."""
+
+    _fields_ = [("struct_size", _C.c_size_t), ("batch", _C.c_int), ("q_len", _C.c_int),
+                ("num_query_heads", _C.c_int), ("num_kv_heads", _C.c_int),
+                ("head_dim", _C.c_int), ("page_size", _C.c_int), ("num_groups", _C.c_int),
+                ("num_items", _C.c_int), ("block_rows", _C.c_int), ("most_pages", _C.c_int),
+                ("least_pages", _C.c_int), ("partial_rows", _C.c_int64),
+                ("table_bytes", _C.c_size_t)]
 
 
 class AppendArgs(ctypes.Structure):
@@ -398,6 +416,51 @@ def launch_windowed(query, output, k_view, v_view, k_scale, v_scale, block_table
                            fields or part_fields(query, k_view, k_scale, block_tables, draft_mask))
     if lib.sqa_paged_attention_windowed(a, scales, window, sink) != SQA_OK:
         raise RuntimeError(f"sqa_paged_attention_windowed failed: {last_error(lib)}")
+
+
+def plan_shared_prefix(device_index: int, groups, batch: int, q_len: int, num_query_heads: int,
+                       num_kv_heads: int, head_dim: int, page_size: int):
+    """``sqa_plan_shared_prefix`` -> (:class:`SharedPlan`, table bytes); ``groups``: (first,
+    count, pages) triples."""
+    lib = load()
+    flat = [int(x) for g in groups for x in g]
+    given = (ctypes.c_int32 * max(len(flat), 1))(*flat)
+    plan = SharedPlan()
+    shape = (device_index, batch, q_len, num_query_heads, num_kv_heads, head_dim, page_size,
+             len(flat) // 3, given, ctypes.byref(plan))
+    table = None
+    for _ in range(2):
+        if lib.sqa_plan_shared_prefix(*shape, table) != SQA_OK:
+            raise RuntimeError(f"sqa_plan_shared_prefix failed: {last_error(lib)}")
+        if table is None:
+            table = (ctypes.c_int64 * -(-plan.table_bytes // 8))()
+    return plan, bytes(table)[:plan.table_bytes]
+
+
+def plan_shared_own(device_index: int, plan, max_seq_len: int, max_pages: int):
+    """``(splits, workspace bytes)`` of a call under ``plan`` (``max_pages``: 16-token
+    pages)."""
+    lib = load()
+    ns = ctypes.c_int(0)
+    rc = lib.sqa_plan_shared_own(device_index, ctypes.byref(plan), max_seq_len, max_pages,
+                                 ctypes.byref(ns))
+    if rc != SQA_OK:
+        raise RuntimeError(f"sqa_plan_shared_own failed: {last_error(lib)}")
+    return ns.value, int(lib.sqa_shared_workspace_bytes(ctypes.byref(plan), ns.value))
+
+
+def launch_shared_prefix(query, output, k_view, v_view, k_scale, v_scale, block_tables, seq_lens,
+                         draft_mask, plan, table, scale: float, out_scale: float, num_splits: int,
+                         workspace, stream_handle: int, fields=None):
+    """Call ``sqa_paged_attention_shared_prefix`` (``table``: the plan's, on the device; the
+    rest as for :func:`launch_windowed`)."""
+    lib = _LIB if _LIB is not None else load()
+    a, scales = _part_args(query, output, k_view, v_view, k_scale, v_scale, block_tables, seq_lens,
+                           draft_mask, scale, out_scale, num_splits, workspace, stream_handle,
+                           fields or part_fields(query, k_view, k_scale, block_tables, draft_mask))
+    rc = lib.sqa_paged_attention_shared_prefix(a, scales, ctypes.byref(plan), table.data_ptr())
+    if rc != SQA_OK:
+        raise RuntimeError(f"sqa_paged_attention_shared_prefix failed: {last_error(lib)}")
 
 
 def append_fields(key, value, k_view, k_scale, block_tables):

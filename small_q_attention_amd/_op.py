@@ -7,7 +7,7 @@ implementation only shapes the output, so the op traces under
 :func:`paged_mtp_attention_planned`, which makes the split plan at run time.
 """
 
-from typing import Optional
+from typing import List, Optional
 
 import torch
 
@@ -125,6 +125,29 @@ def paged_attention_windowed(query: torch.Tensor, key_cache: torch.Tensor,
 def _paged_attention_windowed_fake(query, key_cache, value_cache, key_scale, value_scale,
                                    block_tables, seq_lens, draft_mask, window, sink, scale,
                                    out_scale, max_seq_len):
+    return torch.empty_like(query)
+
+
+@torch.library.custom_op("sqa::paged_attention_shared_prefix", mutates_args=())
+def paged_attention_shared_prefix(query: torch.Tensor, key_cache: torch.Tensor,
+                                  value_cache: torch.Tensor, key_scale: Optional[torch.Tensor],
+                                  value_scale: Optional[torch.Tensor], block_tables: torch.Tensor,
+                                  seq_lens: torch.Tensor, draft_mask: Optional[torch.Tensor],
+                                  plan: List[int], table: torch.Tensor, scale: float,
+                                  out_scale: float, max_seq_len: int) -> torch.Tensor:
+    """Attention over shared prefixes (``shared_prefix``) under a plan of these numbers, given
+    its workspace at run time."""
+    from . import scaled_cache, shared_prefix
+
+    return scaled_cache.on_device(query.device, lambda: shared_prefix.run_shared_prefix(
+        query, key_cache, value_cache, key_scale, value_scale, block_tables, seq_lens, draft_mask,
+        _lib.SharedPlan(*plan), table, scale, out_scale, max_seq_len, None, None))
+
+
+@paged_attention_shared_prefix.register_fake
+def _paged_attention_shared_prefix_fake(query, key_cache, value_cache, key_scale, value_scale,
+                                        block_tables, seq_lens, draft_mask, plan, table, scale,
+                                        out_scale, max_seq_len):
     return torch.empty_like(query)
 
 

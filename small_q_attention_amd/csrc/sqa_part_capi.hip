@@ -193,6 +193,80 @@ int place(const sqa_attention_args& a, long long rows, size_t need, sqa::PartArg
   return SQA_OK;
 }
 
+// Where the parts of a plan's table are, in bytes.
+struct SharedTable {
+  size_t group_of, items, bytes;
+};
+SharedTable table_of(int num_groups, int batch, long long num_items) {
+  SharedTable t;
+  t.group_of = (size_t)num_groups * sizeof(sqa::SharedGroup);
+  t.items = t.group_of + ((size_t)batch * 4 + 15) / 16 * 16;
+  t.bytes = t.items + (size_t)num_items * sizeof(sqa::SharedItem);
+  return t;
+}
+
+// Rows of a block: the widest group's, as one wave takes them, while they fit one.
+int rows_of_block(long long most, int head_dim) {
+  if (most <= 16) return 16;
+  if (most <= 32 || head_dim == 256) return 32;
+  return 64;
+}
+
+// Splits of `pages` pages of at most `size` each, all alike but for the last.
+long long splits_of(long long pages, long long size) {
+  return ceil_div(pages, ceil_div(pages, ceil_div(pages, size)));
+}
+
+// Pages of a split, so that the rounds the groups' workgroups take times (pages of a split +
+// what a workgroup costs besides) is least.
+struct SharedCut {
+  int cus, num_kv_heads, block_rows;
+  long long workgroups(long long items) const {
+    const int wgh = wg_heads(num_kv_heads);
+    return ceil_div(items, 4 / wgh) * ceil_div(num_kv_heads, wgh);
+  }
+  template <typename Groups>
+  long long pages(const Groups& groups, int num_groups) const {
+    constexpr long long kStart = 12;
+    long long longest = 1;
+    for (int g = 0; g < num_groups; ++g) longest = std::max(longest, (long long)groups(g).pages);
+    const auto items = [&](long long size) {
+      long long n = 0;
+      for (int g = 0; g < num_groups; ++g)
+        n += groups(g).blocks * ceil_div(groups(g).pages, size);
+      return n;
+    };
+    long long best = longest, best_cost = -1;
+    for (int rounds = 1; rounds <= 8; ++rounds) {
+      long long lo = sqa::kMinSplitPages, hi = std::max(longest, lo);  // the fewest that fit
+      while (lo < hi) {
+        const long long mid = (lo + hi) / 2;
+        if (workgroups(items(mid)) <= (long long)rounds * cus)
+          hi = mid;
+        else
+          lo = mid + 1;
+      }
+      const long long real = ceil_div(workgroups(items(lo)), cus);
+      const long long cost = real * (lo + kStart);
+      if (best_cost < 0 || cost < best_cost) {
+        best = lo;
+        best_cost = cost;
+      }
+    }
+    return best;
+  }
+};
+
+int check_plan(const sqa_shared_plan* p) {
+  if (!p) return fail(SQA_ERR_INVALID, "null plan");
+  if (p->struct_size != sizeof(sqa_shared_plan))
+    return fail(SQA_ERR_INVALID, "struct_size %zu does not match this library's %zu",
+                p->struct_size, sizeof(sqa_shared_plan));
+  if (p->num_groups < 0 || p->num_items < 0 || p->partial_rows < 0)
+    return fail(SQA_ERR_INVALID, "not a plan of sqa_plan_shared_prefix");
+  return SQA_OK;
+}
+
 bool workgroups_fit(const sqa::PartArgs& s) {
   return (long long)s.p.batch * s.splits * s.p.hkv <= 0x7fffffffLL;
 }
@@ -246,6 +320,169 @@ int sqa_paged_attention_windowed(const sqa_attention_args* args, const sqa_block
     return hip_fail(e, "windowed attention kernel launch");
   if (ev && (e = hipEventRecord(ev[1], stream)) != hipSuccess) return hip_fail(e, "hipEventRecord");
   if (a.num_splits > 1 && (e = sqa::launch_join(s, stream)) != hipSuccess)
+    return hip_fail(e, "join kernel launch");
+  if (ev && (e = hipEventRecord(ev[2], stream)) != hipSuccess) return hip_fail(e, "hipEventRecord");
+  return SQA_OK;
+}
+
+int sqa_plan_shared_prefix(int device, int batch, int q_len, int num_query_heads,
+                           int num_kv_heads, int head_dim, int page_size, int num_groups,
+                           const int32_t* groups, sqa_shared_plan* plan, void* table) {
+  if (!plan) return fail(SQA_ERR_INVALID, "null output pointer");
+  long long rows = 0;
+  if (int rc = check_shape(batch, q_len, num_query_heads, num_kv_heads, head_dim, &rows)) return rc;
+  const int shift = page_shift_of(page_size);
+  if (shift < 0)
+    return fail(SQA_ERR_UNSUPPORTED, "page_size must be 16, 32, 64, 128 or 256 (got %d)",
+                page_size);
+  if (num_groups < 0 || (num_groups > 0 && !groups))
+    return fail(SQA_ERR_INVALID, "null or negative groups");
+  const int cus = sqa_device_cu_count(device);
+  if (cus <= 0) return SQA_ERR_HIP;
+  // A group of one sequence, or of no pages, shares nothing.
+  long long most_rows = 0, most_pages = 0, least = 0;
+  int shared = 0, end = 0, covered = 0;
+  for (int i = 0; i < num_groups; ++i) {
+    const int first = groups[3 * i], count = groups[3 * i + 1], pages = groups[3 * i + 2];
+    if (first < end || count <= 0 || pages < 0 || count > batch - first)
+      return fail(SQA_ERR_INVALID,
+                  "groups are (first, count, pages) in order, apart and within the batch");
+    if (((long long)pages << shift) >= (1LL << 26))
+      return fail(SQA_ERR_INVALID, "block-table rows must be under 2^30 tokens");
+    end = first + count;
+    if (count == 1 || pages == 0) continue;
+    ++shared;
+    covered += count;
+    most_rows = std::max(most_rows, count * rows);
+    most_pages = std::max(most_pages, (long long)pages);
+    least = shared == 1 ? pages : std::min(least, (long long)pages);
+  }
+  const int block_rows = rows_of_block(most_rows, head_dim);
+  struct Group {
+    long long blocks, pages;
+    int first, count;
+  };
+  // The i-th group that shares something; groups are few beside the work they stand for.
+  const auto shared_group = [&](int want) {
+    for (int i = 0;; ++i) {
+      if (groups[3 * i + 1] == 1 || groups[3 * i + 2] == 0 || want-- > 0) continue;
+      return Group{ceil_div(groups[3 * i + 1] * rows, block_rows),
+                   (long long)groups[3 * i + 2] << shift, groups[3 * i], groups[3 * i + 1]};
+    }
+  };
+  const SharedCut cut{cus, num_kv_heads, block_rows};
+  const long long size = shared ? cut.pages(shared_group, shared) : 1;
+  long long items = 0, partial_rows = 0;
+  for (int g = 0; g < shared; ++g) {
+    const Group x = shared_group(g);
+    const long long splits = splits_of(x.pages, size);
+    items += x.blocks * splits;
+    partial_rows += splits * num_kv_heads * x.count * rows;
+  }
+  if (items * num_kv_heads > 0x7fffffffLL) return fail(SQA_ERR_INVALID, "grid too large");
+  const SharedTable t = table_of(shared, batch, items);
+  sqa_shared_plan out;
+  memset(&out, 0, sizeof(out));
+  out.struct_size = sizeof(out);
+  out.batch = batch;
+  out.q_len = q_len;
+  out.num_query_heads = num_query_heads;
+  out.num_kv_heads = num_kv_heads;
+  out.head_dim = head_dim;
+  out.page_size = page_size;
+  out.num_groups = shared;
+  out.num_items = (int)items;
+  out.block_rows = block_rows;
+  out.most_pages = (int)most_pages;
+  out.least_pages = covered == batch ? (int)least : 0;
+  out.partial_rows = partial_rows;
+  out.table_bytes = t.bytes;
+  *plan = out;
+  if (!table) return SQA_OK;
+  sqa::SharedGroup* to = (sqa::SharedGroup*)table;
+  int32_t* group_of = (int32_t*)((char*)table + t.group_of);
+  sqa::SharedItem* item = (sqa::SharedItem*)((char*)table + t.items);
+  memset(table, 0, t.items);
+  for (int b = 0; b < batch; ++b) group_of[b] = -1;
+  long long base = 0;
+  for (int g = 0; g < shared; ++g) {
+    const Group x = shared_group(g);
+    const int splits = (int)splits_of(x.pages, size);
+    const int each = (int)ceil_div(x.pages, splits);
+    to[g] = {x.first, x.count, (int)x.pages, splits, each, (int)x.blocks, base};
+    base += (long long)splits * num_kv_heads * x.count * rows;
+    for (int b = x.first; b < x.first + x.count; ++b) group_of[b] = g;
+    for (int j = 0; j < splits; ++j)
+      for (int k = 0; k < x.blocks; ++k) *item++ = {g, k, j, 0};
+  }
+  return SQA_OK;
+}
+
+int sqa_plan_shared_own(int device, const sqa_shared_plan* plan, int max_seq_len, int max_pages,
+                        int* num_splits) {
+  if (!num_splits) return fail(SQA_ERR_INVALID, "null output pointer");
+  if (int rc = check_plan(plan)) return rc;
+  if (max_pages <= 0) return fail(SQA_ERR_INVALID, "max_pages must be positive");
+  const int cus = sqa_device_cu_count(device);
+  if (cus <= 0) return SQA_ERR_HIP;
+  long long pages = max_pages;
+  if (max_seq_len > 0) pages = std::min(pages, ceil_div(max_seq_len, sqa::kPageSize));
+  pages -= (long long)plan->least_pages * (plan->page_size / sqa::kPageSize);
+  *num_splits = (int)own_splits(cus, plan->batch, plan->num_kv_heads, std::max(pages, 1LL));
+  return SQA_OK;
+}
+
+size_t sqa_shared_workspace_bytes(const sqa_shared_plan* plan, int num_splits) {
+  if (check_plan(plan) || num_splits <= 0) return 0;
+  if (num_splits == 1 && plan->num_groups == 0) return 0;
+  const size_t rows = (size_t)plan->q_len * (plan->num_query_heads / plan->num_kv_heads);
+  const size_t own = (size_t)plan->batch * num_splits * plan->num_kv_heads * rows;
+  return (own + (size_t)plan->partial_rows) * ((size_t)plan->head_dim + 2) * sizeof(float);
+}
+
+int sqa_paged_attention_shared_prefix(const sqa_attention_args* args,
+                                      const sqa_block_scales* scales, const sqa_shared_plan* plan,
+                                      const void* table) {
+  if (!args) return fail(SQA_ERR_INVALID, "null argument struct");
+  if (args->struct_size != sizeof(sqa_attention_args))
+    return fail(SQA_ERR_INVALID, "struct_size %zu does not match this library's %zu",
+                args->struct_size, sizeof(sqa_attention_args));
+  if (int rc = check_plan(plan)) return rc;
+  const sqa_attention_args& a = *args;
+  sqa::PartArgs s;
+  if (int rc = fill(a, scales, &s)) return rc;
+  if (plan->batch != a.batch || plan->q_len != a.q_len ||
+      plan->num_query_heads != a.num_query_heads || plan->num_kv_heads != a.num_kv_heads ||
+      plan->head_dim != a.head_dim || plan->page_size != a.page_size)
+    return fail(SQA_ERR_INVALID, "the plan was made for another batch, q_len, heads or page size");
+  if (plan->most_pages > a.max_pages)
+    return fail(SQA_ERR_INVALID, "the plan shares %d pages, block_tables rows hold %d",
+                plan->most_pages, a.max_pages);
+  if (plan->num_groups > 0) {
+    if (!table) return fail(SQA_ERR_INVALID, "null plan table");
+    if ((uintptr_t)table % 16) return fail(SQA_ERR_INVALID, "plan table must be 16-byte aligned");
+    const SharedTable t = table_of(plan->num_groups, plan->batch, plan->num_items);
+    s.groups = (const sqa::SharedGroup*)table;
+    s.group_of = (const int32_t*)((const char*)table + t.group_of);
+    s.items = (const sqa::SharedItem*)((const char*)table + t.items);
+    s.n_items = plan->num_items;
+    s.block_rows = plan->block_rows;
+  }
+  if (!workgroups_fit(s)) return fail(SQA_ERR_INVALID, "grid too large");
+  s.shared_at = (long long)a.batch * a.num_splits * a.num_kv_heads * s.p.rows;
+  const size_t need = sqa_shared_workspace_bytes(plan, a.num_splits);
+  if (int rc = place(a, s.shared_at + plan->partial_rows, need, &s)) return rc;
+
+  hipStream_t stream = (hipStream_t)a.stream;
+  hipEvent_t* ev = (hipEvent_t*)a.timing_events;
+  hipError_t e;
+  if (ev && (e = hipEventRecord(ev[0], stream)) != hipSuccess) return hip_fail(e, "hipEventRecord");
+  if (s.n_items > 0 && (e = sqa::launch_shared(s, stream)) != hipSuccess)
+    return hip_fail(e, "shared prefix kernel launch");
+  if ((e = sqa::launch_own(s, stream)) != hipSuccess)
+    return hip_fail(e, "own part kernel launch");
+  if (ev && (e = hipEventRecord(ev[1], stream)) != hipSuccess) return hip_fail(e, "hipEventRecord");
+  if ((a.num_splits > 1 || s.n_items > 0) && (e = sqa::launch_join(s, stream)) != hipSuccess)
     return hip_fail(e, "join kernel launch");
   if (ev && (e = hipEventRecord(ev[2], stream)) != hipSuccess) return hip_fail(e, "hipEventRecord");
   return SQA_OK;

@@ -1,0 +1,175 @@
+"""Small-q attention for batches whose sequences begin with the same pages: answers sampled
+from one prompt, requests under one system prompt or over one document. The shared pages are
+read once for each group of sequences and not once for each sequence.
+
+:func:`plan_shared_prefix` says which sequences share how many pages, once for as long as
+that stays; :func:`paged_attention_shared_prefix` is the attention call, with the result of
+attention over the whole block tables. It runs on the current stream of the query's device,
+allocates nothing but its result and a workspace, never synchronises and can be captured in a
+HIP graph (keep the plan as long as the graph).
+"""
+
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+
+from . import _lib
+from . import scaled_cache as sc
+from .cuda import HEAD_DIMS, SUPPORTED_PAGE_SIZES, _tracing
+from .masks import as_words
+from .windowed import check_call, take_workspace
+
+
+class SharedPrefixPlan:
+    """What :func:`plan_shared_prefix` returns: ``shape`` (batch, q_len, query heads, kv
+    heads, head_dim, page_size), ``groups`` as given, and the tables on ``device``."""
+
+    def __init__(self, shape, groups, device, plan, table):
+        self.shape, self.groups, self.device = shape, groups, device
+        self.plan, self.table = plan, table
+        self.numbers = [int(getattr(plan, name)) for name, _ in plan._fields_]  # for traced calls
+        self.most_pages = int(plan.most_pages)
+        self.known = sc.Layouts()
+
+
+def plan_shared_prefix(groups, batch: int, q_len: int, num_query_heads: int, num_kv_heads: int,
+                       head_dim: int, page_size: int, device=None) -> SharedPrefixPlan:
+    """Plan for a batch and the prefixes its sequences share.
+
+    ``groups``: ``(first, count, pages)`` triples, in ascending order and apart: sequences
+    ``first .. first + count - 1`` begin with the same ``pages`` entries of their block
+    tables. Sequences of no group share nothing. The plan holds for as long as the groups and
+    what they share stay, whatever the sequences' lengths and the pages' ids; calls with
+    another shape refuse it. One small copy to ``device`` (``None``: the current one).
+    """
+    groups = [tuple(int(x) for x in g) for g in groups]
+    shape = tuple(int(x) for x in (batch, q_len, num_query_heads, num_kv_heads, head_dim,
+                                   page_size))
+    b, q, hq, hkv, d, page = shape
+    if min(b, q, hq, hkv) <= 0 or hq % hkv:
+        raise ValueError("batch, q_len and heads must be positive, query heads a multiple of kv "
+                         "heads")
+    if d not in HEAD_DIMS:
+        raise ValueError("this build supports head_dim 64, 128 or 256")
+    if page not in SUPPORTED_PAGE_SIZES:
+        raise ValueError("this build supports page_size 16, 32, 64, 128 or 256")
+    most = 32 if d == 256 else 64
+    if q * (hq // hkv) > most:
+        raise ValueError(f"Q * (Hq / Hkv) must be at most {most} at head_dim {d}")
+    end = 0
+    for g in groups:
+        if len(g) != 3 or g[0] < end or g[1] <= 0 or g[2] < 0 or g[0] + g[1] > b:
+            raise ValueError("groups are (first, count, pages), in ascending order, apart and "
+                             f"within the batch; got {g}")
+        if g[2] * page >= 2**30:
+            raise ValueError("block-table rows must be under 2^30 tokens")
+        end = g[0] + g[1]
+    device = torch.device("cuda" if device is None else device)
+    if device.type != "cuda":
+        raise ValueError("the plan's device must be a GPU")
+    if device.index is None:
+        device = torch.device("cuda", torch.cuda.current_device())
+    plan, table = _lib.plan_shared_prefix(device.index, groups, *shape)
+    return SharedPrefixPlan(shape, groups, device, plan, torch.frombuffer(
+        bytearray(table), dtype=torch.uint8).to(device))
+
+
+def _check(query, key_cache, value_cache, key_scale, value_scale, block_tables, seq_lens, words,
+           plan, out, workspace_buffer):
+    check_call(query, key_cache, value_cache, key_scale, value_scale, block_tables, seq_lens, words,
+               out, workspace_buffer)
+    shape = (*query.shape[:3], key_cache.shape[2], query.shape[3], key_cache.shape[1])
+    if shape != plan.shape:
+        raise ValueError(f"the plan was made for (batch, q_len, query heads, kv heads, head_dim, "
+                         f"page_size) {plan.shape}, the call has {tuple(shape)}")
+    if plan.device != query.device:
+        raise ValueError(f"the plan lives on {plan.device}, query on {query.device}")
+    if plan.most_pages > block_tables.shape[1]:
+        raise ValueError(f"the plan shares {plan.most_pages} pages, block_tables rows hold "
+                         f"{block_tables.shape[1]}")
+
+
+def _plan_call(query, key_cache, key_scale, block_tables, words, plan, max_seq_len):
+    splits, need = _lib.plan_shared_own(query.device.index, plan, max_seq_len,
+                                        block_tables.shape[1] * (key_cache.shape[1] // 16))
+    return splits, need, _lib.part_fields(query, key_cache, key_scale, block_tables, words)
+
+
+def run_shared_prefix(query, key_cache, value_cache, key_scale, value_scale, block_tables, seq_lens,
+                      words, plan, table, scale, out_scale, max_seq_len, out, workspace,
+                      known=None):
+    """Plan and launch a checked call (``plan``, ``table``: a plan's; ``known``: the call's
+    :func:`_plan_call`)."""
+    splits, need, fields = known or _plan_call(query, key_cache, key_scale, block_tables, words,
+                                               plan, max_seq_len)
+    stream = _lib.raw_stream(query.device.index)
+    workspace = take_workspace(workspace, need, query, stream)
+    if out is None:
+        out = torch.empty_like(query)
+    _lib.launch_shared_prefix(query, out, key_cache, value_cache, key_scale, value_scale,
+                              block_tables, seq_lens, words, plan, table, scale, out_scale, splits,
+                              workspace, stream, fields)
+    return out
+
+
+def paged_attention_shared_prefix(query, key_cache, value_cache, block_tables, seq_lens,
+                                  plan: SharedPrefixPlan, key_scale=None, value_scale=None,
+                                  max_seq_len: int = 0, scale: Optional[float] = None,
+                                  out_scale: float = 1.0, mask=None, out=None,
+                                  workspace_buffer=None):
+    """Small-q attention of a batch whose sequences share prefixes.
+
+    ``query`` ``[B, Q, Hq, D]`` (fp16 or bf16), caches ``[P, page, Hkv, D]`` of the query's
+    type, of ``torch.float8_e4m3fn``, or codes with ``key_scale``/``value_scale``;
+    ``block_tables`` ``[B, max_pages]`` and ``seq_lens`` ``[B]`` int32 as for the other
+    attention calls: whole tables and whole lengths, shared pages and draft tokens counted.
+    Row ``i`` of a sequence sees the tokens before its draft block and, of the block, those
+    up to its own or those ``mask`` names (the packed draft mask of
+    :mod:`small_q_attention_amd.masks`); rows that see no token are 0. A group's shared pages
+    are taken from the table row of its first sequence that is long enough for all of its
+    rows to lie behind them; the entries of the others' rows are not read there. A sequence
+    that is not (a padded batch's) goes over its own row from the start.
+
+    ``max_seq_len`` > 0 only sizes the call (0: the block table's width), and with it the
+    last bits of a result may change; ``scale`` is the softmax scale (``None``: ``D **
+    -0.5``), ``out_scale`` multiplies the output. In bf16 the shared pages' probabilities are
+    rounded as the plan's kernel for its group sizes does. ``workspace_buffer``: a caller's
+    buffer for the partial rows; ``None`` takes one kept per host thread and stream, or, under
+    graph capture, one of the graph's own. Returns ``out`` (``[B, Q, Hq, D]``).
+    """
+    if query.dim() != 4:
+        raise ValueError("query must be a contiguous [B, Q, Hq, D] tensor")
+    if not isinstance(plan, SharedPrefixPlan):
+        raise ValueError("plan must come from plan_shared_prefix()")
+    scale = sc.check_softmax_scale(scale, query.shape[3])
+    words = None if mask is None else as_words(mask, query.shape[0], query.shape[1])
+    max_seq_len = min(max(int(max_seq_len), 0), 2**31 - 1)
+    if _tracing():
+        _check(query, key_cache, value_cache, key_scale, value_scale, block_tables, seq_lens, words,
+               plan, out, workspace_buffer)
+        from . import _op  # noqa: F401  (registers the ops)
+
+        res = torch.ops.sqa.paged_attention_shared_prefix(
+            query, key_cache, value_cache, key_scale, value_scale, block_tables, seq_lens, words,
+            plan.numbers, plan.table, scale, float(out_scale), max_seq_len)
+        return res if out is None else out.copy_(res)
+    layout = sc.layout
+    seen = (layout(query), layout(key_cache), layout(value_cache), layout(key_scale),
+            layout(value_scale), layout(block_tables), layout(seq_lens), layout(words),
+            layout(out), workspace_buffer is None or workspace_buffer.device, max_seq_len)
+    known = plan.known.get(seen)
+    if known is None:
+        _check(query, key_cache, value_cache, key_scale, value_scale, block_tables, seq_lens, words,
+               plan, out, workspace_buffer)
+        known = plan.known.keep(seen, sc.on_device(query.device, _plan_call, query, key_cache,
+                                                   key_scale, block_tables, words, plan.plan,
+                                                   max_seq_len))
+    sc.check_aligned(16, query, key_cache, value_cache)
+    return sc.on_device(query.device, run_shared_prefix, query, key_cache, value_cache, key_scale,
+                        value_scale, block_tables, seq_lens, words, plan.plan, plan.table, scale,
+                        float(out_scale), max_seq_len, out, workspace_buffer, known)
+
+
+__all__ = ["SharedPrefixPlan", "plan_shared_prefix", "paged_attention_shared_prefix"]

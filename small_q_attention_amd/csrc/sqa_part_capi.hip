@@ -205,11 +205,13 @@ SharedTable table_of(int num_groups, int batch, long long num_items) {
   return t;
 }
 
-// Rows of a block: the widest group's, as one wave takes them, while they fit one.
+// Rows of a block: those of the widest group, as one wave takes them while they fit one,
+// else as a workgroup does.
 int rows_of_block(long long most, int head_dim) {
   if (most <= 16) return 16;
-  if (most <= 32 || head_dim == 256) return 32;
-  return 64;
+  if (most <= 32) return 32;
+  if (most <= 64 && head_dim != 256) return 64;
+  return most <= 128 || head_dim == 256 ? 128 : 256;
 }
 
 // Splits of `pages` pages of at most `size` each, all alike but for the last.
@@ -222,6 +224,7 @@ long long splits_of(long long pages, long long size) {
 struct SharedCut {
   int cus, num_kv_heads, block_rows;
   long long workgroups(long long items) const {
+    if (block_rows > 64) return items * num_kv_heads;
     const int wgh = wg_heads(num_kv_heads);
     return ceil_div(items, 4 / wgh) * ceil_div(num_kv_heads, wgh);
   }

@@ -283,13 +283,14 @@ int sqa_plan_scaled(int device, int batch, int num_kv_heads, int max_seq_len, in
 int sqa_paged_attention_scaled(const sqa_attention_args* args, const sqa_block_scales* scales);
 
 /*
- * Splits per sequence (*num_splits >= 1) of an sqa_paged_attention_windowed call whose
- * sequences have at most max_seq_len tokens (<= 0: as many as max_pages 16-token pages
- * hold). Any count serves any lengths; this one fills the device.
+ * The cut of an sqa_paged_attention_windowed call whose sequences have at most max_seq_len
+ * tokens (<= 0: as many as max_pages 16-token pages hold): splits per sequence (*num_splits
+ * >= 1) and kv heads per workgroup (*wg_heads 1, 2 or 4). Any cut serves any lengths; this
+ * one fills the device.
  */
 int sqa_plan_windowed(int device, int batch, int q_len, int num_query_heads, int num_kv_heads,
                       int head_dim, int64_t window, int sink, int max_seq_len, int max_pages,
-                      int* num_splits);
+                      int* num_splits, int* wg_heads);
 
 /*
  * sqa_paged_attention where row qi of sequence b, at position p = seq_lens[b] - q_len + qi,
@@ -297,16 +298,16 @@ int sqa_plan_windowed(int device, int batch, int q_len, int num_query_heads, int
  * p - window (window > 0, sink >= 0). Pages that no row sees are not read, their table
  * entries not used. kv_dtype: dtype, SQA_DTYPE_FP8_E4M3, or with `scales` (else NULL) e4m3
  * or int8 codes as for sqa_paged_attention_scaled; flags and pages_per_split 0, num_splits
- * from sqa_plan_windowed, workspace sqa_workspace_bytes(..., num_splits, 1) bytes (0 for one
- * split). A value that is not finite reaches the rows that see its token. Equal inputs and
- * splits give equal bits.
+ * and wg_heads from sqa_plan_windowed, workspace sqa_workspace_bytes(..., num_splits, 1)
+ * bytes (0 for one split). A value that is not finite reaches the rows that see its token.
+ * Equal inputs and cuts give equal bits.
  */
 int sqa_paged_attention_windowed(const sqa_attention_args* args, const sqa_block_scales* scales,
-                                 int64_t window, int sink);
+                                 int64_t window, int sink, int wg_heads);
 
 /*
- * What sqa_plan_shared_prefix decides, the shape it decided it for, and the sizes of the
- * table that goes with it. Read-only for callers, but for table_bytes.
+ * What sqa_plan_shared_prefix decides, and the shape it decided it for. Read-only for
+ * callers.
  */
 typedef struct sqa_shared_plan {
   size_t struct_size;
@@ -316,51 +317,44 @@ typedef struct sqa_shared_plan {
   int num_kv_heads;
   int head_dim;
   int page_size;
-  int num_groups;  /* that share something */
-  int num_items;
-  int block_rows;
-  int most_pages;  /* block_tables columns that the plan reads */
-  int least_pages; /* of them every sequence shares at least these */
-  int64_t partial_rows;
-  size_t table_bytes;
+  int num_groups;
+  int most_pages;    /* of a group, in block_tables columns */
+  int num_splits;    /* of what follows in a sequence */
+  int wg_heads;      /* kv heads of its workgroups */
+  int block_rows;    /* rows of a group that go over its pages together */
+  int shared_size;   /* most 16-token pages of a group's split */
+  int shared_splits; /* most splits of a group */
+  int num_items;     /* blocks x splits of all groups */
 } sqa_shared_plan;
 
 /*
- * Plans attention over a batch whose sequences share prefixes. groups: num_groups x (first,
- * count, pages): sequences first .. first + count - 1 begin with the same `pages` entries of
- * their block tables; in ascending order, apart, within the batch. Sequences of no group,
- * and groups of one sequence or no page, share nothing. Writes *plan, and, where `table` is
- * not NULL, the plan's table (table_bytes bytes of host memory, 8-byte aligned; a first call
- * with NULL tells how many): the caller copies it to the device. Lengths and pages may
- * change under a plan; only the shape, the groups and what they share are in it.
+ * Plans attention over a batch whose sequences share prefixes. groups (host memory):
+ * num_groups x (first, count, pages): sequences first .. first + count - 1 begin with the
+ * same `pages` entries of their block tables; in ascending order, apart, within the batch.
+ * Sequences of no group, and groups of one sequence or no page, share nothing. max_seq_len
+ * and max_pages (block_tables columns) as elsewhere: shared tokens counted, and only sizing
+ * the call. Lengths and page ids may change under a plan.
  */
 int sqa_plan_shared_prefix(int device, int batch, int q_len, int num_query_heads,
-                           int num_kv_heads, int head_dim, int page_size, int num_groups,
-                           const int32_t* groups, sqa_shared_plan* plan, void* table);
-
-/*
- * Splits (*num_splits >= 1) of what follows the shared pages, for sequences of at most
- * max_seq_len tokens (<= 0: as many as max_pages 16-token pages hold), shared ones counted.
- * Any count serves any lengths.
- */
-int sqa_plan_shared_own(int device, const sqa_shared_plan* plan, int max_seq_len, int max_pages,
-                        int* num_splits);
+                           int num_kv_heads, int head_dim, int page_size, int kv_dtype,
+                           int num_groups, const int32_t* groups, int max_seq_len, int max_pages,
+                           sqa_shared_plan* plan);
 
 /* Workspace bytes of a call (0: none needed, or not a plan). */
-size_t sqa_shared_workspace_bytes(const sqa_shared_plan* plan, int num_splits);
+size_t sqa_shared_workspace_bytes(const sqa_shared_plan* plan);
 
 /*
  * sqa_paged_attention of a batch with shared prefixes: the same result, the shared pages
- * read once for each group. `table`: the plan's, in device memory, 16-byte aligned. The
- * shared pages are read through the table row of the group's first sequence that reaches
- * past them with all of its rows (seq_lens[b] - q_len >= shared tokens); sequences that do
- * not (a padded batch's) go over their own pages from the first on. kv_dtype and `scales` as
- * for sqa_paged_attention_windowed; flags and pages_per_split 0, num_splits from
- * sqa_plan_shared_own. Equal inputs, plan and splits give equal bits.
+ * read once for each block of a group's rows. groups: those the plan was made for, in device
+ * memory. The shared pages are read through the table row of the group's first sequence
+ * that reaches past them with all of its rows (seq_lens[b] - q_len >= shared tokens);
+ * sequences that do not (a padded batch's) go over their own pages from the first on.
+ * kv_dtype and `scales` as for sqa_paged_attention_windowed; flags and pages_per_split 0,
+ * num_splits the plan's. Equal inputs and plans give equal bits.
  */
 int sqa_paged_attention_shared_prefix(const sqa_attention_args* args,
                                       const sqa_block_scales* scales, const sqa_shared_plan* plan,
-                                      const void* table);
+                                      const int32_t* groups);
 
 /*
  * Arguments of sqa_append_scaled (set struct_size = sizeof(sqa_append_args)).

@@ -34,14 +34,12 @@ _SIGNATURES = [
     ("sqa_plan_scaled", _C.c_int, [_C.c_int] * 5 + [_C.POINTER(_C.c_int)]),
     ("sqa_paged_attention_scaled", _C.c_int, [_C.c_void_p, _C.c_void_p]),
     ("sqa_plan_windowed", _C.c_int,
-     [_C.c_int] * 6 + [_C.c_int64] + [_C.c_int] * 3 + [_C.POINTER(_C.c_int)]),
+     [_C.c_int] * 6 + [_C.c_int64] + [_C.c_int] * 3 + [_C.POINTER(_C.c_int)] * 2),
     ("sqa_paged_attention_windowed", _C.c_int,
-     [_C.c_void_p, _C.c_void_p, _C.c_int64, _C.c_int]),
+     [_C.c_void_p, _C.c_void_p, _C.c_int64, _C.c_int, _C.c_int]),
     ("sqa_plan_shared_prefix", _C.c_int,
-     [_C.c_int] * 8 + [_C.c_void_p, _C.c_void_p, _C.c_void_p]),
-    ("sqa_plan_shared_own", _C.c_int,
-     [_C.c_int, _C.c_void_p, _C.c_int, _C.c_int, _C.POINTER(_C.c_int)]),
-    ("sqa_shared_workspace_bytes", _C.c_size_t, [_C.c_void_p, _C.c_int]),
+     [_C.c_int] * 9 + [_C.c_void_p, _C.c_int, _C.c_int, _C.c_void_p]),
+    ("sqa_shared_workspace_bytes", _C.c_size_t, [_C.c_void_p]),
     ("sqa_paged_attention_shared_prefix", _C.c_int,
      [_C.c_void_p, _C.c_void_p, _C.c_void_p, _C.c_void_p]),
     ("sqa_append_scaled", _C.c_int, [_C.c_void_p]),
@@ -88,12 +86,10 @@ class BlockScales(ctypes.Structure):
 class SharedPlan(ctypes.Structure):
     """``sqa_shared_plan`` of include/sqa.h."""
 
-    _fields_ = [("struct_size", _C.c_size_t), ("batch", _C.c_int), ("q_len", _C.c_int),
-                ("num_query_heads", _C.c_int), ("num_kv_heads", _C.c_int),
-                ("head_dim", _C.c_int), ("page_size", _C.c_int), ("num_groups", _C.c_int),
-                ("num_items", _C.c_int), ("block_rows", _C.c_int), ("most_pages", _C.c_int),
-                ("least_pages", _C.c_int), ("partial_rows", _C.c_int64),
-                ("table_bytes", _C.c_size_t)]
+    _fields_ = [("struct_size", _C.c_size_t)] + [(name, _C.c_int) for name in (
+        "batch", "q_len", "num_query_heads", "num_kv_heads", "head_dim", "page_size", "num_groups",
+        "most_pages", "num_splits", "wg_heads", "block_rows", "shared_size", "shared_splits",
+        "num_items")]
 
 
 class AppendArgs(ctypes.Structure):
@@ -368,16 +364,16 @@ def launch_scaled(query, output, k_view, v_view, k_scale, v_scale, block_tables,
 @functools.lru_cache(maxsize=4096)
 def plan_windowed(device_index: int, batch: int, q_len: int, num_query_heads: int,
                   num_kv_heads: int, head_dim: int, window: int, sink: int, max_seq_len: int,
-                  max_pages: int) -> int:
-    """``sqa_plan_windowed``: splits per sequence of a windowed call (``max_pages``: 16-token
-    pages)."""
+                  max_pages: int):
+    """``sqa_plan_windowed`` -> ``(num_splits, wg_heads)`` (``max_pages``: 16-token pages)."""
     lib = load()
-    ns = ctypes.c_int(0)
+    ns, heads = ctypes.c_int(0), ctypes.c_int(0)
     rc = lib.sqa_plan_windowed(device_index, batch, q_len, num_query_heads, num_kv_heads, head_dim,
-                               window, sink, max_seq_len, max_pages, ctypes.byref(ns))
+                               window, sink, max_seq_len, max_pages, ctypes.byref(ns),
+                               ctypes.byref(heads))
     if rc != SQA_OK:
         raise RuntimeError(f"sqa_plan_windowed failed: {last_error(lib)}")
-    return ns.value
+    return ns.value, heads.value
 
 
 def part_fields(query, k_view, k_scale, block_tables, draft_mask):
@@ -407,58 +403,44 @@ def _part_args(query, output, k_view, v_view, k_scale, v_scale, block_tables, se
 
 def launch_windowed(query, output, k_view, v_view, k_scale, v_scale, block_tables, seq_lens,
                     draft_mask, window: int, sink: int, scale: float, out_scale: float,
-                    num_splits: int, workspace, stream_handle: int, fields=None):
-    """Call ``sqa_paged_attention_windowed``: views and scales (or ``None``) as for
+                    cut, workspace, stream_handle: int, fields=None):
+    """Call ``sqa_paged_attention_windowed``: ``cut`` from :func:`plan_windowed`, views and scales (or ``None``) as for
     :func:`launch_scaled`, ``fields`` from :func:`part_fields`."""
     lib = _LIB if _LIB is not None else load()
     a, scales = _part_args(query, output, k_view, v_view, k_scale, v_scale, block_tables, seq_lens,
-                           draft_mask, scale, out_scale, num_splits, workspace, stream_handle,
+                           draft_mask, scale, out_scale, cut[0], workspace, stream_handle,
                            fields or part_fields(query, k_view, k_scale, block_tables, draft_mask))
-    if lib.sqa_paged_attention_windowed(a, scales, window, sink) != SQA_OK:
+    if lib.sqa_paged_attention_windowed(a, scales, window, sink, cut[1]) != SQA_OK:
         raise RuntimeError(f"sqa_paged_attention_windowed failed: {last_error(lib)}")
 
 
-def plan_shared_prefix(device_index: int, groups, batch: int, q_len: int, num_query_heads: int,
-                       num_kv_heads: int, head_dim: int, page_size: int):
-    """``sqa_plan_shared_prefix`` -> (:class:`SharedPlan`, table bytes); ``groups``: (first,
-    count, pages) triples."""
+@functools.lru_cache(maxsize=1024)
+def plan_shared_prefix(device_index: int, groups, shape, kv_dtype: int, max_seq_len: int,
+                       max_pages: int):
+    """``sqa_plan_shared_prefix`` -> (:class:`SharedPlan`, workspace bytes); ``groups``: a tuple
+    of (first, count, pages), ``shape``: (batch, q_len, query heads, kv heads, head_dim, page
+    size), ``max_pages``: block-table columns."""
     lib = load()
-    flat = [int(x) for g in groups for x in g]
-    given = (ctypes.c_int32 * max(len(flat), 1))(*flat)
+    flat = [x for g in groups for x in g]
     plan = SharedPlan()
-    shape = (device_index, batch, q_len, num_query_heads, num_kv_heads, head_dim, page_size,
-             len(flat) // 3, given, ctypes.byref(plan))
-    table = None
-    for _ in range(2):
-        if lib.sqa_plan_shared_prefix(*shape, table) != SQA_OK:
-            raise RuntimeError(f"sqa_plan_shared_prefix failed: {last_error(lib)}")
-        if table is None:
-            table = (ctypes.c_int64 * -(-plan.table_bytes // 8))()
-    return plan, bytes(table)[:plan.table_bytes]
-
-
-def plan_shared_own(device_index: int, plan, max_seq_len: int, max_pages: int):
-    """``(splits, workspace bytes)`` of a call under ``plan`` (``max_pages``: 16-token
-    pages)."""
-    lib = load()
-    ns = ctypes.c_int(0)
-    rc = lib.sqa_plan_shared_own(device_index, ctypes.byref(plan), max_seq_len, max_pages,
-                                 ctypes.byref(ns))
+    rc = lib.sqa_plan_shared_prefix(device_index, *shape, kv_dtype, len(groups),
+                                    (ctypes.c_int32 * max(len(flat), 1))(*flat), max_seq_len,
+                                    max_pages, ctypes.byref(plan))
     if rc != SQA_OK:
-        raise RuntimeError(f"sqa_plan_shared_own failed: {last_error(lib)}")
-    return ns.value, int(lib.sqa_shared_workspace_bytes(ctypes.byref(plan), ns.value))
+        raise RuntimeError(f"sqa_plan_shared_prefix failed: {last_error(lib)}")
+    return plan, int(lib.sqa_shared_workspace_bytes(ctypes.byref(plan)))
 
 
 def launch_shared_prefix(query, output, k_view, v_view, k_scale, v_scale, block_tables, seq_lens,
-                         draft_mask, plan, table, scale: float, out_scale: float, num_splits: int,
-                         workspace, stream_handle: int, fields=None):
-    """Call ``sqa_paged_attention_shared_prefix`` (``table``: the plan's, on the device; the
-    rest as for :func:`launch_windowed`)."""
+                         draft_mask, plan, groups, scale: float, out_scale: float, workspace,
+                         stream_handle: int, fields=None):
+    """Call ``sqa_paged_attention_shared_prefix`` (``plan`` from :func:`plan_shared_prefix`,
+    ``groups``: its groups on the device; the rest as for :func:`launch_windowed`)."""
     lib = _LIB if _LIB is not None else load()
     a, scales = _part_args(query, output, k_view, v_view, k_scale, v_scale, block_tables, seq_lens,
-                           draft_mask, scale, out_scale, num_splits, workspace, stream_handle,
+                           draft_mask, scale, out_scale, plan.num_splits, workspace, stream_handle,
                            fields or part_fields(query, k_view, k_scale, block_tables, draft_mask))
-    rc = lib.sqa_paged_attention_shared_prefix(a, scales, ctypes.byref(plan), table.data_ptr())
+    rc = lib.sqa_paged_attention_shared_prefix(a, scales, ctypes.byref(plan), groups.data_ptr())
     if rc != SQA_OK:
         raise RuntimeError(f"sqa_paged_attention_shared_prefix failed: {last_error(lib)}")
 

@@ -133,20 +133,20 @@ def paged_attention_shared_prefix(query: torch.Tensor, key_cache: torch.Tensor,
                                   value_cache: torch.Tensor, key_scale: Optional[torch.Tensor],
                                   value_scale: Optional[torch.Tensor], block_tables: torch.Tensor,
                                   seq_lens: torch.Tensor, draft_mask: Optional[torch.Tensor],
-                                  plan: List[int], table: torch.Tensor, scale: float,
+                                  groups: List[int], table: torch.Tensor, scale: float,
                                   out_scale: float, max_seq_len: int) -> torch.Tensor:
-    """Attention over shared prefixes (``shared_prefix``) under a plan of these numbers, given
-    its workspace at run time."""
+    """Attention over shared prefixes (``shared_prefix``) under a plan of these groups, cut and
+    given its workspace at run time."""
     from . import scaled_cache, shared_prefix
 
     return scaled_cache.on_device(query.device, lambda: shared_prefix.run_shared_prefix(
         query, key_cache, value_cache, key_scale, value_scale, block_tables, seq_lens, draft_mask,
-        _lib.SharedPlan(*plan), table, scale, out_scale, max_seq_len, None, None))
+        tuple(zip(groups[::3], groups[1::3], groups[2::3])), table, scale, out_scale, max_seq_len, None, None))
 
 
 @paged_attention_shared_prefix.register_fake
 def _paged_attention_shared_prefix_fake(query, key_cache, value_cache, key_scale, value_scale,
-                                        block_tables, seq_lens, draft_mask, plan, table, scale,
+                                        block_tables, seq_lens, draft_mask, groups, table, scale,
                                         out_scale, max_seq_len):
     return torch.empty_like(query)
 

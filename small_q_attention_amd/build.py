@@ -31,9 +31,11 @@ INCLUDE = REPO_DIR / "include"
 LIB_PATH = PKG_DIR / "libsqa.so"
 SOURCES = [CSRC / name for name in ("sqa_kernels.hip", "sqa_capi.hip", "sqa_scaled.hip",
                                     "sqa_evict.hip", "sqa_cache_capi.hip", "sqa_part.hip",
-                                    "sqa_shared.hip", "sqa_part_capi.hip")]
+                                    "sqa_groups.hip", "sqa_tiles_f16.hip", "sqa_tiles_bf16.hip",
+                                    "sqa_part_capi.hip")]
 HEADERS = [CSRC / "sqa_internal.h", CSRC / "sqa_device.h", CSRC / "sqa_cache_device.h",
-           CSRC / "sqa_cache.h", CSRC / "sqa_part.h", CSRC / "sqa_part_device.h", INCLUDE / "sqa.h"]
+           CSRC / "sqa_cache.h", CSRC / "sqa_part.h", CSRC / "sqa_part_device.h",
+           CSRC / "sqa_tiles.h", INCLUDE / "sqa.h"]
 ARCH = "gfx950"
 
 

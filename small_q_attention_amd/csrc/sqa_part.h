@@ -1,51 +1,50 @@
 // Internal interface between the C ABI (sqa_part_capi.hip) and the kernels of attention
-// over a part of every sequence (sqa_part.hip: a window and the first tokens, what follows
-// a shared prefix) and over the pages that a group of sequences shares (sqa_shared.hip).
+// over a part of every sequence (a window and the first tokens; what follows a shared
+// prefix) and over the pages that a group of sequences shares.
 #pragma once
 
 #include "sqa_cache.h"
 
 namespace sqa {
 
-// Sequences first .. first + count - 1, whose first `pages` 16-token pages are the same
-// ones. Their rows, count * rows of a kv head, go over those pages together, in
-// `splits` splits of `size` pages. Row r of sequence first + i, split j and kv head h leaves
-// its partial at row base + ((j * hkv + h) * count + i) * rows + r of the partials.
-struct SharedGroup {
-  int first, count;
-  int pages, splits, size;
-  int blocks;      // blocks of rows
-  long long base;
+// Splits of `pages` pages of at most `size`, all alike but for the last.
+struct EvenSplits {
+  int count, size;
 };
-
-// One workgroup's share, or one wave's where a group's rows fit one: a block of a group's
-// rows and a split of its pages (and one kv head, or each wave one).
-struct SharedItem {
-  int group, block, split, unused;
-};
+inline EvenSplits even_splits(long long pages, long long size) {
+  const long long n = (pages + size - 1) / size;
+  const long long each = n > 0 ? (pages + n - 1) / n : 1;
+  return {(int)((pages + each - 1) / each), (int)each};
+}
 
 struct PartArgs {
   // Of PartialArgs the fields that name buffers, shapes, strides and scales. part_o, part_ml:
-  // fp32 sums and (max in log2 units, sum) of the partial rows; sequence b's own splits are
-  // slots b * splits + s.
+  // fp32 sums and (max in log2 units, sum) of the partial rows. Slot s of sequence b and kv
+  // head h starts at row ((s * batch + b) * hkv + h) * rows; slots 0 .. splits - 1 are the
+  // sequence's own splits, splits + j its group's split j.
   PartialArgs p;
-  BlockScales scales;          // of codes with block scales
-  int kv_type, scaled;         // kF16 (the query's type), kE4M3 or kInt8
-  int wg_heads;                // kv heads a workgroup of single waves serves
-  int splits;                  // most splits of a sequence's own pages
-  long long window;            // a row sees the last `window` tokens up to its own (0: all)
-  int sink;                    // and the first `sink`
-  const SharedGroup* groups;   // null: none
-  const int32_t* group_of;     // [B], -1: none
-  const SharedItem* items;
-  int n_items;
-  long long shared_at;         // partial row of the groups' first one
-  FastDiv by_rows;             // p.rows
-  int block_rows;              // rows of a block: 16, 32 or 64 (one wave's), 128 or 256
+  BlockScales scales;      // of codes with block scales
+  int kv_type, scaled;     // kF16 (the query's type), kE4M3 or kInt8
+  int splits;              // most splits of a sequence's own pages
+  int wg_heads;            // kv heads a workgroup of single waves serves, 4 / wg_heads waves each
+  long long window;        // a row sees the last `window` tokens up to its own (0: all)
+  int sink;                // and the first `sink`
+  // Groups: n_groups x (first, count, pages): sequences first .. first + count - 1 begin with
+  // the same `pages` table entries. Their rows, count * rows of a kv head, go over those pages
+  // together, in blocks of block_rows (16, 32 or 64: one wave's; 128 or 256: a workgroup's)
+  // and splits of at most shared_size 16-token pages; n_items blocks x splits in all.
+  const int32_t* groups;
+  int n_groups, n_items, block_rows, shared_size;
+  int shared_splits;       // most splits of a group
+  int shared_wgs;          // workgroups that serve the groups, the first of the grid
+  FastDiv by_rows;         // p.rows
+  FastDiv by_shared_heads; // workgroups per item
 };
 
 hipError_t launch_own(const PartArgs& a, hipStream_t stream);
-hipError_t launch_shared(const PartArgs& a, hipStream_t stream);
+hipError_t launch_waves(const PartArgs& a, hipStream_t stream);  // groups of one wave's rows
+hipError_t launch_tiles_f16(const PartArgs& a, hipStream_t stream);  // of a workgroup's
+hipError_t launch_tiles_bf16(const PartArgs& a, hipStream_t stream);
 hipError_t launch_join(const PartArgs& a, hipStream_t stream);
 
 }  // namespace sqa

@@ -35,34 +35,31 @@ __global__ __launch_bounds__(256) void sqa_join_kernel(PartArgs args) {
   const int len = max(scalar_load(a.seq_lens + b), 0);
   const Span span = span_of(args, b, len);
   const int own = __builtin_amdgcn_readfirstlane(span.count);
-  if (!span.shared && own <= 1) return;  // uniform
-  const long long own_at = ((long long)b * args.splits * a.hkv + kvh) * a.rows + r;
-  const long long own_step = (long long)a.hkv * a.rows;
-  long long group_at = 0, group_step = 0;
-  int total = own;
-  if (span.shared) {  // uniform
-    const SharedGroup g = args.groups[scalar_load(args.group_of + b)];
-    group_at = args.shared_at + g.base + ((long long)kvh * g.count + (b - g.first)) * a.rows + r;
-    group_step = (long long)a.hkv * g.count * a.rows;
-    total += g.splits;
+  if (span.group.pages == 0 && own <= 1) return;  // uniform
+  int shared = 0;
+  if (span.group.pages > 0) {  // uniform
+    int size;
+    even_splits(span.group.pages, args.shared_size, &shared, &size);
+    shared = __builtin_amdgcn_readfirstlane(min(shared, args.shared_splits));
   }
-  auto place = [&](int j) {
-    return j < own ? own_at + j * own_step : group_at + (j - own) * group_step;
-  };
+  const int total = own + shared;
+  const long long at = ((long long)b * a.hkv + kvh) * a.rows + r;
+  const long long step = (long long)a.batch * a.hkv * a.rows;
+  auto place = [&](int j) { return at + (j < own ? j : args.splits + j - own) * step; };
   const int c = lane % CH, sg = lane / CH;
   float m = -INFINITY, l = 0.f;
   f4 acc = {0.f, 0.f, 0.f, 0.f};
   for (int j0 = 0; j0 < total; j0 += 64) {
     const int j = min(j0 + lane, total - 1);
     const float2 ml = *(const float2*)(a.part_ml + place(j) * 2);
-    // No key (l = 0): no weight, whatever the maximum.
-    const bool is = j0 + lane < total && ml.y != 0.f;
-    float top = is ? ml.x : -INFINITY;
+    const bool is = j0 + lane < total;
+    float top = is && ml.y != 0.f ? ml.x : -INFINITY;
 #pragma unroll
     for (int o = 1; o < 64; o *= 2) top = fmaxf(top, __shfl_xor(top, o));
     const float mn = fmaxf(m, top);
     const float base = mn == -INFINITY ? 0.f : mn;
-    const float w = is ? fast_exp2(ml.x - base) : 0.f;
+    // A NaN sum counts whatever the maxima; of a split that saw no key the sums are 0.
+    const float w = is ? (ml.y != ml.y ? 1.f : fast_exp2(ml.x - base)) : 0.f;
     float ls = is ? w * ml.y : 0.f;
 #pragma unroll
     for (int o = 1; o < 64; o *= 2) ls += __shfl_xor(ls, o);
@@ -81,7 +78,7 @@ __global__ __launch_bounds__(256) void sqa_join_kernel(PartArgs args) {
       for (int u = 0; u < U; ++u) {
         const int at = k + u * SG + sg;
         const float x = __shfl(w, min(at, 63));
-        if (at < n && x != 0.f) acc += o[u] * x;
+        if (at < n) acc += o[u] * x;
       }
     }
   }
@@ -101,7 +98,7 @@ __global__ __launch_bounds__(256) void sqa_join_kernel(PartArgs args) {
 }  // namespace
 
 hipError_t launch_own(const PartArgs& a, hipStream_t stream) {
-  const dim3 grid = part_grid(a, (long long)a.p.batch * a.splits);
+  const dim3 grid((unsigned)own_workgroups(a));
   if (a.p.bf16)
     launch_part<ElemBF16, false>(a, a.p.rows, grid, stream);
   else

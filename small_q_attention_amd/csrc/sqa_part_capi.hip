@@ -41,24 +41,43 @@ int check_shape(int batch, int q_len, int num_query_heads, int num_kv_heads, int
   return SQA_OK;
 }
 
-// kv heads a workgroup of single waves serves.
-int wg_heads(int num_kv_heads) { return num_kv_heads >= 3 ? 4 : num_kv_heads; }
+// How sequences' own pages are dealt to workgroups of four waves: `splits` shares a
+// sequence, `wg_heads` kv heads to a workgroup and 4 / wg_heads waves to a head.
+struct OwnCut {
+  int splits, wg_heads;
+  long long workgroups(long long batch, int num_kv_heads) const {
+    return batch * splits * ceil_div(num_kv_heads, wg_heads);
+  }
+  long long wave_pages(long long pages) const {
+    return ceil_div(ceil_div(pages, splits), 4 / wg_heads);
+  }
+};
 
-// Splits of sequences that span up to `pages` pages each: workgroups of four waves, one to
-// a compute unit, so that the rounds they take times (pages of a split + what a workgroup
-// costs besides, in pages) is least; two splits and more also pay for the join.
-long long own_splits(int cus, long long batch, int num_kv_heads, long long pages) {
-  constexpr long long kStart = 6, kJoin = 8;
-  const int wgh = wg_heads(num_kv_heads);
-  const long long head_groups = ceil_div(num_kv_heads, wgh);
-  const long long most = std::max(pages / sqa::kMinSplitPages, 1LL);
-  long long best = 1, best_cost = 0;
-  for (long long n = 1; n <= std::min(most, 256LL); ++n) {
-    const long long rounds = ceil_div(ceil_div(batch * n, 4 / wgh) * head_groups, cus);
-    const long long cost = rounds * (ceil_div(pages, n) + kStart) + (n > 1 ? kJoin : 0);
-    if (n == 1 || cost < best_cost) {
-      best = n;
-      best_cost = cost;
+// Rounds that `n` workgroups take on `cus` compute units, one to a unit: whole ones while
+// they are few, then (they end one by one) about as many as there is work for.
+double rounds_of(long long n, int cus) {
+  const double r = (double)n / cus;
+  return r <= 2 ? (double)ceil_div(n, cus) : r + 0.5;
+}
+
+// The cut of `batch` sequences of up to `pages` pages for which the rounds times (pages of a
+// wave + what a workgroup costs besides, in pages) is least; from two splits on the join
+// kernel costs too. Four heads to a workgroup where that is as good: neighbouring heads'
+// slices of a token are then read together.
+OwnCut own_cut(int cus, long long batch, int num_kv_heads, long long pages) {
+  constexpr double kStart = 6, kJoin = 7;
+  OwnCut best = {1, 1};
+  double best_cost = -1;
+  for (int heads = 4; heads >= 1; heads /= 2) {
+    if (heads / 2 >= num_kv_heads) continue;  // a smaller workgroup holds them all
+    for (int n = 1; n <= 256 && (n == 1 || n * sqa::kMinSplitPages <= pages); ++n) {
+      const OwnCut c = {n, heads};
+      const double cost = rounds_of(c.workgroups(batch, num_kv_heads), cus) *
+                              ((double)c.wave_pages(pages) + kStart) + (n > 1 ? kJoin : 0);
+      if (best_cost < 0 || cost < best_cost * 0.99) {
+        best = c;
+        best_cost = cost;
+      }
     }
   }
   return best;
@@ -73,7 +92,8 @@ long long window_pages(long long pages, long long window, long long sink, int q_
 }
 
 // The checks of a call and its kernel arguments, but for the plan.
-int fill(const sqa_attention_args& a, const sqa_block_scales* scales, sqa::PartArgs* out) {
+int fill(const sqa_attention_args& a, const sqa_block_scales* scales, int wg_heads,
+         sqa::PartArgs* out) {
   if (!a.query || !a.kv.k || !a.kv.v || !a.block_tables || !a.seq_lens || !a.output)
     return fail(SQA_ERR_INVALID, "null tensor pointer");
   long long rows = 0;
@@ -131,6 +151,8 @@ int fill(const sqa_attention_args& a, const sqa_block_scales* scales, sqa::PartA
   if (a.pages_per_split != 0)
     return fail(SQA_ERR_INVALID, "pages_per_split must be 0: the device cuts the pages");
   if (a.num_splits <= 0) return fail(SQA_ERR_INVALID, "num_splits must be positive");
+  if (wg_heads != 1 && wg_heads != 2 && wg_heads != 4)
+    return fail(SQA_ERR_INVALID, "wg_heads must be 1, 2 or 4, got %d", wg_heads);
 
   memset(out, 0, sizeof(*out));
   sqa::PartialArgs& p = out->p;
@@ -166,9 +188,9 @@ int fill(const sqa_attention_args& a, const sqa_block_scales* scales, sqa::PartA
                    (unsigned)(4 * scales->head_stride)};
   out->scaled = scales != nullptr;
   out->kv_type = codes ? (a.kv_dtype == SQA_DTYPE_INT8 ? sqa::kInt8 : sqa::kE4M3) : sqa::kF16;
-  out->wg_heads = wg_heads(a.num_kv_heads);
   out->splits = a.num_splits;
-  p.by_head_groups = sqa::fast_div((unsigned)ceil_div(a.num_kv_heads, out->wg_heads));
+  out->wg_heads = wg_heads;
+  p.by_head_groups = sqa::fast_div((unsigned)ceil_div(a.num_kv_heads, wg_heads));
   p.by_splits = sqa::fast_div(a.num_splits);
   p.by_group = sqa::fast_div(p.group);
   out->by_rows = sqa::fast_div(p.rows);
@@ -193,18 +215,6 @@ int place(const sqa_attention_args& a, long long rows, size_t need, sqa::PartArg
   return SQA_OK;
 }
 
-// Where the parts of a plan's table are, in bytes.
-struct SharedTable {
-  size_t group_of, items, bytes;
-};
-SharedTable table_of(int num_groups, int batch, long long num_items) {
-  SharedTable t;
-  t.group_of = (size_t)num_groups * sizeof(sqa::SharedGroup);
-  t.items = t.group_of + ((size_t)batch * 4 + 15) / 16 * 16;
-  t.bytes = t.items + (size_t)num_items * sizeof(sqa::SharedItem);
-  return t;
-}
-
 // Rows of a block: those of the widest group, as one wave takes them while they fit one,
 // else as a workgroup does.
 int rows_of_block(long long most, int head_dim) {
@@ -214,64 +224,89 @@ int rows_of_block(long long most, int head_dim) {
   return most <= 128 || head_dim == 256 ? 128 : 256;
 }
 
-// Splits of `pages` pages of at most `size` each, all alike but for the last.
-long long splits_of(long long pages, long long size) {
-  return ceil_div(pages, ceil_div(pages, ceil_div(pages, size)));
-}
+struct SharedGroup {
+  long long count, pages;  // 16-token pages
+};
 
-// Pages of a split, so that the rounds the groups' workgroups take times (pages of a split +
-// what a workgroup costs besides) is least.
+// The cut of a batch with groups, by a model of the call's time in microseconds. A workgroup
+// takes `page` for a page per wave of what waits for memory (a page of 16 x 128 16-bit
+// elements of K and V: between 0.65 and 1.05 as few or all compute units stream), `tile_page`
+// for a page of the tiles, whose blocks are bound by the matrix cores, and 6 or 10 besides;
+// n1 workgroups for the groups begin first, those for the sequences fill the units they
+// leave; a partial row is written and read once.
 struct SharedCut {
-  int cus, num_kv_heads, block_rows;
-  long long workgroups(long long items) const {
-    if (block_rows > 64) return items * num_kv_heads;
-    const int wgh = wg_heads(num_kv_heads);
-    return ceil_div(items, 4 / wgh) * ceil_div(num_kv_heads, wgh);
-  }
-  template <typename Groups>
-  long long pages(const Groups& groups, int num_groups) const {
-    constexpr long long kStart = 12;
-    long long longest = 1;
-    for (int g = 0; g < num_groups; ++g) longest = std::max(longest, (long long)groups(g).pages);
-    const auto items = [&](long long size) {
-      long long n = 0;
-      for (int g = 0; g < num_groups; ++g)
-        n += groups(g).blocks * ceil_div(groups(g).pages, size);
-      return n;
-    };
-    long long best = longest, best_cost = -1;
-    for (int rounds = 1; rounds <= 8; ++rounds) {
-      long long lo = sqa::kMinSplitPages, hi = std::max(longest, lo);  // the fewest that fit
-      while (lo < hi) {
-        const long long mid = (lo + hi) / 2;
-        if (workgroups(items(mid)) <= (long long)rounds * cus)
-          hi = mid;
-        else
-          lo = mid + 1;
+  OwnCut own;
+  long long size;  // most pages of a group's split
+};
+template <typename Groups>
+SharedCut shared_cut(int cus, long long batch, long long rows, int num_kv_heads, int head_dim,
+                     int kv_bytes, int block_rows, int num_groups, const Groups& group,
+                     long long own_pages) {
+  const double wide = head_dim / 128.0;
+  const double page = std::max(0.9 * wide * kv_bytes / 2, 0.35);
+  const double tile_page = (block_rows == 256 ? 0.6 : 0.35) * wide;
+  const bool tiles = block_rows > 64;
+  // Half of the room: sequences of a batch seldom all have the greatest length.
+  const double own_mean = std::max(0.6 * own_pages, 1.0);
+  long long longest = 1;
+  for (int g = 0; g < num_groups; ++g) longest = std::max(longest, group(g).pages);
+  SharedCut best{};
+  double best_cost = -1;
+  long long last_size = 0;
+  for (int heads = 4; heads >= 1; heads /= 2) {
+    if (heads / 2 >= num_kv_heads) continue;
+    const int waves = 4 / heads;
+    last_size = 0;
+    for (int n = 1; n <= 256 && (n == 1 || n * sqa::kMinSplitPages <= longest); ++n) {
+      const long long size = ceil_div(longest, n);
+      if (size == last_size) continue;
+      last_size = size;
+      long long items = 0, part = 0;
+      for (int g = 0; g < num_groups; ++g) {
+        const long long splits = sqa::even_splits(group(g).pages, size).count;
+        items += ceil_div(group(g).count * rows, block_rows) * splits;
+        part += group(g).count * splits;
       }
-      const long long real = ceil_div(workgroups(items(lo)), cus);
-      const long long cost = real * (lo + kStart);
-      if (best_cost < 0 || cost < best_cost) {
-        best = lo;
-        best_cost = cost;
+      const double n1 = (double)items * (tiles ? num_kv_heads : ceil_div(num_kv_heads, heads));
+      const double t1 = tiles ? size * tile_page + 10 : ceil_div(size, waves) * page + 6;
+      for (int m = 1; m <= 256 && (m == 1 || m * sqa::kMinSplitPages <= own_pages); m += m < 8 ? 1 : m / 4) {
+        const double splits = std::max(std::min((double)m, own_mean / sqa::kMinSplitPages), 1.0);
+        const double n2 = batch * splits * ceil_div(num_kv_heads, heads);
+        const double mean = own_mean / splits / waves, most = (double)own_pages / m / waves;
+        const double t2 = std::max(mean, 1.0) * page + 6;
+        const double work = (n1 * t1 + n2 * t2) / cus;
+        const double join = (part + batch * splits) * num_kv_heads * rows * head_dim * 8 / 4e6;
+        const double cost = std::max({t1 * ceil_div((long long)n1, cus), most * page + 6,
+                                      work + 0.5 * (n1 > cus ? std::max(t1, t2) : t2)}) + join;
+        if (best_cost < 0 || cost < best_cost * 0.99) {
+          best = {{m, heads}, size};
+          best_cost = cost;
+        }
       }
     }
-    return best;
   }
-};
+  return best;
+}
 
 int check_plan(const sqa_shared_plan* p) {
   if (!p) return fail(SQA_ERR_INVALID, "null plan");
   if (p->struct_size != sizeof(sqa_shared_plan))
     return fail(SQA_ERR_INVALID, "struct_size %zu does not match this library's %zu",
                 p->struct_size, sizeof(sqa_shared_plan));
-  if (p->num_groups < 0 || p->num_items < 0 || p->partial_rows < 0)
+  if (p->batch <= 0 || p->q_len <= 0 || p->num_kv_heads <= 0 || p->num_query_heads <= 0 ||
+      p->head_dim <= 0 || p->num_groups < 0 || p->num_items < 0 || p->num_splits <= 0 ||
+      p->shared_splits < 0 || p->shared_size <= 0)
     return fail(SQA_ERR_INVALID, "not a plan of sqa_plan_shared_prefix");
   return SQA_OK;
 }
 
+// Partial rows of a plan's slots.
+long long plan_rows(const sqa_shared_plan& p) {
+  return ((long long)p.num_splits + p.shared_splits) * p.batch * p.q_len * p.num_query_heads;
+}
+
 bool workgroups_fit(const sqa::PartArgs& s) {
-  return (long long)s.p.batch * s.splits * s.p.hkv <= 0x7fffffffLL;
+  return (long long)s.p.batch * s.splits * s.p.hkv <= 0x3fffffffLL;
 }
 
 }  // namespace
@@ -280,8 +315,8 @@ extern "C" {
 
 int sqa_plan_windowed(int device, int batch, int q_len, int num_query_heads, int num_kv_heads,
                       int head_dim, int64_t window, int sink, int max_seq_len, int max_pages,
-                      int* num_splits) {
-  if (!num_splits) return fail(SQA_ERR_INVALID, "null output pointer");
+                      int* num_splits, int* wg_heads) {
+  if (!num_splits || !wg_heads) return fail(SQA_ERR_INVALID, "null output pointer");
   long long rows = 0;
   if (int rc = check_shape(batch, q_len, num_query_heads, num_kv_heads, head_dim, &rows)) return rc;
   if (max_pages <= 0) return fail(SQA_ERR_INVALID, "max_pages must be positive");
@@ -292,12 +327,14 @@ int sqa_plan_windowed(int device, int batch, int q_len, int num_query_heads, int
   long long pages = max_pages;
   if (max_seq_len > 0) pages = std::min(pages, ceil_div(max_seq_len, sqa::kPageSize));
   pages = window_pages(pages, std::min(window, (int64_t)1 << 31), sink, q_len);
-  *num_splits = (int)own_splits(cus, batch, num_kv_heads, pages);
+  const OwnCut cut = own_cut(cus, batch, num_kv_heads, pages);
+  *num_splits = cut.splits;
+  *wg_heads = cut.wg_heads;
   return SQA_OK;
 }
 
 int sqa_paged_attention_windowed(const sqa_attention_args* args, const sqa_block_scales* scales,
-                                 int64_t window, int sink) {
+                                 int64_t window, int sink, int wg_heads) {
   if (!args) return fail(SQA_ERR_INVALID, "null argument struct");
   if (args->struct_size != sizeof(sqa_attention_args))
     return fail(SQA_ERR_INVALID, "struct_size %zu does not match this library's %zu",
@@ -306,7 +343,7 @@ int sqa_paged_attention_windowed(const sqa_attention_args* args, const sqa_block
   if (window <= 0 || sink < 0)
     return fail(SQA_ERR_INVALID, "window must be positive and sink not negative");
   sqa::PartArgs s;
-  if (int rc = fill(a, scales, &s)) return rc;
+  if (int rc = fill(a, scales, wg_heads, &s)) return rc;
   s.window = std::min(window, (int64_t)1 << 31);
   s.sink = sink;
   if (!workgroups_fit(s)) return fail(SQA_ERR_INVALID, "grid too large");
@@ -329,8 +366,9 @@ int sqa_paged_attention_windowed(const sqa_attention_args* args, const sqa_block
 }
 
 int sqa_plan_shared_prefix(int device, int batch, int q_len, int num_query_heads,
-                           int num_kv_heads, int head_dim, int page_size, int num_groups,
-                           const int32_t* groups, sqa_shared_plan* plan, void* table) {
+                           int num_kv_heads, int head_dim, int page_size, int kv_dtype,
+                           int num_groups, const int32_t* groups, int max_seq_len, int max_pages,
+                           sqa_shared_plan* plan) {
   if (!plan) return fail(SQA_ERR_INVALID, "null output pointer");
   long long rows = 0;
   if (int rc = check_shape(batch, q_len, num_query_heads, num_kv_heads, head_dim, &rows)) return rc;
@@ -340,50 +378,37 @@ int sqa_plan_shared_prefix(int device, int batch, int q_len, int num_query_heads
                 page_size);
   if (num_groups < 0 || (num_groups > 0 && !groups))
     return fail(SQA_ERR_INVALID, "null or negative groups");
+  if (max_pages <= 0) return fail(SQA_ERR_INVALID, "max_pages must be positive");
+  if (((long long)max_pages << shift) >= (1LL << 26))
+    return fail(SQA_ERR_INVALID, "block-table rows must be under 2^30 tokens");
   const int cus = sqa_device_cu_count(device);
   if (cus <= 0) return SQA_ERR_HIP;
   // A group of one sequence, or of no pages, shares nothing.
-  long long most_rows = 0, most_pages = 0, least = 0;
-  int shared = 0, end = 0, covered = 0;
+  const auto group = [&](int i) {
+    const bool shares = groups[3 * i + 1] > 1;
+    return SharedGroup{groups[3 * i + 1], shares ? (long long)groups[3 * i + 2] << shift : 0};
+  };
+  long long most_rows = 0, most_pages = 0, covered = 0, longest = 0;
+  int end = 0;
   for (int i = 0; i < num_groups; ++i) {
     const int first = groups[3 * i], count = groups[3 * i + 1], pages = groups[3 * i + 2];
     if (first < end || count <= 0 || pages < 0 || count > batch - first)
       return fail(SQA_ERR_INVALID,
                   "groups are (first, count, pages) in order, apart and within the batch");
-    if (((long long)pages << shift) >= (1LL << 26))
-      return fail(SQA_ERR_INVALID, "block-table rows must be under 2^30 tokens");
+    if (count > 1 && pages > max_pages)
+      return fail(SQA_ERR_INVALID, "a group shares %d pages, block_tables rows hold %d", pages,
+                  max_pages);
     end = first + count;
-    if (count == 1 || pages == 0) continue;
-    ++shared;
     covered += count;
+    if (group(i).pages == 0) continue;
     most_rows = std::max(most_rows, count * rows);
+    longest = std::max(longest, group(i).pages);
     most_pages = std::max(most_pages, (long long)pages);
-    least = shared == 1 ? pages : std::min(least, (long long)pages);
   }
-  const int block_rows = rows_of_block(most_rows, head_dim);
-  struct Group {
-    long long blocks, pages;
-    int first, count;
-  };
-  // The i-th group that shares something; groups are few beside the work they stand for.
-  const auto shared_group = [&](int want) {
-    for (int i = 0;; ++i) {
-      if (groups[3 * i + 1] == 1 || groups[3 * i + 2] == 0 || want-- > 0) continue;
-      return Group{ceil_div(groups[3 * i + 1] * rows, block_rows),
-                   (long long)groups[3 * i + 2] << shift, groups[3 * i], groups[3 * i + 1]};
-    }
-  };
-  const SharedCut cut{cus, num_kv_heads, block_rows};
-  const long long size = shared ? cut.pages(shared_group, shared) : 1;
-  long long items = 0, partial_rows = 0;
-  for (int g = 0; g < shared; ++g) {
-    const Group x = shared_group(g);
-    const long long splits = splits_of(x.pages, size);
-    items += x.blocks * splits;
-    partial_rows += splits * num_kv_heads * x.count * rows;
-  }
-  if (items * num_kv_heads > 0x7fffffffLL) return fail(SQA_ERR_INVALID, "grid too large");
-  const SharedTable t = table_of(shared, batch, items);
+  long long own = (long long)max_pages << shift;
+  if (max_seq_len > 0) own = std::min(own, ceil_div(max_seq_len, sqa::kPageSize));
+  // The longest sequences follow the longest prefix, where all share one.
+  if (covered == batch) own = std::max(own - longest, 1LL);
   sqa_shared_plan out;
   memset(&out, 0, sizeof(out));
   out.struct_size = sizeof(out);
@@ -393,59 +418,45 @@ int sqa_plan_shared_prefix(int device, int batch, int q_len, int num_query_heads
   out.num_kv_heads = num_kv_heads;
   out.head_dim = head_dim;
   out.page_size = page_size;
-  out.num_groups = shared;
-  out.num_items = (int)items;
-  out.block_rows = block_rows;
+  out.block_rows = 16;
+  out.shared_size = 1;
   out.most_pages = (int)most_pages;
-  out.least_pages = covered == batch ? (int)least : 0;
-  out.partial_rows = partial_rows;
-  out.table_bytes = t.bytes;
-  *plan = out;
-  if (!table) return SQA_OK;
-  sqa::SharedGroup* to = (sqa::SharedGroup*)table;
-  int32_t* group_of = (int32_t*)((char*)table + t.group_of);
-  sqa::SharedItem* item = (sqa::SharedItem*)((char*)table + t.items);
-  memset(table, 0, t.items);
-  for (int b = 0; b < batch; ++b) group_of[b] = -1;
-  long long base = 0;
-  for (int g = 0; g < shared; ++g) {
-    const Group x = shared_group(g);
-    const int splits = (int)splits_of(x.pages, size);
-    const int each = (int)ceil_div(x.pages, splits);
-    to[g] = {x.first, x.count, (int)x.pages, splits, each, (int)x.blocks, base};
-    base += (long long)splits * num_kv_heads * x.count * rows;
-    for (int b = x.first; b < x.first + x.count; ++b) group_of[b] = g;
-    for (int j = 0; j < splits; ++j)
-      for (int k = 0; k < x.blocks; ++k) *item++ = {g, k, j, 0};
+  if (longest == 0) {
+    const OwnCut cut = own_cut(cus, batch, num_kv_heads, own);
+    out.num_splits = cut.splits;
+    out.wg_heads = cut.wg_heads;
+  } else {
+    out.num_groups = num_groups;
+    out.block_rows = std::max(rows_of_block(most_rows, head_dim), rows_of_block(rows, head_dim));
+    const int bytes = kv_dtype == SQA_DTYPE_FP8_E4M3 || kv_dtype == SQA_DTYPE_INT8 ? 1 : 2;
+    const SharedCut cut = shared_cut(cus, batch, rows, num_kv_heads, head_dim, bytes,
+                                     out.block_rows, num_groups, group, own);
+    long long items = 0;
+    for (int i = 0; i < num_groups; ++i) {
+      const SharedGroup g = group(i);
+      const int splits = sqa::even_splits(g.pages, cut.size).count;
+      items += ceil_div(g.count * rows, out.block_rows) * splits;
+      out.shared_splits = std::max(out.shared_splits, splits);
+    }
+    if (items * num_kv_heads > 0x3fffffffLL) return fail(SQA_ERR_INVALID, "grid too large");
+    out.num_splits = cut.own.splits;
+    out.wg_heads = cut.own.wg_heads;
+    out.num_items = (int)items;
+    out.shared_size = (int)cut.size;
   }
+  *plan = out;
   return SQA_OK;
 }
 
-int sqa_plan_shared_own(int device, const sqa_shared_plan* plan, int max_seq_len, int max_pages,
-                        int* num_splits) {
-  if (!num_splits) return fail(SQA_ERR_INVALID, "null output pointer");
-  if (int rc = check_plan(plan)) return rc;
-  if (max_pages <= 0) return fail(SQA_ERR_INVALID, "max_pages must be positive");
-  const int cus = sqa_device_cu_count(device);
-  if (cus <= 0) return SQA_ERR_HIP;
-  long long pages = max_pages;
-  if (max_seq_len > 0) pages = std::min(pages, ceil_div(max_seq_len, sqa::kPageSize));
-  pages -= (long long)plan->least_pages * (plan->page_size / sqa::kPageSize);
-  *num_splits = (int)own_splits(cus, plan->batch, plan->num_kv_heads, std::max(pages, 1LL));
-  return SQA_OK;
-}
-
-size_t sqa_shared_workspace_bytes(const sqa_shared_plan* plan, int num_splits) {
-  if (check_plan(plan) || num_splits <= 0) return 0;
-  if (num_splits == 1 && plan->num_groups == 0) return 0;
-  const size_t rows = (size_t)plan->q_len * (plan->num_query_heads / plan->num_kv_heads);
-  const size_t own = (size_t)plan->batch * num_splits * plan->num_kv_heads * rows;
-  return (own + (size_t)plan->partial_rows) * ((size_t)plan->head_dim + 2) * sizeof(float);
+size_t sqa_shared_workspace_bytes(const sqa_shared_plan* plan) {
+  if (check_plan(plan)) return 0;
+  if (plan->num_splits == 1 && plan->num_items == 0) return 0;
+  return (size_t)plan_rows(*plan) * ((size_t)plan->head_dim + 2) * sizeof(float);
 }
 
 int sqa_paged_attention_shared_prefix(const sqa_attention_args* args,
                                       const sqa_block_scales* scales, const sqa_shared_plan* plan,
-                                      const void* table) {
+                                      const int32_t* groups) {
   if (!args) return fail(SQA_ERR_INVALID, "null argument struct");
   if (args->struct_size != sizeof(sqa_attention_args))
     return fail(SQA_ERR_INVALID, "struct_size %zu does not match this library's %zu",
@@ -453,39 +464,54 @@ int sqa_paged_attention_shared_prefix(const sqa_attention_args* args,
   if (int rc = check_plan(plan)) return rc;
   const sqa_attention_args& a = *args;
   sqa::PartArgs s;
-  if (int rc = fill(a, scales, &s)) return rc;
+  if (int rc = fill(a, scales, plan->wg_heads, &s)) return rc;
   if (plan->batch != a.batch || plan->q_len != a.q_len ||
       plan->num_query_heads != a.num_query_heads || plan->num_kv_heads != a.num_kv_heads ||
-      plan->head_dim != a.head_dim || plan->page_size != a.page_size)
-    return fail(SQA_ERR_INVALID, "the plan was made for another batch, q_len, heads or page size");
+      plan->head_dim != a.head_dim || plan->page_size != a.page_size ||
+      plan->num_splits != a.num_splits)
+    return fail(SQA_ERR_INVALID, "the plan was made for another batch, q_len, heads, page size or "
+                                 "number of splits");
   if (plan->most_pages > a.max_pages)
     return fail(SQA_ERR_INVALID, "the plan shares %d pages, block_tables rows hold %d",
                 plan->most_pages, a.max_pages);
-  if (plan->num_groups > 0) {
-    if (!table) return fail(SQA_ERR_INVALID, "null plan table");
-    if ((uintptr_t)table % 16) return fail(SQA_ERR_INVALID, "plan table must be 16-byte aligned");
-    const SharedTable t = table_of(plan->num_groups, plan->batch, plan->num_items);
-    s.groups = (const sqa::SharedGroup*)table;
-    s.group_of = (const int32_t*)((const char*)table + t.group_of);
-    s.items = (const sqa::SharedItem*)((const char*)table + t.items);
+  const bool tiles = plan->block_rows > 64;
+  if (plan->num_items > 0) {
+    if (!groups || (uintptr_t)groups % 4)
+      return fail(SQA_ERR_INVALID, "groups must be given, 4-byte aligned, in device memory");
+    const int b = plan->block_rows;
+    if ((b != 16 && b != 32 && b != 64 && b != 128 && b != 256) ||
+        (a.head_dim == 256 && (b == 64 || b == 256)) || (!tiles && b < s.p.rows))
+      return fail(SQA_ERR_INVALID, "not a plan of sqa_plan_shared_prefix");
+    s.groups = groups;
+    s.n_groups = plan->num_groups;
     s.n_items = plan->num_items;
-    s.block_rows = plan->block_rows;
+    s.block_rows = b;
+    s.shared_size = plan->shared_size;
+    s.shared_splits = plan->shared_splits;
+    const long long heads = tiles ? a.num_kv_heads : ceil_div(a.num_kv_heads, s.wg_heads);
+    if (heads * s.n_items > 0x3fffffffLL) return fail(SQA_ERR_INVALID, "grid too large");
+    s.shared_wgs = (int)(heads * s.n_items);
+    s.by_shared_heads = sqa::fast_div((unsigned)heads);
   }
   if (!workgroups_fit(s)) return fail(SQA_ERR_INVALID, "grid too large");
-  s.shared_at = (long long)a.batch * a.num_splits * a.num_kv_heads * s.p.rows;
-  const size_t need = sqa_shared_workspace_bytes(plan, a.num_splits);
-  if (int rc = place(a, s.shared_at + plan->partial_rows, need, &s)) return rc;
+  const size_t need = sqa_shared_workspace_bytes(plan);
+  if (int rc = place(a, plan_rows(*plan), need, &s)) return rc;
 
   hipStream_t stream = (hipStream_t)a.stream;
   hipEvent_t* ev = (hipEvent_t*)a.timing_events;
   hipError_t e;
   if (ev && (e = hipEventRecord(ev[0], stream)) != hipSuccess) return hip_fail(e, "hipEventRecord");
-  if (s.n_items > 0 && (e = sqa::launch_shared(s, stream)) != hipSuccess)
-    return hip_fail(e, "shared prefix kernel launch");
-  if ((e = sqa::launch_own(s, stream)) != hipSuccess)
-    return hip_fail(e, "own part kernel launch");
+  if (s.n_items == 0)
+    e = sqa::launch_own(s, stream);
+  else if (!tiles)
+    e = sqa::launch_waves(s, stream);
+  else if (s.p.bf16)
+    e = sqa::launch_tiles_bf16(s, stream);
+  else
+    e = sqa::launch_tiles_f16(s, stream);
+  if (e != hipSuccess) return hip_fail(e, "shared prefix attention kernel launch");
   if (ev && (e = hipEventRecord(ev[1], stream)) != hipSuccess) return hip_fail(e, "hipEventRecord");
-  if ((a.num_splits > 1 || s.n_items > 0) && (e = sqa::launch_join(s, stream)) != hipSuccess)
+  if (need > 0 && (e = sqa::launch_join(s, stream)) != hipSuccess)
     return hip_fail(e, "join kernel launch");
   if (ev && (e = hipEventRecord(ev[2], stream)) != hipSuccess) return hip_fail(e, "hipEventRecord");
   return SQA_OK;

@@ -8,13 +8,71 @@
 namespace sqa {
 namespace {
 
-// The kernel pages of a sequence that its own splits cover: [0, head) and [tail, head's
-// pages + tail ...): n pages in all, page v of them at() of the sequence.
+// ceil(n / d) with d the same in every lane.
+__device__ __forceinline__ int ceil_over(int n, int d) {
+  return ceil_quotient(n, d, __builtin_amdgcn_rcpf((float)d));
+}
+
+// even_splits() on the device (0 <= pages < 2^26, size > 0).
+__device__ __forceinline__ void even_splits(int pages, int size, int* count, int* each) {
+  const int n = ceil_over(pages, size);
+  *each = n > 0 ? ceil_quotient(pages, n, __builtin_amdgcn_rcpf((float)n)) : 1;
+  *count = ceil_quotient(pages, *each, __builtin_amdgcn_rcpf((float)*each));
+}
+
+// A group as the kernels use it: within the batch, its pages in 16 tokens; a group of one
+// sequence shares nothing (pages 0).
+struct Group {
+  int first, count, pages;
+};
+__device__ __forceinline__ Group load_group(const PartArgs& a, int i) {
+  const int32_t* g = a.groups + 3 * min(i, a.n_groups - 1);
+  Group x{g[0], g[1], g[2]};
+  x.first = min(max(x.first, 0), a.p.batch);
+  x.count = min(max(x.count, 0), a.p.batch - x.first);
+  x.pages = x.count > 1 && i < a.n_groups ? min(max(x.pages, 0), a.p.bt_stride) << a.p.page_shift
+                                          : 0;
+  return x;
+}
+__device__ __forceinline__ Group from_lane(const Group& g, int src) {
+  return {__builtin_amdgcn_readlane(g.first, src), __builtin_amdgcn_readlane(g.count, src),
+          __builtin_amdgcn_readlane(g.pages, src)};
+}
+
+// Sequence b's group (pages 0: none). The whole wave looks, a lane to a group.
+__device__ __forceinline__ Group group_of(const PartArgs& a, int b) {
+  for (int k = 0; k < a.n_groups; k += 64) {
+    const Group g = load_group(a, k + (threadIdx.x & 63));
+    const unsigned long long hit =
+        __ballot(g.pages > 0 && b >= g.first && b - g.first < g.count);
+    if (hit) return from_lane(g, __builtin_ctzll(hit));
+  }
+  return {0, 0, 0};
+}
+
+// Whether all rows of a sequence of `len` tokens lie behind `pages` shared pages.
+__device__ __forceinline__ bool reaches(const PartArgs& a, int len, int pages) {
+  return len >= a.p.q_len && (len - a.p.q_len) / kPageSize >= pages;
+}
+
+// The first sequence of a group that reaches past the shared pages, -1: none (then nobody
+// reads the group's partials). Its table row names the pages: a padded sequence's need not.
+__device__ __forceinline__ int leader_of(const PartArgs& a, const Group& g) {
+  const int lane = threadIdx.x & 63;
+  for (int i = 0; i < g.count; i += 64) {
+    const int b = g.first + min(i + lane, g.count - 1);
+    const unsigned long long hit = __ballot(reaches(a, a.p.seq_lens[b], g.pages));
+    if (hit) return g.first + min(i + (int)__builtin_ctzll(hit), g.count - 1);
+  }
+  return -1;
+}
+
+// The kernel pages that a sequence's own splits cover: [0, head) and from `tail` on, n in
+// all, page v of them at v or, past `head`, v - head + tail.
 struct Span {
   int head, tail, n;
   int count, size;  // splits and pages per split
-  bool shared;      // the pages before `tail` are a group's
-  __device__ __forceinline__ int at(int v) const { return v < head ? v : v - head + tail; }
+  Group group;      // pages > 0: shared, and before `tail`
 };
 
 // Window: of the pages before row 0's window (the earliest) only those of the first `sink`
@@ -25,27 +83,61 @@ __device__ __forceinline__ Span span_of(const PartArgs& a, int b, int len) {
   Span s;
   s.head = 0;
   s.tail = 0;
-  s.shared = false;
+  s.group = {0, 0, 0};
   if (a.window > 0) {
     const long long from = (long long)len - a.p.q_len + 1 - a.window;
     s.head = min((int)(((unsigned)a.sink + kPageSize - 1) / kPageSize), pages);
     s.tail = from > 0 ? (int)min(from / kPageSize, (long long)pages) : 0;
     s.tail = max(s.tail, s.head);
   }
-  if (a.groups != nullptr) {
-    const int g = scalar_load(a.group_of + b);
-    if (g >= 0) {
-      const int shared = scalar_load(&a.groups[g].pages);
-      s.shared = shared > 0 && (len - a.p.q_len) / kPageSize >= shared && len >= a.p.q_len;
-      s.tail = s.shared ? shared : 0;
+  if (a.n_groups > 0) {
+    const Group g = group_of(a, b);
+    if (reaches(a, len, g.pages)) {
+      s.group = g;
+      s.tail = g.pages;
     }
   }
   s.n = s.head + max(pages - s.tail, 0);
   // Splits of equal size, none of them under kMinSplitPages while there are two.
   const int most = max(min(a.splits, s.n / kMinSplitPages), 1);
-  s.size = max(ceil_quotient(s.n, most, __builtin_amdgcn_rcpf((float)most)), 1);
-  s.count = ceil_quotient(s.n, s.size, __builtin_amdgcn_rcpf((float)s.size));
+  s.size = max(ceil_over(s.n, most), 1);
+  s.count = ceil_over(s.n, s.size);
   return s;
+}
+
+// One item of the groups: a block of a group's rows over a split of its pages.
+struct SharedItem {
+  Group group;  // pages 0: no such item
+  int split, block, begin, n;  // pages begin .. begin + n
+};
+__device__ __forceinline__ SharedItem item_of(const PartArgs& a, int item) {
+  const int lane = threadIdx.x & 63;
+  SharedItem it{{0, 0, 0}, 0, 0, 0, 0};
+  int base = 0;
+  for (int k = 0; k < a.n_groups; k += 64) {
+    const Group g = load_group(a, k + lane);
+    int count, size;
+    even_splits(g.pages, a.shared_size, &count, &size);
+    const int blocks = (g.count * a.p.rows + a.block_rows - 1) / a.block_rows;
+    const int items = g.pages > 0 ? blocks * count : 0;
+    const int incl = wave_inclusive_scan_int(items);
+    const int first = base + incl - items;
+    const unsigned long long hit = __ballot(item >= first && item < first + items);
+    if (hit) {
+      const int src = __builtin_ctzll(hit);
+      it.group = from_lane(g, src);
+      const int at = item - __builtin_amdgcn_readlane(first, src);
+      const int per = __builtin_amdgcn_readlane(blocks, src);
+      it.split = __builtin_amdgcn_readfirstlane(at / per);
+      it.block = at - it.split * per;
+      const int each = __builtin_amdgcn_readlane(size, src);
+      it.begin = it.split * each;
+      it.n = max(min(each, it.group.pages - it.begin), 0);
+      return it;
+    }
+    base += __builtin_amdgcn_readlane(incl, 63);
+  }
+  return it;
 }
 
 // Values of a masked page that are not finite: in the PV product one would reach every row
@@ -115,17 +207,43 @@ __device__ __forceinline__ void wild_values(WaveState<NB, HD>& st, PageV<HD, 1>&
     }
 }
 
-// Leaves one wave's rows: normalised rows of the output, or fp32 sums and (max, sum) at
-// partial rows. Block nb's row slot r is real(nb, r); its partial row is first + 16 nb + r,
-// its place in the output out_row(nb, r) (in rows of HD). Through LDS one block at a time,
-// so that a store instruction writes whole rows (write_results() in sqa_device.h has the
-// figures); partial rows are fp32 for both types of queries, as after block scales.
-template <int NB, int HD, typename E, typename Real, typename OutRow>
-__device__ __forceinline__ void leave_rows(const PartialArgs& a, WaveState<NB, HD>& st,
-                                           float* stage, bool direct, long long first,
-                                           Real&& real, OutRow&& out_row) {
+// Where row x of a share is: x counts the rows of one kv head of the sequences from `first`
+// on, Q * (Hq / Hkv) each.
+struct RowMap {
+  int first, kvh, slot;
+  struct Place {
+    int b, y;  // sequence, row of its kv head
+  };
+  __device__ __forceinline__ Place place(const PartArgs& a, int x) const {
+    const int i = x / a.by_rows;
+    return {first + i, x - i * a.p.rows};
+  }
+  // In query and output, in rows of HD.
+  __device__ __forceinline__ long long out_row(const PartArgs& a, int x) const {
+    const Place p = place(a, x);
+    const int qi = p.y / a.p.by_group;
+    return ((long long)p.b * a.p.q_len + qi) * a.p.hq + kvh * a.p.group + (p.y - qi * a.p.group);
+  }
+  __device__ __forceinline__ long long part_row(const PartArgs& a, int x) const {
+    const Place p = place(a, x);
+    return (((long long)slot * a.p.batch + p.b) * a.p.hkv + kvh) * a.p.rows + p.y;
+  }
+};
+
+// Leaves the rows of one wave, or of the `waves` ones that have gone over pages of one share
+// (wave `mine` of them; their stages follow one another): normalised rows of the output, or
+// fp32 sums and (max, sum) at partial rows. Through LDS one block of 16 rows at a time, so
+// that a store instruction writes whole rows (write_results() in sqa_device.h has the
+// figures); partial rows are fp32 for both types of queries, as after block scales. Rows
+// row0 + 16 nb + r below n_rows are there; without `store` nothing is written.
+template <int NB, int HD, typename E>
+__device__ __forceinline__ void leave_rows(const PartArgs& args, WaveState<NB, HD>& st,
+                                           float* stage, int waves, int mine, bool direct,
+                                           const RowMap& map, int row0, int n_rows, bool store) {
+  const PartialArgs& a = args.p;
   constexpr int MB = Dims<HD>::MB;
   constexpr int kStageRow = HD + 4;
+  constexpr int kStage = 16 * kStageRow;
   constexpr int CPR = HD / 4;  // 4-value chunks per row
   const int lane = piece_tid() & 63;
   const int g16 = lane >> 4, l16 = lane & 15;
@@ -133,69 +251,68 @@ __device__ __forceinline__ void leave_rows(const PartialArgs& a, WaveState<NB, H
   for (int nb = 0; nb < NB; ++nb) st.l[nb] = xor_sum(st.l[nb]);
   const __amdgpu_buffer_rsrc_t pr = __builtin_amdgcn_make_buffer_rsrc(
       (void*)a.part_o, (short)0, (int)a.part_o_bytes, kBufferFlags);
+  float* own = stage + mine * kStage;
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) {
-    if (!real(nb, 0)) break;  // uniform
-    // l = 0: the row saw no key (written as 0). A NaN l passes.
-    const float inv_l = !(st.l[nb] <= 0.f) ? 1.f / st.l[nb] : 0.f;
-    const float sc = direct ? a.out_scale * inv_l : 1.f;
-    float* dst = stage + l16 * kStageRow + (HD / 4) * g16;
+    const int x0 = row0 + 16 * nb;
+    if (x0 >= n_rows) break;  // uniform over the waves of a share
+    float* dst = own + l16 * kStageRow + (HD / 4) * g16;
 #pragma unroll
     for (int rr = 0; rr < 4; ++rr)
 #pragma unroll
       for (int h = 0; h < MB / 4; ++h) {
         f4 o;
 #pragma unroll
-        for (int mb = 0; mb < 4; ++mb) o[mb] = st.acc[4 * h + mb][nb][rr] * sc;
+        for (int mb = 0; mb < 4; ++mb) o[mb] = st.acc[4 * h + mb][nb][rr];
         *(f4*)(dst + MB * rr + 4 * h) = o;
       }
-    // The staging rows are this wave's own: LDS keeps a wave's accesses in order, the
-    // fences keep the compiler from moving them.
-    __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
-    f4 v[CPR / 4];
-#pragma unroll
-    for (int i = 0; i < CPR / 4; ++i) {
-      const int e = i * 64 + lane;  // row e / CPR (< 16), chunk e % CPR
-      v[i] = *(const f4*)(stage + (e / CPR) * kStageRow + 4 * (e % CPR));
-    }
-    __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
-#pragma unroll
-    for (int i = 0; i < CPR / 4; ++i) {
+    // (max, sum) beside the row, where its padding is. A NaN sum travels with a finite max,
+    // so that it counts.
+    const float m_out = st.l[nb] == st.l[nb] ? st.m[nb] : 0.f;
+    if (g16 == 0) *(float2*)(own + l16 * kStageRow + HD) = float2{m_out, st.l[nb]};
+    if (waves > 1)  // uniform
+      __syncthreads();
+    else
+      __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+    // Chunk e % CPR of row e / CPR (< 16), the waves in turn.
+    for (int i = waves > 1 ? mine : 0; i < CPR / 4; i += waves) {
       const int e = i * 64 + lane;
       const int rs = e / CPR;
+      const float* row = stage + (waves > 1 ? 0 : mine * kStage) + rs * kStageRow;
+      float m = -INFINITY, l = 0.f;
+      f4 v = {0.f, 0.f, 0.f, 0.f};
+      for (int w = 0; w < waves; ++w) {
+        const float2 ml = *(const float2*)(row + w * kStage + HD);
+        m = ml.y != 0.f ? fmaxf(m, ml.x) : m;
+      }
+      const float base = m == -INFINITY ? 0.f : m;
+      for (int w = 0; w < waves; ++w) {
+        const float2 ml = *(const float2*)(row + w * kStage + HD);
+        const f4 o = *(const f4*)(row + w * kStage + 4 * (e % CPR));
+        const float f = waves == 1 || ml.y != ml.y ? 1.f : fast_exp2(ml.x - base);
+        v += o * f;
+        l += ml.y * f;
+      }
+      const bool is = store && x0 + rs < n_rows;
       if (direct) {
-        if (real(nb, rs)) {
-          const float o[4] = {v[i][0], v[i][1], v[i][2], v[i][3]};
-          *(u2*)(a.out + out_row(nb, rs) * HD + 4 * (e % CPR)) = E::pack4(o);
-        }
+        // l = 0: the row saw no key (written as 0). A NaN l passes.
+        const float sc = !(l <= 0.f) ? a.out_scale / l : 0.f;
+        const float o[4] = {v[0] * sc, v[1] * sc, v[2] * sc, v[3] * sc};
+        if (is) *(u2*)(a.out + map.out_row(args, x0 + rs) * HD + 4 * (e % CPR)) = E::pack4(o);
       } else {
-        const unsigned at = (unsigned)(((first + 16 * nb + rs) * HD + 4 * (e % CPR)) * 4);
-        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4, v[i]), pr,
-                                               real(nb, rs) ? at : kDroppedOffset, 0, kThroughAux);
+        const long long at = is ? map.part_row(args, x0 + rs) : 0;
+        __builtin_amdgcn_raw_buffer_store_b128(
+            __builtin_bit_cast(u4, v), pr,
+            is ? (unsigned)((at * HD + 4 * (e % CPR)) * 4) : kDroppedOffset, 0, kThroughAux);
+        if (is && e % CPR == 0)
+          store_through(a.part_ml + at * 2, __builtin_bit_cast(unsigned long long, float2{m, l}));
       }
     }
-    if (!direct && g16 == 0 && real(nb, l16)) {
-      // A NaN sum travels with a finite max, so the join counts the split.
-      const float m_out = st.l[nb] == st.l[nb] ? st.m[nb] : 0.f;
-      store_through(a.part_ml + (first + 16 * nb + l16) * 2,
-                    __builtin_bit_cast(unsigned long long, float2{m_out, st.l[nb]}));
-    }
+    if (waves > 1)  // uniform
+      __syncthreads();
+    else
+      __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
   }
-}
-
-// The first sequence of a group whose rows all lie behind the shared pages, -1: none (then
-// nobody reads the group's partials). Its table row names the pages: a padded sequence's
-// need not.
-__device__ __forceinline__ int leader_of(const PartArgs& a, const SharedGroup& g) {
-  const int lane = threadIdx.x & 63;
-  for (int i = 0; i < g.count; i += 64) {
-    const int b = g.first + min(i + lane, g.count - 1);
-    const int len = a.p.seq_lens[b];
-    const unsigned long long hit =
-        __ballot(len >= a.p.q_len && (len - a.p.q_len) / kPageSize >= g.pages);
-    if (hit) return g.first + min(i + (int)__builtin_ctzll(hit), g.count - 1);
-  }
-  return -1;
 }
 
 // How a cache's elements go to the products. kScaled: codes with block scales.
@@ -269,66 +386,77 @@ __device__ __forceinline__ void scaled_page(WaveState<NB, HD>& st, const typenam
   }
 }
 
-// One workgroup = four waves on their own, wave w with kv head w % wg_heads of the
-// workgroup's heads and share w / wg_heads of its shares; a share is a split of a
-// sequence's own pages (SHARED false) or a block of a group's rows over a split of the
-// shared pages (true; NB 16 rows at most). A wave holds all rows of its share and keeps a
-// ring of D pages in flight in registers; no barrier.
-template <int NB, int D, int HD, typename E, typename KV, bool SHARED>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1)))
-void sqa_part_kernel(PartArgs args) {
+// One workgroup = four waves, wave w with kv head w % wg_heads of the workgroup's heads; the
+// 4 / wg_heads waves of a head divide the pages of one share, each on its own, and join
+// their rows at the end. A share is a split of a sequence's own pages, or (`shared`) a block
+// of a group's rows over a split of the shared pages. A wave holds all rows of its share (NB
+// blocks of 16) and keeps a ring of D pages in flight in registers.
+template <int NB, int D, int HD, typename E, typename KV>
+__device__ __forceinline__ void part_share(const PartArgs& args, float* sm_stage, int block,
+                                           bool shared) {
   const PartialArgs& a = args.p;
   constexpr int KK = Dims<HD>::KK, MB = Dims<HD>::MB;
-  __shared__ float sm_stage[4 * 16 * (HD + 4)];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;
   const int g16 = lane >> 4, l16 = lane & 15;
   const int wgh = args.wg_heads;
-  const int rest = (int)blockIdx.x / a.by_head_groups;
-  const int kvh = ((int)blockIdx.x - rest * ((a.hkv + wgh - 1) / wgh)) * wgh + wave % wgh;
-  const int share = rest * (4 / wgh) + wave / wgh;
-  if (kvh >= a.hkv) return;
+  const int waves = wgh == 4 ? 1 : (wgh == 2 ? 2 : 4);
+  const int mine = wgh == 4 ? 0 : (wgh == 2 ? wave >> 1 : wave);
+  const int head_in = wgh == 4 ? wave : (wgh == 2 ? wave & 1 : 0);
+  const int share = block / a.by_head_groups;
+  const int kvh = (block - share * ((a.hkv + wgh - 1) / wgh)) * wgh + head_in;
 
-  // The share: its table row, the pages v0 .. v0 + n_pages of `span`, its rows.
-  Span span;
-  int b, len, v0, n_pages, row0 = 0, n_rows;
-  long long first;  // its first partial row
+  // The share: its table row, its pages v0 .. v0 + n_pages (page v of the sequence at v, or
+  // past `head` at v + skip), its rows.
+  int b, len, head = 0, skip = 0, v0, n_pages, row0 = 0, n_rows;
+  RowMap map;
+  map.kvh = kvh;
   bool direct = false;
-  if constexpr (SHARED) {
-    if (share >= args.n_items) return;
-    const SharedItem it = args.items[share];
-    const SharedGroup g = args.groups[__builtin_amdgcn_readfirstlane(it.group)];
-    const int split = __builtin_amdgcn_readfirstlane(it.split);
-    row0 = __builtin_amdgcn_readfirstlane(it.block) * (16 * NB);
-    b = __builtin_amdgcn_readfirstlane(leader_of(args, g));
-    if (b < 0) return;  // uniform
+  if (shared) {  // uniform
+    const SharedItem it = item_of(args, share);
+    b = it.group.pages > 0 ? leader_of(args, it.group) : -1;
+    if (b < 0 || it.split >= args.shared_splits) return;  // uniform over the workgroup
     len = 0x7fffffff;
-    span.head = 0;
-    span.tail = 0;
-    n_rows = __builtin_amdgcn_readfirstlane(g.count) * a.rows - row0;
-    v0 = split * __builtin_amdgcn_readfirstlane(g.size);
-    n_pages = max(min(v0 + __builtin_amdgcn_readfirstlane(g.size),
-                      min(__builtin_amdgcn_readfirstlane(g.pages), a.max_pages)) - v0, 0);
-    first = args.shared_at + g.base + ((long long)split * a.hkv + kvh) * g.count * a.rows + row0;
-    // Rows of all sequences of the group: from the group's first query on.
-    b = __builtin_amdgcn_readfirstlane(b);
+    row0 = it.block * (16 * NB);
+    n_rows = it.group.count * a.rows;
+    v0 = it.begin;
+    n_pages = it.n;
+    map.first = it.group.first;
+    map.slot = args.splits + it.split;
   } else {
-    if (share >= a.batch * args.splits) return;
     b = share / a.by_splits;
+    if (b >= a.batch) return;  // uniform over the workgroup
     const int split = share - b * args.splits;
     len = max(scalar_load(a.seq_lens + b), 0);
-    span = span_of(args, b, len);
-    direct = !span.shared && span.count <= 1;
-    if (split >= max(span.count, 1)) return;  // uniform
+    const Span span = span_of(args, b, len);
+    if (split >= max(span.count, 1)) return;  // uniform over the workgroup
+    direct = span.group.pages == 0 && span.count <= 1;
+    head = span.head;
+    skip = span.tail - span.head;
     v0 = split * span.size;
     n_pages = max(min(v0 + span.size, span.n) - v0, 0);
     n_rows = a.rows;
-    first = ((long long)share * a.hkv + kvh) * a.rows;
+    map.first = b;
+    map.slot = split;
   }
+  if (waves > 1) {  // uniform: this wave's part of the share
+    const int each = (n_pages + waves - 1) >> (waves == 2 ? 1 : 2);
+    v0 += mine * each;
+    n_pages = max(min(each, n_pages - mine * each), 0);
+  }
+  // No such head: nothing to do, but to wait with the other heads' waves.
+  const bool is_head = kvh < a.hkv;
+  if (!is_head) {
+    n_pages = 0;
+    map.kvh = 0;
+  }
+  b = __builtin_amdgcn_readfirstlane(b);
   v0 = __builtin_amdgcn_readfirstlane(v0);
   n_pages = __builtin_amdgcn_readfirstlane(n_pages);
-  const int head = __builtin_amdgcn_readfirstlane(span.head);
-  const int skip = __builtin_amdgcn_readfirstlane(span.tail - span.head);
+  row0 = __builtin_amdgcn_readfirstlane(row0);
+  n_rows = __builtin_amdgcn_readfirstlane(n_rows);
+  head = __builtin_amdgcn_readfirstlane(head);
+  skip = __builtin_amdgcn_readfirstlane(skip);
   auto page_at = [&](int v) { return v < head ? v : v + skip; };
   const int shift = a.page_shift, sub_mask = (1 << shift) - 1;
 
@@ -344,48 +472,33 @@ void sqa_part_kernel(PartArgs args) {
   load_ids(0, first_ids);
   load_ids(D, ids);
 
-  auto real = [&](int nb, int r) { return 16 * nb + r < n_rows; };
-  // Place of a row in query and output, in rows of HD.
-  auto out_row = [&](int nb, int r) -> long long {
-    const int x = row0 + 16 * nb + r;
-    int i = 0, y = x;
-    long long at = b;
-    if constexpr (SHARED) {
-      i = x / args.by_rows;
-      y = x - i * a.rows;
-      at = args.groups[args.items[share].group].first + i;
-    }
-    const int qi = y / a.by_group;
-    return (at * a.q_len + qi) * a.hq + kvh * a.group + (y - qi * a.group);
-  };
   u4 q[NB][KK];
   RegBits<NB> bits;
   int from[NB];  // first token of the row's window
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) {
-    const bool is = real(nb, l16);
-    const _Float16* qp = a.q + (is ? out_row(nb, l16) : out_row(0, 0)) * HD;
+    const int x = row0 + 16 * nb + l16;
+    const bool is = x < n_rows;
+    const _Float16* qp = a.q + map.out_row(args, is ? x : row0) * HD;
 #pragma unroll
     for (int kk = 0; kk < KK; ++kk) {
       const u4 x = *(const u4*)(qp + KV::q_dims(kk, g16));
       q[nb][kk] = is ? x : u4{0u, 0u, 0u, 0u};
     }
-    if constexpr (!SHARED) {
-      const int qi = is ? (16 * nb + l16) / a.by_group : 0;
-      bits.b[nb] = draft_bits(a, b, qi, is);
-      from[nb] = args.window > 0
-                     ? (int)max((long long)len - a.q_len + qi + 1 - args.window, 0LL) : 0;
-    }
+    const int qi = map.place(args, is ? x : row0).y / a.by_group;
+    bits.b[nb] = draft_bits(a, b, qi, is);
+    from[nb] = args.window > 0
+                   ? (int)max((long long)len - a.q_len + qi + 1 - args.window, 0LL) : 0;
   }
 
   const unsigned tok_bytes = a.token_stride;
-  const unsigned k_lane = l16 * tok_bytes + kvh * a.head_stride + KV::k_lane_bytes(g16);
-  const unsigned v_lane = 4 * g16 * tok_bytes + kvh * a.head_stride + KV::v_lane_bytes(l16);
+  const unsigned k_lane = l16 * tok_bytes + map.kvh * a.head_stride + KV::k_lane_bytes(g16);
+  const unsigned v_lane = 4 * g16 * tok_bytes + map.kvh * a.head_stride + KV::v_lane_bytes(l16);
   const size_t sub_bytes = (size_t)kPageSize * tok_bytes;
   // Lanes 0-31 load the page's K scale, 32-63 its V scale.
   const char* scale_lane = KV::kScaled
                                ? (const char*)(lane < 32 ? args.scales.k : args.scales.v) +
-                                     (size_t)kvh * args.scales.head_stride
+                                     (size_t)map.kvh * args.scales.head_stride
                                : nullptr;
   struct Slot {
     typename KV::Regs kv;
@@ -418,11 +531,10 @@ void sqa_part_kernel(PartArgs args) {
 #pragma unroll
     for (int mb = 0; mb < MB; ++mb) st.acc[mb][nb] = f4{0.f, 0.f, 0.f, 0.f};
   }
-  // Masked pages: with a token from the draft block on, or before the last row's window and
-  // past the first tokens.
+  // Masked pages: with a token from the draft block on (never a shared page: `len`), or
+  // before the last row's window and past the first tokens.
   const int mask_from = len - a.q_len;
-  const int all_from = SHARED || args.window <= 0
-                           ? 0 : (int)max((long long)len - args.window, 0LL);
+  const int all_from = args.window > 0 ? (int)max((long long)len - args.window, 0LL) : 0;
 
   for (int i = 0; i < n_pages; i += D) {
     load_ids(i + 2 * D, ids_next);
@@ -432,8 +544,8 @@ void sqa_part_kernel(PartArgs args) {
       if (ii < n_pages) {
         const int p = page_at(v0 + ii);
         const int t0 = p * kPageSize;
-        const bool masked = !SHARED && (t0 + kPageSize > mask_from ||
-                                        (t0 < all_from && t0 + kPageSize > args.sink));
+        const bool masked = t0 + kPageSize > mask_from ||
+                            (t0 < all_from && t0 + kPageSize > args.sink);  // uniform
         f4 s[NB];
         code_scores<NB, HD, E, KV>(s, ring[j].kv, q);
         auto mask = [&] {
@@ -458,21 +570,17 @@ void sqa_part_kernel(PartArgs args) {
           const float inv_vs = loud ? __builtin_amdgcn_rcpf(vs) : 0x1p64f;
           float c = a.scale_log2 * ks, add = lv;
           if (masked) {
-            if constexpr (!SHARED) {
-              // After the scales, so that one of 0, infinity or NaN leaves them -inf.
+            // After the scales, so that one of 0, infinity or NaN leaves them -inf.
 #pragma unroll
-              for (int nb = 0; nb < NB; ++nb) s[nb] = s[nb] * c + lv;
-              c = 1.f;
-              add = 0.f;
-              mask();
-              if constexpr (KV::kNan) nan_values<NB, HD, KV>(st, ring[j].kv, s);
-            }
+            for (int nb = 0; nb < NB; ++nb) s[nb] = s[nb] * c + lv;
+            c = 1.f;
+            add = 0.f;
+            mask();
+            if constexpr (KV::kNan) nan_values<NB, HD, KV>(st, ring[j].kv, s);
           }
           scaled_page<NB, HD, KV>(st, ring[j].kv, s, masked, c, add, inv_vs, loud);
         } else {
-          if (masked) {
-            if constexpr (!SHARED) mask();
-          }
+          if (masked) mask();
           plain_page<NB, HD, E, KV>(st, ring[j].kv, s, masked, a.scale_log2, a.bf16);
         }
       }
@@ -482,49 +590,59 @@ void sqa_part_kernel(PartArgs args) {
 #pragma unroll
     for (int j = 0; j < D; ++j) ids[j] = ids_next[j];
   }
-  leave_rows<NB, HD, E>(a, st, sm_stage + wave * 16 * (HD + 4), direct, first, real, out_row);
+  leave_rows<NB, HD, E>(args, st, sm_stage + head_in * waves * 16 * (HD + 4), waves, mine, direct,
+                        map, row0, n_rows, is_head);
+}
+
+// GROUPS: the first shared_wgs workgroups serve the groups, the others sequences.
+template <int NB, int D, int HD, typename E, typename KV, bool GROUPS>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1)))
+void sqa_part_kernel(PartArgs args) {
+  __shared__ float sm_stage[4 * 16 * (HD + 4)];
+  const bool shared = GROUPS && (int)blockIdx.x < args.shared_wgs;
+  part_share<NB, D, HD, E, KV>(args, sm_stage, GROUPS && !shared ? blockIdx.x - args.shared_wgs
+                                                                 : blockIdx.x, shared);
 }
 
 // Ring depths: about 32 KiB of a 16-bit cache or 16 of codes in flight per wave, half of
 // that at 33 to 64 rows, whose accumulators take the registers.
-template <int HD, typename E, typename KV, bool SHARED>
+template <int HD, typename E, typename KV, bool GROUPS>
 void launch_part_hd(const PartArgs& a, int rows, dim3 grid, hipStream_t stream) {
   constexpr int D = 4 * 128 / HD;
   const dim3 block(256);
   if (rows <= 16)
-    hipLaunchKernelGGL((sqa_part_kernel<1, D, HD, E, KV, SHARED>), grid, block, 0, stream, a);
+    hipLaunchKernelGGL((sqa_part_kernel<1, D, HD, E, KV, GROUPS>), grid, block, 0, stream, a);
   else if (rows <= 32)
-    hipLaunchKernelGGL((sqa_part_kernel<2, D, HD, E, KV, SHARED>), grid, block, 0, stream, a);
+    hipLaunchKernelGGL((sqa_part_kernel<2, D, HD, E, KV, GROUPS>), grid, block, 0, stream, a);
   else if constexpr (HD != 256)
-    hipLaunchKernelGGL((sqa_part_kernel<4, D / 2, HD, E, KV, SHARED>), grid, block, 0, stream, a);
+    hipLaunchKernelGGL((sqa_part_kernel<4, D / 2, HD, E, KV, GROUPS>), grid, block, 0, stream, a);
 }
 
-template <typename E, template <int> class KV, bool SHARED>
+template <typename E, template <int> class KV, bool GROUPS>
 void launch_part_as(const PartArgs& a, int rows, dim3 grid, hipStream_t stream) {
   if (a.p.head_dim == 64)
-    launch_part_hd<64, E, KV<64>, SHARED>(a, rows, grid, stream);
+    launch_part_hd<64, E, KV<64>, GROUPS>(a, rows, grid, stream);
   else if (a.p.head_dim == 128)
-    launch_part_hd<128, E, KV<128>, SHARED>(a, rows, grid, stream);
+    launch_part_hd<128, E, KV<128>, GROUPS>(a, rows, grid, stream);
   else
-    launch_part_hd<256, E, KV<256>, SHARED>(a, rows, grid, stream);
+    launch_part_hd<256, E, KV<256>, GROUPS>(a, rows, grid, stream);
 }
 
-template <typename E, bool SHARED>
+template <typename E, bool GROUPS>
 void launch_part(const PartArgs& a, int rows, dim3 grid, hipStream_t stream) {
   if (a.scaled && a.kv_type == kInt8)
-    launch_part_as<E, PartCodesInt8, SHARED>(a, rows, grid, stream);
+    launch_part_as<E, PartCodesInt8, GROUPS>(a, rows, grid, stream);
   else if (a.scaled)
-    launch_part_as<E, PartCodesFp8, SHARED>(a, rows, grid, stream);
+    launch_part_as<E, PartCodesFp8, GROUPS>(a, rows, grid, stream);
   else if (a.kv_type == kE4M3)
-    launch_part_as<E, PartFp8, SHARED>(a, rows, grid, stream);
+    launch_part_as<E, PartFp8, GROUPS>(a, rows, grid, stream);
   else
-    launch_part_as<E, PartNative, SHARED>(a, rows, grid, stream);
+    launch_part_as<E, PartNative, GROUPS>(a, rows, grid, stream);
 }
 
-dim3 part_grid(const PartArgs& a, long long shares) {
-  const int head_groups = (a.p.hkv + a.wg_heads - 1) / a.wg_heads;
-  const int per_wg = 4 / a.wg_heads;
-  return dim3((unsigned)((shares + per_wg - 1) / per_wg * head_groups));
+// Workgroups that the sequences' own splits take.
+inline long long own_workgroups(const PartArgs& a) {
+  return (long long)a.p.batch * a.splits * ((a.p.hkv + a.wg_heads - 1) / a.wg_heads);
 }
 
 }  // namespace

@@ -1,0 +1,529 @@
+// Attention over the pages that a group of sequences shares, where its rows are more than
+// one wave holds: the rows of all of them, count * Q * (Hq / Hkv) of a kv head, against one K
+// and V, so that a page is read once for a block of rows and not once for each sequence.
+#pragma once
+
+#include "sqa_part.h"
+#include "sqa_part_device.h"
+
+namespace sqa {
+namespace {
+
+typedef float f16v __attribute__((ext_vector_type(16)));
+typedef short s4v __attribute__((ext_vector_type(4)));
+
+// Products over 16 k: operands of 8 elements per lane (lane l: m or n = l % 32, k = 8 (l / 32)
+// + 0 .. 7), results in 16 registers (r: m = 8 (r / 4) + 4 (l / 32) + r % 4, n = l % 32).
+template <typename E>
+__device__ __forceinline__ f16v mma32(u4 a, u4 b, f16v c) {
+  if constexpr (E::kHalfPartials)
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, a),
+                                                  __builtin_bit_cast(h8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8, a),
+                                                   __builtin_bit_cast(b8, b), c, 0, 0, 0);
+}
+
+constexpr int kTilePages = 4;                      // 64 keys
+constexpr int kTileKeys = kTilePages * kPageSize;
+
+// A tile of 64 rows (tokens) of HD 16-bit elements in LDS. The 16-byte chunks of a row are
+// permuted by the row, so that neither eight rows' reads of one chunk (K) nor four rows'
+// reads of 64 neighbouring bytes (V, transposed) meet in a bank.
+template <int HD>
+struct Tile {
+  static constexpr int kRow = 2 * HD;  // bytes
+  static constexpr int kBytes = kTileKeys * kRow;
+  static __device__ __forceinline__ int swizzle(int row) {
+    if constexpr (HD == 64)
+      return ((row >> 1) & 1) << 2 | ((row >> 2) & 3);
+    else
+      return (row & 3) << 2 | ((row >> 2) & 3);
+  }
+  static __device__ __forceinline__ int at(int row, int chunk) {
+    return row * kRow + ((chunk ^ swizzle(row)) << 4);
+  }
+};
+
+// How a page travels from memory to LDS: 16-byte loads, 16-bit elements kept, codes widened
+// (exactly) as they are stored.
+template <int HD, int BYTES>
+struct PageLoads {
+  static constexpr int kLanes = HD * BYTES / 16;     // lanes per token
+  static constexpr int kTokens = 64 / kLanes;        // tokens per load
+  static constexpr int kLoads = kPageSize / kTokens;
+  u4 x[kLoads];
+  __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t r, unsigned lane_at, unsigned tok) {
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i)
+      x[i] = __builtin_amdgcn_raw_buffer_load_b128(r, lane_at, i * kTokens * tok, 0);
+  }
+};
+
+struct StoreNative {
+  static constexpr int kBytes = 2;
+  static constexpr bool kScaled = false;
+  template <typename E>
+  static __device__ __forceinline__ void widen(u4 x, u4 (&to)[1]) { to[0] = x; }
+};
+struct StoreFp8 {
+  static constexpr int kBytes = 1;
+  static constexpr bool kScaled = false;
+  template <typename E>
+  static __device__ __forceinline__ void widen(u4 x, u4 (&to)[2]) {
+    to[0] = E::widen_fp8(u2{x[0], x[1]});
+    to[1] = E::widen_fp8(u2{x[2], x[3]});
+  }
+};
+struct StoreCodesFp8 : StoreFp8 {
+  static constexpr bool kScaled = true;
+};
+struct StoreCodesInt8 {
+  static constexpr int kBytes = 1;
+  static constexpr bool kScaled = true;
+  template <typename E>
+  static __device__ __forceinline__ void widen(u4 x, u4 (&to)[2]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      auto byte = [&](int e) { return (float)(signed char)(x[i] >> (8 * e)); };
+      to[i / 2][2 * (i & 1)] = E::pack2(byte(0), byte(1));
+      to[i / 2][2 * (i & 1) + 1] = E::pack2(byte(2), byte(3));
+    }
+  }
+};
+
+// One workgroup: a block of 128 NBW of a group's rows of one kv head, 32 NBW to a wave, over
+// one split of the shared pages, 64 keys at a time. Each wave brings one of a tile's four
+// pages to LDS, two buffers in turn; all waves read all of it.
+//
+// S^T = K Q^T leaves a lane with half of the keys of its row, so that maxima and sums stay
+// in the lane but for one exchange between two lanes; O^T = V^T P^T takes P from those
+// registers as they are: the product's k order is the order the registers hold the keys in,
+// and V comes transposed from LDS in the same order.
+template <int HD, int NBW, typename E, typename KV>
+struct TileShare {
+  using EV = std::conditional_t<KV::kScaled, ElemF16, E>;  // type of P and V
+  using T = Tile<HD>;
+  using Loads = PageLoads<HD, KV::kBytes>;
+  static constexpr int KS = HD / 16;  // k steps of the scores
+  static constexpr int MB = HD / 32;  // blocks of 32 output dims
+  static constexpr int kStageRow = HD + 4;
+  static constexpr int kStage = 4 * 32 * kStageRow * 4;
+  static constexpr int kLds = 4 * T::kBytes > kStage ? 4 * T::kBytes : kStage;
+
+  static __device__ __forceinline__ void run(const PartArgs& args, char* lds,
+                                             float (&lds_scale)[2][2][kTilePages], int block) {
+  const PartialArgs& a = args.p;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+  const int l32 = lane & 31, h = lane >> 5;
+  const int share = block / args.by_shared_heads;
+  const int kvh = block - share * a.hkv;
+  const SharedItem it = item_of(args, share);
+  const int b = it.group.pages > 0 ? __builtin_amdgcn_readfirstlane(leader_of(args, it.group)) : -1;
+  if (b < 0 || it.split >= args.shared_splits) return;  // uniform over the workgroup
+  const int first_page = __builtin_amdgcn_readfirstlane(it.begin);
+  const int n_pages = __builtin_amdgcn_readfirstlane(it.n);
+  const int tiles = (n_pages + kTilePages - 1) / kTilePages;
+  const int row0 = __builtin_amdgcn_readfirstlane(it.block) * (128 * NBW) + wave * (32 * NBW);
+  const int n_rows = __builtin_amdgcn_readfirstlane(it.group.count) * a.rows;
+  const RowMap map{__builtin_amdgcn_readfirstlane(it.group.first), kvh,
+                   args.splits + __builtin_amdgcn_readfirstlane(it.split)};
+
+  // This wave's page of a tile, from memory to registers.
+  const int shift = a.page_shift, sub_mask = (1 << shift) - 1;
+  const int32_t* table = a.block_tables + (size_t)b * a.bt_stride;
+  const unsigned tok = a.token_stride;
+  const size_t sub_bytes = (size_t)kPageSize * tok;
+  const int ltok = lane / Loads::kLanes, lchunk = lane % Loads::kLanes;
+  const unsigned lane_at = ltok * tok + kvh * a.head_stride + 16 * lchunk;
+  auto id_of = [&](int tile) {
+    const int p = min(first_page + max(min(tile * kTilePages + wave, n_pages - 1), 0),
+                      a.max_pages - 1);
+    return scalar_load(table + (p >> shift));
+  };
+  Loads kreg, vreg;
+  float scale_reg = 0.f;
+  auto fetch = [&](int tile, int id) {
+    const int i = tile * kTilePages + wave;
+    const int pid = i < n_pages ? clamp_page(id, a.num_pages) : -1;
+    const size_t off = pid >= 0 ? (size_t)pid * (size_t)a.page_stride +
+                                      (size_t)((first_page + i) & sub_mask) * sub_bytes : 0;
+    const int nrec = pid >= 0 ? (int)a.page_extent : 0;
+    kreg.load(__builtin_amdgcn_make_buffer_rsrc((void*)((const char*)a.k + off), (short)0, nrec,
+                                                kBufferFlags), lane_at, tok);
+    vreg.load(__builtin_amdgcn_make_buffer_rsrc((void*)((const char*)a.v + off), (short)0, nrec,
+                                                kBufferFlags), lane_at, tok);
+    if constexpr (KV::kScaled)  // lanes 0-31 the page's K scale, 32-63 its V scale
+      scale_reg = *(const float*)((const char*)(h == 0 ? args.scales.k : args.scales.v) +
+                                  max(pid, 0) * args.scales.page_stride +
+                                  (size_t)kvh * args.scales.head_stride);
+  };
+  auto put = [&](int buffer) {
+    char* to = lds + buffer * 2 * T::kBytes;
+    constexpr int N = 2 / KV::kBytes;  // LDS chunks per loaded chunk
+#pragma unroll
+    for (int i = 0; i < Loads::kLoads; ++i) {
+      const int row = wave * kPageSize + i * Loads::kTokens + ltok;
+      u4 x[N], y[N];
+      KV::template widen<E>(kreg.x[i], x);
+      KV::template widen<EV>(vreg.x[i], y);
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        *(u4*)(to + T::at(row, N * lchunk + n)) = x[n];
+        *(u4*)(to + T::kBytes + T::at(row, N * lchunk + n)) = y[n];
+      }
+    }
+    if constexpr (KV::kScaled)
+      if (l32 == 0) lds_scale[buffer][h][wave] = scale_reg;
+  };
+
+  // Rows of the queries as the scores' B operand.
+  int id_next = id_of(0);
+  fetch(0, id_next);
+  id_next = id_of(1);
+  u4 q[NBW][KS];
+#pragma unroll
+  for (int nb = 0; nb < NBW; ++nb) {
+    const int x = row0 + 32 * nb + l32;
+    const _Float16* qp = a.q + map.out_row(args, min(x, n_rows - 1)) * HD + 8 * h;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      q[nb][ks] = *(const u4*)(qp + 16 * ks);
+      if (x >= n_rows) q[nb][ks] = u4{0u, 0u, 0u, 0u};
+    }
+  }
+  f16v acc[MB][NBW];
+  float m[NBW], l[NBW];
+#pragma unroll
+  for (int nb = 0; nb < NBW; ++nb) {
+    m[nb] = -INFINITY;
+    l[nb] = 0.f;
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[mb][nb][r] = 0.f;
+  }
+  // Where the lane reads its operands in a tile.
+  int k_at[KS], v_at[MB][2];
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) k_at[ks] = T::at(l32, 2 * ks + h);
+#pragma unroll
+  for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const int l16 = lane & 15, pair = (lane >> 4) & 1;
+      v_at[mb][half] = T::at(8 * half + 4 * h + l16 / 4, 4 * mb + 2 * pair + (l16 % 4) / 2) +
+                       8 * (l16 % 2) + T::kBytes;
+    }
+
+  const float c = a.scale_log2;
+  // With codes (see sqa_scaled_attention_kernel): 1 / V scale of the two pages of a step, and
+  // whether they add to the output.
+  struct Pages {
+    float inv[2];
+    bool loud[2];
+  };
+  auto read_k = [&](int buffer, int kb, int ks) {
+    return *(const u4*)(lds + buffer * 2 * T::kBytes + kb * 32 * T::kRow + k_at[ks]);
+  };
+  // Dims 32 mb .. + 31 of 16 keys, transposed.
+  auto read_v = [&](int buffer, int kb, int i) {
+    const int st = i / MB, mb = i % MB;
+    u4 v;
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const int at = buffer * 2 * T::kBytes + v_at[mb][half] + (32 * kb + 16 * st) * T::kRow;
+      const u2 x = __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                              (__attribute__((address_space(3))) s4v*)(lds + at)));
+      v[2 * half] = x[0];
+      v[2 * half + 1] = x[1];
+    }
+    return v;
+  };
+  // Codes: scores in log2 units of their exponent, the V scale in it. All: scores past the
+  // split's end become -inf.
+  auto finish = [&](int t, int kb, f16v (&s)[NBW], Pages& pages) {
+    if constexpr (KV::kScaled) {
+#pragma unroll
+      for (int pg = 0; pg < 2; ++pg) {
+        auto uniform = [](float x) {
+          return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, x)));
+        };
+        const float ks = c * uniform(lds_scale[t & 1][0][2 * kb + pg]);
+        const float vs = uniform(lds_scale[t & 1][1][2 * kb + pg]);
+        pages.loud[pg] = !(vs < 0x1p-64f);
+        const float lv = pages.loud[pg] ? __builtin_amdgcn_logf(vs) : -64.f;
+        pages.inv[pg] = pages.loud[pg] ? __builtin_amdgcn_rcpf(vs) : 0x1p64f;
+#pragma unroll
+        for (int nb = 0; nb < NBW; ++nb)
+#pragma unroll
+          for (int r = 8 * pg; r < 8 * pg + 8; ++r) s[nb][r] = fmaf(s[nb][r], ks, lv);
+      }
+    }
+    const int left = n_pages - t * kTilePages - 2 * kb;  // pages from these two on
+    if (left < 2) {                                      // uniform
+#pragma unroll
+      for (int nb = 0; nb < NBW; ++nb)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[nb][r] = r / 8 < left ? s[nb][r] : -INFINITY;
+    }
+  };
+  // The running maxima, raised where some lane is too far ahead of its own (`top`: the
+  // largest score of each lane).
+  auto raise = [&](const float (&top)[NBW]) {
+    float lm[NBW];
+    bool grow = false;
+#pragma unroll
+    for (int nb = 0; nb < NBW; ++nb) {
+      lm[nb] = KV::kScaled ? top[nb] : top[nb] * c;
+      grow |= lm[nb] > m[nb] + kMaxLag;
+    }
+    if (__any(grow)) {
+#pragma unroll
+      for (int nb = 0; nb < NBW; ++nb) {
+        const LanePair both = lane_pair<32>(lm[nb]);
+        const float mn = fmaxf(m[nb], fmaxf(both.lo, both.hi));
+        const float alpha = fast_exp2(m[nb] - (mn == -INFINITY ? 0.f : mn));
+        m[nb] = mn;
+        l[nb] *= alpha;
+#pragma unroll
+        for (int mb = 0; mb < MB; ++mb) acc[mb][nb] *= alpha;
+      }
+    }
+  };
+  auto scores_of = [&](u4 k, int ks, f16v (&s)[NBW]) {
+#pragma unroll
+    for (int nb = 0; nb < NBW; ++nb) {
+      // Where they do not all fit the vector registers, the queries live in accumulation
+      // registers, which the products read as they are; the empty asm says so.
+      if constexpr (NBW * HD >= 256) asm("" : "+a"(q[nb][ks]));
+      if (ks == 0)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[nb][r] = 0.f;
+      s[nb] = mma32<E>(k, q[nb][ks], s[nb]);
+    }
+  };
+  auto fold_top = [&](const f16v (&s)[NBW], int i, float (&top)[NBW]) {  // i of 8
+#pragma unroll
+    for (int nb = 0; nb < NBW; ++nb)
+      top[nb] = i == 0 ? fmaxf(s[nb][0], s[nb][1]) : max3_raw(top[nb], s[nb][2 * i], s[nb][2 * i + 1]);
+  };
+  // 32 keys a step: P = 2^(s - m) of the scores `now`, added up into l, and their product with
+  // V (`v_buffer`, `v_kb`), while the scores `next` of other keys (`k_buffer`, `k_kb`) come
+  // about. The matrix cores and the vector units run beside each other only where a wave
+  // gives both something to do, so the next scores' products stand among this step's
+  // exponentials, the maxima of the next among the products with V, and reads from LDS
+  // kAhead pieces before their use; the compiler, left alone, puts one after the other.
+  constexpr int kAhead = 3;
+  auto step = [&](const f16v (&now)[NBW], const Pages& pages, int v_buffer, int v_kb,
+                  f16v (&next)[NBW], Pages& next_pages, int k_buffer, int k_kb, int next_tile) {
+    u4 k[KS], v[2 * MB];
+    u4 p[2][NBW];
+    float mu[NBW];
+#pragma unroll
+    for (int nb = 0; nb < NBW; ++nb) mu[nb] = m[nb] == -INFINITY ? 0.f : m[nb];
+#pragma unroll
+    for (int ks = 0; ks < kAhead; ++ks) k[ks] = read_k(k_buffer, k_kb, ks);
+    __builtin_amdgcn_sched_barrier(0);
+    float e[NBW][8];
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      if (ks + kAhead < KS)
+        k[ks + kAhead] = read_k(k_buffer, k_kb, ks + kAhead);
+      else
+        v[ks + kAhead - KS] = read_v(v_buffer, v_kb, ks + kAhead - KS);
+      scores_of(k[ks], ks, next);
+#pragma unroll
+      for (int w = 8 * ks / KS; w < 8 * (ks + 1) / KS; ++w) {  // pairs of scores
+        const int st = w / 4;
+#pragma unroll
+        for (int nb = 0; nb < NBW; ++nb) {
+          const float cs = KV::kScaled ? 1.f : c;
+          const float x = fast_exp2(fmaf(now[nb][2 * w], cs, -mu[nb]));
+          const float y = fast_exp2(fmaf(now[nb][2 * w + 1], cs, -mu[nb]));
+          const unsigned packed = EV::pack2(x, y);
+          if constexpr (KV::kScaled) {
+            l[nb] = fmaf(x + y, pages.inv[st], l[nb]);
+            p[st][nb][w % 4] = pages.loud[st] ? packed : 0u;
+          } else if constexpr (EV::kHalfPartials) {
+            const h2 ones = {(_Float16)1.0f, (_Float16)1.0f};
+            l[nb] = __builtin_amdgcn_fdot2(__builtin_bit_cast(h2, packed), ones, l[nb], false);
+            p[st][nb][w % 4] = packed;
+          } else {
+            l[nb] += x + y;
+            p[st][nb][w % 4] = packed;
+          }
+          unsigned here = p[st][nb][w % 4];  // not after the branch below
+          asm volatile("" : "+v"(here), "+v"(l[nb]));
+          p[st][nb][w % 4] = here;
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    finish(next_tile, k_kb, next, next_pages);
+    float top[NBW];
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < 2 * MB; ++i) {
+      if (i + kAhead < 2 * MB) v[i + kAhead] = read_v(v_buffer, v_kb, i + kAhead);
+#pragma unroll
+      for (int nb = 0; nb < NBW; ++nb)
+        acc[i % MB][nb] = mma32<EV>(v[i], p[i / MB][nb], acc[i % MB][nb]);
+#pragma unroll
+      for (int w = 8 * i / (2 * MB); w < 8 * (i + 1) / (2 * MB); ++w) fold_top(next, w, top);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    raise(top);
+  };
+
+  // A tile's second step takes the next tile's first scores, so tile t + 1 comes to LDS
+  // half-way through tile t.
+  put(0);
+  __syncthreads();
+  if (tiles > 1) fetch(1, id_next);
+  id_next = id_of(2);
+  f16v s0[NBW], s1[NBW];
+  Pages pg0, pg1;
+  float top[NBW];
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) scores_of(read_k(0, 0, ks), ks, s0);
+  finish(0, 0, s0, pg0);
+#pragma unroll
+  for (int w = 0; w < 8; ++w) fold_top(s0, w, top);
+  raise(top);
+  for (int t = 0; t < tiles; ++t) {
+    step(s0, pg0, t & 1, 0, s1, pg1, t & 1, 1, t);
+    if (t + 1 < tiles) put((t + 1) & 1);
+    __syncthreads();
+    if (t + 2 < tiles) {  // uniform
+      fetch(t + 2, id_next);
+      id_next = id_of(t + 3);
+    }
+    // Past the last tile the scores are of what the buffer holds, all masked.
+    step(s1, pg1, t & 1, 1, s0, pg0, (t + 1) & 1, 0, t + 1);
+    __syncthreads();
+  }
+
+  // Partial rows, a block of 32 at a time through LDS.
+  float* stage = (float*)lds + wave * 32 * kStageRow;
+  const __amdgpu_buffer_rsrc_t pr = __builtin_amdgcn_make_buffer_rsrc(
+      (void*)a.part_o, (short)0, (int)a.part_o_bytes, kBufferFlags);
+#pragma unroll
+  for (int nb = 0; nb < NBW; ++nb) {
+    const int x0 = row0 + 32 * nb;
+    if (x0 >= n_rows) break;  // uniform
+    const LanePair both = lane_pair<32>(l[nb]);
+    const float sum = both.lo + both.hi;
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        f4 o;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) o[r] = acc[mb][nb][4 * i + r];
+        *(f4*)(stage + l32 * kStageRow + 32 * mb + 8 * i + 4 * h) = o;
+      }
+    __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+    constexpr int CPR = HD / 4;
+#pragma unroll
+    for (int i = 0; i < CPR / 2; ++i) {
+      const int e = i * 64 + lane;  // row e / CPR (< 32), chunk e % CPR
+      const int rs = e / CPR;
+      const f4 v = *(const f4*)(stage + rs * kStageRow + 4 * (e % CPR));
+      const bool is = x0 + rs < n_rows;
+      const long long at = is ? map.part_row(args, x0 + rs) : 0;
+      __builtin_amdgcn_raw_buffer_store_b128(
+          __builtin_bit_cast(u4, v), pr,
+          is ? (unsigned)((at * HD + 4 * (e % CPR)) * 4) : kDroppedOffset, 0, kThroughAux);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+    if (h == 0 && x0 + l32 < n_rows) {
+      // A NaN sum travels with a finite max, so the join counts the split.
+      const float m_out = sum == sum ? m[nb] : 0.f;
+      store_through(a.part_ml + map.part_row(args, x0 + l32) * 2,
+                    __builtin_bit_cast(unsigned long long, float2{m_out, sum}));
+    }
+  }
+}
+};
+
+// How the sequences' own splits read the same cache.
+template <int HD, typename KV>
+struct OwnCache;
+template <int HD>
+struct OwnCache<HD, StoreNative> { using Type = PartNative<HD>; };
+template <int HD>
+struct OwnCache<HD, StoreFp8> { using Type = PartFp8<HD>; };
+template <int HD>
+struct OwnCache<HD, StoreCodesFp8> { using Type = PartCodesFp8<HD>; };
+template <int HD>
+struct OwnCache<HD, StoreCodesInt8> { using Type = PartCodesInt8<HD>; };
+
+// The kernel's arguments, where the compiler cannot know that they were asked for before:
+// each of two branches then loads its own, and neither keeps the other's in registers.
+__device__ __forceinline__ const PartArgs& own_args() {
+  auto* p = (const __attribute__((address_space(4))) PartArgs*)
+      __builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return *(const PartArgs*)p;
+}
+
+// One launch for both: the first shared_wgs workgroups serve the groups, the others what
+// follows in every sequence (NB blocks of 16 rows). The one waits for the matrix cores, the
+// other for memory.
+template <int HD, int NBW, int NB, typename E, typename KV>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1)))
+void sqa_tiles_kernel(PartArgs args) {
+  using Share = TileShare<HD, NBW, E, KV>;
+  constexpr int kOwn = 4 * 16 * (HD + 4) * 4;
+  __shared__ __attribute__((aligned(16))) char lds[Share::kLds > kOwn ? Share::kLds : kOwn];
+  __shared__ float lds_scale[2][2][kTilePages];  // of a tile's pages: buffer, K and V, page
+  if ((int)blockIdx.x < args.shared_wgs)
+    Share::run(own_args(), lds, lds_scale, blockIdx.x);
+  else
+    part_share<NB, (NB > 2 ? 2 : 4) * 128 / HD, HD, E, typename OwnCache<HD, KV>::Type>(
+        own_args(), (float*)lds, blockIdx.x - args.shared_wgs, false);
+}
+
+template <int HD, int NBW, typename E, typename KV>
+void launch_tiles_rows(const PartArgs& a, dim3 grid, hipStream_t stream) {
+  if (a.p.rows <= 32)
+    hipLaunchKernelGGL((sqa_tiles_kernel<HD, NBW, 2, E, KV>), grid, dim3(256), 0, stream, a);
+  else if constexpr (HD != 256)
+    hipLaunchKernelGGL((sqa_tiles_kernel<HD, NBW, 4, E, KV>), grid, dim3(256), 0, stream, a);
+}
+
+template <int HD, typename E, typename KV>
+void launch_tiles_hd(const PartArgs& a, dim3 grid, hipStream_t stream) {
+  if constexpr (HD != 256)
+    if (a.block_rows == 256) return launch_tiles_rows<HD, 2, E, KV>(a, grid, stream);
+  launch_tiles_rows<HD, 1, E, KV>(a, grid, stream);
+}
+
+template <typename E, typename KV>
+void launch_tiles_as(const PartArgs& a, dim3 grid, hipStream_t stream) {
+  if (a.p.head_dim == 64)
+    launch_tiles_hd<64, E, KV>(a, grid, stream);
+  else if (a.p.head_dim == 128)
+    launch_tiles_hd<128, E, KV>(a, grid, stream);
+  else
+    launch_tiles_hd<256, E, KV>(a, grid, stream);
+}
+
+template <typename E>
+hipError_t launch_tiles_of(const PartArgs& a, hipStream_t stream) {
+  const dim3 grid((unsigned)(a.shared_wgs + own_workgroups(a)));
+  if (a.scaled && a.kv_type == kInt8)
+    launch_tiles_as<E, StoreCodesInt8>(a, grid, stream);
+  else if (a.scaled)
+    launch_tiles_as<E, StoreCodesFp8>(a, grid, stream);
+  else if (a.kv_type == kE4M3)
+    launch_tiles_as<E, StoreFp8>(a, grid, stream);
+  else
+    launch_tiles_as<E, StoreNative>(a, grid, stream);
+  return hipGetLastError();
+}
+
+}  // namespace
+}  // namespace sqa

@@ -1,0 +1,10 @@
+// gfx950 kernels of attention over shared prefixes, groups of many rows, fp16 queries.
+#include "sqa_tiles.h"
+
+namespace sqa {
+
+hipError_t launch_tiles_f16(const PartArgs& a, hipStream_t stream) {
+  return launch_tiles_of<ElemF16>(a, stream);
+}
+
+}  // namespace sqa

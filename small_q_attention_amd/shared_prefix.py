@@ -24,13 +24,13 @@ from .windowed import check_call, take_workspace
 
 class SharedPrefixPlan:
     """What :func:`plan_shared_prefix` returns: ``shape`` (batch, q_len, query heads, kv
-    heads, head_dim, page_size), ``groups`` as given, and the tables on ``device``."""
+    heads, head_dim, page_size), ``groups`` as given, and those on ``device``."""
 
-    def __init__(self, shape, groups, device, plan, table):
-        self.shape, self.groups, self.device = shape, groups, device
-        self.plan, self.table = plan, table
-        self.numbers = [int(getattr(plan, name)) for name, _ in plan._fields_]  # for traced calls
-        self.most_pages = int(plan.most_pages)
+    def __init__(self, shape, groups, device, table):
+        self.shape, self.groups, self.device, self.table = shape, groups, device, table
+        # What traced calls pass on, and the most table columns that a group shares.
+        self.flat = [x for g in groups for x in g]
+        self.most_pages = max([pages for _, count, pages in groups if count > 1] + [0])
         self.known = sc.Layouts()
 
 
@@ -71,9 +71,8 @@ def plan_shared_prefix(groups, batch: int, q_len: int, num_query_heads: int, num
         raise ValueError("the plan's device must be a GPU")
     if device.index is None:
         device = torch.device("cuda", torch.cuda.current_device())
-    plan, table = _lib.plan_shared_prefix(device.index, groups, *shape)
-    return SharedPrefixPlan(shape, groups, device, plan, torch.frombuffer(
-        bytearray(table), dtype=torch.uint8).to(device))
+    table = torch.tensor(groups or [(0, 0, 0)], dtype=torch.int32).to(device)
+    return SharedPrefixPlan(shape, tuple(groups), device, table)
 
 
 def _check(query, key_cache, value_cache, key_scale, value_scale, block_tables, seq_lens, words,
@@ -91,25 +90,27 @@ def _check(query, key_cache, value_cache, key_scale, value_scale, block_tables, 
                          f"{block_tables.shape[1]}")
 
 
-def _plan_call(query, key_cache, key_scale, block_tables, words, plan, max_seq_len):
-    splits, need = _lib.plan_shared_own(query.device.index, plan, max_seq_len,
-                                        block_tables.shape[1] * (key_cache.shape[1] // 16))
-    return splits, need, _lib.part_fields(query, key_cache, key_scale, block_tables, words)
+def _plan_call(query, key_cache, key_scale, block_tables, words, groups, max_seq_len):
+    b, q_len, hq, d = query.shape
+    plan, need = _lib.plan_shared_prefix(
+        query.device.index, groups, (b, q_len, hq, key_cache.shape[2], d, key_cache.shape[1]),
+        _lib.dtype_code(key_cache.dtype), max_seq_len, block_tables.shape[1])
+    return plan, need, _lib.part_fields(query, key_cache, key_scale, block_tables, words)
 
 
 def run_shared_prefix(query, key_cache, value_cache, key_scale, value_scale, block_tables, seq_lens,
-                      words, plan, table, scale, out_scale, max_seq_len, out, workspace,
+                      words, groups, table, scale, out_scale, max_seq_len, out, workspace,
                       known=None):
-    """Plan and launch a checked call (``plan``, ``table``: a plan's; ``known``: the call's
+    """Plan and launch a checked call (``groups``, ``table``: a plan's; ``known``: the call's
     :func:`_plan_call`)."""
-    splits, need, fields = known or _plan_call(query, key_cache, key_scale, block_tables, words,
-                                               plan, max_seq_len)
+    plan, need, fields = known or _plan_call(query, key_cache, key_scale, block_tables, words,
+                                             groups, max_seq_len)
     stream = _lib.raw_stream(query.device.index)
     workspace = take_workspace(workspace, need, query, stream)
     if out is None:
         out = torch.empty_like(query)
     _lib.launch_shared_prefix(query, out, key_cache, value_cache, key_scale, value_scale,
-                              block_tables, seq_lens, words, plan, table, scale, out_scale, splits,
+                              block_tables, seq_lens, words, plan, table, scale, out_scale,
                               workspace, stream, fields)
     return out
 
@@ -153,7 +154,7 @@ def paged_attention_shared_prefix(query, key_cache, value_cache, block_tables, s
 
         res = torch.ops.sqa.paged_attention_shared_prefix(
             query, key_cache, value_cache, key_scale, value_scale, block_tables, seq_lens, words,
-            plan.numbers, plan.table, scale, float(out_scale), max_seq_len)
+            plan.flat, plan.table, scale, float(out_scale), max_seq_len)
         return res if out is None else out.copy_(res)
     layout = sc.layout
     seen = (layout(query), layout(key_cache), layout(value_cache), layout(key_scale),
@@ -164,11 +165,11 @@ def paged_attention_shared_prefix(query, key_cache, value_cache, block_tables, s
         _check(query, key_cache, value_cache, key_scale, value_scale, block_tables, seq_lens, words,
                plan, out, workspace_buffer)
         known = plan.known.keep(seen, sc.on_device(query.device, _plan_call, query, key_cache,
-                                                   key_scale, block_tables, words, plan.plan,
+                                                   key_scale, block_tables, words, plan.groups,
                                                    max_seq_len))
     sc.check_aligned(16, query, key_cache, value_cache)
     return sc.on_device(query.device, run_shared_prefix, query, key_cache, value_cache, key_scale,
-                        value_scale, block_tables, seq_lens, words, plan.plan, plan.table, scale,
+                        value_scale, block_tables, seq_lens, words, plan.groups, plan.table, scale,
                         float(out_scale), max_seq_len, out, workspace_buffer, known)
 
 

@@ -71,23 +71,23 @@ def take_workspace(workspace_buffer, need, query, stream):
 def _plan(query, key_cache, key_scale, block_tables, words, window, sink, max_seq_len):
     b, q_len, hq, d = query.shape
     page, hkv = key_cache.shape[1], key_cache.shape[2]
-    splits = _lib.plan_windowed(query.device.index, b, q_len, hq, hkv, d, window, sink, max_seq_len,
-                                block_tables.shape[1] * (page // 16))
-    return (splits, _lib.workspace_bytes(b, q_len, hq, hkv, d, splits, 1),
+    cut = _lib.plan_windowed(query.device.index, b, q_len, hq, hkv, d, window, sink, max_seq_len,
+                             block_tables.shape[1] * (page // 16))
+    return (cut, _lib.workspace_bytes(b, q_len, hq, hkv, d, cut[0], 1),
             _lib.part_fields(query, key_cache, key_scale, block_tables, words))
 
 
 def run_windowed(query, key_cache, value_cache, key_scale, value_scale, block_tables, seq_lens,
                  words, window, sink, scale, out_scale, max_seq_len, out, workspace, known=None):
     """Plan and launch a checked call (``known``: its :func:`_plan`)."""
-    splits, need, fields = known or _plan(query, key_cache, key_scale, block_tables, words, window,
-                                          sink, max_seq_len)
+    cut, need, fields = known or _plan(query, key_cache, key_scale, block_tables, words, window,
+                                       sink, max_seq_len)
     stream = _lib.raw_stream(query.device.index)
     workspace = take_workspace(workspace, need, query, stream)
     if out is None:
         out = torch.empty_like(query)
     _lib.launch_windowed(query, out, key_cache, value_cache, key_scale, value_scale, block_tables,
-                         seq_lens, words, window, sink, scale, out_scale, splits, workspace, stream,
+                         seq_lens, words, window, sink, scale, out_scale, cut, workspace, stream,
                          fields)
     return out
 

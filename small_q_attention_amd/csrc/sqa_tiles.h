@@ -218,11 +218,33 @@ struct TileShare {
     }
 
   const float c = a.scale_log2;
-  // With codes (see sqa_scaled_attention_kernel): 1 / V scale of the two pages of a step, and
-  // whether they add to the output.
+  // The two pages of a step: exponents are s mul + add - m. With codes mul holds the K scale,
+  // add log2 of the V scale, inv 1 / V scale for the row sum (see
+  // sqa_scaled_attention_kernel); pages past the split's end get add -infinity.
   struct Pages {
-    float inv[2];
+    float mul[2], add[2], inv[2];
     bool loud[2];
+  };
+  auto pages_of = [&](int t, int kb) {
+    Pages x;
+    const int left = n_pages - t * kTilePages - 2 * kb;  // pages from these two on
+#pragma unroll
+    for (int pg = 0; pg < 2; ++pg) {
+      x.mul[pg] = c;
+      x.add[pg] = 0.f;
+      if constexpr (KV::kScaled) {
+        auto uniform = [](float y) {
+          return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, y)));
+        };
+        const float vs = uniform(lds_scale[t & 1][1][2 * kb + pg]);
+        x.mul[pg] = c * uniform(lds_scale[t & 1][0][2 * kb + pg]);
+        x.loud[pg] = !(vs < 0x1p-64f);
+        x.add[pg] = x.loud[pg] ? __builtin_amdgcn_logf(vs) : -64.f;
+        x.inv[pg] = x.loud[pg] ? __builtin_amdgcn_rcpf(vs) : 0x1p64f;
+      }
+      if (pg >= left) x.add[pg] = -INFINITY;
+    }
+    return x;
   };
   auto read_k = [&](int buffer, int kb, int ks) {
     return *(const u4*)(lds + buffer * 2 * T::kBytes + kb * 32 * T::kRow + k_at[ks]);
@@ -241,42 +263,15 @@ struct TileShare {
     }
     return v;
   };
-  // Codes: scores in log2 units of their exponent, the V scale in it. All: scores past the
-  // split's end become -inf.
-  auto finish = [&](int t, int kb, f16v (&s)[NBW], Pages& pages) {
-    if constexpr (KV::kScaled) {
-#pragma unroll
-      for (int pg = 0; pg < 2; ++pg) {
-        auto uniform = [](float x) {
-          return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, x)));
-        };
-        const float ks = c * uniform(lds_scale[t & 1][0][2 * kb + pg]);
-        const float vs = uniform(lds_scale[t & 1][1][2 * kb + pg]);
-        pages.loud[pg] = !(vs < 0x1p-64f);
-        const float lv = pages.loud[pg] ? __builtin_amdgcn_logf(vs) : -64.f;
-        pages.inv[pg] = pages.loud[pg] ? __builtin_amdgcn_rcpf(vs) : 0x1p64f;
-#pragma unroll
-        for (int nb = 0; nb < NBW; ++nb)
-#pragma unroll
-          for (int r = 8 * pg; r < 8 * pg + 8; ++r) s[nb][r] = fmaf(s[nb][r], ks, lv);
-      }
-    }
-    const int left = n_pages - t * kTilePages - 2 * kb;  // pages from these two on
-    if (left < 2) {                                      // uniform
-#pragma unroll
-      for (int nb = 0; nb < NBW; ++nb)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s[nb][r] = r / 8 < left ? s[nb][r] : -INFINITY;
-    }
-  };
   // The running maxima, raised where some lane is too far ahead of its own (`top`: the
-  // largest score of each lane).
-  auto raise = [&](const float (&top)[NBW]) {
+  // largest score of each lane and page).
+  auto raise = [&](const float (&top)[NBW][2], const Pages& pages) {
     float lm[NBW];
     bool grow = false;
 #pragma unroll
     for (int nb = 0; nb < NBW; ++nb) {
-      lm[nb] = KV::kScaled ? top[nb] : top[nb] * c;
+      lm[nb] = __builtin_elementwise_maximum(fmaf(top[nb][0], pages.mul[0], pages.add[0]),
+                                             fmaf(top[nb][1], pages.mul[1], pages.add[1]));
       grow |= lm[nb] > m[nb] + kMaxLag;
     }
     if (__any(grow)) {
@@ -292,22 +287,19 @@ struct TileShare {
       }
     }
   };
-  auto scores_of = [&](u4 k, int ks, f16v (&s)[NBW]) {
+  auto score = [&](u4 k, int ks, int nb, f16v (&s)[NBW]) {
+    // Where they do not all fit the vector registers, the queries live in accumulation
+    // registers, which the products read as they are; the empty asm says so.
+    if constexpr (NBW * HD >= 256) asm("" : "+a"(q[nb][ks]));
+    if (ks == 0)
 #pragma unroll
-    for (int nb = 0; nb < NBW; ++nb) {
-      // Where they do not all fit the vector registers, the queries live in accumulation
-      // registers, which the products read as they are; the empty asm says so.
-      if constexpr (NBW * HD >= 256) asm("" : "+a"(q[nb][ks]));
-      if (ks == 0)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s[nb][r] = 0.f;
-      s[nb] = mma32<E>(k, q[nb][ks], s[nb]);
-    }
+      for (int r = 0; r < 16; ++r) s[nb][r] = 0.f;
+    s[nb] = mma32<E>(k, q[nb][ks], s[nb]);
   };
-  auto fold_top = [&](const f16v (&s)[NBW], int i, float (&top)[NBW]) {  // i of 8
-#pragma unroll
-    for (int nb = 0; nb < NBW; ++nb)
-      top[nb] = i == 0 ? fmaxf(s[nb][0], s[nb][1]) : max3_raw(top[nb], s[nb][2 * i], s[nb][2 * i + 1]);
+  auto fold_top = [&](const f16v (&s)[NBW], int i, int nb, float (&top)[NBW][2]) {  // i of 8
+    float& x = top[nb][i / 4];
+    x = i % 4 == 0 ? __builtin_elementwise_maximum(s[nb][2 * i], s[nb][2 * i + 1])
+                   : max3_raw(x, s[nb][2 * i], s[nb][2 * i + 1]);
   };
   // 32 keys a step: P = 2^(s - m) of the scores `now`, added up into l, and their product with
   // V (`v_buffer`, `v_kb`), while the scores `next` of other keys (`k_buffer`, `k_kb`) come
@@ -317,64 +309,71 @@ struct TileShare {
   // kAhead pieces before their use; the compiler, left alone, puts one after the other.
   constexpr int kAhead = 3;
   auto step = [&](const f16v (&now)[NBW], const Pages& pages, int v_buffer, int v_kb,
-                  f16v (&next)[NBW], Pages& next_pages, int k_buffer, int k_kb, int next_tile) {
+                  f16v (&next)[NBW], const Pages& next_pages, int k_buffer, int k_kb) {
     u4 k[KS], v[2 * MB];
     u4 p[2][NBW];
-    float mu[NBW];
+    float off[NBW][2];
 #pragma unroll
-    for (int nb = 0; nb < NBW; ++nb) mu[nb] = m[nb] == -INFINITY ? 0.f : m[nb];
+    for (int nb = 0; nb < NBW; ++nb)
+#pragma unroll
+      for (int pg = 0; pg < 2; ++pg) off[nb][pg] = pages.add[pg] - (m[nb] == -INFINITY ? 0.f : m[nb]);
 #pragma unroll
     for (int ks = 0; ks < kAhead; ++ks) k[ks] = read_k(k_buffer, k_kb, ks);
     __builtin_amdgcn_sched_barrier(0);
-    float e[NBW][8];
+    auto weigh = [&](int w, int nb) {  // pair w of 8: registers 2 w and 2 w + 1
+      const int st = w / 4;
+      const float x = fast_exp2(fmaf(now[nb][2 * w], pages.mul[st], off[nb][st]));
+      const float y = fast_exp2(fmaf(now[nb][2 * w + 1], pages.mul[st], off[nb][st]));
+      unsigned packed = EV::pack2(x, y);
+      if constexpr (KV::kScaled) {
+        l[nb] = fmaf(x + y, pages.inv[st], l[nb]);
+        packed = pages.loud[st] ? packed : 0u;
+      } else if constexpr (EV::kHalfPartials) {
+        const h2 ones = {(_Float16)1.0f, (_Float16)1.0f};
+        l[nb] = __builtin_amdgcn_fdot2(__builtin_bit_cast(h2, packed), ones, l[nb], false);
+      } else {
+        l[nb] += x + y;
+      }
+      p[st][nb][w % 4] = packed;
+    };
+    // Five of a row's eight pairs among the scores' products, three among the first half of
+    // those with V, which take the pairs before.
+    constexpr int kEarly = 5;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
       if (ks + kAhead < KS)
         k[ks + kAhead] = read_k(k_buffer, k_kb, ks + kAhead);
       else
         v[ks + kAhead - KS] = read_v(v_buffer, v_kb, ks + kAhead - KS);
-      scores_of(k[ks], ks, next);
 #pragma unroll
-      for (int w = 8 * ks / KS; w < 8 * (ks + 1) / KS; ++w) {  // pairs of scores
-        const int st = w / 4;
+      for (int nb = 0; nb < NBW; ++nb) {
+        score(k[ks], ks, nb, next);
 #pragma unroll
-        for (int nb = 0; nb < NBW; ++nb) {
-          const float cs = KV::kScaled ? 1.f : c;
-          const float x = fast_exp2(fmaf(now[nb][2 * w], cs, -mu[nb]));
-          const float y = fast_exp2(fmaf(now[nb][2 * w + 1], cs, -mu[nb]));
-          const unsigned packed = EV::pack2(x, y);
-          if constexpr (KV::kScaled) {
-            l[nb] = fmaf(x + y, pages.inv[st], l[nb]);
-            p[st][nb][w % 4] = pages.loud[st] ? packed : 0u;
-          } else if constexpr (EV::kHalfPartials) {
-            const h2 ones = {(_Float16)1.0f, (_Float16)1.0f};
-            l[nb] = __builtin_amdgcn_fdot2(__builtin_bit_cast(h2, packed), ones, l[nb], false);
-            p[st][nb][w % 4] = packed;
-          } else {
-            l[nb] += x + y;
-            p[st][nb][w % 4] = packed;
-          }
-          unsigned here = p[st][nb][w % 4];  // not after the branch below
-          asm volatile("" : "+v"(here), "+v"(l[nb]));
-          p[st][nb][w % 4] = here;
-        }
+        for (int w = 0; w < kEarly; ++w)
+          if (w * KS / kEarly == ks) weigh(w, nb);
+        __builtin_amdgcn_sched_barrier(0);
       }
-      __builtin_amdgcn_sched_barrier(0);
     }
-    finish(next_tile, k_kb, next, next_pages);
-    float top[NBW];
-    __builtin_amdgcn_sched_barrier(0);
+    float top[NBW][2];
 #pragma unroll
     for (int i = 0; i < 2 * MB; ++i) {
       if (i + kAhead < 2 * MB) v[i + kAhead] = read_v(v_buffer, v_kb, i + kAhead);
 #pragma unroll
-      for (int nb = 0; nb < NBW; ++nb)
+      for (int nb = 0; nb < NBW; ++nb) {
         acc[i % MB][nb] = mma32<EV>(v[i], p[i / MB][nb], acc[i % MB][nb]);
+        if (i < MB) {
 #pragma unroll
-      for (int w = 8 * i / (2 * MB); w < 8 * (i + 1) / (2 * MB); ++w) fold_top(next, w, top);
-      __builtin_amdgcn_sched_barrier(0);
+          for (int w = kEarly; w < 8; ++w)
+            if ((w - kEarly) * MB / (8 - kEarly) == i) weigh(w, nb);
+        } else {
+#pragma unroll
+          for (int w = 0; w < 8; ++w)
+            if (w * MB / 8 == i - MB) fold_top(next, w, nb, top);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
     }
-    raise(top);
+    raise(top, next_pages);
   };
 
   // A tile's second step takes the next tile's first scores, so tile t + 1 comes to LDS
@@ -384,24 +383,29 @@ struct TileShare {
   if (tiles > 1) fetch(1, id_next);
   id_next = id_of(2);
   f16v s0[NBW], s1[NBW];
-  Pages pg0, pg1;
-  float top[NBW];
+  float top[NBW][2];
+  Pages pages = pages_of(0, 0);
 #pragma unroll
-  for (int ks = 0; ks < KS; ++ks) scores_of(read_k(0, 0, ks), ks, s0);
-  finish(0, 0, s0, pg0);
+  for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-  for (int w = 0; w < 8; ++w) fold_top(s0, w, top);
-  raise(top);
+    for (int nb = 0; nb < NBW; ++nb) score(read_k(0, 0, ks), ks, nb, s0);
+#pragma unroll
+  for (int w = 0; w < 8; ++w)
+#pragma unroll
+    for (int nb = 0; nb < NBW; ++nb) fold_top(s0, w, nb, top);
+  raise(top, pages);
   for (int t = 0; t < tiles; ++t) {
-    step(s0, pg0, t & 1, 0, s1, pg1, t & 1, 1, t);
+    const Pages second = pages_of(t, 1);
+    step(s0, pages, t & 1, 0, s1, second, t & 1, 1);
     if (t + 1 < tiles) put((t + 1) & 1);
     __syncthreads();
     if (t + 2 < tiles) {  // uniform
       fetch(t + 2, id_next);
       id_next = id_of(t + 3);
     }
-    // Past the last tile the scores are of what the buffer holds, all masked.
-    step(s1, pg1, t & 1, 1, s0, pg0, (t + 1) & 1, 0, t + 1);
+    // Past the last tile the scores are of what the buffer holds, and nobody's.
+    pages = pages_of(t + 1, 0);
+    step(s1, second, t & 1, 1, s0, pages, (t + 1) & 1, 0);
     __syncthreads();
   }
 

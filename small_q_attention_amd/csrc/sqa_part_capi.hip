@@ -216,12 +216,13 @@ int place(const sqa_attention_args& a, long long rows, size_t need, sqa::PartArg
 }
 
 // Rows of a block: those of the widest group, as one wave takes them while they fit one,
-// else as a workgroup does.
-int rows_of_block(long long most, int head_dim) {
-  if (most <= 16) return 16;
-  if (most <= 32) return 32;
-  if (most <= 64 && head_dim != 256) return 64;
-  return most <= 128 || head_dim == 256 ? 128 : 256;
+// else as a workgroup does (256 with up to 32 rows of a sequence, at head dims 64 and 128).
+int rows_of_block(long long most, long long rows, int head_dim) {
+  const long long n = std::max(most, rows);
+  if (n <= 16) return 16;
+  if (n <= 32) return 32;
+  if (n <= 64 && head_dim != 256) return 64;
+  return n <= 128 || head_dim == 256 || rows > 32 ? 128 : 256;
 }
 
 struct SharedGroup {
@@ -427,7 +428,7 @@ int sqa_plan_shared_prefix(int device, int batch, int q_len, int num_query_heads
     out.wg_heads = cut.wg_heads;
   } else {
     out.num_groups = num_groups;
-    out.block_rows = std::max(rows_of_block(most_rows, head_dim), rows_of_block(rows, head_dim));
+    out.block_rows = rows_of_block(most_rows, rows, head_dim);
     const int bytes = kv_dtype == SQA_DTYPE_FP8_E4M3 || kv_dtype == SQA_DTYPE_INT8 ? 1 : 2;
     const SharedCut cut = shared_cut(cus, batch, rows, num_kv_heads, head_dim, bytes,
                                      out.block_rows, num_groups, group, own);
@@ -480,7 +481,8 @@ int sqa_paged_attention_shared_prefix(const sqa_attention_args* args,
       return fail(SQA_ERR_INVALID, "groups must be given, 4-byte aligned, in device memory");
     const int b = plan->block_rows;
     if ((b != 16 && b != 32 && b != 64 && b != 128 && b != 256) ||
-        (a.head_dim == 256 && (b == 64 || b == 256)) || (!tiles && b < s.p.rows))
+        (a.head_dim == 256 && (b == 64 || b == 256)) || (b == 256 && s.p.rows > 32) ||
+        (!tiles && b < s.p.rows))
       return fail(SQA_ERR_INVALID, "not a plan of sqa_plan_shared_prefix");
     s.groups = groups;
     s.n_groups = plan->num_groups;

@@ -386,12 +386,12 @@ __device__ __forceinline__ void scaled_page(WaveState<NB, HD>& st, const typenam
   }
 }
 
-// One workgroup = four waves, wave w with kv head w % wg_heads of the workgroup's heads; the
-// 4 / wg_heads waves of a head divide the pages of one share, each on its own, and join
+// One workgroup = W waves, wave w with kv head w % wg_heads of the workgroup's heads; the
+// W / wg_heads waves of a head divide the pages of one share, each on its own, and join
 // their rows at the end. A share is a split of a sequence's own pages, or (`shared`) a block
 // of a group's rows over a split of the shared pages. A wave holds all rows of its share (NB
 // blocks of 16) and keeps a ring of D pages in flight in registers.
-template <int NB, int D, int HD, typename E, typename KV>
+template <int NB, int D, int HD, int W, typename E, typename KV>
 __device__ __forceinline__ void part_share(const PartArgs& args, float* sm_stage, int block,
                                            bool shared) {
   const PartialArgs& a = args.p;
@@ -400,9 +400,10 @@ __device__ __forceinline__ void part_share(const PartArgs& args, float* sm_stage
   const int lane = threadIdx.x & 63;
   const int g16 = lane >> 4, l16 = lane & 15;
   const int wgh = args.wg_heads;
-  const int waves = wgh == 4 ? 1 : (wgh == 2 ? 2 : 4);
-  const int mine = wgh == 4 ? 0 : (wgh == 2 ? wave >> 1 : wave);
-  const int head_in = wgh == 4 ? wave : (wgh == 2 ? wave & 1 : 0);
+  const int log_heads = wgh >> 1;  // of 1, 2 and 4
+  const int waves = W >> log_heads;
+  const int mine = wave >> log_heads;
+  const int head_in = wave & (wgh - 1);
   const int share = block / a.by_head_groups;
   const int kvh = (block - share * ((a.hkv + wgh - 1) / wgh)) * wgh + head_in;
 
@@ -440,7 +441,7 @@ __device__ __forceinline__ void part_share(const PartArgs& args, float* sm_stage
     map.slot = split;
   }
   if (waves > 1) {  // uniform: this wave's part of the share
-    const int each = (n_pages + waves - 1) >> (waves == 2 ? 1 : 2);
+    const int each = (n_pages + waves - 1) >> ((W == 8 ? 3 : 2) - log_heads);
     v0 += mine * each;
     n_pages = max(min(each, n_pages - mine * each), 0);
   }
@@ -600,7 +601,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1)))
 void sqa_part_kernel(PartArgs args) {
   __shared__ float sm_stage[4 * 16 * (HD + 4)];
   const bool shared = GROUPS && (int)blockIdx.x < args.shared_wgs;
-  part_share<NB, D, HD, E, KV>(args, sm_stage, GROUPS && !shared ? blockIdx.x - args.shared_wgs
+  part_share<NB, D, HD, 4, E, KV>(args, sm_stage, GROUPS && !shared ? blockIdx.x - args.shared_wgs
                                                                  : blockIdx.x, shared);
 }
 

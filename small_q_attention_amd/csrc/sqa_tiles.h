@@ -45,18 +45,27 @@ struct Tile {
   }
 };
 
-// How a page travels from memory to LDS: 16-byte loads, 16-bit elements kept, codes widened
-// (exactly) as they are stored.
-template <int HD, int BYTES>
+// How tokens travel from memory to LDS: 16-byte loads (8 where a wave's tokens are fewer than
+// fill them), 16-bit elements kept, codes widened (exactly) as they are stored.
+template <int HD, int BYTES, int TOKENS>
 struct PageLoads {
-  static constexpr int kLanes = HD * BYTES / 16;     // lanes per token
-  static constexpr int kTokens = 64 / kLanes;        // tokens per load
-  static constexpr int kLoads = kPageSize / kTokens;
+  static constexpr int kWidth = TOKENS * HD * BYTES < 64 * 16 ? 8 : 16;  // bytes of a load
+  static constexpr int kLanes = HD * BYTES / kWidth;                     // lanes per token
+  static constexpr int kTokens = 64 / kLanes;                            // tokens per load
+  static constexpr int kLoads = TOKENS / kTokens;
+  static constexpr int kChunks = kWidth / BYTES / 8;                     // of LDS, per load
+  static_assert(kLoads >= 1, "a wave brings at least one load's tokens");
   u4 x[kLoads];
   __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t r, unsigned lane_at, unsigned tok) {
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i)
-      x[i] = __builtin_amdgcn_raw_buffer_load_b128(r, lane_at, i * kTokens * tok, 0);
+    for (int i = 0; i < kLoads; ++i) {
+      if constexpr (kWidth == 16) {
+        x[i] = __builtin_amdgcn_raw_buffer_load_b128(r, lane_at, i * kTokens * tok, 0);
+      } else {
+        const u2 y = __builtin_amdgcn_raw_buffer_load_b64(r, lane_at, i * kTokens * tok, 0);
+        x[i] = u4{y[0], y[1], 0u, 0u};
+      }
+    }
   }
 };
 
@@ -92,23 +101,24 @@ struct StoreCodesInt8 {
   }
 };
 
-// One workgroup: a block of 128 NBW of a group's rows of one kv head, 32 NBW to a wave, over
-// one split of the shared pages, 64 keys at a time. Each wave brings one of a tile's four
+// One workgroup: a block of 32 W of a group's rows of one kv head, 32 to a wave, over one
+// split of the shared pages, 64 keys at a time. Each wave brings a part of a tile's four
 // pages to LDS, two buffers in turn; all waves read all of it.
 //
 // S^T = K Q^T leaves a lane with half of the keys of its row, so that maxima and sums stay
 // in the lane but for one exchange between two lanes; O^T = V^T P^T takes P from those
 // registers as they are: the product's k order is the order the registers hold the keys in,
 // and V comes transposed from LDS in the same order.
-template <int HD, int NBW, typename E, typename KV>
+template <int HD, int W, typename E, typename KV>
 struct TileShare {
   using EV = std::conditional_t<KV::kScaled, ElemF16, E>;  // type of P and V
   using T = Tile<HD>;
-  using Loads = PageLoads<HD, KV::kBytes>;
+  static constexpr int kTokens = kTileKeys / W;  // of a tile that a wave brings
+  using Loads = PageLoads<HD, KV::kBytes, kTokens>;
   static constexpr int KS = HD / 16;  // k steps of the scores
   static constexpr int MB = HD / 32;  // blocks of 32 output dims
   static constexpr int kStageRow = HD + 4;
-  static constexpr int kStage = 4 * 32 * kStageRow * 4;
+  static constexpr int kStage = W * 32 * kStageRow * 4;
   static constexpr int kLds = 4 * T::kBytes > kStage ? 4 * T::kBytes : kStage;
 
   static __device__ __forceinline__ void run(const PartArgs& args, char* lds,
@@ -125,7 +135,7 @@ struct TileShare {
   const int first_page = __builtin_amdgcn_readfirstlane(it.begin);
   const int n_pages = __builtin_amdgcn_readfirstlane(it.n);
   const int tiles = (n_pages + kTilePages - 1) / kTilePages;
-  const int row0 = __builtin_amdgcn_readfirstlane(it.block) * (128 * NBW) + wave * (32 * NBW);
+  const int row0 = __builtin_amdgcn_readfirstlane(it.block) * (32 * W) + wave * 32;
   const int n_rows = __builtin_amdgcn_readfirstlane(it.group.count) * a.rows;
   const RowMap map{__builtin_amdgcn_readfirstlane(it.group.first), kvh,
                    args.splits + __builtin_amdgcn_readfirstlane(it.split)};
@@ -136,24 +146,26 @@ struct TileShare {
   const unsigned tok = a.token_stride;
   const size_t sub_bytes = (size_t)kPageSize * tok;
   const int ltok = lane / Loads::kLanes, lchunk = lane % Loads::kLanes;
-  const unsigned lane_at = ltok * tok + kvh * a.head_stride + 16 * lchunk;
+  const unsigned lane_at = ltok * tok + kvh * a.head_stride + Loads::kWidth * lchunk;
+  const int my_page = wave * kTokens / kPageSize, my_slot = wave * kTokens % kPageSize;
   auto id_of = [&](int tile) {
-    const int p = min(first_page + max(min(tile * kTilePages + wave, n_pages - 1), 0),
+    const int p = min(first_page + max(min(tile * kTilePages + my_page, n_pages - 1), 0),
                       a.max_pages - 1);
     return scalar_load(table + (p >> shift));
   };
   Loads kreg, vreg;
   float scale_reg = 0.f;
   auto fetch = [&](int tile, int id) {
-    const int i = tile * kTilePages + wave;
+    const int i = tile * kTilePages + my_page;
     const int pid = i < n_pages ? clamp_page(id, a.num_pages) : -1;
     const size_t off = pid >= 0 ? (size_t)pid * (size_t)a.page_stride +
                                       (size_t)((first_page + i) & sub_mask) * sub_bytes : 0;
     const int nrec = pid >= 0 ? (int)a.page_extent : 0;
+    const unsigned at = lane_at + my_slot * tok;
     kreg.load(__builtin_amdgcn_make_buffer_rsrc((void*)((const char*)a.k + off), (short)0, nrec,
-                                                kBufferFlags), lane_at, tok);
+                                                kBufferFlags), at, tok);
     vreg.load(__builtin_amdgcn_make_buffer_rsrc((void*)((const char*)a.v + off), (short)0, nrec,
-                                                kBufferFlags), lane_at, tok);
+                                                kBufferFlags), at, tok);
     if constexpr (KV::kScaled)  // lanes 0-31 the page's K scale, 32-63 its V scale
       scale_reg = *(const float*)((const char*)(h == 0 ? args.scales.k : args.scales.v) +
                                   max(pid, 0) * args.scales.page_stride +
@@ -161,11 +173,11 @@ struct TileShare {
   };
   auto put = [&](int buffer) {
     char* to = lds + buffer * 2 * T::kBytes;
-    constexpr int N = 2 / KV::kBytes;  // LDS chunks per loaded chunk
+    constexpr int N = Loads::kChunks;
 #pragma unroll
     for (int i = 0; i < Loads::kLoads; ++i) {
-      const int row = wave * kPageSize + i * Loads::kTokens + ltok;
-      u4 x[N], y[N];
+      const int row = wave * kTokens + i * Loads::kTokens + ltok;
+      u4 x[2 / KV::kBytes], y[2 / KV::kBytes];
       KV::template widen<E>(kreg.x[i], x);
       KV::template widen<EV>(vreg.x[i], y);
 #pragma unroll
@@ -175,35 +187,29 @@ struct TileShare {
       }
     }
     if constexpr (KV::kScaled)
-      if (l32 == 0) lds_scale[buffer][h][wave] = scale_reg;
+      if (l32 == 0) lds_scale[buffer][h][my_page] = scale_reg;
   };
 
   // Rows of the queries as the scores' B operand.
   int id_next = id_of(0);
   fetch(0, id_next);
   id_next = id_of(1);
-  u4 q[NBW][KS];
-#pragma unroll
-  for (int nb = 0; nb < NBW; ++nb) {
-    const int x = row0 + 32 * nb + l32;
+  u4 q[KS];
+  {
+    const int x = row0 + l32;
     const _Float16* qp = a.q + map.out_row(args, min(x, n_rows - 1)) * HD + 8 * h;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
-      q[nb][ks] = *(const u4*)(qp + 16 * ks);
-      if (x >= n_rows) q[nb][ks] = u4{0u, 0u, 0u, 0u};
+      q[ks] = *(const u4*)(qp + 16 * ks);
+      if (x >= n_rows) q[ks] = u4{0u, 0u, 0u, 0u};
     }
   }
-  f16v acc[MB][NBW];
-  float m[NBW], l[NBW];
+  f16v acc[MB];
+  float m = -INFINITY, l = 0.f;
 #pragma unroll
-  for (int nb = 0; nb < NBW; ++nb) {
-    m[nb] = -INFINITY;
-    l[nb] = 0.f;
+  for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
-    for (int mb = 0; mb < MB; ++mb)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) acc[mb][nb][r] = 0.f;
-  }
+    for (int r = 0; r < 16; ++r) acc[mb][r] = 0.f;
   // Where the lane reads its operands in a tile.
   int k_at[KS], v_at[MB][2];
 #pragma unroll
@@ -263,78 +269,63 @@ struct TileShare {
     }
     return v;
   };
-  // The running maxima, raised where some lane is too far ahead of its own (`top`: the
-  // largest score of each lane and page).
-  auto raise = [&](const float (&top)[NBW][2], const Pages& pages) {
-    float lm[NBW];
-    bool grow = false;
+  // The running maximum, raised where some lane is too far ahead of its own (`top`: the
+  // largest score of each page in the lane).
+  auto raise = [&](const float (&top)[2], const Pages& pages) {
+    const float lm = __builtin_elementwise_maximum(fmaf(top[0], pages.mul[0], pages.add[0]),
+                                                   fmaf(top[1], pages.mul[1], pages.add[1]));
+    if (__any(lm > m + kMaxLag)) {
+      const LanePair both = lane_pair<32>(lm);
+      const float mn = fmaxf(m, fmaxf(both.lo, both.hi));
+      const float alpha = fast_exp2(m - (mn == -INFINITY ? 0.f : mn));
+      m = mn;
+      l *= alpha;
 #pragma unroll
-    for (int nb = 0; nb < NBW; ++nb) {
-      lm[nb] = __builtin_elementwise_maximum(fmaf(top[nb][0], pages.mul[0], pages.add[0]),
-                                             fmaf(top[nb][1], pages.mul[1], pages.add[1]));
-      grow |= lm[nb] > m[nb] + kMaxLag;
-    }
-    if (__any(grow)) {
-#pragma unroll
-      for (int nb = 0; nb < NBW; ++nb) {
-        const LanePair both = lane_pair<32>(lm[nb]);
-        const float mn = fmaxf(m[nb], fmaxf(both.lo, both.hi));
-        const float alpha = fast_exp2(m[nb] - (mn == -INFINITY ? 0.f : mn));
-        m[nb] = mn;
-        l[nb] *= alpha;
-#pragma unroll
-        for (int mb = 0; mb < MB; ++mb) acc[mb][nb] *= alpha;
-      }
+      for (int mb = 0; mb < MB; ++mb) acc[mb] *= alpha;
     }
   };
-  auto score = [&](u4 k, int ks, int nb, f16v (&s)[NBW]) {
-    // Where they do not all fit the vector registers, the queries live in accumulation
-    // registers, which the products read as they are; the empty asm says so.
-    if constexpr (NBW * HD >= 256) asm("" : "+a"(q[nb][ks]));
+  auto score = [&](u4 k, int ks, f16v& s) {
     if (ks == 0)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[nb][r] = 0.f;
-    s[nb] = mma32<E>(k, q[nb][ks], s[nb]);
+      for (int r = 0; r < 16; ++r) s[r] = 0.f;
+    s = mma32<E>(k, q[ks], s);
   };
-  auto fold_top = [&](const f16v (&s)[NBW], int i, int nb, float (&top)[NBW][2]) {  // i of 8
-    float& x = top[nb][i / 4];
-    x = i % 4 == 0 ? __builtin_elementwise_maximum(s[nb][2 * i], s[nb][2 * i + 1])
-                   : max3_raw(x, s[nb][2 * i], s[nb][2 * i + 1]);
+  auto fold_top = [&](const f16v& s, int i, float (&top)[2]) {  // i of 8
+    float& x = top[i / 4];
+    x = i % 4 == 0 ? __builtin_elementwise_maximum(s[2 * i], s[2 * i + 1])
+                   : max3_raw(x, s[2 * i], s[2 * i + 1]);
   };
   // 32 keys a step: P = 2^(s - m) of the scores `now`, added up into l, and their product with
   // V (`v_buffer`, `v_kb`), while the scores `next` of other keys (`k_buffer`, `k_kb`) come
-  // about. The matrix cores and the vector units run beside each other only where a wave
-  // gives both something to do, so the next scores' products stand among this step's
+  // about. The matrix cores and the vector units run beside each other where a wave gives
+  // both something to do, so the next scores' products stand among this step's
   // exponentials, the maxima of the next among the products with V, and reads from LDS
   // kAhead pieces before their use; the compiler, left alone, puts one after the other.
   constexpr int kAhead = 3;
-  auto step = [&](const f16v (&now)[NBW], const Pages& pages, int v_buffer, int v_kb,
-                  f16v (&next)[NBW], const Pages& next_pages, int k_buffer, int k_kb) {
-    u4 k[KS], v[2 * MB];
-    u4 p[2][NBW];
-    float off[NBW][2];
+  auto step = [&](const f16v& now, const Pages& pages, int v_buffer, int v_kb, f16v& next,
+                  const Pages& next_pages, int k_buffer, int k_kb) {
+    u4 k[KS], v[2 * MB], p[2];
+    float off[2];
 #pragma unroll
-    for (int nb = 0; nb < NBW; ++nb)
-#pragma unroll
-      for (int pg = 0; pg < 2; ++pg) off[nb][pg] = pages.add[pg] - (m[nb] == -INFINITY ? 0.f : m[nb]);
+    for (int pg = 0; pg < 2; ++pg) off[pg] = pages.add[pg] - (m == -INFINITY ? 0.f : m);
 #pragma unroll
     for (int ks = 0; ks < kAhead; ++ks) k[ks] = read_k(k_buffer, k_kb, ks);
     __builtin_amdgcn_sched_barrier(0);
-    auto weigh = [&](int w, int nb) {  // pair w of 8: registers 2 w and 2 w + 1
+    auto weigh = [&](int w) {  // pair w of 8: registers 2 w and 2 w + 1
       const int st = w / 4;
-      const float x = fast_exp2(fmaf(now[nb][2 * w], pages.mul[st], off[nb][st]));
-      const float y = fast_exp2(fmaf(now[nb][2 * w + 1], pages.mul[st], off[nb][st]));
+      const float x = fast_exp2(fmaf(now[2 * w], pages.mul[st], off[st]));
+      const float y = fast_exp2(fmaf(now[2 * w + 1], pages.mul[st], off[st]));
       unsigned packed = EV::pack2(x, y);
       if constexpr (KV::kScaled) {
-        l[nb] = fmaf(x + y, pages.inv[st], l[nb]);
+        l = fmaf(x + y, pages.inv[st], l);
         packed = pages.loud[st] ? packed : 0u;
       } else if constexpr (EV::kHalfPartials) {
         const h2 ones = {(_Float16)1.0f, (_Float16)1.0f};
-        l[nb] = __builtin_amdgcn_fdot2(__builtin_bit_cast(h2, packed), ones, l[nb], false);
+        l = __builtin_amdgcn_fdot2(__builtin_bit_cast(h2, packed), ones, l, false);
       } else {
-        l[nb] += x + y;
+        l += x + y;
       }
-      p[st][nb][w % 4] = packed;
+      p[st][w % 4] = packed;
     };
     // Five of a row's eight pairs among the scores' products, three among the first half of
     // those with V, which take the pairs before.
@@ -345,33 +336,27 @@ struct TileShare {
         k[ks + kAhead] = read_k(k_buffer, k_kb, ks + kAhead);
       else
         v[ks + kAhead - KS] = read_v(v_buffer, v_kb, ks + kAhead - KS);
+      score(k[ks], ks, next);
 #pragma unroll
-      for (int nb = 0; nb < NBW; ++nb) {
-        score(k[ks], ks, nb, next);
-#pragma unroll
-        for (int w = 0; w < kEarly; ++w)
-          if (w * KS / kEarly == ks) weigh(w, nb);
-        __builtin_amdgcn_sched_barrier(0);
-      }
+      for (int w = 0; w < kEarly; ++w)
+        if (w * KS / kEarly == ks) weigh(w);
+      __builtin_amdgcn_sched_barrier(0);
     }
-    float top[NBW][2];
+    float top[2];
 #pragma unroll
     for (int i = 0; i < 2 * MB; ++i) {
       if (i + kAhead < 2 * MB) v[i + kAhead] = read_v(v_buffer, v_kb, i + kAhead);
+      acc[i % MB] = mma32<EV>(v[i], p[i / MB], acc[i % MB]);
+      if (i < MB) {
 #pragma unroll
-      for (int nb = 0; nb < NBW; ++nb) {
-        acc[i % MB][nb] = mma32<EV>(v[i], p[i / MB][nb], acc[i % MB][nb]);
-        if (i < MB) {
+        for (int w = kEarly; w < 8; ++w)
+          if ((w - kEarly) * MB / (8 - kEarly) == i) weigh(w);
+      } else {
 #pragma unroll
-          for (int w = kEarly; w < 8; ++w)
-            if ((w - kEarly) * MB / (8 - kEarly) == i) weigh(w, nb);
-        } else {
-#pragma unroll
-          for (int w = 0; w < 8; ++w)
-            if (w * MB / 8 == i - MB) fold_top(next, w, nb, top);
-        }
-        __builtin_amdgcn_sched_barrier(0);
+        for (int w = 0; w < 8; ++w)
+          if (w * MB / 8 == i - MB) fold_top(next, w, top);
       }
+      __builtin_amdgcn_sched_barrier(0);
     }
     raise(top, next_pages);
   };
@@ -382,17 +367,13 @@ struct TileShare {
   __syncthreads();
   if (tiles > 1) fetch(1, id_next);
   id_next = id_of(2);
-  f16v s0[NBW], s1[NBW];
-  float top[NBW][2];
+  f16v s0, s1;
+  float top[2];
   Pages pages = pages_of(0, 0);
 #pragma unroll
-  for (int ks = 0; ks < KS; ++ks)
+  for (int ks = 0; ks < KS; ++ks) score(read_k(0, 0, ks), ks, s0);
 #pragma unroll
-    for (int nb = 0; nb < NBW; ++nb) score(read_k(0, 0, ks), ks, nb, s0);
-#pragma unroll
-  for (int w = 0; w < 8; ++w)
-#pragma unroll
-    for (int nb = 0; nb < NBW; ++nb) fold_top(s0, w, nb, top);
+  for (int w = 0; w < 8; ++w) fold_top(s0, w, top);
   raise(top, pages);
   for (int t = 0; t < tiles; ++t) {
     const Pages second = pages_of(t, 1);
@@ -409,47 +390,41 @@ struct TileShare {
     __syncthreads();
   }
 
-  // Partial rows, a block of 32 at a time through LDS.
+  // Partial rows through LDS.
   float* stage = (float*)lds + wave * 32 * kStageRow;
   const __amdgpu_buffer_rsrc_t pr = __builtin_amdgcn_make_buffer_rsrc(
       (void*)a.part_o, (short)0, (int)a.part_o_bytes, kBufferFlags);
+  const LanePair both = lane_pair<32>(l);
+  const float sum = both.lo + both.hi;
 #pragma unroll
-  for (int nb = 0; nb < NBW; ++nb) {
-    const int x0 = row0 + 32 * nb;
-    if (x0 >= n_rows) break;  // uniform
-    const LanePair both = lane_pair<32>(l[nb]);
-    const float sum = both.lo + both.hi;
+  for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
-    for (int mb = 0; mb < MB; ++mb)
+    for (int i = 0; i < 4; ++i) {
+      f4 o;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        f4 o;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) o[r] = acc[mb][nb][4 * i + r];
-        *(f4*)(stage + l32 * kStageRow + 32 * mb + 8 * i + 4 * h) = o;
-      }
-    __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
-    constexpr int CPR = HD / 4;
-#pragma unroll
-    for (int i = 0; i < CPR / 2; ++i) {
-      const int e = i * 64 + lane;  // row e / CPR (< 32), chunk e % CPR
-      const int rs = e / CPR;
-      const f4 v = *(const f4*)(stage + rs * kStageRow + 4 * (e % CPR));
-      const bool is = x0 + rs < n_rows;
-      const long long at = is ? map.part_row(args, x0 + rs) : 0;
-      __builtin_amdgcn_raw_buffer_store_b128(
-          __builtin_bit_cast(u4, v), pr,
-          is ? (unsigned)((at * HD + 4 * (e % CPR)) * 4) : kDroppedOffset, 0, kThroughAux);
+      for (int r = 0; r < 4; ++r) o[r] = acc[mb][4 * i + r];
+      *(f4*)(stage + l32 * kStageRow + 32 * mb + 8 * i + 4 * h) = o;
     }
-    __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
-    if (h == 0 && x0 + l32 < n_rows) {
-      // A NaN sum travels with a finite max, so the join counts the split.
-      const float m_out = sum == sum ? m[nb] : 0.f;
-      store_through(a.part_ml + map.part_row(args, x0 + l32) * 2,
-                    __builtin_bit_cast(unsigned long long, float2{m_out, sum}));
-    }
+  __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+  constexpr int CPR = HD / 4;
+#pragma unroll
+  for (int i = 0; i < CPR / 2; ++i) {
+    const int e = i * 64 + lane;  // row e / CPR (< 32), chunk e % CPR
+    const int rs = e / CPR;
+    const f4 v = *(const f4*)(stage + rs * kStageRow + 4 * (e % CPR));
+    const bool is = row0 + rs < n_rows;
+    const long long at = is ? map.part_row(args, row0 + rs) : 0;
+    __builtin_amdgcn_raw_buffer_store_b128(
+        __builtin_bit_cast(u4, v), pr,
+        is ? (unsigned)((at * HD + 4 * (e % CPR)) * 4) : kDroppedOffset, 0, kThroughAux);
   }
-}
+  if (h == 0 && row0 + l32 < n_rows) {
+    // A NaN sum travels with a finite max, so the join counts the split.
+    const float m_out = sum == sum ? m : 0.f;
+    store_through(a.part_ml + map.part_row(args, row0 + l32) * 2,
+                  __builtin_bit_cast(unsigned long long, float2{m_out, sum}));
+  }
+  }
 };
 
 // How the sequences' own splits read the same cache.
@@ -476,33 +451,34 @@ __device__ __forceinline__ const PartArgs& own_args() {
 // One launch for both: the first shared_wgs workgroups serve the groups, the others what
 // follows in every sequence (NB blocks of 16 rows). The one waits for the matrix cores, the
 // other for memory.
-template <int HD, int NBW, int NB, typename E, typename KV>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1)))
+template <int HD, int W, int NB, typename E, typename KV>
+__global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(W / 4)))
 void sqa_tiles_kernel(PartArgs args) {
-  using Share = TileShare<HD, NBW, E, KV>;
-  constexpr int kOwn = 4 * 16 * (HD + 4) * 4;
+  using Share = TileShare<HD, W, E, KV>;
+  constexpr int kOwn = W * 16 * (HD + 4) * 4;
   __shared__ __attribute__((aligned(16))) char lds[Share::kLds > kOwn ? Share::kLds : kOwn];
   __shared__ float lds_scale[2][2][kTilePages];  // of a tile's pages: buffer, K and V, page
   if ((int)blockIdx.x < args.shared_wgs)
     Share::run(own_args(), lds, lds_scale, blockIdx.x);
   else
-    part_share<NB, (NB > 2 ? 2 : 4) * 128 / HD, HD, E, typename OwnCache<HD, KV>::Type>(
+    part_share<NB, (NB > 2 || W > 4 ? 2 : 4) * 128 / HD, HD, W, E, typename OwnCache<HD, KV>::Type>(
         own_args(), (float*)lds, blockIdx.x - args.shared_wgs, false);
 }
 
-template <int HD, int NBW, typename E, typename KV>
-void launch_tiles_rows(const PartArgs& a, dim3 grid, hipStream_t stream) {
-  if (a.p.rows <= 32)
-    hipLaunchKernelGGL((sqa_tiles_kernel<HD, NBW, 2, E, KV>), grid, dim3(256), 0, stream, a);
-  else if constexpr (HD != 256)
-    hipLaunchKernelGGL((sqa_tiles_kernel<HD, NBW, 4, E, KV>), grid, dim3(256), 0, stream, a);
-}
-
+// Eight waves have 256 registers each, too few for 64 rows of a sequence beside the page ring.
 template <int HD, typename E, typename KV>
 void launch_tiles_hd(const PartArgs& a, dim3 grid, hipStream_t stream) {
-  if constexpr (HD != 256)
-    if (a.block_rows == 256) return launch_tiles_rows<HD, 2, E, KV>(a, grid, stream);
-  launch_tiles_rows<HD, 1, E, KV>(a, grid, stream);
+  if constexpr (HD != 256) {
+    if (a.block_rows == 256) {
+      hipLaunchKernelGGL((sqa_tiles_kernel<HD, 8, 2, E, KV>), grid, dim3(512), 0, stream, a);
+      return;
+    }
+    if (a.p.rows > 32) {
+      hipLaunchKernelGGL((sqa_tiles_kernel<HD, 4, 4, E, KV>), grid, dim3(256), 0, stream, a);
+      return;
+    }
+  }
+  hipLaunchKernelGGL((sqa_tiles_kernel<HD, 4, 2, E, KV>), grid, dim3(256), 0, stream, a);
 }
 
 template <typename E, typename KV>

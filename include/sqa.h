@@ -284,22 +284,23 @@ int sqa_paged_attention_scaled(const sqa_attention_args* args, const sqa_block_s
 
 /*
  * The cut of an sqa_paged_attention_windowed call whose sequences have at most max_seq_len
- * tokens (<= 0: as many as max_pages 16-token pages hold): splits per sequence (*num_splits
- * >= 1) and kv heads per workgroup (*wg_heads 1, 2 or 4). Any cut serves any lengths; this
- * one fills the device.
+ * tokens (<= 0: as many as max_pages 16-token pages hold). *pages_per_split 1: every
+ * sequence by itself, in up to *num_splits equal splits; 0: all pages that are looked at,
+ * end to end, in *num_splits - batch equal items. *wg_heads 1, 2 or 4: kv heads per
+ * workgroup. Any cut serves any lengths; this one fills the device.
  */
 int sqa_plan_windowed(int device, int batch, int q_len, int num_query_heads, int num_kv_heads,
                       int head_dim, int64_t window, int sink, int max_seq_len, int max_pages,
-                      int* num_splits, int* wg_heads);
+                      int kv_dtype, int* num_splits, int* pages_per_split, int* wg_heads);
 
 /*
  * sqa_paged_attention where row qi of sequence b, at position p = seq_lens[b] - q_len + qi,
  * sees of the tokens it would see there only those before `sink` and those after
  * p - window (window > 0, sink >= 0). Pages that no row sees are not read, their table
  * entries not used. kv_dtype: dtype, SQA_DTYPE_FP8_E4M3, or with `scales` (else NULL) e4m3
- * or int8 codes as for sqa_paged_attention_scaled; flags and pages_per_split 0, num_splits
- * and wg_heads from sqa_plan_windowed, workspace sqa_workspace_bytes(..., num_splits, 1)
- * bytes (0 for one split). A value that is not finite reaches the rows that see its token.
+ * or int8 codes as for sqa_paged_attention_scaled; flags 0, num_splits, pages_per_split and
+ * wg_heads from sqa_plan_windowed, workspace sqa_workspace_bytes(..., num_splits,
+ * pages_per_split) bytes (0 for one split each). A value that is not finite reaches the rows that see its token.
  * Equal inputs and cuts give equal bits.
  */
 int sqa_paged_attention_windowed(const sqa_attention_args* args, const sqa_block_scales* scales,
@@ -319,8 +320,9 @@ typedef struct sqa_shared_plan {
   int page_size;
   int num_groups;
   int most_pages;    /* of a group, in block_tables columns */
-  int num_splits;    /* of what follows in a sequence */
-  int wg_heads;      /* kv heads of its workgroups */
+  int num_splits;    /* of what follows in the sequences: as sqa_plan_windowed has them */
+  int pages_per_split;
+  int wg_heads;
   int block_rows;    /* rows of a group that go over its pages together */
   int shared_size;   /* most 16-token pages of a group's split */
   int shared_splits; /* most splits of a group */
@@ -333,28 +335,30 @@ typedef struct sqa_shared_plan {
  * same `pages` entries of their block tables; in ascending order, apart, within the batch.
  * Sequences of no group, and groups of one sequence or no page, share nothing. max_seq_len
  * and max_pages (block_tables columns) as elsewhere: shared tokens counted, and only sizing
- * the call. Lengths and page ids may change under a plan.
+ * the call. Writes *plan and, where `table` is not NULL, the 3 * num_groups + 2 * batch
+ * numbers that the caller copies to the device: the same for every max_seq_len, max_pages
+ * and kv_dtype. Lengths and page ids may change under a plan.
  */
 int sqa_plan_shared_prefix(int device, int batch, int q_len, int num_query_heads,
                            int num_kv_heads, int head_dim, int page_size, int kv_dtype,
                            int num_groups, const int32_t* groups, int max_seq_len, int max_pages,
-                           sqa_shared_plan* plan);
+                           sqa_shared_plan* plan, int32_t* table);
 
 /* Workspace bytes of a call (0: none needed, or not a plan). */
 size_t sqa_shared_workspace_bytes(const sqa_shared_plan* plan);
 
 /*
  * sqa_paged_attention of a batch with shared prefixes: the same result, the shared pages
- * read once for each block of a group's rows. groups: those the plan was made for, in device
- * memory. The shared pages are read through the table row of the group's first sequence
+ * read once for each block of a group's rows. table: the plan's, in device memory (not used
+ * where num_items is 0). The shared pages are read through the table row of the group's first sequence
  * that reaches past them with all of its rows (seq_lens[b] - q_len >= shared tokens);
  * sequences that do not (a padded batch's) go over their own pages from the first on.
- * kv_dtype and `scales` as for sqa_paged_attention_windowed; flags and pages_per_split 0,
- * num_splits the plan's. Equal inputs and plans give equal bits.
+ * kv_dtype and `scales` as for sqa_paged_attention_windowed; flags 0, num_splits and
+ * pages_per_split the plan's. Equal inputs and plans give equal bits.
  */
 int sqa_paged_attention_shared_prefix(const sqa_attention_args* args,
                                       const sqa_block_scales* scales, const sqa_shared_plan* plan,
-                                      const int32_t* groups);
+                                      const int32_t* table);
 
 /*
  * Arguments of sqa_append_scaled (set struct_size = sizeof(sqa_append_args)).

@@ -34,11 +34,11 @@ _SIGNATURES = [
     ("sqa_plan_scaled", _C.c_int, [_C.c_int] * 5 + [_C.POINTER(_C.c_int)]),
     ("sqa_paged_attention_scaled", _C.c_int, [_C.c_void_p, _C.c_void_p]),
     ("sqa_plan_windowed", _C.c_int,
-     [_C.c_int] * 6 + [_C.c_int64] + [_C.c_int] * 3 + [_C.POINTER(_C.c_int)] * 2),
+     [_C.c_int] * 6 + [_C.c_int64] + [_C.c_int] * 4 + [_C.POINTER(_C.c_int)] * 3),
     ("sqa_paged_attention_windowed", _C.c_int,
      [_C.c_void_p, _C.c_void_p, _C.c_int64, _C.c_int, _C.c_int]),
     ("sqa_plan_shared_prefix", _C.c_int,
-     [_C.c_int] * 9 + [_C.c_void_p, _C.c_int, _C.c_int, _C.c_void_p]),
+     [_C.c_int] * 9 + [_C.c_void_p, _C.c_int, _C.c_int, _C.c_void_p, _C.c_void_p]),
     ("sqa_shared_workspace_bytes", _C.c_size_t, [_C.c_void_p]),
     ("sqa_paged_attention_shared_prefix", _C.c_int,
      [_C.c_void_p, _C.c_void_p, _C.c_void_p, _C.c_void_p]),
@@ -88,7 +88,7 @@ class SharedPlan(ctypes.Structure):
 
     _fields_ = [("struct_size", _C.c_size_t)] + [(name, _C.c_int) for name in (
         "batch", "q_len", "num_query_heads", "num_kv_heads", "head_dim", "page_size", "num_groups",
-        "most_pages", "num_splits", "wg_heads", "block_rows", "shared_size", "shared_splits",
+        "most_pages", "num_splits", "pages_per_split", "wg_heads", "block_rows", "shared_size", "shared_splits",
         "num_items")]
 
 
@@ -364,16 +364,17 @@ def launch_scaled(query, output, k_view, v_view, k_scale, v_scale, block_tables,
 @functools.lru_cache(maxsize=4096)
 def plan_windowed(device_index: int, batch: int, q_len: int, num_query_heads: int,
                   num_kv_heads: int, head_dim: int, window: int, sink: int, max_seq_len: int,
-                  max_pages: int):
-    """``sqa_plan_windowed`` -> ``(num_splits, wg_heads)`` (``max_pages``: 16-token pages)."""
+                  max_pages: int, kv_dtype: int):
+    """``sqa_plan_windowed`` -> ``(num_splits, pages_per_split, wg_heads)`` (``max_pages``:
+    16-token pages)."""
     lib = load()
-    ns, heads = ctypes.c_int(0), ctypes.c_int(0)
+    ns, pps, heads = ctypes.c_int(0), ctypes.c_int(0), ctypes.c_int(0)
     rc = lib.sqa_plan_windowed(device_index, batch, q_len, num_query_heads, num_kv_heads, head_dim,
-                               window, sink, max_seq_len, max_pages, ctypes.byref(ns),
-                               ctypes.byref(heads))
+                               window, sink, max_seq_len, max_pages, kv_dtype, ctypes.byref(ns),
+                               ctypes.byref(pps), ctypes.byref(heads))
     if rc != SQA_OK:
         raise RuntimeError(f"sqa_plan_windowed failed: {last_error(lib)}")
-    return ns.value, heads.value
+    return ns.value, pps.value, heads.value
 
 
 def part_fields(query, k_view, k_scale, block_tables, draft_mask):
@@ -387,7 +388,7 @@ def part_fields(query, k_view, k_scale, block_tables, draft_mask):
 
 
 def _part_args(query, output, k_view, v_view, k_scale, v_scale, block_tables, seq_lens, draft_mask,
-               scale, out_scale, num_splits, workspace, stream_handle, fields):
+               scale, out_scale, num_splits, pages_per_split, workspace, stream_handle, fields):
     """``(sqa_attention_args, sqa_block_scales or None)`` of a call over part of a cache."""
     pool, max_pages, words, shape, types, scales = fields
     ws, ws_bytes = (0, 0) if workspace is None else (
@@ -396,7 +397,7 @@ def _part_args(query, output, k_view, v_view, k_scale, v_scale, block_tables, se
         _ARGS.size, query.data_ptr(), output.data_ptr(), k_view.data_ptr(), v_view.data_ptr(),
         *pool, block_tables.data_ptr(), seq_lens.data_ptr(), max_pages,
         0 if draft_mask is None else draft_mask.data_ptr(), words, scale, out_scale, *shape,
-        num_splits, 0, ws, ws_bytes, stream_handle or 0, 0, *types)
+        num_splits, pages_per_split, ws, ws_bytes, stream_handle or 0, 0, *types)
     return a, None if scales is None else _SCALES.pack(k_scale.data_ptr(), v_scale.data_ptr(),
                                                        *scales)
 
@@ -408,39 +409,40 @@ def launch_windowed(query, output, k_view, v_view, k_scale, v_scale, block_table
     :func:`launch_scaled`, ``fields`` from :func:`part_fields`."""
     lib = _LIB if _LIB is not None else load()
     a, scales = _part_args(query, output, k_view, v_view, k_scale, v_scale, block_tables, seq_lens,
-                           draft_mask, scale, out_scale, cut[0], workspace, stream_handle,
+                           draft_mask, scale, out_scale, cut[0], cut[1], workspace, stream_handle,
                            fields or part_fields(query, k_view, k_scale, block_tables, draft_mask))
-    if lib.sqa_paged_attention_windowed(a, scales, window, sink, cut[1]) != SQA_OK:
+    if lib.sqa_paged_attention_windowed(a, scales, window, sink, cut[2]) != SQA_OK:
         raise RuntimeError(f"sqa_paged_attention_windowed failed: {last_error(lib)}")
 
 
 @functools.lru_cache(maxsize=1024)
 def plan_shared_prefix(device_index: int, groups, shape, kv_dtype: int, max_seq_len: int,
                        max_pages: int):
-    """``sqa_plan_shared_prefix`` -> (:class:`SharedPlan`, workspace bytes); ``groups``: a tuple
-    of (first, count, pages), ``shape``: (batch, q_len, query heads, kv heads, head_dim, page
-    size), ``max_pages``: block-table columns."""
+    """``sqa_plan_shared_prefix`` -> (:class:`SharedPlan`, workspace bytes, table as a list);
+    ``groups``: a tuple of (first, count, pages), ``shape``: (batch, q_len, query heads, kv
+    heads, head_dim, page size), ``max_pages``: block-table columns."""
     lib = load()
     flat = [x for g in groups for x in g]
     plan = SharedPlan()
+    table = (ctypes.c_int32 * (len(flat) + 2 * shape[0]))()
     rc = lib.sqa_plan_shared_prefix(device_index, *shape, kv_dtype, len(groups),
                                     (ctypes.c_int32 * max(len(flat), 1))(*flat), max_seq_len,
-                                    max_pages, ctypes.byref(plan))
+                                    max_pages, ctypes.byref(plan), table)
     if rc != SQA_OK:
         raise RuntimeError(f"sqa_plan_shared_prefix failed: {last_error(lib)}")
-    return plan, int(lib.sqa_shared_workspace_bytes(ctypes.byref(plan)))
+    return plan, int(lib.sqa_shared_workspace_bytes(ctypes.byref(plan))), list(table)
 
 
 def launch_shared_prefix(query, output, k_view, v_view, k_scale, v_scale, block_tables, seq_lens,
-                         draft_mask, plan, groups, scale: float, out_scale: float, workspace,
+                         draft_mask, plan, table, scale: float, out_scale: float, workspace,
                          stream_handle: int, fields=None):
     """Call ``sqa_paged_attention_shared_prefix`` (``plan`` from :func:`plan_shared_prefix`,
-    ``groups``: its groups on the device; the rest as for :func:`launch_windowed`)."""
+    ``table``: its table on the device; the rest as for :func:`launch_windowed`)."""
     lib = _LIB if _LIB is not None else load()
     a, scales = _part_args(query, output, k_view, v_view, k_scale, v_scale, block_tables, seq_lens,
-                           draft_mask, scale, out_scale, plan.num_splits, workspace, stream_handle,
-                           fields or part_fields(query, k_view, k_scale, block_tables, draft_mask))
-    rc = lib.sqa_paged_attention_shared_prefix(a, scales, ctypes.byref(plan), groups.data_ptr())
+                           draft_mask, scale, out_scale, plan.num_splits, plan.pages_per_split,
+                           workspace, stream_handle, fields or part_fields(query, k_view, k_scale, block_tables, draft_mask))
+    rc = lib.sqa_paged_attention_shared_prefix(a, scales, ctypes.byref(plan), table.data_ptr())
     if rc != SQA_OK:
         raise RuntimeError(f"sqa_paged_attention_shared_prefix failed: {last_error(lib)}")
 

@@ -19,14 +19,18 @@ inline EvenSplits even_splits(long long pages, long long size) {
 
 struct PartArgs {
   // Of PartialArgs the fields that name buffers, shapes, strides and scales. part_o, part_ml:
-  // fp32 sums and (max in log2 units, sum) of the partial rows. Slot s of sequence b and kv
-  // head h starts at row ((s * batch + b) * hkv + h) * rows; slots 0 .. splits - 1 are the
-  // sequence's own splits, splits + j its group's split j.
+  // fp32 sums and (max in log2 units, sum) of the partial rows. A slot of kv head h and
+  // sequence b is `rows` of them. Own slot s starts at row (s * hkv + h) * rows, s = b *
+  // splits + j for the sequence's split j, or (splits 0) from seq_splits[b].first on; split j
+  // of the sequence's group at row shared_at + ((j * batch + b) * hkv + h) * rows.
   PartialArgs p;
   BlockScales scales;      // of codes with block scales
   int kv_type, scaled;     // kF16 (the query's type), kE4M3 or kInt8
-  int splits;              // most splits of a sequence's own pages
-  int wg_heads;            // kv heads a workgroup of single waves serves, 4 / wg_heads waves each
+  // Sequences' own pages. splits > 0: every sequence by itself, in at most that many equal
+  // splits. 0: the batch's pages end to end, cut into own_items equal items, of which the
+  // part in sequence b leaves slot item + b.
+  int splits, own_items;
+  int wg_heads;            // kv heads a workgroup of single waves serves
   long long window;        // a row sees the last `window` tokens up to its own (0: all)
   int sink;                // and the first `sink`
   // Groups: n_groups x (first, count, pages): sequences first .. first + count - 1 begin with
@@ -34,9 +38,11 @@ struct PartArgs {
   // together, in blocks of block_rows (16, 32 or 64: one wave's; 128 or 256: a workgroup's)
   // and splits of at most shared_size 16-token pages; n_items blocks x splits in all.
   const int32_t* groups;
+  const int2* seq_groups;  // [B]: (index of the group, -1: none; its pages)
   int n_groups, n_items, block_rows, shared_size;
   int shared_splits;       // most splits of a group
   int shared_wgs;          // workgroups that serve the groups, the first of the grid
+  long long shared_at;     // partial row of the groups' first slot
   FastDiv by_rows;         // p.rows
   FastDiv by_shared_heads; // workgroups per item
 };

@@ -34,18 +34,32 @@ __global__ __launch_bounds__(256) void sqa_join_kernel(PartArgs args) {
   const int r = qi * a.group + h - kvh * a.group;
   const int len = max(scalar_load(a.seq_lens + b), 0);
   const Span span = span_of(args, b, len);
-  const int own = __builtin_amdgcn_readfirstlane(span.count);
-  if (span.group.pages == 0 && own <= 1) return;  // uniform
-  int shared = 0;
-  if (span.group.pages > 0) {  // uniform
+  int own, first;
+  if (args.splits > 0) {
     int size;
-    even_splits(span.group.pages, args.shared_size, &shared, &size);
+    own_splits(args, span.n, &own, &size);
+    first = b * args.splits;
+    if (span.group < 0 && own <= 1) return;  // uniform: in the output
+  } else {
+    const SeqSplits t = a.seq_splits[b];
+    own = t.count;
+    first = t.first;
+    if (span.group < 0 && own == 1) return;  // uniform: in the output
+  }
+  own = __builtin_amdgcn_readfirstlane(own);
+  int shared = 0;
+  if (span.group >= 0) {  // uniform
+    int size;
+    even_splits(span.shared, args.shared_size, &shared, &size);
     shared = __builtin_amdgcn_readfirstlane(min(shared, args.shared_splits));
   }
   const int total = own + shared;
-  const long long at = ((long long)b * a.hkv + kvh) * a.rows + r;
-  const long long step = (long long)a.batch * a.hkv * a.rows;
-  auto place = [&](int j) { return at + (j < own ? j : args.splits + j - own) * step; };
+  const long long own_at = ((long long)first * a.hkv + kvh) * a.rows + r;
+  const long long group_at = args.shared_at + ((long long)b * a.hkv + kvh) * a.rows + r;
+  const long long step = (long long)a.hkv * a.rows;
+  auto place = [&](int j) {
+    return j < own ? own_at + j * step : group_at + (j - own) * step * a.batch;
+  };
   const int c = lane % CH, sg = lane / CH;
   float m = -INFINITY, l = 0.f;
   f4 acc = {0.f, 0.f, 0.f, 0.f};

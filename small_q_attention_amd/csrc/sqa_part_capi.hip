@@ -5,6 +5,8 @@
 #include "sqa_part.h"
 
 #include <math.h>
+
+#include <cmath>
 #include <string.h>
 
 #include <algorithm>
@@ -41,46 +43,97 @@ int check_shape(int batch, int q_len, int num_query_heads, int num_kv_heads, int
   return SQA_OK;
 }
 
-// How sequences' own pages are dealt to workgroups of four waves: `splits` shares a
-// sequence, `wg_heads` kv heads to a workgroup and 4 / wg_heads waves to a head.
-struct OwnCut {
-  int splits, wg_heads;
-  long long workgroups(long long batch, int num_kv_heads) const {
-    return batch * splits * ceil_div(num_kv_heads, wg_heads);
+// A model of a call's time, in microseconds, by which the cuts are chosen. Workgroups of
+// `waves` waves, one to a compute unit: a second one there waits for the first one's loads,
+// so what counts is rounds.
+struct Model {
+  int cus, batch, rows, num_kv_heads, head_dim, kv_bytes;
+
+  // A page (16 tokens of one head's K and V) for each wave of a workgroup, `n` of them at
+  // work: the device's 6.6 TB/s shared out, at most 34 GB/s to a unit (both measured, 16 to
+  // 128 sequences of 34 to 258 pages), less where the heads read together make short runs.
+  double page(long long n, int heads, int waves) const {
+    const int run = std::min(heads, num_kv_heads) * head_dim * kv_bytes;
+    const double worse = run >= 1024 ? 1.0 : run >= 512 ? 1.05 : run >= 256 ? 1.15 : 1.35;
+    const double bytes = 32.0 * head_dim * kv_bytes * waves * worse;
+    return std::max({0.55, bytes * std::min<long long>(n, cus) / 6.6e6, bytes / 34e3});
   }
-  long long wave_pages(long long pages) const {
-    return ceil_div(ceil_div(pages, splits), 4 / wg_heads);
+  // Partial rows written and read again, and the kernel that joins them.
+  double join(double slots) const {
+    return 4 + slots * num_kv_heads * rows * head_dim * 8 / 4e6;
   }
 };
 
-// Rounds that `n` workgroups take on `cus` compute units, one to a unit: whole ones while
-// they are few, then (they end one by one) about as many as there is work for.
-double rounds_of(long long n, int cus) {
-  const double r = (double)n / cus;
-  return r <= 2 ? (double)ceil_div(n, cus) : r + 0.5;
-}
+// How the sequences' own pages are dealt out: `splits` equal splits of every sequence, or
+// (0) `items` equal items of the whole batch; `heads` kv heads to a workgroup.
+struct OwnCut {
+  int splits, items, heads;
+  double workgroups, time;  // of one of them
+  double slots;             // partial slots that are written
+};
 
-// The cut of `batch` sequences of up to `pages` pages for which the rounds times (pages of a
-// wave + what a workgroup costs besides, in pages) is least; from two splits on the join
-// kernel costs too. Four heads to a workgroup where that is as good: neighbouring heads'
-// slices of a token are then read together.
-OwnCut own_cut(int cus, long long batch, int num_kv_heads, long long pages) {
-  constexpr double kStart = 6, kJoin = 7;
-  OwnCut best = {1, 1};
-  double best_cost = -1;
+// Calls try(cut) for the cuts worth a look. Sequences have up to `most` pages, `mean` on
+// average.
+template <typename Try>
+void own_cuts(const Model& m, int waves, long long most, double mean, bool may_cross, Try&& attempt) {
+  constexpr double kStart = 5, kPiece = 4;
   for (int heads = 4; heads >= 1; heads /= 2) {
-    if (heads / 2 >= num_kv_heads) continue;  // a smaller workgroup holds them all
-    for (int n = 1; n <= 256 && (n == 1 || n * sqa::kMinSplitPages <= pages); ++n) {
-      const OwnCut c = {n, heads};
-      const double cost = rounds_of(c.workgroups(batch, num_kv_heads), cus) *
-                              ((double)c.wave_pages(pages) + kStart) + (n > 1 ? kJoin : 0);
-      if (best_cost < 0 || cost < best_cost * 0.99) {
-        best = c;
-        best_cost = cost;
-      }
+    if (heads / 2 >= m.num_kv_heads) continue;  // a smaller workgroup holds them all
+    const long long head_groups = ceil_div(m.num_kv_heads, heads);
+    const int share = waves / heads;  // waves that divide a share's pages
+    for (int n = 1; n <= 256 && (n == 1 || n * sqa::kMinSplitPages <= most);
+         n += std::max(1, n / 8)) {
+      const long long wgs = m.batch * n * head_groups;
+      const long long pages = ceil_div(ceil_div(most, n), share);
+      attempt(OwnCut{n, 0, heads, (double)wgs, kStart + pages * m.page(wgs, heads, waves),
+                     n > 1 ? (double)m.batch * n : 0.0});
+    }
+    if (m.batch == 1 || !may_cross) continue;
+    const double total = std::max(m.batch * mean, 1.0);
+    const long long all = std::max<long long>(m.cus / head_groups, 1);
+    for (long long n = all; n >= 1; n = n > 8 ? n * 7 / 8 : n - 1) {
+      if (n > 1 && total / n < sqa::kMinSplitPages) continue;
+      const double pages = std::max(std::ceil(total / n / share), 1.0);
+      attempt(OwnCut{0, (int)n, heads, (double)(n * head_groups),
+                     kStart + kPiece * (1 + (double)m.batch / n) +
+                         pages * m.page(n * head_groups, heads, waves),
+                     (double)(n + m.batch)});
     }
   }
+}
+
+// When `first` workgroups of time t1, then n of time t2, have run on the device, each unit
+// taking the next as it gets free.
+double finish(int cus, double first, double t1, double n, double t2) {
+  if (first + n > 2 * cus) {  // many: they end one by one
+    const double each = (first * t1 + n * t2) / (first + n);
+    return (first * t1 + n * t2) / cus + each / 2;
+  }
+  const double whole = std::floor(first / cus), rest = first - whole * cus, free = cus - rest;
+  const double base = whole * t1;
+  const double beside = rest > 0 ? std::floor(t1 / t2) * free : 0;  // while the last of those run
+  if (n <= beside) return base + std::max(t1, std::ceil(n / free) * t2);
+  return base + (rest > 0 ? t1 : 0) + std::ceil((n - beside) / cus) * t2;
+}
+
+// The cut of sequences without a group.
+OwnCut best_own(const Model& m, long long most, double mean, bool may_cross) {
+  OwnCut best{};
+  double best_cost = -1;
+  own_cuts(m, 4, most, mean, may_cross, [&](const OwnCut& c) {
+    const double cost = finish(m.cus, 0, 1, c.workgroups, c.time) +
+                        (c.slots > 0 ? m.join(c.slots) : 0);
+    if (best_cost < 0 || cost < best_cost * 0.995) {
+      best = c;
+      best_cost = cost;
+    }
+  });
   return best;
+}
+
+// Whether the pages of a batch can be numbered from end to end.
+bool may_cross(long long batch, long long kernel_pages) {
+  return batch * kernel_pages < (1LL << 27);
 }
 
 // Pages that a window leaves of a sequence of up to `pages`: the first tokens', and those
@@ -148,9 +201,13 @@ int fill(const sqa_attention_args& a, const sqa_block_scales* scales, int wg_hea
   if (!(a.scale > 0.f) || !isfinite(a.scale) || !isfinite(a.out_scale))
     return fail(SQA_ERR_INVALID, "scale must be positive and finite, out_scale finite");
   if (a.flags) return fail(SQA_ERR_INVALID, "unknown flags %#x", (unsigned)a.flags);
-  if (a.pages_per_split != 0)
-    return fail(SQA_ERR_INVALID, "pages_per_split must be 0: the device cuts the pages");
-  if (a.num_splits <= 0) return fail(SQA_ERR_INVALID, "num_splits must be positive");
+  if (a.pages_per_split != 0 && a.pages_per_split != 1)
+    return fail(SQA_ERR_INVALID, "pages_per_split must be 0 or 1, as the plan has it");
+  if (a.num_splits <= 0 || (a.pages_per_split == 0 && a.num_splits <= a.batch))
+    return fail(SQA_ERR_INVALID, "num_splits must be positive, and more than the batch where "
+                                 "splits cross sequence ends");
+  if (a.pages_per_split == 0 && !may_cross(a.batch, (long long)a.max_pages << shift))
+    return fail(SQA_ERR_INVALID, "batch * pages per row must be under 2^27");
   if (wg_heads != 1 && wg_heads != 2 && wg_heads != 4)
     return fail(SQA_ERR_INVALID, "wg_heads must be 1, 2 or 4, got %d", wg_heads);
 
@@ -188,7 +245,8 @@ int fill(const sqa_attention_args& a, const sqa_block_scales* scales, int wg_hea
                    (unsigned)(4 * scales->head_stride)};
   out->scaled = scales != nullptr;
   out->kv_type = codes ? (a.kv_dtype == SQA_DTYPE_INT8 ? sqa::kInt8 : sqa::kE4M3) : sqa::kF16;
-  out->splits = a.num_splits;
+  out->splits = a.pages_per_split ? a.num_splits : 0;
+  out->own_items = a.pages_per_split ? 0 : a.num_splits - a.batch;
   out->wg_heads = wg_heads;
   p.by_head_groups = sqa::fast_div((unsigned)ceil_div(a.num_kv_heads, wg_heads));
   p.by_splits = sqa::fast_div(a.num_splits);
@@ -197,7 +255,13 @@ int fill(const sqa_attention_args& a, const sqa_block_scales* scales, int wg_hea
   return SQA_OK;
 }
 
-// The partials' place in the workspace: `rows` rows of sums, then of (max, sum).
+// Slots of the sequences' own pages.
+long long own_slots(int batch, int num_splits, int pages_per_split) {
+  return pages_per_split ? (long long)batch * num_splits : num_splits;
+}
+
+// The partials' place in the workspace: `rows` rows of sums, then of (max, sum), then the
+// sequences' first slots and counts.
 int place(const sqa_attention_args& a, long long rows, size_t need, sqa::PartArgs* s) {
   if (need == 0) return SQA_OK;
   if (!a.workspace || a.workspace_bytes < need)
@@ -212,6 +276,7 @@ int place(const sqa_attention_args& a, long long rows, size_t need, sqa::PartArg
   s->p.part_o = (float*)a.workspace;
   s->p.part_o_bytes = (unsigned)bytes;
   s->p.part_ml = s->p.part_o + rows * a.head_dim;
+  s->p.seq_splits = (sqa::SeqSplits*)(s->p.part_ml + rows * 2);
   return SQA_OK;
 }
 
@@ -229,63 +294,60 @@ struct SharedGroup {
   long long count, pages;  // 16-token pages
 };
 
-// The cut of a batch with groups, by a model of the call's time in microseconds. A workgroup
-// takes `page` for a page per wave of what waits for memory (a page of 16 x 128 16-bit
-// elements of K and V: between 0.65 and 1.05 as few or all compute units stream), `tile_page`
-// for a page of the tiles, whose blocks are bound by the matrix cores, and 6 or 10 besides;
-// n1 workgroups for the groups begin first, those for the sequences fill the units they
-// leave; a partial row is written and read once.
 struct SharedCut {
   OwnCut own;
   long long size;  // most pages of a group's split
 };
+
+// The cut of a batch with groups. The groups' workgroups begin first. Where a wave holds a
+// block's rows they take their pages like the sequences'; tiles, bound by the matrix cores,
+// 0.56 us for a page of head dim 128 and 256 rows, 0.35 for 128 rows.
 template <typename Groups>
-SharedCut shared_cut(int cus, long long batch, long long rows, int num_kv_heads, int head_dim,
-                     int kv_bytes, int block_rows, int num_groups, const Groups& group,
-                     long long own_pages) {
-  const double wide = head_dim / 128.0;
-  const double page = std::max(0.9 * wide * kv_bytes / 2, 0.35);
-  const double tile_page = (block_rows == 256 ? 0.6 : 0.35) * wide;
+SharedCut shared_cut(const Model& m, int block_rows, int num_groups, const Groups& group,
+                     long long own_most, double own_mean, bool crosses) {
   const bool tiles = block_rows > 64;
-  // Half of the room: sequences of a batch seldom all have the greatest length.
-  const double own_mean = std::max(0.6 * own_pages, 1.0);
+  const int waves = block_rows == 256 ? 8 : 4;
+  const double tile_page = (block_rows == 256 ? 0.56 : 0.35) * m.head_dim / 128;
   long long longest = 1;
   for (int g = 0; g < num_groups; ++g) longest = std::max(longest, group(g).pages);
+  struct Option {
+    long long size;
+    double items, slots;
+  };
+  Option options[64];
+  int n_options = 0;
+  for (int n = 1; n <= 256 && (n == 1 || n * sqa::kMinSplitPages <= longest);
+       n += std::max(1, n / 8)) {
+    Option o{ceil_div(longest, n), 0, 0};
+    if (n_options > 0 && o.size == options[n_options - 1].size) continue;
+    for (int g = 0; g < num_groups; ++g) {
+      const long long splits = sqa::even_splits(group(g).pages, o.size).count;
+      o.items += (double)ceil_div(group(g).count * m.rows, block_rows) * splits;
+      o.slots += (double)group(g).count * splits;
+    }
+    options[n_options++] = o;
+    if (n_options == 64) break;
+  }
   SharedCut best{};
   double best_cost = -1;
-  long long last_size = 0;
-  for (int heads = 4; heads >= 1; heads /= 2) {
-    if (heads / 2 >= num_kv_heads) continue;
-    const int waves = 4 / heads;
-    last_size = 0;
-    for (int n = 1; n <= 256 && (n == 1 || n * sqa::kMinSplitPages <= longest); ++n) {
-      const long long size = ceil_div(longest, n);
-      if (size == last_size) continue;
-      last_size = size;
-      long long items = 0, part = 0;
-      for (int g = 0; g < num_groups; ++g) {
-        const long long splits = sqa::even_splits(group(g).pages, size).count;
-        items += ceil_div(group(g).count * rows, block_rows) * splits;
-        part += group(g).count * splits;
-      }
-      const double n1 = (double)items * (tiles ? num_kv_heads : ceil_div(num_kv_heads, heads));
-      const double t1 = tiles ? size * tile_page + 10 : ceil_div(size, waves) * page + 6;
-      for (int m = 1; m <= 256 && (m == 1 || m * sqa::kMinSplitPages <= own_pages); m += m < 8 ? 1 : m / 4) {
-        const double splits = std::max(std::min((double)m, own_mean / sqa::kMinSplitPages), 1.0);
-        const double n2 = batch * splits * ceil_div(num_kv_heads, heads);
-        const double mean = own_mean / splits / waves, most = (double)own_pages / m / waves;
-        const double t2 = std::max(mean, 1.0) * page + 6;
-        const double work = (n1 * t1 + n2 * t2) / cus;
-        const double join = (part + batch * splits) * num_kv_heads * rows * head_dim * 8 / 4e6;
-        const double cost = std::max({t1 * ceil_div((long long)n1, cus), most * page + 6,
-                                      work + 0.5 * (n1 > cus ? std::max(t1, t2) : t2)}) + join;
-        if (best_cost < 0 || cost < best_cost * 0.99) {
-          best = {{m, heads}, size};
-          best_cost = cost;
-        }
+  own_cuts(m, waves, own_most, own_mean, crosses, [&](const OwnCut& c) {
+    const double head_groups = (double)ceil_div(m.num_kv_heads, c.heads);
+    // Every sequence that shares leaves partial rows.
+    const double slots = c.splits > 0 ? (double)m.batch * std::max(std::min((double)c.splits,
+                                            own_mean / sqa::kMinSplitPages), 1.0) : c.slots;
+    for (int i = 0; i < n_options; ++i) {
+      const Option& o = options[i];
+      const double n1 = o.items * (tiles ? m.num_kv_heads : head_groups);
+      const double t1 = tiles ? 10 + o.size * tile_page
+                              : 6 + ceil_div(o.size, waves / c.heads) *
+                                        m.page((long long)(n1 + c.workgroups), c.heads, waves);
+      const double cost = finish(m.cus, n1, t1, c.workgroups, c.time) + m.join(slots + o.slots);
+      if (best_cost < 0 || cost < best_cost * 0.995) {
+        best = {c, o.size};
+        best_cost = cost;
       }
     }
-  }
+  });
   return best;
 }
 
@@ -296,18 +358,26 @@ int check_plan(const sqa_shared_plan* p) {
                 p->struct_size, sizeof(sqa_shared_plan));
   if (p->batch <= 0 || p->q_len <= 0 || p->num_kv_heads <= 0 || p->num_query_heads <= 0 ||
       p->head_dim <= 0 || p->num_groups < 0 || p->num_items < 0 || p->num_splits <= 0 ||
-      p->shared_splits < 0 || p->shared_size <= 0)
+      p->shared_splits < 0 || p->shared_size <= 0 ||
+      (p->pages_per_split == 0 && p->num_splits <= p->batch))
     return fail(SQA_ERR_INVALID, "not a plan of sqa_plan_shared_prefix");
   return SQA_OK;
 }
 
-// Partial rows of a plan's slots.
+// Partial rows of a plan's own slots, and of all.
+long long own_rows(const sqa_shared_plan& p) {
+  return own_slots(p.batch, p.num_splits, p.pages_per_split) * p.q_len * p.num_query_heads;
+}
 long long plan_rows(const sqa_shared_plan& p) {
-  return ((long long)p.num_splits + p.shared_splits) * p.batch * p.q_len * p.num_query_heads;
+  return own_rows(p) + (long long)p.shared_splits * p.batch * p.q_len * p.num_query_heads;
+}
+
+int kv_bytes(int kv_dtype) {
+  return kv_dtype == SQA_DTYPE_FP8_E4M3 || kv_dtype == SQA_DTYPE_INT8 ? 1 : 2;
 }
 
 bool workgroups_fit(const sqa::PartArgs& s) {
-  return (long long)s.p.batch * s.splits * s.p.hkv <= 0x3fffffffLL;
+  return ((long long)s.p.batch * s.splits + s.own_items) * s.p.hkv <= 0x3fffffffLL;
 }
 
 }  // namespace
@@ -316,8 +386,8 @@ extern "C" {
 
 int sqa_plan_windowed(int device, int batch, int q_len, int num_query_heads, int num_kv_heads,
                       int head_dim, int64_t window, int sink, int max_seq_len, int max_pages,
-                      int* num_splits, int* wg_heads) {
-  if (!num_splits || !wg_heads) return fail(SQA_ERR_INVALID, "null output pointer");
+                      int kv_dtype, int* num_splits, int* pages_per_split, int* wg_heads) {
+  if (!num_splits || !pages_per_split || !wg_heads) return fail(SQA_ERR_INVALID, "null output pointer");
   long long rows = 0;
   if (int rc = check_shape(batch, q_len, num_query_heads, num_kv_heads, head_dim, &rows)) return rc;
   if (max_pages <= 0) return fail(SQA_ERR_INVALID, "max_pages must be positive");
@@ -327,10 +397,14 @@ int sqa_plan_windowed(int device, int batch, int q_len, int num_query_heads, int
   if (cus <= 0) return SQA_ERR_HIP;
   long long pages = max_pages;
   if (max_seq_len > 0) pages = std::min(pages, ceil_div(max_seq_len, sqa::kPageSize));
-  pages = window_pages(pages, std::min(window, (int64_t)1 << 31), sink, q_len);
-  const OwnCut cut = own_cut(cus, batch, num_kv_heads, pages);
-  *num_splits = cut.splits;
-  *wg_heads = cut.wg_heads;
+  const long long left = window_pages(pages, std::min(window, (int64_t)1 << 31), sink, q_len);
+  const Model m{cus, batch, (int)rows, num_kv_heads, head_dim, kv_bytes(kv_dtype)};
+  // Sequences longer than the window are all alike, shorter ones seldom.
+  const OwnCut cut = best_own(m, left, left < pages ? left : 0.65 * left,
+                              may_cross(batch, max_pages));
+  *pages_per_split = cut.splits > 0;
+  *num_splits = cut.splits > 0 ? cut.splits : cut.items + batch;
+  *wg_heads = cut.heads;
   return SQA_OK;
 }
 
@@ -348,9 +422,10 @@ int sqa_paged_attention_windowed(const sqa_attention_args* args, const sqa_block
   s.window = std::min(window, (int64_t)1 << 31);
   s.sink = sink;
   if (!workgroups_fit(s)) return fail(SQA_ERR_INVALID, "grid too large");
-  const long long rows = (long long)a.batch * a.num_splits * a.num_kv_heads * s.p.rows;
+  const long long rows = own_slots(a.batch, a.num_splits, a.pages_per_split) * a.num_kv_heads *
+                         s.p.rows;
   const size_t need = sqa_workspace_bytes(a.batch, a.q_len, a.num_query_heads, a.num_kv_heads,
-                                          a.head_dim, a.num_splits, 1);
+                                          a.head_dim, a.num_splits, a.pages_per_split);
   if (int rc = place(a, rows, need, &s)) return rc;
 
   hipStream_t stream = (hipStream_t)a.stream;
@@ -360,7 +435,7 @@ int sqa_paged_attention_windowed(const sqa_attention_args* args, const sqa_block
   if ((e = sqa::launch_own(s, stream)) != hipSuccess)
     return hip_fail(e, "windowed attention kernel launch");
   if (ev && (e = hipEventRecord(ev[1], stream)) != hipSuccess) return hip_fail(e, "hipEventRecord");
-  if (a.num_splits > 1 && (e = sqa::launch_join(s, stream)) != hipSuccess)
+  if (need > 0 && (e = sqa::launch_join(s, stream)) != hipSuccess)
     return hip_fail(e, "join kernel launch");
   if (ev && (e = hipEventRecord(ev[2], stream)) != hipSuccess) return hip_fail(e, "hipEventRecord");
   return SQA_OK;
@@ -369,7 +444,7 @@ int sqa_paged_attention_windowed(const sqa_attention_args* args, const sqa_block
 int sqa_plan_shared_prefix(int device, int batch, int q_len, int num_query_heads,
                            int num_kv_heads, int head_dim, int page_size, int kv_dtype,
                            int num_groups, const int32_t* groups, int max_seq_len, int max_pages,
-                           sqa_shared_plan* plan) {
+                           sqa_shared_plan* plan, int32_t* table) {
   if (!plan) return fail(SQA_ERR_INVALID, "null output pointer");
   long long rows = 0;
   if (int rc = check_shape(batch, q_len, num_query_heads, num_kv_heads, head_dim, &rows)) return rc;
@@ -422,16 +497,16 @@ int sqa_plan_shared_prefix(int device, int batch, int q_len, int num_query_heads
   out.block_rows = 16;
   out.shared_size = 1;
   out.most_pages = (int)most_pages;
+  const Model m{cus, batch, (int)rows, num_kv_heads, head_dim, kv_bytes(kv_dtype)};
+  const bool crosses = may_cross(batch, (long long)max_pages << shift);
+  OwnCut own_cut;
   if (longest == 0) {
-    const OwnCut cut = own_cut(cus, batch, num_kv_heads, own);
-    out.num_splits = cut.splits;
-    out.wg_heads = cut.wg_heads;
+    own_cut = best_own(m, own, 0.65 * own, crosses);
   } else {
     out.num_groups = num_groups;
     out.block_rows = rows_of_block(most_rows, rows, head_dim);
-    const int bytes = kv_dtype == SQA_DTYPE_FP8_E4M3 || kv_dtype == SQA_DTYPE_INT8 ? 1 : 2;
-    const SharedCut cut = shared_cut(cus, batch, rows, num_kv_heads, head_dim, bytes,
-                                     out.block_rows, num_groups, group, own);
+    const SharedCut cut = shared_cut(m, out.block_rows, num_groups, group, own, 0.65 * own,
+                                     crosses);
     long long items = 0;
     for (int i = 0; i < num_groups; ++i) {
       const SharedGroup g = group(i);
@@ -440,24 +515,39 @@ int sqa_plan_shared_prefix(int device, int batch, int q_len, int num_query_heads
       out.shared_splits = std::max(out.shared_splits, splits);
     }
     if (items * num_kv_heads > 0x3fffffffLL) return fail(SQA_ERR_INVALID, "grid too large");
-    out.num_splits = cut.own.splits;
-    out.wg_heads = cut.own.wg_heads;
+    own_cut = cut.own;
     out.num_items = (int)items;
     out.shared_size = (int)cut.size;
   }
+  out.pages_per_split = own_cut.splits > 0;
+  out.num_splits = own_cut.splits > 0 ? own_cut.splits : own_cut.items + batch;
+  out.wg_heads = own_cut.heads;
   *plan = out;
+  if (!table) return SQA_OK;
+  for (int i = 0; i < 3 * num_groups; ++i) table[i] = groups[i];
+  int32_t* of = table + 3 * num_groups;
+  for (int b = 0; b < batch; ++b) {
+    of[2 * b] = -1;
+    of[2 * b + 1] = 0;
+  }
+  for (int i = 0; i < num_groups; ++i)
+    for (int b = groups[3 * i]; group(i).pages > 0 && b < groups[3 * i] + groups[3 * i + 1]; ++b) {
+      of[2 * b] = i;
+      of[2 * b + 1] = groups[3 * i + 2];
+    }
   return SQA_OK;
 }
 
 size_t sqa_shared_workspace_bytes(const sqa_shared_plan* plan) {
   if (check_plan(plan)) return 0;
-  if (plan->num_splits == 1 && plan->num_items == 0) return 0;
-  return (size_t)plan_rows(*plan) * ((size_t)plan->head_dim + 2) * sizeof(float);
+  if (plan->pages_per_split && plan->num_splits == 1 && plan->num_items == 0) return 0;
+  return (size_t)plan_rows(*plan) * ((size_t)plan->head_dim + 2) * sizeof(float) +
+         (plan->pages_per_split ? 0 : (size_t)plan->batch * sizeof(sqa::SeqSplits));
 }
 
 int sqa_paged_attention_shared_prefix(const sqa_attention_args* args,
                                       const sqa_block_scales* scales, const sqa_shared_plan* plan,
-                                      const int32_t* groups) {
+                                      const int32_t* table) {
   if (!args) return fail(SQA_ERR_INVALID, "null argument struct");
   if (args->struct_size != sizeof(sqa_attention_args))
     return fail(SQA_ERR_INVALID, "struct_size %zu does not match this library's %zu",
@@ -469,7 +559,7 @@ int sqa_paged_attention_shared_prefix(const sqa_attention_args* args,
   if (plan->batch != a.batch || plan->q_len != a.q_len ||
       plan->num_query_heads != a.num_query_heads || plan->num_kv_heads != a.num_kv_heads ||
       plan->head_dim != a.head_dim || plan->page_size != a.page_size ||
-      plan->num_splits != a.num_splits)
+      plan->num_splits != a.num_splits || plan->pages_per_split != a.pages_per_split)
     return fail(SQA_ERR_INVALID, "the plan was made for another batch, q_len, heads, page size or "
                                  "number of splits");
   if (plan->most_pages > a.max_pages)
@@ -477,14 +567,15 @@ int sqa_paged_attention_shared_prefix(const sqa_attention_args* args,
                 plan->most_pages, a.max_pages);
   const bool tiles = plan->block_rows > 64;
   if (plan->num_items > 0) {
-    if (!groups || (uintptr_t)groups % 4)
-      return fail(SQA_ERR_INVALID, "groups must be given, 4-byte aligned, in device memory");
+    if (!table || (uintptr_t)table % 4)
+      return fail(SQA_ERR_INVALID, "the plan's table must be given, 4-byte aligned");
     const int b = plan->block_rows;
     if ((b != 16 && b != 32 && b != 64 && b != 128 && b != 256) ||
         (a.head_dim == 256 && (b == 64 || b == 256)) || (b == 256 && s.p.rows > 32) ||
         (!tiles && b < s.p.rows))
       return fail(SQA_ERR_INVALID, "not a plan of sqa_plan_shared_prefix");
-    s.groups = groups;
+    s.groups = table;
+    s.seq_groups = (const int2*)(table + 3 * plan->num_groups);
     s.n_groups = plan->num_groups;
     s.n_items = plan->num_items;
     s.block_rows = b;
@@ -496,6 +587,7 @@ int sqa_paged_attention_shared_prefix(const sqa_attention_args* args,
     s.by_shared_heads = sqa::fast_div((unsigned)heads);
   }
   if (!workgroups_fit(s)) return fail(SQA_ERR_INVALID, "grid too large");
+  s.shared_at = own_rows(*plan);
   const size_t need = sqa_shared_workspace_bytes(plan);
   if (int rc = place(a, plan_rows(*plan), need, &s)) return rc;
 

@@ -39,17 +39,6 @@ __device__ __forceinline__ Group from_lane(const Group& g, int src) {
           __builtin_amdgcn_readlane(g.pages, src)};
 }
 
-// Sequence b's group (pages 0: none). The whole wave looks, a lane to a group.
-__device__ __forceinline__ Group group_of(const PartArgs& a, int b) {
-  for (int k = 0; k < a.n_groups; k += 64) {
-    const Group g = load_group(a, k + (threadIdx.x & 63));
-    const unsigned long long hit =
-        __ballot(g.pages > 0 && b >= g.first && b - g.first < g.count);
-    if (hit) return from_lane(g, __builtin_ctzll(hit));
-  }
-  return {0, 0, 0};
-}
-
 // Whether all rows of a sequence of `len` tokens lie behind `pages` shared pages.
 __device__ __forceinline__ bool reaches(const PartArgs& a, int len, int pages) {
   return len >= a.p.q_len && (len - a.p.q_len) / kPageSize >= pages;
@@ -67,23 +56,20 @@ __device__ __forceinline__ int leader_of(const PartArgs& a, const Group& g) {
   return -1;
 }
 
-// The kernel pages that a sequence's own splits cover: [0, head) and from `tail` on, n in
+// The kernel pages that a sequence goes over by itself: [0, head) and from `tail` on, n in
 // all, page v of them at v or, past `head`, v - head + tail.
 struct Span {
   int head, tail, n;
-  int count, size;  // splits and pages per split
-  Group group;      // pages > 0: shared, and before `tail`
+  int group;   // whose pages, `shared` of them, lie before `tail`; -1: none
+  int shared;
 };
 
 // Window: of the pages before row 0's window (the earliest) only those of the first `sink`
 // tokens. Shared prefix: what follows it, provided that every row lies behind it; a shorter
-// sequence goes over all of its pages by itself.
+// sequence goes over all of its pages by itself. Any lane's sequence.
 __device__ __forceinline__ Span span_of(const PartArgs& a, int b, int len) {
   const int pages = min((int)(((unsigned)len + kPageSize - 1) / kPageSize), a.p.max_pages);
-  Span s;
-  s.head = 0;
-  s.tail = 0;
-  s.group = {0, 0, 0};
+  Span s{0, 0, 0, -1, 0};
   if (a.window > 0) {
     const long long from = (long long)len - a.p.q_len + 1 - a.window;
     s.head = min((int)(((unsigned)a.sink + kPageSize - 1) / kPageSize), pages);
@@ -91,18 +77,87 @@ __device__ __forceinline__ Span span_of(const PartArgs& a, int b, int len) {
     s.tail = max(s.tail, s.head);
   }
   if (a.n_groups > 0) {
-    const Group g = group_of(a, b);
-    if (reaches(a, len, g.pages)) {
-      s.group = g;
-      s.tail = g.pages;
+    const int2 g = a.seq_groups[b];
+    const int shared = min(max(g.y, 0), a.p.bt_stride) << a.p.page_shift;
+    if (g.x >= 0 && g.x < a.n_groups && shared > 0 && reaches(a, len, shared)) {
+      s.group = g.x;
+      s.shared = s.tail = shared;
     }
   }
   s.n = s.head + max(pages - s.tail, 0);
-  // Splits of equal size, none of them under kMinSplitPages while there are two.
-  const int most = max(min(a.splits, s.n / kMinSplitPages), 1);
-  s.size = max(ceil_over(s.n, most), 1);
-  s.count = ceil_over(s.n, s.size);
   return s;
+}
+
+// Equal splits of one sequence's n pages, none under kMinSplitPages while there are two.
+__device__ __forceinline__ void own_splits(const PartArgs& a, int n, int* count, int* size) {
+  const int most = max(min(a.splits, n / kMinSplitPages), 1);
+  *size = max(ceil_over(n, most), 1);
+  *count = ceil_over(n, *size);
+}
+
+// The batch's own pages end to end, cut into own_items items of `size` pages: every wave
+// finds that for itself, a lane to a sequence, 64 at a time. Workgroups of one item each
+// then take the same time whatever the lengths (an extra workgroup on a compute unit waits
+// for the first: 128 sequences of 34 pages, 8 kv heads, 256 workgroups, 49 us; 130 of them,
+// one sequence to a workgroup, 77).
+// Every sequence counts kSeamPages more than it has, before its first one: about what a
+// workgroup pays to begin it (96 sequences of 16 to 128 pages: 94 -> 85 us).
+constexpr int kSeamPages = 4;
+struct OwnCut {
+  int size, total;
+  int n, len;  // of the lane's sequence among the first 64
+};
+__device__ __forceinline__ int own_pages(const PartArgs& a, int b, int* len) {
+  if (b >= a.p.batch) return 0;
+  *len = max(a.p.seq_lens[b], 0);
+  const int n = span_of(a, b, *len).n;
+  return n > 0 ? n + kSeamPages : 0;
+}
+__device__ __forceinline__ OwnCut own_cut(const PartArgs& a, bool writer) {
+  const int lane = threadIdx.x & 63;
+  OwnCut c{0, 0, 0, 0};
+  c.n = own_pages(a, lane, &c.len);
+  for (int k = 0; k < a.p.batch; k += 64) {
+    int len;
+    c.total += wave_sum_int(k == 0 ? c.n : own_pages(a, k + lane, &len));
+  }
+  c.size = max(ceil_over(c.total, a.own_items), kMinSplitPages);
+  if (!writer) return c;
+  int base = 0;  // the join's table
+  for (int k = 0; k < a.p.batch; k += 64) {
+    int len;
+    const int n = k == 0 ? c.n : own_pages(a, k + lane, &len);
+    const int incl = wave_inclusive_scan_int(n);
+    const int start = base + incl - n, first = (start + kSeamPages) / c.size;
+    if (k + lane < a.p.batch)
+      a.p.seq_splits[k + lane] =
+          SeqSplits{first + k + lane, n > 0 ? (start + n - 1) / c.size - first + 1 : 0};
+    base += __builtin_amdgcn_readlane(incl, 63);
+  }
+  return c;
+}
+// The sequence with page `at` of the batch, the first of its pages (past the seam) and how
+// many it has (b < 0: none).
+struct OwnPiece {
+  int b, len, start, n;
+};
+__device__ __forceinline__ OwnPiece own_piece(const PartArgs& a, const OwnCut& c, int at) {
+  const int lane = threadIdx.x & 63;
+  int base = 0;
+  for (int k = 0; k < a.p.batch; k += 64) {
+    int len = c.len;
+    const int n = k == 0 ? c.n : own_pages(a, k + lane, &len);
+    const int incl = wave_inclusive_scan_int(n);
+    const unsigned long long hit = __ballot(n > 0 && at < base + incl);
+    if (hit) {
+      const int src = __builtin_ctzll(hit);
+      return {k + src, __builtin_amdgcn_readlane(len, src),
+              base + __builtin_amdgcn_readlane(incl - n, src) + kSeamPages,
+              __builtin_amdgcn_readlane(n, src) - kSeamPages};
+    }
+    base += __builtin_amdgcn_readlane(incl, 63);
+  }
+  return {-1, 0, 0, 0};
 }
 
 // One item of the groups: a block of a group's rows over a split of its pages.
@@ -210,7 +265,8 @@ __device__ __forceinline__ void wild_values(WaveState<NB, HD>& st, PageV<HD, 1>&
 // Where row x of a share is: x counts the rows of one kv head of the sequences from `first`
 // on, Q * (Hq / Hkv) each.
 struct RowMap {
-  int first, kvh, slot;
+  int first, kvh;
+  long long at;  // partial row of row 0
   struct Place {
     int b, y;  // sequence, row of its kv head
   };
@@ -226,7 +282,7 @@ struct RowMap {
   }
   __device__ __forceinline__ long long part_row(const PartArgs& a, int x) const {
     const Place p = place(a, x);
-    return (((long long)slot * a.p.batch + p.b) * a.p.hkv + kvh) * a.p.rows + p.y;
+    return at + (long long)(p.b - first) * a.p.hkv * a.p.rows + p.y;
   }
 };
 
@@ -315,6 +371,16 @@ __device__ __forceinline__ void leave_rows(const PartArgs& args, WaveState<NB, H
   }
 }
 
+// The kernel's (first and only) argument, where the compiler cannot know that it was asked
+// for before: what a branch or a piece of work takes from it is loaded there, and not held in
+// scalar registers through all others (a hundred of them spilled otherwise).
+__device__ __forceinline__ const PartArgs& own_args() {
+  auto* p = (const __attribute__((address_space(4))) PartArgs*)
+      __builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return *(const PartArgs*)p;
+}
+
 // How a cache's elements go to the products. kScaled: codes with block scales.
 template <int HD>
 struct PartNative : KvNative<HD> {
@@ -392,28 +458,54 @@ __device__ __forceinline__ void scaled_page(WaveState<NB, HD>& st, const typenam
 // of a group's rows over a split of the shared pages. A wave holds all rows of its share (NB
 // blocks of 16) and keeps a ring of D pages in flight in registers.
 template <int NB, int D, int HD, int W, typename E, typename KV>
-__device__ __forceinline__ void part_share(const PartArgs& args, float* sm_stage, int block,
-                                           bool shared) {
-  const PartialArgs& a = args.p;
+__device__ __forceinline__ void part_share(float* sm_stage, int block, bool shared) {
   constexpr int KK = Dims<HD>::KK, MB = Dims<HD>::MB;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;
   const int g16 = lane >> 4, l16 = lane & 15;
-  const int wgh = args.wg_heads;
+  const PartArgs& first_args = own_args();
+  const int wgh = first_args.wg_heads;
   const int log_heads = wgh >> 1;  // of 1, 2 and 4
   const int waves = W >> log_heads;
   const int mine = wave >> log_heads;
   const int head_in = wave & (wgh - 1);
-  const int share = block / a.by_head_groups;
-  const int kvh = (block - share * ((a.hkv + wgh - 1) / wgh)) * wgh + head_in;
+  const int share = block / first_args.p.by_head_groups;
+  const int hkv = first_args.p.hkv;
+  const int kvh = (block - share * ((hkv + wgh - 1) / wgh)) * wgh + head_in;
 
-  // The share: its table row, its pages v0 .. v0 + n_pages (page v of the sequence at v, or
-  // past `head` at v + skip), its rows.
-  int b, len, head = 0, skip = 0, v0, n_pages, row0 = 0, n_rows;
+  // No such head: nothing to do, but to wait with the other heads' waves.
+  const bool is_head = kvh < hkv;
+  const int head_at = is_head ? kvh : 0;
+
+  // What the wave goes over: pages v0 .. v0 + n_pages of table row b (page v of the sequence
+  // at v, or past `head` at v + skip), for n_rows rows from row0 on.
+  int b, len, head = 0, skip = 0, v0, n_pages, row0 = 0, n_rows = first_args.p.rows;
   RowMap map;
-  map.kvh = kvh;
+  map.kvh = head_at;
   bool direct = false;
+  OwnCut cut;
+  int at = 0, end = 0;  // of an item that may cross sequence ends
+  const bool crosses = !shared && first_args.splits == 0;
+  auto piece = [&] {  // of the item, from page `at` on
+    const PartArgs& args = own_args();
+    const OwnPiece x = own_piece(args, cut, at);
+    b = __builtin_amdgcn_readfirstlane(max(x.b, 0));
+    len = __builtin_amdgcn_readfirstlane(x.len);
+    const Span span = span_of(args, b, len);
+    const int start = __builtin_amdgcn_readfirstlane(x.start);
+    const int n = __builtin_amdgcn_readfirstlane(x.n);
+    head = span.head;
+    skip = span.tail - span.head;
+    v0 = max(at - start, 0);
+    n_pages = max(min(end - start, n) - v0, 0);  // 0: the item ends in the seam
+    direct = span.group < 0 && n_pages == n;
+    map.first = b;
+    map.at = ((long long)(share + b) * args.p.hkv + head_at) * args.p.rows;
+    at = x.b < 0 ? end : start + n;
+  };
   if (shared) {  // uniform
+    const PartArgs& args = own_args();
+    const PartialArgs& a = args.p;
     const SharedItem it = item_of(args, share);
     b = it.group.pages > 0 ? leader_of(args, it.group) : -1;
     if (b < 0 || it.split >= args.shared_splits) return;  // uniform over the workgroup
@@ -423,34 +515,46 @@ __device__ __forceinline__ void part_share(const PartArgs& args, float* sm_stage
     v0 = it.begin;
     n_pages = it.n;
     map.first = it.group.first;
-    map.slot = args.splits + it.split;
+    map.at = args.shared_at +
+             (((long long)it.split * a.batch + it.group.first) * a.hkv + head_at) * a.rows;
+  } else if (crosses) {
+    const PartArgs& args = own_args();
+    cut = own_cut(args, block == 0 && wave == 0);
+    at = __builtin_amdgcn_readfirstlane(share * cut.size);
+    end = __builtin_amdgcn_readfirstlane(min(at + cut.size, cut.total));
+    if (share >= args.own_items || at >= end) return;  // uniform over the workgroup
   } else {
+    const PartArgs& args = own_args();
+    const PartialArgs& a = args.p;
     b = share / a.by_splits;
     if (b >= a.batch) return;  // uniform over the workgroup
     const int split = share - b * args.splits;
     len = max(scalar_load(a.seq_lens + b), 0);
     const Span span = span_of(args, b, len);
-    if (split >= max(span.count, 1)) return;  // uniform over the workgroup
-    direct = span.group.pages == 0 && span.count <= 1;
+    int count, size;
+    own_splits(args, span.n, &count, &size);
+    if (split >= max(count, 1)) return;  // uniform over the workgroup
+    direct = span.group < 0 && count <= 1;
     head = span.head;
     skip = span.tail - span.head;
-    v0 = split * span.size;
-    n_pages = max(min(v0 + span.size, span.n) - v0, 0);
-    n_rows = a.rows;
+    v0 = split * size;
+    n_pages = max(min(v0 + size, span.n) - v0, 0);
     map.first = b;
-    map.slot = split;
+    map.at = ((long long)share * a.hkv + head_at) * a.rows;
   }
-  if (waves > 1) {  // uniform: this wave's part of the share
+  for (;;) {  // pieces
+  if (crosses) {
+    piece();
+    if (n_pages <= 0) return;  // uniform over the workgroup
+  }
+  const PartArgs& args = own_args();
+  const PartialArgs& a = args.p;
+  if (waves > 1) {  // uniform: this wave's part
     const int each = (n_pages + waves - 1) >> ((W == 8 ? 3 : 2) - log_heads);
     v0 += mine * each;
     n_pages = max(min(each, n_pages - mine * each), 0);
   }
-  // No such head: nothing to do, but to wait with the other heads' waves.
-  const bool is_head = kvh < a.hkv;
-  if (!is_head) {
-    n_pages = 0;
-    map.kvh = 0;
-  }
+  if (!is_head) n_pages = 0;
   b = __builtin_amdgcn_readfirstlane(b);
   v0 = __builtin_amdgcn_readfirstlane(v0);
   n_pages = __builtin_amdgcn_readfirstlane(n_pages);
@@ -591,8 +695,10 @@ __device__ __forceinline__ void part_share(const PartArgs& args, float* sm_stage
 #pragma unroll
     for (int j = 0; j < D; ++j) ids[j] = ids_next[j];
   }
-  leave_rows<NB, HD, E>(args, st, sm_stage + head_in * waves * 16 * (HD + 4), waves, mine, direct,
+  leave_rows<NB, HD, E>(own_args(), st, sm_stage + head_in * waves * 16 * (HD + 4), waves, mine, direct,
                         map, row0, n_rows, is_head);
+  if (!crosses || at >= end) return;  // uniform over the workgroup
+  }
 }
 
 // GROUPS: the first shared_wgs workgroups serve the groups, the others sequences.
@@ -601,7 +707,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1)))
 void sqa_part_kernel(PartArgs args) {
   __shared__ float sm_stage[4 * 16 * (HD + 4)];
   const bool shared = GROUPS && (int)blockIdx.x < args.shared_wgs;
-  part_share<NB, D, HD, 4, E, KV>(args, sm_stage, GROUPS && !shared ? blockIdx.x - args.shared_wgs
+  part_share<NB, D, HD, 4, E, KV>(sm_stage, GROUPS && !shared ? blockIdx.x - args.shared_wgs
                                                                  : blockIdx.x, shared);
 }
 
@@ -641,9 +747,10 @@ void launch_part(const PartArgs& a, int rows, dim3 grid, hipStream_t stream) {
     launch_part_as<E, PartNative, GROUPS>(a, rows, grid, stream);
 }
 
-// Workgroups that the sequences' own splits take.
+// Workgroups that the sequences' own pages take.
 inline long long own_workgroups(const PartArgs& a) {
-  return (long long)a.p.batch * a.splits * ((a.p.hkv + a.wg_heads - 1) / a.wg_heads);
+  const long long shares = a.splits > 0 ? (long long)a.p.batch * a.splits : a.own_items;
+  return shares * ((a.p.hkv + a.wg_heads - 1) / a.wg_heads);
 }
 
 }  // namespace

@@ -137,8 +137,10 @@ struct TileShare {
   const int tiles = (n_pages + kTilePages - 1) / kTilePages;
   const int row0 = __builtin_amdgcn_readfirstlane(it.block) * (32 * W) + wave * 32;
   const int n_rows = __builtin_amdgcn_readfirstlane(it.group.count) * a.rows;
-  const RowMap map{__builtin_amdgcn_readfirstlane(it.group.first), kvh,
-                   args.splits + __builtin_amdgcn_readfirstlane(it.split)};
+  const int first = __builtin_amdgcn_readfirstlane(it.group.first);
+  const RowMap map{first, kvh,
+                   args.shared_at + (((long long)__builtin_amdgcn_readfirstlane(it.split) * a.batch +
+                                      first) * a.hkv + kvh) * a.rows};
 
   // This wave's page of a tile, from memory to registers.
   const int shift = a.page_shift, sub_mask = (1 << shift) - 1;
@@ -439,15 +441,6 @@ struct OwnCache<HD, StoreCodesFp8> { using Type = PartCodesFp8<HD>; };
 template <int HD>
 struct OwnCache<HD, StoreCodesInt8> { using Type = PartCodesInt8<HD>; };
 
-// The kernel's arguments, where the compiler cannot know that they were asked for before:
-// each of two branches then loads its own, and neither keeps the other's in registers.
-__device__ __forceinline__ const PartArgs& own_args() {
-  auto* p = (const __attribute__((address_space(4))) PartArgs*)
-      __builtin_amdgcn_kernarg_segment_ptr();
-  asm volatile("" : "+s"(p));
-  return *(const PartArgs*)p;
-}
-
 // One launch for both: the first shared_wgs workgroups serve the groups, the others what
 // follows in every sequence (NB blocks of 16 rows). The one waits for the matrix cores, the
 // other for memory.
@@ -462,7 +455,7 @@ void sqa_tiles_kernel(PartArgs args) {
     Share::run(own_args(), lds, lds_scale, blockIdx.x);
   else
     part_share<NB, (NB > 2 || W > 4 ? 2 : 4) * 128 / HD, HD, W, E, typename OwnCache<HD, KV>::Type>(
-        own_args(), (float*)lds, blockIdx.x - args.shared_wgs, false);
+        (float*)lds, blockIdx.x - args.shared_wgs, false);
 }
 
 // Eight waves have 256 registers each, too few for 64 rows of a sequence beside the page ring.

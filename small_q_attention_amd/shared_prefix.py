@@ -24,7 +24,7 @@ from .windowed import check_call, take_workspace
 
 class SharedPrefixPlan:
     """What :func:`plan_shared_prefix` returns: ``shape`` (batch, q_len, query heads, kv
-    heads, head_dim, page_size), ``groups`` as given, and those on ``device``."""
+    heads, head_dim, page_size), ``groups`` as given, and their table on ``device``."""
 
     def __init__(self, shape, groups, device, table):
         self.shape, self.groups, self.device, self.table = shape, groups, device, table
@@ -71,8 +71,10 @@ def plan_shared_prefix(groups, batch: int, q_len: int, num_query_heads: int, num
         raise ValueError("the plan's device must be a GPU")
     if device.index is None:
         device = torch.device("cuda", torch.cuda.current_device())
-    table = torch.tensor(groups or [(0, 0, 0)], dtype=torch.int32).to(device)
-    return SharedPrefixPlan(shape, tuple(groups), device, table)
+    groups = tuple(groups)
+    most = max([pages for *_, pages in groups] + [1])
+    _, _, table = _lib.plan_shared_prefix(device.index, groups, shape, 0, 0, most)
+    return SharedPrefixPlan(shape, groups, device, torch.tensor(table, dtype=torch.int32).to(device))
 
 
 def _check(query, key_cache, value_cache, key_scale, value_scale, block_tables, seq_lens, words,
@@ -92,7 +94,7 @@ def _check(query, key_cache, value_cache, key_scale, value_scale, block_tables, 
 
 def _plan_call(query, key_cache, key_scale, block_tables, words, groups, max_seq_len):
     b, q_len, hq, d = query.shape
-    plan, need = _lib.plan_shared_prefix(
+    plan, need, _ = _lib.plan_shared_prefix(
         query.device.index, groups, (b, q_len, hq, key_cache.shape[2], d, key_cache.shape[1]),
         _lib.dtype_code(key_cache.dtype), max_seq_len, block_tables.shape[1])
     return plan, need, _lib.part_fields(query, key_cache, key_scale, block_tables, words)

@@ -72,8 +72,9 @@ def _plan(query, key_cache, key_scale, block_tables, words, window, sink, max_se
     b, q_len, hq, d = query.shape
     page, hkv = key_cache.shape[1], key_cache.shape[2]
     cut = _lib.plan_windowed(query.device.index, b, q_len, hq, hkv, d, window, sink, max_seq_len,
-                             block_tables.shape[1] * (page // 16))
-    return (cut, _lib.workspace_bytes(b, q_len, hq, hkv, d, cut[0], 1),
+                             block_tables.shape[1] * (page // 16),
+                             _lib.dtype_code(key_cache.dtype))
+    return (cut, _lib.workspace_bytes(b, q_len, hq, hkv, d, cut[0], cut[1]),
             _lib.part_fields(query, key_cache, key_scale, block_tables, words))
 
 

@@ -76,7 +76,7 @@ struct OwnCut {
 // average.
 template <typename Try>
 void own_cuts(const Model& m, int waves, long long most, double mean, bool may_cross, Try&& attempt) {
-  constexpr double kStart = 5, kPiece = 4;
+  const double start_us = 5, piece_us = 3 + m.rows / 8.0;
   for (int heads = 4; heads >= 1; heads /= 2) {
     if (heads / 2 >= m.num_kv_heads) continue;  // a smaller workgroup holds them all
     const long long head_groups = ceil_div(m.num_kv_heads, heads);
@@ -85,7 +85,7 @@ void own_cuts(const Model& m, int waves, long long most, double mean, bool may_c
          n += std::max(1, n / 8)) {
       const long long wgs = m.batch * n * head_groups;
       const long long pages = ceil_div(ceil_div(most, n), share);
-      attempt(OwnCut{n, 0, heads, (double)wgs, kStart + pages * m.page(wgs, heads, waves),
+      attempt(OwnCut{n, 0, heads, (double)wgs, start_us + pages * m.page(wgs, heads, waves),
                      n > 1 ? (double)m.batch * n : 0.0});
     }
     if (m.batch == 1 || !may_cross) continue;
@@ -95,7 +95,7 @@ void own_cuts(const Model& m, int waves, long long most, double mean, bool may_c
       if (n > 1 && total / n < sqa::kMinSplitPages) continue;
       const double pages = std::max(std::ceil(total / n / share), 1.0);
       attempt(OwnCut{0, (int)n, heads, (double)(n * head_groups),
-                     kStart + kPiece * (1 + (double)m.batch / n) +
+                     start_us + piece_us * (1 + (double)m.batch / n) +
                          pages * m.page(n * head_groups, heads, waves),
                      (double)(n + m.batch)});
     }
@@ -105,15 +105,12 @@ void own_cuts(const Model& m, int waves, long long most, double mean, bool may_c
 // When `first` workgroups of time t1, then n of time t2, have run on the device, each unit
 // taking the next as it gets free.
 double finish(int cus, double first, double t1, double n, double t2) {
-  if (first + n > 2 * cus) {  // many: they end one by one
-    const double each = (first * t1 + n * t2) / (first + n);
-    return (first * t1 + n * t2) / cus + each / 2;
-  }
   const double whole = std::floor(first / cus), rest = first - whole * cus, free = cus - rest;
   const double base = whole * t1;
   const double beside = rest > 0 ? std::floor(t1 / t2) * free : 0;  // while the last of those run
   if (n <= beside) return base + std::max(t1, std::ceil(n / free) * t2);
-  return base + (rest > 0 ? t1 : 0) + std::ceil((n - beside) / cus) * t2;
+  const double left = n - beside, rounds = left / cus;  // many end one by one
+  return base + (rest > 0 ? t1 : 0) + t2 * (rounds > 2 ? rounds + 0.5 : std::ceil(rounds));
 }
 
 // The cut of sequences without a group.
@@ -301,13 +298,13 @@ struct SharedCut {
 
 // The cut of a batch with groups. The groups' workgroups begin first. Where a wave holds a
 // block's rows they take their pages like the sequences'; tiles, bound by the matrix cores,
-// 0.56 us for a page of head dim 128 and 256 rows, 0.35 for 128 rows.
+// 0.56 us for a page of head dim 128 and 256 rows, 0.28 for 128 rows, and 12 besides.
 template <typename Groups>
 SharedCut shared_cut(const Model& m, int block_rows, int num_groups, const Groups& group,
                      long long own_most, double own_mean, bool crosses) {
   const bool tiles = block_rows > 64;
   const int waves = block_rows == 256 ? 8 : 4;
-  const double tile_page = (block_rows == 256 ? 0.56 : 0.35) * m.head_dim / 128;
+  const double tile_page = (block_rows == 256 ? 0.56 : 0.28) * m.head_dim / 128;
   long long longest = 1;
   for (int g = 0; g < num_groups; ++g) longest = std::max(longest, group(g).pages);
   struct Option {
@@ -338,7 +335,7 @@ SharedCut shared_cut(const Model& m, int block_rows, int num_groups, const Group
     for (int i = 0; i < n_options; ++i) {
       const Option& o = options[i];
       const double n1 = o.items * (tiles ? m.num_kv_heads : head_groups);
-      const double t1 = tiles ? 10 + o.size * tile_page
+      const double t1 = tiles ? 12 + o.size * tile_page
                               : 6 + ceil_div(o.size, waves / c.heads) *
                                         m.page((long long)(n1 + c.workgroups), c.heads, waves);
       const double cost = finish(m.cus, n1, t1, c.workgroups, c.time) + m.join(slots + o.slots);

@@ -54,13 +54,13 @@ struct Model {
   // 128 sequences of 34 to 258 pages), less where the heads read together make short runs.
   double page(long long n, int heads, int waves) const {
     const int run = std::min(heads, num_kv_heads) * head_dim * kv_bytes;
-    const double worse = run >= 1024 ? 1.0 : run >= 512 ? 1.05 : run >= 256 ? 1.15 : 1.35;
+    const double worse = run >= 1024 ? 1.0 : run >= 512 ? 1.08 : run >= 256 ? 1.2 : 1.4;
     const double bytes = 32.0 * head_dim * kv_bytes * waves * worse;
     return std::max({0.55, bytes * std::min<long long>(n, cus) / 6.6e6, bytes / 34e3});
   }
   // Partial rows written and read again, and the kernel that joins them.
   double join(double slots) const {
-    return 4 + slots * num_kv_heads * rows * head_dim * 8 / 4e6;
+    return 4 + slots * num_kv_heads * rows * head_dim * 8 / 3e6;
   }
 };
 

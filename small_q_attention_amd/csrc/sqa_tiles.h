@@ -119,10 +119,15 @@ struct TileShare {
   static constexpr int MB = HD / 32;  // blocks of 32 output dims
   static constexpr int kStageRow = HD + 4;
   static constexpr int kStage = W * 32 * kStageRow * 4;
-  static constexpr int kLds = 4 * T::kBytes > kStage ? 4 * T::kBytes : kStage;
+  // Tiles in LDS. With three, a wave that has a tile's first half behind it may bring the next
+  // one but one over what no wave can still be reading: one barrier a tile. Two (where three
+  // do not fit, or would keep a second workgroup away) take one more.
+  static constexpr int kBuffers = W == 8 ? 3 : 2;
+  static constexpr int kBuffer = 2 * T::kBytes;  // K, then V
+  static constexpr int kLds = kBuffers * kBuffer > kStage ? kBuffers * kBuffer : kStage;
 
   static __device__ __forceinline__ void run(const PartArgs& args, char* lds,
-                                             float (&lds_scale)[2][2][kTilePages], int block) {
+                                             float (&lds_scale)[3][2][kTilePages], int block) {
   const PartialArgs& a = args.p;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;
@@ -174,7 +179,7 @@ struct TileShare {
                                   (size_t)kvh * args.scales.head_stride);
   };
   auto put = [&](int buffer) {
-    char* to = lds + buffer * 2 * T::kBytes;
+    char* to = lds + buffer * kBuffer;
     constexpr int N = Loads::kChunks;
 #pragma unroll
     for (int i = 0; i < Loads::kLoads; ++i) {
@@ -233,7 +238,7 @@ struct TileShare {
     float mul[2], add[2], inv[2];
     bool loud[2];
   };
-  auto pages_of = [&](int t, int kb) {
+  auto pages_of = [&](int t, int buffer, int kb) {
     Pages x;
     const int left = n_pages - t * kTilePages - 2 * kb;  // pages from these two on
 #pragma unroll
@@ -244,8 +249,8 @@ struct TileShare {
         auto uniform = [](float y) {
           return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, y)));
         };
-        const float vs = uniform(lds_scale[t & 1][1][2 * kb + pg]);
-        x.mul[pg] = c * uniform(lds_scale[t & 1][0][2 * kb + pg]);
+        const float vs = uniform(lds_scale[buffer][1][2 * kb + pg]);
+        x.mul[pg] = c * uniform(lds_scale[buffer][0][2 * kb + pg]);
         x.loud[pg] = !(vs < 0x1p-64f);
         x.add[pg] = x.loud[pg] ? __builtin_amdgcn_logf(vs) : -64.f;
         x.inv[pg] = x.loud[pg] ? __builtin_amdgcn_rcpf(vs) : 0x1p64f;
@@ -254,16 +259,14 @@ struct TileShare {
     }
     return x;
   };
-  auto read_k = [&](int buffer, int kb, int ks) {
-    return *(const u4*)(lds + buffer * 2 * T::kBytes + kb * 32 * T::kRow + k_at[ks]);
-  };
+  auto read_k = [&](int kb, int ks) { return *(const u4*)(lds + kb * 32 * T::kRow + k_at[ks]); };
   // Dims 32 mb .. + 31 of 16 keys, transposed.
-  auto read_v = [&](int buffer, int kb, int i) {
+  auto read_v = [&](int kb, int i) {
     const int st = i / MB, mb = i % MB;
     u4 v;
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
-      const int at = buffer * 2 * T::kBytes + v_at[mb][half] + (32 * kb + 16 * st) * T::kRow;
+      const int at = v_at[mb][half] + (32 * kb + 16 * st) * T::kRow;
       const u2 x = __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
                                               (__attribute__((address_space(3))) s4v*)(lds + at)));
       v[2 * half] = x[0];
@@ -298,20 +301,20 @@ struct TileShare {
                    : max3_raw(x, s[2 * i], s[2 * i + 1]);
   };
   // 32 keys a step: P = 2^(s - m) of the scores `now`, added up into l, and their product with
-  // V (`v_buffer`, `v_kb`), while the scores `next` of other keys (`k_buffer`, `k_kb`) come
-  // about. The matrix cores and the vector units run beside each other where a wave gives
+  // V (half v_kb of the tile at v_at), while the scores `next` of other keys (half k_kb of the
+  // tile at k_at) come about. The matrix cores and the vector units run beside each other where a wave gives
   // both something to do, so the next scores' products stand among this step's
   // exponentials, the maxima of the next among the products with V, and reads from LDS
   // kAhead pieces before their use; the compiler, left alone, puts one after the other.
   constexpr int kAhead = 3;
-  auto step = [&](const f16v& now, const Pages& pages, int v_buffer, int v_kb, f16v& next,
-                  const Pages& next_pages, int k_buffer, int k_kb) {
+  auto step = [&](const f16v& now, const Pages& pages, int v_kb, f16v& next,
+                  const Pages& next_pages, int k_kb) {
     u4 k[KS], v[2 * MB], p[2];
     float off[2];
 #pragma unroll
     for (int pg = 0; pg < 2; ++pg) off[pg] = pages.add[pg] - (m == -INFINITY ? 0.f : m);
 #pragma unroll
-    for (int ks = 0; ks < kAhead; ++ks) k[ks] = read_k(k_buffer, k_kb, ks);
+    for (int ks = 0; ks < kAhead; ++ks) k[ks] = read_k(k_kb, ks);
     __builtin_amdgcn_sched_barrier(0);
     auto weigh = [&](int w) {  // pair w of 8: registers 2 w and 2 w + 1
       const int st = w / 4;
@@ -335,9 +338,9 @@ struct TileShare {
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
       if (ks + kAhead < KS)
-        k[ks + kAhead] = read_k(k_buffer, k_kb, ks + kAhead);
+        k[ks + kAhead] = read_k(k_kb, ks + kAhead);
       else
-        v[ks + kAhead - KS] = read_v(v_buffer, v_kb, ks + kAhead - KS);
+        v[ks + kAhead - KS] = read_v(v_kb, ks + kAhead - KS);
       score(k[ks], ks, next);
 #pragma unroll
       for (int w = 0; w < kEarly; ++w)
@@ -347,7 +350,7 @@ struct TileShare {
     float top[2];
 #pragma unroll
     for (int i = 0; i < 2 * MB; ++i) {
-      if (i + kAhead < 2 * MB) v[i + kAhead] = read_v(v_buffer, v_kb, i + kAhead);
+      if (i + kAhead < 2 * MB) v[i + kAhead] = read_v(v_kb, i + kAhead);
       acc[i % MB] = mma32<EV>(v[i], p[i / MB], acc[i % MB]);
       if (i < MB) {
 #pragma unroll
@@ -371,26 +374,37 @@ struct TileShare {
   id_next = id_of(2);
   f16v s0, s1;
   float top[2];
-  Pages pages = pages_of(0, 0);
+  Pages pages = pages_of(0, 0, 0);
 #pragma unroll
-  for (int ks = 0; ks < KS; ++ks) score(read_k(0, 0, ks), ks, s0);
+  for (int ks = 0; ks < KS; ++ks) score(read_k(0, ks), ks, s0);
 #pragma unroll
   for (int w = 0; w < 8; ++w) fold_top(s0, w, top);
   raise(top, pages);
+  int buffer = 0;
   for (int t = 0; t < tiles; ++t) {
-    const Pages second = pages_of(t, 1);
-    step(s0, pages, t & 1, 0, s1, second, t & 1, 1);
-    if (t + 1 < tiles) put((t + 1) & 1);
+    const int following = buffer == kBuffers - 1 ? 0 : buffer + 1;
+    const int onward = (following - buffer) * kBuffer;
+    const Pages second = pages_of(t, buffer, 1);
+    step(s0, pages, 0, s1, second, 1);
+    if (t + 1 < tiles) put(following);
     __syncthreads();
     if (t + 2 < tiles) {  // uniform
       fetch(t + 2, id_next);
       id_next = id_of(t + 3);
     }
     // Past the last tile the scores are of what the buffer holds, and nobody's.
-    pages = pages_of(t + 1, 0);
-    step(s1, second, t & 1, 1, s0, pages, (t + 1) & 1, 0);
-    __syncthreads();
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) k_at[ks] += onward;
+    pages = pages_of(t + 1, following, 0);
+    step(s1, second, 1, s0, pages, 0);
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+      for (int half = 0; half < 2; ++half) v_at[mb][half] += onward;
+    buffer = following;
+    if constexpr (kBuffers == 2) __syncthreads();
   }
+  __syncthreads();  // before the tiles' place is taken
 
   // Partial rows through LDS.
   float* stage = (float*)lds + wave * 32 * kStageRow;
@@ -450,7 +464,7 @@ void sqa_tiles_kernel(PartArgs args) {
   using Share = TileShare<HD, W, E, KV>;
   constexpr int kOwn = W * 16 * (HD + 4) * 4;
   __shared__ __attribute__((aligned(16))) char lds[Share::kLds > kOwn ? Share::kLds : kOwn];
-  __shared__ float lds_scale[2][2][kTilePages];  // of a tile's pages: buffer, K and V, page
+  __shared__ float lds_scale[3][2][kTilePages];  // of a tile's pages: buffer, K and V, page
   if ((int)blockIdx.x < args.shared_wgs)
     Share::run(own_args(), lds, lds_scale, blockIdx.x);
   else

@@ -88,8 +88,8 @@ class SharedPlan(ctypes.Structure):
 
     _fields_ = [("struct_size", _C.c_size_t)] + [(name, _C.c_int) for name in (
         "batch", "q_len", "num_query_heads", "num_kv_heads", "head_dim", "page_size", "num_groups",
-        "most_pages", "num_splits", "pages_per_split", "wg_heads", "block_rows", "shared_size", "shared_splits",
-        "num_items")]
+        "most_pages", "num_splits", "pages_per_split", "wg_heads", "block_rows", "shared_size",
+        "shared_splits", "num_items")]
 
 
 class AppendArgs(ctypes.Structure):
@@ -405,8 +405,8 @@ def _part_args(query, output, k_view, v_view, k_scale, v_scale, block_tables, se
 def launch_windowed(query, output, k_view, v_view, k_scale, v_scale, block_tables, seq_lens,
                     draft_mask, window: int, sink: int, scale: float, out_scale: float,
                     cut, workspace, stream_handle: int, fields=None):
-    """Call ``sqa_paged_attention_windowed``: ``cut`` from :func:`plan_windowed`, views and scales (or ``None``) as for
-    :func:`launch_scaled`, ``fields`` from :func:`part_fields`."""
+    """Call ``sqa_paged_attention_windowed``: ``cut`` from :func:`plan_windowed`, views and
+    scales (or ``None``) as for :func:`launch_scaled`, ``fields`` from :func:`part_fields`."""
     lib = _LIB if _LIB is not None else load()
     a, scales = _part_args(query, output, k_view, v_view, k_scale, v_scale, block_tables, seq_lens,
                            draft_mask, scale, out_scale, cut[0], cut[1], workspace, stream_handle,
@@ -441,7 +441,8 @@ def launch_shared_prefix(query, output, k_view, v_view, k_scale, v_scale, block_
     lib = _LIB if _LIB is not None else load()
     a, scales = _part_args(query, output, k_view, v_view, k_scale, v_scale, block_tables, seq_lens,
                            draft_mask, scale, out_scale, plan.num_splits, plan.pages_per_split,
-                           workspace, stream_handle, fields or part_fields(query, k_view, k_scale, block_tables, draft_mask))
+                           workspace, stream_handle,
+                           fields or part_fields(query, k_view, k_scale, block_tables, draft_mask))
     rc = lib.sqa_paged_attention_shared_prefix(a, scales, ctypes.byref(plan), table.data_ptr())
     if rc != SQA_OK:
         raise RuntimeError(f"sqa_paged_attention_shared_prefix failed: {last_error(lib)}")

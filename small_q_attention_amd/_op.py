@@ -141,7 +141,8 @@ def paged_attention_shared_prefix(query: torch.Tensor, key_cache: torch.Tensor,
 
     return scaled_cache.on_device(query.device, lambda: shared_prefix.run_shared_prefix(
         query, key_cache, value_cache, key_scale, value_scale, block_tables, seq_lens, draft_mask,
-        tuple(zip(groups[::3], groups[1::3], groups[2::3])), table, scale, out_scale, max_seq_len, None, None))
+        tuple(zip(groups[::3], groups[1::3], groups[2::3])), table, scale, out_scale, max_seq_len,
+        None, None))
 
 
 @paged_attention_shared_prefix.register_fake

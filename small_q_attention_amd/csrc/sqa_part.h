@@ -17,6 +17,11 @@ inline EvenSplits even_splits(long long pages, long long size) {
   return {(int)((pages + each - 1) / each), (int)each};
 }
 
+// What a workgroup pays to begin a sequence, in pages: where a batch's pages are cut from end
+// to end, every sequence counts so many more than it has (96 sequences of 16 to 128 pages,
+// q_len 4: 94 us in the kernel without, 84 with).
+constexpr int kSeamPages = 4;
+
 struct PartArgs {
   // Of PartialArgs the fields that name buffers, shapes, strides and scales. part_o, part_ml:
   // fp32 sums and (max in log2 units, sum) of the partial rows. A slot of kv head h and
@@ -38,7 +43,7 @@ struct PartArgs {
   // together, in blocks of block_rows (16, 32 or 64: one wave's; 128 or 256: a workgroup's)
   // and splits of at most shared_size 16-token pages; n_items blocks x splits in all.
   const int32_t* groups;
-  const int2* seq_groups;  // [B]: (index of the group, -1: none; its pages)
+  const int32_t* seq_groups;  // [B][2]: (index of the group, -1: none; its pages)
   int n_groups, n_items, block_rows, shared_size;
   int shared_splits;       // most splits of a group
   int shared_wgs;          // workgroups that serve the groups, the first of the grid

@@ -1,6 +1,6 @@
 // C ABI of attention over a window and over a shared prefix (declared in include/sqa.h):
-// validates arguments, plans, and launches the kernels of sqa_part.hip and sqa_shared.hip
-// on the caller's stream. Allocates nothing.
+// validates arguments, plans, and launches the kernels of sqa_part.hip, sqa_groups.hip and
+// sqa_tiles.h on the caller's stream. Allocates nothing.
 #include "sqa.h"
 #include "sqa_part.h"
 
@@ -68,14 +68,15 @@ struct Model {
 // (0) `items` equal items of the whole batch; `heads` kv heads to a workgroup.
 struct OwnCut {
   int splits, items, heads;
-  double workgroups, time;  // of one of them
-  double slots;             // partial slots that are written
+  double workgroups, longest, mean;  // times of one of them
+  double slots;                      // partial slots that are written
 };
 
 // Calls try(cut) for the cuts worth a look. Sequences have up to `most` pages, `mean` on
 // average.
 template <typename Try>
-void own_cuts(const Model& m, int waves, long long most, double mean, bool may_cross, Try&& attempt) {
+void own_cuts(const Model& m, int waves, long long most, double mean, bool may_cross,
+              Try&& attempt) {
   const double start_us = 5, piece_us = 3 + m.rows / 8.0;
   for (int heads = 4; heads >= 1; heads /= 2) {
     if (heads / 2 >= m.num_kv_heads) continue;  // a smaller workgroup holds them all
@@ -84,8 +85,11 @@ void own_cuts(const Model& m, int waves, long long most, double mean, bool may_c
     for (int n = 1; n <= 256 && (n == 1 || n * sqa::kMinSplitPages <= most);
          n += std::max(1, n / 8)) {
       const long long wgs = m.batch * n * head_groups;
-      const long long pages = ceil_div(ceil_div(most, n), share);
-      attempt(OwnCut{n, 0, heads, (double)wgs, start_us + pages * m.page(wgs, heads, waves),
+      const double pages = (double)ceil_div(ceil_div(most, n), share);
+      const double at_mean = std::max(std::ceil(mean / n / share), 1.0) * m.page(wgs, heads, waves);
+      // The longest, as others have ended, takes what a unit gives.
+      attempt(OwnCut{n, 0, heads, (double)wgs,
+                     start_us + std::max(pages * m.page(1, heads, waves), at_mean), 2 + at_mean,
                      n > 1 ? (double)m.batch * n : 0.0});
     }
     if (m.batch == 1 || !may_cross) continue;
@@ -94,23 +98,26 @@ void own_cuts(const Model& m, int waves, long long most, double mean, bool may_c
     for (long long n = all; n >= 1; n = n > 8 ? n * 7 / 8 : n - 1) {
       if (n > 1 && total / n < sqa::kMinSplitPages) continue;
       const double pages = std::max(std::ceil(total / n / share), 1.0);
-      attempt(OwnCut{0, (int)n, heads, (double)(n * head_groups),
-                     start_us + piece_us * (1 + (double)m.batch / n) +
-                         pages * m.page(n * head_groups, heads, waves),
+      const double time = start_us + piece_us * (1 + (double)m.batch / n) +
+                          pages * m.page(n * head_groups, heads, waves);
+      attempt(OwnCut{0, (int)n, heads, (double)(n * head_groups), time, time,
                      (double)(n + m.batch)});
     }
   }
 }
 
-// When `first` workgroups of time t1, then n of time t2, have run on the device, each unit
-// taking the next as it gets free.
-double finish(int cus, double first, double t1, double n, double t2) {
+// When `first` workgroups of time t1, then those of a cut, have run on the device, each unit
+// taking the next as it gets free (which in a long row of them begins beside the last).
+double finish(int cus, double first, double t1, const OwnCut& c) {
   const double whole = std::floor(first / cus), rest = first - whole * cus, free = cus - rest;
   const double base = whole * t1;
-  const double beside = rest > 0 ? std::floor(t1 / t2) * free : 0;  // while the last of those run
-  if (n <= beside) return base + std::max(t1, std::ceil(n / free) * t2);
-  const double left = n - beside, rounds = left / cus;  // many end one by one
-  return base + (rest > 0 ? t1 : 0) + t2 * (rounds > 2 ? rounds + 0.5 : std::ceil(rounds));
+  // While the last of those run:
+  const double beside = rest > 0 ? std::floor(t1 / c.longest) * free : 0;
+  if (c.workgroups <= beside)
+    return base + std::max(t1, std::ceil(c.workgroups / free) * c.longest);
+  const double rounds = (c.workgroups - beside) / cus;  // many end one by one
+  return base + (rest > 0 ? t1 : 0) +
+         (rounds > 2 ? rounds * c.mean + 0.5 * c.longest : std::ceil(rounds) * c.longest);
 }
 
 // The cut of sequences without a group.
@@ -118,7 +125,7 @@ OwnCut best_own(const Model& m, long long most, double mean, bool may_cross) {
   OwnCut best{};
   double best_cost = -1;
   own_cuts(m, 4, most, mean, may_cross, [&](const OwnCut& c) {
-    const double cost = finish(m.cus, 0, 1, c.workgroups, c.time) +
+    const double cost = finish(m.cus, 0, 1, c) +
                         (c.slots > 0 ? m.join(c.slots) : 0);
     if (best_cost < 0 || cost < best_cost * 0.995) {
       best = c;
@@ -128,9 +135,10 @@ OwnCut best_own(const Model& m, long long most, double mean, bool may_cross) {
   return best;
 }
 
-// Whether the pages of a batch can be numbered from end to end.
+// Whether the pages of a batch, with what every sequence counts besides, can be numbered from
+// end to end.
 bool may_cross(long long batch, long long kernel_pages) {
-  return batch * kernel_pages < (1LL << 27);
+  return batch * (kernel_pages + sqa::kSeamPages) < (1LL << 27);
 }
 
 // Pages that a window leaves of a sequence of up to `pages`: the first tokens', and those
@@ -338,7 +346,7 @@ SharedCut shared_cut(const Model& m, int block_rows, int num_groups, const Group
       const double t1 = tiles ? 12 + o.size * tile_page
                               : 6 + ceil_div(o.size, waves / c.heads) *
                                         m.page((long long)(n1 + c.workgroups), c.heads, waves);
-      const double cost = finish(m.cus, n1, t1, c.workgroups, c.time) + m.join(slots + o.slots);
+      const double cost = finish(m.cus, n1, t1, c) + m.join(slots + o.slots);
       if (best_cost < 0 || cost < best_cost * 0.995) {
         best = {c, o.size};
         best_cost = cost;
@@ -355,7 +363,7 @@ int check_plan(const sqa_shared_plan* p) {
                 p->struct_size, sizeof(sqa_shared_plan));
   if (p->batch <= 0 || p->q_len <= 0 || p->num_kv_heads <= 0 || p->num_query_heads <= 0 ||
       p->head_dim <= 0 || p->num_groups < 0 || p->num_items < 0 || p->num_splits <= 0 ||
-      p->shared_splits < 0 || p->shared_size <= 0 ||
+      p->shared_splits < 0 || p->shared_size <= 0 || (p->num_items > 0 && p->num_groups == 0) ||
       (p->pages_per_split == 0 && p->num_splits <= p->batch))
     return fail(SQA_ERR_INVALID, "not a plan of sqa_plan_shared_prefix");
   return SQA_OK;
@@ -384,7 +392,8 @@ extern "C" {
 int sqa_plan_windowed(int device, int batch, int q_len, int num_query_heads, int num_kv_heads,
                       int head_dim, int64_t window, int sink, int max_seq_len, int max_pages,
                       int kv_dtype, int* num_splits, int* pages_per_split, int* wg_heads) {
-  if (!num_splits || !pages_per_split || !wg_heads) return fail(SQA_ERR_INVALID, "null output pointer");
+  if (!num_splits || !pages_per_split || !wg_heads)
+    return fail(SQA_ERR_INVALID, "null output pointer");
   long long rows = 0;
   if (int rc = check_shape(batch, q_len, num_query_heads, num_kv_heads, head_dim, &rows)) return rc;
   if (max_pages <= 0) return fail(SQA_ERR_INVALID, "max_pages must be positive");
@@ -572,7 +581,7 @@ int sqa_paged_attention_shared_prefix(const sqa_attention_args* args,
         (!tiles && b < s.p.rows))
       return fail(SQA_ERR_INVALID, "not a plan of sqa_plan_shared_prefix");
     s.groups = table;
-    s.seq_groups = (const int2*)(table + 3 * plan->num_groups);
+    s.seq_groups = table + 3 * plan->num_groups;
     s.n_groups = plan->num_groups;
     s.n_items = plan->num_items;
     s.block_rows = b;

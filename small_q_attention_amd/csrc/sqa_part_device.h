@@ -77,10 +77,10 @@ __device__ __forceinline__ Span span_of(const PartArgs& a, int b, int len) {
     s.tail = max(s.tail, s.head);
   }
   if (a.n_groups > 0) {
-    const int2 g = a.seq_groups[b];
-    const int shared = min(max(g.y, 0), a.p.bt_stride) << a.p.page_shift;
-    if (g.x >= 0 && g.x < a.n_groups && shared > 0 && reaches(a, len, shared)) {
-      s.group = g.x;
+    const int group = a.seq_groups[2 * b];
+    const int shared = min(max(a.seq_groups[2 * b + 1], 0), a.p.bt_stride) << a.p.page_shift;
+    if (group >= 0 && group < a.n_groups && shared > 0 && reaches(a, len, shared)) {
+      s.group = group;
       s.shared = s.tail = shared;
     }
   }
@@ -100,12 +100,11 @@ __device__ __forceinline__ void own_splits(const PartArgs& a, int n, int* count,
 // then take the same time whatever the lengths (an extra workgroup on a compute unit waits
 // for the first: 128 sequences of 34 pages, 8 kv heads, 256 workgroups, 49 us; 130 of them,
 // one sequence to a workgroup, 77).
-// Every sequence counts kSeamPages more than it has, before its first one: about what a
-// workgroup pays to begin it (96 sequences of 16 to 128 pages: 94 -> 85 us).
-constexpr int kSeamPages = 4;
+// Every sequence counts kSeamPages more than it has, before its first one.
 struct OwnCut {
   int size, total;
-  int n, len;  // of the lane's sequence among the first 64
+  // The 64 sequences from k on, after `base` pages: the lane's, its pages and length.
+  int k, base, n, len;
 };
 __device__ __forceinline__ int own_pages(const PartArgs& a, int b, int* len) {
   if (b >= a.p.batch) return 0;
@@ -115,12 +114,15 @@ __device__ __forceinline__ int own_pages(const PartArgs& a, int b, int* len) {
 }
 __device__ __forceinline__ OwnCut own_cut(const PartArgs& a, bool writer) {
   const int lane = threadIdx.x & 63;
-  OwnCut c{0, 0, 0, 0};
+  OwnCut c{0, 0, 0, 0, 0, 0};
   c.n = own_pages(a, lane, &c.len);
-  for (int k = 0; k < a.p.batch; k += 64) {
+  int sum = c.n;  // of every 64th sequence from the lane's on
+#pragma unroll 4
+  for (int k = 64; k < a.p.batch; k += 64) {
     int len;
-    c.total += wave_sum_int(k == 0 ? c.n : own_pages(a, k + lane, &len));
+    sum += own_pages(a, k + lane, &len);
   }
+  c.total = wave_sum_int(sum);
   c.size = max(ceil_over(c.total, a.own_items), kMinSplitPages);
   if (!writer) return c;
   int base = 0;  // the join's table
@@ -137,27 +139,26 @@ __device__ __forceinline__ OwnCut own_cut(const PartArgs& a, bool writer) {
   return c;
 }
 // The sequence with page `at` of the batch, the first of its pages (past the seam) and how
-// many it has (b < 0: none).
+// many it has (b < 0: none). For pages in ascending order.
 struct OwnPiece {
   int b, len, start, n;
 };
-__device__ __forceinline__ OwnPiece own_piece(const PartArgs& a, const OwnCut& c, int at) {
+__device__ __forceinline__ OwnPiece own_piece(const PartArgs& a, OwnCut& c, int at) {
   const int lane = threadIdx.x & 63;
-  int base = 0;
-  for (int k = 0; k < a.p.batch; k += 64) {
-    int len = c.len;
-    const int n = k == 0 ? c.n : own_pages(a, k + lane, &len);
-    const int incl = wave_inclusive_scan_int(n);
-    const unsigned long long hit = __ballot(n > 0 && at < base + incl);
+  for (;;) {
+    const int incl = wave_inclusive_scan_int(c.n);
+    const unsigned long long hit = __ballot(c.n > 0 && at < c.base + incl);
     if (hit) {
       const int src = __builtin_ctzll(hit);
-      return {k + src, __builtin_amdgcn_readlane(len, src),
-              base + __builtin_amdgcn_readlane(incl - n, src) + kSeamPages,
-              __builtin_amdgcn_readlane(n, src) - kSeamPages};
+      return {c.k + src, __builtin_amdgcn_readlane(c.len, src),
+              c.base + __builtin_amdgcn_readlane(incl - c.n, src) + kSeamPages,
+              __builtin_amdgcn_readlane(c.n, src) - kSeamPages};
     }
-    base += __builtin_amdgcn_readlane(incl, 63);
+    c.base += __builtin_amdgcn_readlane(incl, 63);
+    c.k += 64;
+    if (c.k >= a.p.batch) return {-1, 0, 0, 0};
+    c.n = own_pages(a, c.k + lane, &c.len);
   }
-  return {-1, 0, 0, 0};
 }
 
 // One item of the groups: a block of a group's rows over a split of its pages.
@@ -695,8 +696,8 @@ __device__ __forceinline__ void part_share(float* sm_stage, int block, bool shar
 #pragma unroll
     for (int j = 0; j < D; ++j) ids[j] = ids_next[j];
   }
-  leave_rows<NB, HD, E>(own_args(), st, sm_stage + head_in * waves * 16 * (HD + 4), waves, mine, direct,
-                        map, row0, n_rows, is_head);
+  leave_rows<NB, HD, E>(own_args(), st, sm_stage + head_in * waves * 16 * (HD + 4), waves, mine,
+                        direct, map, row0, n_rows, is_head);
   if (!crosses || at >= end) return;  // uniform over the workgroup
   }
 }

@@ -103,12 +103,20 @@ struct StoreCodesInt8 {
 
 // One workgroup: a block of 32 W of a group's rows of one kv head, 32 to a wave, over one
 // split of the shared pages, 64 keys at a time. Each wave brings a part of a tile's four
-// pages to LDS, two buffers in turn; all waves read all of it.
+// pages to LDS, two or three buffers in turn; all waves read all of it.
 //
 // S^T = K Q^T leaves a lane with half of the keys of its row, so that maxima and sums stay
 // in the lane but for one exchange between two lanes; O^T = V^T P^T takes P from those
 // registers as they are: the product's k order is the order the registers hold the keys in,
 // and V comes transposed from LDS in the same order.
+//
+// The products bound it: 512 rows over 32K tokens, 8 kv heads, head dim 128, fp16, take 285 us
+// in these workgroups, 965 TFLOP/s, where a large product of the library's reaches 1160. The
+// device lowers its clock under them (the same call on zeros: a quarter less time), so what is
+// left to gain is in instructions saved, not in waits. 32 rows to a wave: with 64, and one wave
+// to a SIMD, half the reads from LDS and the same time (338 and 340 us). Eight waves to a
+// block of 256 rows rather than two workgroups of four beside each other: every tile is
+// brought for twice the rows (96 sequences over two prefixes, bf16: 204 and 212 us).
 template <int HD, int W, typename E, typename KV>
 struct TileShare {
   using EV = std::conditional_t<KV::kScaled, ElemF16, E>;  // type of P and V
@@ -247,7 +255,8 @@ struct TileShare {
       x.add[pg] = 0.f;
       if constexpr (KV::kScaled) {
         auto uniform = [](float y) {
-          return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, y)));
+          return __builtin_bit_cast(
+              float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, y)));
         };
         const float vs = uniform(lds_scale[buffer][1][2 * kb + pg]);
         x.mul[pg] = c * uniform(lds_scale[buffer][0][2 * kb + pg]);
@@ -255,7 +264,13 @@ struct TileShare {
         x.add[pg] = x.loud[pg] ? __builtin_amdgcn_logf(vs) : -64.f;
         x.inv[pg] = x.loud[pg] ? __builtin_amdgcn_rcpf(vs) : 0x1p64f;
       }
-      if (pg >= left) x.add[pg] = -INFINITY;
+      if (pg >= left) {  // zeros in LDS, and some page's scales
+        x.add[pg] = -INFINITY;
+        if constexpr (KV::kScaled) {
+          x.mul[pg] = x.inv[pg] = 0.f;
+          x.loud[pg] = false;
+        }
+      }
     }
     return x;
   };
@@ -302,10 +317,14 @@ struct TileShare {
   };
   // 32 keys a step: P = 2^(s - m) of the scores `now`, added up into l, and their product with
   // V (half v_kb of the tile at v_at), while the scores `next` of other keys (half k_kb of the
-  // tile at k_at) come about. The matrix cores and the vector units run beside each other where a wave gives
-  // both something to do, so the next scores' products stand among this step's
-  // exponentials, the maxima of the next among the products with V, and reads from LDS
-  // kAhead pieces before their use; the compiler, left alone, puts one after the other.
+  // tile at k_at) come about. The matrix cores and the vector units run beside each other where
+  // a wave gives both something to do, so the next scores' products stand among this step's
+  // exponentials, the maxima of the next among the products with V, and reads from LDS kAhead
+  // pieces before their use; the compiler, left alone, puts one after the other (64 sequences
+  // over 32K tokens, q_len 8: 345 us so, 338 in this order).
+  // P is rounded once to the type of the products, in bf16 too (2^-9 of a probability, as the
+  // output's own rounding; sums stay in 32 bits): a second product for what is rounded off, as
+  // pages in waves have it, would cost half of the products again, and these bound the kernel.
   constexpr int kAhead = 3;
   auto step = [&](const f16v& now, const Pages& pages, int v_kb, f16v& next,
                   const Pages& next_pages, int k_kb) {

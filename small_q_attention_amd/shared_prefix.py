@@ -19,7 +19,7 @@ from . import _lib
 from . import scaled_cache as sc
 from .cuda import HEAD_DIMS, SUPPORTED_PAGE_SIZES, _tracing
 from .masks import as_words
-from .windowed import check_call, take_workspace
+from .windowed import check_apart, check_call, take_workspace
 
 
 class SharedPrefixPlan:
@@ -74,7 +74,8 @@ def plan_shared_prefix(groups, batch: int, q_len: int, num_query_heads: int, num
     groups = tuple(groups)
     most = max([pages for *_, pages in groups] + [1])
     _, _, table = _lib.plan_shared_prefix(device.index, groups, shape, 0, 0, most)
-    return SharedPrefixPlan(shape, groups, device, torch.tensor(table, dtype=torch.int32).to(device))
+    table = torch.tensor(table, dtype=torch.int32).to(device)
+    return SharedPrefixPlan(shape, groups, device, table)
 
 
 def _check(query, key_cache, value_cache, key_scale, value_scale, block_tables, seq_lens, words,
@@ -137,10 +138,13 @@ def paged_attention_shared_prefix(query, key_cache, value_cache, block_tables, s
 
     ``max_seq_len`` > 0 only sizes the call (0: the block table's width), and with it the
     last bits of a result may change; ``scale`` is the softmax scale (``None``: ``D **
-    -0.5``), ``out_scale`` multiplies the output. In bf16 the shared pages' probabilities are
-    rounded as the plan's kernel for its group sizes does. ``workspace_buffer``: a caller's
-    buffer for the partial rows; ``None`` takes one kept per host thread and stream, or, under
-    graph capture, one of the graph's own. Returns ``out`` (``[B, Q, Hq, D]``).
+    -0.5``), ``out_scale`` multiplies the output. In bf16, without block scales, the
+    probabilities of shared pages are rounded once to bf16 (2^-9 of each) for groups of more
+    than 64 rows of a kv head (32 at head_dim 256), and kept to 2^-17 otherwise.
+    ``workspace_buffer``: a caller's buffer for the partial rows; ``None`` takes one kept per
+    host thread and stream, or, under graph capture, one of the graph's own. A graph reads
+    the plan's table: the plan is kept for as long as the graph is replayed. Returns ``out``
+    (``[B, Q, Hq, D]``).
     """
     if query.dim() != 4:
         raise ValueError("query must be a contiguous [B, Q, Hq, D] tensor")
@@ -170,6 +174,7 @@ def paged_attention_shared_prefix(query, key_cache, value_cache, block_tables, s
                                                    key_scale, block_tables, words, plan.groups,
                                                    max_seq_len))
     sc.check_aligned(16, query, key_cache, value_cache)
+    check_apart(query, out)
     return sc.on_device(query.device, run_shared_prefix, query, key_cache, value_cache, key_scale,
                         value_scale, block_tables, seq_lens, words, plan.groups, plan.table, scale,
                         float(out_scale), max_seq_len, out, workspace_buffer, known)

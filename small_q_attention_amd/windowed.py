@@ -56,6 +56,12 @@ def check_call(query, key_cache, value_cache, key_scale, value_scale, block_tabl
         raise ValueError("out must be a contiguous tensor shaped and typed like query")
 
 
+def check_apart(query, out):
+    """ValueError for a result in the queries' place: they are read until the end."""
+    if out is not None and out.data_ptr() == query.data_ptr():
+        raise ValueError("out must not be query")
+
+
 def take_workspace(workspace_buffer, need, query, stream):
     """The caller's buffer, checked, or one kept for the stream (``None`` where none is
     needed)."""
@@ -149,6 +155,7 @@ def paged_attention_windowed(query, key_cache, value_cache, block_tables, seq_le
         known = _KNOWN.keep(seen, sc.on_device(query.device, _plan, query, key_cache, key_scale,
                                                block_tables, words, window, sink, max_seq_len))
     sc.check_aligned(16, query, key_cache, value_cache)
+    check_apart(query, out)
     return sc.on_device(query.device, run_windowed, query, key_cache, value_cache, key_scale,
                         value_scale, block_tables, seq_lens, words, window, sink, scale,
                         float(out_scale), max_seq_len, out, workspace_buffer, known)

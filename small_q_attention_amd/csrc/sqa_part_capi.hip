@@ -301,18 +301,25 @@ struct SharedGroup {
 
 struct SharedCut {
   OwnCut own;
+  int block_rows;
   long long size;  // most pages of a group's split
+  double cost;
 };
 
-// The cut of a batch with groups. The groups' workgroups begin first. Where a wave holds a
-// block's rows they take their pages like the sequences'; tiles, bound by the matrix cores,
-// 0.56 us for a page of head dim 128 and 256 rows, 0.28 for 128 rows, and 12 besides.
+// The cut of a batch with groups, whose workgroups begin first, in blocks of block_rows. Where
+// a wave holds a block's rows they take their pages like the sequences'; tiles are bound by the
+// matrix cores and by what the clock is then: a page of head dim 128 takes 0.40 us for 256
+// rows on a few units and 0.54 on all, 0.34 for 128 rows, where a second workgroup on a unit
+// takes as much again, and one of head dim 256 0.56; all of them 12 besides.
 template <typename Groups>
 SharedCut shared_cut(const Model& m, int block_rows, int num_groups, const Groups& group,
                      long long own_most, double own_mean, bool crosses) {
   const bool tiles = block_rows > 64;
   const int waves = block_rows == 256 ? 8 : 4;
-  const double tile_page = (block_rows == 256 ? 0.56 : 0.28) * m.head_dim / 128;
+  const auto tile_page = [&](double n) {
+    if (m.head_dim == 256) return 0.56;
+    return (block_rows == 256 ? 0.40 + 0.14 * std::min(n / m.cus, 1.0) : 0.34) * m.head_dim / 128;
+  };
   long long longest = 1;
   for (int g = 0; g < num_groups; ++g) longest = std::max(longest, group(g).pages);
   struct Option {
@@ -334,7 +341,6 @@ SharedCut shared_cut(const Model& m, int block_rows, int num_groups, const Group
     if (n_options == 64) break;
   }
   SharedCut best{};
-  double best_cost = -1;
   own_cuts(m, waves, own_most, own_mean, crosses, [&](const OwnCut& c) {
     const double head_groups = (double)ceil_div(m.num_kv_heads, c.heads);
     // Every sequence that shares leaves partial rows.
@@ -343,14 +349,11 @@ SharedCut shared_cut(const Model& m, int block_rows, int num_groups, const Group
     for (int i = 0; i < n_options; ++i) {
       const Option& o = options[i];
       const double n1 = o.items * (tiles ? m.num_kv_heads : head_groups);
-      const double t1 = tiles ? 12 + o.size * tile_page
+      const double t1 = tiles ? 12 + o.size * tile_page(n1)
                               : 6 + ceil_div(o.size, waves / c.heads) *
                                         m.page((long long)(n1 + c.workgroups), c.heads, waves);
       const double cost = finish(m.cus, n1, t1, c) + m.join(slots + o.slots);
-      if (best_cost < 0 || cost < best_cost * 0.995) {
-        best = {c, o.size};
-        best_cost = cost;
-      }
+      if (best.cost == 0 || cost < best.cost * 0.995) best = {c, block_rows, o.size, cost};
     }
   });
   return best;
@@ -511,8 +514,12 @@ int sqa_plan_shared_prefix(int device, int batch, int q_len, int num_query_heads
   } else {
     out.num_groups = num_groups;
     out.block_rows = rows_of_block(most_rows, rows, head_dim);
-    const SharedCut cut = shared_cut(m, out.block_rows, num_groups, group, own, 0.65 * own,
-                                     crosses);
+    SharedCut cut = shared_cut(m, out.block_rows, num_groups, group, own, 0.65 * own, crosses);
+    if (out.block_rows == 256) {  // less of it empty where groups are small
+      const SharedCut halves = shared_cut(m, 128, num_groups, group, own, 0.65 * own, crosses);
+      if (halves.cost < 0.97 * cut.cost) cut = halves;
+    }
+    out.block_rows = cut.block_rows;
     long long items = 0;
     for (int i = 0; i < num_groups; ++i) {
       const SharedGroup g = group(i);

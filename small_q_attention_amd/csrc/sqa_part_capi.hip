@@ -51,12 +51,14 @@ struct Model {
 
   // A page (16 tokens of one head's K and V) for each wave of a workgroup, `n` of them at
   // work: the device's 6.6 TB/s shared out, at most 34 GB/s to a unit (both measured, 16 to
-  // 128 sequences of 34 to 258 pages), less where the heads read together make short runs.
+  // 128 sequences of 34 to 258 pages), less where the heads read together make short runs; no
+  // less than a wave's chain over a page takes, codes widened or not.
   double page(long long n, int heads, int waves) const {
     const int run = std::min(heads, num_kv_heads) * head_dim * kv_bytes;
-    const double worse = run >= 1024 ? 1.0 : run >= 512 ? 1.08 : run >= 256 ? 1.2 : 1.4;
+    const double worse = run >= 1024 ? 1.0 : run >= 512 ? 1.04 : run >= 256 ? 1.2 : 1.4;
     const double bytes = 32.0 * head_dim * kv_bytes * waves * worse;
-    return std::max({0.55, bytes * std::min<long long>(n, cus) / 6.6e6, bytes / 34e3});
+    return std::max({kv_bytes == 1 ? 0.58 : 0.55, bytes * std::min<long long>(n, cus) / 6.6e6,
+                     bytes / 34e3});
   }
   // Partial rows written and read again, and the kernel that joins them.
   double join(double slots) const {

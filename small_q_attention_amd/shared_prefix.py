@@ -2,6 +2,10 @@
 from one prompt, requests under one system prompt or over one document. The shared pages are
 read once for each group of sequences and not once for each sequence.
 
+That takes a few microseconds more than attention over the whole rows of few and short
+sequences, and pays from about 32K tokens saved on, (sequences - 1) * shared tokens: the same
+result comes from ``cuda.paged_mtp_attention`` or a window over everything.
+
 :func:`plan_shared_prefix` says which sequences share how many pages, once for as long as
 that stays; :func:`paged_attention_shared_prefix` is the attention call, with the result of
 attention over the whole block tables. It runs on the current stream of the query's device,

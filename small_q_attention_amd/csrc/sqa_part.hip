@@ -63,9 +63,18 @@ __global__ __launch_bounds__(256) void sqa_join_kernel(PartArgs args) {
   const int c = lane % CH, sg = lane / CH;
   float m = -INFINITY, l = 0.f;
   f4 acc = {0.f, 0.f, 0.f, 0.f};
+  constexpr int U = 4;
   for (int j0 = 0; j0 < total; j0 += 64) {
+    const int n = min(total - j0, 64);
+    auto fetch = [&](int k, f4 (&o)[U]) {
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        o[u] = *(const f4*)(a.part_o + place(j0 + min(k + u * SG + sg, n - 1)) * HD + 4 * c);
+    };
     const int j = min(j0 + lane, total - 1);
     const float2 ml = *(const float2*)(a.part_ml + place(j) * 2);
+    f4 o[U];
+    fetch(0, o);  // on their way beside the maxima
     const bool is = j0 + lane < total;
     float top = is && ml.y != 0.f ? ml.x : -INFINITY;
 #pragma unroll
@@ -81,13 +90,8 @@ __global__ __launch_bounds__(256) void sqa_join_kernel(PartArgs args) {
     l = l * alpha + ls;
     acc *= alpha;
     m = mn;
-    const int n = min(total - j0, 64);
-    constexpr int U = 4;
     for (int k = 0; k < n; k += U * SG) {
-      f4 o[U];
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-        o[u] = *(const f4*)(a.part_o + place(j0 + min(k + u * SG + sg, n - 1)) * HD + 4 * c);
+      if (k > 0) fetch(k, o);
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const int at = k + u * SG + sg;

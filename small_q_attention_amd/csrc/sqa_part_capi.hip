@@ -52,12 +52,13 @@ struct Model {
   // A page (16 tokens of one head's K and V) for each wave of a workgroup, `n` of them at
   // work: the device's 6.6 TB/s shared out, at most 34 GB/s to a unit (both measured, 16 to
   // 128 sequences of 34 to 258 pages), less where the heads read together make short runs; no
-  // less than a wave's chain over a page takes, codes widened or not.
+  // less than a wave's chain over a page takes, by its dims and rows, codes widened or not.
   double page(long long n, int heads, int waves) const {
     const int run = std::min(heads, num_kv_heads) * head_dim * kv_bytes;
     const double worse = run >= 1024 ? 1.0 : run >= 512 ? 1.04 : run >= 256 ? 1.2 : 1.4;
     const double bytes = 32.0 * head_dim * kv_bytes * waves * worse;
-    return std::max({kv_bytes == 1 ? 0.58 : 0.55, bytes * std::min<long long>(n, cus) / 6.6e6,
+    const double work = std::max(head_dim / 128.0 * ((rows + 15) / 16), 1.0);
+    return std::max({(kv_bytes == 1 ? 0.58 : 0.55) * work, bytes * std::min<long long>(n, cus) / 6.6e6,
                      bytes / 34e3});
   }
   // Partial rows written and read again, and the kernel that joins them.
@@ -492,10 +493,22 @@ int sqa_plan_shared_prefix(int device, int batch, int q_len, int num_query_heads
     longest = std::max(longest, group(i).pages);
     most_pages = std::max(most_pages, (long long)pages);
   }
-  long long own = (long long)max_pages << shift;
-  if (max_seq_len > 0) own = std::min(own, ceil_div(max_seq_len, sqa::kPageSize));
-  // The longest sequences follow the longest prefix, where all share one.
-  if (covered == batch) own = std::max(own - longest, 1LL);
+  // Own pages, as far as they can be guessed: what follows a prefix is as long as what the
+  // longest sequence has past the longest one; a group that shares nothing has its prefix to
+  // itself, and a sequence of no group anything.
+  long long whole = (long long)max_pages << shift, longest_named = 0;
+  if (max_seq_len > 0) whole = std::min(whole, ceil_div(max_seq_len, sqa::kPageSize));
+  const auto named = [&](int i) { return std::min((long long)groups[3 * i + 2] << shift, whole); };
+  for (int i = 0; i < num_groups; ++i) longest_named = std::max(longest_named, named(i));
+  const long long tail = std::max(whole - longest_named, 1LL);
+  long long own = covered < batch ? whole : tail;
+  double own_pages = 0.65 * whole * (batch - covered);
+  for (int i = 0; i < num_groups; ++i) {
+    const long long alone = group(i).pages > 0 ? 0 : named(i);
+    own = std::max(own, alone + tail);
+    own_pages += groups[3 * i + 1] * (alone + 0.65 * tail);
+  }
+  const double own_mean = std::max(own_pages / batch, 1.0);
   sqa_shared_plan out;
   memset(&out, 0, sizeof(out));
   out.struct_size = sizeof(out);
@@ -512,13 +525,13 @@ int sqa_plan_shared_prefix(int device, int batch, int q_len, int num_query_heads
   const bool crosses = may_cross(batch, (long long)max_pages << shift);
   OwnCut own_cut;
   if (longest == 0) {
-    own_cut = best_own(m, own, 0.65 * own, crosses);
+    own_cut = best_own(m, own, own_mean, crosses);
   } else {
     out.num_groups = num_groups;
     out.block_rows = rows_of_block(most_rows, rows, head_dim);
-    SharedCut cut = shared_cut(m, out.block_rows, num_groups, group, own, 0.65 * own, crosses);
+    SharedCut cut = shared_cut(m, out.block_rows, num_groups, group, own, own_mean, crosses);
     if (out.block_rows == 256) {  // less of it empty where groups are small
-      const SharedCut halves = shared_cut(m, 128, num_groups, group, own, 0.65 * own, crosses);
+      const SharedCut halves = shared_cut(m, 128, num_groups, group, own, own_mean, crosses);
       if (halves.cost < 0.97 * cut.cost) cut = halves;
     }
     out.block_rows = cut.block_rows;

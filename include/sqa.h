@@ -325,7 +325,7 @@ typedef struct sqa_shared_plan {
   int wg_heads;
   int block_rows;    /* rows of a group that go over its pages together */
   int shared_size;   /* most 16-token pages of a group's split */
-  int shared_splits; /* most splits of a group */
+  int shared_splits; /* slots of the groups' partial rows, in multiples of batch */
   int num_items;     /* blocks x splits of all groups */
 } sqa_shared_plan;
 

@@ -27,7 +27,7 @@ struct PartArgs {
   // fp32 sums and (max in log2 units, sum) of the partial rows. A slot of kv head h and
   // sequence b is `rows` of them. Own slot s starts at row (s * hkv + h) * rows, s = b *
   // splits + j for the sequence's split j, or (splits 0) from seq_splits[b].first on; split j
-  // of the sequence's group at row shared_at + ((j * batch + b) * hkv + h) * rows.
+  // of the sequence's group at row shared_at + ((shared_slot() + j) * hkv + h) * rows.
   PartialArgs p;
   BlockScales scales;      // of codes with block scales
   int kv_type, scaled;     // kF16 (the query's type), kE4M3 or kInt8
@@ -43,14 +43,27 @@ struct PartArgs {
   // together, in blocks of block_rows (16, 32 or 64: one wave's; 128 or 256: a workgroup's)
   // and splits of at most shared_size 16-token pages; n_items blocks x splits in all.
   const int32_t* groups;
-  const int32_t* seq_groups;  // [B][2]: (index of the group, -1: none; its pages)
+  // [B][2]: (16-token pages that the sequences before this one share, a page counted for
+  // each, -1: this one shares none; its group's pages)
+  const int32_t* seq_groups;
   int n_groups, n_items, block_rows, shared_size;
-  int shared_splits;       // most splits of a group
+  // Slots of the groups' splits, shared_slots in all: seq_slots for every sequence, one after
+  // the other, or `packed` (where prefixes are so unlike that most of those would stay empty)
+  // as many as a sequence's group has splits.
+  int shared_slots, seq_slots, packed;
+  FastDiv by_shared_size;
   int shared_wgs;          // workgroups that serve the groups, the first of the grid
   long long shared_at;     // partial row of the groups' first slot
   FastDiv by_rows;         // p.rows
   FastDiv by_shared_heads; // workgroups per item
 };
+
+// Slots of all groups' splits, packed: sequence b's first is b + before / size, `before` the
+// pages that the sequences before it share. A sequence of p = k size + r pages (r < size) has
+// at most k splits, k + 1 where r > 0, and to the next one's first slot it is at least 1 + k.
+inline long long packed_slots(long long batch, long long pages, long long size) {
+  return batch + pages / size;
+}
 
 hipError_t launch_own(const PartArgs& a, hipStream_t stream);
 hipError_t launch_waves(const PartArgs& a, hipStream_t stream);  // groups of one wave's rows

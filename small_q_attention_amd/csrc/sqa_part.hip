@@ -39,26 +39,27 @@ __global__ __launch_bounds__(256) void sqa_join_kernel(PartArgs args) {
     int size;
     own_splits(args, span.n, &own, &size);
     first = b * args.splits;
-    if (span.group < 0 && own <= 1) return;  // uniform: in the output
+    if (span.before < 0 && own <= 1) return;  // uniform: in the output
   } else {
     const SeqSplits t = a.seq_splits[b];
     own = t.count;
     first = t.first;
-    if (span.group < 0 && own == 1) return;  // uniform: in the output
+    if (span.before < 0 && own == 1) return;  // uniform: in the output
   }
   own = __builtin_amdgcn_readfirstlane(own);
-  int shared = 0;
-  if (span.group >= 0) {  // uniform
+  int shared = 0, slot = 0;
+  if (span.before >= 0) {  // uniform
     int size;
     even_splits(span.shared, args.shared_size, &shared, &size);
-    shared = __builtin_amdgcn_readfirstlane(min(shared, args.shared_splits));
+    slot = shared_slot(args, b, span.before);
+    shared = __builtin_amdgcn_readfirstlane(min(shared, args.shared_slots - slot));
   }
   const int total = own + shared;
   const long long own_at = ((long long)first * a.hkv + kvh) * a.rows + r;
-  const long long group_at = args.shared_at + ((long long)b * a.hkv + kvh) * a.rows + r;
+  const long long group_at = args.shared_at + ((long long)slot * a.hkv + kvh) * a.rows + r;
   const long long step = (long long)a.hkv * a.rows;
   auto place = [&](int j) {
-    return j < own ? own_at + j * step : group_at + (j - own) * step * a.batch;
+    return j < own ? own_at + j * step : group_at + (j - own) * step;
   };
   const int c = lane % CH, sg = lane / CH;
   float m = -INFINITY, l = 0.f;

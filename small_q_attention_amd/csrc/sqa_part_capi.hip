@@ -387,6 +387,11 @@ int kv_bytes(int kv_dtype) {
   return kv_dtype == SQA_DTYPE_FP8_E4M3 || kv_dtype == SQA_DTYPE_INT8 ? 1 : 2;
 }
 
+// Slots for each sequence that serve every group's splits: as many as the longest prefix has.
+int even_slots(const sqa_shared_plan& p, int shift) {
+  return sqa::even_splits((long long)p.most_pages << shift, p.shared_size).count;
+}
+
 bool workgroups_fit(const sqa::PartArgs& s) {
   return ((long long)s.p.batch * s.splits + s.own_items) * s.p.hkv <= 0x3fffffffLL;
 }
@@ -476,7 +481,7 @@ int sqa_plan_shared_prefix(int device, int batch, int q_len, int num_query_heads
     const bool shares = groups[3 * i + 1] > 1;
     return SharedGroup{groups[3 * i + 1], shares ? (long long)groups[3 * i + 2] << shift : 0};
   };
-  long long most_rows = 0, most_pages = 0, covered = 0, longest = 0;
+  long long most_rows = 0, most_pages = 0, covered = 0, longest = 0, all_shared = 0;
   int end = 0;
   for (int i = 0; i < num_groups; ++i) {
     const int first = groups[3 * i], count = groups[3 * i + 1], pages = groups[3 * i + 2];
@@ -491,6 +496,7 @@ int sqa_plan_shared_prefix(int device, int batch, int q_len, int num_query_heads
     if (group(i).pages == 0) continue;
     most_rows = std::max(most_rows, count * rows);
     longest = std::max(longest, group(i).pages);
+    all_shared += count * group(i).pages;
     most_pages = std::max(most_pages, (long long)pages);
   }
   // Own pages, as far as they can be guessed: what follows a prefix is as long as what the
@@ -540,12 +546,17 @@ int sqa_plan_shared_prefix(int device, int batch, int q_len, int num_query_heads
       const SharedGroup g = group(i);
       const int splits = sqa::even_splits(g.pages, cut.size).count;
       items += ceil_div(g.count * rows, out.block_rows) * splits;
-      out.shared_splits = std::max(out.shared_splits, splits);
     }
     if (items * num_kv_heads > 0x3fffffffLL) return fail(SQA_ERR_INVALID, "grid too large");
     own_cut = cut.own;
     out.num_items = (int)items;
     out.shared_size = (int)cut.size;
+    // Slots for each sequence as the longest prefix needs them, or packed where that takes
+    // fewer (and pages can be counted in 32 bits).
+    out.shared_splits = even_slots(out, shift);
+    if (all_shared <= 0x7fffffffLL)
+      out.shared_splits = (int)std::min<long long>(
+          out.shared_splits, ceil_div(sqa::packed_slots(batch, all_shared, cut.size), batch));
   }
   out.pages_per_split = own_cut.splits > 0;
   out.num_splits = own_cut.splits > 0 ? own_cut.splits : own_cut.items + batch;
@@ -558,10 +569,12 @@ int sqa_plan_shared_prefix(int device, int batch, int q_len, int num_query_heads
     of[2 * b] = -1;
     of[2 * b + 1] = 0;
   }
+  long long before = 0;
   for (int i = 0; i < num_groups; ++i)
     for (int b = groups[3 * i]; group(i).pages > 0 && b < groups[3 * i] + groups[3 * i + 1]; ++b) {
-      of[2 * b] = i;
+      of[2 * b] = (int32_t)std::min(before, 0x7fffffffLL);
       of[2 * b + 1] = groups[3 * i + 2];
+      before += group(i).pages;
     }
   return SQA_OK;
 }
@@ -600,7 +613,7 @@ int sqa_paged_attention_shared_prefix(const sqa_attention_args* args,
     const int b = plan->block_rows;
     if ((b != 16 && b != 32 && b != 64 && b != 128 && b != 256) ||
         (a.head_dim == 256 && (b == 64 || b == 256)) || (b == 256 && s.p.rows > 32) ||
-        (!tiles && b < s.p.rows))
+        (!tiles && b < s.p.rows) || plan->shared_splits == 0)
       return fail(SQA_ERR_INVALID, "not a plan of sqa_plan_shared_prefix");
     s.groups = table;
     s.seq_groups = table + 3 * plan->num_groups;
@@ -608,7 +621,12 @@ int sqa_paged_attention_shared_prefix(const sqa_attention_args* args,
     s.n_items = plan->num_items;
     s.block_rows = b;
     s.shared_size = plan->shared_size;
-    s.shared_splits = plan->shared_splits;
+    if ((long long)plan->shared_splits * a.batch > 0x7fffffffLL)
+      return fail(SQA_ERR_INVALID, "grid too large");
+    s.shared_slots = plan->shared_splits * a.batch;
+    s.packed = plan->shared_splits < even_slots(*plan, s.p.page_shift);
+    s.seq_slots = s.packed ? 1 : plan->shared_splits;
+    s.by_shared_size = sqa::fast_div((unsigned)plan->shared_size);
     const long long heads = tiles ? a.num_kv_heads : ceil_div(a.num_kv_heads, s.wg_heads);
     if (heads * s.n_items > 0x3fffffffLL) return fail(SQA_ERR_INVALID, "grid too large");
     s.shared_wgs = (int)(heads * s.n_items);

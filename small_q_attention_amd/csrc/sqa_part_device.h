@@ -60,9 +60,16 @@ __device__ __forceinline__ int leader_of(const PartArgs& a, const Group& g) {
 // all, page v of them at v or, past `head`, v - head + tail.
 struct Span {
   int head, tail, n;
-  int group;   // whose pages, `shared` of them, lie before `tail`; -1: none
+  int before;  // of seq_groups, where `shared` pages of its group lie before `tail`; -1: none
   int shared;
 };
+
+// The first slot of the groups' splits for sequence b. Held to what there is: a table that is
+// not the plan's names wrong places, and none outside.
+__device__ __forceinline__ int shared_slot(const PartArgs& a, int b, int before) {
+  const int at = b * a.seq_slots + (a.packed ? before / a.by_shared_size : 0);
+  return min(max(at, 0), a.shared_slots - 1);
+}
 
 // Window: of the pages before row 0's window (the earliest) only those of the first `sink`
 // tokens. Shared prefix: what follows it, provided that every row lies behind it; a shorter
@@ -77,10 +84,10 @@ __device__ __forceinline__ Span span_of(const PartArgs& a, int b, int len) {
     s.tail = max(s.tail, s.head);
   }
   if (a.n_groups > 0) {
-    const int group = a.seq_groups[2 * b];
+    const int before = a.seq_groups[2 * b];
     const int shared = min(max(a.seq_groups[2 * b + 1], 0), a.p.bt_stride) << a.p.page_shift;
-    if (group >= 0 && group < a.n_groups && shared > 0 && reaches(a, len, shared)) {
-      s.group = group;
+    if (before >= 0 && shared > 0 && reaches(a, len, shared)) {
+      s.before = before;
       s.shared = s.tail = shared;
     }
   }
@@ -267,7 +274,8 @@ __device__ __forceinline__ void wild_values(WaveState<NB, HD>& st, PageV<HD, 1>&
 // on, Q * (Hq / Hkv) each.
 struct RowMap {
   int first, kvh;
-  long long at;  // partial row of row 0
+  long long at;  // partial row of row 0, of a sequence's own split
+  int split = -1, before = 0, pages = 0;  // of a group's: Span's of its first sequence
   struct Place {
     int b, y;  // sequence, row of its kv head
   };
@@ -283,7 +291,10 @@ struct RowMap {
   }
   __device__ __forceinline__ long long part_row(const PartArgs& a, int x) const {
     const Place p = place(a, x);
-    return at + (long long)(p.b - first) * a.p.hkv * a.p.rows + p.y;
+    if (split < 0) return at + p.y;
+    const int slot = shared_slot(a, p.b, before + (p.b - first) * pages) + split;
+    return a.shared_at +
+           ((long long)min(slot, a.shared_slots - 1) * a.p.hkv + kvh) * a.p.rows + p.y;
   }
 };
 
@@ -506,7 +517,7 @@ __device__ __forceinline__ void part_share(float* sm_stage, int block, bool shar
     skip = span.tail - span.head;
     v0 = max(at - start, 0);
     n_pages = max(min(end - start, n) - v0, 0);  // 0: the item ends in the seam
-    direct = span.group < 0 && n_pages == n;
+    direct = span.before < 0 && n_pages == n;
     map.first = b;
     map.at = ((long long)(share + b) * args.p.hkv + head_at) * args.p.rows;
     at = x.b < 0 ? end : start + n;
@@ -516,15 +527,16 @@ __device__ __forceinline__ void part_share(float* sm_stage, int block, bool shar
     const PartialArgs& a = args.p;
     const SharedItem it = item_of(args, share);
     b = it.group.pages > 0 ? leader_of(args, it.group) : -1;
-    if (b < 0 || it.split >= args.shared_splits) return;  // uniform over the workgroup
+    if (b < 0) return;  // uniform over the workgroup
     len = 0x7fffffff;
     row0 = it.block * (16 * NB);
     n_rows = it.group.count * a.rows;
     v0 = it.begin;
     n_pages = it.n;
     map.first = it.group.first;
-    map.at = args.shared_at +
-             (((long long)it.split * a.batch + it.group.first) * a.hkv + head_at) * a.rows;
+    map.split = it.split;
+    map.before = scalar_load(args.seq_groups + 2 * it.group.first);
+    map.pages = it.group.pages;
   } else if (crosses) {
     const PartArgs& args = own_args();
     cut = own_cut(args, block == 0 && wave == 0);
@@ -542,7 +554,7 @@ __device__ __forceinline__ void part_share(float* sm_stage, int block, bool shar
     int count, size;
     own_splits(args, span.n, &count, &size);
     if (split >= max(count, 1)) return;  // uniform over the workgroup
-    direct = span.group < 0 && count <= 1;
+    direct = span.before < 0 && count <= 1;
     head = span.head;
     skip = span.tail - span.head;
     v0 = split * size;

@@ -144,16 +144,16 @@ struct TileShare {
   const int kvh = block - share * a.hkv;
   const SharedItem it = item_of(args, share);
   const int b = it.group.pages > 0 ? __builtin_amdgcn_readfirstlane(leader_of(args, it.group)) : -1;
-  if (b < 0 || it.split >= args.shared_splits) return;  // uniform over the workgroup
+  if (b < 0) return;  // uniform over the workgroup
   const int first_page = __builtin_amdgcn_readfirstlane(it.begin);
   const int n_pages = __builtin_amdgcn_readfirstlane(it.n);
   const int tiles = (n_pages + kTilePages - 1) / kTilePages;
   const int row0 = __builtin_amdgcn_readfirstlane(it.block) * (32 * W) + wave * 32;
   const int n_rows = __builtin_amdgcn_readfirstlane(it.group.count) * a.rows;
   const int first = __builtin_amdgcn_readfirstlane(it.group.first);
-  const RowMap map{first, kvh,
-                   args.shared_at + (((long long)__builtin_amdgcn_readfirstlane(it.split) * a.batch +
-                                      first) * a.hkv + kvh) * a.rows};
+  const RowMap map{first, kvh, 0, __builtin_amdgcn_readfirstlane(it.split),
+                   scalar_load(args.seq_groups + 2 * first),
+                   __builtin_amdgcn_readfirstlane(it.group.pages)};
 
   // This wave's page of a tile, from memory to registers.
   const int shift = a.page_shift, sub_mask = (1 << shift) - 1;

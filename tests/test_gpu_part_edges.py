@@ -1,0 +1,112 @@
+"""Attention over a window and over shared prefixes on the GPU where it is least alike to the
+usual call: prefixes of very unlike lengths in one batch."""
+
+import ctypes
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from small_q_attention_amd import _lib  # noqa: E402
+from small_q_attention_amd.shared_prefix import (paged_attention_shared_prefix,  # noqa: E402
+                                                 plan_shared_prefix)
+from tests import _part_reference as ref  # noqa: E402
+from tests._part_reference import BF16, E4M3, F16, INT8  # noqa: E402
+from tests.test_gpu_shared_prefix import inputs, p_step  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+
+CACHES = [(F16, None, False), (BF16, None, False), (F16, E4M3, False), (BF16, E4M3, False),
+          (F16, E4M3, True), (BF16, INT8, True)]
+
+
+def everything(q_len):
+    return lambda i, n: ref.window_seen(n, q_len, 1 << 30, 0)
+
+
+def _copy(plan):
+    p = _lib.SharedPlan()
+    ctypes.memmove(ctypes.byref(p), ctypes.byref(plan), ctypes.sizeof(plan))
+    return p
+
+
+def _splits(pages, size):
+    """As many splits of at most `size` pages as it takes, all alike."""
+    return -(-pages // -(-pages // -(-pages // size))) if pages else 0
+
+
+def _forge(monkeypatch, change):
+    """Plans that ``change(plan, groups in 16-token pages)`` has altered; collects them."""
+    real, made = _lib.plan_shared_prefix, []
+
+    def forged(device, groups, shape, kv, most, width):
+        plan, _, table = real(device, groups, shape, kv, most, width)
+        plan = _copy(plan)
+        change(plan, [(n, pages * (shape[5] // 16) * (n > 1)) for _, n, pages in groups])
+        made.append(plan)
+        return plan, int(_lib.load().sqa_shared_workspace_bytes(ctypes.byref(plan))), table
+
+    monkeypatch.setattr(_lib, "plan_shared_prefix", forged)
+    return made
+
+
+# --------------------------------------------------------------------------------------
+# Prefixes of very unlike lengths: the groups' partial rows lie packed.
+# --------------------------------------------------------------------------------------
+
+UNLIKE = [
+    # A long one first, last and between short ones, groups of one and of no pages, sequences of
+    # no group, some that do not reach; then with a group of more rows than a wave holds.
+    [(0, 2, 90), (2, 5, 2), (8, 1, 7), (9, 3, 3)],
+    [(1, 4, 2), (5, 2, 0), (7, 3, 5), (11, 2, 90)],
+    [(0, 3, 4), (3, 2, 61), (6, 40, 3)],
+    [(0, 40, 1), (42, 2, 61), (44, 3, 9)],
+]
+
+
+@pytest.mark.parametrize("groups", UNLIKE)
+@pytest.mark.parametrize("dtype,kv,scaled", CACHES)
+def test_prefixes_of_unlike_lengths(monkeypatch, groups, dtype, kv, scaled):
+    page, q_len = 16, 2
+    b = groups[-1][0] + groups[-1][1] + 2
+    lens = [17 + 5 * i % 60 for i in range(b)]
+    for first, count, pages in groups:
+        for i in range(first, first + count):
+            lens[i] = pages * page + q_len + (7 * i) % 50
+    lens[groups[0][0]] -= 40  # padded: it goes over its own row
+    q, caches, scales, tables, full, sl = inputs(groups, lens, q_len, 8, 2, 64, page, dtype, kv,
+                                                 scaled, seed=b)
+    want, bound = ref.attention(q, *caches, *scales, full, sl, everything(q_len),
+                                p_step=p_step(dtype, scaled))
+    qc, kc, vc, ks, vs, bt, slc = ref.cuda(q, *caches, *scales, tables, sl)
+
+    for size in (1, 4, 7, 30):
+        def change(p, shared):
+            splits = [_splits(pages, size) for _, pages in shared]
+            p.shared_size, even = size, max(splits)
+            p.num_items = sum(-(-n * 8 // p.block_rows) * s for (n, _), s in zip(shared, splits))
+            p.shared_splits = min(even, -(-(b + sum(n * x for n, x in shared) // size) // b))
+            assert p.shared_splits < even
+
+        with monkeypatch.context() as m:
+            made = _forge(m, change)
+            plan = plan_shared_prefix(groups, b, q_len, 8, 2, 64, page)
+            out = paged_attention_shared_prefix(qc, kc, vc, bt, slc, plan, key_scale=ks,
+                                                value_scale=vs)
+        assert made and made[-1].shared_size == size
+        ref.assert_within(out, want, bound, f"size {size}")
+
+
+def test_a_long_prefix_of_two_in_a_large_batch():
+    """As the plan itself has it: 2 sequences over 16K tokens beside 254 over 64."""
+    groups, q_len = [(0, 2, 1024), (2, 254, 4)], 1
+    lens = [1024 * 16 + 5, 1024 * 16 + 90] + [64 + 1 + i % 40 for i in range(254)]
+    q, (k, v), _, tables, full, sl = inputs(groups, lens, q_len, 8, 2, 128, 16, F16, None, False)
+    want, bound = ref.attention(q, k, v, None, None, full, sl, everything(q_len))
+    made, need, _ = _lib.plan_shared_prefix(0, tuple(groups), (256, q_len, 8, 2, 128, 16),
+                                            _lib.DTYPE_F16, 0, tables.shape[1])
+    assert 1 <= made.shared_splits < _splits(1024, made.shared_size)
+    assert need < 256 << 20
+    args = ref.cuda(q, k, v, tables, sl)
+    plan = plan_shared_prefix(groups, 256, q_len, 8, 2, 128, 16)
+    ref.assert_within(paged_attention_shared_prefix(*args, plan), want, bound)

@@ -54,6 +54,7 @@ struct PartArgs {
   FastDiv by_shared_size;
   int shared_wgs;          // workgroups that serve the groups, the first of the grid
   long long shared_at;     // partial row of the groups' first slot
+  int far_rows;            // partials past 32-bit offsets (p.part_o_bytes is not theirs)
   FastDiv by_rows;         // p.rows
   FastDiv by_shared_heads; // workgroups per item
 };

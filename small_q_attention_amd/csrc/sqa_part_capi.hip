@@ -65,6 +65,11 @@ struct Model {
   double join(double slots) const {
     return 4 + slots * num_kv_heads * rows * head_dim * 8 / 3e6;
   }
+  // Keeps cuts of huge batches from a workspace of more than 4 GiB where others do with less.
+  double memory(double slots) const {
+    return std::max(slots * num_kv_heads * rows * head_dim * 4 - (double)sqa::kMaxPartialBytes, 0.0) /
+           1e3;
+  }
 };
 
 // How the sequences' own pages are dealt out: `splits` equal splits of every sequence, or
@@ -73,6 +78,9 @@ struct OwnCut {
   int splits, items, heads;
   double workgroups, longest, mean;  // times of one of them
   double slots;                      // partial slots that are written
+  double places(int batch) const {   // and that there are, with a group
+    return splits > 0 ? (double)batch * splits : slots;
+  }
 };
 
 // Calls try(cut) for the cuts worth a look. Sequences have up to `most` pages, `mean` on
@@ -129,7 +137,7 @@ OwnCut best_own(const Model& m, long long most, double mean, bool may_cross) {
   double best_cost = -1;
   own_cuts(m, 4, most, mean, may_cross, [&](const OwnCut& c) {
     const double cost = finish(m.cus, 0, 1, c) +
-                        (c.slots > 0 ? m.join(c.slots) : 0);
+                        (c.slots > 0 ? m.join(c.slots) + m.memory(c.slots) : 0);
     if (best_cost < 0 || cost < best_cost * 0.995) {
       best = c;
       best_cost = cost;
@@ -278,11 +286,9 @@ int place(const sqa_attention_args& a, long long rows, size_t need, sqa::PartArg
   if ((uintptr_t)a.workspace % 16)
     return fail(SQA_ERR_WORKSPACE, "workspace must be 16-byte aligned");
   const unsigned long long bytes = (unsigned long long)rows * a.head_dim * 4;
-  if (bytes > sqa::kMaxPartialBytes)
-    return fail(SQA_ERR_INVALID, "the plan's partials (%llu bytes) exceed %llu bytes", bytes,
-                sqa::kMaxPartialBytes);
   s->p.part_o = (float*)a.workspace;
-  s->p.part_o_bytes = (unsigned)bytes;
+  s->far_rows = bytes > sqa::kMaxPartialBytes;
+  s->p.part_o_bytes = s->far_rows ? 0 : (unsigned)bytes;
   s->p.part_ml = s->p.part_o + rows * a.head_dim;
   s->p.seq_splits = (sqa::SeqSplits*)(s->p.part_ml + rows * 2);
   return SQA_OK;
@@ -301,6 +307,15 @@ int rows_of_block(long long most, long long rows, int head_dim) {
 struct SharedGroup {
   long long count, pages;  // 16-token pages
 };
+
+// Slots for the groups' splits, in multiples of the batch: for each sequence as many as the
+// longest prefix has splits, or packed where that takes fewer (and the pages of all sequences'
+// prefixes can be counted in 32 bits).
+int shared_places(int batch, long long longest, long long all, long long size) {
+  const int even = sqa::even_splits(longest, size).count;
+  if (all > 0x7fffffffLL) return even;
+  return (int)std::min<long long>(even, ceil_div(sqa::packed_slots(batch, all, size), batch));
+}
 
 struct SharedCut {
   OwnCut own;
@@ -323,23 +338,27 @@ SharedCut shared_cut(const Model& m, int block_rows, int num_groups, const Group
     if (m.head_dim == 256) return 0.56;
     return (block_rows == 256 ? 0.40 + 0.14 * std::min(n / m.cus, 1.0) : 0.34) * m.head_dim / 128;
   };
-  long long longest = 1;
-  for (int g = 0; g < num_groups; ++g) longest = std::max(longest, group(g).pages);
+  long long longest = 1, all = 0;
+  for (int g = 0; g < num_groups; ++g) {
+    longest = std::max(longest, group(g).pages);
+    all += group(g).count * group(g).pages;
+  }
   struct Option {
     long long size;
-    double items, slots;
+    double items, slots, places;
   };
   Option options[64];
   int n_options = 0;
   for (int n = 1; n <= 256 && (n == 1 || n * sqa::kMinSplitPages <= longest);
        n += std::max(1, n / 8)) {
-    Option o{ceil_div(longest, n), 0, 0};
+    Option o{ceil_div(longest, n), 0, 0, 0};
     if (n_options > 0 && o.size == options[n_options - 1].size) continue;
     for (int g = 0; g < num_groups; ++g) {
       const long long splits = sqa::even_splits(group(g).pages, o.size).count;
       o.items += (double)ceil_div(group(g).count * m.rows, block_rows) * splits;
       o.slots += (double)group(g).count * splits;
     }
+    o.places = shared_places(m.batch, longest, all, o.size) * (double)m.batch;
     options[n_options++] = o;
     if (n_options == 64) break;
   }
@@ -355,7 +374,8 @@ SharedCut shared_cut(const Model& m, int block_rows, int num_groups, const Group
       const double t1 = tiles ? 12 + o.size * tile_page(n1)
                               : 6 + ceil_div(o.size, waves / c.heads) *
                                         m.page((long long)(n1 + c.workgroups), c.heads, waves);
-      const double cost = finish(m.cus, n1, t1, c) + m.join(slots + o.slots);
+      const double cost = finish(m.cus, n1, t1, c) + m.join(slots + o.slots) +
+                          m.memory(c.places(m.batch) + o.places);
       if (best.cost == 0 || cost < best.cost * 0.995) best = {c, block_rows, o.size, cost};
     }
   });
@@ -385,11 +405,6 @@ long long plan_rows(const sqa_shared_plan& p) {
 
 int kv_bytes(int kv_dtype) {
   return kv_dtype == SQA_DTYPE_FP8_E4M3 || kv_dtype == SQA_DTYPE_INT8 ? 1 : 2;
-}
-
-// Slots for each sequence that serve every group's splits: as many as the longest prefix has.
-int even_slots(const sqa_shared_plan& p, int shift) {
-  return sqa::even_splits((long long)p.most_pages << shift, p.shared_size).count;
 }
 
 bool workgroups_fit(const sqa::PartArgs& s) {
@@ -551,12 +566,9 @@ int sqa_plan_shared_prefix(int device, int batch, int q_len, int num_query_heads
     own_cut = cut.own;
     out.num_items = (int)items;
     out.shared_size = (int)cut.size;
-    // Slots for each sequence as the longest prefix needs them, or packed where that takes
-    // fewer (and pages can be counted in 32 bits).
-    out.shared_splits = even_slots(out, shift);
-    if (all_shared <= 0x7fffffffLL)
-      out.shared_splits = (int)std::min<long long>(
-          out.shared_splits, ceil_div(sqa::packed_slots(batch, all_shared, cut.size), batch));
+    out.shared_splits = shared_places(batch, longest, all_shared, cut.size);
+    if ((long long)out.shared_splits * batch > 0x7fffffffLL)
+      return fail(SQA_ERR_INVALID, "grid too large");
   }
   out.pages_per_split = own_cut.splits > 0;
   out.num_splits = own_cut.splits > 0 ? own_cut.splits : own_cut.items + batch;
@@ -624,7 +636,8 @@ int sqa_paged_attention_shared_prefix(const sqa_attention_args* args,
     if ((long long)plan->shared_splits * a.batch > 0x7fffffffLL)
       return fail(SQA_ERR_INVALID, "grid too large");
     s.shared_slots = plan->shared_splits * a.batch;
-    s.packed = plan->shared_splits < even_slots(*plan, s.p.page_shift);
+    s.packed = plan->shared_splits < sqa::even_splits((long long)plan->most_pages << s.p.page_shift,
+                                                      plan->shared_size).count;
     s.seq_slots = s.packed ? 1 : plan->shared_splits;
     s.by_shared_size = sqa::fast_div((unsigned)plan->shared_size);
     const long long heads = tiles ? a.num_kv_heads : ceil_div(a.num_kv_heads, s.wg_heads);

@@ -298,6 +298,25 @@ struct RowMap {
   }
 };
 
+// Chunk c (of HD / 4) of partial row `at`, where `is`. Past 32-bit offsets two stores by
+// address take the place of one through the buffer.
+template <int HD>
+__device__ __forceinline__ void store_partial(const PartArgs& args, __amdgpu_buffer_rsrc_t pr,
+                                              f4 v, long long at, int c, bool is) {
+  if (args.far_rows) {  // uniform
+    const u4 x = __builtin_bit_cast(u4, v);
+    float* to = args.p.part_o + at * HD + 4 * c;
+    if (is) {
+      store_through(to, __builtin_bit_cast(unsigned long long, u2{x[0], x[1]}));
+      store_through(to + 2, __builtin_bit_cast(unsigned long long, u2{x[2], x[3]}));
+    }
+    return;
+  }
+  __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4, v), pr,
+                                         is ? (unsigned)((at * HD + 4 * c) * 4) : kDroppedOffset, 0,
+                                         kThroughAux);
+}
+
 // Leaves the rows of one wave, or of the `waves` ones that have gone over pages of one share
 // (wave `mine` of them; their stages follow one another): normalised rows of the output, or
 // fp32 sums and (max, sum) at partial rows. Through LDS one block of 16 rows at a time, so
@@ -369,9 +388,7 @@ __device__ __forceinline__ void leave_rows(const PartArgs& args, WaveState<NB, H
         if (is) *(u2*)(a.out + map.out_row(args, x0 + rs) * HD + 4 * (e % CPR)) = E::pack4(o);
       } else {
         const long long at = is ? map.part_row(args, x0 + rs) : 0;
-        __builtin_amdgcn_raw_buffer_store_b128(
-            __builtin_bit_cast(u4, v), pr,
-            is ? (unsigned)((at * HD + 4 * (e % CPR)) * 4) : kDroppedOffset, 0, kThroughAux);
+        store_partial<HD>(args, pr, v, at, e % CPR, is);
         if (is && e % CPR == 0)
           store_through(a.part_ml + at * 2, __builtin_bit_cast(unsigned long long, float2{m, l}));
       }

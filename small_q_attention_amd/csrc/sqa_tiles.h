@@ -449,9 +449,7 @@ struct TileShare {
     const f4 v = *(const f4*)(stage + rs * kStageRow + 4 * (e % CPR));
     const bool is = row0 + rs < n_rows;
     const long long at = is ? map.part_row(args, row0 + rs) : 0;
-    __builtin_amdgcn_raw_buffer_store_b128(
-        __builtin_bit_cast(u4, v), pr,
-        is ? (unsigned)((at * HD + 4 * (e % CPR)) * 4) : kDroppedOffset, 0, kThroughAux);
+    store_partial<HD>(args, pr, v, at, e % CPR, is);
   }
   if (h == 0 && row0 + l32 < n_rows) {
     // A NaN sum travels with a finite max, so the join counts the split.

@@ -1,5 +1,5 @@
 """Attention over a window and over shared prefixes on the GPU where it is least alike to the
-usual call: prefixes of very unlike lengths in one batch."""
+usual call: prefixes of very unlike lengths in one batch, partial rows past 32-bit offsets."""
 
 import ctypes
 
@@ -7,9 +7,10 @@ import pytest
 
 torch = pytest.importorskip("torch")
 
-from small_q_attention_amd import _lib  # noqa: E402
+from small_q_attention_amd import _lib, scaled_cache, windowed  # noqa: E402
 from small_q_attention_amd.shared_prefix import (paged_attention_shared_prefix,  # noqa: E402
                                                  plan_shared_prefix)
+from small_q_attention_amd.windowed import paged_attention_windowed  # noqa: E402
 from tests import _part_reference as ref  # noqa: E402
 from tests._part_reference import BF16, E4M3, F16, INT8  # noqa: E402
 from tests.test_gpu_shared_prefix import inputs, p_step  # noqa: E402
@@ -110,3 +111,40 @@ def test_a_long_prefix_of_two_in_a_large_batch():
     args = ref.cuda(q, k, v, tables, sl)
     plan = plan_shared_prefix(groups, 256, q_len, 8, 2, 128, 16)
     ref.assert_within(paged_attention_shared_prefix(*args, plan), want, bound)
+
+
+# --------------------------------------------------------------------------------------
+# Partial rows past 32-bit offsets.
+# --------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype,kv,scaled", CACHES[:2] + CACHES[4:5])
+@pytest.mark.parametrize("count", [2, 10])
+def test_partial_rows_past_4_gib(monkeypatch, dtype, kv, scaled, count):
+    """Cuts with slots for 100000 splits in all, which nearly all stay empty: own rows on both
+    sides of 4 GiB, and past it a group's (of one wave's rows, and in tiles)."""
+    page, q_len, hq, hkv, d = 16, 4, 32, 8, 128
+    groups, b = [(0, count, 40)], count + 2
+    each = 100000 // b
+    lens = [640 + 30 + 90 * i for i in range(count)] + [900, 2000]
+    q, caches, scales, tables, full, sl = inputs(groups, lens, q_len, hq, hkv, d, page, dtype, kv,
+                                                 scaled, seed=count)
+    qc, kc, vc, ks, vs, bt, ft, slc = ref.cuda(q, *caches, *scales, tables, full, sl)
+
+    def change(p, shared):
+        p.num_splits, p.pages_per_split, p.wg_heads = each, 1, 4
+
+    with monkeypatch.context() as m:
+        _forge(m, change)
+        plan = plan_shared_prefix(groups, b, q_len, hq, hkv, d, page)
+        out = paged_attention_shared_prefix(qc, kc, vc, bt, slc, plan, key_scale=ks, value_scale=vs)
+    assert each * (b - 1) * q_len * hq * d * 4 > 4 << 30
+    want, bound = ref.attention(q, *caches, *scales, full, sl, everything(q_len),
+                                p_step=p_step(dtype, scaled))
+    ref.assert_within(out, want, bound, "shared prefix")
+    with monkeypatch.context() as m:
+        m.setattr(windowed, "_KNOWN", scaled_cache.Layouts())
+        m.setattr(_lib, "plan_windowed", lambda *a: (each, 1, 2))
+        out = paged_attention_windowed(qc, kc, vc, ft, slc, 500, sink=9, key_scale=ks, value_scale=vs)
+    want, bound = ref.attention(q, *caches, *scales, full, sl,
+                                lambda i, n: ref.window_seen(n, q_len, 500, 9))
+    ref.assert_within(out, want, bound, "window")

@@ -57,6 +57,7 @@ def plans(tmp_path_factory):
         assert res.returncode == 0, res.stderr
         return json.loads(res.stdout)
 
+    make.units = str(at / "units.so")
     return make
 
 
@@ -145,3 +146,48 @@ def test_slots_of_all_sequences_are_apart(plans):
                 end = slot + n
         assert end <= plan["shared_splits"] * shape[0]
     assert packed > 20
+
+
+def test_plans_of_huge_batches_keep_to_a_few_gib(plans):
+    """Thousands of sequences over long tables: cuts into many splits, whose partial rows take
+    tens of GB, are left for others; what a batch cannot do without (a row of its own and one of
+    its group's each) is not refused."""
+    rng = random.Random(3)
+    calls = []
+    for _ in range(300):
+        batch = rng.choice([1000, 3000, 8192])
+        hkv, d = rng.choice([1, 8, 16]), rng.choice([64, 128, 256])
+        hq = hkv * rng.choice([1, 4, 8])
+        q = rng.randint(1, (32 if d == 256 else 64) // (hq // hkv))
+        width, groups, at = rng.choice([500, 8000, 150000]), [], 0
+        for _ in range(rng.choice([1, 3, 40])):
+            count = min(rng.choice([2, 3, 600, 8192]), batch - at)
+            if count > 0:
+                groups.append((at, count, rng.randint(1, width)))
+            at += count
+        calls.append((groups, (batch, q, hq, hkv, d, 16), 0, rng.choice([0, 16 * width]), width))
+    for (groups, shape, *_, width), plan in zip(calls, plans(calls)):
+        assert plan["rc"] == 0, plan["error"]
+        least = 3 * shape[0] * _slot_bytes(shape)
+        assert plan["bytes"] <= max(5 << 30, least + 8 * shape[0])
+
+
+def test_cuts_of_windows_keep_to_a_few_gib(plans):
+    script = """
+import ctypes, json, sys
+units = ctypes.CDLL(sys.argv[1], mode=ctypes.RTLD_GLOBAL)
+lib = ctypes.CDLL(sys.argv[2])
+lib.sqa_workspace_bytes.restype = ctypes.c_size_t
+n = [ctypes.c_int() for _ in range(3)]
+for batch, q, hq, hkv, d, window, width in json.load(sys.stdin):
+    assert lib.sqa_plan_windowed(0, batch, q, hq, hkv, d, ctypes.c_int64(window), 4, 0, width, 0,
+                                 *(ctypes.byref(x) for x in n)) == 0
+    assert lib.sqa_workspace_bytes(batch, q, hq, hkv, d, n[0].value, n[1].value) < 5 << 30
+"""
+    rng = random.Random(4)
+    calls = [(rng.choice([1300, 2000, 4464]), 8 // g, 16 * g, 16, d, rng.choice([900000, 10**6]),
+              rng.choice([96000, 180000])) for g in (1, 4, 8) for d in (64, 128) for _ in range(8)]
+    calls.append((1937, 8, 128, 16, 128, 1044825, 95985))
+    res = subprocess.run([sys.executable, "-c", script, plans.units, str(build.LIB_PATH)],
+                         input=json.dumps(calls), capture_output=True, text=True)
+    assert res.returncode == 0, res.stderr

@@ -83,11 +83,11 @@ __global__ __launch_bounds__(256) void sqa_join_kernel(PartArgs args) {
     const float mn = fmaxf(m, top);
     const float base = mn == -INFINITY ? 0.f : mn;
     // A NaN sum counts whatever the maxima; of a split that saw no key the sums are 0.
-    const float w = is ? (ml.y != ml.y ? 1.f : fast_exp2(ml.x - base)) : 0.f;
+    const float w = is ? (ml.y != ml.y ? 1.f : weight_of(ml.x - base)) : 0.f;
     float ls = is ? w * ml.y : 0.f;
 #pragma unroll
     for (int o = 1; o < 64; o *= 2) ls += __shfl_xor(ls, o);
-    const float alpha = fast_exp2(m - base);
+    const float alpha = weight_of(m - base);
     l = l * alpha + ls;
     acc *= alpha;
     m = mn;

@@ -203,13 +203,11 @@ __device__ __forceinline__ SharedItem item_of(const PartArgs& a, int item) {
   return it;
 }
 
-// Values of a masked page that are not finite: in the PV product one would reach every row
-// of its block, those that do not see its token too (0 * NaN). They become 0 here, and what
-// they are in the sums of the rows that do see them. Rare: pages without one pay a few
-// instructions, on masked pages only.
+// Values of a page that are not finite, added up in `to` as the rows see them (tokens of a
+// score of -infinity are not seen). Returns whether there are any.
 template <int NB, int HD, typename E>
-__device__ __forceinline__ void wild_values(WaveState<NB, HD>& st, PageV<HD, 1>& pv,
-                                            const f4 (&s)[NB], bool bf16) {
+__device__ __forceinline__ bool add_wild(f4 (&to)[Dims<HD>::MB][NB], const PageV<HD, 1>& pv,
+                                         const f4 (&s)[NB], bool bf16) {
   constexpr int MB = Dims<HD>::MB, VW = Dims<HD>::VW;
   const unsigned inf = bf16 ? 0x7f80u : 0x7c00u, one = bf16 ? 0x3f80u : 0x3c00u;
   const unsigned up = (0x8000u - inf) * 0x10001u;
@@ -218,7 +216,7 @@ __device__ __forceinline__ void wild_values(WaveState<NB, HD>& st, PageV<HD, 1>&
   for (int e = 0; e < 4; ++e)
 #pragma unroll
     for (int w = 0; w < VW; ++w) any |= (pv.v[0][e][w] & 0x7fff7fffu) + up;
-  if (!__any((any & 0x80008000u) != 0u)) return;  // uniform
+  if (!__any((any & 0x80008000u) != 0u)) return false;  // uniform
   u2 rows[NB];
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) {
@@ -228,22 +226,19 @@ __device__ __forceinline__ void wild_values(WaveState<NB, HD>& st, PageV<HD, 1>&
     for (int e = 0; e < 4; ++e) seen[e] = s[nb][e] == -INFINITY ? 0.f : 1.f;
     rows[nb] = E::round_p(seen[0], seen[1], seen[2], seen[3], sum, none);
   }
-  // Sums of ones: over what is NaN or +infinity, then over what is NaN or -infinity.
-#pragma unroll
+  // Sums of ones: over what is NaN or +infinity, then over what is NaN or -infinity. (By bits of
+  // both halves of a word at once: compares, two to an element, took a hundred scalars.)
+#pragma unroll 1
   for (int sign = 0; sign < 2; ++sign) {
     unsigned mark[4][VW];
 #pragma unroll
     for (int e = 0; e < 4; ++e)
 #pragma unroll
       for (int w = 0; w < VW; ++w) {
-        unsigned m = 0u;
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const unsigned x = pv.v[0][e][w] >> (16 * half) & 0xffffu;
-          const bool other = x == (sign ? inf : inf | 0x8000u);
-          m |= ((x & 0x7fffu) >= inf && !other ? one : 0u) << (16 * half);
-        }
-        mark[e][w] = m;
+        const unsigned x = pv.v[0][e][w];
+        const unsigned y = x ^ (sign ? inf : inf | 0x8000u) * 0x10001u;  // 0: the other infinity
+        const unsigned bad = (x & 0x7fff7fffu) + up, apart = ((y & 0x7fff7fffu) + 0x7fff7fffu) | y;
+        mark[e][w] = ((bad & apart & 0x80008000u) >> 15) * one;
       }
 #pragma unroll
     for (int mb = 0; mb < MB; ++mb) {
@@ -256,10 +251,23 @@ __device__ __forceinline__ void wild_values(WaveState<NB, HD>& st, PageV<HD, 1>&
         const f4 hits = E::mma_pv(av, rows[nb], u2{0u, 0u}, f4{0.f, 0.f, 0.f, 0.f});
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          st.acc[mb][nb][e] += hits[e] > 0.f ? (sign ? -INFINITY : INFINITY) : 0.f;
+          to[mb][nb][e] += hits[e] > 0.f ? (sign ? -INFINITY : INFINITY) : 0.f;
       }
     }
   }
+  return true;
+}
+
+// Values of a masked page that are not finite: in the PV product one would reach every row
+// of its block, those that do not see its token too (0 * NaN). They become 0 here, and what
+// they are in the sums of the rows that do see them. Rare: pages without one pay a few
+// instructions, on masked pages only.
+template <int NB, int HD, typename E>
+__device__ __forceinline__ void wild_values(WaveState<NB, HD>& st, PageV<HD, 1>& pv,
+                                            const f4 (&s)[NB], bool bf16) {
+  constexpr int VW = Dims<HD>::VW;
+  if (!add_wild<NB, HD, E>(st.acc, pv, s, bf16)) return;
+  const unsigned up = (0x8000u - (bf16 ? 0x7f80u : 0x7c00u)) * 0x10001u;
 #pragma unroll
   for (int e = 0; e < 4; ++e)
 #pragma unroll
@@ -269,6 +277,10 @@ __device__ __forceinline__ void wild_values(WaveState<NB, HD>& st, PageV<HD, 1>&
       pv.v[0][e][w] = x & ~(bad * 0xffffu);
     }
 }
+
+// 2^x for a sum's weight, never 0: an infinity stays one however far its token's score lies
+// behind. (The smallest number there is, so that finite sums do not notice.)
+__device__ __forceinline__ float weight_of(float x) { return fmaxf(fast_exp2(x), 0x1p-149f); }
 
 // Where row x of a share is: x counts the rows of one kv head of the sequences from `first`
 // on, Q * (Hq / Hkv) each.
@@ -376,7 +388,7 @@ __device__ __forceinline__ void leave_rows(const PartArgs& args, WaveState<NB, H
       for (int w = 0; w < waves; ++w) {
         const float2 ml = *(const float2*)(row + w * kStage + HD);
         const f4 o = *(const f4*)(row + w * kStage + 4 * (e % CPR));
-        const float f = waves == 1 || ml.y != ml.y ? 1.f : fast_exp2(ml.x - base);
+        const float f = waves == 1 || ml.y != ml.y ? 1.f : weight_of(ml.x - base);
         v += o * f;
         l += ml.y * f;
       }
@@ -411,21 +423,22 @@ __device__ __forceinline__ const PartArgs& own_args() {
 }
 
 // How a cache's elements go to the products. kScaled: codes with block scales.
+// kInf: elements may be infinite.
 template <int HD>
 struct PartNative : KvNative<HD> {
-  static constexpr bool kScaled = false;
+  static constexpr bool kScaled = false, kInf = true;
 };
 template <int HD>
 struct PartFp8 : KvFp8<HD> {
-  static constexpr bool kScaled = false;
+  static constexpr bool kScaled = false, kInf = false;
 };
 template <int HD>
 struct PartCodesFp8 : CodesFp8<HD> {
-  static constexpr bool kScaled = true;
+  static constexpr bool kScaled = true, kInf = false;
 };
 template <int HD>
 struct PartCodesInt8 : CodesInt8<HD> {
-  static constexpr bool kScaled = true;
+  static constexpr bool kScaled = true, kInf = false;
 };
 
 // The softmax step of one page without block scales: P = 2^(c s - m) against a maximum that
@@ -678,6 +691,19 @@ __device__ __forceinline__ void part_share(float* sm_stage, int block, bool shar
   const int mask_from = len - a.q_len;
   const int all_from = args.window > 0 ? (int)max((long long)len - args.window, 0LL) : 0;
 
+  auto mask = [&](f4 (&s)[NB], int t0) {  // scores of the page at token t0
+    const int tok0 = t0 + 4 * g16;
+    mask_scores<NB>(s, bits.b, mask_from, tok0, len);
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int t = tok0 + e;
+        const unsigned in = (unsigned)(t >= from[nb]) | (unsigned)(t < args.sink);
+        s[nb][e] = in ? s[nb][e] : -INFINITY;
+      }
+  };
+
   for (int i = 0; i < n_pages; i += D) {
     load_ids(i + 2 * D, ids_next);
 #pragma unroll
@@ -690,18 +716,6 @@ __device__ __forceinline__ void part_share(float* sm_stage, int block, bool shar
                             (t0 < all_from && t0 + kPageSize > args.sink);  // uniform
         f4 s[NB];
         code_scores<NB, HD, E, KV>(s, ring[j].kv, q);
-        auto mask = [&] {
-          const int tok0 = t0 + 4 * g16;
-          mask_scores<NB>(s, bits.b, mask_from, tok0, len);
-#pragma unroll
-          for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int t = tok0 + e;
-              const unsigned in = (unsigned)(t >= from[nb]) | (unsigned)(t < args.sink);
-              s[nb][e] = in ? s[nb][e] : -INFINITY;
-            }
-        };
         if constexpr (KV::kScaled) {
           const float ks = __builtin_bit_cast(
               float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, ring[j].scale), 0));
@@ -717,12 +731,12 @@ __device__ __forceinline__ void part_share(float* sm_stage, int block, bool shar
             for (int nb = 0; nb < NB; ++nb) s[nb] = s[nb] * c + lv;
             c = 1.f;
             add = 0.f;
-            mask();
+            mask(s, t0);
             if constexpr (KV::kNan) nan_values<NB, HD, KV>(st, ring[j].kv, s);
           }
           scaled_page<NB, HD, KV>(st, ring[j].kv, s, masked, c, add, inv_vs, loud);
         } else {
-          if (masked) mask();
+          if (masked) mask(s, t0);
           plain_page<NB, HD, E, KV>(st, ring[j].kv, s, masked, a.scale_log2, a.bf16);
         }
       }
@@ -731,6 +745,46 @@ __device__ __forceinline__ void part_share(float* sm_stage, int block, bool shar
     }
 #pragma unroll
     for (int j = 0; j < D; ++j) ids[j] = ids_next[j];
+  }
+  // An infinity on a page that is not masked is NaN by now in bf16, whose second part of P may
+  // be 0 or negative, and under a probability or a change of the maximum that rounds to 0. The
+  // values that are not finite are added up once more by themselves, and are what they add up
+  // to.
+  if constexpr (KV::kInf) {
+    float sum = 0.f;
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum += st.acc[mb][nb][e];
+    if (__any(sum != sum)) {  // uniform; rare
+      f4 wild[MB][NB];
+#pragma unroll
+      for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) wild[mb][nb] = f4{0.f, 0.f, 0.f, 0.f};
+      for (int i = 0; i < n_pages; ++i) {
+        const int p = page_at(v0 + i);
+        Slot slot;
+        load_page(clamp_page(scalar_load(row + (min(p, a.max_pages - 1) >> shift)), a.num_pages), p,
+                  slot);
+        PageV<HD, 1> pv;
+        KV::template expand_v<E>(slot.kv, pv.v[0]);
+        f4 s[NB];
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) s[nb] = f4{0.f, 0.f, 0.f, 0.f};
+        mask(s, p * kPageSize);
+        add_wild<NB, HD, E>(wild, pv, s, a.bf16);
+      }
+#pragma unroll
+      for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            st.acc[mb][nb][e] = wild[mb][nb][e] == 0.f ? st.acc[mb][nb][e] : wild[mb][nb][e];
+    }
   }
   leave_rows<NB, HD, E>(own_args(), st, sm_stage + head_in * waves * 16 * (HD + 4), waves, mine,
                         direct, map, row0, n_rows, is_head);

@@ -69,15 +69,16 @@ struct PageLoads {
   }
 };
 
+// kInf: elements may be infinite.
 struct StoreNative {
   static constexpr int kBytes = 2;
-  static constexpr bool kScaled = false;
+  static constexpr bool kScaled = false, kInf = true;
   template <typename E>
   static __device__ __forceinline__ void widen(u4 x, u4 (&to)[1]) { to[0] = x; }
 };
 struct StoreFp8 {
   static constexpr int kBytes = 1;
-  static constexpr bool kScaled = false;
+  static constexpr bool kScaled = false, kInf = false;
   template <typename E>
   static __device__ __forceinline__ void widen(u4 x, u4 (&to)[2]) {
     to[0] = E::widen_fp8(u2{x[0], x[1]});
@@ -85,11 +86,11 @@ struct StoreFp8 {
   }
 };
 struct StoreCodesFp8 : StoreFp8 {
-  static constexpr bool kScaled = true;
+  static constexpr bool kScaled = true, kInf = false;
 };
 struct StoreCodesInt8 {
   static constexpr int kBytes = 1;
-  static constexpr bool kScaled = true;
+  static constexpr bool kScaled = true, kInf = false;
   template <typename E>
   static __device__ __forceinline__ void widen(u4 x, u4 (&to)[2]) {
 #pragma unroll
@@ -425,8 +426,51 @@ struct TileShare {
   }
   __syncthreads();  // before the tiles' place is taken
 
-  // Partial rows through LDS.
   float* stage = (float*)lds + wave * 32 * kStageRow;
+  // An infinity is NaN by now under a probability, or a change of the maximum, that rounds to
+  // 0. All rows see all tokens, so what is not finite is added up once more, by dims.
+  if constexpr (KV::kInf) {
+    float any = 0.f;
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) any += acc[mb][r];
+    if (__any(any != any)) {  // uniform; rare
+      constexpr int N = HD / 64;  // dims of a lane
+      float wild[N];
+#pragma unroll
+      for (int n = 0; n < N; ++n) wild[n] = 0.f;
+      for (int i = 0; i < n_pages; ++i) {
+        const int p = first_page + i;
+        const int id = clamp_page(scalar_load(table + (min(p, a.max_pages - 1) >> shift)),
+                                  a.num_pages);
+        const unsigned short* v =
+            (const unsigned short*)((const char*)a.v + (size_t)id * (size_t)a.page_stride +
+                                    (size_t)(p & sub_mask) * sub_bytes + kvh * a.head_stride) +
+            N * lane;
+        for (int t = 0; t < kPageSize; ++t, v += tok / 2)
+#pragma unroll
+          for (int n = 0; n < N; ++n) {
+            const float x = E::kHalfPartials ? (float)__builtin_bit_cast(_Float16, v[n])
+                                             : __builtin_bit_cast(float, (unsigned)v[n] << 16);
+            wild[n] += fabsf(x) < INFINITY ? 0.f : x;
+          }
+      }
+#pragma unroll
+      for (int n = 0; n < N; ++n) stage[N * lane + n] = wild[n];
+      __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+#pragma unroll
+      for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const float w = stage[32 * mb + 8 * (r / 4) + 4 * h + r % 4];
+          acc[mb][r] = w == 0.f ? acc[mb][r] : w;
+        }
+      __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+    }
+  }
+
+  // Partial rows through LDS.
   const __amdgpu_buffer_rsrc_t pr = __builtin_amdgcn_make_buffer_rsrc(
       (void*)a.part_o, (short)0, (int)a.part_o_bytes, kBufferFlags);
   const LanePair both = lane_pair<32>(l);

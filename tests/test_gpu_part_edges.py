@@ -1,5 +1,6 @@
 """Attention over a window and over shared prefixes on the GPU where it is least alike to the
-usual call: prefixes of very unlike lengths in one batch, partial rows past 32-bit offsets."""
+usual call: prefixes of very unlike lengths in one batch, partial rows past 32-bit offsets,
+values that are not finite."""
 
 import ctypes
 
@@ -148,3 +149,84 @@ def test_partial_rows_past_4_gib(monkeypatch, dtype, kv, scaled, count):
     want, bound = ref.attention(q, *caches, *scales, full, sl,
                                 lambda i, n: ref.window_seen(n, q_len, 500, 9))
     ref.assert_within(out, want, bound, "window")
+
+
+# --------------------------------------------------------------------------------------
+# Values that are not finite where every row sees them.
+# --------------------------------------------------------------------------------------
+
+INF, NAN = float("inf"), float("nan")
+
+
+def _put(cache, table, t, head, dim, x):
+    """Value x at token t of a table row (e4m3 has no infinities: NaN)."""
+    page = cache.shape[1]
+    raw = cache.view(torch.uint8) if cache.element_size() == 1 else cache
+    raw[int(table[t // page]), t % page, head, dim] = 0x7F if cache.element_size() == 1 else x
+
+
+@pytest.mark.parametrize("dtype,kv", [(F16, None), (BF16, None), (BF16, E4M3)])
+@pytest.mark.parametrize("d,q_len", [(64, 3), (64, 16), (128, 1), (128, 6), (128, 12), (256, 2), (256, 8)])
+@pytest.mark.parametrize("sharp", [1, 40])
+def test_values_inside_a_window(dtype, kv, d, q_len, sharp):
+    """Infinities and NaN on pages that no edge of a window crosses; with large scores too, where
+    most probabilities and weights of splits round to 0."""
+    hkv, page, window, sink, lens = 2, 16, 2000, 20, [2600, 700, 3000]
+    q, (k, v), _, tables, sl = ref.window_inputs(lens, q_len, 4 * hkv, hkv, d, page, dtype, kv, False,
+                                                 window, sink, seed=d + q_len)
+    q = q * sharp
+    for i, t, h, e, x in ((0, 1500, 0, 5, INF), (0, 900, 0, 6, -INF), (0, 2570, 1, 7, NAN),
+                          (0, 1000, 1, 9, INF), (0, 2400, 1, 9, -INF), (0, 3, 0, 30, -INF),
+                          (1, 33, 1, d - 1, INF), (1, 650, 1, d - 1, INF), (1, 400, 0, 0, -INF)):
+        _put(v, tables[i], t, h, e, x)
+    want, bound = ref.attention(q, k, v, None, None, tables, sl,
+                                lambda i, n: ref.window_seen(n, q_len, window, sink))
+    assert want.isnan().any() and (kv or want.isinf().any()) and want[2].isfinite().all()
+    qc, kc, vc, bt, slc = ref.cuda(q, k, v, tables, sl)
+    for most in (0, 3000):
+        out = paged_attention_windowed(qc, kc, vc, bt, slc, window, sink=sink, max_seq_len=most)
+        ref.assert_within(out, want, bound, f"max_seq_len {most}")
+
+
+@pytest.mark.parametrize("dtype,kv", [(F16, None), (BF16, None), (BF16, E4M3)])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("count,q_len", [(2, 2), (4, 4), (7, 4), (20, 4), (70, 1)])
+@pytest.mark.parametrize("sharp", [1, 40])
+def test_values_on_shared_pages(dtype, kv, d, count, q_len, sharp):
+    """16 to 320 rows of a kv head: in waves, and in tiles of 128 and 256."""
+    hkv, page, shared = 2, 16, 67
+    lens = [shared * page + q_len + 11 * i % 300 for i in range(count)]
+    lens[1] = 100  # goes over its own row
+    q, (k, v), _, tables, full, sl = inputs([(0, count, shared)], lens, q_len, 4 * hkv, hkv, d, page,
+                                            dtype, kv, False, seed=count)
+    q = q * sharp
+    for i, t, h, e, x in ((0, 100, 0, 5, INF), (0, 1000, 0, 6, -INF), (0, 64, 1, 7, NAN),
+                          (0, 33, 1, 9, INF), (0, 990, 1, 9, -INF), (0, shared * page - 1, 0, 0, INF),
+                          (0, 0, 1, d - 1, -INF), (1, 50, 0, 33, INF),
+                          (count - 1, shared * page, 1, 40, INF)):
+        _put(v, full[i], t, h, e, x)
+    want, bound = ref.attention(q, k, v, None, None, full, sl, everything(q_len),
+                                p_step=p_step(dtype, False))
+    assert want.isnan().any() and (kv or want.isinf().any()) and want.isfinite().any()
+    qc, kc, vc, bt, slc = ref.cuda(q, k, v, tables, sl)
+    plan = plan_shared_prefix([(0, count, shared)], count, q_len, 4 * hkv, hkv, d, page)
+    ref.assert_within(paged_attention_shared_prefix(qc, kc, vc, bt, slc, plan), want, bound)
+
+
+@pytest.mark.parametrize("scaled", [E4M3, INT8])
+def test_codes_that_are_nan_in_tiles(scaled):
+    """Under block scales: NaN codes (e4m3) and NaN scales of a shared page reach all rows that
+    share it, in tiles."""
+    count, q_len, page, shared, d = 30, 4, 16, 21, 128
+    lens = [shared * page + q_len + 7 * i % 90 for i in range(count)]
+    q, (k, v), (ks, vs), tables, full, sl = inputs([(0, count, shared)], lens, q_len, 8, 2, d, page,
+                                                   BF16, scaled, True, seed=3)
+    if scaled is E4M3:
+        _put(v, full[0], 200, 1, 9, NAN)
+    vs[int(full[0, 3]), 0] = NAN
+    want, bound = ref.attention(q, k, v, ks, vs, full, sl, everything(q_len))
+    qc, kc, vc, ksc, vsc, bt, slc = ref.cuda(q, k, v, ks, vs, tables, sl)
+    plan = plan_shared_prefix([(0, count, shared)], count, q_len, 8, 2, d, page)
+    out = paged_attention_shared_prefix(qc, kc, vc, bt, slc, plan, key_scale=ksc, value_scale=vsc)
+    assert want.isnan().any() and want.isfinite().any()
+    ref.assert_within(out, want, bound)

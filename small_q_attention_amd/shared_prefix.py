@@ -10,7 +10,8 @@ result comes from ``cuda.paged_mtp_attention`` or a window over everything.
 that stays; :func:`paged_attention_shared_prefix` is the attention call, with the result of
 attention over the whole block tables. It runs on the current stream of the query's device,
 allocates nothing but its result and a workspace, never synchronises and can be captured in a
-HIP graph (keep the plan as long as the graph).
+HIP graph (keep the plan as long as the graph). A plan serves any stream, and may be dropped
+while its eager calls still wait to run.
 """
 
 from __future__ import annotations
@@ -36,6 +37,7 @@ class SharedPrefixPlan:
         self.flat = [x for g in groups for x in g]
         self.most_pages = max([pages for _, count, pages in groups if count > 1] + [0])
         self.known = sc.Layouts()
+        self.streams = set()  # of the eager calls so far
 
 
 def plan_shared_prefix(groups, batch: int, q_len: int, num_query_heads: int, num_kv_heads: int,
@@ -105,14 +107,29 @@ def _plan_call(query, key_cache, key_scale, block_tables, words, groups, max_seq
     return plan, need, _lib.part_fields(query, key_cache, key_scale, block_tables, words)
 
 
+def hold_table(table, stream, device, streams=None):
+    """Keep a plan's table for the calls on ``stream``, the current one: dropped with the plan
+    before they have run, its memory goes to nobody until they have. Once for each of
+    ``streams``. (Not under graph capture: there the caller keeps the plan.)"""
+    if streams is not None and stream in streams:
+        return
+    _, capturing = _lib._CUDA_STATE or _lib._cuda_state(torch)
+    if capturing():
+        return
+    table.record_stream(torch.cuda.current_stream(device))
+    if streams is not None:
+        streams.add(stream)
+
+
 def run_shared_prefix(query, key_cache, value_cache, key_scale, value_scale, block_tables, seq_lens,
                       words, groups, table, scale, out_scale, max_seq_len, out, workspace,
-                      known=None):
-    """Plan and launch a checked call (``groups``, ``table``: a plan's; ``known``: the call's
-    :func:`_plan_call`)."""
+                      known=None, streams=None):
+    """Plan and launch a checked call (``groups``, ``table``, ``streams``: a plan's; ``known``:
+    the call's :func:`_plan_call`)."""
     plan, need, fields = known or _plan_call(query, key_cache, key_scale, block_tables, words,
                                              groups, max_seq_len)
     stream = _lib.raw_stream(query.device.index)
+    hold_table(table, stream, query.device, streams)
     workspace = take_workspace(workspace, need, query, stream)
     if out is None:
         out = torch.empty_like(query)
@@ -181,7 +198,7 @@ def paged_attention_shared_prefix(query, key_cache, value_cache, block_tables, s
     check_apart(query, out)
     return sc.on_device(query.device, run_shared_prefix, query, key_cache, value_cache, key_scale,
                         value_scale, block_tables, seq_lens, words, plan.groups, plan.table, scale,
-                        float(out_scale), max_seq_len, out, workspace_buffer, known)
+                        float(out_scale), max_seq_len, out, workspace_buffer, known, plan.streams)
 
 
 __all__ = ["SharedPrefixPlan", "plan_shared_prefix", "paged_attention_shared_prefix"]

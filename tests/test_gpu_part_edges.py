@@ -1,6 +1,6 @@
 """Attention over a window and over shared prefixes on the GPU where it is least alike to the
 usual call: prefixes of very unlike lengths in one batch, partial rows past 32-bit offsets,
-values that are not finite."""
+values that are not finite, plans dropped while their calls wait."""
 
 import ctypes
 
@@ -8,7 +8,7 @@ import pytest
 
 torch = pytest.importorskip("torch")
 
-from small_q_attention_amd import _lib, scaled_cache, windowed  # noqa: E402
+from small_q_attention_amd import _lib, _op, scaled_cache, windowed  # noqa: E402,F401
 from small_q_attention_amd.shared_prefix import (paged_attention_shared_prefix,  # noqa: E402
                                                  plan_shared_prefix)
 from small_q_attention_amd.windowed import paged_attention_windowed  # noqa: E402
@@ -230,3 +230,38 @@ def test_codes_that_are_nan_in_tiles(scaled):
     out = paged_attention_shared_prefix(qc, kc, vc, bt, slc, plan, key_scale=ksc, value_scale=vsc)
     assert want.isnan().any() and want.isfinite().any()
     ref.assert_within(out, want, bound)
+
+
+# --------------------------------------------------------------------------------------
+# Plans and streams.
+# --------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("traced", [False, True])
+def test_a_plan_dropped_before_its_call_has_run(traced):
+    """A call waits on another stream than its plan was made on, behind a second of other work;
+    the plan goes and others are made meanwhile. The table's memory is not theirs."""
+    groups, b = [(0, 3, 8), (3, 30, 20)], 33
+    lens = [8 * 16 + 5 + i for i in range(3)] + [20 * 16 + 5 + i for i in range(30)]
+    q, (k, v), _, tables, full, sl = inputs(groups, lens, 4, 8, 2, 128, 16, F16, None, False)
+    args = ref.cuda(q, k, v, tables, sl)
+
+    def call(plan):
+        if not traced:
+            return paged_attention_shared_prefix(*args, plan)
+        return torch.ops.sqa.paged_attention_shared_prefix(
+            *args[:3], None, None, *args[3:], None, plan.flat, plan.table, 128 ** -0.5, 1.0, 0)
+
+    want = call(plan_shared_prefix(groups, b, 4, 8, 2, 128, 16)).clone()
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    plan = plan_shared_prefix(groups, b, 4, 8, 2, 128, 16)
+    at = plan.table.data_ptr()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(2_000_000_000)
+        out = call(plan)
+    del plan
+    others = [plan_shared_prefix([(0, 33, 1)], b, 4, 8, 2, 128, 16) for _ in range(8)]
+    assert not side.query()  # the call still waits
+    assert all(p.table.data_ptr() != at for p in others)
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)

@@ -295,3 +295,24 @@ def test_traced_ops_are_registered():
                                                       0.1, 1.0, 0)
     assert out.shape == q.shape
     assert spec_dec_mask(1, 2).shape == (1, 2, 2)
+
+
+def test_a_plans_table_is_held_for_each_stream(monkeypatch):
+    """Once for a stream of eager calls, every time where no plan counts them, never under
+    capture."""
+    held, capturing = [], [False]
+
+    class Table:
+        def record_stream(self, stream):
+            held.append(stream)
+
+    monkeypatch.setattr(_lib, "_CUDA_STATE", (lambda: 0, lambda: capturing[0]))
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device: f"current of {device}")
+    seen = _plan().streams
+    for stream, streams, count in ((7, seen, 1), (7, seen, 1), (9, seen, 2), (9, None, 3),
+                                   (9, None, 4)):
+        shared_prefix.hold_table(Table(), stream, "cuda:0", streams)
+        assert len(held) == count
+    capturing[0] = True
+    shared_prefix.hold_table(Table(), 11, "cuda:0", seen)
+    assert len(held) == 4 and seen == {7, 9} and held[0] == "current of cuda:0"

@@ -27,7 +27,7 @@ struct PartArgs {
   // fp32 sums and (max in log2 units, sum) of the partial rows. A slot of kv head h and
   // sequence b is `rows` of them. Own slot s starts at row (s * hkv + h) * rows, s = b *
   // splits + j for the sequence's split j, or (splits 0) from seq_splits[b].first on; split j
-  // of the sequence's group at row shared_at + ((shared_slot() + j) * hkv + h) * rows.
+  // of the sequence's group at row shared_at + (shared_slot(j) * hkv + h) * rows.
   PartialArgs p;
   BlockScales scales;      // of codes with block scales
   int kv_type, scaled;     // kF16 (the query's type), kE4M3 or kInt8
@@ -47,16 +47,17 @@ struct PartArgs {
   // each, -1: this one shares none; its group's pages)
   const int32_t* seq_groups;
   int n_groups, n_items, block_rows, shared_size;
-  // Slots of the groups' splits, shared_slots in all: seq_slots for every sequence, one after
-  // the other, or `packed` (where prefixes are so unlike that most of those would stay empty)
-  // as many as a sequence's group has splits.
-  int shared_slots, seq_slots, packed;
-  FastDiv by_shared_size;
+  int most_splits;         // of a group
   int shared_wgs;          // workgroups that serve the groups, the first of the grid
   long long shared_at;     // partial row of the groups' first slot
-  int far_rows;            // partials past 32-bit offsets (p.part_o_bytes is not theirs)
   FastDiv by_rows;         // p.rows
   FastDiv by_shared_heads; // workgroups per item
+  // Slots of the groups' splits, shared_slots in all: the batch's for each split, one after the
+  // other (slot_step the batch), or `packed` (where prefixes are so unlike that most of those
+  // would stay empty) a sequence's (slot_step 1).
+  int packed, shared_slots, slot_step;
+  int far_rows;            // partials past 32-bit offsets (p.part_o_bytes is not theirs)
+  FastDiv by_shared_size;
 };
 
 // Slots of all groups' splits, packed: sequence b's first is b + before / size, `before` the

@@ -52,14 +52,15 @@ __global__ __launch_bounds__(256) void sqa_join_kernel(PartArgs args) {
     int size;
     even_splits(span.shared, args.shared_size, &shared, &size);
     slot = shared_slot(args, b, span.before);
-    shared = __builtin_amdgcn_readfirstlane(min(shared, args.shared_slots - slot));
+    shared = __builtin_amdgcn_readfirstlane(
+        min(shared, args.packed ? args.shared_slots - slot : args.most_splits));
   }
   const int total = own + shared;
   const long long own_at = ((long long)first * a.hkv + kvh) * a.rows + r;
   const long long group_at = args.shared_at + ((long long)slot * a.hkv + kvh) * a.rows + r;
   const long long step = (long long)a.hkv * a.rows;
   auto place = [&](int j) {
-    return j < own ? own_at + j * step : group_at + (j - own) * step;
+    return j < own ? own_at + j * step : group_at + (j - own) * step * args.slot_step;
   };
   const int c = lane % CH, sg = lane / CH;
   float m = -INFINITY, l = 0.f;

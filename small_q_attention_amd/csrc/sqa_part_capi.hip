@@ -285,6 +285,7 @@ int place(const sqa_attention_args& a, long long rows, size_t need, sqa::PartArg
                 a.workspace ? a.workspace_bytes : (size_t)0);
   if ((uintptr_t)a.workspace % 16)
     return fail(SQA_ERR_WORKSPACE, "workspace must be 16-byte aligned");
+  if (rows > 0x7fffffffLL) return fail(SQA_ERR_INVALID, "grid too large");
   const unsigned long long bytes = (unsigned long long)rows * a.head_dim * 4;
   s->p.part_o = (float*)a.workspace;
   s->far_rows = bytes > sqa::kMaxPartialBytes;
@@ -636,9 +637,10 @@ int sqa_paged_attention_shared_prefix(const sqa_attention_args* args,
     if ((long long)plan->shared_splits * a.batch > 0x7fffffffLL)
       return fail(SQA_ERR_INVALID, "grid too large");
     s.shared_slots = plan->shared_splits * a.batch;
-    s.packed = plan->shared_splits < sqa::even_splits((long long)plan->most_pages << s.p.page_shift,
-                                                      plan->shared_size).count;
-    s.seq_slots = s.packed ? 1 : plan->shared_splits;
+    s.most_splits = sqa::even_splits((long long)plan->most_pages << s.p.page_shift,
+                                     plan->shared_size).count;
+    s.packed = plan->shared_splits < s.most_splits;
+    s.slot_step = s.packed ? 1 : a.batch;
     s.by_shared_size = sqa::fast_div((unsigned)plan->shared_size);
     const long long heads = tiles ? a.num_kv_heads : ceil_div(a.num_kv_heads, s.wg_heads);
     if (heads * s.n_items > 0x3fffffffLL) return fail(SQA_ERR_INVALID, "grid too large");

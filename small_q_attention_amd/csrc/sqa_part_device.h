@@ -64,11 +64,11 @@ struct Span {
   int shared;
 };
 
-// The first slot of the groups' splits for sequence b. Held to what there is: a table that is
-// not the plan's names wrong places, and none outside.
+// The slot of the first split of its group for sequence b; further ones follow slot_step apart.
+// Held to what there is: a table that is not the plan's names wrong places, and none outside.
 __device__ __forceinline__ int shared_slot(const PartArgs& a, int b, int before) {
-  const int at = b * a.seq_slots + (a.packed ? before / a.by_shared_size : 0);
-  return min(max(at, 0), a.shared_slots - 1);
+  if (!a.packed) return b;  // uniform
+  return min(max(b + before / a.by_shared_size, 0), a.shared_slots - 1);
 }
 
 // Window: of the pages before row 0's window (the earliest) only those of the first `sink`
@@ -278,6 +278,18 @@ __device__ __forceinline__ void wild_values(WaveState<NB, HD>& st, PageV<HD, 1>&
     }
 }
 
+// Whether sums are NaN somewhere in the wave: maxima that pass one on, in four chains.
+struct NanOf {
+  float top[4] = {0.f, 0.f, 0.f, 0.f};
+  __device__ __forceinline__ void add(int i, f4 x) {
+    top[i % 4] = max3_raw(max3_raw(top[i % 4], x[0], x[1]), x[2], x[3]);
+  }
+  __device__ __forceinline__ bool any() const {
+    const float x = max3_raw(max3_raw(top[0], top[1], top[2]), top[3], top[3]);
+    return __any(x != x);
+  }
+};
+
 // 2^x for a sum's weight, never 0: an infinity stays one however far its token's score lies
 // behind. (The smallest number there is, so that finite sums do not notice.)
 __device__ __forceinline__ float weight_of(float x) { return fmaxf(fast_exp2(x), 0x1p-149f); }
@@ -286,8 +298,10 @@ __device__ __forceinline__ float weight_of(float x) { return fmaxf(fast_exp2(x),
 // on, Q * (Hq / Hkv) each.
 struct RowMap {
   int first, kvh;
-  long long at;  // partial row of row 0, of a sequence's own split
-  int split = -1, before = 0, pages = 0;  // of a group's: Span's of its first sequence
+  long long at;  // partial row of row 0
+  // Of a group's share where its slots are packed (else pages is 0): the split, the first
+  // sequence's entry in seq_groups, the group's pages.
+  int split = 0, before = 0, pages = 0;
   struct Place {
     int b, y;  // sequence, row of its kv head
   };
@@ -303,10 +317,10 @@ struct RowMap {
   }
   __device__ __forceinline__ long long part_row(const PartArgs& a, int x) const {
     const Place p = place(a, x);
-    if (split < 0) return at + p.y;
-    const int slot = shared_slot(a, p.b, before + (p.b - first) * pages) + split;
+    if (pages == 0) return at + (long long)(p.b - first) * a.p.hkv * a.p.rows + p.y;
+    const unsigned slot = shared_slot(a, p.b, before + (p.b - first) * pages) + split;
     return a.shared_at +
-           ((long long)min(slot, a.shared_slots - 1) * a.p.hkv + kvh) * a.p.rows + p.y;
+           ((long long)min(slot, (unsigned)a.shared_slots - 1) * a.p.hkv + kvh) * a.p.rows + p.y;
   }
 };
 
@@ -327,6 +341,19 @@ __device__ __forceinline__ void store_partial(const PartArgs& args, __amdgpu_buf
   __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4, v), pr,
                                          is ? (unsigned)((at * HD + 4 * c) * 4) : kDroppedOffset, 0,
                                          kThroughAux);
+}
+
+// The map of a group's share for kv head kvh.
+__device__ __forceinline__ RowMap shared_map(const PartArgs& a, int first, int split, int pages,
+                                             int kvh) {
+  RowMap map{first, kvh,
+             a.shared_at + (((long long)split * a.p.batch + first) * a.p.hkv + kvh) * a.p.rows};
+  if (a.packed) {  // uniform
+    map.split = split;
+    map.before = scalar_load(a.seq_groups + 2 * first);
+    map.pages = pages;
+  }
+  return map;
 }
 
 // Leaves the rows of one wave, or of the `waves` ones that have gone over pages of one share
@@ -373,6 +400,10 @@ __device__ __forceinline__ void leave_rows(const PartArgs& args, WaveState<NB, H
       __syncthreads();
     else
       __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+    // Where the lane's row goes, in rows of HD (less than 2^31 of either), -1: nowhere.
+    const int to = !store || x0 + l16 >= n_rows ? -1
+                   : direct                     ? (int)map.out_row(args, x0 + l16)
+                                                : (int)map.part_row(args, x0 + l16);
     // Chunk e % CPR of row e / CPR (< 16), the waves in turn.
     for (int i = waves > 1 ? mine : 0; i < CPR / 4; i += waves) {
       const int e = i * 64 + lane;
@@ -392,14 +423,14 @@ __device__ __forceinline__ void leave_rows(const PartArgs& args, WaveState<NB, H
         v += o * f;
         l += ml.y * f;
       }
-      const bool is = store && x0 + rs < n_rows;
+      const long long at = __shfl(to, rs);
+      const bool is = at >= 0;
       if (direct) {
         // l = 0: the row saw no key (written as 0). A NaN l passes.
         const float sc = !(l <= 0.f) ? a.out_scale / l : 0.f;
         const float o[4] = {v[0] * sc, v[1] * sc, v[2] * sc, v[3] * sc};
-        if (is) *(u2*)(a.out + map.out_row(args, x0 + rs) * HD + 4 * (e % CPR)) = E::pack4(o);
+        if (is) *(u2*)(a.out + at * HD + 4 * (e % CPR)) = E::pack4(o);
       } else {
-        const long long at = is ? map.part_row(args, x0 + rs) : 0;
         store_partial<HD>(args, pr, v, at, e % CPR, is);
         if (is && e % CPR == 0)
           store_through(a.part_ml + at * 2, __builtin_bit_cast(unsigned long long, float2{m, l}));
@@ -557,16 +588,13 @@ __device__ __forceinline__ void part_share(float* sm_stage, int block, bool shar
     const PartialArgs& a = args.p;
     const SharedItem it = item_of(args, share);
     b = it.group.pages > 0 ? leader_of(args, it.group) : -1;
-    if (b < 0) return;  // uniform over the workgroup
+    if (b < 0 || it.split >= args.most_splits) return;  // uniform over the workgroup
     len = 0x7fffffff;
     row0 = it.block * (16 * NB);
     n_rows = it.group.count * a.rows;
     v0 = it.begin;
     n_pages = it.n;
-    map.first = it.group.first;
-    map.split = it.split;
-    map.before = scalar_load(args.seq_groups + 2 * it.group.first);
-    map.pages = it.group.pages;
+    map = shared_map(args, it.group.first, it.split, it.group.pages, head_at);
   } else if (crosses) {
     const PartArgs& args = own_args();
     cut = own_cut(args, block == 0 && wave == 0);
@@ -751,14 +779,12 @@ __device__ __forceinline__ void part_share(float* sm_stage, int block, bool shar
   // values that are not finite are added up once more by themselves, and are what they add up
   // to.
   if constexpr (KV::kInf) {
-    float sum = 0.f;
+    NanOf nan;
 #pragma unroll
     for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) sum += st.acc[mb][nb][e];
-    if (__any(sum != sum)) {  // uniform; rare
+      for (int nb = 0; nb < NB; ++nb) nan.add(mb * NB + nb, st.acc[mb][nb]);
+    if (nan.any()) {  // uniform; rare
       f4 wild[MB][NB];
 #pragma unroll
       for (int mb = 0; mb < MB; ++mb)

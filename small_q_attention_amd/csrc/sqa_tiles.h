@@ -145,16 +145,15 @@ struct TileShare {
   const int kvh = block - share * a.hkv;
   const SharedItem it = item_of(args, share);
   const int b = it.group.pages > 0 ? __builtin_amdgcn_readfirstlane(leader_of(args, it.group)) : -1;
-  if (b < 0) return;  // uniform over the workgroup
+  if (b < 0 || it.split >= args.most_splits) return;  // uniform over the workgroup
   const int first_page = __builtin_amdgcn_readfirstlane(it.begin);
   const int n_pages = __builtin_amdgcn_readfirstlane(it.n);
   const int tiles = (n_pages + kTilePages - 1) / kTilePages;
   const int row0 = __builtin_amdgcn_readfirstlane(it.block) * (32 * W) + wave * 32;
   const int n_rows = __builtin_amdgcn_readfirstlane(it.group.count) * a.rows;
   const int first = __builtin_amdgcn_readfirstlane(it.group.first);
-  const RowMap map{first, kvh, 0, __builtin_amdgcn_readfirstlane(it.split),
-                   scalar_load(args.seq_groups + 2 * first),
-                   __builtin_amdgcn_readfirstlane(it.group.pages)};
+  const RowMap map = shared_map(args, first, __builtin_amdgcn_readfirstlane(it.split),
+                                __builtin_amdgcn_readfirstlane(it.group.pages), kvh);
 
   // This wave's page of a tile, from memory to registers.
   const int shift = a.page_shift, sub_mask = (1 << shift) - 1;
@@ -430,12 +429,13 @@ struct TileShare {
   // An infinity is NaN by now under a probability, or a change of the maximum, that rounds to
   // 0. All rows see all tokens, so what is not finite is added up once more, by dims.
   if constexpr (KV::kInf) {
-    float any = 0.f;
+    NanOf nan;
 #pragma unroll
     for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) any += acc[mb][r];
-    if (__any(any != any)) {  // uniform; rare
+      for (int i = 0; i < 4; ++i)
+        nan.add(i, f4{acc[mb][4 * i], acc[mb][4 * i + 1], acc[mb][4 * i + 2], acc[mb][4 * i + 3]});
+    if (nan.any()) {  // uniform; rare
       constexpr int N = HD / 64;  // dims of a lane
       float wild[N];
 #pragma unroll
@@ -485,20 +485,27 @@ struct TileShare {
       *(f4*)(stage + l32 * kStageRow + 32 * mb + 8 * i + 4 * h) = o;
     }
   __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+  const bool mine = row0 + l32 < n_rows;
+  const int to = mine ? (int)map.part_row(args, row0 + l32) : -1;  // there are less than 2^31
   constexpr int CPR = HD / 4;
-#pragma unroll
-  for (int i = 0; i < CPR / 2; ++i) {
+  auto leave = [&](int i) {
     const int e = i * 64 + lane;  // row e / CPR (< 32), chunk e % CPR
     const int rs = e / CPR;
     const f4 v = *(const f4*)(stage + rs * kStageRow + 4 * (e % CPR));
-    const bool is = row0 + rs < n_rows;
-    const long long at = is ? map.part_row(args, row0 + rs) : 0;
-    store_partial<HD>(args, pr, v, at, e % CPR, is);
+    const int at = __shfl(to, rs);
+    store_partial<HD>(args, pr, v, at, e % CPR, at >= 0);
+  };
+  if (args.far_rows) {  // uniform
+#pragma unroll 1
+    for (int i = 0; i < CPR / 2; ++i) leave(i);
+  } else {
+#pragma unroll
+    for (int i = 0; i < CPR / 2; ++i) leave(i);
   }
-  if (h == 0 && row0 + l32 < n_rows) {
+  if (h == 0 && mine) {
     // A NaN sum travels with a finite max, so the join counts the split.
     const float m_out = sum == sum ? m : 0.f;
-    store_through(a.part_ml + map.part_row(args, row0 + l32) * 2,
+    store_through(a.part_ml + (long long)to * 2,
                   __builtin_bit_cast(unsigned long long, float2{m_out, sum}));
   }
   }

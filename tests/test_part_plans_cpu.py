@@ -133,7 +133,7 @@ def test_slots_of_all_sequences_are_apart(plans):
         is_packed = plan["shared_splits"] < max(splits)
         packed += is_packed
         of = plan["table"][3 * len(groups):]
-        end = 0
+        used = set()
         for (first, count, pages), n in zip(groups, splits):
             for b in range(first, first + count):
                 before, own = of[2 * b:2 * b + 2]
@@ -141,10 +141,11 @@ def test_slots_of_all_sequences_are_apart(plans):
                     assert before == -1
                     continue
                 assert own == pages
-                slot = b + before // size if is_packed else b * plan["shared_splits"]
-                assert slot >= end
-                end = slot + n
-        assert end <= plan["shared_splits"] * shape[0]
+                mine = ({b + before // size + j for j in range(n)} if is_packed
+                        else {b + j * shape[0] for j in range(n)})
+                assert not used & mine
+                used |= mine
+        assert max(used) < plan["shared_splits"] * shape[0]
     assert packed > 20
 
 

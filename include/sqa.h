@@ -301,7 +301,7 @@ int sqa_plan_windowed(int device, int batch, int q_len, int num_query_heads, int
  * or int8 codes as for sqa_paged_attention_scaled; flags 0, num_splits, pages_per_split and
  * wg_heads from sqa_plan_windowed, workspace sqa_workspace_bytes(..., num_splits,
  * pages_per_split) bytes (0 for one split each). A value that is not finite reaches the rows
- * that see its token. output is not query's buffer. Equal inputs and cuts give equal bits.
+ * that see its token. output does not overlap query. Equal inputs and cuts give equal bits.
  */
 int sqa_paged_attention_windowed(const sqa_attention_args* args, const sqa_block_scales* scales,
                                  int64_t window, int sink, int wg_heads);
@@ -353,7 +353,7 @@ size_t sqa_shared_workspace_bytes(const sqa_shared_plan* plan);
  * where num_items is 0). The shared pages are read through the table row of the group's
  * first sequence that reaches past them with all of its rows (seq_lens[b] - q_len >= shared
  * tokens); sequences that do not (a padded batch's) go over their own pages from the first
- * on. output is not query's buffer.
+ * on. output does not overlap query.
  * kv_dtype and `scales` as for sqa_paged_attention_windowed; flags 0, num_splits and
  * pages_per_split the plan's. Equal inputs and plans give equal bits.
  */

@@ -271,6 +271,15 @@ int fill(const sqa_attention_args& a, const sqa_block_scales* scales, int wg_hea
   return SQA_OK;
 }
 
+// The queries are read until the end, by workgroups beside those that write results.
+int check_apart(const sqa_attention_args& a) {
+  const unsigned long long bytes =
+      2ull * a.batch * a.q_len * (unsigned long long)a.num_query_heads * a.head_dim;
+  const uintptr_t q = (uintptr_t)a.query, o = (uintptr_t)a.output;
+  if ((q < o ? o - q : q - o) < bytes) return fail(SQA_ERR_INVALID, "output overlaps query");
+  return SQA_OK;
+}
+
 // Slots of the sequences' own pages.
 long long own_slots(int batch, int num_splits, int pages_per_split) {
   return pages_per_split ? (long long)batch * num_splits : num_splits;
@@ -460,6 +469,7 @@ int sqa_paged_attention_windowed(const sqa_attention_args* args, const sqa_block
   const size_t need = sqa_workspace_bytes(a.batch, a.q_len, a.num_query_heads, a.num_kv_heads,
                                           a.head_dim, a.num_splits, a.pages_per_split);
   if (int rc = place(a, rows, need, &s)) return rc;
+  if (int rc = check_apart(a)) return rc;
 
   hipStream_t stream = (hipStream_t)a.stream;
   hipEvent_t* ev = (hipEvent_t*)a.timing_events;
@@ -651,6 +661,7 @@ int sqa_paged_attention_shared_prefix(const sqa_attention_args* args,
   s.shared_at = own_rows(*plan);
   const size_t need = sqa_shared_workspace_bytes(plan);
   if (int rc = place(a, plan_rows(*plan), need, &s)) return rc;
+  if (int rc = check_apart(a)) return rc;
 
   hipStream_t stream = (hipStream_t)a.stream;
   hipEvent_t* ev = (hipEvent_t*)a.timing_events;

@@ -57,9 +57,10 @@ def check_call(query, key_cache, value_cache, key_scale, value_scale, block_tabl
 
 
 def check_apart(query, out):
-    """ValueError for a result in the queries' place: they are read until the end."""
-    if out is not None and out.data_ptr() == query.data_ptr():
-        raise ValueError("out must not be query")
+    """ValueError for a result that takes some of the queries' place: they are read until the
+    end. (Both are contiguous, of one size.)"""
+    if out is not None and abs(out.data_ptr() - query.data_ptr()) < query.nbytes:
+        raise ValueError("out must not be query, nor overlap it")
 
 
 def take_workspace(workspace_buffer, need, query, stream):

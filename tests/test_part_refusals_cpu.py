@@ -316,3 +316,25 @@ def test_a_plans_table_is_held_for_each_stream(monkeypatch):
     capturing[0] = True
     shared_prefix.hold_table(Table(), 11, "cuda:0", seen)
     assert len(held) == 4 and seen == {7, 9} and held[0] == "current of cuda:0"
+
+
+def test_out_does_not_overlap_the_query():
+    """A result that begins within the queries, or they within it, is refused; one that begins
+    where they end is not."""
+    store = torch.zeros(40, dtype=F16)
+    q = store[8:24].view(2, 8)
+    for at in (0, 1, 7, 9, 16, 23):
+        with pytest.raises(ValueError, match="overlap"):
+            windowed.check_apart(q, store[at:at + 16].view(2, 8))
+    windowed.check_apart(store[:16].view(2, 8), store[16:32].view(2, 8))
+    windowed.check_apart(store[16:32].view(2, 8), store[:16].view(2, 8))
+
+
+@pytest.mark.parametrize("off", [0, 16, -16, 3 * 3 * 8 * 64 * 2 - 8, -(3 * 3 * 8 * 64 * 2 - 8)])
+def test_c_entries_refuse_an_output_over_the_query(lib, off):
+    a = _args(output=(1 << 20) + off)
+    assert lib.sqa_paged_attention_windowed(ctypes.byref(a), None, 10, 0, 2) == 1
+    assert "overlaps" in lib.sqa_last_error().decode()
+    assert lib.sqa_paged_attention_shared_prefix(ctypes.byref(a), None, ctypes.byref(_c_plan()),
+                                                 1 << 20) == 1
+    assert "overlaps" in lib.sqa_last_error().decode()

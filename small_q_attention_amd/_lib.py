@@ -18,6 +18,7 @@ _LOCK = threading.Lock()
 _LIB = None
 
 SQA_OK = 0
+SQA_ERR_HIP = 4
 
 # (name, restype, argtypes) for every symbol include/sqa.h declares.
 _C = ctypes
@@ -361,6 +362,13 @@ def launch_scaled(query, output, k_view, v_view, k_scale, v_scale, block_tables,
         raise RuntimeError(f"sqa_paged_attention_scaled failed: {last_error(lib)}")
 
 
+def refusal(lib, name: str, rc: int):
+    """The exception for a status: what the library finds outside its contract (a stride, an
+    alignment, a factor that only it looks at) is a ValueError, like the checks before it."""
+    kind = RuntimeError if rc == SQA_ERR_HIP else ValueError
+    return kind(f"{name} failed: {last_error(lib)}")
+
+
 @functools.lru_cache(maxsize=4096)
 def plan_windowed(device_index: int, batch: int, q_len: int, num_query_heads: int,
                   num_kv_heads: int, head_dim: int, window: int, sink: int, max_seq_len: int,
@@ -373,7 +381,7 @@ def plan_windowed(device_index: int, batch: int, q_len: int, num_query_heads: in
                                window, sink, max_seq_len, max_pages, kv_dtype, ctypes.byref(ns),
                                ctypes.byref(pps), ctypes.byref(heads))
     if rc != SQA_OK:
-        raise RuntimeError(f"sqa_plan_windowed failed: {last_error(lib)}")
+        raise refusal(lib, "sqa_plan_windowed", rc)
     return ns.value, pps.value, heads.value
 
 
@@ -411,8 +419,9 @@ def launch_windowed(query, output, k_view, v_view, k_scale, v_scale, block_table
     a, scales = _part_args(query, output, k_view, v_view, k_scale, v_scale, block_tables, seq_lens,
                            draft_mask, scale, out_scale, cut[0], cut[1], workspace, stream_handle,
                            fields or part_fields(query, k_view, k_scale, block_tables, draft_mask))
-    if lib.sqa_paged_attention_windowed(a, scales, window, sink, cut[2]) != SQA_OK:
-        raise RuntimeError(f"sqa_paged_attention_windowed failed: {last_error(lib)}")
+    rc = lib.sqa_paged_attention_windowed(a, scales, window, sink, cut[2])
+    if rc != SQA_OK:
+        raise refusal(lib, "sqa_paged_attention_windowed", rc)
 
 
 @functools.lru_cache(maxsize=1024)
@@ -429,7 +438,7 @@ def plan_shared_prefix(device_index: int, groups, shape, kv_dtype: int, max_seq_
                                     (ctypes.c_int32 * max(len(flat), 1))(*flat), max_seq_len,
                                     max_pages, ctypes.byref(plan), table)
     if rc != SQA_OK:
-        raise RuntimeError(f"sqa_plan_shared_prefix failed: {last_error(lib)}")
+        raise refusal(lib, "sqa_plan_shared_prefix", rc)
     return plan, int(lib.sqa_shared_workspace_bytes(ctypes.byref(plan))), list(table)
 
 
@@ -445,7 +454,7 @@ def launch_shared_prefix(query, output, k_view, v_view, k_scale, v_scale, block_
                            fields or part_fields(query, k_view, k_scale, block_tables, draft_mask))
     rc = lib.sqa_paged_attention_shared_prefix(a, scales, ctypes.byref(plan), table.data_ptr())
     if rc != SQA_OK:
-        raise RuntimeError(f"sqa_paged_attention_shared_prefix failed: {last_error(lib)}")
+        raise refusal(lib, "sqa_paged_attention_shared_prefix", rc)
 
 
 def append_fields(key, value, k_view, k_scale, block_tables):

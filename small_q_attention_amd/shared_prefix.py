@@ -24,7 +24,7 @@ from . import _lib
 from . import scaled_cache as sc
 from .cuda import HEAD_DIMS, SUPPORTED_PAGE_SIZES, _tracing
 from .masks import as_words
-from .windowed import check_apart, check_call, take_workspace
+from .windowed import check_apart, check_call, check_factors, take_workspace
 
 
 class SharedPrefixPlan:
@@ -171,7 +171,7 @@ def paged_attention_shared_prefix(query, key_cache, value_cache, block_tables, s
         raise ValueError("query must be a contiguous [B, Q, Hq, D] tensor")
     if not isinstance(plan, SharedPrefixPlan):
         raise ValueError("plan must come from plan_shared_prefix()")
-    scale = sc.check_softmax_scale(scale, query.shape[3])
+    scale, out_scale = check_factors(scale, out_scale, query.shape[3])
     words = None if mask is None else as_words(mask, query.shape[0], query.shape[1])
     max_seq_len = min(max(int(max_seq_len), 0), 2**31 - 1)
     if _tracing():
@@ -181,7 +181,7 @@ def paged_attention_shared_prefix(query, key_cache, value_cache, block_tables, s
 
         res = torch.ops.sqa.paged_attention_shared_prefix(
             query, key_cache, value_cache, key_scale, value_scale, block_tables, seq_lens, words,
-            plan.flat, plan.table, scale, float(out_scale), max_seq_len)
+            plan.flat, plan.table, scale, out_scale, max_seq_len)
         return res if out is None else out.copy_(res)
     layout = sc.layout
     seen = (layout(query), layout(key_cache), layout(value_cache), layout(key_scale),
@@ -198,7 +198,7 @@ def paged_attention_shared_prefix(query, key_cache, value_cache, block_tables, s
     check_apart(query, out)
     return sc.on_device(query.device, run_shared_prefix, query, key_cache, value_cache, key_scale,
                         value_scale, block_tables, seq_lens, words, plan.groups, plan.table, scale,
-                        float(out_scale), max_seq_len, out, workspace_buffer, known, plan.streams)
+                        out_scale, max_seq_len, out, workspace_buffer, known, plan.streams)
 
 
 __all__ = ["SharedPrefixPlan", "plan_shared_prefix", "paged_attention_shared_prefix"]

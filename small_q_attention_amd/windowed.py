@@ -56,6 +56,18 @@ def check_call(query, key_cache, value_cache, key_scale, value_scale, block_tabl
         raise ValueError("out must be a contiguous tensor shaped and typed like query")
 
 
+_LARGEST = 2.0 ** 128 - 2.0 ** 103  # numbers from here on are no float32
+
+
+def check_factors(scale, out_scale, d):
+    """The softmax scale (``None``: ``d ** -0.5``) and the output's factor, as floats that 32
+    bits hold."""
+    scale, out_scale = sc.check_softmax_scale(scale, d), float(out_scale)
+    if not 2.0 ** -150 < scale < _LARGEST or not abs(out_scale) < _LARGEST:
+        raise ValueError("scale must be positive and finite and out_scale finite, in 32 bits")
+    return scale, out_scale
+
+
 def check_apart(query, out):
     """ValueError for a result that takes some of the queries' place: they are read until the
     end. (Both are contiguous, of one size.)"""
@@ -128,7 +140,7 @@ def paged_attention_windowed(query, key_cache, value_cache, block_tables, seq_le
     """
     if query.dim() != 4:
         raise ValueError("query must be a contiguous [B, Q, Hq, D] tensor")
-    scale = sc.check_softmax_scale(scale, query.shape[3])
+    scale, out_scale = check_factors(scale, out_scale, query.shape[3])
     window, sink = int(window), int(sink)
     if window <= 0 or sink < 0:
         raise ValueError("window must be positive and sink not negative")
@@ -142,7 +154,7 @@ def paged_attention_windowed(query, key_cache, value_cache, block_tables, seq_le
 
         res = torch.ops.sqa.paged_attention_windowed(
             query, key_cache, value_cache, key_scale, value_scale, block_tables, seq_lens, words,
-            window, sink, scale, float(out_scale), max_seq_len)
+            window, sink, scale, out_scale, max_seq_len)
         return res if out is None else out.copy_(res)
     layout = sc.layout
     seen = (layout(query), layout(key_cache), layout(value_cache), layout(key_scale),
@@ -159,7 +171,7 @@ def paged_attention_windowed(query, key_cache, value_cache, block_tables, seq_le
     check_apart(query, out)
     return sc.on_device(query.device, run_windowed, query, key_cache, value_cache, key_scale,
                         value_scale, block_tables, seq_lens, words, window, sink, scale,
-                        float(out_scale), max_seq_len, out, workspace_buffer, known)
+                        out_scale, max_seq_len, out, workspace_buffer, known)
 
 
 __all__ = ["paged_attention_windowed"]

@@ -338,3 +338,39 @@ def test_c_entries_refuse_an_output_over_the_query(lib, off):
     assert lib.sqa_paged_attention_shared_prefix(ctypes.byref(a), None, ctypes.byref(_c_plan()),
                                                  1 << 20) == 1
     assert "overlaps" in lib.sqa_last_error().decode()
+
+
+@pytest.mark.parametrize("call", CALLS)
+@pytest.mark.parametrize("factors", [
+    dict(out_scale=float("nan")), dict(out_scale=float("inf")), dict(out_scale=-float("inf")),
+    dict(out_scale=2.0 ** 128), dict(scale=2.0 ** 128), dict(scale=1e300), dict(scale=2.0 ** -150)])
+def test_factors_that_32_bits_do_not_hold(call, factors):
+    with pytest.raises(ValueError, match="in 32 bits"):
+        CALLS[call](_base(), **factors)
+    assert windowed.check_factors(None, -2.0, 64) == (0.125, -2.0)
+    assert windowed.check_factors(2.0 ** -149, 3.4028234e38, 64) == (2.0 ** -149, 3.4028234e38)
+
+
+def test_what_the_library_refuses_is_a_value_error(lib):
+    """Alignments, strides and workspaces that only the C entries look at."""
+    a = _base()
+    store = torch.zeros(a["query"].numel() + 8, dtype=F16)
+    args = lambda **kw: [{**a, "out": store[:-8].view(a["query"].shape), **kw}[n] for n in (  # noqa: E731
+        "query", "out", "key_cache", "value_cache", "key_scale", "value_scale", "block_tables",
+        "seq_lens")]
+    odd = store[1:a["query"].numel() + 1].view(a["query"].shape)
+    # (Never touched, so never more than addresses.)
+    far = torch.empty(15 << 27 | 128, dtype=F16).as_strided((6, 16, 2, 64), (0, 1 << 27, 64, 1))
+    ws = torch.zeros(1 << 20, dtype=torch.uint8)[4:]
+    plan = _c_plan()
+    for launch, rest in ((_lib.launch_windowed, (None, 8, 0, 0.1, 1.0, (2, 1, 2))),
+                         (_lib.launch_shared_prefix, (None, plan, torch.zeros(32, dtype=torch.int32),
+                                                      0.1, 1.0))):
+        for change, space, match in ((dict(out=odd), None, "aligned"),
+                                     (dict(key_cache=far, value_cache=far), None, "2 GiB"),
+                                     ({}, ws, "aligned"), ({}, ws[:16], "workspace of")):
+            with pytest.raises(ValueError, match=match):
+                launch(*args(**change), *rest, space, 0)
+    with pytest.raises(ValueError, match="grid too large"):
+        _lib.plan_windowed(0, 2**20, 16, 2**10, 2**10, 64, 5, 0, 0, 4, 0)
+    assert isinstance(_lib.refusal(lib, "x", _lib.SQA_ERR_HIP), RuntimeError)

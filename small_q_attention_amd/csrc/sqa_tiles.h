@@ -120,7 +120,8 @@ struct StoreCodesInt8 {
 // brought for twice the rows (96 sequences over two prefixes, bf16: 204 and 212 us).
 template <int HD, int W, typename E, typename KV>
 struct TileShare {
-  using EV = std::conditional_t<KV::kScaled, ElemF16, E>;  // type of P and V
+  // The type of P and V: every 8-bit code is an fp16 number.
+  using EV = std::conditional_t<KV::kBytes == 1, ElemF16, E>;
   using T = Tile<HD>;
   static constexpr int kTokens = kTileKeys / W;  // of a tile that a wave brings
   using Loads = PageLoads<HD, KV::kBytes, kTokens>;
@@ -322,9 +323,10 @@ struct TileShare {
   // exponentials, the maxima of the next among the products with V, and reads from LDS kAhead
   // pieces before their use; the compiler, left alone, puts one after the other (64 sequences
   // over 32K tokens, q_len 8: 345 us so, 338 in this order).
-  // P is rounded once to the type of the products, in bf16 too (2^-9 of a probability, as the
-  // output's own rounding; sums stay in 32 bits): a second product for what is rounded off, as
-  // pages in waves have it, would cost half of the products again, and these bound the kernel.
+  // P is rounded once to the type of the products, over bf16 caches too (2^-8 of a probability,
+  // as the output's own rounding; sums stay in 32 bits): a second product for what is rounded
+  // off, as pages in waves have it, would cost half of the products again, and these bound the
+  // kernel.
   constexpr int kAhead = 3;
   auto step = [&](const f16v& now, const Pages& pages, int v_kb, f16v& next,
                   const Pages& next_pages, int k_kb) {

@@ -265,3 +265,41 @@ def test_a_plan_dropped_before_its_call_has_run(traced):
     assert all(p.table.data_ptr() != at for p in others)
     torch.cuda.synchronize()
     assert torch.equal(out, want)
+
+
+# --------------------------------------------------------------------------------------
+# Probabilities of shared pages in tiles.
+# --------------------------------------------------------------------------------------
+
+def _heavy(dtype, kv, d, count, keys, seed=0):
+    """Queries along dim 0, of 2^0.5 to 2^7.9 against a key of 2: a first key of 0 sets the
+    maximum, those of ``keys`` {token: key} carry nearly all of the weight without raising it,
+    all others none."""
+    q_len, hq, hkv, page, shared = 4, 8, 2, 16, 9
+    lens = [shared * page + q_len + i % 60 for i in range(count)]
+    q, (k, v), _, tables, full, sl = inputs([(0, count, shared)], lens, q_len, hq, hkv, d, page,
+                                            dtype, kv, False, seed)
+    size = torch.linspace(0.5, 7.9, q[..., 0].numel()) * d ** 0.5 / 2 * 0.6931471805599453
+    q = torch.zeros_like(q)
+    q[..., 0] = size.view(q[..., 0].shape).to(dtype)
+    k = torch.zeros(k.shape)
+    k[..., 0] = -60
+    for t, x in {0: 0.0, **keys}.items():
+        k[int(full[0, t // page]), t % page, :, 0] = x
+    plan = plan_shared_prefix([(0, count, shared)], count, q_len, hq, hkv, d, page)
+    return q, k.to(kv or dtype), v, tables, full, sl, plan
+
+
+TILES = [(d, count) for d in (64, 128, 256) for count in (7, 33)]  # 112 and 528 rows of a kv head
+
+
+@pytest.mark.parametrize("d,count", TILES)
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_probabilities_over_e4m3_have_11_bits(dtype, d, count):
+    """Two keys share a row's weight, their values opposite."""
+    q, k, v, tables, full, sl, plan = _heavy(dtype, E4M3, d, count, {40: 2.0, 41: 1.875})
+    raw = v.view(torch.uint8)
+    raw[int(full[0, 2]), 9] = raw[int(full[0, 2]), 8] ^ 0x80
+    want, bound = ref.attention(q, k, v, None, None, full, sl, everything(4), p_step=2.0 ** -11)
+    out = paged_attention_shared_prefix(*ref.cuda(q, k, v, tables, sl), plan)
+    ref.assert_within(out, want, bound)

@@ -342,6 +342,8 @@ struct TileShare {
       const float x = fast_exp2(fmaf(now[2 * w], pages.mul[st], off[st]));
       const float y = fast_exp2(fmaf(now[2 * w + 1], pages.mul[st], off[st]));
       unsigned packed = EV::pack2(x, y);
+      // The row sum is that of the rounded ones (but with V scales, which lie between the two),
+      // so that the weights of a row add up to one.
       if constexpr (KV::kScaled) {
         l = fmaf(x + y, pages.inv[st], l);
         packed = pages.loud[st] ? packed : 0u;
@@ -349,7 +351,9 @@ struct TileShare {
         const h2 ones = {(_Float16)1.0f, (_Float16)1.0f};
         l = __builtin_amdgcn_fdot2(__builtin_bit_cast(h2, packed), ones, l, false);
       } else {
-        l += x + y;
+        typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+        const b2 ones = {(__bf16)1.0f, (__bf16)1.0f};
+        l = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(b2, packed), ones, l, false);
       }
       p[st][w % 4] = packed;
     };

@@ -160,8 +160,9 @@ def paged_attention_shared_prefix(query, key_cache, value_cache, block_tables, s
     ``max_seq_len`` > 0 only sizes the call (0: the block table's width), and with it the
     last bits of a result may change; ``scale`` is the softmax scale (``None``: ``D **
     -0.5``), ``out_scale`` multiplies the output. Over bf16 caches the
-    probabilities of shared pages are rounded once to bf16 (2^-8 of each) for groups of more
-    than 64 rows of a kv head (32 at head_dim 256), and kept to 2^-16 otherwise.
+    probabilities of shared pages are rounded once to bf16 (2^-8 of each; a row's weights still
+    add up to one) for groups of more than 64 rows of a kv head (32 at head_dim 256), and kept to
+    2^-16 otherwise.
     ``workspace_buffer``: a caller's buffer for the partial rows; ``None`` takes one kept per
     host thread and stream, or, under graph capture, one of the graph's own. A graph reads
     the plan's table: the plan is kept for as long as the graph is replayed. Returns ``out``

@@ -303,3 +303,17 @@ def test_probabilities_over_e4m3_have_11_bits(dtype, d, count):
     want, bound = ref.attention(q, k, v, None, None, full, sl, everything(4), p_step=2.0 ** -11)
     out = paged_attention_shared_prefix(*ref.cuda(q, k, v, tables, sl), plan)
     ref.assert_within(out, want, bound)
+
+
+@pytest.mark.parametrize("d,count", TILES)
+@pytest.mark.parametrize("dtype,kv", [(F16, None), (BF16, None), (F16, E4M3), (BF16, E4M3)])
+def test_weights_of_a_row_add_up_to_one(dtype, kv, d, count):
+    """Where all tokens have one value, so has every row, to the bit: the rounding of a heavy
+    probability is in its row's sum as in the product."""
+    q, k, v, tables, full, sl, plan = _heavy(dtype, kv, d, count, {40: 2.0})
+    # (A weight off by more than 2^-9 shows in values just below a power of two, where the steps of
+    # the type are smallest beside the value.)
+    value = torch.tensor([1.875, -3.75]).repeat(d // 2)
+    v = torch.zeros(v.shape).add(value).to(v.dtype)
+    out = paged_attention_shared_prefix(*ref.cuda(q, k, v, tables, sl), plan)
+    assert torch.equal(out.float().cpu(), value.expand(q.shape))

@@ -374,3 +374,38 @@ def test_what_the_library_refuses_is_a_value_error(lib):
     with pytest.raises(ValueError, match="grid too large"):
         _lib.plan_windowed(0, 2**20, 16, 2**10, 2**10, 64, 5, 0, 0, 4, 0)
     assert isinstance(_lib.refusal(lib, "x", _lib.SQA_ERR_HIP), RuntimeError)
+
+
+@pytest.mark.parametrize("change,status,match", [x for x in BAD if "num_splits" not in x[0]
+                                                 and "pages_per_split" not in x[0]])
+def test_shared_prefix_names_what_it_refuses(lib, change, status, match):
+    """Each by its own check, not by the plan's other shape."""
+    rc = lib.sqa_paged_attention_shared_prefix(ctypes.byref(_args(**change)), None,
+                                               ctypes.byref(_c_plan()), 1 << 20)
+    assert rc == status
+    assert match in lib.sqa_last_error().decode()
+
+
+@pytest.mark.parametrize("shape", [dict(batch=2), dict(q_len=2), dict(num_query_heads=4),
+                                   dict(num_kv_heads=1), dict(head_dim=128), dict(page_size=32),
+                                   dict(num_splits=3), dict(num_splits=9, pages_per_split=0)])
+def test_shared_prefix_refuses_a_plan_of_another_shape(lib, shape):
+    strides = dict(kv_page_stride=2**16, kv_token_stride=512)
+    for a, plan in ((_args(**strides), _c_plan(**shape)), (_args(**strides, **shape), _c_plan())):
+        assert lib.sqa_paged_attention_shared_prefix(ctypes.byref(a), None, ctypes.byref(plan),
+                                                     1 << 20) == 1
+        assert "another batch" in lib.sqa_last_error().decode()
+
+
+@pytest.mark.parametrize("shape,plan", [
+    ({}, dict(block_rows=48)), ({}, dict(block_rows=8)), ({}, dict(block_rows=0)),
+    ({}, dict(block_rows=512)), (dict(q_len=12), dict(block_rows=32)),
+    (dict(q_len=12), dict(block_rows=256)), (dict(head_dim=256), dict(block_rows=64)),
+    (dict(head_dim=256), dict(block_rows=256)), ({}, dict(shared_splits=0))])
+def test_shared_prefix_refuses_blocks_that_no_kernel_has(lib, shape, plan):
+    """Plans that agree with the call in all but how the groups are cut."""
+    a = _args(**shape, kv_page_stride=2**16, kv_token_stride=512)
+    assert lib.sqa_paged_attention_shared_prefix(ctypes.byref(a), None,
+                                                 ctypes.byref(_c_plan(**shape, **plan)),
+                                                 1 << 20) == 1
+    assert lib.sqa_last_error().decode() == "not a plan of sqa_plan_shared_prefix"

@@ -67,8 +67,8 @@ struct Model {
   }
   // Keeps cuts of huge batches from a workspace of more than 4 GiB where others do with less.
   double memory(double slots) const {
-    return std::max(slots * num_kv_heads * rows * head_dim * 4 - (double)sqa::kMaxPartialBytes, 0.0) /
-           1e3;
+    return 1e-3 * std::max(slots * num_kv_heads * rows * head_dim * 4 -
+                               (double)sqa::kMaxPartialBytes, 0.0);
   }
 };
 

@@ -24,7 +24,7 @@ from . import _lib
 from . import scaled_cache as sc
 from .cuda import HEAD_DIMS, SUPPORTED_PAGE_SIZES, _tracing
 from .masks import as_words
-from .windowed import check_apart, check_call, check_factors, take_workspace
+from .windowed import check_apart, check_call, check_factors, take_workspace, whole_pages
 
 
 class SharedPrefixPlan:
@@ -158,7 +158,9 @@ def paged_attention_shared_prefix(query, key_cache, value_cache, block_tables, s
     that is not (a padded batch's) goes over its own row from the start.
 
     ``max_seq_len`` > 0 only sizes the call (0: the block table's width), and with it the
-    last bits of a result may change; ``scale`` is the softmax scale (``None``: ``D **
+    last bits of a result may change; a call of another layout or number of 16-token pages is
+    planned anew, 50 to 300 us on the host, so a loop better passes a bound that stays for many
+    calls. ``scale`` is the softmax scale (``None``: ``D **
     -0.5``), ``out_scale`` multiplies the output. Over bf16 caches the
     probabilities of shared pages are rounded once to bf16 (2^-8 of each; a row's weights still
     add up to one) for groups of more than 64 rows of a kv head (32 at head_dim 256), and kept to
@@ -174,7 +176,7 @@ def paged_attention_shared_prefix(query, key_cache, value_cache, block_tables, s
         raise ValueError("plan must come from plan_shared_prefix()")
     scale, out_scale = check_factors(scale, out_scale, query.shape[3])
     words = None if mask is None else as_words(mask, query.shape[0], query.shape[1])
-    max_seq_len = min(max(int(max_seq_len), 0), 2**31 - 1)
+    max_seq_len = whole_pages(max_seq_len)
     if _tracing():
         _check(query, key_cache, value_cache, key_scale, value_scale, block_tables, seq_lens, words,
                plan, out, workspace_buffer)

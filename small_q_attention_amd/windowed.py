@@ -68,6 +68,12 @@ def check_factors(scale, out_scale, d):
     return scale, out_scale
 
 
+def whole_pages(max_seq_len) -> int:
+    """``max_seq_len`` as the plans look at it, in whole pages of 16 tokens: a loop whose longest
+    sequence grows by one plans again every sixteenth call."""
+    return min((max(int(max_seq_len), 0) + 15) // 16 * 16, 2**31 - 16)
+
+
 def check_apart(query, out):
     """ValueError for a result that takes some of the queries' place: they are read until the
     end. (Both are contiguous, of one size.)"""
@@ -133,7 +139,8 @@ def paged_attention_windowed(query, key_cache, value_cache, block_tables, seq_le
     ``key_scale``/``value_scale`` ``[P, Hkv]`` float32: block scales of e4m3 or int8 codes,
     within the ranges of :func:`scaled_cache.paged_attention_scaled`. ``max_seq_len`` > 0
     only sizes the call (0: the block table's width), and with it the last bits of a result
-    may change; ``scale`` is the softmax scale (``None``: ``D ** -0.5``), ``out_scale``
+    may change; a call of another layout, window or number of 16-token pages is planned anew,
+    about 10 us on the host. ``scale`` is the softmax scale (``None``: ``D ** -0.5``), ``out_scale``
     multiplies the output. ``workspace_buffer``: a caller's buffer for the split partials;
     ``None`` takes one kept per host thread and stream, or, under graph capture, one of the
     graph's own. Returns ``out`` (``[B, Q, Hq, D]``).
@@ -146,7 +153,7 @@ def paged_attention_windowed(query, key_cache, value_cache, block_tables, seq_le
         raise ValueError("window must be positive and sink not negative")
     window, sink = min(window, 2**31 - 1), min(sink, 2**31 - 1)
     words = None if mask is None else as_words(mask, query.shape[0], query.shape[1])
-    max_seq_len = min(max(int(max_seq_len), 0), 2**31 - 1)
+    max_seq_len = whole_pages(max_seq_len)
     if _tracing():
         check_call(query, key_cache, value_cache, key_scale, value_scale, block_tables, seq_lens,
                    words, out, workspace_buffer)

@@ -409,3 +409,10 @@ def test_shared_prefix_refuses_blocks_that_no_kernel_has(lib, shape, plan):
                                                  ctypes.byref(_c_plan(**shape, **plan)),
                                                  1 << 20) == 1
     assert lib.sqa_last_error().decode() == "not a plan of sqa_plan_shared_prefix"
+
+
+def test_calls_are_planned_by_pages():
+    """Lengths on one page are one to the plans and their caches."""
+    for n, pages in ((-3, 0), (0, 0), (1, 16), (16, 16), (17, 32), (8191, 8192),
+                     (2**31 - 1, 2**31 - 16), (2**40, 2**31 - 16)):
+        assert windowed.whole_pages(n) == pages

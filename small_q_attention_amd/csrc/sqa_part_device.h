@@ -204,11 +204,13 @@ __device__ __forceinline__ SharedItem item_of(const PartArgs& a, int item) {
 }
 
 // Values of a page that are not finite, added up in `to` as the rows see them (tokens of a
-// score of -infinity are not seen). Returns whether there are any.
-template <int NB, int HD, typename E>
+// score of -infinity are not seen). Returns whether there are any. INF: there may be infinities,
+// and not NaN alone.
+template <int NB, int HD, typename E, bool INF>
 __device__ __forceinline__ bool add_wild(f4 (&to)[Dims<HD>::MB][NB], const PageV<HD, 1>& pv,
                                          const f4 (&s)[NB], bool bf16) {
-  constexpr int MB = Dims<HD>::MB, VW = Dims<HD>::VW;
+  constexpr int VW = Dims<HD>::VW;
+  static_assert(Dims<HD>::MB == 2 * VW, "two blocks of dims to a word");
   const unsigned inf = bf16 ? 0x7f80u : 0x7c00u, one = bf16 ? 0x3f80u : 0x3c00u;
   const unsigned up = (0x8000u - inf) * 0x10001u;
   unsigned any = 0u;
@@ -216,7 +218,7 @@ __device__ __forceinline__ bool add_wild(f4 (&to)[Dims<HD>::MB][NB], const PageV
   for (int e = 0; e < 4; ++e)
 #pragma unroll
     for (int w = 0; w < VW; ++w) any |= (pv.v[0][e][w] & 0x7fff7fffu) + up;
-  if (!__any((any & 0x80008000u) != 0u)) return false;  // uniform
+  if (__builtin_expect(!__any((any & 0x80008000u) != 0u), 1)) return false;  // uniform
   u2 rows[NB];
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) {
@@ -226,33 +228,37 @@ __device__ __forceinline__ bool add_wild(f4 (&to)[Dims<HD>::MB][NB], const PageV
     for (int e = 0; e < 4; ++e) seen[e] = s[nb][e] == -INFINITY ? 0.f : 1.f;
     rows[nb] = E::round_p(seen[0], seen[1], seen[2], seen[3], sum, none);
   }
-  // Sums of ones: over what is NaN or +infinity, then over what is NaN or -infinity. (By bits of
-  // both halves of a word at once: compares, two to an element, took a hundred scalars.)
+  // Sums of ones: over what is NaN or +infinity, then over what is NaN or -infinity; where there
+  // are no infinities, over what is NaN. (By bits of both halves of a word at once: compares, two
+  // to an element, took a hundred scalars.)
 #pragma unroll 1
-  for (int sign = 0; sign < 2; ++sign) {
-    unsigned mark[4][VW];
+  for (int sign = 0; sign < (INF ? 2 : 1); ++sign) {
+    const float value = INF ? (sign ? -INFINITY : INFINITY) : __builtin_nanf("");
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
+    for (int j = 0; j < VW; ++j) {
+      unsigned mark[4];
 #pragma unroll
-      for (int w = 0; w < VW; ++w) {
-        const unsigned x = pv.v[0][e][w];
-        const unsigned y = x ^ (sign ? inf : inf | 0x8000u) * 0x10001u;  // 0: the other infinity
-        const unsigned bad = (x & 0x7fff7fffu) + up, apart = ((y & 0x7fff7fffu) + 0x7fff7fffu) | y;
-        mark[e][w] = ((bad & apart & 0x80008000u) >> 15) * one;
+      for (int e = 0; e < 4; ++e) {
+        const unsigned x = pv.v[0][e][j];
+        unsigned bad = (x & 0x7fff7fffu) + up;
+        if constexpr (INF) {
+          const unsigned y = x ^ (sign ? inf : inf | 0x8000u) * 0x10001u;  // 0: the other infinity
+          bad &= ((y & 0x7fff7fffu) + 0x7fff7fffu) | y;
+        }
+        mark[e] = ((bad & 0x80008000u) >> 15) * one;
       }
 #pragma unroll
-    for (int mb = 0; mb < MB; ++mb) {
-      const int j = mb >> 1;
-      const u2 av = (mb & 1) == 0
-                        ? u2{pack_lo(mark[0][j], mark[1][j]), pack_lo(mark[2][j], mark[3][j])}
-                        : u2{pack_hi(mark[0][j], mark[1][j]), pack_hi(mark[2][j], mark[3][j])};
+      for (int half = 0; half < 2; ++half) {
+        const u2 av = half == 0 ? u2{pack_lo(mark[0], mark[1]), pack_lo(mark[2], mark[3])}
+                                : u2{pack_hi(mark[0], mark[1]), pack_hi(mark[2], mark[3])};
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb) {
-        const f4 hits = E::mma_pv(av, rows[nb], u2{0u, 0u}, f4{0.f, 0.f, 0.f, 0.f});
+        for (int nb = 0; nb < NB; ++nb) {
+          const f4 hits = E::mma_pv(av, rows[nb], u2{0u, 0u}, f4{0.f, 0.f, 0.f, 0.f});
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          to[mb][nb][e] += hits[e] > 0.f ? (sign ? -INFINITY : INFINITY) : 0.f;
+          for (int e = 0; e < 4; ++e) to[2 * j + half][nb][e] += hits[e] > 0.f ? value : 0.f;
+        }
       }
+      __builtin_amdgcn_sched_barrier(0);  // few registers rather than few waits
     }
   }
   return true;
@@ -262,11 +268,11 @@ __device__ __forceinline__ bool add_wild(f4 (&to)[Dims<HD>::MB][NB], const PageV
 // of its block, those that do not see its token too (0 * NaN). They become 0 here, and what
 // they are in the sums of the rows that do see them. Rare: pages without one pay a few
 // instructions, on masked pages only.
-template <int NB, int HD, typename E>
+template <int NB, int HD, typename E, bool INF>
 __device__ __forceinline__ void wild_values(WaveState<NB, HD>& st, PageV<HD, 1>& pv,
                                             const f4 (&s)[NB], bool bf16) {
   constexpr int VW = Dims<HD>::VW;
-  if (!add_wild<NB, HD, E>(st.acc, pv, s, bf16)) return;
+  if (!add_wild<NB, HD, E, INF>(st.acc, pv, s, bf16)) return;
   const unsigned up = (0x8000u - (bf16 ? 0x7f80u : 0x7c00u)) * 0x10001u;
 #pragma unroll
   for (int e = 0; e < 4; ++e)
@@ -317,7 +323,8 @@ struct RowMap {
   }
   __device__ __forceinline__ long long part_row(const PartArgs& a, int x) const {
     const Place p = place(a, x);
-    if (pages == 0) return at + (long long)(p.b - first) * a.p.hkv * a.p.rows + p.y;
+    if (__builtin_expect(pages == 0, 1))
+      return at + (long long)(p.b - first) * a.p.hkv * a.p.rows + p.y;
     const unsigned slot = shared_slot(a, p.b, before + (p.b - first) * pages) + split;
     return a.shared_at +
            ((long long)min(slot, (unsigned)a.shared_slots - 1) * a.p.hkv + kvh) * a.p.rows + p.y;
@@ -329,7 +336,7 @@ struct RowMap {
 template <int HD>
 __device__ __forceinline__ void store_partial(const PartArgs& args, __amdgpu_buffer_rsrc_t pr,
                                               f4 v, long long at, int c, bool is) {
-  if (args.far_rows) {  // uniform
+  if (__builtin_expect(args.far_rows, 0)) {  // uniform
     const u4 x = __builtin_bit_cast(u4, v);
     float* to = args.p.part_o + at * HD + 4 * c;
     if (is) {
@@ -348,7 +355,7 @@ __device__ __forceinline__ RowMap shared_map(const PartArgs& a, int first, int s
                                              int kvh) {
   RowMap map{first, kvh,
              a.shared_at + (((long long)split * a.p.batch + first) * a.p.hkv + kvh) * a.p.rows};
-  if (a.packed) {  // uniform
+  if (__builtin_expect(a.packed, 0)) {  // uniform
     map.split = split;
     map.before = scalar_load(a.seq_groups + 2 * first);
     map.pages = pages;
@@ -484,7 +491,7 @@ __device__ __forceinline__ void plain_page(WaveState<NB, HD>& st, const typename
   for (int nb = 0; nb < NB; ++nb) lm[nb] = max4(s[nb]) * c;
   raise_max<NB, HD>(st, lm);
   // After the first maximum, whose factor is 0.
-  if (masked) wild_values<NB, HD, E>(st, pv, s, bf16);
+  if (masked) wild_values<NB, HD, E, KV::kInf>(st, pv, s, bf16);
   page_pv<NB, HD, E, KV, 1>(st, s, pv, false, c);
 }
 
@@ -784,7 +791,7 @@ __device__ __forceinline__ void part_share(float* sm_stage, int block, bool shar
     for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) nan.add(mb * NB + nb, st.acc[mb][nb]);
-    if (nan.any()) {  // uniform; rare
+    if (__builtin_expect(nan.any(), 0)) {  // uniform
       f4 wild[MB][NB];
 #pragma unroll
       for (int mb = 0; mb < MB; ++mb)
@@ -801,7 +808,7 @@ __device__ __forceinline__ void part_share(float* sm_stage, int block, bool shar
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) s[nb] = f4{0.f, 0.f, 0.f, 0.f};
         mask(s, p * kPageSize);
-        add_wild<NB, HD, E>(wild, pv, s, a.bf16);
+        add_wild<NB, HD, E, true>(wild, pv, s, a.bf16);
       }
 #pragma unroll
       for (int mb = 0; mb < MB; ++mb)

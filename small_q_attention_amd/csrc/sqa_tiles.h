@@ -441,7 +441,7 @@ struct TileShare {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         nan.add(i, f4{acc[mb][4 * i], acc[mb][4 * i + 1], acc[mb][4 * i + 2], acc[mb][4 * i + 3]});
-    if (nan.any()) {  // uniform; rare
+    if (__builtin_expect(nan.any(), 0)) {  // uniform
       constexpr int N = HD / 64;  // dims of a lane
       float wild[N];
 #pragma unroll
@@ -501,7 +501,7 @@ struct TileShare {
     const int at = __shfl(to, rs);
     store_partial<HD>(args, pr, v, at, e % CPR, at >= 0);
   };
-  if (args.far_rows) {  // uniform
+  if (__builtin_expect(args.far_rows, 0)) {  // uniform
 #pragma unroll 1
     for (int i = 0; i < CPR / 2; ++i) leave(i);
   } else {

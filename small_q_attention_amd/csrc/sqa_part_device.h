@@ -452,7 +452,7 @@ __device__ __forceinline__ void leave_rows(const PartArgs& args, WaveState<NB, H
 
 // The kernel's (first and only) argument, where the compiler cannot know that it was asked
 // for before: what a branch or a piece of work takes from it is loaded there, and not held in
-// scalar registers through all others (a hundred of them spilled otherwise).
+// scalar registers through all others (a third to a half more of them spilled otherwise).
 __device__ __forceinline__ const PartArgs& own_args() {
   auto* p = (const __attribute__((address_space(4))) PartArgs*)
       __builtin_amdgcn_kernarg_segment_ptr();

@@ -320,3 +320,83 @@ def test_weights_of_a_row_add_up_to_one(dtype, kv, d, count):
     v = torch.zeros(v.shape).add(value).to(v.dtype)
     out = paged_attention_shared_prefix(*ref.cuda(q, k, v, tables, sl), plan)
     assert torch.equal(out.float().cpu(), value.expand(q.shape))
+
+
+# --------------------------------------------------------------------------------------
+# All of it at once.
+# --------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("heads,splits,items", [(1, 1, 0), (4, 3, 0), (2, 40, 0), (1, 0, 1), (2, 0, 5),
+                                                (4, 0, 64)])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_values_at_every_cut_of_a_window(monkeypatch, dtype, heads, splits, items):
+    """Infinities in pieces of items that cross sequence ends, and in parts of several waves."""
+    lens, q_len, hq, hkv, d, page, window, sink = [700, 0, 33, 1500, 64, 900], 3, 12, 3, 64, 16, 600, 9
+    q, (k, v), _, tables, sl = ref.window_inputs(lens, q_len, hq, hkv, d, page, dtype, None, False,
+                                                 window, sink, seed=items)
+    for i, n in enumerate(lens):
+        for t, h, e, x in ((n // 2 + 200, 0, 1, INF), (n - 40, 2, 5, -INF), (n - 300, 1, 8, INF),
+                           (n - 200, 1, 8, -INF), (2, 2, 30, INF)):
+            if 0 <= t < n and (t < sink or t >= n - q_len + 1 - window):
+                _put(v, tables[i], t, h, e, x)
+    monkeypatch.setattr(windowed, "_KNOWN", scaled_cache.Layouts())
+    monkeypatch.setattr(_lib, "plan_windowed", lambda *a: (
+        splits or items + len(lens), int(splits > 0), heads))
+    out = paged_attention_windowed(*ref.cuda(q * 20, k, v, tables, sl), window, sink=sink)
+    want, bound = ref.attention(q * 20, k, v, None, None, tables, sl,
+                                lambda i, n: ref.window_seen(n, q_len, window, sink))
+    assert want.isinf().any() and want.isnan().any()
+    ref.assert_within(out, want, bound)
+
+
+@pytest.mark.parametrize("seed", range(40))
+def test_drawn_batches(monkeypatch, seed):
+    """Drawn groups of unlike lengths, padded and short sequences, split sizes, values that are
+    not finite where somebody sees them."""
+    g = torch.Generator().manual_seed(5000 + seed)
+
+    def draw(n):
+        return int(torch.randint(n, (1,), generator=g))
+
+    dtype, kv, scaled = CACHES[draw(len(CACHES))]
+    d, page, hkv, group = (64, 128, 256)[draw(3)], (16, 16, 64)[draw(3)], 1 + draw(4), 1 + draw(8)
+    q_len = 1 + draw(max(1, min(8, (32 if d == 256 else 64) // group)))
+    groups, lens = [], []
+    for _ in range(1 + draw(5)):
+        lens += [draw(150) for _ in range(draw(3))]
+        count, pages = 1 + draw((4, 30)[draw(2)]), draw((5, 60)[draw(2)] * 16 // page + 1)
+        groups.append((len(lens), count, pages))
+        lens += [pages * page + q_len + draw(200) if draw(6) else draw(pages * page + 40)
+                 for _ in range(count)]
+    b = len(lens)
+    if max(lens) == 0:
+        lens[0] = 5
+    q, caches, scales, tables, full, sl = inputs(groups, lens, q_len, hkv * group, hkv, d, page, dtype,
+                                                 kv, scaled, seed)
+    if not scaled and draw(2):
+        for _ in range(6):
+            i = draw(b)
+            if lens[i]:
+                _put(caches[1], full[i], draw(lens[i]), draw(hkv), draw(d), (INF, -INF, NAN)[draw(3)])
+    size = 1 + draw(40)
+
+    def change(p, shared):
+        splits = [_splits(pages, size) for _, pages in shared]
+        if not p.num_items:
+            return
+        rows = q_len * group
+        p.shared_size, even = size, max(splits)
+        p.num_items = sum(-(-n * rows // p.block_rows) * s for (n, _), s in zip(shared, splits))
+        p.shared_splits = min(even, -(-(b + sum(n * x for n, x in shared) // size) // b))
+
+    qc, kc, vc, ks, vs, bt, slc = ref.cuda(q, *caches, *scales, tables, sl)
+    want, bound = ref.attention(q, *caches, *scales, full, sl, everything(q_len),
+                                p_step=p_step(dtype, scaled))
+    for forged in (False, True):
+        with monkeypatch.context() as m:
+            if forged:
+                _forge(m, change)
+            plan = plan_shared_prefix(groups, b, q_len, hkv * group, hkv, d, page)
+            out = paged_attention_shared_prefix(qc, kc, vc, bt, slc, plan, key_scale=ks,
+                                                value_scale=vs)
+        ref.assert_within(out, want, bound, f"forged {forged}")

@@ -27,7 +27,7 @@ struct PartArgs {
   // fp32 sums and (max in log2 units, sum) of the partial rows. A slot of kv head h and
   // sequence b is `rows` of them. Own slot s starts at row (s * hkv + h) * rows, s = b *
   // splits + j for the sequence's split j, or (splits 0) from seq_splits[b].first on; split j
-  // of the sequence's group at row shared_at + (shared_slot(j) * hkv + h) * rows.
+  // of the sequence's group at row shared_at + ((shared_slot() + j * slot_step) * hkv + h) * rows.
   PartialArgs p;
   BlockScales scales;      // of codes with block scales
   int kv_type, scaled;     // kF16 (the query's type), kE4M3 or kInt8
